@@ -1,0 +1,461 @@
+"""The operators of a paged cache for Selective Attention, at the sizes a server runs them, for timing and for
+checking what they compute.
+
+    plan      page_plan: one step's block tables, slot map and lengths, made on the GPU from the requests' lengths
+    append    paged_append: the step's new keys and values into the cache's pages
+    attend    selective_attention_paged: the step's new tokens of every request (one each when generating, a chunk of
+              a prompt, a few drafted ones to verify, or any mixture) over the pages, updating the selection state
+
+Operator, per request with c cached positions, n new tokens and t = c + n, s = 1 / sqrt(D); group g's heads share the
+selector, the group's first head (one group: head 0 selects for every head; a group per head: each for itself):
+
+    L_h[i, j] = s q_h[i] . k_h[j]                          key j <= c + i
+    S[i, j]   = max(L_sel[i, j], 0)                        exempt <= j < c + i, else 0
+    F[i, j]   = state[j] (j < c, else 0) + sum of S[r, j] over r < i
+    out_h     = softmax over j of (L_h - F), times v_h;    state[j] = F after the last new token
+
+`own` says which side runs: the plain form below, or the package's operators. `select`: how often the selector selects:
+
+    normal    queries and keys N(0, 1): half of all pairs, so that a key's history grows by 0.4 a query and keys a few
+              hundred queries back have no weight left
+    sparse    the selector's logits are centred on -3: one pair in a hundred, every key keeps weight
+"""
+
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+_DTYPES = {"bf16": torch.bfloat16, "f32": torch.float32, "f16": torch.float16}
+
+
+def _ops():
+    pkg = os.path.join(os.getcwd(), "selective-attention-study_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import selective_attention
+
+    return selective_attention
+
+
+# -- cases ------------------------------------------------------------------------------------------------
+
+def _plan(name=None, *, R, P, ctx, new, ones=0.0, ended=0.0):
+    """R request rows with up to `ctx` cached positions; a share `ones` of them generates one token, the others take
+    chunks of up to `new`; a share `ended` has finished, its row starting a new request in this step."""
+    return _named(dict(kind="plan", R=R, P=P, ctx=ctx, new=new, ones=ones, ended=ended), name)
+
+
+def _append(name=None, *, N, H, D=64, P=16, dtype="bf16", source="bf16", packed=False):
+    """N new tokens' rows in dtype `source` into a cache of `dtype`; packed: views into a (N, 3, H, D) projection."""
+    return _named(dict(kind="append", N=N, H=H, D=D, P=P, dtype=dtype, source=source, packed=packed), name)
+
+
+def _attend(name=None, *, R, H, D=64, P=16, dtype="bf16", per_head=False, exempt=1, select="sparse", ctx=(0, 0),
+            new=(1, 1), ones=0.0):
+    """R requests with `ctx` cached positions and `new` new tokens (both spread over the range); a share `ones` of the
+    requests has one new token."""
+    return _named(dict(kind="attend", R=R, H=H, D=D, P=P, dtype=dtype, per_head=per_head, exempt=exempt, select=select,
+                       ctx_lo=ctx[0], ctx_hi=ctx[1], new_lo=new[0], new_hi=new[1], ones=ones), name)
+
+
+def _named(case, name):
+    if name:
+        case["name"] = name
+    return case
+
+
+def listed():
+    return [
+        # the tables of a generation step of a small batch: the smallest call, once per step whatever the layers
+        _plan("plan_step_8", R=8, P=16, ctx=1500, new=1, ones=1.0),
+        # a busy server's step: 512 rows, most generating, some taking chunks of prompts, some replaced by new requests
+        _plan("plan_mixed_512", R=512, P=16, ctx=8192, new=512, ones=0.9, ended=0.05),
+        # the cache write of that small generation step, one layer
+        _append("append_step_8", N=8, H=12),
+        # the cache write of a prompt of the study's 16K length, straight from the layer's packed projection
+        _append("append_packed_16k", N=16384, H=12, packed=True),
+        # a generation step of a small batch at a short context (latency is the work)
+        _attend("decode_8x1500", R=8, H=12, ctx=(900, 1500)),
+        # a generation step of a full batch of mixed lengths (the cache read is the work)
+        _attend("decode_64x8k", R=64, H=16, P=64, ctx=(500, 8191)),
+        # a generation step at the end of one 131072-token prompt
+        _attend("decode_131k", R=1, H=16, P=64, ctx=(131071, 131071)),
+        # drafted tokens verified in one step, fp32 cache, narrow heads
+        _attend("verify_f32_d32", R=16, H=8, D=32, dtype="f32", ctx=(300, 3000), new=(2, 9)),
+        # a batch of new prompts of uneven lengths through the study's 12-head model
+        _attend("prompts_ragged", R=12, H=12, new=(60, 2000)),
+        # a server's mixed step: most requests generate, a few take a chunk of their prompt
+        _attend("mixed_40", R=40, H=16, P=32, ctx=(0, 8000), new=(300, 512), ones=0.9),
+        # a chunk of a long prompt (the largest call: the products are the work)
+        _attend("chunk_4k_of_32k", R=1, H=16, P=64, ctx=(28672, 28672), new=(4096, 4096)),
+        # the per-head variant, wider heads, fp16 cache, histories that have outgrown most keys
+        _attend("chunk_perhead_f16_d128", R=3, H=8, D=128, P=16, dtype="f16", per_head=True, select="normal",
+                ctx=(0, 4000), new=(300, 700)),
+    ]
+
+
+def _log_uniform(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+# what a drawn case stays under: products (matrix rates of the types differ), and the cache's bytes
+_MOST_FLOPS = {"bf16": 5e11, "f16": 5e11, "f32": 6e10}
+_MOST_CACHE = 1.0e9
+
+
+def draw(rng):
+    while True:
+        P = rng.choice([8, 16, 16, 32, 64, 128])
+        kind = rng.choice(["plan", "append", "attend", "attend", "attend", "attend"])
+        if kind == "plan":
+            return _plan(R=_log_uniform(rng, 1, 512), P=P, ctx=_log_uniform(rng, 1, 16384),
+                         new=_log_uniform(rng, 1, 512), ones=rng.choice([0.0, 0.5, 0.9, 1.0]), ended=rng.choice([0.0, 0.1]))
+        D = rng.choice([64] * 6 + [128, 128, 32, 16])
+        H = rng.choice([1, 2, 4, 6, 8, 12, 12, 16, 16, 20])
+        dtype = rng.choice(["bf16"] * 7 + ["f32"] * 2 + ["f16"] * 2)
+        if kind == "append":
+            N = _log_uniform(rng, 1, 16384)
+            if N * H * D > 16384 * 12 * 64:
+                continue
+            return _append(N=N, H=H, D=D, P=P, dtype=dtype, source=rng.choice([dtype, dtype, "f32"]),
+                           packed=rng.random() < 0.5)
+        lo, hi = sorted(_log_uniform(rng, 1, 32768) - 1 for _ in range(2))
+        if rng.random() < 0.3:
+            lo = hi = 0   # new prompts
+        nlo, nhi = sorted(_log_uniform(rng, 1, 4096) for _ in range(2))
+        ones = rng.choice([0.0, 0.0, 0.5, 0.9])
+        if rng.random() < 0.4:
+            nlo, nhi, ones = 1, 1, 0.0
+        c = _attend(R=_log_uniform(rng, 1, 64), H=H, D=D, P=P, dtype=dtype, per_head=rng.random() < 0.25,
+                    exempt=rng.choice([1, 1, 1, 16, 3]), select=rng.choice(["normal", "sparse", "sparse"]),
+                    ctx=(lo, hi), new=(nlo, nhi), ones=ones)
+        cs, ns = _lengths(c)
+        es = 4 if dtype == "f32" else 2
+        t = max(a + b for a, b in zip(cs, ns))
+        if 4.0 * H * D * _pairs(cs, ns) > _MOST_FLOPS[dtype] or 2 * H * D * es * sum(a + b for a, b in zip(cs, ns)) > _MOST_CACHE:
+            continue
+        if (H if c["per_head"] else 1) * (sum(ns) / 32 + len(ns)) * t * 4 > 4e9:   # a selection sum per 32 queries and key
+            continue
+        return c
+
+
+def _spread(i, step):
+    return (0.5 + i * step) % 1.0
+
+
+def _lengths(case):
+    """(cached, new) of every request."""
+    if case["kind"] == "plan":
+        lo, hi, nlo, nhi = case["ctx"] // 2, case["ctx"], 1, case["new"]
+    else:
+        lo, hi, nlo, nhi = case["ctx_lo"], case["ctx_hi"], case["new_lo"], case["new_hi"]
+    cs = [lo + int(_spread(i, 0.6180339887) * (hi - lo + 1)) for i in range(case["R"])]
+    ns = [nlo + int(_spread(i, 0.7548776662) * (nhi - nlo + 1)) for i in range(case["R"])]
+    generating = round(case["ones"] * case["R"])
+    return cs, [1 if i < generating else n for i, n in enumerate(ns)]
+
+
+def _pairs(cs, ns):
+    """(query, key) pairs with the key at or before the query."""
+    return sum(n * c + n * (n + 1) // 2 for c, n in zip(cs, ns))
+
+
+# -- inputs -----------------------------------------------------------------------------------------------
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return {"plan": _prepare_plan, "append": _prepare_append, "attend": _prepare_attend}[case["kind"]](case, g, seed)
+
+
+def _pages_of(t, P):
+    return (t + P - 1) // P
+
+
+def _prepare_plan(case, g, seed):
+    P, R = case["P"], case["R"]
+    cs, ns = _lengths(case)
+    rng = random.Random(seed)
+    pool = sum(_pages_of(c, P) for c in cs) + sum(_pages_of(n, P) + 1 for n in ns)
+    cs = [max(1, c - rng.randrange(P)) for c in cs]
+    ended = [rng.random() < case["ended"] for _ in range(R)]
+    W = _pages_of(case["ctx"] + case["new"], P) + 1
+    held = [_pages_of(c, P) for c in cs]
+    order = torch.randperm(pool, generator=g, device="cuda").to(torch.int32)   # the pages held, then the free ones
+    table = torch.full((R, W), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for r, n in enumerate(held):
+        table[r, :n] = order[at:at + n]
+        at += n
+    return dict(case=case, cached=_ints(cs), new=_ints(ns), table=table, free=order, taken=_ints([at]),
+                finished=torch.tensor(ended, device="cuda") if case["ended"] else None, tokens=sum(ns))
+
+
+def _prepare_append(case, g, seed):
+    N, H, D, P = case["N"], case["H"], case["D"], case["P"]
+    dt, src = _DTYPES[case["dtype"]], _DTYPES[case["source"]]
+    generating = N <= 256   # every token of a request of its own, on a page of its own
+    pages = N + 3 if generating else _pages_of(N, P) + 3
+    k, v = torch.randn(N, 3, H, D, device="cuda", generator=g).to(src)[:, 1:].unbind(1)
+    if not case["packed"]:
+        k, v = k.contiguous(), v.contiguous()
+    kp, vp = (torch.randn(pages, H, P, D, device="cuda", generator=g).to(dt) for _ in range(2))
+    order = torch.randperm(pages, generator=g, device="cuda")
+    pos = torch.arange(N, device="cuda")
+    slots = order[pos] * P + (7 * pos) % P if generating else order[pos // P] * P + pos % P
+    return dict(case=case, k=k, v=v, k_pages=kp, v_pages=vp, slots=slots)
+
+
+def _prepare_attend(case, g, seed):
+    R, H, D, P = case["R"], case["H"], case["D"], case["P"]
+    dt = _DTYPES[case["dtype"]]
+    cs, ns = _lengths(case)
+    ts = [c + n for c, n in zip(cs, ns)]
+    G = H if case["per_head"] else 1
+    W = _pages_of(max(ts), P)
+    held = [_pages_of(t, P) for t in ts]
+    pages = sum(held) + 5
+    kp, vp = (torch.empty(pages, H, P, D, dtype=dt, device="cuda") for _ in range(2))
+    q = torch.randn(sum(ns), H, D, device="cuda", generator=g)
+    apart = math.sqrt(3.0 / math.sqrt(D)) if case["select"] == "sparse" else 0.0
+    selectors = slice(None) if G == H else slice(0, 1)
+    q[:, selectors] += apart
+    step = max(1, (1 << 26) // (H * P * D))
+    for a in range(0, pages, step):   # (a part at a time: the cache is large, and made in fp32)
+        part = torch.randn(min(step, pages - a), H, P, D, device="cuda", generator=g)
+        part[:, selectors] -= apart
+        kp[a:a + step] = part.to(dt)
+        vp[a:a + step] = part.normal_(generator=g).to(dt)
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((R, W), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for r, n in enumerate(held):
+        table[r, :n] = order[at:at + n]
+        at += n
+    # the selection that the cached keys have received from the queries before, as those would have left it
+    pos = torch.arange(W * P, device="cuda", dtype=torch.float32)
+    c = _ints(cs)[:, None]
+    rate = 0.4 if case["select"] == "normal" else 0.005
+    state = rate * (c - 1 - pos).clamp_min(0.0)
+    state[:, :case["exempt"]] = 0.0
+    selected = state[:, None].expand(R, G, W * P).contiguous()
+    starts = _ints([sum(ns[:r]) for r in range(R + 1)])
+    return dict(case=case, q=q.to(dt), k_pages=kp, v_pages=vp, table=table, lengths=_ints(ts), starts=starts,
+                selected=selected, max_new=max(ns), max_len=max(ts), cs=cs, ns=ns)
+
+
+# -- one pass ---------------------------------------------------------------------------------------------
+
+def run(state):
+    kind = state["case"]["kind"]
+    if kind == "plan":
+        args = (state["cached"], state["new"], state["table"], state["free"], state["taken"], state["case"]["P"],
+                state["tokens"], state["finished"])
+        plan = _ops().page_plan(*args) if own else _plain_plan(*args)
+        return dict(plan._asdict() if own else plan, table=state["table"], free=state["free"])
+    if kind == "append":
+        args = (state["k"], state["v"], state["k_pages"], state["v_pages"], state["slots"])
+        (_ops().paged_append if own else _plain_append)(*args)
+        return state["k_pages"], state["v_pages"]
+    selected = state["selected"]
+    if state["max_new"] > 1:   # several tokens: the next pass starts from the same history again
+        selected = selected.clone()
+    if own:
+        out = _ops().selective_attention_paged(
+            state["q"], state["k_pages"], state["v_pages"], state["table"], state["lengths"], state["starts"], selected,
+            exempt=state["case"]["exempt"], max_new=state["max_new"], max_len=state["max_len"])
+    elif state["max_new"] == 1:
+        out = _plain_step(state, selected)
+    else:
+        out = _plain_chunks(state, selected)
+    return out, selected
+
+
+def _plain_plan(cached, new, table, free, taken, P, tokens, finished):
+    W, F = table.shape[1], free.shape[0]
+    column = torch.arange(W, device=table.device)
+    zero = torch.zeros_like(cached)
+    before = cached if finished is None else torch.where(finished, zero, cached)
+    back = zero if finished is None else torch.where(finished, (cached + P - 1) // P, zero)
+    base = taken - back.sum()
+    if finished is not None:   # finished requests' pages go back on the stack, in request order
+        at = base + torch.cumsum(back, 0) - back
+        at = torch.where(column < back[:, None], at[:, None] + column, F)
+        wide = torch.cat([free, free.new_zeros(1)])
+        wide[at.flatten()] = table.flatten()
+        free.copy_(wide[:F])
+    have, want = (before + P - 1) // P, (before + new + P - 1) // P
+    need = torch.where(want <= W, want - have, 0)
+    upto = torch.cumsum(need, 0)
+    ends = torch.cumsum(new, 0)
+    served = (want <= W) & ((need == 0) | (upto <= F - base)) & (ends <= tokens)
+    take = base + upto - need
+    fresh = (column >= have[:, None]) & (column < want[:, None]) & served[:, None]
+    table.copy_(torch.where(fresh, free[(take[:, None] + column - have[:, None]).clamp(0, F - 1)], table))
+    after = base + torch.where(served, upto, 0).max()
+    starts = torch.cat([zero[:1], ends])
+    token = torch.arange(tokens, device=table.device)
+    r = torch.searchsorted(ends, token, right=True).clamp(max=cached.shape[0] - 1)
+    pos = before[r] + token - starts[r]
+    slot = table[r, (pos // P).clamp(max=W - 1)].long() * P + pos % P
+    slots = torch.where(served[r] & (token < ends[-1]), slot, -1)
+    return dict(starts=starts.int(), lengths=torch.where(served, before + new, 0).int(),
+                cached=torch.where(served, before + new, before).int(), slots=slots, taken=after.int().reshape(1))
+
+
+def _plain_append(k, v, k_pages, v_pages, slots):
+    P = k_pages.shape[2]
+    page, row = slots // P, slots % P
+    k_pages[page, :, row] = k.to(k_pages.dtype)
+    v_pages[page, :, row] = v.to(v_pages.dtype)
+
+
+def _weights(z):
+    z = torch.exp(z - z.amax(-1, keepdim=True))
+    return z / z.sum(-1, keepdim=True)
+
+
+def _plain_step(state, selected):
+    """Every request one new token: the batch padded to its longest request."""
+    case = state["case"]
+    R, H, D, P, E = case["R"], case["H"], case["D"], case["P"], case["exempt"]
+    G = selected.shape[1]
+    table = state["table"].clamp_min(0)
+    T = table.shape[1] * P
+
+    def rows(pages):
+        return pages[table].transpose(1, 2).reshape(R, H, T, D).float()
+
+    logits = (rows(state["k_pages"]) @ state["q"].float()[..., None])[..., 0] / math.sqrt(D)   # (R, H, T)
+    pos = torch.arange(T, device=logits.device)
+    last = state["lengths"][:, None, None] - 1
+    history = torch.where(pos < last, selected[..., :T], 0.0)
+    z = logits.view(R, G, H // G, T) - history[:, :, None]
+    p = _weights(z.masked_fill((pos > last)[:, :, None], float("-inf"))).view(R, H, 1, T)
+    out = (p @ torch.where((pos <= last)[..., None], rows(state["v_pages"]), 0.0))[:, :, 0]
+    chosen = torch.where((pos >= E) & (pos < last), logits.view(R, G, H // G, T)[:, :, 0].clamp_min(0.0), 0.0)
+    selected[..., :T] = torch.where(pos <= last, history + chosen, selected[..., :T])
+    return out.to(state["q"].dtype)
+
+
+def _plain_chunks(state, selected):
+    """Request after request, group after group; the heads of a group together as far as memory allows."""
+    case = state["case"]
+    H, D, P, E = case["H"], case["D"], case["P"], case["exempt"]
+    G = selected.shape[1]
+    per = H // G
+    q, out = state["q"], torch.empty_like(state["q"])
+    first = 0
+    for r, (c, n) in enumerate(zip(state["cs"], state["ns"])):
+        t = c + n
+        pages = [x[state["table"][r, :_pages_of(t, P)]].transpose(0, 1).reshape(H, -1, D)[:, :t].float()
+                 for x in (state["k_pages"], state["v_pages"])]
+        rows = q[first:first + n].transpose(0, 1).float()
+        pos = torch.arange(t, device=q.device)
+        at = pos[c:, None]
+        masked = pos > at
+        selectable = (pos >= E) & (pos < at)
+        together = max(1, min(per, (1 << 28) // (n * t)))
+        for g in range(G):
+            for h in range(g * per, (g + 1) * per, together):
+                heads = slice(h, min(h + together, (g + 1) * per))
+                logits = (rows[heads] @ pages[0][heads].transpose(1, 2)) / math.sqrt(D)
+                if h == g * per:
+                    chosen = torch.where(selectable, logits[0].clamp_min(0.0), 0.0)
+                    upto = torch.cumsum(chosen, 0)
+                    before = selected[r, g, :t]
+                    before[c:] = 0.0
+                    F = before + (upto - chosen)
+                    before += upto[-1]
+                p = _weights((logits - F).masked_fill(masked, float("-inf")))
+                out[first:first + n, heads] = (p @ pages[1][heads]).transpose(0, 1).to(out.dtype)
+        first += n
+    return out
+
+
+# -- what a pass cannot do without ------------------------------------------------------------------------
+
+# Under normal selection a key's weight falls below the smallest fp32 number about this many queries after it.
+_REACH = 260
+
+
+def work(case):
+    """Each input once, each output once. Attention: two products on every pair that carries weight, and the
+    selectors' logits on all of them; the pages of every key some query gives weight to, the selectors' keys all."""
+    cs, ns = _lengths(case) if case["kind"] != "append" else (None, None)
+    P = case["P"]
+    if case["kind"] == "plan":
+        N, R = sum(ns), case["R"]
+        pages = sum(_pages_of(c + n, P) - _pages_of(c, P) for c, n in zip(cs, ns))
+        pages += round(case["ended"] * sum(_pages_of(c, P) for c in cs))
+        return {"bytes": float(8 * R + 8 * pages + 12 * R + 8 * N), "flops": 0.0}
+    es = 4 if case["dtype"] == "f32" else 2
+    if case["kind"] == "append":
+        row = case["H"] * case["D"]
+        return {"bytes": float(case["N"] * (2 * row * ((4 if case["source"] == "f32" else 2) + es) + 8)), "flops": 0.0}
+    H, D = case["H"], case["D"]
+    G = H if case["per_head"] else 1
+    tokens, keys = sum(ns), sum(c + n for c, n in zip(cs, ns))
+    pairs = weighted = _pairs(cs, ns)
+    live = keys
+    if case["select"] == "normal":
+        near = [(min(c, _REACH), n) for c, n in zip(cs, ns)]
+        weighted = sum(min(n * c + n * (n + 1) // 2, n * (_REACH + case["exempt"])) for c, n in zip(cs, ns))
+        live = min(keys, sum(a + n + case["exempt"] for a, n in near))
+    rows = (H + H) * live + (keys - live) * G
+    return {"bytes": float(rows * D * es + 2 * tokens * H * D * es + 8 * G * keys + 4 * keys / P),
+            "flops": 4.0 * H * D * weighted + 2.0 * G * D * (pairs - weighted)}
+
+
+# -- the same in 64 bits ----------------------------------------------------------------------------------
+
+def exact(case, seed):
+    """From the definition, in float64, by blocks of queries with the history carried between them."""
+    if case["kind"] == "plan":
+        return None   # whole numbers only
+    s = prepare(case, seed)
+    if case["kind"] == "append":
+        kp, vp = s["k_pages"].double(), s["v_pages"].double()
+        flat = [x.transpose(1, 2).reshape(-1, case["H"], case["D"]) for x in (kp, vp)]   # slot-major
+        for x, new in zip(flat, (s["k"], s["v"])):
+            x[s["slots"]] = new.double()
+        return tuple(x.reshape(-1, case["P"], case["H"], case["D"]).transpose(1, 2).contiguous() for x in flat)
+    H, D, P = case["H"], case["D"], case["P"]
+    f64 = dict(dtype=torch.float64, device="cuda")
+    out, after = torch.empty(s["q"].shape, **f64), s["selected"].double()
+    G = after.shape[1]
+    scale = D ** -0.5
+    for r in range(case["R"]):
+        c, n = s["cs"][r], s["ns"][r]
+        t, first = c + n, sum(s["ns"][:r])
+        pages = s["table"][r, :_pages_of(t, P)].long()
+        key = torch.arange(t, device="cuda")
+        for g in range(G):
+            heads = range(g * (H // G), (g + 1) * (H // G))
+            K = [s["k_pages"][pages][:, h].reshape(-1, D)[:t].double() for h in heads]
+            V = [s["v_pages"][pages][:, h].reshape(-1, D)[:t].double() for h in heads]
+            run = after[r, g, :t].clone()
+            run[c:] = 0.0
+            for a in range(0, n, 512):
+                b = min(a + 512, n)
+                hi = c + b   # no query of the block sees a key past it
+                where = torch.arange(c + a, c + b, device="cuda")[:, None]
+                Q = [s["q"][first + a:first + b, h].double() for h in heads]
+                sel = (Q[0] @ K[0][:hi].T * scale).clamp_min(0.0)
+                sel *= (key[:hi] >= case["exempt"]) & (key[:hi] < where)
+                F = run[:hi] + torch.cumsum(sel, 0) - sel
+                for u, h in enumerate(heads):
+                    z = Q[u] @ K[u][:hi].T * scale - F
+                    z = z.masked_fill(key[:hi] > where, -math.inf)
+                    out[first + a:first + b, h] = torch.softmax(z, -1) @ V[u][:hi]
+                run[:hi] += sel.sum(0)
+            after[r, g, :t] = run
+    return out, after
