@@ -300,7 +300,7 @@ def _plain_plan(cached, new, table, free, taken, P, tokens, finished):
     take = base + upto - need
     fresh = (column >= have[:, None]) & (column < want[:, None]) & served[:, None]
     table.copy_(torch.where(fresh, free[(take[:, None] + column - have[:, None]).clamp(0, F - 1)], table))
-    after = base + torch.where(served, upto, 0).max()
+    after = base + torch.where(served & (need > 0), upto, 0).max()
     starts = torch.cat([zero[:1], ends])
     token = torch.arange(tokens, device=table.device)
     r = torch.searchsorted(ends, token, right=True).clamp(max=cached.shape[0] - 1)
