@@ -39,6 +39,7 @@ extern "C" {
 
 #define SA_DTYPE_BF16 0
 #define SA_DTYPE_F32 1
+#define SA_DTYPE_F16 2          /* the paged cache's entry points only */
 
 #define SA_OK 0
 #define SA_ERR_ARGUMENT -1      /* a size, pointer or option is invalid */
@@ -238,6 +239,60 @@ int sa_decode(const void* q, const void* k, const void* v, float* out, float* se
 int sa_decode_noalloc(const void* q, const void* k, const void* v, float* out, float* selected, int64_t state_ld,
                       int64_t nseq, int64_t heads, int64_t groups, int64_t t, int64_t kv_stride, int64_t head_dim,
                       float scale, int dtype, int exempt, void* stream);
+
+/*
+ * A paged cache, for batches of requests of different lengths (no counterpart in the reference). k_pages and
+ * v_pages are (pages, heads, page_size, head_dim), contiguous, page_size a power of two from 8 on; position j of
+ * request r sits in page table[r][j / page_size], row j % page_size. Lengths, tables and counts are int32 on the
+ * device: no entry point reads them on the host. head_dim 16, 32, 64 or 128; up to 65535 requests, 2^24 - 1 tokens.
+ *
+ * sa_page_plan: the tables of one step, from the requests' lengths. Request r has cached[r] positions in the cache
+ * and gets new_tokens[r] new ones (0: none; negative counts as 0). free_pages[taken[0] .. pool) are the free pages,
+ * a stack. First, for every request whose finished[r] is not 0 (finished may be NULL), the pages of its cached positions
+ * go back on the stack, request after request, and its row starts again with no position. Then requests get, in
+ * order, the pages their new positions need; a request whose pages and those of the requests before it are more
+ * than there are, or whose positions the table's `width` columns do not hold, or whose rows lie past `tokens`, is
+ * left out of the step. Writes:
+ *   table      the new entries of the requests served
+ *   starts     (requests + 1) the first token row of every request: the sums of new_tokens, at most `tokens`
+ *   lengths    (requests) positions after the step; 0 for a request left out
+ *   cached_out (requests) what the cache holds after the step
+ *   slots      (tokens) page * page_size + row of every token; -1: a request left out, or a row behind the last
+ *   taken_out  (1) may be `taken` itself
+ */
+int sa_page_plan(const int32_t* cached, const int32_t* new_tokens, const uint8_t* finished, int32_t* table, int64_t table_ld,
+                 int32_t* free_pages, const int32_t* taken, int32_t* starts, int32_t* lengths, int32_t* cached_out,
+                 int64_t* slots, int32_t* taken_out, int64_t requests, int64_t width, int64_t pool, int64_t tokens,
+                 int64_t page_size, void* stream);
+
+/* Writes tokens' key and value rows into the cache: row i to slot slots[i] (distinct; slots outside the cache: row left
+ * out), rounded from src_dtype to the cache's dtype. k, v: element strides of a token and of a head, 16-byte
+ * multiples, 16-byte aligned rows. */
+int sa_paged_append(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                    void* k_pages, void* v_pages, const int64_t* slots, int64_t tokens, int64_t heads, int64_t head_dim,
+                    int64_t pages, int64_t page_size, int src_dtype, int dtype, void* stream);
+
+/*
+ * The attention of one step: token rows starts[r] .. starts[r + 1] - 1 of q are the newest positions of request r,
+ * whose keys and values, these tokens' included, are the cache's first lengths[r] positions. The operator is
+ * sa_forward's with the carried selection (per request q_offset = lengths[r] - its new tokens):
+ *   q         element strides of a token and of a head (16-byte multiples, as for sa_paged_append), the cache's dtype
+ *   out       (tokens, heads, head_dim), the cache's dtype; rows of no request, and of requests left out, become 0
+ *   selected  (requests, groups, state_ld) fp32: the selection every cached position has received (groups as for
+ *             sa_decode); updated in place, entries of the new positions overwritten whatever they held
+ * max_new, max_len: upper bounds of a request's new tokens and positions, max_len within the table's `width` columns
+ * and state_ld. A request past them, or with fewer positions than new tokens, is left out: its state stays. Positions
+ * whose page lies outside the cache read as zero keys and values. max_new 1 runs the single-token kernels, which read the
+ * cache once; the workspace (16-byte aligned) depends on both bounds. The cache's arithmetic: logits, F, statistics and sums fp32; with several
+ * tokens a bf16 or fp16 cache's products run on matrix instructions of that type, the weights rounded to it.
+ */
+int64_t sa_paged_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t head_dim,
+                                           int64_t max_new, int64_t max_len, int dtype);
+int sa_paged_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_pages, const void* v_pages, void* out,
+                       const int32_t* table, int64_t table_ld, const int32_t* lengths, const int32_t* starts, float* selected,
+                       int64_t state_ld, void* workspace, int64_t workspace_bytes, int64_t requests, int64_t tokens,
+                       int64_t heads, int64_t groups, int64_t head_dim, int64_t pages, int64_t page_size, int64_t width,
+                       int64_t max_new, int64_t max_len, float scale, int dtype, int exempt, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,6 +18,8 @@
 #   sa_bf16_prep.hip  the bf16 backward preparation, the compiler's own accumulator placement (the
 #                options of sa_bf16.hip crash this compiler on one of its instances)
 #   sa_f32.hip   fp32-storage kernels, the compiler's own accumulator placement
+#   sa_paged_bf16.hip, sa_paged_f16.hip, sa_paged_f32.hip  attention over a paged cache of that type
+#   sa_paged.hip the paged cache's C ABI, its tables and its write
 #   sa_abi.hip   the C ABI (host code only)
 # Every HIP compile: -packed-fp32-ops off (no v_pk_*_f32 from the compiler).
 set -euo pipefail
@@ -62,6 +64,14 @@ unit sa_f32.hip sa_f32.o &
 p2=$!
 unit sa_abi.hip sa_abi.o &
 p3=$!
+unit sa_paged_bf16.hip sa_paged_bf16.o -mllvm -amdgpu-mfma-vgpr-form &
+p9=$!
+unit sa_paged_f16.hip sa_paged_f16.o -mllvm -amdgpu-mfma-vgpr-form &
+p10=$!
+unit sa_paged_f32.hip sa_paged_f32.o &
+p11=$!
+unit sa_paged.hip sa_paged.o &
+p12=$!
 rc=0
 wait $p1 || rc=1
 wait $p2 || rc=1
@@ -71,9 +81,13 @@ wait $p5 || rc=1
 wait $p6 || rc=1
 wait $p7 || rc=1
 wait $p8 || rc=1
+wait $p9 || rc=1
+wait $p10 || rc=1
+wait $p11 || rc=1
+wait $p12 || rc=1
 [ $rc -eq 0 ] || { echo "build.sh: a compile failed" >&2; exit 1; }
 hipcc --offload-arch=gfx950 -shared -fPIC "$tmp/sa_bf16.o" "$tmp/sa_bf16_kv.o" "$tmp/sa_bf16_kv1.o" "$tmp/sa_bf16_kvg.o" "$tmp/sa_bf16_dec.o" "$tmp/sa_bf16_prep.o" "$tmp/sa_f32.o" \
-  "$tmp/sa_abi.o" \
+  "$tmp/sa_paged_bf16.o" "$tmp/sa_paged_f16.o" "$tmp/sa_paged_f32.o" "$tmp/sa_paged.o" "$tmp/sa_abi.o" \
   -o "$out.tmp"
 mv "$out.tmp" "$out"
 echo "built $out"

@@ -21,7 +21,7 @@ using namespace sa_host;
 
 extern "C" {
 
-int sa_abi_version(void) { return 7; }
+int sa_abi_version(void) { return 8; }
 
 int sa_timing_enable(int on) {
   TimingRegistry& r = timing();
@@ -57,7 +57,7 @@ const char* sa_status_string(int status) {
   switch (status) {
     case SA_OK: return "ok";
     case SA_ERR_ARGUMENT: return "invalid argument (size, pointer or option)";
-    case SA_ERR_HEAD_DIM: return "head_dim must be 32, 64 or 128 at the C ABI";
+    case SA_ERR_HEAD_DIM: return "head_dim must be 32, 64 or 128 at the C ABI (a paged cache: or 16)";
     case SA_ERR_DTYPE: return "unknown dtype code";
     case SA_ERR_WORKSPACE: return "workspace too small";
     case SA_ERR_LAUNCH: return "HIP kernel launch failed";

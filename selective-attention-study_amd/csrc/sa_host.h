@@ -353,4 +353,71 @@ SA_HIDDEN int backward_f32(const BwdCall& c);
 SA_HIDDEN int decode_bf16(const DecCall& c);     // sa_bf16_dec.hip
 SA_HIDDEN int decode_f32(const DecCall& c);      // sa_f32.hip
 
+// One sa_paged_attention call after its checks.
+struct PagedLaunch {
+  const void *q, *k_pages, *v_pages;
+  void* out;
+  const int *table, *lengths, *starts;
+  float* selected;
+  int64_t q_token, q_head, table_ld, state_ld;
+  void* ws;
+  int64_t R, N, H, G, pages, max_new, max_len;
+  int pshift;
+  float scale;
+  int exempt, head_dim;
+  hipStream_t st;
+};
+SA_HIDDEN int paged_bf16(const PagedLaunch& c);   // sa_paged_bf16.hip
+SA_HIDDEN int paged_f16(const PagedLaunch& c);    // sa_paged_f16.hip
+SA_HIDDEN int paged_f32(const PagedLaunch& c);    // sa_paged_f32.hip
+
+// How a step over a paged cache is launched, and its workspace. One new token per request (step): chunks of keys
+// per workgroup, partial maxima, sums and outputs, then the new state rows. Several: the selectors' histories
+// (carry), and where the key range is split the spans' partials.
+struct PagedShape {
+  bool step;
+  int nw, hg;                 // several tokens: wavefronts (32 query rows each) per workgroup, heads per wavefront
+  int splits, span_tiles;     // key spans, and their 32-key tiles
+  int chunk, carry_blocks;    // one token: keys per workgroup; several: workgroups along the keys of the histories
+  int64_t carry_ld;           // floats of a history row (one token: of a new state row)
+  int64_t carry, m, l, o, total;   // byte offsets (m: maxima, with several tokens (maximum, sum) pairs)
+};
+inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_t D, int64_t es, int64_t max_new, int64_t max_len) {
+  PagedShape s{};
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) { int64_t o = off; off = align_up(off + bytes, 256); return o; };
+  s.step = max_new == 1;
+  s.carry_ld = align_up(max_len, TILE);
+  if (s.step) {
+    // as decode_chunk: workgroups enough to fill the chip, chunks long enough to stream
+    int64_t chunk = 256;
+    while (chunk < 4096 && R * H * cdiv(max_len, chunk) > 2048) chunk *= 2;
+    s.chunk = (int)chunk;
+    s.splits = (int)cdiv(max_len, chunk);
+    s.m = take(R * H * s.splits * 4);
+    s.l = take(R * H * s.splits * 4);
+    s.o = take(R * H * s.splits * D * 4);
+    s.carry = take(R * G * s.carry_ld * 4);
+  } else {
+    const int64_t per = H / G;
+    s.nw = max_new <= TILE ? 1 : 4;
+    s.hg = es == 2 && D <= 64 && per % 2 == 0 ? 2 : 1;
+    const int64_t rows = (int64_t)s.nw * TILE;
+    const int64_t tiles = cdiv(max_len, TILE);
+    const int64_t workgroups = std::max(cdiv(N, rows), std::min(R, N)) * (H / s.hg);   // (of live tiles)
+    const int64_t target = s.nw == 4 ? 512 : 2048;
+    const int64_t splits = std::max<int64_t>(1, std::min(cdiv(target, workgroups), cdiv(tiles, 16)));
+    s.span_tiles = (int)cdiv(tiles, splits);
+    s.splits = (int)cdiv(tiles, s.span_tiles);
+    s.carry_blocks = (int)std::max<int64_t>(1, std::min(cdiv(tiles, NWAVES), cdiv(8192, R * G)));
+    s.carry = take((N / TILE + R) * G * s.carry_ld * 4);
+    if (s.splits > 1) {
+      s.m = take(s.splits * N * H * 8);
+      s.o = take(s.splits * N * H * D * 4);
+    }
+  }
+  s.total = off;
+  return s;
+}
+
 }  // namespace sa_host

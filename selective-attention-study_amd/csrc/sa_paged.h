@@ -1,0 +1,1218 @@
+// Selective Attention over a paged cache (gfx950): the step's tables, the cache write, and the attention of a
+// ragged batch of new tokens over pages.
+//
+// A cache is k_pages, v_pages (pages, H, P, D): a page holds P consecutive positions of one request, every head's
+// rows together, so that one head's keys of a page are P D contiguous elements. A request's positions are found
+// through its table row: position j in page table[r][j / P], row j % P. The per-key selection state belongs to the
+// request, not to the page (two requests that share a page have asked different queries): (R, G, L) fp32 rows.
+//
+// Per request with c cached and n new tokens, t = c + n (operator: sa_kernels.h):
+//   F[i, j] = state[j] (j < c, else 0) + sum over the chunk's queries r < i of relu(s q_sel[r].k_sel[j]),
+//             exempt <= j < c + r;    out_h = softmax_j(s q_h.k_h - F) V_h;    state[j] = F after the last query
+//
+// Kernels:
+//   page_plan, page_slots   the step's tables from the requests' lengths
+//   paged_append            new rows into the pages
+//   paged_carry             n > 1: each selector's history on entry to every 32-query tile, and the new state
+//   paged_fwd               n > 1: a wavefront's 32 queries of one or two heads over the key tiles of a span
+//   paged_join              the spans' partial results of a query joined
+//   paged_step, paged_step_join    n = 1: the cache read once in fp32 arithmetic, split over workgroups
+
+#pragma once
+
+#include "sa_kernels.h"
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// Cache element types: 16-byte chunks of a row are the unit that loads, LDS and the matrix operands share. mma
+// contracts one chunk per lane (lanes 0-31 the even, lanes 32-63 the odd chunk of their row): one bf16 or fp16
+// instruction, or four fp32 ones that take element e of both halves' chunks (the order of a contraction is free as
+// long as both operands have the same).
+struct PagedBF16 {
+  typedef uint16_t elem;
+  static constexpr int EPC = 8;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ u32x4 pack(const f32x16& x, int s) {   // round to nearest even
+    bf16x8 f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) f[t] = (bf16_t)x[8 * s + t];
+    return __builtin_bit_cast(u32x4, f);
+  }
+  static __device__ __forceinline__ float to_float(elem x) { return __uint_as_float((uint32_t)x << 16); }
+  static __device__ __forceinline__ elem to_elem(float x) { return __builtin_bit_cast(elem, (bf16_t)x); }
+};
+struct PagedF16 {
+  typedef uint16_t elem;
+  static constexpr int EPC = 8;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ u32x4 pack(const f32x16& x, int s) {
+    f16x8 f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) f[t] = (_Float16)x[8 * s + t];
+    return __builtin_bit_cast(u32x4, f);
+  }
+  static __device__ __forceinline__ float to_float(elem x) { return (float)__builtin_bit_cast(_Float16, x); }
+  static __device__ __forceinline__ elem to_elem(float x) { return __builtin_bit_cast(elem, (_Float16)x); }
+};
+struct PagedF32 {
+  typedef float elem;
+  static constexpr int EPC = 4;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ float to_float(elem x) { return x; }
+  static __device__ __forceinline__ elem to_elem(float x) { return x; }
+};
+
+// ---------------------------------------------------------------------------------------------
+// Requests of a ragged batch. Tiles of 1 << sh query rows are numbered without a table of their own: request r's
+// tiles take the numbers from (starts[r] >> sh) + r on, as many as it can need (a request of n rows covers at most
+// ((starts[r] + n) >> sh) - (starts[r] >> sh) + 1 tiles), so N rows of R requests have (N >> sh) + R numbers. sh = 31
+// numbers the requests themselves, sh = 0 with `plain` the rows.
+//
+// The request that holds number x: the last r with first(r) <= x. All 64 lanes probe at once, 64-fold narrower each
+// round: one round of loads up to 64 requests, two up to 4096. Called by whole wavefronts; any contents of `starts`
+// give an r in [0, R).
+template <bool ROWS>
+__device__ __forceinline__ int find_request(const int* starts, int R, int x, int sh) {
+  const int lane = threadIdx.x & 63;
+  int base = 0, n = R;
+  while (n > 1) {
+    const int stride = (n + 63) >> 6;
+    const int i = lane * stride;
+    bool at = false;
+    if (i < n) {
+      const int s = starts[base + i];
+      at = ROWS ? s <= x : (s >> sh) + base + i <= x;
+    }
+    const int hit = max(__popcll(__ballot(at)), 1) - 1;
+    base += hit * stride;
+    n = min(stride, n - hit * stride);
+    if (stride == 1) break;
+  }
+  return __builtin_amdgcn_readfirstlane(min(base, R - 1));
+}
+
+struct PagedCall {
+  const void *q, *k_pages, *v_pages;
+  void* out;
+  const int *table, *lengths, *starts;
+  float* selected;
+  int64_t q_token, q_head, table_ld, state_ld;
+  int R, N, H, G, pages, pshift;
+  int max_new, max_len;
+  float scale;
+  int exempt;
+};
+
+// One request's step: n new rows from token `first` on, c cached positions, t = c + n. A request that cannot be
+// served is left out (live = false): fewer positions than new rows, more than the table row, the state row or the
+// caller's bound holds, rows outside the batch, more new rows than the bound.
+struct PagedRequest {
+  int first, n, c, t;
+  bool live;
+};
+__device__ __forceinline__ PagedRequest paged_request(const PagedCall& a, int r) {
+  PagedRequest q;
+  q.first = __builtin_amdgcn_readfirstlane(a.starts[r]);
+  const int end = __builtin_amdgcn_readfirstlane(a.starts[r + 1]);
+  q.t = __builtin_amdgcn_readfirstlane(a.lengths[r]);
+  const bool rows = q.first >= 0 && end > q.first && end <= a.N;
+  q.n = rows ? end - q.first : 0;
+  q.c = q.t - q.n;
+  q.live = rows && q.t >= q.n && q.t <= a.max_len && q.n <= a.max_new;   // (max_len: within the table and state rows)
+  return q;
+}
+
+static __device__ uint4 paged_zero_row;   // what rows without a page read
+
+// ---------------------------------------------------------------------------------------------
+// The step's tables. One workgroup (a step's scans run over the requests, some hundreds); bound by its latency:
+// two block scans and one round trip each for the lengths, the stack and the table.
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_WAVES = PLAN_THREADS / 64;
+constexpr int PLAN_SLOTS = 4096;   // tokens up to which the same workgroup makes the slot map
+
+struct PlanCall {
+  const int *cached, *fresh;
+  const uint8_t* finished;
+  int* table;
+  int* stack;
+  const int* taken;
+  int *starts, *lengths, *cached_out, *taken_out;
+  int64_t* slots;
+  int64_t table_ld;
+  int R, W, F, N, pshift;
+  bool slots_here;   // the slot map too; else page_slots_kernel makes it
+};
+
+__device__ __forceinline__ int wave_scan_incl(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// Inclusive sums over the workgroup's threads of two values, and their totals. Saturated inputs (each at most 2^30
+// over 1024 threads) would overflow 32 bits: the callers clamp what they add.
+struct Sum2 {
+  int64_t a, b, ta, tb;
+};
+__device__ __forceinline__ int64_t wave_scan_incl64(int64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ Sum2 block_scan2(int64_t a, int64_t b, int64_t (*sh)[2]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  a = wave_scan_incl64(a);
+  b = wave_scan_incl64(b);
+  if (lane == 63) {
+    sh[wave][0] = a;
+    sh[wave][1] = b;
+  }
+  __syncthreads();
+  Sum2 s{a, b, 0, 0};
+#pragma unroll
+  for (int w = 0; w < PLAN_WAVES; ++w) {
+    if (w < wave) {
+      s.a += sh[w][0];
+      s.b += sh[w][1];
+    }
+    s.ta += sh[w][0];
+    s.tb += sh[w][1];
+  }
+  __syncthreads();
+  return s;
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanCall a) {
+  __shared__ int64_t sh[PLAN_WAVES][2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int P = 1 << a.pshift;
+  const auto pages_of = [&](int64_t x) { return (int)((x + P - 1) >> a.pshift); };
+  int64_t base = min(max(a.taken[0], 0), a.F);   // first free entry of the stack
+
+  // finished requests' pages go back, request after request
+  if (a.finished) {
+    int64_t total = 0;
+    for (int r0 = 0; r0 < a.R; r0 += PLAN_THREADS) {
+      const int r = r0 + tid;
+      const int back = r < a.R && a.finished[r] ? min(pages_of(max(a.cached[r], 0)), a.W) : 0;
+      total += block_scan2(back, 0, sh).ta;
+    }
+    int64_t at = base - total;
+    base = max(at, (int64_t)0);
+    for (int r0 = 0; r0 < a.R; r0 += PLAN_THREADS) {
+      const int r = r0 + tid;
+      const int back = r < a.R && a.finished[r] ? min(pages_of(max(a.cached[r], 0)), a.W) : 0;
+      const Sum2 s = block_scan2(back, 0, sh);
+      const int64_t to = at + s.a - back;
+      uint64_t todo = __ballot(back > 0);
+      while (todo) {   // a wavefront copies its requests' table rows one after another
+        const int l = __ffsll((unsigned long long)todo) - 1;
+        todo &= todo - 1;
+        const int rr = __shfl(r, l), nn = __shfl(back, l);
+        const int64_t tt = __shfl(to, l);
+        for (int i = lane; i < nn; i += 64)
+          if (tt + i >= 0) a.stack[tt + i] = a.table[rr * a.table_ld + i];
+      }
+      at += s.ta;
+    }
+    __threadfence_block();
+    __syncthreads();
+  }
+
+  // pages for the new tokens, in request order: all a request needs, or none
+  int64_t row = 0, given = 0;   // rows and needs of the requests before this strip
+  int64_t most = 0;             // needs up to the last request served
+  const int64_t avail = a.F - base;
+  for (int r0 = 0; r0 < a.R; r0 += PLAN_THREADS) {
+    const int r = r0 + tid;
+    int c = 0, n = 0;
+    if (r < a.R) {
+      c = a.finished && a.finished[r] ? 0 : max(a.cached[r], 0);
+      n = max(a.fresh[r], 0);
+    }
+    const int64_t t = (int64_t)c + n;
+    const int have = pages_of(c);
+    const bool fits = t <= ((int64_t)a.W << a.pshift);
+    const int need = fits ? pages_of(t) - have : 0;
+    const Sum2 s = block_scan2(n, need, sh);
+    const int64_t first = row + s.a - n, end = row + s.a, upto = given + s.b;
+    const bool served = r < a.R && fits && end <= a.N && (need == 0 || upto <= avail);
+    const int64_t from = base + upto - need;   // the request's first entry of the stack
+    if (served && need) most = max(most, upto);
+    if (r < a.R) {
+      a.starts[r] = (int)min(first, (int64_t)a.N);
+      a.lengths[r] = served ? (int)t : 0;
+      a.cached_out[r] = served ? (int)t : c;
+      if (r == a.R - 1) a.starts[a.R] = (int)min(end, (int64_t)a.N);
+    }
+    int* trow = a.table + (int64_t)r * a.table_ld;
+    // the page of the first new token: the last one held, unless that is full
+    const bool one = served && need <= 1 && n <= 1;
+    if (one && n == 1) {
+      int page;
+      if (need) {
+        page = a.stack[from];
+        trow[have] = page;
+      } else {
+        page = trow[c >> a.pshift];
+      }
+      if (a.slots_here) a.slots[first] = ((int64_t)page << a.pshift) + (c & (P - 1));
+    }
+    uint64_t todo = __ballot(r < a.R && n > 0 && !one);
+    while (todo) {   // the others: a wavefront's lanes together, request after request
+      const int l = __ffsll((unsigned long long)todo) - 1;
+      todo &= todo - 1;
+      const int rr = r0 + (tid & ~63) + l, nn = __shfl(n, l), cc = __shfl(c, l), hv = __shfl(have, l), nd = __shfl(need, l);
+      const bool ok = __shfl((int)served, l) != 0;
+      const int64_t fr = __shfl(from, l), ro = __shfl(first, l);
+      int* tr = a.table + (int64_t)rr * a.table_ld;
+      if (ok)
+        for (int i = lane; i < nd; i += 64) tr[hv + i] = a.stack[fr + i];
+      if (a.slots_here)
+        for (int i = lane; i < nn && ro + i < a.N; i += 64) {
+          const int pos = cc + i, p = pos >> a.pshift;
+          const int page = !ok ? -1 : p < hv ? tr[p] : a.stack[fr + p - hv];
+          a.slots[ro + i] = ok ? ((int64_t)page << a.pshift) + (pos & (P - 1)) : -1;
+        }
+    }
+    row += s.ta;
+    given += s.tb;
+  }
+  if (a.slots_here)
+    for (int64_t i = row + tid; i < a.N; i += PLAN_THREADS) a.slots[i] = -1;   // rows behind the last request
+  // the last served request's needs: the largest over the threads
+  for (int o = 32; o > 0; o >>= 1) most = max(most, (int64_t)__shfl_xor(most, o));
+  __syncthreads();
+  if (lane == 0) sh[tid >> 6][0] = most;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < PLAN_WAVES; ++w) most = max(most, sh[w][0]);
+    a.taken_out[0] = (int)(base + most);
+  }
+}
+
+// The slot map of a long batch: a thread per token, its request found by bisection of `starts` (in the L2).
+__global__ __launch_bounds__(NTHREADS) void page_slots_kernel(const int* __restrict__ starts, const int* __restrict__ lengths,
+                                                              const int* __restrict__ table, int64_t table_ld,
+                                                              int64_t* __restrict__ slots, int R, int W, int N, int pshift) {
+  const int i = blockIdx.x * NTHREADS + threadIdx.x;
+  if (i >= N) return;
+  int lo = 0, hi = R;   // starts[lo] <= i < starts[hi]
+  int64_t slot = -1;
+  if (i < starts[R]) {
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (starts[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+    const int first = starts[lo], t = lengths[lo];
+    const int pos = t - (starts[lo + 1] - first) + i - first;
+    if (t > 0 && pos >= 0) slot = ((int64_t)table[lo * table_ld + (pos >> pshift)] << pshift) + (pos & ((1 << pshift) - 1));
+  }
+  slots[i] = slot;
+}
+
+// ---------------------------------------------------------------------------------------------
+// New rows into the pages: a thread per 16-byte chunk of the cache (k's and v's), so that eight lanes write one
+// head's row of a page and neighbouring lanes the next heads'. Bound by HBM. Rows whose slot is not in the cache
+// are left out.
+struct AppendCall {
+  const void *k, *v;
+  void *k_pages, *v_pages;
+  const int64_t* slots;
+  int64_t k_token, k_head, v_token, v_head;
+  int64_t total;   // slots of the cache
+  int N, H, pshift;
+};
+
+// `n` elements of type S from p as the cache's type.
+template <class S, class P>
+__device__ __forceinline__ u32x4 convert_chunk(const typename S::elem* p) {
+  if constexpr (std::is_same<S, P>::value) {
+    return *reinterpret_cast<const u32x4*>(p);
+  } else {
+    union {
+      u32x4 u[2];
+      typename S::elem e[32 / sizeof(typename S::elem)];
+    } in;
+    union {
+      u32x4 u;
+      typename P::elem e[P::EPC];
+    } out;
+    if constexpr (sizeof(typename S::elem) * P::EPC == 8) {   // four 16-bit elements to fp32
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      in.u[0][0] = x.x;
+      in.u[0][1] = x.y;
+    } else {
+      in.u[0] = reinterpret_cast<const u32x4*>(p)[0];
+      if constexpr (sizeof(typename S::elem) * P::EPC == 32) in.u[1] = reinterpret_cast<const u32x4*>(p)[1];
+    }
+#pragma unroll
+    for (int e = 0; e < P::EPC; ++e) out.e[e] = P::to_elem(S::to_float(in.e[e]));
+    return out.u;
+  }
+}
+
+template <class S, class P, int D>
+__global__ __launch_bounds__(NTHREADS) void paged_append_kernel(AppendCall a) {
+  constexpr int CPR = D / P::EPC;
+  const uint32_t per = (uint32_t)a.H * CPR;
+  const uint64_t id = (uint64_t)blockIdx.x * NTHREADS + threadIdx.x;
+  const int token = (int)(id / per);
+  if (token >= a.N) return;
+  const uint32_t x = (uint32_t)(id - (uint64_t)token * per);
+  const int head = (int)(x / CPR), c = (int)(x % CPR);
+  const int64_t slot = a.slots[token];
+  if (slot < 0 || slot >= a.total) return;
+  const int64_t page = slot >> a.pshift;
+  const int rowi = (int)(slot & ((1 << a.pshift) - 1));
+  const int64_t to = (((page * a.H + head) << a.pshift) + rowi) * D + c * P::EPC;
+  typedef typename S::elem se;
+  typedef typename P::elem pe;
+  const u32x4 kc = convert_chunk<S, P>(static_cast<const se*>(a.k) + token * a.k_token + head * a.k_head + c * P::EPC);
+  const u32x4 vc = convert_chunk<S, P>(static_cast<const se*>(a.v) + token * a.v_token + head * a.v_head + c * P::EPC);
+  *reinterpret_cast<u32x4*>(static_cast<pe*>(a.k_pages) + to) = kc;
+  *reinterpret_cast<u32x4*>(static_cast<pe*>(a.v_pages) + to) = vc;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Tiles of 32 rows in LDS, rows of CPR 16-byte chunks end to end, chunk c of row r stored at chunk c ^ swz(r): read
+// both by lane-per-row fragments (16 rows, one logical chunk, per pass over the 64 banks) and transposed (four
+// consecutive rows, two or four consecutive chunks of each). Rows of 256 bytes or more cover every bank, so four
+// consecutive rows go to distinct quarters and the 16 rows of a pass to the 16 chunks; at 128 bytes two rows
+// share the banks and the pattern is swzq's; at 64 and 32 bytes four and eight rows do.
+template <int CPR>
+__device__ __forceinline__ int paged_swz(int r) {
+  if constexpr (CPR >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (CPR == 8) return ((r & 3) << 1) ^ ((r >> 2) & 3);
+  else if constexpr (CPR == 4) return (r >> 2) & 3;
+  else return (r >> 3) & 1;
+}
+
+template <class P, int D>
+struct PagedTile {
+  typedef typename P::elem elem;
+  static constexpr int ES = (int)sizeof(elem), RB = D * ES, CPR = RB / 16, BYTES = TILE * RB;
+  static constexpr int NS = CPR / 2 > 0 ? CPR / 2 : 1;   // contraction steps of a row
+  static constexpr int PARTS = BYTES / 1024;             // direct loads that fill a tile
+  static constexpr int DB = D < 32 ? 1 : D / 32;         // 32-column blocks of a value row
+  static_assert(CPR >= 2, "a row of at least two chunks");
+
+  // the fragment of step s of row n
+  static __device__ __forceinline__ u32x4 row_frag(const char* t, int n, int h, int s) {
+    return *reinterpret_cast<const u32x4*>(t + n * RB + (((2 * s + h) ^ paged_swz<CPR>(n)) << 4));
+  }
+  // o (columns 32 db ..) += V^T P for the tile's rows, P in the accumulator's layout (lane = query)
+  static __device__ __forceinline__ f32x16 values(const char* t, int lane, int db, const u32x4* pf, const f32x16& p, f32x16 o) {
+    if constexpr (ES == 2) {
+      const int g = lane >> 4, k = lane & 15;
+      // (a row of 16 columns: its upper 16 lanes read some of the same, for output rows that nobody keeps)
+      const int c = (4 * db + 2 * (g & 1) + ((k & 3) >> 1)) & (CPR - 1);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4 f;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int r = 16 * s + 8 * hf + 4 * (g >> 1) + (k >> 2);
+          typedef __attribute__((address_space(3))) short4v* lds_s4;
+          const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s4)lds_ptr(t + r * RB + ((c ^ paged_swz<CPR>(r)) << 4) + 8 * (k & 1)));
+          const uint2 u = __builtin_bit_cast(uint2, x);
+          f[2 * hf] = u.x;
+          f[2 * hf + 1] = u.y;
+        }
+        o = P::mma(f, pf[s], o);
+      }
+    } else {
+      const int n = lane & 31, h = lane >> 5, d = (32 * db + n) & (D - 1);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = crow(i, h);
+        const float x = *reinterpret_cast<const float*>(t + r * RB + (((d >> 2) ^ paged_swz<CPR>(r)) << 4) + 4 * (d & 3));
+        o = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], o, 0, 0, 0);
+      }
+    }
+    return o;
+  }
+};
+
+__device__ __forceinline__ void g2l16(const void* g, void* l) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, lds_ptr(l), 16, 0, 0);
+}
+
+// A lane's rows of the tiles that NW wavefronts load together: part m of a tile (m = wave, wave + NW, ...) is 64
+// chunks, lane l's the chunk at 64 m + l, which holds logical chunk (l % CPR) ^ swz(row) of row (64 m + l) / CPR.
+template <class P, int D, int NW>
+struct PagedRows {
+  typedef PagedTile<P, D> T;
+  static constexpr int PER = (T::PARTS + NW - 1) / NW;
+  const int* trow;      // the request's table row
+  int pshift, pages, t;
+  int64_t page_bytes;   // all heads of a page
+  int row[PER], col[PER];
+
+  __device__ __forceinline__ PagedRows(const PagedCall& a, int r, int t_, int wave, int lane)
+      : trow(a.table + r * a.table_ld), pshift(a.pshift), pages(a.pages), t(t_),
+        page_bytes(((int64_t)a.H << a.pshift) * T::RB) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = 64 * (wave + NW * i) + lane;
+      row[i] = at / T::CPR;
+      col[i] = ((at % T::CPR) ^ paged_swz<T::CPR>(row[i])) << 4;
+    }
+  }
+  // the pages of key tile kt's rows (-1: none); a tile before the first has none
+  __device__ __forceinline__ void pages_of(int kt, int (&pg)[PER]) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int j = kt * TILE + row[i];
+      pg[i] = (kt >= 0 && j < t) ? trow[j >> pshift] : -1;
+    }
+  }
+  // byte offsets of the lane's chunks in the cache (head 0; -1: no page in the cache)
+  __device__ __forceinline__ void offsets(int kt, const int (&pg)[PER], int64_t (&off)[PER]) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int in = (kt * TILE + row[i]) & ((1 << pshift) - 1);
+      off[i] = (uint32_t)pg[i] < (uint32_t)pages ? pg[i] * page_bytes + in * T::RB + col[i] : -1;
+    }
+  }
+  // the rows of one head (its offset within a page: `head`) into a tile
+  __device__ __forceinline__ void load(char* tile, const char* base, const int64_t (&off)[PER], int wave) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int m = wave + NW * i;
+      if (m < T::PARTS) g2l16(off[i] >= 0 ? base + off[i] : reinterpret_cast<const char*>(&paged_zero_row), tile + 1024 * m);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// The selectors' histories of a step of several tokens: carry[tile][g][j], what key j has received before the
+// tile's first query, and the state after the step. A wavefront owns 32 keys of one selector (rows in registers)
+// and walks the request's query tiles, as sel_carry64_kernel does; the query rows come straight from the L2, one
+// tile ahead. Rows of keys that no query of a tile sees are not written: the forward masks those keys.
+template <class P, int D>
+__global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, float* __restrict__ carry, int64_t carry_ld) {
+  typedef PagedTile<P, D> T;
+  typedef typename P::elem elem;
+  const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
+  const int r = blockIdx.z, g = blockIdx.y;
+  const PagedRequest rq = paged_request(a, r);
+  if (!rq.live) return;
+  const int hd = g * (a.H / a.G);
+  const int nkb = (rq.t + TILE - 1) / TILE, ntile = (rq.n + TILE - 1) / TILE;
+  const int tile0 = (rq.first >> 5) + r;
+  const elem* q = static_cast<const elem*>(a.q) + rq.first * a.q_token + hd * a.q_head;
+  const int* trow = a.table + r * a.table_ld;
+  float* state = a.selected + ((int64_t)r * a.G + g) * a.state_ld;
+  for (int kb = blockIdx.x * NWAVES + wave; kb < nkb; kb += gridDim.x * NWAVES) {
+    const int j = kb * TILE + n;
+    u32x4 kf[T::NS];
+    {
+      const int pg = j < rq.t ? trow[j >> a.pshift] : -1;
+      const bool ok = (uint32_t)pg < (uint32_t)a.pages;
+      const elem* k = static_cast<const elem*>(a.k_pages) +
+                      ((((int64_t)(ok ? pg : 0) * a.H + hd) << a.pshift) + (j & ((1 << a.pshift) - 1))) * D;
+#pragma unroll
+      for (int s = 0; s < T::NS; ++s)
+        kf[s] = ok ? *reinterpret_cast<const u32x4*>(k + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
+    }
+    float run = j < rq.c ? state[j] : 0.f;
+    auto load_q = [&](int rb, u32x4 (&qf)[T::NS]) {
+      const int row = rb * TILE + n;
+#pragma unroll
+      for (int s = 0; s < T::NS; ++s)
+        qf[s] = row < rq.n ? *reinterpret_cast<const u32x4*>(q + row * a.q_token + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
+    };
+    // tiles before rb_lo end before the block's first key
+    const int rb_lo = max(kb * TILE - rq.c, 0) / TILE;
+    u32x4 qa[T::NS], qb[T::NS];
+    load_q(rb_lo, qa);
+    for (int rb = rb_lo; rb < ntile; ++rb) {
+      load_q(rb + 1, qb);
+      if (h == 0 && j < rq.t) carry[((int64_t)(tile0 + rb) * a.G + g) * carry_ld + j] = run;
+      f32x16 acc = zero16();
+#pragma unroll
+      for (int s = 0; s < T::NS; ++s) acc = P::mma(qa[s], kf[s], acc);
+      const int qbase = rq.c + rb * TILE;
+      const bool interior = qbase > kb * TILE + TILE - 1 && kb * TILE >= a.exempt;
+      run += block_selection_sum(acc, interior, j >= a.exempt ? j - qbase - 4 * h : 32, a.scale);
+#pragma unroll
+      for (int s = 0; s < T::NS; ++s) qa[s] = qb[s];
+    }
+    if (h == 0 && j < rq.t) state[j] = run;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// The attention of a step of several tokens. Workgroup (x, y, z): query tiles of NW x 32 rows of one request
+// (numbered as above), heads y HG .. + HG - 1 (of one selector), key span z. As fwd64_kernel: a wavefront's 32
+// queries against one 32-key tile at a time, newest first, every operand loaded straight into LDS one tile ahead,
+// the selection (-F, through the wavefront's LDS rows) one tile ahead of the softmax. What differs is where rows come
+// from: each lane looks its row's page up one tile before the load.
+//
+// WHOLE: every head selects for itself (HG = 1): the wavefront's logits arrive with F already subtracted, and the
+// key tile is loaded once.
+//
+// P is rounded to the cache's type for the product with V (relative 2^-9 bf16, 2^-12 fp16 at random, the size of the
+// output's own rounding; fp32 not at all); logits, F, row statistics and sums are fp32.
+template <class P, int D, int HG, int NW>
+struct FwdLds {
+  typedef PagedTile<P, D> T;
+  struct Tiles {
+    __attribute__((aligned(16))) char k[HG][T::BYTES];
+    __attribute__((aligned(16))) char v[HG][T::BYTES];
+  };
+};
+
+template <class P, int D, int HG, int NW, bool WHOLE>
+__global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) == 2 && D <= 64) ? (HG == 1 ? 3 : 2) : 1)) void paged_fwd_kernel(
+    PagedCall a, const float* __restrict__ carry, int64_t carry_ld, int span_tiles, float* __restrict__ part_ml,
+    float* __restrict__ part_o) {
+  typedef PagedTile<P, D> T;
+  typedef typename P::elem elem;
+  typedef PagedRows<P, D, NW> Rows;
+  constexpr int NS = T::NS, DB = T::DB, PER = Rows::PER, LDF = TILE + 4;
+  constexpr int SH = NW == 4 ? 7 : 5;   // rows of a workgroup: 1 << SH
+  static_assert(!WHOLE || HG == 1, "a head that selects for itself alone");
+  // separate variables, so that the compiler knows a step's reads do not touch the buffers being filled. Lifetimes as
+  // in fwd64_kernel: sB0, sB1 the K and V rows of the t-th tile visited (buffer t mod 2; filled in step t - 1, read
+  // in step t); sS0, sS1 its selector's K rows (filled in step t - 2, read by the selection at the end of step t - 1); sF
+  // each wavefront's own. A step ends with every load landed and a barrier.
+  __shared__ typename FwdLds<P, D, HG, NW>::Tiles sB0, sB1;
+  __shared__ __attribute__((aligned(16))) char sS0[T::BYTES], sS1[T::BYTES];
+  __shared__ __attribute__((aligned(16))) float sF[NW][TILE * LDF];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = NW == 1 ? 0 : wave_id();
+  const int n = lane & 31, h = lane >> 5;
+  const int x = gridDim.x - 1 - blockIdx.x;
+  const int hd0 = blockIdx.y * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
+  elem* out = static_cast<elem*>(a.out);
+  const bool split = part_o != nullptr;
+
+  if (!split && blockIdx.z == 0) {   // rows behind the last request
+    const int hi = min((x + 1) << SH, a.N), lo = min(max(x << SH, a.starts[a.R]), hi);
+    for (int i = tid; i < (hi - lo) * (HG * D); i += NW * 64)
+      out[(int64_t)(lo + i / (HG * D)) * a.H * D + hd0 * D + i % (HG * D)] = P::to_elem(0.f);
+  }
+  const int r = find_request<false>(a.starts, a.R, x, SH);
+  const PagedRequest rq = paged_request(a, r);
+  const int row0 = (x - ((rq.first >> SH) + r)) << SH;   // the workgroup's first row of the request
+  if (row0 < 0 || row0 >= rq.n) return;
+  if (!rq.live) {
+    if (!split && blockIdx.z == 0)
+      for (int i = tid; i < min(1 << SH, rq.n - row0) * (HG * D); i += NW * 64)
+        out[(int64_t)(rq.first + row0 + i / (HG * D)) * a.H * D + hd0 * D + i % (HG * D)] = P::to_elem(0.f);
+    return;
+  }
+  const int kt_lo = blockIdx.z * span_tiles;
+  const int last_row = min(row0 + (1 << SH), rq.n) - 1;
+  const int kt_hi = min((rq.c + last_row) / TILE + 1, kt_lo + span_tiles);
+  if (kt_lo >= kt_hi) return;
+
+  const int rb0 = row0 + wave * TILE;          // the wavefront's first row
+  const int qpos0 = rq.c + rb0;                // and its position
+  const int q_row = rb0 + n, q_pos = qpos0 + n;
+  // tiles the wavefront needs: those up to its last row's
+  const int my_end = rb0 < rq.n ? min((qpos0 + TILE - 1) / TILE + 1, kt_hi) : 0;
+
+  u32x4 qf[HG][NS], qs[NS];
+  {
+    const elem* qt = static_cast<const elem*>(a.q) + (int64_t)(rq.first + q_row) * a.q_token;
+    const bool ok = q_row < rq.n;
+    auto frag = [&](int head, int s) -> u32x4 {
+      return ok ? *reinterpret_cast<const u32x4*>(qt + head * a.q_head + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
+    };
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int g = 0; g < HG; ++g) qf[g][s] = frag(hd0 + g, s);
+      qs[s] = WHOLE ? qf[0][s] : frag(hsel, s);
+    }
+  }
+  float m[HG], l[HG];
+  f32x16 o[HG][DB];
+#pragma unroll
+  for (int g = 0; g < HG; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[g][db] = zero16();
+  }
+  const float sl2 = a.scale * LOG2E, neg_inv_scale = -1.f / a.scale;
+
+  const Rows rows(a, r, rq.t, wave, lane);
+  const int64_t head_bytes = (int64_t)T::RB << a.pshift;
+  const char* kp = static_cast<const char*>(a.k_pages);
+  const char* vp = static_cast<const char*>(a.v_pages);
+  const float* crow_p = carry + ((int64_t)((rq.first >> 5) + r + (min(rb0, rq.n - 1) >> 5)) * a.G + g0) * carry_ld;
+
+  auto load_tile = [&](typename FwdLds<P, D, HG, NW>::Tiles& B, const int64_t (&off)[PER]) {
+#pragma unroll
+    for (int g = 0; g < HG; ++g) {
+      if (!WHOLE) rows.load(B.k[g], kp + (hd0 + g) * head_bytes, off, wave);
+      rows.load(B.v[g], vp + (hd0 + g) * head_bytes, off, wave);
+    }
+  };
+  auto load_sel = [&](char* S, const int64_t (&off)[PER]) { rows.load(S, kp + hsel * head_bytes, off, wave); };
+  auto carry_of = [&](int kt) { return kt >= 0 ? crow_p[min(kt * TILE + n, rq.t - 1)] : 0.f; };
+
+  // Tile kt's selection into the wavefront's F rows (fwd64_kernel's select)
+  auto select = [&](int kt, const char* S, float entry) {
+    const int kbase = kt * TILE;
+    f32x16 l0 = zero16();
+#pragma unroll
+    for (int s = 0; s < NS; ++s) l0 = P::mma(qs[s], T::row_frag(S, n, h, s), l0);
+    f32x16 sel;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sel[i] = __builtin_amdgcn_fmed3f(-l0[i], -3.0e38f, 0.f);
+    if (kbase + TILE - 1 >= qpos0 || kbase < a.exempt) {
+      const int jk = kbase + n, thr = jk >= a.exempt ? jk - qpos0 - 4 * h : 32;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sel[i] = crow(i, 0) > thr ? sel[i] : 0.f;
+    }
+    float run = entry * neg_inv_scale;
+    float* fw = sF[wave];
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const Halves s4 = halves(((sel[4 * q4] + sel[4 * q4 + 1]) + sel[4 * q4 + 2]) + sel[4 * q4 + 3]);
+      float p = (h == 0) ? run : run + s4.lo;
+#pragma unroll
+      for (int t2 = 0; t2 < 4; ++t2) {
+        fw[crow(4 * q4 + t2, h) * LDF + n] = WHOLE ? p + l0[4 * q4 + t2] : p;
+        p += sel[4 * q4 + t2];
+      }
+      run = (run + s4.lo) + s4.hi;
+    }
+  };
+
+  // the tiles, newest first: cur in the buffers, cur - 1's selector rows too, cur - 2's pages known
+  int cur = kt_hi - 1;
+  int64_t off1[PER], off2[PER];   // of tiles cur - 1 and cur - 2
+  int pg[PER];
+  {
+    int64_t off0[PER];
+    rows.pages_of(cur, pg);
+    rows.offsets(cur, pg, off0);
+    load_tile(sB0, off0);
+    load_sel(sS0, off0);
+    rows.pages_of(cur - 1 >= kt_lo ? cur - 1 : -1, pg);
+    rows.offsets(cur - 1, pg, off1);
+    if (cur - 1 >= kt_lo) load_sel(sS1, off1);
+    rows.pages_of(cur - 2 >= kt_lo ? cur - 2 : -1, pg);
+  }
+  float entry1 = carry_of(cur - 1);
+  const float entry0 = carry_of(cur);
+  wait_loads();
+  __syncthreads();
+  if (cur < my_end) select(cur, sS0, entry0);
+  __syncthreads();   // every wavefront is past its reads of sS0, which the first step fills
+
+  auto step = [&](auto odd_tag) __attribute__((always_inline)) {
+    constexpr bool ODD = decltype(odd_tag)::value;
+    auto& B = ODD ? sB1 : sB0;
+    rows.offsets(cur - 2, pg, off2);
+    if (cur - 1 >= kt_lo) load_tile(ODD ? sB0 : sB1, off1);
+    if (cur - 2 >= kt_lo) load_sel(ODD ? sS1 : sS0, off2);
+    rows.pages_of(cur - 3 >= kt_lo ? cur - 3 : -1, pg);
+    const float entry2 = cur - 2 >= kt_lo ? carry_of(cur - 2) : 0.f;
+    if (cur < my_end) {
+      const int kbase = cur * TILE;
+      f32x16 fs;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 f4 = *reinterpret_cast<const float4*>(&sF[wave][n * LDF + 8 * q4 + 4 * h]);
+        fs[4 * q4] = f4.x;
+        fs[4 * q4 + 1] = f4.y;
+        fs[4 * q4 + 2] = f4.z;
+        fs[4 * q4 + 3] = f4.w;
+      }
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        f32x16 lg = fs;   // the product accumulates onto -F
+        if (!WHOLE) {
+#pragma unroll
+          for (int s = 0; s < NS; ++s) lg = P::mma(T::row_frag(B.k[g], n, h, s), qf[g][s], lg);
+        }
+        if (kbase + TILE - 1 > qpos0) {   // keys past a query (those past the last position among them)
+          const int thr = q_pos - kbase - 4 * h;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) lg[i] = crow(i, 0) <= thr ? lg[i] : -INFINITY;
+        }
+        float zmax = lg[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) zmax = fmaxf(zmax, lg[i]);
+        const Halves zh = halves(zmax);
+        const float m_new = fmaxf(m[g], fmaxf(zh.lo, zh.hi) * sl2);
+        if (__any(m_new > m[g])) {
+          const float alpha = (m_new == -INFINITY) ? 1.f : fast_exp2(m[g] - m_new);
+          m[g] = m_new;
+          l[g] *= alpha;
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[g][db][i] *= alpha;
+        }
+        const float mu = (m[g] == -INFINITY) ? 0.f : m[g];
+        float psum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = fast_exp2(fmaf(lg[i], sl2, -mu));
+          lg[i] = p;
+          psum += p;
+        }
+        l[g] += psum;
+        u32x4 pf[2];
+        if constexpr (T::ES == 2) {
+          pf[0] = P::pack(lg, 0);
+          pf[1] = P::pack(lg, 1);
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[g][db] = T::values(B.v[g], lane, db, pf, lg, o[g][db]);
+      }
+    }
+    if (cur - 1 >= kt_lo && cur - 1 < my_end) select(cur - 1, ODD ? sS0 : sS1, entry1);
+    entry1 = entry2;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) off1[i] = off2[i];
+    wait_loads();
+    __syncthreads();
+    --cur;
+  };
+  while (true) {
+    step(std::false_type{});
+    if (cur < kt_lo) break;
+    step(std::true_type{});
+    if (cur < kt_lo) break;
+  }
+
+  if (q_row >= rq.n) return;
+  const int64_t token = rq.first + q_row;
+#pragma unroll
+  for (int g = 0; g < HG; ++g) {
+    const Halves lh = halves(l[g]);
+    const float ltot = lh.lo + lh.hi;
+    const int64_t row = token * a.H + hd0 + g;
+    if (split) {
+      const int64_t prow = (int64_t)blockIdx.z * a.N * a.H + row;
+      if (h == 0) {
+        part_ml[2 * prow] = m[g];
+        part_ml[2 * prow + 1] = ltot;
+      }
+    }
+    const float inv = split ? 1.f : 1.f / ltot;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int d = db * 32 + 8 * q4 + 4 * h;
+        if (D < 32 && d >= D) continue;
+        const float4 v4 = make_float4(o[g][db][4 * q4] * inv, o[g][db][4 * q4 + 1] * inv, o[g][db][4 * q4 + 2] * inv,
+                                      o[g][db][4 * q4 + 3] * inv);
+        if (split) {
+          *reinterpret_cast<float4*>(part_o + ((int64_t)blockIdx.z * a.N * a.H + row) * D + d) = v4;
+        } else if constexpr (T::ES == 2) {
+          *reinterpret_cast<uint2*>(out + row * D + d) =
+              make_uint2((uint32_t)P::to_elem(v4.x) | ((uint32_t)P::to_elem(v4.y) << 16),
+                         (uint32_t)P::to_elem(v4.z) | ((uint32_t)P::to_elem(v4.w) << 16));
+        } else {
+          *reinterpret_cast<float4*>(out + row * D + d) = v4;
+        }
+      }
+    }
+  }
+}
+
+// The spans of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the spans that begin at
+// or before the query. A workgroup per row, a thread per four output columns.
+template <class P, int D>
+__global__ __launch_bounds__(NTHREADS) void paged_join_kernel(PagedCall a, int span_tiles, const float* __restrict__ part_ml,
+                                                              const float* __restrict__ part_o) {
+  typedef typename P::elem elem;
+  const int row = blockIdx.x;
+  const int r = find_request<true>(a.starts, a.R, row, 0);
+  const PagedRequest rq = paged_request(a, r);
+  const bool live = rq.live && row >= rq.first && row < rq.first + rq.n;
+  const int spans = live ? (rq.c + row - rq.first) / TILE / span_tiles + 1 : 0;
+  elem* out = static_cast<elem*>(a.out) + (int64_t)row * a.H * D;
+  for (int i = threadIdx.x; i < a.H * (D / 4); i += NTHREADS) {
+    const int hd = i / (D / 4);
+    float M = -INFINITY;
+    for (int z = 0; z < spans; ++z) M = fmaxf(M, part_ml[2 * (((int64_t)z * a.N + row) * a.H + hd)]);
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int z = 0; z < spans; ++z) {
+      const int64_t at = ((int64_t)z * a.N + row) * a.H + hd;
+      const float2 ml = *reinterpret_cast<const float2*>(part_ml + 2 * at);
+      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+      const float4 x = *reinterpret_cast<const float4*>(part_o + at * D + 4 * (i % (D / 4)));
+      l = fmaf(w, ml.y, l);
+      acc.x = fmaf(w, x.x, acc.x);
+      acc.y = fmaf(w, x.y, acc.y);
+      acc.z = fmaf(w, x.z, acc.z);
+      acc.w = fmaf(w, x.w, acc.w);
+    }
+    const float inv = live ? 1.f / l : 0.f;
+    const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[4 * i + e] = P::to_elem(y[e]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// One new token per request. Workgroup (chunk, head, request) reads its chunk of the head's cached keys and
+// values once, 16 bytes per lane, as decode_partial_kernel does (logits reduced over the lanes of a row, one
+// probability per lane, values added into each lane's column slice); a lane looks up the pages of its rows one step
+// ahead. The selector head's workgroups write the new state rows to the workspace, which paged_step_join copies
+// over the state after every head has read the old one.
+template <class P, int D>
+struct StepLayout {
+  static constexpr int EPC = P::EPC, LPK = D / EPC, KPI = 64 / LPK;
+  static constexpr int NR = 8 < LPK ? 8 : LPK;
+  static constexpr int DUP = LPK / NR, STEP = KPI * NR;
+};
+
+template <class P, int D>
+__global__ __launch_bounds__(NTHREADS) void paged_step_kernel(PagedCall a, float* __restrict__ pm, float* __restrict__ pl,
+                                                              float* __restrict__ po, float* __restrict__ next_state,
+                                                              int64_t next_ld, int chunk, int nchunk) {
+  using L = StepLayout<P, D>;
+  typedef typename P::elem elem;
+  constexpr int EPC = L::EPC, LPK = L::LPK, KPI = L::KPI, NR = L::NR, DUP = L::DUP, STEP = L::STEP;
+  union Row {
+    u32x4 u;
+    elem e[EPC];
+  };
+  __shared__ __align__(16) float sP[NWAVES][STEP];
+  __shared__ float sPart[NWAVES][D + 2];
+
+  const int cidx = blockIdx.x;
+  const int r = blockIdx.z, hd = blockIdx.y;
+  const PagedRequest rq = paged_request(a, r);
+  if (!rq.live || cidx * chunk >= rq.t) return;
+  const int t = rq.t, per = a.H / a.G;
+  const int64_t sg = (int64_t)r * a.G + hd / per;
+  const bool selector = (hd % per) == 0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int kq = lane / LPK, dc = lane % LPK;
+  const int ri = dc / DUP;
+  const bool owner = dc % DUP == 0;
+  const int wkeys = chunk / NWAVES;
+  const int kw0 = cidx * chunk + wave * wkeys, kw_end = min(kw0 + wkeys, t);
+  const float* selrow = a.selected + sg * a.state_ld;
+  float* nextrow = next_state + sg * next_ld;
+  const int* trow = a.table + r * a.table_ld;
+  const int pmask = (1 << a.pshift) - 1;
+
+  float qf[EPC];
+  {
+    Row qq;
+    qq.u = *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.q) + rq.first * a.q_token + hd * a.q_head + EPC * dc);
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) qf[e] = P::to_float(qq.e[e]) * a.scale;
+  }
+  float m = -INFINITY, l = 0.f, o[EPC];
+#pragma unroll
+  for (int e = 0; e < EPC; ++e) o[e] = 0.f;
+
+  auto lookup = [&](int kw, int (&pg)[NR]) {
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int j = kw + i * KPI + kq;
+      pg[i] = j < kw_end ? trow[j >> a.pshift] : -1;
+    }
+  };
+  int pg[NR];
+  lookup(kw0, pg);
+  for (int kw = kw0; kw < kw_end; kw += STEP) {
+    Row kr[NR], vr[NR];
+    int64_t off[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int j = kw + i * KPI + kq;
+      const bool ok = (uint32_t)pg[i] < (uint32_t)a.pages;
+      off[i] = ok ? ((((int64_t)pg[i] * a.H + hd) << a.pshift) + (j & pmask)) * D + EPC * dc : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+      kr[i].u = off[i] >= 0 ? *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.k_pages) + off[i]) : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+      vr[i].u = off[i] >= 0 ? *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.v_pages) + off[i]) : u32x4{0, 0, 0, 0};
+    const int j = kw + ri * KPI + kq;
+    const bool jok = j < kw_end;
+    const float sel = j < t - 1 && jok ? selrow[j] : 0.f;
+    if (kw + STEP < kw_end) lookup(kw + STEP, pg);
+    float z1[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) s = fmaf(qf[e], P::to_float(kr[i].e[e]), s);
+      z1[i] = s;
+    }
+#pragma unroll
+    for (int st = 1; st < NR; st <<= 1) {   // reduce-scatter over the row's lanes (decode_partial_kernel)
+      const int half = NR / (2 * st), s = LPK / (2 * st);
+      const uint32_t up = (lane & s) ? 0xffffffffu : 0u;
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const uint32_t lo = __float_as_uint(z1[i]), hi = __float_as_uint(z1[i + half]);
+        const float send = __uint_as_float((lo & up) | (hi & ~up));
+        const float keep = __uint_as_float((hi & up) | (lo & ~up));
+        z1[i] = keep + __shfl_xor(send, s);
+      }
+    }
+#pragma unroll
+    for (int s = DUP / 2; s >= 1; s >>= 1) z1[0] += __shfl_xor(z1[0], s);
+    const float raw = z1[0];
+    if (selector && owner && jok) nextrow[j] = sel + (j >= a.exempt && j < t - 1 ? fmaxf(raw, 0.f) : 0.f);
+    const float z = jok ? (raw - sel) * LOG2E : -INFINITY;
+    const float m_new = fmaxf(m, wave_max(z));
+    const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m - m_new);
+    const float p = jok && m_new > -INFINITY ? fast_exp2(z - m_new) : 0.f;
+    l = fmaf(l, alpha, owner ? p : 0.f);
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) o[e] *= alpha;
+    m = m_new;
+    if (owner) sP[wave][kq * NR + ri] = p;
+    lds_wave_sync();
+    float pr[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) pr[i] = sP[wave][kq * NR + i];
+    lds_wave_sync();
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int e = 0; e < EPC; ++e) o[e] = fmaf(pr[i], P::to_float(vr[i].e[e]), o[e]);
+  }
+  l = wave_sum(l);
+#pragma unroll
+  for (int sh = LPK; sh < 64; sh <<= 1)
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) o[e] += __shfl_xor(o[e], sh);
+  if (kq == 0) {
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) sPart[wave][2 + EPC * dc + e] = o[e];
+  }
+  if (lane == 0) {
+    sPart[wave][0] = m;
+    sPart[wave][1] = l;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NWAVES; ++w) mx = fmaxf(mx, sPart[w][0]);
+    const int64_t slot = ((int64_t)r * a.H + hd) * nchunk + cidx;
+    for (int c = lane; c < D + 2; c += 64) {
+      float acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < NWAVES; ++w) {
+        const float wt = sPart[w][0] == -INFINITY ? 0.f : fast_exp2(sPart[w][0] - mx);
+        acc = fmaf(wt, sPart[w][c], acc);
+      }
+      if (c == 0) pm[slot] = mx;
+      else if (c == 1) pl[slot] = acc;
+      else po[slot * D + c - 2] = acc;
+    }
+  }
+}
+
+// Blocks [0, rows * H): one row's head, its chunks' partials joined (rows of no request, or of one left out, become
+// zero). Blocks from there on: the new state rows, `sblocks` blocks of 1024 keys each.
+template <class P, int D>
+__global__ __launch_bounds__(NTHREADS) void paged_step_join_kernel(PagedCall a, const float* __restrict__ pm,
+                                                                   const float* __restrict__ pl, const float* __restrict__ po,
+                                                                   const float* __restrict__ next_state, int64_t next_ld,
+                                                                   int chunk, int nchunk, int sblocks) {
+  typedef typename P::elem elem;
+  constexpr int QPP = D / 4, SLOTS = NTHREADS / QPP;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int64_t out_blocks = (int64_t)a.N * a.H;
+  if (blockIdx.x >= out_blocks) {
+    const int64_t s = blockIdx.x - out_blocks;
+    const int64_t sg = s / sblocks;
+    const int j0 = (int)(s % sblocks) * (4 * NTHREADS);
+    const PagedRequest rq = paged_request(a, (int)(sg / a.G));
+    if (!rq.live) return;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + u * NTHREADS + tid;
+      if (j < rq.t) a.selected[sg * a.state_ld + j] = next_state[sg * next_ld + j];
+    }
+    return;
+  }
+  __shared__ float sRed[NWAVES][2];
+  __shared__ float4 sO[NWAVES][QPP];
+  const int row = (int)(blockIdx.x / a.H), hd = (int)(blockIdx.x % a.H);
+  const int r = find_request<true>(a.starts, a.R, row, 0);
+  const PagedRequest rq = paged_request(a, r);
+  elem* out = static_cast<elem*>(a.out) + ((int64_t)row * a.H + hd) * D;
+  if (!rq.live || rq.first != row) {
+    if (tid < D) out[tid] = P::to_elem(0.f);
+    return;
+  }
+  const int nparts = (rq.t + chunk - 1) / chunk;
+  const int64_t at = ((int64_t)r * a.H + hd) * nchunk;
+  float mx = -INFINITY;
+  for (int i = tid; i < nparts; i += NTHREADS) mx = fmaxf(mx, pm[at + i]);
+  mx = wave_max(mx);
+  if (lane == 0) sRed[wave][0] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(sRed[0][0], sRed[1][0]), fmaxf(sRed[2][0], sRed[3][0]));
+  float l = 0.f;
+  for (int i = tid; i < nparts; i += NTHREADS) l = fmaf(fast_exp2(pm[at + i] - mx), pl[at + i], l);
+  l = wave_sum(l);
+  if (lane == 0) sRed[wave][1] = l;
+  const int slot = tid / QPP, cq = tid % QPP;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = slot; i < nparts; i += SLOTS) {
+    const float w = fast_exp2(pm[at + i] - mx);
+    const float4 x = *reinterpret_cast<const float4*>(po + (at + i) * D + 4 * cq);
+    acc.x = fmaf(w, x.x, acc.x);
+    acc.y = fmaf(w, x.y, acc.y);
+    acc.z = fmaf(w, x.z, acc.z);
+    acc.w = fmaf(w, x.w, acc.w);
+  }
+#pragma unroll
+  for (int sh = QPP; sh < 64; sh <<= 1) {
+    acc.x += __shfl_xor(acc.x, sh);
+    acc.y += __shfl_xor(acc.y, sh);
+    acc.z += __shfl_xor(acc.z, sh);
+    acc.w += __shfl_xor(acc.w, sh);
+  }
+  if (lane < QPP) sO[wave][lane] = acc;
+  __syncthreads();
+  if (tid < QPP) {
+    l = (sRed[0][1] + sRed[1][1]) + (sRed[2][1] + sRed[3][1]);
+    const float inv = 1.f / l;
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NWAVES; ++w) {
+      y[0] += sO[w][tid].x;
+      y[1] += sO[w][tid].y;
+      y[2] += sO[w][tid].z;
+      y[3] += sO[w][tid].w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[4 * tid + e] = P::to_elem(y[e] * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Launches (sizes: paged_shape, sa_host.h).
+inline PagedCall paged_call(const PagedLaunch& c) {
+  PagedCall a{};
+  a.q = c.q;
+  a.k_pages = c.k_pages;
+  a.v_pages = c.v_pages;
+  a.out = c.out;
+  a.table = c.table;
+  a.lengths = c.lengths;
+  a.starts = c.starts;
+  a.selected = c.selected;
+  a.q_token = c.q_token;
+  a.q_head = c.q_head;
+  a.table_ld = c.table_ld;
+  a.state_ld = c.state_ld;
+  a.R = (int)c.R;
+  a.N = (int)c.N;
+  a.H = (int)c.H;
+  a.G = (int)c.G;
+  a.pages = (int)c.pages;
+  a.pshift = c.pshift;
+  a.max_new = (int)c.max_new;
+  a.max_len = (int)c.max_len;
+  a.scale = c.scale;
+  a.exempt = c.exempt;
+  return a;
+}
+
+template <class P, int D, int HG, int NW, bool WHOLE>
+void launch_paged_fwd(const PagedCall& a, const PagedShape& s, const float* carry, float* ml, float* o, hipStream_t st) {
+  const unsigned tiles = (unsigned)((a.N >> (NW == 4 ? 7 : 5)) + a.R);
+  hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE>), dim3(tiles, (unsigned)(a.H / HG), (unsigned)s.splits), dim3(NW * 64), 0, st,
+                     a, carry, s.carry_ld, s.span_tiles, ml, o);
+}
+
+template <class P, int D>
+int paged_launch(const PagedLaunch& c) {
+  const PagedCall a = paged_call(c);
+  const PagedShape s = paged_shape(c.R, c.N, c.H, c.G, D, sizeof(typename P::elem), c.max_new, c.max_len);
+  char* ws = static_cast<char*>(c.ws);
+  auto at = [&](int64_t off) { return reinterpret_cast<float*>(ws + off); };
+  if (s.step) {
+    float *pm = at(s.m), *pl = at(s.l), *po = at(s.o), *next = at(s.carry);
+    {
+      TimedLaunch timed(SA_KERNEL_DECODE, c.st);
+      hipLaunchKernelGGL((paged_step_kernel<P, D>), dim3((unsigned)s.splits, (unsigned)a.H, (unsigned)a.R), dim3(NTHREADS), 0, c.st, a,
+                         pm, pl, po, next, s.carry_ld, s.chunk, s.splits);
+    }
+    const int sblocks = (int)cdiv(a.max_len, 4 * NTHREADS);
+    const int64_t blocks = (int64_t)a.N * a.H + (int64_t)a.R * a.G * sblocks;
+    hipLaunchKernelGGL((paged_step_join_kernel<P, D>), dim3((unsigned)blocks), dim3(NTHREADS), 0, c.st, a, pm, pl, po, next,
+                       s.carry_ld, s.chunk, s.splits, sblocks);
+    return launch_status();
+  }
+  float *carry = at(s.carry), *ml = s.splits > 1 ? at(s.m) : nullptr, *o = s.splits > 1 ? at(s.o) : nullptr;
+  {
+    TimedLaunch timed(SA_KERNEL_SELECTION, c.st);
+    hipLaunchKernelGGL((paged_carry_kernel<P, D>), dim3((unsigned)s.carry_blocks, (unsigned)a.G, (unsigned)a.R), dim3(NTHREADS), 0, c.st,
+                       a, carry, s.carry_ld);
+  }
+  {
+    TimedLaunch timed(SA_KERNEL_FORWARD, c.st);
+    const bool whole = a.G == a.H;
+    if constexpr (sizeof(typename P::elem) == 2 && D <= 64) {
+      if (s.hg == 2) {
+        if (s.nw == 4) launch_paged_fwd<P, D, 2, 4, false>(a, s, carry, ml, o, c.st);
+        else launch_paged_fwd<P, D, 2, 1, false>(a, s, carry, ml, o, c.st);
+      }
+    }
+    if (s.hg == 1) {
+      if (s.nw == 4) {
+        if (whole) launch_paged_fwd<P, D, 1, 4, true>(a, s, carry, ml, o, c.st);
+        else launch_paged_fwd<P, D, 1, 4, false>(a, s, carry, ml, o, c.st);
+      } else {
+        if (whole) launch_paged_fwd<P, D, 1, 1, true>(a, s, carry, ml, o, c.st);
+        else launch_paged_fwd<P, D, 1, 1, false>(a, s, carry, ml, o, c.st);
+      }
+    }
+  }
+  if (s.splits > 1)
+    hipLaunchKernelGGL((paged_join_kernel<P, D>), dim3((unsigned)a.N), dim3(NTHREADS), 0, c.st, a, s.span_tiles, ml, o);
+  return launch_status();
+}
+
+template <class P>
+int paged_entry(const PagedLaunch& c) {
+  if (c.head_dim == 16) return paged_launch<P, 16>(c);
+  if (c.head_dim == 32) return paged_launch<P, 32>(c);
+  if (c.head_dim == 64) return paged_launch<P, 64>(c);
+  return paged_launch<P, 128>(c);
+}
+
+}  // namespace

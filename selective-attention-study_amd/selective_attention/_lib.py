@@ -18,6 +18,7 @@ LIB_PATH = os.environ.get("SA_HIP_LIBRARY") or os.path.join(os.path.dirname(os.p
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_F16 = 2   # the paged cache's entry points
 
 # Kernel ids of sa_timing_read.
 KERNEL_FORWARD = 0
@@ -58,6 +59,11 @@ SIGNATURES = {
                          _I64, _I64, _I64, _I64, _F, _I, _I, _I, _I, _P]),
     "sa_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
     "sa_decode": (_I, [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I, _P]),
+    "sa_page_plan": (_I, [_P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P]),
+    "sa_paged_append": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _I, _P]),
+    "sa_paged_attention_workspace_bytes": (_I64, [_I64] * 7 + [_I]),
+    "sa_paged_attention": (_I, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64,
+                                _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I, _P]),
     "sa_decode_noalloc": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I, _P]),
 }
 
