@@ -436,8 +436,9 @@ struct PagedTile {
         for (int hf = 0; hf < 2; ++hf) {
           const int r = 16 * s + 8 * hf + 4 * (g >> 1) + (k >> 2);
           typedef __attribute__((address_space(3))) short4v* lds_s4;
-          const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s4)lds_ptr(t + r * RB + ((c ^ paged_swz<CPR>(r)) << 4) + 8 * (k & 1)));
+          // (a pointer cast: through an integer the compiler would no longer know which tile is read, and wait for
+          // the loads into the other)
+          const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + r * RB + ((c ^ paged_swz<CPR>(r)) << 4) + 8 * (k & 1)));
           const uint2 u = __builtin_bit_cast(uint2, x);
           f[2 * hf] = u.x;
           f[2 * hf + 1] = u.y;
