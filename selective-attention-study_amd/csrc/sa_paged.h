@@ -462,16 +462,33 @@ __device__ __forceinline__ void g2l16(const void* g, void* l) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, lds_ptr(l), 16, 0, 0);
 }
 
-// A lane's rows of the tiles that NW wavefronts load together: part m of a tile (m = wave, wave + NW, ...) is 64
-// chunks, lane l's the chunk at 64 m + l, which holds logical chunk (l % CPR) ^ swz(row) of row (64 m + l) / CPR.
+// 16 bytes per lane from p + off into LDS; zeros past `bytes`
+__device__ __forceinline__ void b2l16(const char* p, int bytes, char* l, int off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(p, bytes), lds_ptr(l), 16, off, 0, 0, 0);
+}
+
+// The loads of the tiles that NW wavefronts fill together: part m of a tile (m = wave, wave + NW, ...) is 64 chunks,
+// lane l's the chunk at 64 m + l, which holds logical chunk (l % CPR) ^ swz(row) of row (64 m + l) / CPR. A request's
+// table is read one tile before its rows.
+//
+// A part of at most 8 rows lies in one page whatever the page size: its address is one number for the wavefront, the
+// loads go through a buffer resource that starts at the part and ends with the request's last row (or holds nothing,
+// where the table names no page), and the vector unit computes nothing per load. Narrower rows (16 or 32 rows per part)
+// look up a page per lane and read zeros from a row of their own.
 template <class P, int D, int NW>
 struct PagedRows {
   typedef PagedTile<P, D> T;
   static constexpr int PER = (T::PARTS + NW - 1) / NW;
+  static constexpr int ROWS = 64 / T::CPR;   // of a part
+  static constexpr bool UNIFORM = ROWS <= 8;
+  struct Place {     // of a part's rows in the cache, head 0
+    int64_t at;      // byte offset (per lane: -1, none)
+    int bytes;       // from there to the last row (uniform parts)
+  };
   const int* trow;      // the request's table row
   int pshift, pages, t;
   int64_t page_bytes;   // all heads of a page
-  int row[PER], col[PER];
+  int row[PER], col[PER];   // per lane: row of the tile, byte offset of its chunk (uniform parts: of the part)
 
   __device__ __forceinline__ PagedRows(const PagedCall& a, int r, int t_, int wave, int lane)
       : trow(a.table + r * a.table_ld), pshift(a.pshift), pages(a.pages), t(t_),
@@ -479,11 +496,12 @@ struct PagedRows {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int at = 64 * (wave + NW * i) + lane;
-      row[i] = at / T::CPR;
-      col[i] = ((at % T::CPR) ^ paged_swz<T::CPR>(row[i])) << 4;
+      row[i] = UNIFORM ? ROWS * (wave + NW * i) : at / T::CPR;
+      col[i] = ((at % T::CPR) ^ paged_swz<T::CPR>(at / T::CPR)) << 4;
+      if (UNIFORM) col[i] += lane / T::CPR * T::RB;
     }
   }
-  // the pages of key tile kt's rows (-1: none); a tile before the first has none
+  // the table entries of key tile kt's rows (-1: none; a tile before the first has none)
   __device__ __forceinline__ void pages_of(int kt, int (&pg)[PER]) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -491,78 +509,138 @@ struct PagedRows {
       pg[i] = (kt >= 0 && j < t) ? trow[j >> pshift] : -1;
     }
   }
-  // byte offsets of the lane's chunks in the cache (head 0; -1: no page in the cache)
-  __device__ __forceinline__ void offsets(int kt, const int (&pg)[PER], int64_t (&off)[PER]) const {
+  __device__ __forceinline__ void places(int kt, const int (&pg)[PER], Place (&pl)[PER]) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int in = (kt * TILE + row[i]) & ((1 << pshift) - 1);
-      off[i] = (uint32_t)pg[i] < (uint32_t)pages ? pg[i] * page_bytes + in * T::RB + col[i] : -1;
+      const int j = kt * TILE + row[i], in = (j & ((1 << pshift) - 1)) * T::RB;
+      const int page = UNIFORM ? __builtin_amdgcn_readfirstlane(pg[i]) : pg[i];
+      const bool ok = (uint32_t)page < (uint32_t)pages;
+      if constexpr (UNIFORM) {
+        pl[i].at = ok ? page * page_bytes + in : 0;
+        pl[i].bytes = ok ? min(ROWS, t - j) * T::RB : 0;
+      } else {
+        pl[i].at = ok ? page * page_bytes + in + col[i] : -1;
+      }
     }
   }
-  // the rows of one head (its offset within a page: `head`) into a tile
-  __device__ __forceinline__ void load(char* tile, const char* base, const int64_t (&off)[PER], int wave) const {
+  // the rows of one head, whose rows of page 0 begin at `base`, into a tile
+  __device__ __forceinline__ void load(char* tile, const char* base, const Place (&pl)[PER], int wave) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int m = wave + NW * i;
-      if (m < T::PARTS) g2l16(off[i] >= 0 ? base + off[i] : reinterpret_cast<const char*>(&paged_zero_row), tile + 1024 * m);
+      if (T::PARTS % NW != 0 && m >= T::PARTS) continue;
+      if constexpr (UNIFORM)
+        b2l16(base + pl[i].at, pl[i].bytes, tile + 1024 * m, col[i]);
+      else
+        g2l16(pl[i].at >= 0 ? base + pl[i].at : reinterpret_cast<const char*>(&paged_zero_row), tile + 1024 * m);
     }
   }
 };
 
 // ---------------------------------------------------------------------------------------------
 // The selectors' histories of a step of several tokens: carry[tile][g][j], what key j has received before the
-// tile's first query, and the state after the step. A wavefront owns 32 keys of one selector (rows in registers)
-// and walks the request's query tiles, as sel_carry64_kernel does; the query rows come straight from the L2, one
-// tile ahead. Rows of keys that no query of a tile sees are not written: the forward masks those keys.
+// tile's first query, and the state after the step. A wavefront owns 32 keys of one selector (rows in registers) and
+// its workgroup walks the request's query tiles, as sel_carry64_kernel does, U tiles at a time: a step rarely has keys
+// enough for more than one wavefront per SIMD, so the walk is bound by the latency of its own instructions and the U
+// products and sums are kept independent; the rows are loaded into LDS three steps ahead, once for the workgroup. At 4096
+// queries on 32768 keys (us): 48; one tile at a time from the L2 105, four at a time 64, through LDS one step ahead 55. Rows
+// of keys that no query of a tile sees hold no history: the forward masks those keys.
 template <class P, int D>
 __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, float* __restrict__ carry, int64_t carry_ld) {
   typedef PagedTile<P, D> T;
   typedef typename P::elem elem;
+  constexpr int NS = T::NS, U = T::BYTES > 8192 ? 1 : T::BYTES > 4096 ? 2 : 4, PER = U * T::PARTS / NWAVES;
+  // The U tiles of step t are in buffer t mod 4 (variables of their own: a step's reads touch none of the others), filled
+  // by loads that step t - 3 issues (the prologue for the first three). Every step issues PER loads (past the last tile: of
+  // nothing), then U stores, so at its end the loads of step t + 1, issued in step t - 2, have landed once
+  // no more than 2 PER + 3 U newer operations run.
+  __shared__ __attribute__((aligned(16))) char sQ0[U * T::BYTES], sQ1[U * T::BYTES], sQ2[U * T::BYTES], sQ3[U * T::BYTES];
   const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
   const int r = blockIdx.z, g = blockIdx.y;
   const PagedRequest rq = paged_request(a, r);
   if (!rq.live) return;
   const int hd = g * (a.H / a.G);
   const int nkb = (rq.t + TILE - 1) / TILE, ntile = (rq.n + TILE - 1) / TILE;
-  const int tile0 = (rq.first >> 5) + r;
   const elem* q = static_cast<const elem*>(a.q) + rq.first * a.q_token + hd * a.q_head;
   const int* trow = a.table + r * a.table_ld;
   float* state = a.selected + ((int64_t)r * a.G + g) * a.state_ld;
-  for (int kb = blockIdx.x * NWAVES + wave; kb < nkb; kb += gridDim.x * NWAVES) {
-    const int j = kb * TILE + n;
-    u32x4 kf[T::NS];
+  const int64_t plane = a.G * carry_ld;   // from one tile's histories to the next's
+  float* cr = carry + (int64_t)((rq.first >> 5) + r) * plane + g * carry_ld;
+  // part m = wave + NWAVES i of the U tiles' 16-byte chunks; rows past the last read as zeros
+  int off[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = 64 * (wave + NWAVES * i) + lane, row = at / T::CPR;
+    off[i] = row * (int)a.q_token * T::ES + (((at % T::CPR) ^ paged_swz<T::CPR>(row % TILE)) << 4);
+  }
+  auto load_q = [&](int rb, char* buf) {
+    const int left = max(min(rq.n - rb * TILE, U * TILE), 0);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      b2l16(reinterpret_cast<const char*>(q + rb * TILE * a.q_token), left * (int)a.q_token * T::ES, buf + 1024 * (wave + NWAVES * i), off[i]);
+  };
+  for (int kb0 = blockIdx.x * NWAVES; kb0 < nkb; kb0 += gridDim.x * NWAVES) {
+    const int kb = kb0 + wave, j = kb * TILE + n;
+    // tiles before this end before the workgroup's first key
+    int rb = max(kb0 * TILE - rq.c, 0) / TILE;
+    load_q(rb, sQ0);
+    load_q(rb + U, sQ1);
+    load_q(rb + 2 * U, sQ2);
+    u32x4 kf[NS];
     {
       const int pg = j < rq.t ? trow[j >> a.pshift] : -1;
       const bool ok = (uint32_t)pg < (uint32_t)a.pages;
       const elem* k = static_cast<const elem*>(a.k_pages) +
                       ((((int64_t)(ok ? pg : 0) * a.H + hd) << a.pshift) + (j & ((1 << a.pshift) - 1))) * D;
 #pragma unroll
-      for (int s = 0; s < T::NS; ++s)
+      for (int s = 0; s < NS; ++s)
         kf[s] = ok ? *reinterpret_cast<const u32x4*>(k + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
     }
     float run = j < rq.c ? state[j] : 0.f;
-    auto load_q = [&](int rb, u32x4 (&qf)[T::NS]) {
-      const int row = rb * TILE + n;
+    const uint32_t end = (uint32_t)rq.t * 4, own = h == 0 && j < rq.t ? (uint32_t)j * 4 : end;   // byte offset of the lane's key in a row of histories
+    auto step = [&](const char* buf, char* next) {
+      load_q(rb + 3 * U, next);
+      f32x16 acc[U];
 #pragma unroll
-      for (int s = 0; s < T::NS; ++s)
-        qf[s] = row < rq.n ? *reinterpret_cast<const u32x4*>(q + row * a.q_token + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
-    };
-    // tiles before rb_lo end before the block's first key
-    const int rb_lo = max(kb * TILE - rq.c, 0) / TILE;
-    u32x4 qa[T::NS], qb[T::NS];
-    load_q(rb_lo, qa);
-    for (int rb = rb_lo; rb < ntile; ++rb) {
-      load_q(rb + 1, qb);
-      if (h == 0 && j < rq.t) carry[((int64_t)(tile0 + rb) * a.G + g) * carry_ld + j] = run;
-      f32x16 acc = zero16();
+      for (int u = 0; u < U; ++u) acc[u] = zero16();
 #pragma unroll
-      for (int s = 0; s < T::NS; ++s) acc = P::mma(qa[s], kf[s], acc);
+      for (int s = 0; s < NS; ++s)   // (the U chains side by side)
+#pragma unroll
+        for (int u = 0; u < U; ++u) acc[u] = P::mma(T::row_frag(buf + u * T::BYTES, n, h, s), kf[s], acc[u]);
+      float sum[U];
       const int qbase = rq.c + rb * TILE;
-      const bool interior = qbase > kb * TILE + TILE - 1 && kb * TILE >= a.exempt;
-      run += block_selection_sum(acc, interior, j >= a.exempt ? j - qbase - 4 * h : 32, a.scale);
+      // (one choice for the U tiles: their sums interleave too)
+      if (qbase > kb * TILE + TILE - 1 && kb * TILE >= a.exempt) {
 #pragma unroll
-      for (int s = 0; s < T::NS; ++s) qa[s] = qb[s];
+        for (int u = 0; u < U; ++u) sum[u] = block_selection_sum(acc[u], true, 0, a.scale);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          sum[u] = block_selection_sum(acc[u], false, j >= a.exempt ? j - qbase - u * TILE - 4 * h : 32, a.scale);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {   // (every lane stores, past the row's end where it has no key or the tile is none)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(run), rsrc(cr + (rb + u) * plane, rb + u < ntile ? end : 0), own, 0, 0);
+        run += sum[u];
+      }
+      rb += U;
+      // (one asm block: at a barrier of its own the compiler waits for everything)
+      __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER + 3 * U) : "memory");
+    };
+    wait_loads();
+    __syncthreads();
+    while (true) {
+      step(sQ0, sQ3);
+      if (rb >= ntile) break;
+      step(sQ1, sQ0);
+      if (rb >= ntile) break;
+      step(sQ2, sQ1);
+      if (rb >= ntile) break;
+      step(sQ3, sQ2);
+      if (rb >= ntile) break;
     }
+    wait_loads();   // nothing on its way into LDS when the workgroup ends or takes its next keys
+    __syncthreads();
     if (h == 0 && j < rq.t) state[j] = run;
   }
 }
@@ -670,14 +748,14 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   const char* vp = static_cast<const char*>(a.v_pages);
   const float* crow_p = carry + ((int64_t)((rq.first >> 5) + r + (min(rb0, rq.n - 1) >> 5)) * a.G + g0) * carry_ld;
 
-  auto load_tile = [&](typename FwdLds<P, D, HG, NW>::Tiles& B, const int64_t (&off)[PER]) {
+  auto load_tile = [&](typename FwdLds<P, D, HG, NW>::Tiles& B, const typename Rows::Place (&off)[PER]) {
 #pragma unroll
     for (int g = 0; g < HG; ++g) {
       if (!WHOLE) rows.load(B.k[g], kp + (hd0 + g) * head_bytes, off, wave);
       rows.load(B.v[g], vp + (hd0 + g) * head_bytes, off, wave);
     }
   };
-  auto load_sel = [&](char* S, const int64_t (&off)[PER]) { rows.load(S, kp + hsel * head_bytes, off, wave); };
+  auto load_sel = [&](char* S, const typename Rows::Place (&off)[PER]) { rows.load(S, kp + hsel * head_bytes, off, wave); };
   auto carry_of = [&](int kt) { return kt >= 0 ? crow_p[min(kt * TILE + n, rq.t - 1)] : 0.f; };
 
   // Tile kt's selection into the wavefront's F rows (fwd64_kernel's select)
@@ -711,16 +789,16 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
 
   // the tiles, newest first: cur in the buffers, cur - 1's selector rows too, cur - 2's pages known
   int cur = kt_hi - 1;
-  int64_t off1[PER], off2[PER];   // of tiles cur - 1 and cur - 2
+  typename Rows::Place off1[PER], off2[PER];   // of tiles cur - 1 and cur - 2
   int pg[PER];
   {
-    int64_t off0[PER];
+    typename Rows::Place off0[PER];
     rows.pages_of(cur, pg);
-    rows.offsets(cur, pg, off0);
+    rows.places(cur, pg, off0);
     load_tile(sB0, off0);
     load_sel(sS0, off0);
     rows.pages_of(cur - 1 >= kt_lo ? cur - 1 : -1, pg);
-    rows.offsets(cur - 1, pg, off1);
+    rows.places(cur - 1, pg, off1);
     if (cur - 1 >= kt_lo) load_sel(sS1, off1);
     rows.pages_of(cur - 2 >= kt_lo ? cur - 2 : -1, pg);
   }
@@ -734,7 +812,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   auto step = [&](auto odd_tag) __attribute__((always_inline)) {
     constexpr bool ODD = decltype(odd_tag)::value;
     auto& B = ODD ? sB1 : sB0;
-    rows.offsets(cur - 2, pg, off2);
+    rows.places(cur - 2, pg, off2);
     if (cur - 1 >= kt_lo) load_tile(ODD ? sB0 : sB1, off1);
     if (cur - 2 >= kt_lo) load_sel(ODD ? sS1 : sS0, off2);
     rows.pages_of(cur - 3 >= kt_lo ? cur - 3 : -1, pg);

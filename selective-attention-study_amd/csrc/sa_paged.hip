@@ -21,9 +21,11 @@ int64_t elem_size(int dtype) { return dtype == SA_DTYPE_F32 ? 4 : dtype == SA_DT
 bool batch_ok(int64_t requests, int64_t tokens) {
   return requests >= 1 && requests < 65536 && tokens >= 1 && tokens < MAX_TOKENS;
 }
-// element strides of (token, head) rows that are read in 16-byte pieces
-bool rows_ok(const void* p, int64_t token, int64_t head, int64_t es) {
-  return p && (uintptr_t)p % 16 == 0 && token >= 0 && head >= 0 && token * es % 16 == 0 && head * es % 16 == 0;
+bool aligned(const void* p) { return p && (uintptr_t)p % 16 == 0; }
+// element strides of (token, head) rows that are read in 16-byte pieces, 128 rows within a buffer resource's 2 GiB
+bool rows_ok(const void* p, int64_t token, int64_t head, int64_t head_dim, int64_t es) {
+  return aligned(p) && token >= head_dim && token < ((int64_t)1 << 31) / (128 * es) && head >= 0 && token * es % 16 == 0 &&
+         head * es % 16 == 0;
 }
 
 template <class S, class P>
@@ -91,8 +93,8 @@ int sa_paged_append(const void* k, int64_t k_token, int64_t k_head, const void* 
   if (!head_dim_ok(head_dim)) return SA_ERR_HEAD_DIM;
   if (tokens < 0 || tokens >= MAX_TOKENS || heads < 1 || heads >= 65536 || pages < 1 || pages > INT32_MAX || sh < 0) return SA_ERR_ARGUMENT;
   if (tokens == 0) return SA_OK;
-  if (!rows_ok(k, k_token, k_head, ss) || !rows_ok(v, v_token, v_head, ss) || !rows_ok(k_pages, 0, 0, es) ||
-      !rows_ok(v_pages, 0, 0, es) || !slots)
+  if (!rows_ok(k, k_token, k_head, head_dim, ss) || !rows_ok(v, v_token, v_head, head_dim, ss) || !aligned(k_pages) ||
+      !aligned(v_pages) || !slots)
     return SA_ERR_ARGUMENT;
   if (tokens * heads * head_dim / 4 >= ((int64_t)1 << 31) * NTHREADS) return SA_ERR_ARGUMENT;
   AppendCall c{};
@@ -118,7 +120,7 @@ int sa_paged_append(const void* k, int64_t k_token, int64_t k_head, const void* 
 
 static bool paged_sizes_ok(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t max_new, int64_t max_len) {
   return batch_ok(requests, tokens) && heads >= 1 && heads < 65536 && groups >= 1 && heads % groups == 0 && max_new >= 1 &&
-         max_new <= tokens && max_len >= 1 && max_len <= MAX_LEN && tokens * heads < ((int64_t)1 << 30) &&
+         max_new <= tokens && max_len >= 1 && max_len < MAX_LEN && tokens * heads < ((int64_t)1 << 30) &&
          tokens * heads + requests * groups * cdiv(max_len, 4 * NTHREADS) < ((int64_t)1 << 31);
 }
 
@@ -141,7 +143,7 @@ int sa_paged_attention(const void* q, int64_t q_token, int64_t q_head, const voi
   if (pages < 1 || pages > INT32_MAX || width < 1 || table_ld < width || max_len > width * page_size || state_ld < max_len)
     return SA_ERR_ARGUMENT;
   if (!(scale > 0.f) || !(scale < INFINITY)) return SA_ERR_ARGUMENT;
-  if (!rows_ok(q, q_token, q_head, es) || !rows_ok(k_pages, 0, 0, es) || !rows_ok(v_pages, 0, 0, es) || !rows_ok(out, 0, 0, es) ||
+  if (!rows_ok(q, q_token, q_head, head_dim, es) || !aligned(k_pages) || !aligned(v_pages) || !aligned(out) ||
       !table || !lengths || !starts || !selected)
     return SA_ERR_ARGUMENT;
   const int64_t need = sa_paged_attention_workspace_bytes(requests, tokens, heads, groups, head_dim, max_new, max_len, dtype);

@@ -85,11 +85,13 @@ def _check_cuda(t: Tensor) -> None:
 
 def _rows(x: Tensor) -> Tensor:
     """(N, H, D) rows as the kernels read them: 16-byte pieces of contiguous elements, tokens and heads any 16-byte
-    multiple apart (a slice of a packed projection is read in place); else a contiguous copy."""
-    piece = 16 // x.element_size()
-    if x.stride(2) != 1 or x.stride(0) % piece or x.stride(1) % piece or x.data_ptr() % 16 or x.stride(0) < 0 or x.stride(1) < 0:
-        return x.contiguous() if not x.is_contiguous() else x.clone()
-    return x
+    multiple apart (a slice of a packed projection is read in place), tokens less than 2^24 bytes; else a contiguous copy."""
+    size = x.element_size()
+    token, head, unit = x.stride()
+    if (unit == 1 and x.shape[2] <= token < (1 << 24) // size and head >= 0 and token * size % 16 == 0 and head * size % 16 == 0
+            and x.data_ptr() % 16 == 0):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def _call(device: torch.device, fn, *args) -> None:
@@ -194,7 +196,7 @@ def _check_step(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, leng
             or selected.stride(0) != selected.shape[1] * selected.stride(1) or selected.stride(1) < selected.shape[2]):
         raise ValueError(f"selected must be a ({requests}, G, L) fp32 tensor with G dividing H, rows a fixed stride apart, "
                          f"on q's device; got {selected.dtype} {tuple(selected.shape)} on {selected.device}")
-    holds = min(table.shape[1] * page_size, selected.shape[2], 1 << 30)
+    holds = min(table.shape[1] * page_size, selected.shape[2], (1 << 30) - 1)
     if holds < 1:
         raise ValueError("selected holds no position")
     if max_len is None:
