@@ -376,7 +376,7 @@ SA_HIDDEN int paged_f32(const PagedLaunch& c);    // sa_paged_f32.hip
 // (carry), and where the key range is split the spans' partials.
 struct PagedShape {
   bool step;
-  int nw, hg;                 // several tokens: wavefronts (32 query rows each) per workgroup, heads per wavefront
+  int nw, hg;                 // several tokens: query tiles of 32 rows per workgroup, heads per wavefront (4: per workgroup, paged_fwd4)
   int splits, span_tiles;     // key spans, and their 32-key tiles
   int chunk, carry_blocks;    // one token: keys per workgroup; several: workgroups along the keys of the histories
   int64_t carry_ld;           // floats of a history row (one token: of a new state row)
@@ -401,11 +401,11 @@ inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_
   } else {
     const int64_t per = H / G;
     s.nw = max_new <= TILE ? 1 : 4;
-    s.hg = es == 2 && D <= 64 && per % 2 == 0 ? 2 : 1;
+    s.hg = es == 2 && D == 64 && per % 4 == 0 && s.nw == 4 ? 4 : es == 2 && D <= 64 && per % 2 == 0 ? 2 : 1;
     const int64_t rows = (int64_t)s.nw * TILE;
     const int64_t tiles = cdiv(max_len, TILE);
     const int64_t workgroups = std::max(cdiv(N, rows), std::min(R, N)) * (H / s.hg);   // (of live tiles)
-    const int64_t target = s.nw == 4 ? 512 : 2048;
+    const int64_t target = s.hg == 4 ? 256 : s.nw == 4 ? 512 : 2048;
     const int64_t splits = std::max<int64_t>(1, std::min(cdiv(target, workgroups), cdiv(tiles, 16)));
     s.span_tiles = (int)cdiv(tiles, splits);
     s.splits = (int)cdiv(tiles, s.span_tiles);

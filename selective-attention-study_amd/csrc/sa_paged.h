@@ -423,28 +423,31 @@ struct PagedTile {
   static __device__ __forceinline__ u32x4 row_frag(const char* t, int n, int h, int s) {
     return *reinterpret_cast<const u32x4*>(t + n * RB + (((2 * s + h) ^ paged_swz<CPR>(n)) << 4));
   }
+  // columns 32 db .. of the rows of step s, transposed (16-bit types): the operand of V^T P, rows in the accumulator's order
+  // (the tile at t + at: one sum and one pointer step, since through a longer chain of them the compiler no longer knows
+  // which LDS variable a transposing read is of, and waits for the loads into the others)
+  static __device__ __forceinline__ u32x4 value_frag(const char* t, int at, int lane, int db, int s) {
+    const int g = lane >> 4, k = lane & 15;
+    // (a row of 16 columns: its upper 16 lanes read some of the same, for output rows that nobody keeps)
+    const int c = (4 * db + 2 * (g & 1) + ((k & 3) >> 1)) & (CPR - 1);
+    u32x4 f;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = 16 * s + 8 * hf + 4 * (g >> 1) + (k >> 2);
+      typedef __attribute__((address_space(3))) short4v* lds_s4;
+      const int off = at + r * RB + ((c ^ paged_swz<CPR>(r)) << 4) + 8 * (k & 1);
+      const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + off));
+      const uint2 u = __builtin_bit_cast(uint2, x);
+      f[2 * hf] = u.x;
+      f[2 * hf + 1] = u.y;
+    }
+    return f;
+  }
   // o (columns 32 db ..) += V^T P for the tile's rows, P in the accumulator's layout (lane = query)
   static __device__ __forceinline__ f32x16 values(const char* t, int lane, int db, const u32x4* pf, const f32x16& p, f32x16 o) {
     if constexpr (ES == 2) {
-      const int g = lane >> 4, k = lane & 15;
-      // (a row of 16 columns: its upper 16 lanes read some of the same, for output rows that nobody keeps)
-      const int c = (4 * db + 2 * (g & 1) + ((k & 3) >> 1)) & (CPR - 1);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u32x4 f;
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int r = 16 * s + 8 * hf + 4 * (g >> 1) + (k >> 2);
-          typedef __attribute__((address_space(3))) short4v* lds_s4;
-          // (a pointer cast: through an integer the compiler would no longer know which tile is read, and wait for
-          // the loads into the other)
-          const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + r * RB + ((c ^ paged_swz<CPR>(r)) << 4) + 8 * (k & 1)));
-          const uint2 u = __builtin_bit_cast(uint2, x);
-          f[2 * hf] = u.x;
-          f[2 * hf + 1] = u.y;
-        }
-        o = P::mma(f, pf[s], o);
-      }
+      for (int s = 0; s < 2; ++s) o = P::mma(value_frag(t, 0, lane, db, s), pf[s], o);
     } else {
       const int n = lane & 31, h = lane >> 5, d = (32 * db + n) & (D - 1);
 #pragma unroll
@@ -657,6 +660,75 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
 //
 // P is rounded to the cache's type for the product with V (relative 2^-9 bf16, 2^-12 fp16 at random, the size of the
 // output's own rounding; fp32 not at all); logits, F, row statistics and sums are fp32.
+struct PagedTiles {   // what a workgroup of query tiles has to do
+  PagedRequest rq;
+  int r, row0;        // request, its first row
+  int kt_lo, kt_hi;   // the key tiles of its span that one of its rows sees
+};
+// Workgroup number x (1 << SH rows, numbered as above) and key span z; false: nothing. Rows that no workgroup computes, those
+// behind the last request and those of requests left out, become zero here, COLS columns from col0 on, unless the spans are
+// joined afterwards (the join does it).
+template <class P, int SH, int COLS, int THREADS>
+__device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, int span_tiles, int64_t row_elems, int col0, bool joined,
+                                            PagedTiles& w) {
+  auto clear = [&](int first, int count) {
+    typename P::elem* out = static_cast<typename P::elem*>(a.out) + first * row_elems + col0;
+    for (int i = threadIdx.x; i < count * COLS; i += THREADS) out[i / COLS * row_elems + i % COLS] = P::to_elem(0.f);
+  };
+  const bool zeros = !joined && z == 0;
+  if (zeros) {
+    const int hi = min((x + 1) << SH, a.N), lo = min(max(x << SH, a.starts[a.R]), hi);
+    clear(lo, hi - lo);
+  }
+  w.r = find_request<false>(a.starts, a.R, x, SH);
+  w.rq = paged_request(a, w.r);
+  w.row0 = (x - ((w.rq.first >> SH) + w.r)) << SH;
+  if (w.row0 < 0 || w.row0 >= w.rq.n) return false;
+  if (!w.rq.live) {
+    if (zeros) clear(w.rq.first + w.row0, min(1 << SH, w.rq.n - w.row0));
+    return false;
+  }
+  w.kt_lo = z * span_tiles;
+  w.kt_hi = min((w.rq.c + min(w.row0 + (1 << SH), w.rq.n) - 1) / TILE + 1, w.kt_lo + span_tiles);
+  return w.kt_lo < w.kt_hi;
+}
+
+// A wavefront's results for the request's row `row` (lane = row; o transposed, 4 columns per quarter): the output, or the
+// span's part of it: reference m (log2 units), sum l, and the sums of weighted values.
+template <class P, int D>
+__device__ __forceinline__ void paged_write(const PagedCall& a, const PagedTiles& w, int row, int head, int z, float m, float l,
+                                            const f32x16 (&o)[PagedTile<P, D>::DB], int h, float* part_ml, float* part_o) {
+  typedef typename P::elem elem;
+  const Halves lh = halves(l);
+  if (row >= w.rq.n) return;
+  const float ltot = lh.lo + lh.hi;
+  const int64_t at = (int64_t)(w.rq.first + row) * a.H + head, part = (int64_t)z * a.N * a.H + at;
+  const bool joined = part_o != nullptr;
+  if (joined && h == 0) {
+    part_ml[2 * part] = m;
+    part_ml[2 * part + 1] = ltot;
+  }
+  const float inv = joined ? 1.f : 1.f / ltot;
+#pragma unroll
+  for (int db = 0; db < PagedTile<P, D>::DB; ++db) {
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int d = db * 32 + 8 * q4 + 4 * h;
+      if (D < 32 && d >= D) continue;
+      const float4 v4 = make_float4(o[db][4 * q4] * inv, o[db][4 * q4 + 1] * inv, o[db][4 * q4 + 2] * inv, o[db][4 * q4 + 3] * inv);
+      elem* out = static_cast<elem*>(a.out) + at * D + d;
+      if (joined) {
+        *reinterpret_cast<float4*>(part_o + part * D + d) = v4;
+      } else if constexpr (sizeof(elem) == 2) {
+        *reinterpret_cast<uint2*>(out) = make_uint2((uint32_t)P::to_elem(v4.x) | ((uint32_t)P::to_elem(v4.y) << 16),
+                                                    (uint32_t)P::to_elem(v4.z) | ((uint32_t)P::to_elem(v4.w) << 16));
+      } else {
+        *reinterpret_cast<float4*>(out) = v4;
+      }
+    }
+  }
+}
+
 template <class P, int D, int HG, int NW>
 struct FwdLds {
   typedef PagedTile<P, D> T;
@@ -688,28 +760,10 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   const int n = lane & 31, h = lane >> 5;
   const int x = gridDim.x - 1 - blockIdx.x;
   const int hd0 = blockIdx.y * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
-  elem* out = static_cast<elem*>(a.out);
-  const bool split = part_o != nullptr;
-
-  if (!split && blockIdx.z == 0) {   // rows behind the last request
-    const int hi = min((x + 1) << SH, a.N), lo = min(max(x << SH, a.starts[a.R]), hi);
-    for (int i = tid; i < (hi - lo) * (HG * D); i += NW * 64)
-      out[(int64_t)(lo + i / (HG * D)) * a.H * D + hd0 * D + i % (HG * D)] = P::to_elem(0.f);
-  }
-  const int r = find_request<false>(a.starts, a.R, x, SH);
-  const PagedRequest rq = paged_request(a, r);
-  const int row0 = (x - ((rq.first >> SH) + r)) << SH;   // the workgroup's first row of the request
-  if (row0 < 0 || row0 >= rq.n) return;
-  if (!rq.live) {
-    if (!split && blockIdx.z == 0)
-      for (int i = tid; i < min(1 << SH, rq.n - row0) * (HG * D); i += NW * 64)
-        out[(int64_t)(rq.first + row0 + i / (HG * D)) * a.H * D + hd0 * D + i % (HG * D)] = P::to_elem(0.f);
-    return;
-  }
-  const int kt_lo = blockIdx.z * span_tiles;
-  const int last_row = min(row0 + (1 << SH), rq.n) - 1;
-  const int kt_hi = min((rq.c + last_row) / TILE + 1, kt_lo + span_tiles);
-  if (kt_lo >= kt_hi) return;
+  PagedTiles w;
+  if (!paged_tiles<P, SH, HG * D, NW * 64>(a, x, blockIdx.z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
+  const PagedRequest& rq = w.rq;
+  const int r = w.r, row0 = w.row0, kt_lo = w.kt_lo, kt_hi = w.kt_hi;
 
   const int rb0 = row0 + wave * TILE;          // the wavefront's first row
   const int qpos0 = rq.c + rb0;                // and its position
@@ -887,41 +941,265 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
     if (cur < kt_lo) break;
   }
 
-  if (q_row >= rq.n) return;
-  const int64_t token = rq.first + q_row;
 #pragma unroll
-  for (int g = 0; g < HG; ++g) {
-    const Halves lh = halves(l[g]);
-    const float ltot = lh.lo + lh.hi;
-    const int64_t row = token * a.H + hd0 + g;
-    if (split) {
-      const int64_t prow = (int64_t)blockIdx.z * a.N * a.H + row;
-      if (h == 0) {
-        part_ml[2 * prow] = m[g];
-        part_ml[2 * prow + 1] = ltot;
+  for (int g = 0; g < HG; ++g) paged_write<P, D>(a, w, q_row, hd0 + g, blockIdx.z, m[g], l[g], o[g], h, part_ml, part_o);
+}
+
+// The same for groups of four heads or more at 16-bit head dim 64, the usual sizes of a long step: eight wavefronts, one
+// workgroup per CU, query tiles 4 x 32 rows, four heads. A wavefront has 64 of the rows of one head, so that every key and value
+// fragment that it reads from LDS serves two products, and each tile's selection is made once for the four heads:
+// wavefront w makes query tile w % 4's F for every second key tile (wavefronts w and w + 4, on one SIMD, take turns).
+//
+// What bounds paged_fwd_kernel is the vector unit, beside it LDS: per head and tile 16 exponentials (256 cycles of a SIMD)
+// and, of some 90 other instructions, half of a selection's 105 and the running maximum's. Here a quarter of a selection,
+// and no maximum: the weights are taken against the reference mu of the tiles before, and only where a row's sum of
+// them over a tile passes 2^14 (or a row has no reference yet) is the maximum looked for, mu moved and the tile's weights
+// taken again. Any reference within 2^14 of the maximum gives the same weights to rounding, fp16's range included.
+// LDS per wavefront and tile: K 4, V 4, F 8 and half of a selection's 8 KB for two head-tiles, against 28.
+constexpr float PAGED_FWD4_BIG = 16384.f;
+
+template <class P>
+__global__ __launch_bounds__(512, 1) void paged_fwd4_kernel(PagedCall a, const float* __restrict__ carry, int64_t carry_ld,
+                                                            int span_tiles, float* __restrict__ part_ml, float* __restrict__ part_o) {
+  constexpr int D = 64, HG = 4, SH = 7, LDF = TILE + 4;
+  typedef PagedTile<P, D> T;
+  typedef typename P::elem elem;
+  typedef PagedRows<P, D, 4> Rows;
+  constexpr int NS = T::NS, DB = T::DB;
+  static_assert(T::ES == 2 && Rows::PER == 1 && Rows::UNIFORM, "parts of eight rows, one per wavefront of four");
+  // lifetimes as in paged_fwd_kernel; sF0, sF1 the four query tiles' F of the t-th tile visited (buffer t mod 2, written at the
+  // end of step t - 1, read in step t)
+  struct Tiles {
+    __attribute__((aligned(16))) char k[HG][T::BYTES];
+    __attribute__((aligned(16))) char v[HG][T::BYTES];
+  };
+  __shared__ Tiles sB0, sB1;
+  __shared__ __attribute__((aligned(16))) char sS0[T::BYTES], sS1[T::BYTES];
+  __shared__ __attribute__((aligned(16))) float sF0[4][TILE * LDF], sF1[4][TILE * LDF];
+  __shared__ u32x4 sQ[4][NS * 64];   // the selector's query fragments (written once: registers are short)
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
+  const int u = wave & 3, half = wave >> 2;   // head and rows of the wavefront; u: also its part of a tile's loads and its selections
+  const int groups = a.H / HG, x = gridDim.y - 1 - blockIdx.y, z = blockIdx.x / groups;
+  const int hd0 = (blockIdx.x % groups) * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
+  PagedTiles w;
+  if (!paged_tiles<P, SH, HG * D, 512>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
+  const PagedRequest& rq = w.rq;
+  const int kt_lo = w.kt_lo;
+
+  const int rb[2] = {w.row0 + (2 * half) * TILE, w.row0 + (2 * half + 1) * TILE};   // the wavefront's query tiles: first rows
+  const int sel0 = w.row0 + u * TILE;                                               // and that of its selections
+  auto end_of = [&](int row) { return row < rq.n ? (rq.c + row + TILE - 1) / TILE + 1 : 0; };   // tiles that it needs
+  const int end[2] = {end_of(rb[0]), end_of(rb[1])}, sel_end = end_of(sel0);
+
+  u32x4 qf[2][NS];
+  {
+    const elem* qp = static_cast<const elem*>(a.q) + (int64_t)rq.first * a.q_token;
+    auto frag = [&](int row, int head, int s) -> u32x4 {
+      return row < rq.n ? *reinterpret_cast<const u32x4*>(qp + row * a.q_token + head * a.q_head + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
+    };
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      qf[0][s] = frag(rb[0] + n, hd0 + u, s);
+      qf[1][s] = frag(rb[1] + n, hd0 + u, s);
+      if (half == 0) sQ[u][s * 64 + lane] = frag(sel0 + n, hsel, s);
+    }
+  }
+  float mu[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};   // (no reference yet: the first weights overflow)
+  f32x16 o[2][DB];
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[b][db] = zero16();
+  const float sl2 = a.scale * LOG2E, neg_inv_scale = -1.f / a.scale;
+
+  const Rows rows(a, w.r, rq.t, u, lane);
+  const int64_t head_bytes = (int64_t)T::RB << a.pshift;
+  const char* kp = static_cast<const char*>(a.k_pages) + (hd0 + 2 * half) * head_bytes;
+  const char* vp = static_cast<const char*>(a.v_pages) + (hd0 + 2 * half) * head_bytes;
+  const char* kselp = static_cast<const char*>(a.k_pages) + hsel * head_bytes;
+  const float* crow_p = carry + ((int64_t)((rq.first >> 5) + w.r + (min(sel0, rq.n - 1) >> 5)) * a.G + g0) * carry_ld;
+
+  auto load_tile = [&](Tiles& B, const typename Rows::Place (&pl)[1]) {   // each half its two heads
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      rows.load(B.k[2 * half + g], kp + g * head_bytes, pl, u);
+      rows.load(B.v[2 * half + g], vp + g * head_bytes, pl, u);
+    }
+  };
+  auto load_sel = [&](char* S, const typename Rows::Place (&pl)[1]) {
+    if (half == 0) rows.load(S, kselp, pl, u);
+  };
+  auto carry_of = [&](int kt) { return kt >= kt_lo ? crow_p[min(kt * TILE + n, rq.t - 1)] : 0.f; };
+
+  auto select = [&](int kt, const char* S, float entry, float* fw) {   // paged_fwd_kernel's
+    const int kbase = kt * TILE, qpos0 = rq.c + sel0;
+    f32x16 l0 = zero16();
+#pragma unroll
+    for (int s = 0; s < NS; ++s) l0 = P::mma(sQ[u][s * 64 + lane], T::row_frag(S, n, h, s), l0);
+    f32x16 sel;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sel[i] = __builtin_amdgcn_fmed3f(-l0[i], -3.0e38f, 0.f);
+    if (kbase + TILE - 1 >= qpos0 || kbase < a.exempt) {
+      const int jk = kbase + n, thr = jk >= a.exempt ? jk - qpos0 - 4 * h : 32;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sel[i] = crow(i, 0) > thr ? sel[i] : 0.f;
+    }
+    float run = entry * neg_inv_scale;
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const Halves s4 = halves(((sel[4 * q4] + sel[4 * q4 + 1]) + sel[4 * q4 + 2]) + sel[4 * q4 + 3]);
+      float p = (h == 0) ? run : run + s4.lo;
+#pragma unroll
+      for (int t2 = 0; t2 < 4; ++t2) {
+        fw[crow(4 * q4 + t2, h) * LDF + n] = p;
+        p += sel[4 * q4 + t2];
+      }
+      run = (run + s4.lo) + s4.hi;
+    }
+  };
+
+  // One key tile against the query tiles b0 .. b1 - 1 of the wavefront; EDGE: keys past a query are masked
+  auto attend = [&](int kt, const Tiles& B, const float (*F)[TILE * LDF], auto b0_tag, auto b1_tag, auto edge_tag)
+                    __attribute__((always_inline)) {
+    constexpr int B0 = decltype(b0_tag)::value, B1 = decltype(b1_tag)::value;
+    constexpr bool EDGE = decltype(edge_tag)::value;
+    f32x16 lg[2];
+#pragma unroll
+    for (int b = B0; b < B1; ++b) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 f4 = *reinterpret_cast<const float4*>(&F[2 * half + b][n * LDF + 8 * q4 + 4 * h]);
+        lg[b][4 * q4] = f4.x;
+        lg[b][4 * q4 + 1] = f4.y;
+        lg[b][4 * q4 + 2] = f4.z;
+        lg[b][4 * q4 + 3] = f4.w;
       }
     }
-    const float inv = split ? 1.f : 1.f / ltot;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const u32x4 kf = T::row_frag(B.k[u], n, h, s);
+#pragma unroll
+      for (int b = B0; b < B1; ++b) lg[b] = P::mma(kf, qf[b][s], lg[b]);
+    }
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int b = B0; b < B1; ++b) {
+        const int thr = rq.c + rb[b] + n - kt * TILE - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lg[b][i] = crow(i, 0) <= thr ? lg[b][i] : -INFINITY;
+      }
+    }
+    u32x4 pf[2][2];
+    float psum[2];
+    bool far = false;
+    auto weights = [&](int b) __attribute__((always_inline)) {
+      f32x16 p;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = fast_exp2(fmaf(lg[b][i], sl2, -mu[b]));
+        s += p[i];
+      }
+      psum[b] = s;
+      pf[b][0] = P::pack(p, 0);
+      pf[b][1] = P::pack(p, 1);
+    };
+#pragma unroll
+    for (int b = B0; b < B1; ++b) {
+      weights(b);
+      far |= !(psum[b] <= PAGED_FWD4_BIG);
+    }
+    if (__builtin_expect(__any(far), 0)) {
+#pragma unroll
+      for (int b = B0; b < B1; ++b) {
+        float zmax = lg[b][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) zmax = fmaxf(zmax, lg[b][i]);
+        const Halves zh = halves(zmax);
+        const float m_new = fmaxf(mu[b], fmaxf(zh.lo, zh.hi) * sl2);
+        const float alpha = fast_exp2(mu[b] - m_new);
+        mu[b] = m_new;
+        l[b] *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[b][db][i] *= alpha;
+        weights(b);
+      }
+    }
+#pragma unroll
+    for (int b = B0; b < B1; ++b) l[b] += psum[b];
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int d = db * 32 + 8 * q4 + 4 * h;
-        if (D < 32 && d >= D) continue;
-        const float4 v4 = make_float4(o[g][db][4 * q4] * inv, o[g][db][4 * q4 + 1] * inv, o[g][db][4 * q4 + 2] * inv,
-                                      o[g][db][4 * q4 + 3] * inv);
-        if (split) {
-          *reinterpret_cast<float4*>(part_o + ((int64_t)blockIdx.z * a.N * a.H + row) * D + d) = v4;
-        } else if constexpr (T::ES == 2) {
-          *reinterpret_cast<uint2*>(out + row * D + d) =
-              make_uint2((uint32_t)P::to_elem(v4.x) | ((uint32_t)P::to_elem(v4.y) << 16),
-                         (uint32_t)P::to_elem(v4.z) | ((uint32_t)P::to_elem(v4.w) << 16));
-        } else {
-          *reinterpret_cast<float4*>(out + row * D + d) = v4;
-        }
+      for (int s = 0; s < 2; ++s) {
+        const u32x4 vf = T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s);
+#pragma unroll
+        for (int b = B0; b < B1; ++b) o[b][db] = P::mma(vf, pf[b][s], o[b][db]);
       }
     }
+  };
+
+  int cur = w.kt_hi - 1;   // the tile of the step; the t-th: t mod 2 names the buffers
+  typename Rows::Place at1[1], at2[1];
+  int pg[1];
+  {
+    typename Rows::Place at0[1];
+    rows.pages_of(cur, pg);
+    rows.places(cur, pg, at0);
+    load_tile(sB0, at0);
+    load_sel(sS0, at0);
+    rows.pages_of(cur - 1 >= kt_lo ? cur - 1 : -1, pg);
+    rows.places(cur - 1, pg, at1);
+    if (cur - 1 >= kt_lo) load_sel(sS1, at1);
+    rows.pages_of(cur - 2 >= kt_lo ? cur - 2 : -1, pg);
   }
+  float entry = carry_of(cur - half);   // of the wavefront's next selection
+  wait_loads();
+  __syncthreads();
+  if (half == 0) {
+    if (cur < sel_end) select(cur, sS0, entry, sF0[u]);
+    entry = carry_of(cur - 2);
+  }
+  __asm__ volatile("" : "+v"(entry));   // (waited for here: in the loop the compiler would wait for the tiles' loads with it)
+  __syncthreads();
+
+  constexpr std::integral_constant<int, 0> i0{};
+  constexpr std::integral_constant<int, 1> i1{};
+  constexpr std::integral_constant<int, 2> i2{};
+  auto step = [&](auto odd_tag) __attribute__((always_inline)) {
+    constexpr int ODD = decltype(odd_tag)::value;
+    Tiles& B = ODD ? sB1 : sB0;
+    const float(*F)[TILE * LDF] = ODD ? sF1 : sF0;
+    rows.places(cur - 2, pg, at2);
+    if (cur - 1 >= kt_lo) load_tile(ODD ? sB0 : sB1, at1);
+    if (cur - 2 >= kt_lo) load_sel(ODD ? sS1 : sS0, at2);
+    rows.pages_of(cur - 3 >= kt_lo ? cur - 3 : -1, pg);
+    // both query tiles have rows (one without has no F), all of which see every key of the tile
+    if (end[1] > 0 && (cur + 1) * TILE <= rq.c + w.row0) {
+      attend(cur, B, F, i0, i2, std::false_type{});
+    } else {
+      if (cur < end[0]) attend(cur, B, F, i0, i1, std::true_type{});
+      if (cur < end[1]) attend(cur, B, F, i1, i2, std::true_type{});
+    }
+    if (half == 1 - ODD) {   // the next tile's F
+      if (cur - 1 >= kt_lo && cur - 1 < sel_end) select(cur - 1, ODD ? sS0 : sS1, entry, ODD ? sF0[u] : sF1[u]);
+      entry = carry_of(cur - 3);
+    }
+    at1[0] = at2[0];
+    wait_loads();
+    __syncthreads();
+    --cur;
+  };
+  while (true) {
+    step(i0);
+    if (cur < kt_lo) break;
+    step(i1);
+    if (cur < kt_lo) break;
+  }
+#pragma unroll
+  for (int b = 0; b < 2; ++b) paged_write<P, D>(a, w, rb[b] + n, hd0 + u, z, mu[b], l[b], o[b], h, part_ml, part_o);
 }
 
 // The spans of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the spans that begin at
@@ -1265,6 +1543,13 @@ int paged_launch(const PagedLaunch& c) {
   {
     TimedLaunch timed(SA_KERNEL_FORWARD, c.st);
     const bool whole = a.G == a.H;
+    if constexpr (sizeof(typename P::elem) == 2 && D == 64) {
+      if (s.hg == 4) {
+        const unsigned tiles = (unsigned)((a.N >> 7) + a.R);
+        hipLaunchKernelGGL((paged_fwd4_kernel<P>), dim3((unsigned)(a.H / 4 * s.splits), tiles), dim3(512), 0, c.st, a, carry, s.carry_ld,
+                           s.span_tiles, ml, o);
+      }
+    }
     if constexpr (sizeof(typename P::elem) == 2 && D <= 64) {
       if (s.hg == 2) {
         if (s.nw == 4) launch_paged_fwd<P, D, 2, 4, false>(a, s, carry, ml, o, c.st);
