@@ -1090,29 +1090,26 @@ __global__ __launch_bounds__(512, 1) void paged_fwd4_kernel(PagedCall a, const f
         for (int i = 0; i < 16; ++i) lg[b][i] = crow(i, 0) <= thr ? lg[b][i] : -INFINITY;
       }
     }
-    u32x4 pf[2][2];
-    float psum[2];
-    bool far = false;
-    auto weights = [&](int b) __attribute__((always_inline)) {
-      f32x16 p;
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = fast_exp2(fmaf(lg[b][i], sl2, -mu[b]));
-        s += p[i];
-      }
-      psum[b] = s;
-      pf[b][0] = P::pack(p, 0);
-      pf[b][1] = P::pack(p, 1);
-    };
+    // query tile after query tile: the first's value products run beneath the second's weights
+    u32x4 vf[DB][2];
 #pragma unroll
     for (int b = B0; b < B1; ++b) {
-      weights(b);
-      far |= !(psum[b] <= PAGED_FWD4_BIG);
-    }
-    if (__builtin_expect(__any(far), 0)) {
+      u32x4 pf[2];
+      float psum;
+      auto weights = [&]() __attribute__((always_inline)) {
+        f32x16 p;
+        float s = 0.f;
 #pragma unroll
-      for (int b = B0; b < B1; ++b) {
+        for (int i = 0; i < 16; ++i) {
+          p[i] = fast_exp2(fmaf(lg[b][i], sl2, -mu[b]));
+          s += p[i];
+        }
+        psum = s;
+        pf[0] = P::pack(p, 0);
+        pf[1] = P::pack(p, 1);
+      };
+      weights();
+      if (__builtin_expect(__any(!(psum <= PAGED_FWD4_BIG)), 0)) {
         float zmax = lg[b][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) zmax = fmaxf(zmax, lg[b][i]);
@@ -1125,19 +1122,16 @@ __global__ __launch_bounds__(512, 1) void paged_fwd4_kernel(PagedCall a, const f
         for (int db = 0; db < DB; ++db)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[b][db][i] *= alpha;
-        weights(b);
+        weights();
       }
-    }
+      l[b] += psum;
 #pragma unroll
-    for (int b = B0; b < B1; ++b) l[b] += psum[b];
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int db = 0; db < DB; ++db) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const u32x4 vf = T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s);
-#pragma unroll
-        for (int b = B0; b < B1; ++b) o[b][db] = P::mma(vf, pf[b][s], o[b][db]);
-      }
+        for (int s = 0; s < 2; ++s) {
+          if (b == B0) vf[db][s] = T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s);
+          o[b][db] = P::mma(vf[db][s], pf[s], o[b][db]);
+        }
     }
   };
 
