@@ -945,30 +945,32 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   for (int g = 0; g < HG; ++g) paged_write<P, D>(a, w, q_row, hd0 + g, blockIdx.z, m[g], l[g], o[g], h, part_ml, part_o);
 }
 
-// The same for groups of four heads or more at 16-bit head dim 64, the usual sizes of a long step: eight wavefronts, one
-// workgroup per CU, query tiles 4 x 32 rows, four heads. A wavefront has 64 of the rows of one head, so that every key and value
-// fragment that it reads from LDS serves two products, and each tile's selection is made once for the four heads:
-// wavefront w makes query tile w % 4's F for every second key tile (wavefronts w and w + 4, on one SIMD, take turns).
+// The same for groups of four heads or more at 16-bit head dim 64, the usual sizes of a long step: sixteen wavefronts, one
+// workgroup per CU, query tiles 4 x 32 rows, four heads; wavefront w has head w % 4, query tile w / 4. Each tile's selection is
+// made once for the four heads (every wavefront one tile in four, its own query tile's, in turns that give each SIMD one
+// of the four selections of a step).
 //
-// What bounds paged_fwd_kernel is the vector unit, beside it LDS: per head and tile 16 exponentials (256 cycles of a SIMD)
-// and, of some 90 other instructions, half of a selection's 105 and the running maximum's. Here a quarter of a selection,
-// and no maximum: the weights are taken against the reference mu of the tiles before, and only where a row's sum of
-// them over a tile passes 2^14 (or a row has no reference yet) is the maximum looked for, mu moved and the tile's weights
-// taken again. Any reference within 2^14 of the maximum gives the same weights to rounding, fp16's range included.
-// LDS per wavefront and tile: K 4, V 4, F 8 and half of a selection's 8 KB for two head-tiles, against 28.
+// What bounds paged_fwd_kernel is the vector unit: per head and tile 16 exponentials (256 cycles of a SIMD) and, of some 90
+// other instructions, half of a selection's 105 and the running maximum's. Here a quarter of a selection, and no maximum: the
+// weights are taken against the reference mu of the tiles before, and only where a row's sum of them over a tile
+// passes 2^14 (or a row has no reference yet) is the maximum looked for, mu moved and the tile's weights taken again.
+// Any reference within 2^14 of the maximum gives the same weights to rounding, fp16's range included. At 4096 queries on
+// 32768 keys, 16 heads: 0.80 ms (644 TFLOP/s of the two products), paged_fwd_kernel 1.04; with the selection after the products 0.91,
+// with eight wavefronts of two query tiles each 0.97 (0.91). What is left over is each step's common start and end: its LDS reads
+// at once (0.46 ms without selection, value products and loads), and the wait for its last wavefront.
 constexpr float PAGED_FWD4_BIG = 16384.f;
 
 template <class P>
-__global__ __launch_bounds__(512, 1) void paged_fwd4_kernel(PagedCall a, const float* __restrict__ carry, int64_t carry_ld,
-                                                            int span_tiles, float* __restrict__ part_ml, float* __restrict__ part_o) {
+__global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const float* __restrict__ carry, int64_t carry_ld,
+                                                          int span_tiles, float* __restrict__ part_ml, float* __restrict__ part_o) {
   constexpr int D = 64, HG = 4, SH = 7, LDF = TILE + 4;
   typedef PagedTile<P, D> T;
   typedef typename P::elem elem;
   typedef PagedRows<P, D, 4> Rows;
   constexpr int NS = T::NS, DB = T::DB;
   static_assert(T::ES == 2 && Rows::PER == 1 && Rows::UNIFORM, "parts of eight rows, one per wavefront of four");
-  // lifetimes as in paged_fwd_kernel; sF0, sF1 the four query tiles' F of the t-th tile visited (buffer t mod 2, written at the
-  // end of step t - 1, read in step t)
+  // lifetimes as in paged_fwd_kernel; sF0, sF1 the four query tiles' F of the t-th tile visited (buffer t mod 2, written in step
+  // t - 1, read in step t)
   struct Tiles {
     __attribute__((aligned(16))) char k[HG][T::BYTES];
     __attribute__((aligned(16))) char v[HG][T::BYTES];
@@ -979,64 +981,57 @@ __global__ __launch_bounds__(512, 1) void paged_fwd4_kernel(PagedCall a, const f
   __shared__ u32x4 sQ[4][NS * 64];   // the selector's query fragments (written once: registers are short)
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
-  const int u = wave & 3, half = wave >> 2;   // head and rows of the wavefront; u: also its part of a tile's loads and its selections
+  const int u = wave & 3, qt = wave >> 2;   // the wavefront's head and query tile
   const int groups = a.H / HG, x = gridDim.y - 1 - blockIdx.y, z = blockIdx.x / groups;
   const int hd0 = (blockIdx.x % groups) * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
   PagedTiles w;
-  if (!paged_tiles<P, SH, HG * D, 512>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
+  if (!paged_tiles<P, SH, HG * D, 1024>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
   const PagedRequest& rq = w.rq;
   const int kt_lo = w.kt_lo;
 
-  const int rb[2] = {w.row0 + (2 * half) * TILE, w.row0 + (2 * half + 1) * TILE};   // the wavefront's query tiles: first rows
-  const int sel0 = w.row0 + u * TILE;                                               // and that of its selections
-  auto end_of = [&](int row) { return row < rq.n ? (rq.c + row + TILE - 1) / TILE + 1 : 0; };   // tiles that it needs
-  const int end[2] = {end_of(rb[0]), end_of(rb[1])}, sel_end = end_of(sel0);
+  const int rb = w.row0 + qt * TILE, qpos0 = rq.c + rb;   // the query tile's first row and its position
+  const int end = rb < rq.n ? (qpos0 + TILE - 1) / TILE + 1 : 0;   // tiles that it needs
 
-  u32x4 qf[2][NS];
+  u32x4 qf[NS];
   {
-    const elem* qp = static_cast<const elem*>(a.q) + (int64_t)rq.first * a.q_token;
-    auto frag = [&](int row, int head, int s) -> u32x4 {
-      return row < rq.n ? *reinterpret_cast<const u32x4*>(qp + row * a.q_token + head * a.q_head + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
+    const int row = rb + n;
+    const elem* qp = static_cast<const elem*>(a.q) + (int64_t)(rq.first + row) * a.q_token;
+    auto frag = [&](int head, int s) -> u32x4 {
+      return row < rq.n ? *reinterpret_cast<const u32x4*>(qp + head * a.q_head + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
     };
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      qf[0][s] = frag(rb[0] + n, hd0 + u, s);
-      qf[1][s] = frag(rb[1] + n, hd0 + u, s);
-      if (half == 0) sQ[u][s * 64 + lane] = frag(sel0 + n, hsel, s);
+      qf[s] = frag(hd0 + u, s);
+      if (u == 0) sQ[qt][s * 64 + lane] = frag(hsel, s);
     }
   }
-  float mu[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};   // (no reference yet: the first weights overflow)
-  f32x16 o[2][DB];
+  float mu = -1e30f, l = 0.f;   // (no reference yet: the first weights overflow)
+  f32x16 o[DB];
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o[b][db] = zero16();
+  for (int db = 0; db < DB; ++db) o[db] = zero16();
   const float sl2 = a.scale * LOG2E, neg_inv_scale = -1.f / a.scale;
 
-  const Rows rows(a, w.r, rq.t, u, lane);
+  // loads: the wavefront's part (qt) of its head's K and V tile; those of head hd0's of the selector's K tile too
+  const Rows rows(a, w.r, rq.t, qt, lane);
   const int64_t head_bytes = (int64_t)T::RB << a.pshift;
-  const char* kp = static_cast<const char*>(a.k_pages) + (hd0 + 2 * half) * head_bytes;
-  const char* vp = static_cast<const char*>(a.v_pages) + (hd0 + 2 * half) * head_bytes;
+  const char* kp = static_cast<const char*>(a.k_pages) + (hd0 + u) * head_bytes;
+  const char* vp = static_cast<const char*>(a.v_pages) + (hd0 + u) * head_bytes;
   const char* kselp = static_cast<const char*>(a.k_pages) + hsel * head_bytes;
-  const float* crow_p = carry + ((int64_t)((rq.first >> 5) + w.r + (min(sel0, rq.n - 1) >> 5)) * a.G + g0) * carry_ld;
-
-  auto load_tile = [&](Tiles& B, const typename Rows::Place (&pl)[1]) {   // each half its two heads
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      rows.load(B.k[2 * half + g], kp + g * head_bytes, pl, u);
-      rows.load(B.v[2 * half + g], vp + g * head_bytes, pl, u);
-    }
+  auto load_tile = [&](Tiles& B, const typename Rows::Place (&pl)[1]) {
+    rows.load(B.k[u], kp, pl, qt);
+    rows.load(B.v[u], vp, pl, qt);
   };
   auto load_sel = [&](char* S, const typename Rows::Place (&pl)[1]) {
-    if (half == 0) rows.load(S, kselp, pl, u);
+    if (u == 0) rows.load(S, kselp, pl, qt);
   };
+  const float* crow_p = carry + ((int64_t)((rq.first >> 5) + w.r + (min(rb, rq.n - 1) >> 5)) * a.G + g0) * carry_ld;
   auto carry_of = [&](int kt) { return kt >= kt_lo ? crow_p[min(kt * TILE + n, rq.t - 1)] : 0.f; };
 
   auto select = [&](int kt, const char* S, float entry, float* fw) {   // paged_fwd_kernel's
-    const int kbase = kt * TILE, qpos0 = rq.c + sel0;
+    const int kbase = kt * TILE;
     f32x16 l0 = zero16();
 #pragma unroll
-    for (int s = 0; s < NS; ++s) l0 = P::mma(sQ[u][s * 64 + lane], T::row_frag(S, n, h, s), l0);
+    for (int s = 0; s < NS; ++s) l0 = P::mma(sQ[qt][s * 64 + lane], T::row_frag(S, n, h, s), l0);
     f32x16 sel;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sel[i] = __builtin_amdgcn_fmed3f(-l0[i], -3.0e38f, 0.f);
@@ -1059,83 +1054,63 @@ __global__ __launch_bounds__(512, 1) void paged_fwd4_kernel(PagedCall a, const f
     }
   };
 
-  // One key tile against the query tiles b0 .. b1 - 1 of the wavefront; EDGE: keys past a query are masked
-  auto attend = [&](int kt, const Tiles& B, const float (*F)[TILE * LDF], auto b0_tag, auto b1_tag, auto edge_tag)
-                    __attribute__((always_inline)) {
-    constexpr int B0 = decltype(b0_tag)::value, B1 = decltype(b1_tag)::value;
-    constexpr bool EDGE = decltype(edge_tag)::value;
-    f32x16 lg[2];
+  auto attend = [&](int kt, const Tiles& B, const float* F) __attribute__((always_inline)) {
+    f32x16 lg;
 #pragma unroll
-    for (int b = B0; b < B1; ++b) {
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const float4 f4 = *reinterpret_cast<const float4*>(&F[2 * half + b][n * LDF + 8 * q4 + 4 * h]);
-        lg[b][4 * q4] = f4.x;
-        lg[b][4 * q4 + 1] = f4.y;
-        lg[b][4 * q4 + 2] = f4.z;
-        lg[b][4 * q4 + 3] = f4.w;
-      }
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const float4 f4 = *reinterpret_cast<const float4*>(F + n * LDF + 8 * q4 + 4 * h);
+      lg[4 * q4] = f4.x;
+      lg[4 * q4 + 1] = f4.y;
+      lg[4 * q4 + 2] = f4.z;
+      lg[4 * q4 + 3] = f4.w;
     }
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const u32x4 kf = T::row_frag(B.k[u], n, h, s);
+    for (int s = 0; s < NS; ++s) lg = P::mma(T::row_frag(B.k[u], n, h, s), qf[s], lg);
+    if (kt * TILE + TILE - 1 > qpos0) {   // keys past a query
+      const int thr = qpos0 + n - kt * TILE - 4 * h;
 #pragma unroll
-      for (int b = B0; b < B1; ++b) lg[b] = P::mma(kf, qf[b][s], lg[b]);
+      for (int i = 0; i < 16; ++i) lg[i] = crow(i, 0) <= thr ? lg[i] : -INFINITY;
     }
-    if constexpr (EDGE) {
+    u32x4 pf[2];
+    float psum;
+    auto weights = [&]() __attribute__((always_inline)) {
+      f32x16 p;
+      float s = 0.f;
 #pragma unroll
-      for (int b = B0; b < B1; ++b) {
-        const int thr = rq.c + rb[b] + n - kt * TILE - 4 * h;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) lg[b][i] = crow(i, 0) <= thr ? lg[b][i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) {
+        p[i] = fast_exp2(fmaf(lg[i], sl2, -mu));
+        s += p[i];
       }
-    }
-    // query tile after query tile: the first's value products run beneath the second's weights
-    u32x4 vf[DB][2];
+      psum = s;
+      pf[0] = P::pack(p, 0);
+      pf[1] = P::pack(p, 1);
+    };
+    weights();
+    if (__builtin_expect(__any(!(psum <= PAGED_FWD4_BIG)), 0)) {
+      float zmax = lg[0];
 #pragma unroll
-    for (int b = B0; b < B1; ++b) {
-      u32x4 pf[2];
-      float psum;
-      auto weights = [&]() __attribute__((always_inline)) {
-        f32x16 p;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          p[i] = fast_exp2(fmaf(lg[b][i], sl2, -mu[b]));
-          s += p[i];
-        }
-        psum = s;
-        pf[0] = P::pack(p, 0);
-        pf[1] = P::pack(p, 1);
-      };
-      weights();
-      if (__builtin_expect(__any(!(psum <= PAGED_FWD4_BIG)), 0)) {
-        float zmax = lg[b][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) zmax = fmaxf(zmax, lg[b][i]);
-        const Halves zh = halves(zmax);
-        const float m_new = fmaxf(mu[b], fmaxf(zh.lo, zh.hi) * sl2);
-        const float alpha = fast_exp2(mu[b] - m_new);
-        mu[b] = m_new;
-        l[b] *= alpha;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[b][db][i] *= alpha;
-        weights();
-      }
-      l[b] += psum;
+      for (int i = 1; i < 16; ++i) zmax = fmaxf(zmax, lg[i]);
+      const Halves zh = halves(zmax);
+      const float m_new = fmaxf(mu, fmaxf(zh.lo, zh.hi) * sl2);
+      const float alpha = fast_exp2(mu - m_new);
+      mu = m_new;
+      l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          if (b == B0) vf[db][s] = T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s);
-          o[b][db] = P::mma(vf[db][s], pf[s], o[b][db]);
-        }
+        for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+      weights();
     }
+    l += psum;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        o[db] = P::mma(T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s), pf[s], o[db]);
   };
 
   int cur = w.kt_hi - 1;   // the tile of the step; the t-th: t mod 2 names the buffers
+  int turn = (u - qt) & 3;   // tiles until the wavefront's next selection (0: the tile at hand)
   typename Rows::Place at1[1], at2[1];
   int pg[1];
   {
@@ -1149,51 +1124,44 @@ __global__ __launch_bounds__(512, 1) void paged_fwd4_kernel(PagedCall a, const f
     if (cur - 1 >= kt_lo) load_sel(sS1, at1);
     rows.pages_of(cur - 2 >= kt_lo ? cur - 2 : -1, pg);
   }
-  float entry = carry_of(cur - half);   // of the wavefront's next selection
+  float entry = carry_of(cur - turn);   // of the wavefront's next selection
   wait_loads();
   __syncthreads();
-  if (half == 0) {
-    if (cur < sel_end) select(cur, sS0, entry, sF0[u]);
-    entry = carry_of(cur - 2);
+  if (turn == 0) {
+    if (cur < end) select(cur, sS0, entry, sF0[qt]);
+    entry = carry_of(cur - 4);
   }
+  turn = (turn - 1) & 3;
   __asm__ volatile("" : "+v"(entry));   // (waited for here: in the loop the compiler would wait for the tiles' loads with it)
   __syncthreads();
 
-  constexpr std::integral_constant<int, 0> i0{};
-  constexpr std::integral_constant<int, 1> i1{};
-  constexpr std::integral_constant<int, 2> i2{};
   auto step = [&](auto odd_tag) __attribute__((always_inline)) {
-    constexpr int ODD = decltype(odd_tag)::value;
-    Tiles& B = ODD ? sB1 : sB0;
-    const float(*F)[TILE * LDF] = ODD ? sF1 : sF0;
+    constexpr bool ODD = decltype(odd_tag)::value;
     rows.places(cur - 2, pg, at2);
     if (cur - 1 >= kt_lo) load_tile(ODD ? sB0 : sB1, at1);
     if (cur - 2 >= kt_lo) load_sel(ODD ? sS1 : sS0, at2);
     rows.pages_of(cur - 3 >= kt_lo ? cur - 3 : -1, pg);
-    // both query tiles have rows (one without has no F), all of which see every key of the tile
-    if (end[1] > 0 && (cur + 1) * TILE <= rq.c + w.row0) {
-      attend(cur, B, F, i0, i2, std::false_type{});
-    } else {
-      if (cur < end[0]) attend(cur, B, F, i0, i1, std::true_type{});
-      if (cur < end[1]) attend(cur, B, F, i1, i2, std::true_type{});
+    if (turn == 0) {
+      // the next tile's F: first, and ahead of the SIMD's other wavefronts, which wait for it at the step's end
+      __builtin_amdgcn_s_setprio(1);
+      if (cur - 1 >= kt_lo && cur - 1 < end) select(cur - 1, ODD ? sS0 : sS1, entry, ODD ? sF0[qt] : sF1[qt]);
+      entry = carry_of(cur - 5);
     }
-    if (half == 1 - ODD) {   // the next tile's F
-      if (cur - 1 >= kt_lo && cur - 1 < sel_end) select(cur - 1, ODD ? sS0 : sS1, entry, ODD ? sF0[u] : sF1[u]);
-      entry = carry_of(cur - 3);
-    }
+    if (cur < end) attend(cur, ODD ? sB1 : sB0, ODD ? sF1[qt] : sF0[qt]);
+    __builtin_amdgcn_s_setprio(0);
+    turn = (turn - 1) & 3;
     at1[0] = at2[0];
     wait_loads();
     __syncthreads();
     --cur;
   };
   while (true) {
-    step(i0);
+    step(std::false_type{});
     if (cur < kt_lo) break;
-    step(i1);
+    step(std::true_type{});
     if (cur < kt_lo) break;
   }
-#pragma unroll
-  for (int b = 0; b < 2; ++b) paged_write<P, D>(a, w, rb[b] + n, hd0 + u, z, mu[b], l[b], o[b], h, part_ml, part_o);
+  paged_write<P, D>(a, w, rb + n, hd0 + u, z, mu, l, o, h, part_ml, part_o);
 }
 
 // The spans of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the spans that begin at
@@ -1540,7 +1508,7 @@ int paged_launch(const PagedLaunch& c) {
     if constexpr (sizeof(typename P::elem) == 2 && D == 64) {
       if (s.hg == 4) {
         const unsigned tiles = (unsigned)((a.N >> 7) + a.R);
-        hipLaunchKernelGGL((paged_fwd4_kernel<P>), dim3((unsigned)(a.H / 4 * s.splits), tiles), dim3(512), 0, c.st, a, carry, s.carry_ld,
+        hipLaunchKernelGGL((paged_fwd4_kernel<P>), dim3((unsigned)(a.H / 4 * s.splits), tiles), dim3(1024), 0, c.st, a, carry, s.carry_ld,
                            s.span_tiles, ml, o);
       }
     }
