@@ -371,46 +371,58 @@ SA_HIDDEN int paged_bf16(const PagedLaunch& c);   // sa_paged_bf16.hip
 SA_HIDDEN int paged_f16(const PagedLaunch& c);    // sa_paged_f16.hip
 SA_HIDDEN int paged_f32(const PagedLaunch& c);    // sa_paged_f32.hip
 
-// How a step over a paged cache is launched, and its workspace. One new token per request (step): chunks of keys
-// per workgroup, partial maxima, sums and outputs, then the new state rows. Several: the selectors' histories
-// (carry), and where the key range is split the spans' partials.
+// How a step over a paged cache is launched, and its workspace (byte offsets). Requests with one new token (ones): chunks of
+// keys per workgroup, their partial maxima, sums and outputs, then the new state rows. Requests with several: the selectors'
+// histories (carry), and where the key range is split into spans, their parts.
 struct PagedShape {
-  bool step;
-  int nw, hg;                 // several tokens: query tiles of 32 rows per workgroup, heads per wavefront (4: per workgroup, paged_fwd4)
+  bool ones, several;         // kernels that run
+  int64_t ld;                 // floats of a history row, or of a new state row
+  int chunk;                  // ones: keys per workgroup
+  int64_t step_m, step_l, step_o, step_state;
+  int nw, hg;                 // several: query tiles of 32 rows per workgroup, heads per wavefront (4: per workgroup, paged_fwd4)
   int splits, span_tiles;     // key spans, and their 32-key tiles
-  int chunk, carry_blocks;    // one token: keys per workgroup; several: workgroups along the keys of the histories
-  int64_t carry_ld;           // floats of a history row (one token: of a new state row)
-  int64_t carry, m, l, o, total;   // byte offsets (m: maxima, with several tokens (maximum, sum) pairs)
+  int carry_blocks;           // workgroups along the keys of the histories
+  int64_t carry, m, o;        // (m: (maximum, sum) pairs)
+  int64_t total;
 };
 inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_t D, int64_t es, int64_t max_new, int64_t max_len) {
   PagedShape s{};
   int64_t off = 0;
   auto take = [&](int64_t bytes) { int64_t o = off; off = align_up(off + bytes, 256); return o; };
-  s.step = max_new == 1;
-  s.carry_ld = align_up(max_len, TILE);
-  if (s.step) {
+  s.several = max_new > 1;
+  // At least `many` of the requests have several new tokens, if N rows are shared out with at most max_new each; the
+  // others may have one. A query tile for one row sweeps its keys at a fraction of HBM's rate, so where the others' keys can
+  // be many, requests with one token run the kernels that stream them (a mixed batch of 40 requests at up to 8000 positions, 36
+  // of them generating, 16 heads: 337 -> 215 us); where they cannot, two more launches that find nothing would cost 7 us.
+  const int64_t many = s.several ? std::min(cdiv(std::max<int64_t>(N - R, 0), max_new - 1), R) : 0;
+  s.ones = !s.several || (R - many) * max_len * H >= ((int64_t)1 << 20);
+  s.ld = align_up(max_len, TILE);
+  if (s.ones) {
     // as decode_chunk: workgroups enough to fill the chip, chunks long enough to stream
     int64_t chunk = 256;
     while (chunk < 4096 && R * H * cdiv(max_len, chunk) > 2048) chunk *= 2;
     s.chunk = (int)chunk;
-    s.splits = (int)cdiv(max_len, chunk);
-    s.m = take(R * H * s.splits * 4);
-    s.l = take(R * H * s.splits * 4);
-    s.o = take(R * H * s.splits * D * 4);
-    s.carry = take(R * G * s.carry_ld * 4);
-  } else {
+    const int64_t parts = R * H * cdiv(max_len, chunk);
+    s.step_m = take(parts * 4);
+    s.step_l = take(parts * 4);
+    s.step_o = take(parts * D * 4);
+    s.step_state = take(R * G * s.ld * 4);
+  }
+  if (s.several) {
     const int64_t per = H / G;
     s.nw = max_new <= TILE ? 1 : 4;
     s.hg = es == 2 && D == 64 && per % 4 == 0 && s.nw == 4 ? 4 : es == 2 && D <= 64 && per % 2 == 0 ? 2 : 1;
     const int64_t rows = (int64_t)s.nw * TILE;
     const int64_t tiles = cdiv(max_len, TILE);
-    const int64_t workgroups = std::max(cdiv(N, rows), std::min(R, N)) * (H / s.hg);   // (of live tiles)
+    // workgroups of live query tiles, about; the key range is split where they are no more than half of what the chip runs
+    // at once (one workgroup per CU, two, or eight of one wavefront)
+    const int64_t workgroups = (s.ones ? cdiv(N, rows) + many / 2 : std::max(cdiv(N, rows), std::min(R, N))) * (H / s.hg);
     const int64_t target = s.hg == 4 ? 256 : s.nw == 4 ? 512 : 2048;
-    const int64_t splits = std::max<int64_t>(1, std::min(cdiv(target, workgroups), cdiv(tiles, 16)));
+    const int64_t splits = std::max<int64_t>(1, std::min(target / workgroups, cdiv(tiles, 8)));
     s.span_tiles = (int)cdiv(tiles, splits);
     s.splits = (int)cdiv(tiles, s.span_tiles);
     s.carry_blocks = (int)std::max<int64_t>(1, std::min(cdiv(tiles, NWAVES), cdiv(8192, R * G)));
-    s.carry = take((N / TILE + R) * G * s.carry_ld * 4);
+    s.carry = take((N / TILE + R) * G * s.ld * 4);
     if (s.splits > 1) {
       s.m = take(s.splits * N * H * 8);
       s.o = take(s.splits * N * H * D * 4);
@@ -419,5 +431,4 @@ inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_
   s.total = off;
   return s;
 }
-
 }  // namespace sa_host

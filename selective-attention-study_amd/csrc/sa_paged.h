@@ -111,6 +111,7 @@ struct PagedCall {
   int64_t q_token, q_head, table_ld, state_ld;
   int R, N, H, G, pages, pshift;
   int max_new, max_len;
+  int ones;   // several tokens: requests with one new token are left to the single-token kernels
   float scale;
   int exempt;
 };
@@ -561,7 +562,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
   const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
   const int r = blockIdx.z, g = blockIdx.y;
   const PagedRequest rq = paged_request(a, r);
-  if (!rq.live) return;
+  if (!rq.live || (a.ones && rq.n == 1)) return;
   const int hd = g * (a.H / a.G);
   const int nkb = (rq.t + TILE - 1) / TILE, ntile = (rq.n + TILE - 1) / TILE;
   const elem* q = static_cast<const elem*>(a.q) + rq.first * a.q_token + hd * a.q_head;
@@ -649,8 +650,9 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
 }
 
 // ---------------------------------------------------------------------------------------------
-// The attention of a step of several tokens. Workgroup (x, y, z): query tiles of NW x 32 rows of one request
-// (numbered as above), heads y HG .. + HG - 1 (of one selector), key span z. As fwd64_kernel: a wavefront's 32
+// The attention of a step of several tokens. Workgroup (HG heads of one selector and a key span, NW x 32 query rows of one
+// request, numbered as above, the last first): workgroups next to each other, which the XCDs take in turns, are of different
+// heads and spans, so that an XCD's L2 holds few heads' keys. As fwd64_kernel: a wavefront's 32
 // queries against one 32-key tile at a time, newest first, every operand loaded straight into LDS one tile ahead,
 // the selection (-F, through the wavefront's LDS rows) one tile ahead of the softmax. What differs is where rows come
 // from: each lane looks its row's page up one tile before the load.
@@ -684,6 +686,7 @@ __device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, in
   w.rq = paged_request(a, w.r);
   w.row0 = (x - ((w.rq.first >> SH) + w.r)) << SH;
   if (w.row0 < 0 || w.row0 >= w.rq.n) return false;
+  if (a.ones && w.rq.n == 1 && w.rq.live) return false;   // (paged_step's)
   if (!w.rq.live) {
     if (zeros) clear(w.rq.first + w.row0, min(1 << SH, w.rq.n - w.row0));
     return false;
@@ -758,10 +761,10 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
 
   const int tid = threadIdx.x, lane = tid & 63, wave = NW == 1 ? 0 : wave_id();
   const int n = lane & 31, h = lane >> 5;
-  const int x = gridDim.x - 1 - blockIdx.x;
-  const int hd0 = blockIdx.y * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
+  const int groups = a.H / HG, x = gridDim.y - 1 - blockIdx.y, z = blockIdx.x / groups;
+  const int hd0 = (blockIdx.x % groups) * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
   PagedTiles w;
-  if (!paged_tiles<P, SH, HG * D, NW * 64>(a, x, blockIdx.z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
+  if (!paged_tiles<P, SH, HG * D, NW * 64>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
   const PagedRequest& rq = w.rq;
   const int r = w.r, row0 = w.row0, kt_lo = w.kt_lo, kt_hi = w.kt_hi;
 
@@ -942,7 +945,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   }
 
 #pragma unroll
-  for (int g = 0; g < HG; ++g) paged_write<P, D>(a, w, q_row, hd0 + g, blockIdx.z, m[g], l[g], o[g], h, part_ml, part_o);
+  for (int g = 0; g < HG; ++g) paged_write<P, D>(a, w, q_row, hd0 + g, z, m[g], l[g], o[g], h, part_ml, part_o);
 }
 
 // The same for groups of four heads or more at 16-bit head dim 64, the usual sizes of a long step: sixteen wavefronts, one
@@ -1174,6 +1177,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_join_kernel(PagedCall a, int s
   const int r = find_request<true>(a.starts, a.R, row, 0);
   const PagedRequest rq = paged_request(a, r);
   const bool live = rq.live && row >= rq.first && row < rq.first + rq.n;
+  if (live && a.ones && rq.n == 1) return;   // (paged_step_join's)
   const int spans = live ? (rq.c + row - rq.first) / TILE / span_tiles + 1 : 0;
   elem* out = static_cast<elem*>(a.out) + (int64_t)row * a.H * D;
   for (int i = threadIdx.x; i < a.H * (D / 4); i += NTHREADS) {
@@ -1230,7 +1234,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_step_kernel(PagedCall a, float
   const int cidx = blockIdx.x;
   const int r = blockIdx.z, hd = blockIdx.y;
   const PagedRequest rq = paged_request(a, r);
-  if (!rq.live || cidx * chunk >= rq.t) return;
+  if (!rq.live || rq.n != 1 || cidx * chunk >= rq.t) return;
   const int t = rq.t, per = a.H / a.G;
   const int64_t sg = (int64_t)r * a.G + hd / per;
   const bool selector = (hd % per) == 0;
@@ -1360,8 +1364,9 @@ __global__ __launch_bounds__(NTHREADS) void paged_step_kernel(PagedCall a, float
   }
 }
 
-// Blocks [0, rows * H): one row's head, its chunks' partials joined (rows of no request, or of one left out, become
-// zero). Blocks from there on: the new state rows, `sblocks` blocks of 1024 keys each.
+// Block (r, head) for the first R * H blocks: the request's chunks' partials joined; without `ones` (every row is here) also
+// zeros for the rows of requests left out, and for those behind the last request, each block every R-th of them. Blocks
+// from there on: the new state rows, `sblocks` blocks of 1024 keys each.
 template <class P, int D>
 __global__ __launch_bounds__(NTHREADS) void paged_step_join_kernel(PagedCall a, const float* __restrict__ pm,
                                                                    const float* __restrict__ pl, const float* __restrict__ po,
@@ -1370,13 +1375,13 @@ __global__ __launch_bounds__(NTHREADS) void paged_step_join_kernel(PagedCall a, 
   typedef typename P::elem elem;
   constexpr int QPP = D / 4, SLOTS = NTHREADS / QPP;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-  const int64_t out_blocks = (int64_t)a.N * a.H;
+  const int64_t out_blocks = (int64_t)a.R * a.H;
   if (blockIdx.x >= out_blocks) {
     const int64_t s = blockIdx.x - out_blocks;
     const int64_t sg = s / sblocks;
     const int j0 = (int)(s % sblocks) * (4 * NTHREADS);
     const PagedRequest rq = paged_request(a, (int)(sg / a.G));
-    if (!rq.live) return;
+    if (!rq.live || rq.n != 1) return;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int j = j0 + u * NTHREADS + tid;
@@ -1386,14 +1391,18 @@ __global__ __launch_bounds__(NTHREADS) void paged_step_join_kernel(PagedCall a, 
   }
   __shared__ float sRed[NWAVES][2];
   __shared__ float4 sO[NWAVES][QPP];
-  const int row = (int)(blockIdx.x / a.H), hd = (int)(blockIdx.x % a.H);
-  const int r = find_request<true>(a.starts, a.R, row, 0);
+  const int r = (int)(blockIdx.x / a.H), hd = (int)(blockIdx.x % a.H);
   const PagedRequest rq = paged_request(a, r);
-  elem* out = static_cast<elem*>(a.out) + ((int64_t)row * a.H + hd) * D;
-  if (!rq.live || rq.first != row) {
-    if (tid < D) out[tid] = P::to_elem(0.f);
-    return;
+  auto row_of = [&](int row) { return static_cast<elem*>(a.out) + ((int64_t)row * a.H + hd) * D; };
+  if (!a.ones) {
+    if (tid < D) {
+      for (int64_t row = max(a.starts[a.R], 0) + (int64_t)r; row < a.N; row += a.R) row_of((int)row)[tid] = P::to_elem(0.f);
+      if (!rq.live)
+        for (int i = 0; i < rq.n; ++i) row_of(rq.first + i)[tid] = P::to_elem(0.f);
+    }
   }
+  if (!rq.live || rq.n != 1) return;
+  elem* out = row_of(rq.first);
   const int nparts = (rq.t + chunk - 1) / chunk;
   const int64_t at = ((int64_t)r * a.H + hd) * nchunk;
   float mx = -INFINITY;
@@ -1473,34 +1482,39 @@ inline PagedCall paged_call(const PagedLaunch& c) {
 template <class P, int D, int HG, int NW, bool WHOLE>
 void launch_paged_fwd(const PagedCall& a, const PagedShape& s, const float* carry, float* ml, float* o, hipStream_t st) {
   const unsigned tiles = (unsigned)((a.N >> (NW == 4 ? 7 : 5)) + a.R);
-  hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE>), dim3(tiles, (unsigned)(a.H / HG), (unsigned)s.splits), dim3(NW * 64), 0, st,
-                     a, carry, s.carry_ld, s.span_tiles, ml, o);
+  hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE>), dim3((unsigned)(a.H / HG * s.splits), tiles), dim3(NW * 64), 0, st,
+                     a, carry, s.ld, s.span_tiles, ml, o);
+}
+
+template <class P, int D>
+void launch_paged_step(const PagedCall& a, const PagedShape& s, char* ws, hipStream_t st) {
+  auto at = [&](int64_t off) { return reinterpret_cast<float*>(ws + off); };
+  float *pm = at(s.step_m), *pl = at(s.step_l), *po = at(s.step_o), *next = at(s.step_state);
+  const int nchunk = (int)cdiv(a.max_len, s.chunk), sblocks = (int)cdiv(a.max_len, 4 * NTHREADS);
+  {
+    TimedLaunch timed(SA_KERNEL_DECODE, st);
+    hipLaunchKernelGGL((paged_step_kernel<P, D>), dim3((unsigned)nchunk, (unsigned)a.H, (unsigned)a.R), dim3(NTHREADS), 0, st, a, pm, pl,
+                       po, next, s.ld, s.chunk, nchunk);
+  }
+  const int64_t blocks = (int64_t)a.R * a.H + (int64_t)a.R * a.G * sblocks;
+  hipLaunchKernelGGL((paged_step_join_kernel<P, D>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, a, pm, pl, po, next, s.ld, s.chunk,
+                     nchunk, sblocks);
 }
 
 template <class P, int D>
 int paged_launch(const PagedLaunch& c) {
-  const PagedCall a = paged_call(c);
+  PagedCall a = paged_call(c);
   const PagedShape s = paged_shape(c.R, c.N, c.H, c.G, D, sizeof(typename P::elem), c.max_new, c.max_len);
   char* ws = static_cast<char*>(c.ws);
   auto at = [&](int64_t off) { return reinterpret_cast<float*>(ws + off); };
-  if (s.step) {
-    float *pm = at(s.m), *pl = at(s.l), *po = at(s.o), *next = at(s.carry);
-    {
-      TimedLaunch timed(SA_KERNEL_DECODE, c.st);
-      hipLaunchKernelGGL((paged_step_kernel<P, D>), dim3((unsigned)s.splits, (unsigned)a.H, (unsigned)a.R), dim3(NTHREADS), 0, c.st, a,
-                         pm, pl, po, next, s.carry_ld, s.chunk, s.splits);
-    }
-    const int sblocks = (int)cdiv(a.max_len, 4 * NTHREADS);
-    const int64_t blocks = (int64_t)a.N * a.H + (int64_t)a.R * a.G * sblocks;
-    hipLaunchKernelGGL((paged_step_join_kernel<P, D>), dim3((unsigned)blocks), dim3(NTHREADS), 0, c.st, a, pm, pl, po, next,
-                       s.carry_ld, s.chunk, s.splits, sblocks);
-    return launch_status();
-  }
+  a.ones = s.several && s.ones;
+  if (s.ones) launch_paged_step<P, D>(a, s, ws, c.st);
+  if (!s.several) return launch_status();
   float *carry = at(s.carry), *ml = s.splits > 1 ? at(s.m) : nullptr, *o = s.splits > 1 ? at(s.o) : nullptr;
   {
     TimedLaunch timed(SA_KERNEL_SELECTION, c.st);
     hipLaunchKernelGGL((paged_carry_kernel<P, D>), dim3((unsigned)s.carry_blocks, (unsigned)a.G, (unsigned)a.R), dim3(NTHREADS), 0, c.st,
-                       a, carry, s.carry_ld);
+                       a, carry, s.ld);
   }
   {
     TimedLaunch timed(SA_KERNEL_FORWARD, c.st);
@@ -1508,7 +1522,7 @@ int paged_launch(const PagedLaunch& c) {
     if constexpr (sizeof(typename P::elem) == 2 && D == 64) {
       if (s.hg == 4) {
         const unsigned tiles = (unsigned)((a.N >> 7) + a.R);
-        hipLaunchKernelGGL((paged_fwd4_kernel<P>), dim3((unsigned)(a.H / 4 * s.splits), tiles), dim3(1024), 0, c.st, a, carry, s.carry_ld,
+        hipLaunchKernelGGL((paged_fwd4_kernel<P>), dim3((unsigned)(a.H / 4 * s.splits), tiles), dim3(1024), 0, c.st, a, carry, s.ld,
                            s.span_tiles, ml, o);
       }
     }

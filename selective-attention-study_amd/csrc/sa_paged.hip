@@ -121,7 +121,7 @@ int sa_paged_append(const void* k, int64_t k_token, int64_t k_head, const void* 
 static bool paged_sizes_ok(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t max_new, int64_t max_len) {
   return batch_ok(requests, tokens) && heads >= 1 && heads < 65536 && groups >= 1 && heads % groups == 0 && max_new >= 1 &&
          max_new <= tokens && max_len >= 1 && max_len < MAX_LEN && tokens * heads < ((int64_t)1 << 30) &&
-         tokens * heads + requests * groups * cdiv(max_len, 4 * NTHREADS) < ((int64_t)1 << 31);
+         requests * heads + requests * groups * cdiv(max_len, 4 * NTHREADS) < ((int64_t)1 << 31);
 }
 
 int64_t sa_paged_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t head_dim,
