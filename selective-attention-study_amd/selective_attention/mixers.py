@@ -16,7 +16,8 @@ silent switch to the listing.
 Cached generation keeps, per sequence and selector, the selection every key has received so far: a
 prefill (single shot, or chunk by chunk with `prefill_chunk`) leaves it in the cache, and each
 decode step subtracts it from every head's logits and then adds the new query's own positive
-selector logits (keys past the exempt prefix, before the query).
+selector logits (keys past the exempt prefix, before the query). `step_paged` does both for a batch of requests of
+different lengths over pages (paged.py).
 """
 
 from __future__ import annotations
@@ -27,7 +28,7 @@ import math
 import torch
 from torch import Tensor
 
-from . import _lib, kernels
+from . import _lib, kernels, paged
 from .slot import AttentionSlot
 
 # name: (exempt, per_head)
@@ -145,6 +146,29 @@ class SelectiveAttention(AttentionSlot):
         else:
             y = self._chunk_listing(q1, keys, vals, cache["selected"], t - 1)
         return self.emit(y.to(x1.dtype))
+
+    # -- paged cache ----------------------------------------------------------------------------
+
+    def new_pages(self, requests: int, pages: int, page_size: int, capacity: int, device, dtype) -> dict:
+        """K and V pages in `dtype`, and the selection state of every request in fp32."""
+        shape = (pages, self.n_heads, page_size, self.head_dim)
+        return {"k": torch.zeros(shape, device=device, dtype=dtype), "v": torch.zeros(shape, device=device, dtype=dtype),
+                "selected": torch.zeros(requests, self.groups, capacity, device=device, dtype=torch.float32)}
+
+    def step_paged(self, x: Tensor, cache: dict, table: Tensor, plan: paged.PagePlan, max_new: int | None = None,
+                   max_len: int | None = None) -> Tensor:
+        """The new tokens of a batch of requests, (1, N, C), request after request (paged.page_plan): their keys and values
+        into the pages, then every request's queries over its own."""
+        q, k, v = (y[0].transpose(0, 1) for y in self.project(x))   # (N, H, D) views of the projection
+        q = q.to(cache["k"].dtype)
+        if self._on_kernels(q):
+            append, attend = paged.paged_append, paged.selective_attention_paged
+        else:
+            append, attend = paged.paged_append_reference, paged.selective_attention_paged_reference
+        append(k, v, cache["k"], cache["v"], plan.slots)
+        y = attend(q, cache["k"], cache["v"], table, plan.lengths, plan.starts, cache["selected"], exempt=self.exempt,
+                   max_new=max_new, max_len=max_len)
+        return self.emit(y.transpose(0, 1)[None].to(x.dtype))
 
     def _chunk_listing(self, q: Tensor, keys: Tensor, vals: Tensor, state: Tensor, c0: int) -> Tensor:
         """Queries at positions [c0, c0 + n) over the cached keys [0, c0 + n) with the carried

@@ -10,7 +10,8 @@ reference's (transformer.wte / h.N.ln_1 / attn.c_attn / ... / lm_head), so its s
 
 Generation keeps one cache per layer (slot.py): `prefill` runs the prompt in one pass, and
 `prefill_chunked` in chunks through all layers, each layer's slot carrying its keys, values and
-per-key selection state between chunks; `decode_step` then adds one token at a time.
+per-key selection state between chunks; `decode_step` then adds one token at a time. `new_paged_cache` and
+`paged_step` serve requests of different lengths together from one pool of pages (paged.py).
 
 Attention slots: the selective variants of `mixers.py` and "softmax" (causal SDPA, the reference's
 control slot).
@@ -25,7 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from . import mixers
+from . import mixers, paged
 from .slot import AttentionSlot
 
 
@@ -144,6 +145,10 @@ class Block(nn.Module):
     def step_cache(self, x1: Tensor, cache: dict) -> Tensor:
         return self._through(x1, self.attn.step_cache(self.ln_1(x1), cache))
 
+    def step_paged(self, x: Tensor, cache: dict, table: Tensor, plan: paged.PagePlan, max_new: int | None,
+                   max_len: int | None) -> Tensor:
+        return self._through(x, self.attn.step_paged(self.ln_1(x), cache, table, plan, max_new, max_len))
+
 
 class SelectiveLM(nn.Module):
     """Decoder-only LM. forward(idx, targets=None) -> (logits, loss): with targets, every position's
@@ -218,3 +223,35 @@ class SelectiveLM(nn.Module):
         for block, cache in zip(self.transformer.h, caches):
             x = block.step_cache(x, cache)
         return self._head(x)
+
+    def new_paged_cache(self, requests: int, pages: int, page_size: int = 64, capacity: int | None = None, device=None,
+                        dtype=None) -> dict:
+        """An empty paged cache: `requests` rows of up to `capacity` positions each (by default the context length) that
+        share `pages` pages of `page_size` positions per layer. Every tensor in it keeps its address from step to step."""
+        weight = self.lm_head.weight
+        device, dtype = device or weight.device, dtype or weight.dtype
+        width = -(-(capacity or self.config.context_length) // page_size)
+        ints = dict(device=device, dtype=torch.int32)
+        return {"layers": [block.attn.new_pages(requests, pages, page_size, width * page_size, device, dtype)
+                           for block in self.transformer.h],
+                "page_size": page_size, "table": torch.full((requests, width), -1, **ints),
+                "free": torch.arange(pages, **ints), "taken": torch.zeros(1, **ints), "cached": torch.zeros(requests, **ints)}
+
+    def paged_step(self, tokens: Tensor, new: Tensor, cache: dict, finished: Tensor | None = None, max_new: int | None = None,
+                   max_len: int | None = None) -> tuple[Tensor, paged.PagePlan]:
+        """One step of a batch of requests over a paged cache: `tokens` (N,), request after request, new[r] (int32) of them
+        request r's next ones (a prompt or a chunk of it, a generated token, none). finished (bool, optional): rows whose
+        request has ended and that start anew in this step. max_new, max_len: bounds known to the caller
+        (selective_attention_paged). Returns (R, vocab) logits after every request's last new token, and the step's plan: a
+        request whose plan.lengths is 0 was left out for want of pages, and rows without a new token in the step have
+        no meaningful logits."""
+        make = paged.page_plan if tokens.is_cuda else paged.page_plan_reference
+        plan = make(cache["cached"], new, cache["table"], cache["free"], cache["taken"], cache["page_size"], tokens.shape[0],
+                    finished)
+        cache["cached"].copy_(plan.cached)
+        cache["taken"].copy_(plan.taken)
+        x = self._embed(tokens[None])
+        for block, layer in zip(self.transformer.h, cache["layers"]):
+            x = block.step_paged(x, layer, cache["table"], plan, max_new, max_len)
+        last = (plan.starts[1:] - 1).clamp_min(0).long()
+        return self._head(x[0, last]), plan

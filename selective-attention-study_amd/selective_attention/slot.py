@@ -9,6 +9,8 @@ A cache is a dict (the reference's caches are dicts too, model.py:76-93):
     "len"        the number of cached positions
     "selected"   (B, G, capacity) fp32, selective slots only: the selection each cached key has
                  received from every cached query (G selectors per layer)
+
+A selective slot also serves a batch of requests of different lengths from pages (paged.py): `new_pages`, `step_paged`.
 """
 
 from __future__ import annotations
@@ -74,3 +76,9 @@ class AttentionSlot(nn.Module):
         cache = self.new_cache(b, max(t, self.context_length if capacity is None else capacity), k.device, k.dtype)
         self.cache_put(cache, k, v)
         return cache
+
+    # -- paged cache ----------------------------------------------------------------------------
+
+    def new_pages(self, requests: int, pages: int, page_size: int, capacity: int, device, dtype) -> dict:
+        """The layer's part of a paged cache of `requests` rows of up to `capacity` positions."""
+        raise NotImplementedError(f"{type(self).__name__} has no paged form; the selective slots do")

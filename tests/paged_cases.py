@@ -143,3 +143,32 @@ class Server:
         assert isinstance(made, paged.PagePlan)
         self.cached, self.taken = made.cached, made.taken
         return made
+
+
+def serve(model, device, dtype, rtol, atol):
+    """A server's run through a decoder: two prompts, one of them in chunks, a request that comes later, one that ends and
+    whose row another takes; every request's logits against its own prefill and decode steps."""
+    g = torch.Generator().manual_seed(1)
+    vocab = model.config.vocab_size
+    cache = model.new_paged_cache(3, 14, 16, capacity=64, dtype=dtype)
+    seen = [[], [], []]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    with torch.no_grad():
+        for new, ended, max_new in (([17, 5, 0], None, None), ([1, 9, 0], None, 9), ([1, 1, 30], None, None), ([1, 1, 1], None, 1),
+                                    ([1, 20, 1], [False, True, False], 20), ([1, 1, 1], None, 1)):
+            ids = torch.randint(0, vocab, (sum(new),), generator=g)
+            for r, part in enumerate(ids.split(new)):
+                if ended and ended[r]:
+                    seen[r] = []
+                seen[r].append(part)
+            logits, plan = model.paged_step(ids.to(device), ints(new), cache, None if ended is None else torch.tensor(ended, device=device),
+                                            max_new=max_new)
+            assert plan.lengths.tolist() == [sum(len(x) for x in row) for row in seen]
+            for r, row in enumerate(seen):
+                if new[r]:
+                    ids = torch.cat(row)[None].to(device)
+                    want = model.prefill(ids[:, :-1], capacity=64)[1] if ids.shape[1] > 1 else None
+                    want = model.prefill(ids)[0] if want is None else model.decode_step(ids[:, -1:], 0, want)
+                    torch.testing.assert_close(logits[r], want[0, 0].to(logits.dtype), rtol=rtol, atol=atol)
+    held = [pages_of(int(n), 16) for n in cache["cached"].tolist()]
+    assert int(cache["taken"]) == sum(held)

@@ -6,8 +6,9 @@ import torch
 
 import selective_attention as sa
 from oracle import sa_oracle
-from paged_cases import Server, Step, check, pages_of
+from paged_cases import Server, Step, check, pages_of, serve
 from selective_attention import _lib, paged
+from selective_attention.model import ModelConfig, SelectiveLM
 
 
 @pytest.mark.parametrize("groups,exempt,page_size", [(1, 1, 16), (2, 3, 8), (4, 16, 32)])
@@ -122,3 +123,18 @@ def test_abi_refuses_before_any_launch():
         assert lib.sa_paged_attention(*attend[:i], value, *attend[i + 1:]) == code, i
     assert lib.sa_paged_attention_workspace_bytes(4, 10, 4, 3, 64, 5, 128, 0) == -1
     assert lib.sa_paged_attention_workspace_bytes(4, 10, 4, 1, 64, 5, 128, 0) > 0
+
+
+@pytest.mark.parametrize("attention", ["selective", "selective_x16", "selective_perhead"])
+def test_model_serves_requests_of_different_lengths(attention):
+    """paged_step's logits after every step are those of each request alone in prefill and decode_step."""
+    torch.manual_seed(0)
+    cfg = ModelConfig(vocab_size=97, n_layers=2, d_model=64, n_heads=4, context_length=64, attention=attention)
+    model = SelectiveLM(cfg).double().eval()
+    serve(model, "cpu", torch.float64, rtol=1e-4, atol=1e-5)   # (the state between steps is fp32)
+
+
+def test_the_softmax_slot_has_no_pages():
+    cfg = ModelConfig(vocab_size=97, n_layers=1, d_model=64, n_heads=4, context_length=64, attention="softmax")
+    with pytest.raises(NotImplementedError, match="paged"):
+        SelectiveLM(cfg).new_paged_cache(2, 4, 16)

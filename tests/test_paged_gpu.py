@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import selective_attention as sa
-from paged_cases import Server, Step, check
+from paged_cases import Server, Step, check, serve
+from selective_attention.model import ModelConfig, SelectiveLM
 
 pytestmark = pytest.mark.gpu
 
@@ -346,3 +347,33 @@ def test_refusals_on_the_gpu(cuda):
         sa.paged_append(args[0], args[0], args[1], args[2], torch.zeros(1, dtype=torch.int32, device=cuda))
     with pytest.raises(ValueError):
         sa.page_plan(args[4], args[4].long(), args[3], args[4], args[4], 16, 1)
+
+
+@pytest.mark.parametrize("attention", ["selective", "selective_x16", "selective_perhead"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_model_serves_requests_of_different_lengths(cuda, attention, dtype):
+    """paged_step against each request alone through prefill and decode_step. fp32: both within fp32 rounding through two
+    layers. bf16: two paths of two layers, whose activations (norm about 1, logits about 0.2) are each rounded to 2^-8 some
+    ten times on the way: 10 * 2^-8 of a logit's size of 1 at most."""
+    torch.manual_seed(0)
+    cfg = ModelConfig(vocab_size=211, n_layers=2, d_model=128, n_heads=4, context_length=64, attention=attention)
+    model = SelectiveLM(cfg).to(cuda, dtype).eval()
+    serve(model, cuda, dtype, rtol=0, atol=1e-4 if dtype == torch.float32 else 4e-2)
+
+
+def test_a_mixed_step_with_many_single_tokens(cuda):
+    """Requests with one new token take the single-token kernels, those with several the others, in one call."""
+    rng = random.Random(2)
+    cached = [rng.randrange(300) for _ in range(40)]
+    new = [1 if r % 10 else 37 for r in range(40)]
+    step = Step(cached, new, heads=4, width=400, pad=3)   # (the bound on positions decides: 6000 of them)
+    out, state = attend(step, cuda)
+    check(out, state, step, ROUNDED[torch.bfloat16])
+    assert (out[-3:] == 0).all()
+    step = Step([c + 40 for c in cached], [1] * 40, heads=4, width=400, pad=1)
+    out, state = attend(step, cuda)   # (no bound given: every request turns out to have one)
+    check(out, state, step)
+    args = step.args(cuda)
+    args[4][3], args[4][7] = 0, 10**7   # left out
+    out = sa.selective_attention_paged(*args)
+    assert (out[[3, 7, 40]] == 0).all() and (out[[2, 4, 6, 8, 39]].abs().sum(-1) > 0).all()
