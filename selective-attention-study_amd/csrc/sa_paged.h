@@ -138,11 +138,12 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedCall& a, int r)
 static __device__ uint4 paged_zero_row;   // what rows without a page read
 
 // ---------------------------------------------------------------------------------------------
-// The step's tables. One workgroup (a step's scans run over the requests, some hundreds); bound by its latency:
-// two block scans and one round trip each for the lengths, the stack and the table.
+// The step's tables. One workgroup (a step's scans run over the requests, some hundreds); bound by its latency: two block
+// scans and one round trip each for the lengths, the stack and the table. A step of 8 requests takes 5 us on the GPU.
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_WAVES = PLAN_THREADS / 64;
 constexpr int PLAN_SLOTS = 4096;   // tokens up to which the same workgroup makes the slot map
+constexpr int PLAN_BATCH = 8;      // loads of a table row under way at a time
 
 struct PlanCall {
   const int *cached, *fresh;
@@ -157,42 +158,32 @@ struct PlanCall {
   bool slots_here;   // the slot map too; else page_slots_kernel makes it
 };
 
-__device__ __forceinline__ int wave_scan_incl(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
-
-// Inclusive sums over the workgroup's threads of two values, and their totals. Saturated inputs (each at most 2^30
-// over 1024 threads) would overflow 32 bits: the callers clamp what they add.
+// Inclusive sums over the workgroup's threads, in request order, and their totals: 32 bits within a wavefront (the callers'
+// values are at most 2^24 each), 64 across.
 struct Sum2 {
   int64_t a, b, ta, tb;
 };
-__device__ __forceinline__ int64_t wave_scan_incl64(int64_t x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_add(int x) { return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xF, false); }
+__device__ __forceinline__ int wave_scan_incl(int x) {
+  x = dpp_add<0x111, 0xF>(x);   // row_shr:1, 2, 4, 8: within rows of 16 lanes
+  x = dpp_add<0x112, 0xF>(x);
+  x = dpp_add<0x114, 0xF>(x);
+  x = dpp_add<0x118, 0xF>(x);
+  x = dpp_add<0x142, 0xA>(x);   // row_bcast:15 into rows 1 and 3
+  return dpp_add<0x143, 0xC>(x);   // row_bcast:31 into rows 2 and 3
 }
-__device__ __forceinline__ Sum2 block_scan2(int64_t a, int64_t b, int64_t (*sh)[2]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  a = wave_scan_incl64(a);
-  b = wave_scan_incl64(b);
+__device__ __forceinline__ Sum2 block_scan2(int a, int b, int (*sh)[2]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  a = wave_scan_incl(a);
+  b = wave_scan_incl(b);
   if (lane == 63) {
     sh[wave][0] = a;
     sh[wave][1] = b;
   }
   __syncthreads();
   Sum2 s{a, b, 0, 0};
-#pragma unroll
-  for (int w = 0; w < PLAN_WAVES; ++w) {
+  for (int w = 0; w < waves; ++w) {
     if (w < wave) {
       s.a += sh[w][0];
       s.b += sh[w][1];
@@ -204,37 +195,62 @@ __device__ __forceinline__ Sum2 block_scan2(int64_t a, int64_t b, int64_t (*sh)[
   return s;
 }
 
+// n integers by a wavefront, PLAN_BATCH loads under way
+__device__ __forceinline__ void wave_copy(int* to, const int* from, int n) {
+  for (int i0 = threadIdx.x & 63; i0 < n; i0 += 64 * PLAN_BATCH) {
+    int x[PLAN_BATCH];
+#pragma unroll
+    for (int u = 0; u < PLAN_BATCH; ++u) x[u] = i0 + 64 * u < n ? from[i0 + 64 * u] : 0;
+#pragma unroll
+    for (int u = 0; u < PLAN_BATCH; ++u)
+      if (i0 + 64 * u < n) to[i0 + 64 * u] = x[u];
+  }
+}
+
+// Requests whose pages a whole wavefront moves, shared out over the workgroup's wavefronts: they come in any order and often
+// next to each other (a batch's prompts behind its generating requests: 31 us at 51 of 512 requests, each wavefront its own;
+// 11 shared out).
+struct PlanJob {
+  int r, n, c, need;   // (a finished request: need = its pages)
+  int64_t from, first;   // entry of the stack, token row; c < 0: left out
+};
+
 __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanCall a) {
-  __shared__ int64_t sh[PLAN_WAVES][2];
-  const int tid = threadIdx.x, lane = tid & 63;
+  __shared__ int sh[PLAN_WAVES][2];
+  __shared__ int64_t sMost[PLAN_WAVES];
+  __shared__ PlanJob sJobs[PLAN_THREADS];
+  __shared__ int sCount;
+  const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
   const int P = 1 << a.pshift;
   const auto pages_of = [&](int64_t x) { return (int)((x + P - 1) >> a.pshift); };
   int64_t base = min(max(a.taken[0], 0), a.F);   // first free entry of the stack
+  // the strip's jobs, each by one wavefront (`mine`: this thread's request is one); between barriers of their own
+  auto share_out = [&](bool mine, const PlanJob& job, auto work) {
+    if (tid == 0) sCount = 0;
+    __syncthreads();
+    const uint64_t all = __ballot(mine);
+    int at = 0;
+    if (lane == 0 && all) at = atomicAdd(&sCount, __popcll(all));
+    at = __shfl(at, 0);
+    if (mine) sJobs[at + __popcll(all & ((1ull << lane) - 1))] = job;
+    __syncthreads();
+    for (int i = tid >> 6; i < sCount; i += threads >> 6) work(sJobs[i]);
+    __syncthreads();
+  };
 
   // finished requests' pages go back, request after request
   if (a.finished) {
+    auto back_of = [&](int r) { return r < a.R && a.finished[r] ? min(min(pages_of(max(a.cached[r], 0)), a.W), 1 << 24) : 0; };
     int64_t total = 0;
-    for (int r0 = 0; r0 < a.R; r0 += PLAN_THREADS) {
-      const int r = r0 + tid;
-      const int back = r < a.R && a.finished[r] ? min(pages_of(max(a.cached[r], 0)), a.W) : 0;
-      total += block_scan2(back, 0, sh).ta;
-    }
+    for (int r0 = 0; r0 < a.R; r0 += threads) total += block_scan2(back_of(r0 + tid), 0, sh).ta;
     int64_t at = base - total;
     base = max(at, (int64_t)0);
-    for (int r0 = 0; r0 < a.R; r0 += PLAN_THREADS) {
-      const int r = r0 + tid;
-      const int back = r < a.R && a.finished[r] ? min(pages_of(max(a.cached[r], 0)), a.W) : 0;
+    for (int r0 = 0; r0 < a.R; r0 += threads) {
+      const int r = r0 + tid, back = back_of(r);
       const Sum2 s = block_scan2(back, 0, sh);
       const int64_t to = at + s.a - back;
-      uint64_t todo = __ballot(back > 0);
-      while (todo) {   // a wavefront copies its requests' table rows one after another
-        const int l = __ffsll((unsigned long long)todo) - 1;
-        todo &= todo - 1;
-        const int rr = __shfl(r, l), nn = __shfl(back, l);
-        const int64_t tt = __shfl(to, l);
-        for (int i = lane; i < nn; i += 64)
-          if (tt + i >= 0) a.stack[tt + i] = a.table[rr * a.table_ld + i];
-      }
+      share_out(back > 0 && to >= 0, PlanJob{r, 0, 0, back, to, 0},
+                [&](const PlanJob& j) { wave_copy(a.stack + j.from, a.table + j.r * a.table_ld, j.need); });
       at += s.ta;
     }
     __threadfence_block();
@@ -245,20 +261,20 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanCall a) {
   int64_t row = 0, given = 0;   // rows and needs of the requests before this strip
   int64_t most = 0;             // needs up to the last request served
   const int64_t avail = a.F - base;
-  for (int r0 = 0; r0 < a.R; r0 += PLAN_THREADS) {
+  for (int r0 = 0; r0 < a.R; r0 += threads) {
     const int r = r0 + tid;
     int c = 0, n = 0;
     if (r < a.R) {
       c = a.finished && a.finished[r] ? 0 : max(a.cached[r], 0);
-      n = max(a.fresh[r], 0);
+      n = min(max(a.fresh[r], 0), a.N + 1);   // (one row more than there are is as many as any more)
     }
     const int64_t t = (int64_t)c + n;
     const int have = pages_of(c);
-    const bool fits = t <= ((int64_t)a.W << a.pshift);
+    const bool fits = r < a.R && t <= ((int64_t)a.W << a.pshift);
     const int need = fits ? pages_of(t) - have : 0;
     const Sum2 s = block_scan2(n, need, sh);
     const int64_t first = row + s.a - n, end = row + s.a, upto = given + s.b;
-    const bool served = r < a.R && fits && end <= a.N && (need == 0 || upto <= avail);
+    const bool served = fits && end <= a.N && (need == 0 || upto <= avail);
     const int64_t from = base + upto - need;   // the request's first entry of the stack
     if (served && need) most = max(most, upto);
     if (r < a.R) {
@@ -269,7 +285,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanCall a) {
     }
     int* trow = a.table + (int64_t)r * a.table_ld;
     // the page of the first new token: the last one held, unless that is full
-    const bool one = served && need <= 1 && n <= 1;
+    const bool one = served && n <= 1;
     if (one && n == 1) {
       int page;
       if (need) {
@@ -280,35 +296,30 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanCall a) {
       }
       if (a.slots_here) a.slots[first] = ((int64_t)page << a.pshift) + (c & (P - 1));
     }
-    uint64_t todo = __ballot(r < a.R && n > 0 && !one);
-    while (todo) {   // the others: a wavefront's lanes together, request after request
-      const int l = __ffsll((unsigned long long)todo) - 1;
-      todo &= todo - 1;
-      const int rr = r0 + (tid & ~63) + l, nn = __shfl(n, l), cc = __shfl(c, l), hv = __shfl(have, l), nd = __shfl(need, l);
-      const bool ok = __shfl((int)served, l) != 0;
-      const int64_t fr = __shfl(from, l), ro = __shfl(first, l);
-      int* tr = a.table + (int64_t)rr * a.table_ld;
-      if (ok)
-        for (int i = lane; i < nd; i += 64) tr[hv + i] = a.stack[fr + i];
+    share_out(r < a.R && n > 0 && !one, PlanJob{r, n, served ? c : -1, need, from, first}, [&](const PlanJob& j) {
+      int* tr = a.table + j.r * a.table_ld;
+      const bool ok = j.c >= 0;
+      const int hv = ok ? pages_of(j.c) : 0;
+      if (ok) wave_copy(tr + hv, a.stack + j.from, j.need);
       if (a.slots_here)
-        for (int i = lane; i < nn && ro + i < a.N; i += 64) {
-          const int pos = cc + i, p = pos >> a.pshift;
-          const int page = !ok ? -1 : p < hv ? tr[p] : a.stack[fr + p - hv];
-          a.slots[ro + i] = ok ? ((int64_t)page << a.pshift) + (pos & (P - 1)) : -1;
+        for (int i = lane; i < j.n && j.first + i < a.N; i += 64) {
+          const int pos = j.c + i, p = pos >> a.pshift;
+          const int page = !ok ? -1 : p < hv ? tr[p] : a.stack[j.from + p - hv];
+          a.slots[j.first + i] = ok ? ((int64_t)page << a.pshift) + (pos & (P - 1)) : -1;
         }
-    }
+    });
     row += s.ta;
     given += s.tb;
   }
   if (a.slots_here)
-    for (int64_t i = row + tid; i < a.N; i += PLAN_THREADS) a.slots[i] = -1;   // rows behind the last request
+    for (int64_t i = row + tid; i < a.N; i += threads) a.slots[i] = -1;   // rows behind the last request
   // the last served request's needs: the largest over the threads
+#pragma unroll
   for (int o = 32; o > 0; o >>= 1) most = max(most, (int64_t)__shfl_xor(most, o));
-  __syncthreads();
-  if (lane == 0) sh[tid >> 6][0] = most;
+  if (lane == 0) sMost[tid >> 6] = most;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < PLAN_WAVES; ++w) most = max(most, sh[w][0]);
+    for (int w = 1; w < threads >> 6; ++w) most = max(most, sMost[w]);
     a.taken_out[0] = (int)(base + most);
   }
 }

@@ -77,7 +77,8 @@ int sa_page_plan(const int32_t* cached, const int32_t* new_tokens, const uint8_t
   c.N = (int)tokens;
   c.pshift = sh;
   c.slots_here = tokens <= PLAN_SLOTS;
-  hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, st, c);
+  const int threads = (int)std::min<int64_t>(std::max<int64_t>(align_up(requests, 64), 256), PLAN_THREADS);
+  hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3((unsigned)threads), 0, st, c);
   if (!c.slots_here)
     hipLaunchKernelGGL(page_slots_kernel, dim3((unsigned)cdiv(tokens, NTHREADS)), dim3(NTHREADS), 0, st, starts, lengths, table,
                        table_ld, slots, (int)requests, (int)width, (int)tokens, sh);

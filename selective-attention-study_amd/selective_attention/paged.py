@@ -45,37 +45,45 @@ class PagePlan(NamedTuple):
 
 # -- checks ---------------------------------------------------------------------------------------------
 
+# (A step's host work is of the size of its kernels' for small batches, so the checks read each attribute once.)
+
 def _check_page_size(page_size: int) -> int:
     if int(page_size) != page_size or not 8 <= page_size <= 1 << 20 or page_size & (page_size - 1):
         raise ValueError(f"page_size must be a power of two from 8 to 2^20; got {page_size}")
     return int(page_size)
 
 
-def _check_ints(name: str, t: Tensor, shape: tuple, device: torch.device, dtype=torch.int32) -> None:
-    if t.dtype != dtype or t.device != device or t.dim() != len(shape) or any(
-            want is not None and have != want for have, want in zip(t.shape, shape)) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape "
-                         f"{tuple('*' if n is None else n for n in shape)} on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _check_ints(name: str, t: Tensor, size: int | None, device: torch.device, dtype=torch.int32) -> None:
+    """A contiguous vector of `size` (None: any) integers."""
+    shape = t.shape
+    if t.dtype is not dtype or t.device != device or len(shape) != 1 or (size is not None and shape[0] != size) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {'any number of' if size is None else size} elements on "
+                         f"{device}; got {t.dtype} {tuple(shape)} on {t.device}")
 
 
-def _check_table(table: Tensor, requests: int, device: torch.device) -> None:
-    if (table.dtype != torch.int32 or table.device != device or table.dim() != 2 or table.shape[0] != requests
-            or table.shape[1] < 1 or table.stride(1) != 1 or table.stride(0) < table.shape[1]):
-        raise ValueError(f"table must be a ({requests}, W) int32 tensor with unit column stride on {device}; got "
-                         f"{table.dtype} {tuple(table.shape)} on {table.device}")
+def _check_table(table: Tensor, requests: int, device: torch.device) -> tuple[int, int]:
+    """(row stride, width) of a block table."""
+    shape = table.shape
+    if table.dtype is torch.int32 and table.device == device and len(shape) == 2 and shape[0] == requests and shape[1] >= 1:
+        ld, unit = table.stride()
+        if unit == 1 and ld >= shape[1]:
+            return ld, shape[1]
+    raise ValueError(f"table must be a ({requests}, W) int32 tensor with unit column stride on {device}; got "
+                     f"{table.dtype} {tuple(shape)} on {table.device}")
 
 
-def _check_pages(k_pages: Tensor, v_pages: Tensor) -> int:
-    """The page size of a cache; ValueError unless the kernels can use it."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[0] < 1 or k_pages.shape[1] < 1:
-        raise ValueError(f"k_pages and v_pages must both be (pages, H, P, D); got {tuple(k_pages.shape)}, {tuple(v_pages.shape)}")
-    if k_pages.dtype not in DTYPES or v_pages.dtype != k_pages.dtype:
-        raise ValueError(f"the cache's dtype must be float16, bfloat16 or float32, one for both; got {k_pages.dtype}, {v_pages.dtype}")
-    if k_pages.shape[3] not in HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {HEAD_DIMS}; got {k_pages.shape[3]}")
-    if v_pages.device != k_pages.device or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+def _check_pages(k_pages: Tensor, v_pages: Tensor) -> tuple[int, int, int, int, torch.dtype, torch.device]:
+    """(pages, heads, page size, head dim, dtype, device) of a cache; ValueError unless the kernels can use it."""
+    shape, dtype, device = k_pages.shape, k_pages.dtype, k_pages.device
+    if len(shape) != 4 or shape != v_pages.shape or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"k_pages and v_pages must both be (pages, H, P, D); got {tuple(shape)}, {tuple(v_pages.shape)}")
+    if dtype not in DTYPES or v_pages.dtype is not dtype:
+        raise ValueError(f"the cache's dtype must be float16, bfloat16 or float32, one for both; got {dtype}, {v_pages.dtype}")
+    if shape[3] not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS}; got {shape[3]}")
+    if v_pages.device != device or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("k_pages and v_pages must be contiguous, on one device")
-    return _check_page_size(k_pages.shape[2])
+    return shape[0], shape[1], _check_page_size(shape[2]), shape[3], dtype, device
 
 
 def _check_cuda(t: Tensor) -> None:
@@ -124,26 +132,24 @@ def page_plan(cached: Tensor, new: Tensor, table: Tensor, free: Tensor, taken: T
     if cached.dim() != 1 or not 1 <= cached.shape[0] < 65536:
         raise ValueError(f"cached must be one length per request, 1 to 65535 of them; got {tuple(cached.shape)}")
     requests = cached.shape[0]
-    _check_ints("cached", cached, (requests,), device)
-    _check_ints("new", new, (requests,), device)
-    _check_table(table, requests, device)
-    _check_ints("free", free, (None,), device)
-    _check_ints("taken", taken, (1,), device)
+    _check_ints("cached", cached, requests, device)
+    _check_ints("new", new, requests, device)
+    ld, width = _check_table(table, requests, device)
+    _check_ints("free", free, None, device)
+    _check_ints("taken", taken, 1, device)
     page_size = _check_page_size(page_size)
     if int(tokens) != tokens or not 0 <= tokens < 1 << 24:
         raise ValueError(f"tokens must be an integer from 0 to 2^24 - 1; got {tokens}")
-    if table.shape[1] * page_size > 1 << 30:
+    if width * page_size > 1 << 30:
         raise ValueError("a table row may hold up to 2^30 positions")
     if finished is not None:
-        _check_ints("finished", finished, (requests,), device, torch.bool)
+        _check_ints("finished", finished, requests, device, torch.bool)
     lib = _lib.load()
-    out = torch.empty(3 * requests + 2, device=device, dtype=torch.int32)
+    starts, lengths, after, now_taken = (torch.empty(n, device=device, dtype=torch.int32) for n in (requests + 1, requests, requests, 1))
     slots = torch.empty(int(tokens), device=device, dtype=torch.int64)
-    starts, lengths, after, now_taken = out.split((requests + 1, requests, requests, 1))
     _call(device, lib.sa_page_plan, cached.data_ptr(), new.data_ptr(), None if finished is None else finished.data_ptr(),
-          table.data_ptr(), table.stride(0), free.data_ptr(), taken.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
-          after.data_ptr(), slots.data_ptr(), now_taken.data_ptr(), requests, table.shape[1], free.shape[0], int(tokens),
-          page_size)
+          table.data_ptr(), ld, free.data_ptr(), taken.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
+          after.data_ptr(), slots.data_ptr(), now_taken.data_ptr(), requests, width, free.shape[0], int(tokens), page_size)
     return PagePlan(starts, lengths, after, slots, now_taken)
 
 
@@ -154,60 +160,62 @@ def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots: 
     to the cache's own."""
 
     _check_cuda(k_pages)
-    page_size = _check_pages(k_pages, v_pages)
-    pages, heads, _, head_dim = k_pages.shape
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (heads, head_dim):
-        raise ValueError(f"k and v must both be (N, {heads}, {head_dim}); got {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.dtype not in DTYPES or v.dtype != k.dtype:
-        raise ValueError(f"dtype must be float16, bfloat16 or float32, one for both; got {k.dtype}, {v.dtype}")
-    if k.device != k_pages.device or v.device != k_pages.device:
+    pages, heads, page_size, head_dim, dtype, device = _check_pages(k_pages, v_pages)
+    shape, source = k.shape, k.dtype
+    if len(shape) != 3 or shape != v.shape or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"k and v must both be (N, {heads}, {head_dim}); got {tuple(shape)}, {tuple(v.shape)}")
+    if source not in DTYPES or v.dtype is not source:
+        raise ValueError(f"dtype must be float16, bfloat16 or float32, one for both; got {source}, {v.dtype}")
+    if k.device != device or v.device != device:
         raise ValueError("k, v and the cache must be on one device")
-    _check_ints("slots", slots, (k.shape[0],), k_pages.device, torch.int64)
-    if k.shape[0] >= 1 << 24:
-        raise ValueError(f"a step holds up to 2^24 - 1 tokens; got {k.shape[0]}")
-    if k.shape[0] == 0:
+    tokens = shape[0]
+    _check_ints("slots", slots, tokens, device, torch.int64)
+    if tokens >= 1 << 24:
+        raise ValueError(f"a step holds up to 2^24 - 1 tokens; got {tokens}")
+    if tokens == 0:
         return
     lib = _lib.load()
     k, v = _rows(k), _rows(v)
-    _call(k.device, lib.sa_paged_append, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-          k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), k.shape[0], heads, head_dim, pages, page_size,
-          _CODES[k.dtype], _CODES[k_pages.dtype])
+    _call(device, lib.sa_paged_append, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+          k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), tokens, heads, head_dim, pages, page_size,
+          _CODES[source], _CODES[dtype])
 
 
 def _check_step(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, starts: Tensor, selected: Tensor,
-                exempt: int, max_new: int | None, max_len: int | None) -> tuple[int, int, int, int]:
-    """(page size, exempt, max_new, max_len) of a step over a paged cache."""
-    page_size = _check_pages(k_pages, v_pages)
-    _, heads, _, head_dim = k_pages.shape
-    device = k_pages.device
-    if q.dim() != 3 or q.shape[1:] != (heads, head_dim) or q.dtype != k_pages.dtype or q.device != device:
-        raise ValueError(f"q must be (N, {heads}, {head_dim}) in the cache's dtype {k_pages.dtype}, on its device; got "
-                         f"{tuple(q.shape)} {q.dtype} on {q.device}")
-    if q.shape[0] >= 1 << 24 or q.shape[0] * heads >= 1 << 30:
-        raise ValueError(f"a step holds up to 2^24 - 1 tokens and 2^30 - 1 head rows; got {tuple(q.shape)}")
+                exempt: int, max_new: int | None, max_len: int | None) -> tuple:
+    """The sizes of a step over a paged cache, as selective_attention_paged passes them on."""
+    pages, heads, page_size, head_dim, dtype, device = _check_pages(k_pages, v_pages)
+    shape = q.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or q.dtype is not dtype or q.device != device:
+        raise ValueError(f"q must be (N, {heads}, {head_dim}) in the cache's dtype {dtype}, on its device; got "
+                         f"{tuple(shape)} {q.dtype} on {q.device}")
+    tokens = shape[0]
+    if tokens >= 1 << 24 or tokens * heads >= 1 << 30:
+        raise ValueError(f"a step holds up to 2^24 - 1 tokens and 2^30 - 1 head rows; got {tuple(shape)}")
     if lengths.dim() != 1 or not 1 <= lengths.shape[0] < 65536:
         raise ValueError(f"lengths must be one per request, 1 to 65535 of them; got {tuple(lengths.shape)}")
     requests = lengths.shape[0]
-    _check_ints("lengths", lengths, (requests,), device)
-    _check_ints("starts", starts, (requests + 1,), device)
-    _check_table(table, requests, device)
-    if (selected.dim() != 3 or selected.shape[0] != requests or selected.shape[1] < 1 or heads % selected.shape[1] != 0
-            or selected.dtype != torch.float32 or selected.device != device or selected.stride(2) != 1
-            or selected.stride(0) != selected.shape[1] * selected.stride(1) or selected.stride(1) < selected.shape[2]):
+    _check_ints("lengths", lengths, requests, device)
+    _check_ints("starts", starts, requests + 1, device)
+    ld, width = _check_table(table, requests, device)
+    state, strides = selected.shape, selected.stride()
+    if (len(state) != 3 or state[0] != requests or state[1] < 1 or heads % state[1] != 0 or selected.dtype is not torch.float32
+            or selected.device != device or strides[2] != 1 or strides[0] != state[1] * strides[1] or strides[1] < state[2]):
         raise ValueError(f"selected must be a ({requests}, G, L) fp32 tensor with G dividing H, rows a fixed stride apart, "
-                         f"on q's device; got {selected.dtype} {tuple(selected.shape)} on {selected.device}")
-    holds = min(table.shape[1] * page_size, selected.shape[2], (1 << 30) - 1)
+                         f"on q's device; got {selected.dtype} {tuple(state)} on {selected.device}")
+    holds = min(width * page_size, state[2], (1 << 30) - 1)
     if holds < 1:
         raise ValueError("selected holds no position")
     if max_len is None:
         max_len = holds
-    if int(max_len) != max_len or not 1 <= max_len <= holds:
+    elif int(max_len) != max_len or not 1 <= max_len <= holds:
         raise ValueError(f"max_len must be an integer from 1 to the {holds} positions that table and selected hold; got {max_len}")
     if max_new is None:
-        max_new = max(q.shape[0], 1)
-    if int(max_new) != max_new or max_new < 1:
+        max_new = tokens
+    elif int(max_new) != max_new or max_new < 1:
         raise ValueError(f"max_new must be an integer >= 1; got {max_new}")
-    return page_size, _check_exempt(exempt), int(max_new), int(max_len)
+    return (requests, tokens, heads, state[1], head_dim, pages, page_size, width, min(int(max_new), tokens), int(max_len), ld,
+            strides[1], dtype, device, _check_exempt(exempt))
 
 
 def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, starts: Tensor,
@@ -233,22 +241,20 @@ def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table
     """
 
     _check_cuda(k_pages)
-    page_size, exempt, max_new, max_len = _check_step(q, k_pages, v_pages, table, lengths, starts, selected, exempt, max_new, max_len)
-    tokens, heads, head_dim = q.shape
-    out = torch.empty(tokens, heads, head_dim, device=q.device, dtype=q.dtype)
+    (requests, tokens, heads, groups, head_dim, pages, page_size, width, max_new, max_len, table_ld, state_ld, dtype, device,
+     exempt) = _check_step(q, k_pages, v_pages, table, lengths, starts, selected, exempt, max_new, max_len)
+    out = torch.empty(tokens, heads, head_dim, device=device, dtype=dtype)
     if tokens == 0:
         return out
     lib = _lib.load()
-    max_new = min(max_new, tokens)
-    requests, groups = lengths.shape[0], selected.shape[1]
-    code = _CODES[q.dtype]
+    code = _CODES[dtype]
     q = _rows(q)
-    ws = torch.empty(lib.sa_paged_attention_workspace_bytes(requests, tokens, heads, groups, head_dim, max_new, max_len, code),
-                     device=q.device, dtype=torch.uint8)
-    _call(q.device, lib.sa_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
-          out.data_ptr(), table.data_ptr(), table.stride(0), lengths.data_ptr(), starts.data_ptr(), selected.data_ptr(),
-          selected.stride(1), ws.data_ptr(), ws.numel(), requests, tokens, heads, groups, head_dim, k_pages.shape[0],
-          page_size, table.shape[1], max_new, max_len, 1.0 / math.sqrt(head_dim), code, exempt)
+    size = lib.sa_paged_attention_workspace_bytes(requests, tokens, heads, groups, head_dim, max_new, max_len, code)
+    ws = torch.empty(size, device=device, dtype=torch.uint8)
+    _call(device, lib.sa_paged_attention, q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), v_pages.data_ptr(),
+          out.data_ptr(), table.data_ptr(), table_ld, lengths.data_ptr(), starts.data_ptr(), selected.data_ptr(), state_ld,
+          ws.data_ptr(), size, requests, tokens, heads, groups, head_dim, pages, page_size, width, max_new, max_len,
+          1.0 / math.sqrt(head_dim), code, exempt)
     return out
 
 
