@@ -382,7 +382,8 @@ struct PagedShape {
   int nw, hg;                 // several: query tiles of 32 rows per workgroup, heads per wavefront (4: per workgroup, paged_fwd4)
   int splits, span_tiles;     // key spans, and their 32-key tiles
   int carry_blocks;           // workgroups along the keys of the histories
-  int64_t carry, m, o;        // (m: (maximum, sum) pairs)
+  bool reach;                 // key tiles without weight are looked for
+  int64_t carry, m, o, least, kn;   // (m: (maximum, sum) pairs)
   int64_t total;
 };
 inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_t D, int64_t es, int64_t max_new, int64_t max_len) {
@@ -423,6 +424,11 @@ inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_
     s.splits = (int)cdiv(tiles, s.span_tiles);
     s.carry_blocks = (int)std::max<int64_t>(1, std::min(cdiv(tiles, NWAVES), cdiv(8192, R * G)));
     s.carry = take((N / TILE + R) * G * s.ld * 4);
+    s.reach = s.nw == 4 && max_len >= REACH_MIN_KEYS;
+    if (s.reach) {
+      s.least = take((N / TILE + R) * G * (s.ld / TILE) * 4);
+      s.kn = take(R * H * (s.ld / TILE) * 4);
+    }
     if (s.splits > 1) {
       s.m = take(s.splits * N * H * 8);
       s.o = take(s.splits * N * H * D * 4);

@@ -112,6 +112,8 @@ struct PagedCall {
   int R, N, H, G, pages, pshift;
   int max_new, max_len;
   int ones;   // several tokens: requests with one new token are left to the single-token kernels
+  float *least, *kn;   // per key tile: least history on entry to a query tile, largest key norm; NULL: every tile is computed
+  int64_t reach_ld;
   float scale;
   int exempt;
 };
@@ -134,6 +136,12 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedCall& a, int r)
   q.live = rows && q.t >= q.n && q.t <= a.max_len && q.n <= a.max_new;   // (max_len: within the table and state rows)
   return q;
 }
+
+struct PagedTiles {   // what a workgroup of query tiles has to do
+  PagedRequest rq;
+  int r, row0;        // request, its first row
+  int kt_lo, kt_hi;   // the key tiles of its span that one of its rows sees
+};
 
 static __device__ uint4 paged_zero_row;   // what rows without a page read
 
@@ -552,6 +560,115 @@ struct PagedRows {
   }
 };
 
+// c + the products of two chunks' elements
+template <class P>
+__device__ __forceinline__ float chunk_dot(u32x4 x, u32x4 y, float c) {
+  union {
+    u32x4 u;
+    typename P::elem e[P::EPC];
+  } a{x}, b{y};
+#pragma unroll
+  for (int e = 0; e < P::EPC; ++e) c = fmaf(P::to_float(a.e[e]), P::to_float(b.e[e]), c);
+  return c;
+}
+
+// The least of a wavefront's 64 values, in every lane.
+__device__ __forceinline__ float least_of(float x) {
+  auto with = [](float y, int z) { return fminf(y, __int_as_float(z)); };
+  x = with(x, __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x111, 0xF, 0xF, false));   // row_shr:1, 2, 4, 8
+  x = with(x, __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x112, 0xF, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x114, 0xF, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x118, 0xF, 0xF, false));
+  x = with(x, __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x142, 0xA, 0xF, false));   // row_bcast:15, 31
+  x = with(x, __builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x143, 0xC, 0xF, false));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// The key tiles of a workgroup's span that its rows can give weight to (as find_reach for the contiguous cache): for a tile
+// before the rows, log2 weight <= s log2e |q| max |k| - log2e (least F) - (row maximum), the row maximum at least the row's logit
+// of its own key, which has no history. Below -REACH_ZERO a weight is an exact fp32 zero (in a part of several spans: once they
+// are joined), and the tile is left out for all of the workgroup's heads together; tiles for which a NaN or an infinity enters
+// the bound stay. A mask in LDS, bit i the span's i-th newest tile; past the mask's end every tile stays.
+struct PagedLive {
+  const uint64_t* mask;   // NULL: every tile
+  int hi, lo;
+  __device__ __forceinline__ int below(int kt) const {   // the next older tile, -1: none
+    int i = hi - kt;
+    if (mask == nullptr) return kt - 1 >= lo ? kt - 1 : -1;
+    while (i < hi - lo) {
+      const int word = i >> 6;
+      if (word >= REACH_MASK_WORDS) return hi - 1 - i;
+      const uint64_t m = uniform64(mask[word]) >> (i & 63);
+      if (m) return hi - 1 - (i + __builtin_ctzll(m));
+      i = (word + 1) << 6;
+    }
+    return -1;
+  }
+};
+
+// Whether any of a sample of the span's tiles has history enough for the search to pay.
+__device__ __forceinline__ bool paged_live_worth(const float* least, int lo, int hi) {
+  if (hi <= lo) return false;
+  const int lane = threadIdx.x & 63, kt = lo + (int)((int64_t)(hi - lo) * lane >> 6);
+  return __any(least[kt] * REACH_F > REACH_WORTH);
+}
+// The larger of a row's two bounds over a wavefront's 32 rows of a head: largest |q|, least logit (log2 units) of a row's own key.
+template <class P, int D>
+__device__ __forceinline__ void paged_live_bounds(const PagedCall& a, const PagedRequest& rq, int r, int row, int head,
+                                                  const u32x4 (&qf)[PagedTile<P, D>::NS], float (&bound)[2]) {
+  const int h = (threadIdx.x >> 5) & 1, pos = rq.c + row;
+  const bool in = row < rq.n;
+  const int pg = in ? a.table[r * a.table_ld + (pos >> a.pshift)] : -1;
+  const typename P::elem* k = static_cast<const typename P::elem*>(a.k_pages) +
+                              ((((int64_t)pg * a.H + head) << a.pshift) + (pos & ((1 << a.pshift) - 1))) * D + h * P::EPC;
+  const bool ok = (uint32_t)pg < (uint32_t)a.pages;
+  float qq = 0.f, qk = 0.f;
+#pragma unroll
+  for (int s = 0; s < PagedTile<P, D>::NS; ++s) {
+    qq = chunk_dot<P>(qf[s], qf[s], qq);
+    if (ok) qk = chunk_dot<P>(qf[s], *reinterpret_cast<const u32x4*>(k + 2 * s * P::EPC), qk);
+  }
+  const Halves q2 = halves(qq), z2 = halves(qk);
+  const float z = (z2.lo + z2.hi) * (a.scale * LOG2E);
+  bound[0] = sqrtf(half_max(q2.lo + q2.hi < REACH_NORM2 ? q2.lo + q2.hi : INFINITY));
+  bound[1] = -half_max(in ? (z > -3.0e38f ? -z : INFINITY) : -INFINITY);
+}
+// The mask, by WAVES wavefronts, a lane per key tile: bound[head][part] as above, `least` and `kn` the rows of the workgroup's
+// first query tile and first head.
+template <int WAVES, int HEADS, int PARTS>
+__device__ __forceinline__ void paged_live_mask(const PagedCall& a, const PagedTiles& w, const float (*bound)[PARTS][2], const float* least,
+                                                const float* kn, uint64_t* mask) {
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  float qa[HEADS], zb[HEADS];
+#pragma unroll
+  for (int g = 0; g < HEADS; ++g) {
+    qa[g] = bound[g][0][0];
+    zb[g] = bound[g][0][1];
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) {
+      qa[g] = fmaxf(qa[g], bound[g][p][0]);
+      zb[g] = fminf(zb[g], bound[g][p][1]);
+    }
+    qa[g] *= a.scale * REACH_Q;
+  }
+  const int words = min((w.kt_hi - w.kt_lo + 63) >> 6, REACH_MASK_WORDS);
+  for (int word = wave; word < words; word += WAVES) {
+    const int kt = w.kt_hi - 1 - (word * 64 + lane);
+    bool live = kt >= w.kt_lo;
+    if (live && (kt + 1) * TILE <= w.rq.c + w.row0) {
+      const float f = least[kt] * REACH_F;
+      if (f > REACH_WORTH) {   // (else a key norm may be missing)
+        bool dead = true;
+#pragma unroll
+        for (int g = 0; g < HEADS; ++g) dead &= qa[g] * kn[g * a.reach_ld + kt] - f - zb[g] < -REACH_ZERO;
+        live = !dead;
+      }
+    }
+    const uint64_t m = __ballot(live);
+    if (lane == 0) mask[word] = m;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // The selectors' histories of a step of several tokens: carry[tile][g][j], what key j has received before the
 // tile's first query, and the state after the step. A wavefront owns 32 keys of one selector (rows in registers) and
@@ -560,6 +677,10 @@ struct PagedRows {
 // products and sums are kept independent; the rows are loaded into LDS three steps ahead, once for the workgroup. At 4096
 // queries on 32768 keys (us): 48; one tile at a time from the L2 105, four at a time 64, through LDS one step ahead 55. Rows
 // of keys that no query of a tile sees hold no history: the forward masks those keys.
+//
+// With a.least, also what the forward needs to leave out key tiles without weight (PagedLive): each key tile's least history
+// on entry to every fourth query tile, and, of key tiles whose least history at the end makes it possible, the largest
+// |k| of every head of the group (infinity where a key or a value is not finite, or a product could overflow).
 template <class P, int D>
 __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, float* __restrict__ carry, int64_t carry_ld) {
   typedef PagedTile<P, D> T;
@@ -567,8 +688,8 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
   constexpr int NS = T::NS, U = T::BYTES > 8192 ? 1 : T::BYTES > 4096 ? 2 : 4, PER = U * T::PARTS / NWAVES;
   // The U tiles of step t are in buffer t mod 4 (variables of their own: a step's reads touch none of the others), filled
   // by loads that step t - 3 issues (the prologue for the first three). Every step issues PER loads (past the last tile: of
-  // nothing), then U stores, so at its end the loads of step t + 1, issued in step t - 2, have landed once
-  // no more than 2 PER + 3 U newer operations run.
+  // nothing), then U + 1 stores, so at its end the loads of step t + 1, issued in step t - 2, have landed once
+  // no more than 2 PER + 3 (U + 1) newer operations run.
   __shared__ __attribute__((aligned(16))) char sQ0[U * T::BYTES], sQ1[U * T::BYTES], sQ2[U * T::BYTES], sQ3[U * T::BYTES];
   const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
   const int r = blockIdx.z, g = blockIdx.y;
@@ -597,7 +718,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
   for (int kb0 = blockIdx.x * NWAVES; kb0 < nkb; kb0 += gridDim.x * NWAVES) {
     const int kb = kb0 + wave, j = kb * TILE + n;
     // tiles before this end before the workgroup's first key
-    int rb = max(kb0 * TILE - rq.c, 0) / TILE;
+    int rb = (max(kb0 * TILE - rq.c, 0) / TILE) & ~3;   // (every fourth one begins a step)
     load_q(rb, sQ0);
     load_q(rb + U, sQ1);
     load_q(rb + 2 * U, sQ2);
@@ -612,6 +733,8 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
         kf[s] = ok ? *reinterpret_cast<const u32x4*>(k + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
     }
     float run = j < rq.c ? state[j] : 0.f;
+    const int64_t lplane = a.G * a.reach_ld;
+    float* least = a.least + ((int64_t)((rq.first >> 5) + r) * a.G + g) * a.reach_ld + kb;   // (not used without a.least)
     const uint32_t end = (uint32_t)rq.t * 4, own = h == 0 && j < rq.t ? (uint32_t)j * 4 : end;   // byte offset of the lane's key in a row of histories
     auto step = [&](const char* buf, char* next) {
       load_q(rb + 3 * U, next);
@@ -633,6 +756,11 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
         for (int u = 0; u < U; ++u)
           sum[u] = block_selection_sum(acc[u], false, j >= a.exempt ? j - qbase - u * TILE - 4 * h : 32, a.scale);
       }
+      {
+        const bool kept = a.least != nullptr && (rb & 3) == 0 && rb < ntile && kb < nkb;
+        const float mn = kept ? least_of(j >= rq.t ? INFINITY : run == run ? run : -INFINITY) : 0.f;   // (a NaN keeps the tile)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mn), rsrc(least + rb * lplane, kept ? 4 : 0), lane * 4, 0, 0);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {   // (every lane stores, past the row's end where it has no key or the tile is none)
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(run), rsrc(cr + (rb + u) * plane, rb + u < ntile ? end : 0), own, 0, 0);
@@ -640,7 +768,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
       }
       rb += U;
       // (one asm block: at a barrier of its own the compiler waits for everything)
-      __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER + 3 * U) : "memory");
+      __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * PER + 3 * (U + 1)) : "memory");
     };
     wait_loads();
     __syncthreads();
@@ -657,6 +785,38 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
     wait_loads();   // nothing on its way into LDS when the workgroup ends or takes its next keys
     __syncthreads();
     if (h == 0 && j < rq.t) state[j] = run;
+    if (a.least != nullptr && kb < nkb && least_of(j < rq.t ? run : INFINITY) * REACH_F > REACH_WORTH) {
+      const int pg = j < rq.t ? trow[j >> a.pshift] : -1;
+      const bool ok = (uint32_t)pg < (uint32_t)a.pages;
+      constexpr int HB = NS <= 4 ? 4 : NS == 8 ? 2 : 1;   // heads whose rows are on their way at a time
+      for (int head = hd; head < hd + a.H / a.G; head += HB) {
+        u32x4 kr[HB][NS], vr[HB][NS];
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+          const int hb = min(head + b, hd + a.H / a.G - 1);
+          const int64_t at = ((((int64_t)(ok ? pg : 0) * a.H + hb) << a.pshift) + (j & ((1 << a.pshift) - 1))) * D + h * P::EPC;
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            kr[b][s] = *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.k_pages) + at + 2 * s * P::EPC);
+            vr[b][s] = *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.v_pages) + at + 2 * s * P::EPC);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+          float kk = 0.f, vv = 0.f;
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            kk = chunk_dot<P>(kr[b][s], kr[b][s], kk);
+            vv = chunk_dot<P>(vr[b][s], vr[b][s], vv);
+          }
+          const Halves k2 = halves(kk), v2 = halves(vv);
+          // (a row without a page is zeros)
+          const float x = !ok ? 0.f : (k2.lo + k2.hi < REACH_NORM2 && v2.lo + v2.hi < REACH_NORM2) ? k2.lo + k2.hi : INFINITY;
+          const float mx = -least_of(-x);
+          if (lane == 0 && head + b < hd + a.H / a.G) a.kn[((int64_t)r * a.H + head + b) * a.reach_ld + kb] = sqrtf(mx);
+        }
+      }
+    }
   }
 }
 
@@ -673,11 +833,13 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
 //
 // P is rounded to the cache's type for the product with V (relative 2^-9 bf16, 2^-12 fp16 at random, the size of the
 // output's own rounding; fp32 not at all); logits, F, row statistics and sums are fp32.
-struct PagedTiles {   // what a workgroup of query tiles has to do
-  PagedRequest rq;
-  int r, row0;        // request, its first row
-  int kt_lo, kt_hi;   // the key tiles of its span that one of its rows sees
-};
+// The grid of the forward kernels: heads and spans, then query tiles, over y and z where a dimension's 65535 would not hold them.
+inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
+  const int64_t rounds = cdiv(tiles, 32768);
+  return dim3((unsigned)per_tile, (unsigned)cdiv(tiles, rounds), (unsigned)rounds);
+}
+__device__ __forceinline__ int last_tile_first() { return gridDim.y * gridDim.z - 1 - (blockIdx.z * gridDim.y + blockIdx.y); }
+
 // Workgroup number x (1 << SH rows, numbered as above) and key span z; false: nothing. Rows that no workgroup computes, those
 // behind the last request and those of requests left out, become zero here, COLS columns from col0 on, unless the spans are
 // joined afterwards (the join does it).
@@ -769,10 +931,12 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   __shared__ typename FwdLds<P, D, HG, NW>::Tiles sB0, sB1;
   __shared__ __attribute__((aligned(16))) char sS0[T::BYTES], sS1[T::BYTES];
   __shared__ __attribute__((aligned(16))) float sF[NW][TILE * LDF];
+  __shared__ uint64_t sMask[NW == 1 ? 1 : REACH_MASK_WORDS];   // PagedLive
+  __shared__ float sBound[HG][NW][2];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = NW == 1 ? 0 : wave_id();
   const int n = lane & 31, h = lane >> 5;
-  const int groups = a.H / HG, x = gridDim.y - 1 - blockIdx.y, z = blockIdx.x / groups;
+  const int groups = a.H / HG, x = last_tile_first(), z = blockIdx.x / groups;
   const int hd0 = (blockIdx.x % groups) * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
   PagedTiles w;
   if (!paged_tiles<P, SH, HG * D, NW * 64>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
@@ -855,36 +1019,59 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
     }
   };
 
-  // the tiles, newest first: cur in the buffers, cur - 1's selector rows too, cur - 2's pages known
-  int cur = kt_hi - 1;
-  typename Rows::Place off1[PER], off2[PER];   // of tiles cur - 1 and cur - 2
+  PagedLive tiles{nullptr, kt_hi, kt_lo};
+  if constexpr (NW > 1) {
+    const float* least = a.least + ((int64_t)((rq.first >> 5) + r + (row0 >> 5)) * a.G + g0) * a.reach_ld;
+    if (a.least != nullptr && paged_live_worth(least, kt_lo, min(kt_hi, (rq.c + row0) / TILE))) {
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        float bound[2];
+        paged_live_bounds<P, D>(a, rq, r, q_row, hd0 + g, qf[g], bound);
+        if (lane == 0) {
+          sBound[g][wave][0] = bound[0];
+          sBound[g][wave][1] = bound[1];
+        }
+      }
+      __syncthreads();
+      paged_live_mask<NW, HG, NW>(a, w, sBound, least, a.kn + ((int64_t)r * a.H + hd0) * a.reach_ld, sMask);
+      __syncthreads();
+      tiles.mask = sMask;
+    }
+  }
+
+  // the tiles, newest first: cur in the buffers, n1's selector rows too, n2's pages known (-1: none)
+  int cur = tiles.below(kt_hi), n1 = cur >= 0 ? tiles.below(cur) : -1, n2 = n1 >= 0 ? tiles.below(n1) : -1;
+  typename Rows::Place off1[PER], off2[PER];   // of tiles n1 and n2
   int pg[PER];
   {
     typename Rows::Place off0[PER];
     rows.pages_of(cur, pg);
     rows.places(cur, pg, off0);
-    load_tile(sB0, off0);
-    load_sel(sS0, off0);
-    rows.pages_of(cur - 1 >= kt_lo ? cur - 1 : -1, pg);
-    rows.places(cur - 1, pg, off1);
-    if (cur - 1 >= kt_lo) load_sel(sS1, off1);
-    rows.pages_of(cur - 2 >= kt_lo ? cur - 2 : -1, pg);
+    if (cur >= 0) {
+      load_tile(sB0, off0);
+      load_sel(sS0, off0);
+    }
+    rows.pages_of(n1, pg);
+    rows.places(n1, pg, off1);
+    if (n1 >= 0) load_sel(sS1, off1);
+    rows.pages_of(n2, pg);
   }
-  float entry1 = carry_of(cur - 1);
+  float entry1 = carry_of(n1);
   const float entry0 = carry_of(cur);
   wait_loads();
   __syncthreads();
-  if (cur < my_end) select(cur, sS0, entry0);
+  if (cur >= 0 && cur < my_end) select(cur, sS0, entry0);
   __syncthreads();   // every wavefront is past its reads of sS0, which the first step fills
 
   auto step = [&](auto odd_tag) __attribute__((always_inline)) {
     constexpr bool ODD = decltype(odd_tag)::value;
     auto& B = ODD ? sB1 : sB0;
-    rows.places(cur - 2, pg, off2);
-    if (cur - 1 >= kt_lo) load_tile(ODD ? sB0 : sB1, off1);
-    if (cur - 2 >= kt_lo) load_sel(ODD ? sS1 : sS0, off2);
-    rows.pages_of(cur - 3 >= kt_lo ? cur - 3 : -1, pg);
-    const float entry2 = cur - 2 >= kt_lo ? carry_of(cur - 2) : 0.f;
+    rows.places(n2, pg, off2);
+    if (n1 >= 0) load_tile(ODD ? sB0 : sB1, off1);
+    if (n2 >= 0) load_sel(ODD ? sS1 : sS0, off2);
+    const int n3 = n2 >= 0 ? tiles.below(n2) : -1;
+    rows.pages_of(n3, pg);
+    const float entry2 = carry_of(n2);
     if (cur < my_end) {
       const int kbase = cur * TILE;
       f32x16 fs;
@@ -940,19 +1127,20 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
         for (int db = 0; db < DB; ++db) o[g][db] = T::values(B.v[g], lane, db, pf, lg, o[g][db]);
       }
     }
-    if (cur - 1 >= kt_lo && cur - 1 < my_end) select(cur - 1, ODD ? sS0 : sS1, entry1);
+    if (n1 >= 0 && n1 < my_end) select(n1, ODD ? sS0 : sS1, entry1);
     entry1 = entry2;
 #pragma unroll
     for (int i = 0; i < PER; ++i) off1[i] = off2[i];
     wait_loads();
     __syncthreads();
-    --cur;
+    cur = n1;
+    n1 = n2;
+    n2 = n3;
   };
-  while (true) {
+  while (cur >= 0) {
     step(std::false_type{});
-    if (cur < kt_lo) break;
+    if (cur < 0) break;
     step(std::true_type{});
-    if (cur < kt_lo) break;
   }
 
 #pragma unroll
@@ -993,10 +1181,12 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
   __shared__ __attribute__((aligned(16))) char sS0[T::BYTES], sS1[T::BYTES];
   __shared__ __attribute__((aligned(16))) float sF0[4][TILE * LDF], sF1[4][TILE * LDF];
   __shared__ u32x4 sQ[4][NS * 64];   // the selector's query fragments (written once: registers are short)
+  __shared__ uint64_t sMask[REACH_MASK_WORDS];   // PagedLive
+  __shared__ float sBound[HG][4][2];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
   const int u = wave & 3, qt = wave >> 2;   // the wavefront's head and query tile
-  const int groups = a.H / HG, x = gridDim.y - 1 - blockIdx.y, z = blockIdx.x / groups;
+  const int groups = a.H / HG, x = last_tile_first(), z = blockIdx.x / groups;
   const int hd0 = (blockIdx.x % groups) * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
   PagedTiles w;
   if (!paged_tiles<P, SH, HG * D, 1024>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
@@ -1039,7 +1229,7 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
     if (u == 0) rows.load(S, kselp, pl, qt);
   };
   const float* crow_p = carry + ((int64_t)((rq.first >> 5) + w.r + (min(rb, rq.n - 1) >> 5)) * a.G + g0) * carry_ld;
-  auto carry_of = [&](int kt) { return kt >= kt_lo ? crow_p[min(kt * TILE + n, rq.t - 1)] : 0.f; };
+  auto carry_of = [&](int kt) { return kt >= 0 ? crow_p[min(kt * TILE + n, rq.t - 1)] : 0.f; };
 
   auto select = [&](int kt, const char* S, float entry, float* fw) {   // paged_fwd_kernel's
     const int kbase = kt * TILE;
@@ -1123,7 +1313,25 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
         o[db] = P::mma(T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s), pf[s], o[db]);
   };
 
-  int cur = w.kt_hi - 1;   // the tile of the step; the t-th: t mod 2 names the buffers
+  PagedLive tiles{nullptr, w.kt_hi, kt_lo};
+  {
+    const float* least = a.least + ((int64_t)((rq.first >> 5) + w.r + (w.row0 >> 5)) * a.G + g0) * a.reach_ld;
+    if (a.least != nullptr && paged_live_worth(least, kt_lo, min(w.kt_hi, (rq.c + w.row0) / TILE))) {
+      float bound[2];
+      paged_live_bounds<P, D>(a, rq, w.r, rb + n, hd0 + u, qf, bound);
+      if (lane == 0) {
+        sBound[u][qt][0] = bound[0];
+        sBound[u][qt][1] = bound[1];
+      }
+      __syncthreads();
+      paged_live_mask<16, HG, 4>(a, w, sBound, least, a.kn + ((int64_t)w.r * a.H + hd0) * a.reach_ld, sMask);
+      __syncthreads();
+      tiles.mask = sMask;
+    }
+  }
+
+  // the tile of the step (the t-th: t mod 2 names the buffers), and the next two; -1: none
+  int cur = tiles.below(w.kt_hi), n1 = cur >= 0 ? tiles.below(cur) : -1, n2 = n1 >= 0 ? tiles.below(n1) : -1;
   int turn = (u - qt) & 3;   // tiles until the wavefront's next selection (0: the tile at hand)
   typename Rows::Place at1[1], at2[1];
   int pg[1];
@@ -1131,49 +1339,51 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
     typename Rows::Place at0[1];
     rows.pages_of(cur, pg);
     rows.places(cur, pg, at0);
-    load_tile(sB0, at0);
-    load_sel(sS0, at0);
-    rows.pages_of(cur - 1 >= kt_lo ? cur - 1 : -1, pg);
-    rows.places(cur - 1, pg, at1);
-    if (cur - 1 >= kt_lo) load_sel(sS1, at1);
-    rows.pages_of(cur - 2 >= kt_lo ? cur - 2 : -1, pg);
+    if (cur >= 0) {
+      load_tile(sB0, at0);
+      load_sel(sS0, at0);
+    }
+    rows.pages_of(n1, pg);
+    rows.places(n1, pg, at1);
+    if (n1 >= 0) load_sel(sS1, at1);
+    rows.pages_of(n2, pg);
   }
-  float entry = carry_of(cur - turn);   // of the wavefront's next selection
+  float entry = carry_of(n1);   // of the next tile, a step ahead (every wavefront: a branch would have the compiler wait)
+  const float entry0 = carry_of(cur);
   wait_loads();
   __syncthreads();
-  if (turn == 0) {
-    if (cur < end) select(cur, sS0, entry, sF0[qt]);
-    entry = carry_of(cur - 4);
-  }
+  if (turn == 0 && cur >= 0 && cur < end) select(cur, sS0, entry0, sF0[qt]);
   turn = (turn - 1) & 3;
-  __asm__ volatile("" : "+v"(entry));   // (waited for here: in the loop the compiler would wait for the tiles' loads with it)
   __syncthreads();
 
   auto step = [&](auto odd_tag) __attribute__((always_inline)) {
     constexpr bool ODD = decltype(odd_tag)::value;
-    rows.places(cur - 2, pg, at2);
-    if (cur - 1 >= kt_lo) load_tile(ODD ? sB0 : sB1, at1);
-    if (cur - 2 >= kt_lo) load_sel(ODD ? sS1 : sS0, at2);
-    rows.pages_of(cur - 3 >= kt_lo ? cur - 3 : -1, pg);
+    rows.places(n2, pg, at2);
+    if (n1 >= 0) load_tile(ODD ? sB0 : sB1, at1);
+    if (n2 >= 0) load_sel(ODD ? sS1 : sS0, at2);
+    const int n3 = n2 >= 0 ? tiles.below(n2) : -1;
+    rows.pages_of(n3, pg);
+    const float entry2 = carry_of(n2);
     if (turn == 0) {
       // the next tile's F: first, and ahead of the SIMD's other wavefronts, which wait for it at the step's end
       __builtin_amdgcn_s_setprio(1);
-      if (cur - 1 >= kt_lo && cur - 1 < end) select(cur - 1, ODD ? sS0 : sS1, entry, ODD ? sF0[qt] : sF1[qt]);
-      entry = carry_of(cur - 5);
+      if (n1 >= 0 && n1 < end) select(n1, ODD ? sS0 : sS1, entry, ODD ? sF0[qt] : sF1[qt]);
     }
     if (cur < end) attend(cur, ODD ? sB1 : sB0, ODD ? sF1[qt] : sF0[qt]);
     __builtin_amdgcn_s_setprio(0);
     turn = (turn - 1) & 3;
     at1[0] = at2[0];
+    entry = entry2;
     wait_loads();
     __syncthreads();
-    --cur;
+    cur = n1;
+    n1 = n2;
+    n2 = n3;
   };
-  while (true) {
+  while (cur >= 0) {
     step(std::false_type{});
-    if (cur < kt_lo) break;
+    if (cur < 0) break;
     step(std::true_type{});
-    if (cur < kt_lo) break;
   }
   paged_write<P, D>(a, w, rb + n, hd0 + u, z, mu, l, o, h, part_ml, part_o);
 }
@@ -1492,8 +1702,8 @@ inline PagedCall paged_call(const PagedLaunch& c) {
 
 template <class P, int D, int HG, int NW, bool WHOLE>
 void launch_paged_fwd(const PagedCall& a, const PagedShape& s, const float* carry, float* ml, float* o, hipStream_t st) {
-  const unsigned tiles = (unsigned)((a.N >> (NW == 4 ? 7 : 5)) + a.R);
-  hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE>), dim3((unsigned)(a.H / HG * s.splits), tiles), dim3(NW * 64), 0, st,
+  const int64_t tiles = (int64_t)(a.N >> (NW == 4 ? 7 : 5)) + a.R;
+  hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE>), tile_grid((int64_t)a.H / HG * s.splits, tiles), dim3(NW * 64), 0, st,
                      a, carry, s.ld, s.span_tiles, ml, o);
 }
 
@@ -1521,6 +1731,11 @@ int paged_launch(const PagedLaunch& c) {
   a.ones = s.several && s.ones;
   if (s.ones) launch_paged_step<P, D>(a, s, ws, c.st);
   if (!s.several) return launch_status();
+  if (s.reach) {
+    a.least = at(s.least);
+    a.kn = at(s.kn);
+    a.reach_ld = s.ld / TILE;
+  }
   float *carry = at(s.carry), *ml = s.splits > 1 ? at(s.m) : nullptr, *o = s.splits > 1 ? at(s.o) : nullptr;
   {
     TimedLaunch timed(SA_KERNEL_SELECTION, c.st);
@@ -1531,11 +1746,9 @@ int paged_launch(const PagedLaunch& c) {
     TimedLaunch timed(SA_KERNEL_FORWARD, c.st);
     const bool whole = a.G == a.H;
     if constexpr (sizeof(typename P::elem) == 2 && D == 64) {
-      if (s.hg == 4) {
-        const unsigned tiles = (unsigned)((a.N >> 7) + a.R);
-        hipLaunchKernelGGL((paged_fwd4_kernel<P>), dim3((unsigned)(a.H / 4 * s.splits), tiles), dim3(1024), 0, c.st, a, carry, s.ld,
-                           s.span_tiles, ml, o);
-      }
+      if (s.hg == 4)
+        hipLaunchKernelGGL((paged_fwd4_kernel<P>), tile_grid((int64_t)a.H / 4 * s.splits, (a.N >> 7) + a.R), dim3(1024), 0, c.st, a,
+                           carry, s.ld, s.span_tiles, ml, o);
     }
     if constexpr (sizeof(typename P::elem) == 2 && D <= 64) {
       if (s.hg == 2) {

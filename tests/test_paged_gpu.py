@@ -377,3 +377,80 @@ def test_a_mixed_step_with_many_single_tokens(cuda):
     args[4][3], args[4][7] = 0, 10**7   # left out
     out = sa.selective_attention_paged(*args)
     assert (out[[3, 7, 40]] == 0).all() and (out[[2, 4, 6, 8, 39]].abs().sum(-1) > 0).all()
+
+
+def outgrown(step, rate):
+    """Histories as queries that select at `rate` would have left them: keys some hundred positions back carry no weight."""
+    for r, c in enumerate(step.cached):
+        step.selected[r, :, :c] = rate * (c - 1 - torch.arange(c)).clamp(min=0)
+        step.selected[r, :, :step.exempt] = 0.0
+    return step
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("head_dim,heads,groups,exempt", [(64, 4, 1, 1), (64, 2, 1, 40), (64, 2, 2, 1), (128, 2, 1, 1), (32, 2, 1, 3), (16, 2, 2, 1)])
+def test_key_tiles_without_weight(cuda, dtype, head_dim, heads, groups, exempt):
+    """Histories that leave most key tiles out, of requests that cross from such tiles into others, and that have none."""
+    step = outgrown(Step([1500, 40, 3000, 0], [70, 200, 33, 130], heads=heads, head_dim=head_dim, groups=groups, dtype=dtype, exempt=exempt,
+                         seed=3), 0.4)
+    out, state = attend(step, cuda)
+    check(out, state, step, ROUNDED[dtype])
+    # a little selection: the oldest tiles only
+    step = outgrown(Step([4000], [50], heads=heads, head_dim=head_dim, groups=groups, dtype=dtype, exempt=exempt, seed=4), 0.04)
+    out, state = attend(step, cuda)
+    check(out, state, step, ROUNDED[dtype])
+
+
+@pytest.mark.parametrize("head_dim,heads", [(64, 4), (128, 2)])
+def test_tiles_left_out_keep_the_bits(cuda, head_dim, heads):
+    """A value that is not finite, in a tile whose weights are all zero, keeps the tile, of every request before and
+    after: the outputs of the heads that do not hold it have the same bits, those of its own are NaN (0 times infinity)."""
+    step = outgrown(Step([2000], [60], heads=heads, head_dim=head_dim, seed=5), 0.4)
+    out, state = attend(step, cuda)
+    page = int(step.table[0, 500 // 16])
+    step.v_pages[page, 1, 500 % 16, 3] = float("inf")
+    kept, again = attend(step, cuda)
+    others = [h for h in range(heads) if h != 1]
+    assert torch.equal(out[:, others], kept[:, others]) and torch.equal(state.nan_to_num(-1), again.nan_to_num(-1))
+    assert kept[:, 1, 3].isnan().all() and torch.equal(kept[:, 1, 4:], out[:, 1, 4:])
+    step.v_pages[page, 1, 500 % 16, 3] = 0.0
+    step.k_pages[page, 1, 500 % 16, 3] = float("nan")   # a key: every weight of its head
+    kept, _ = attend(step, cuda)
+    assert kept[:, 1].isnan().all() and torch.equal(out[:, others], kept[:, others])
+    step.k_pages[page, 1, 500 % 16, 3] = 0.0
+    step.selected[0, 0, 500] = float("nan")   # a history: every weight of every head
+    kept, _ = attend(step, cuda)
+    assert kept.isnan().all()
+
+
+def test_more_query_tiles_than_a_grid_dimension(cuda):
+    """65535 requests, a hundred of them with two new tokens: those, and some of one token, as in a small batch."""
+    R, P, D, c = 65535, 8, 16, 20
+    g = torch.Generator().manual_seed(0)
+    two = torch.arange(100) * 661
+    new = torch.ones(R, dtype=torch.int32)
+    new[two] = 2
+    N = int(new.sum())
+    starts = torch.cat([torch.zeros(1, dtype=torch.int32), new.cumsum(0, dtype=torch.int32)]).int()
+    table = torch.randint(0, 64, (R, 3), generator=g, dtype=torch.int32)   # pages that requests share
+    k, v = (torch.randn(64, 1, P, D, generator=g).to(cuda, torch.bfloat16) for _ in range(2))
+    q = torch.randn(N, 1, D, generator=g).to(cuda, torch.bfloat16)
+    history = torch.rand(R, 1, 3 * P, generator=g)
+
+    def call(rows):
+        at = torch.cat([torch.arange(int(starts[r]), int(starts[r + 1])) for r in rows]) if len(rows) < R else torch.arange(N)
+        begin = torch.cat([torch.zeros(1, dtype=torch.int32), new[rows].cumsum(0, dtype=torch.int32)]).int()
+        selected = history[rows].to(cuda).contiguous()
+        plan = [table[rows].to(cuda), (c + new[rows]).int().to(cuda), begin.to(cuda)]
+        out = sa.selective_attention_paged(q[at.to(cuda)].contiguous(), k, v, *plan, selected, max_new=2, max_len=c + 2)
+        torch.cuda.synchronize()
+        return out, selected, at.to(cuda)
+
+    out, state, _ = call(torch.arange(R))
+    some = torch.cat([two, two + 1]).sort().values
+    few, few_state, at = call(some)
+    assert not out.isnan().any()
+    # the two calls may take different kernels: weights rounded to bf16 (half a step, 2^-9, of values up to 4), and each
+    # output; states of sums of sixteen fp32 products
+    torch.testing.assert_close(out[at].float(), few.float(), rtol=2**-7, atol=2**-7)
+    torch.testing.assert_close(state[some.to(cuda)], few_state, rtol=1e-5, atol=1e-5)
