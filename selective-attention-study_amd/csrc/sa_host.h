@@ -374,13 +374,14 @@ SA_HIDDEN int paged_f32(const PagedLaunch& c);    // sa_paged_f32.hip
 // How a step over a paged cache is launched, and its workspace (byte offsets). Requests with one new token (ones): chunks of
 // keys per workgroup, their partial maxima, sums and outputs, then the new state rows. Requests with several: the selectors'
 // histories (carry), and where the key range is split into spans, their parts.
+constexpr int SHARE_TILES = 8;   // key tiles of a part, at least (PagedLive)
 struct PagedShape {
   bool ones, several;         // kernels that run
   int64_t ld;                 // floats of a history row, or of a new state row
   int chunk;                  // ones: keys per workgroup
   int64_t step_m, step_l, step_o, step_state;
   int nw, hg;                 // several: query tiles of 32 rows per workgroup, heads per wavefront (4: per workgroup, paged_fwd4)
-  int splits, span_tiles;     // key spans, and their 32-key tiles
+  int splits;                 // parts that share a workgroup's key tiles
   int carry_blocks;           // workgroups along the keys of the histories
   bool reach;                 // key tiles without weight are looked for
   int64_t carry, m, o, least, kn;   // (m: (maximum, sum) pairs)
@@ -415,13 +416,11 @@ inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_
     s.hg = es == 2 && D == 64 && per % 4 == 0 && s.nw == 4 ? 4 : es == 2 && D <= 64 && per % 2 == 0 ? 2 : 1;
     const int64_t rows = (int64_t)s.nw * TILE;
     const int64_t tiles = cdiv(max_len, TILE);
-    // workgroups of live query tiles, about; the key range is split where they are no more than half of what the chip runs
-    // at once (one workgroup per CU, two, or eight of one wavefront)
+    // workgroups of live query tiles, about; their key tiles are shared out where they are no more than half of what the chip
+    // runs at once (one workgroup per CU, two, or eight of one wavefront)
     const int64_t workgroups = (s.ones ? cdiv(N, rows) + many / 2 : std::max(cdiv(N, rows), std::min(R, N))) * (H / s.hg);
     const int64_t target = s.hg == 4 ? 256 : s.nw == 4 ? 512 : 2048;
-    const int64_t splits = std::max<int64_t>(1, std::min(target / workgroups, cdiv(tiles, 8)));
-    s.span_tiles = (int)cdiv(tiles, splits);
-    s.splits = (int)cdiv(tiles, s.span_tiles);
+    s.splits = (int)std::max<int64_t>(1, std::min(target / workgroups, cdiv(tiles, SHARE_TILES)));
     s.carry_blocks = (int)std::max<int64_t>(1, std::min(cdiv(tiles, NWAVES), cdiv(8192, R * G)));
     s.carry = take((N / TILE + R) * G * s.ld * 4);
     s.reach = s.nw == 4 && max_len >= REACH_MIN_KEYS;

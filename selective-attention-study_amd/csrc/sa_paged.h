@@ -140,7 +140,7 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedCall& a, int r)
 struct PagedTiles {   // what a workgroup of query tiles has to do
   PagedRequest rq;
   int r, row0;        // request, its first row
-  int kt_lo, kt_hi;   // the key tiles of its span that one of its rows sees
+  int kt_hi;          // the key tiles that one of its rows sees
 };
 
 static __device__ uint4 paged_zero_row;   // what rows without a page read
@@ -589,27 +589,65 @@ __device__ __forceinline__ float least_of(float x) {
 // of its own key, which has no history. Below -REACH_ZERO a weight is an exact fp32 zero (in a part of several spans: once they
 // are joined), and the tile is left out for all of the workgroup's heads together; tiles for which a NaN or an infinity enters
 // the bound stay. A mask in LDS, bit i the span's i-th newest tile; past the mask's end every tile stays.
+//
+// A part of several takes an equal share of the tiles that stay (of some SHARE_TILES at least: a short request's last parts may
+// be empty). Shares of the key range itself would leave the oldest parts idle and the newest ones with all the
+// work: SHAREFIG
 struct PagedLive {
   const uint64_t* mask;   // NULL: every tile
-  int hi, lo;
-  __device__ __forceinline__ int below(int kt) const {   // the next older tile, -1: none
-    int i = hi - kt;
-    if (mask == nullptr) return kt - 1 >= lo ? kt - 1 : -1;
-    while (i < hi - lo) {
-      const int word = i >> 6;
-      if (word >= REACH_MASK_WORDS) return hi - 1 - i;
-      const uint64_t m = uniform64(mask[word]) >> (i & 63);
-      if (m) return hi - 1 - (i + __builtin_ctzll(m));
-      i = (word + 1) << 6;
+  int hi, at, left;       // tiles; the next one's number, counted from the newest; how many to come
+  __device__ __forceinline__ int next() {   // -1: none
+    if (left <= 0) return -1;
+    --left;
+    while (mask != nullptr) {
+      const int word = at >> 6;
+      if (word >= REACH_MASK_WORDS) break;
+      const uint64_t m = uniform64(mask[word]) >> (at & 63);
+      if (m) {
+        at += __builtin_ctzll(m);
+        break;
+      }
+      at = (word + 1) << 6;
     }
-    return -1;
+    return hi - 1 - at++;
+  }
+  // part z of `parts`
+  __device__ __forceinline__ void share(int z, int parts) {
+    const int lane = threadIdx.x & 63, words = min((hi + 63) >> 6, REACH_MASK_WORDS);
+    int marked = 0, two = 0, upto = 0;   // tiles in the mask that stay; in the lane's pair of words; up to its end
+    if (mask != nullptr) {
+      static_assert(REACH_MASK_WORDS <= 128, "two words per lane");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) two += 2 * lane + i < words ? __popcll(mask[2 * lane + i]) : 0;
+      upto = wave_scan_incl(two);
+      marked = __builtin_amdgcn_readlane(upto, 63);
+    }
+    const int total = mask == nullptr ? hi : marked + max(hi - 64 * words, 0);
+    parts = max(min(parts, (total + SHARE_TILES - 1) / SHARE_TILES), 1);
+    if (z >= parts) return;
+    const int first = (int)((int64_t)total * z / parts);
+    left = (int)((int64_t)total * (z + 1) / parts) - first;
+    at = first;
+    if (mask == nullptr) return;
+    at = 64 * words + first - marked;
+    if (first < marked) {
+      const int pair = __popcll(__ballot(upto <= first));
+      int rest = first - (__builtin_amdgcn_readlane(upto, pair) - __builtin_amdgcn_readlane(two, pair)), word = 2 * pair;
+      uint64_t m = uniform64(mask[word]);
+      if (rest >= __popcll(m)) {
+        rest -= __popcll(m);
+        m = uniform64(mask[++word]);
+      }
+      for (; rest > 0; --rest) m &= m - 1;
+      at = 64 * word + __builtin_ctzll(m);
+    }
   }
 };
 
-// Whether any of a sample of the span's tiles has history enough for the search to pay.
-__device__ __forceinline__ bool paged_live_worth(const float* least, int lo, int hi) {
-  if (hi <= lo) return false;
-  const int lane = threadIdx.x & 63, kt = lo + (int)((int64_t)(hi - lo) * lane >> 6);
+// Whether any of a sample of the first `tiles` has history enough for the search to pay.
+__device__ __forceinline__ bool paged_live_worth(const float* least, int tiles) {
+  if (tiles <= 0) return false;
+  const int lane = threadIdx.x & 63, kt = (int)((int64_t)tiles * lane >> 6);
   return __any(least[kt] * REACH_F > REACH_WORTH);
 }
 // The larger of a row's two bounds over a wavefront's 32 rows of a head: largest |q|, least logit (log2 units) of a row's own key.
@@ -651,10 +689,10 @@ __device__ __forceinline__ void paged_live_mask(const PagedCall& a, const PagedT
     }
     qa[g] *= a.scale * REACH_Q;
   }
-  const int words = min((w.kt_hi - w.kt_lo + 63) >> 6, REACH_MASK_WORDS);
+  const int words = min((w.kt_hi + 63) >> 6, REACH_MASK_WORDS);
   for (int word = wave; word < words; word += WAVES) {
     const int kt = w.kt_hi - 1 - (word * 64 + lane);
-    bool live = kt >= w.kt_lo;
+    bool live = kt >= 0;
     if (live && (kt + 1) * TILE <= w.rq.c + w.row0) {
       const float f = least[kt] * REACH_F;
       if (f > REACH_WORTH) {   // (else a key norm may be missing)
@@ -840,11 +878,11 @@ inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
 }
 __device__ __forceinline__ int last_tile_first() { return gridDim.y * gridDim.z - 1 - (blockIdx.z * gridDim.y + blockIdx.y); }
 
-// Workgroup number x (1 << SH rows, numbered as above) and key span z; false: nothing. Rows that no workgroup computes, those
+// Workgroup number x (1 << SH rows, numbered as above), part z; false: nothing. Rows that no workgroup computes, those
 // behind the last request and those of requests left out, become zero here, COLS columns from col0 on, unless the spans are
 // joined afterwards (the join does it).
 template <class P, int SH, int COLS, int THREADS>
-__device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, int span_tiles, int64_t row_elems, int col0, bool joined,
+__device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, int64_t row_elems, int col0, bool joined,
                                             PagedTiles& w) {
   auto clear = [&](int first, int count) {
     typename P::elem* out = static_cast<typename P::elem*>(a.out) + first * row_elems + col0;
@@ -864,9 +902,8 @@ __device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, in
     if (zeros) clear(w.rq.first + w.row0, min(1 << SH, w.rq.n - w.row0));
     return false;
   }
-  w.kt_lo = z * span_tiles;
-  w.kt_hi = min((w.rq.c + min(w.row0 + (1 << SH), w.rq.n) - 1) / TILE + 1, w.kt_lo + span_tiles);
-  return w.kt_lo < w.kt_hi;
+  w.kt_hi = (w.rq.c + min(w.row0 + (1 << SH), w.rq.n) - 1) / TILE + 1;
+  return true;
 }
 
 // A wavefront's results for the request's row `row` (lane = row; o transposed, 4 columns per quarter): the output, or the
@@ -916,7 +953,7 @@ struct FwdLds {
 
 template <class P, int D, int HG, int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) == 2 && D <= 64) ? (HG == 1 ? 3 : 2) : 1)) void paged_fwd_kernel(
-    PagedCall a, const float* __restrict__ carry, int64_t carry_ld, int span_tiles, float* __restrict__ part_ml,
+    PagedCall a, const float* __restrict__ carry, int64_t carry_ld, int splits, float* __restrict__ part_ml,
     float* __restrict__ part_o) {
   typedef PagedTile<P, D> T;
   typedef typename P::elem elem;
@@ -939,9 +976,9 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   const int groups = a.H / HG, x = last_tile_first(), z = blockIdx.x / groups;
   const int hd0 = (blockIdx.x % groups) * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
   PagedTiles w;
-  if (!paged_tiles<P, SH, HG * D, NW * 64>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
+  if (!paged_tiles<P, SH, HG * D, NW * 64>(a, x, z, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
   const PagedRequest& rq = w.rq;
-  const int r = w.r, row0 = w.row0, kt_lo = w.kt_lo, kt_hi = w.kt_hi;
+  const int r = w.r, row0 = w.row0, kt_hi = w.kt_hi;
 
   const int rb0 = row0 + wave * TILE;          // the wavefront's first row
   const int qpos0 = rq.c + rb0;                // and its position
@@ -1019,10 +1056,10 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
     }
   };
 
-  PagedLive tiles{nullptr, kt_hi, kt_lo};
+  PagedLive tiles{nullptr, kt_hi, 0, 0};
   if constexpr (NW > 1) {
     const float* least = a.least + ((int64_t)((rq.first >> 5) + r + (row0 >> 5)) * a.G + g0) * a.reach_ld;
-    if (a.least != nullptr && paged_live_worth(least, kt_lo, min(kt_hi, (rq.c + row0) / TILE))) {
+    if (a.least != nullptr && paged_live_worth(least, (rq.c + row0) / TILE)) {
 #pragma unroll
       for (int g = 0; g < HG; ++g) {
         float bound[2];
@@ -1040,7 +1077,8 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
   }
 
   // the tiles, newest first: cur in the buffers, n1's selector rows too, n2's pages known (-1: none)
-  int cur = tiles.below(kt_hi), n1 = cur >= 0 ? tiles.below(cur) : -1, n2 = n1 >= 0 ? tiles.below(n1) : -1;
+  tiles.share(z, splits);
+  int cur = tiles.next(), n1 = tiles.next(), n2 = tiles.next();
   typename Rows::Place off1[PER], off2[PER];   // of tiles n1 and n2
   int pg[PER];
   {
@@ -1069,7 +1107,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
     rows.places(n2, pg, off2);
     if (n1 >= 0) load_tile(ODD ? sB0 : sB1, off1);
     if (n2 >= 0) load_sel(ODD ? sS1 : sS0, off2);
-    const int n3 = n2 >= 0 ? tiles.below(n2) : -1;
+    const int n3 = tiles.next();
     rows.pages_of(n3, pg);
     const float entry2 = carry_of(n2);
     if (cur < my_end) {
@@ -1164,7 +1202,7 @@ constexpr float PAGED_FWD4_BIG = 16384.f;
 
 template <class P>
 __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const float* __restrict__ carry, int64_t carry_ld,
-                                                          int span_tiles, float* __restrict__ part_ml, float* __restrict__ part_o) {
+                                                          int splits, float* __restrict__ part_ml, float* __restrict__ part_o) {
   constexpr int D = 64, HG = 4, SH = 7, LDF = TILE + 4;
   typedef PagedTile<P, D> T;
   typedef typename P::elem elem;
@@ -1189,9 +1227,8 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
   const int groups = a.H / HG, x = last_tile_first(), z = blockIdx.x / groups;
   const int hd0 = (blockIdx.x % groups) * HG, per = a.H / a.G, g0 = hd0 / per, hsel = g0 * per;
   PagedTiles w;
-  if (!paged_tiles<P, SH, HG * D, 1024>(a, x, z, span_tiles, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
+  if (!paged_tiles<P, SH, HG * D, 1024>(a, x, z, (int64_t)a.H * D, hd0 * D, part_o != nullptr, w)) return;
   const PagedRequest& rq = w.rq;
-  const int kt_lo = w.kt_lo;
 
   const int rb = w.row0 + qt * TILE, qpos0 = rq.c + rb;   // the query tile's first row and its position
   const int end = rb < rq.n ? (qpos0 + TILE - 1) / TILE + 1 : 0;   // tiles that it needs
@@ -1313,10 +1350,10 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
         o[db] = P::mma(T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s), pf[s], o[db]);
   };
 
-  PagedLive tiles{nullptr, w.kt_hi, kt_lo};
+  PagedLive tiles{nullptr, w.kt_hi, 0, 0};
   {
     const float* least = a.least + ((int64_t)((rq.first >> 5) + w.r + (w.row0 >> 5)) * a.G + g0) * a.reach_ld;
-    if (a.least != nullptr && paged_live_worth(least, kt_lo, min(w.kt_hi, (rq.c + w.row0) / TILE))) {
+    if (a.least != nullptr && paged_live_worth(least, (rq.c + w.row0) / TILE)) {
       float bound[2];
       paged_live_bounds<P, D>(a, rq, w.r, rb + n, hd0 + u, qf, bound);
       if (lane == 0) {
@@ -1331,7 +1368,8 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
   }
 
   // the tile of the step (the t-th: t mod 2 names the buffers), and the next two; -1: none
-  int cur = tiles.below(w.kt_hi), n1 = cur >= 0 ? tiles.below(cur) : -1, n2 = n1 >= 0 ? tiles.below(n1) : -1;
+  tiles.share(z, splits);
+  int cur = tiles.next(), n1 = tiles.next(), n2 = tiles.next();
   int turn = (u - qt) & 3;   // tiles until the wavefront's next selection (0: the tile at hand)
   typename Rows::Place at1[1], at2[1];
   int pg[1];
@@ -1361,7 +1399,7 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
     rows.places(n2, pg, at2);
     if (n1 >= 0) load_tile(ODD ? sB0 : sB1, at1);
     if (n2 >= 0) load_sel(ODD ? sS1 : sS0, at2);
-    const int n3 = n2 >= 0 ? tiles.below(n2) : -1;
+    const int n3 = tiles.next();
     rows.pages_of(n3, pg);
     const float entry2 = carry_of(n2);
     if (turn == 0) {
@@ -1388,10 +1426,9 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
   paged_write<P, D>(a, w, rb + n, hd0 + u, z, mu, l, o, h, part_ml, part_o);
 }
 
-// The spans of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z over the spans that begin at
-// or before the query. A workgroup per row, a thread per four output columns.
+// The parts of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z (a part of no key: l_z = 0). A workgroup per row, a thread per four output columns.
 template <class P, int D>
-__global__ __launch_bounds__(NTHREADS) void paged_join_kernel(PagedCall a, int span_tiles, const float* __restrict__ part_ml,
+__global__ __launch_bounds__(NTHREADS) void paged_join_kernel(PagedCall a, int splits, const float* __restrict__ part_ml,
                                                               const float* __restrict__ part_o) {
   typedef typename P::elem elem;
   const int row = blockIdx.x;
@@ -1399,7 +1436,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_join_kernel(PagedCall a, int s
   const PagedRequest rq = paged_request(a, r);
   const bool live = rq.live && row >= rq.first && row < rq.first + rq.n;
   if (live && a.ones && rq.n == 1) return;   // (paged_step_join's)
-  const int spans = live ? (rq.c + row - rq.first) / TILE / span_tiles + 1 : 0;
+  const int spans = live ? splits : 0;
   elem* out = static_cast<elem*>(a.out) + (int64_t)row * a.H * D;
   for (int i = threadIdx.x; i < a.H * (D / 4); i += NTHREADS) {
     const int hd = i / (D / 4);
@@ -1704,7 +1741,7 @@ template <class P, int D, int HG, int NW, bool WHOLE>
 void launch_paged_fwd(const PagedCall& a, const PagedShape& s, const float* carry, float* ml, float* o, hipStream_t st) {
   const int64_t tiles = (int64_t)(a.N >> (NW == 4 ? 7 : 5)) + a.R;
   hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE>), tile_grid((int64_t)a.H / HG * s.splits, tiles), dim3(NW * 64), 0, st,
-                     a, carry, s.ld, s.span_tiles, ml, o);
+                     a, carry, s.ld, s.splits, ml, o);
 }
 
 template <class P, int D>
@@ -1748,7 +1785,7 @@ int paged_launch(const PagedLaunch& c) {
     if constexpr (sizeof(typename P::elem) == 2 && D == 64) {
       if (s.hg == 4)
         hipLaunchKernelGGL((paged_fwd4_kernel<P>), tile_grid((int64_t)a.H / 4 * s.splits, (a.N >> 7) + a.R), dim3(1024), 0, c.st, a,
-                           carry, s.ld, s.span_tiles, ml, o);
+                           carry, s.ld, s.splits, ml, o);
     }
     if constexpr (sizeof(typename P::elem) == 2 && D <= 64) {
       if (s.hg == 2) {
@@ -1767,7 +1804,7 @@ int paged_launch(const PagedLaunch& c) {
     }
   }
   if (s.splits > 1)
-    hipLaunchKernelGGL((paged_join_kernel<P, D>), dim3((unsigned)a.N), dim3(NTHREADS), 0, c.st, a, s.span_tiles, ml, o);
+    hipLaunchKernelGGL((paged_join_kernel<P, D>), dim3((unsigned)a.N), dim3(NTHREADS), 0, c.st, a, s.splits, ml, o);
   return launch_status();
 }
 
