@@ -383,8 +383,9 @@ struct PagedShape {
   int nw, hg;                 // several: query tiles of 32 rows per workgroup, heads per wavefront (4: per workgroup, paged_fwd4)
   int splits;                 // parts that share a workgroup's key tiles
   int carry_blocks;           // workgroups along the keys of the histories
+  int segments, seg_tiles;    // and along the query tiles
   bool reach;                 // key tiles without weight are looked for
-  int64_t carry, m, o, least, kn;   // (m: (maximum, sum) pairs)
+  int64_t carry, totals, m, o, least, kn;   // (m: (maximum, sum) pairs)
   int64_t total;
 };
 inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_t D, int64_t es, int64_t max_new, int64_t max_len) {
@@ -423,6 +424,14 @@ inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_
     s.splits = (int)std::max<int64_t>(1, std::min(target / workgroups, cdiv(tiles, SHARE_TILES)));
     s.carry_blocks = (int)std::max<int64_t>(1, std::min(cdiv(tiles, NWAVES), cdiv(8192, R * G)));
     s.carry = take((N / TILE + R) * G * s.ld * 4);
+    // The walk along the query tiles is cut where it leaves half of the chip idle: into two workgroups per CU, segments
+    // of 32 tiles at least. A prompt of 16384 tokens: its histories 200 -> 100 us (two segments: 139). Where the chip is full the
+    // second kernel costs more than the first gains: a chunk of 4096 at 32768 keys 69 -> 75 us, of segments of 8 tiles 27 -> 28.
+    const int64_t steps = cdiv(max_new, TILE), walks = R * G * s.carry_blocks;
+    const int64_t want = walks <= 128 ? std::min(512 / walks, steps / 32) : 1;
+    s.seg_tiles = (int)align_up(cdiv(steps, std::max<int64_t>(want, 1)), 4);
+    s.segments = (int)cdiv(steps, s.seg_tiles);
+    if (s.segments > 1) s.totals = take(R * G * s.segments * s.ld * 4);
     s.reach = s.nw == 4 && max_len >= REACH_MIN_KEYS;
     if (s.reach) {
       s.least = take((N / TILE + R) * G * (s.ld / TILE) * 4);

@@ -111,6 +111,8 @@ struct PagedCall {
   int64_t q_token, q_head, table_ld, state_ld;
   int R, N, H, G, pages, pshift;
   int max_new, max_len;
+  float* totals;   // (R, G, segments, ld) what each segment of query tiles adds to the histories; of the first, with the state
+  int segments, seg_tiles;   // of query tiles, whose histories are made independently (seg_tiles a multiple of four)
   int ones;   // several tokens: requests with one new token are left to the single-token kernels
   float *least, *kn;   // per key tile: least history on entry to a query tile, largest key norm; NULL: every tile is computed
   int64_t reach_ld;
@@ -707,6 +709,45 @@ __device__ __forceinline__ void paged_live_mask(const PagedCall& a, const PagedT
   }
 }
 
+// The key norms of key tile kb, by a wavefront: `run` each key's history after the step (lane: key lane & 31).
+template <class P, int D>
+__device__ __forceinline__ void paged_key_norms(const PagedCall& a, const PagedRequest& rq, int r, int g, int kb, float run) {
+  typedef typename P::elem elem;
+  constexpr int NS = PagedTile<P, D>::NS;
+  const int lane = threadIdx.x & 63, h = lane >> 5, j = kb * TILE + (lane & 31), hd = g * (a.H / a.G);
+  if (a.least == nullptr || !(least_of(j < rq.t ? run : INFINITY) * REACH_F > REACH_WORTH)) return;
+  const int pg = j < rq.t ? a.table[r * a.table_ld + (j >> a.pshift)] : -1;
+  const bool ok = (uint32_t)pg < (uint32_t)a.pages;
+  constexpr int HB = NS <= 4 ? 4 : NS == 8 ? 2 : 1;   // heads whose rows are on their way at a time
+  for (int head = hd; head < hd + a.H / a.G; head += HB) {
+    u32x4 kr[HB][NS], vr[HB][NS];
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+      const int hb = min(head + b, hd + a.H / a.G - 1);
+      const int64_t at = ((((int64_t)(ok ? pg : 0) * a.H + hb) << a.pshift) + (j & ((1 << a.pshift) - 1))) * D + h * P::EPC;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        kr[b][s] = *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.k_pages) + at + 2 * s * P::EPC);
+        vr[b][s] = *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.v_pages) + at + 2 * s * P::EPC);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+      float kk = 0.f, vv = 0.f;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        kk = chunk_dot<P>(kr[b][s], kr[b][s], kk);
+        vv = chunk_dot<P>(vr[b][s], vr[b][s], vv);
+      }
+      const Halves k2 = halves(kk), v2 = halves(vv);
+      // (a row without a page is zeros)
+      const float x = !ok ? 0.f : (k2.lo + k2.hi < REACH_NORM2 && v2.lo + v2.hi < REACH_NORM2) ? k2.lo + k2.hi : INFINITY;
+      const float mx = -least_of(-x);
+      if (lane == 0 && head + b < hd + a.H / a.G) a.kn[((int64_t)r * a.H + head + b) * a.reach_ld + kb] = sqrtf(mx);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // The selectors' histories of a step of several tokens: carry[tile][g][j], what key j has received before the
 // tile's first query, and the state after the step. A wavefront owns 32 keys of one selector (rows in registers) and
@@ -730,11 +771,11 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
   // no more than 2 PER + 3 (U + 1) newer operations run.
   __shared__ __attribute__((aligned(16))) char sQ0[U * T::BYTES], sQ1[U * T::BYTES], sQ2[U * T::BYTES], sQ3[U * T::BYTES];
   const int lane = threadIdx.x & 63, wave = wave_id(), n = lane & 31, h = lane >> 5;
-  const int r = blockIdx.z, g = blockIdx.y;
+  const int r = blockIdx.z, g = blockIdx.y, seg = blockIdx.x % a.segments;
   const PagedRequest rq = paged_request(a, r);
   if (!rq.live || (a.ones && rq.n == 1)) return;
   const int hd = g * (a.H / a.G);
-  const int nkb = (rq.t + TILE - 1) / TILE, ntile = (rq.n + TILE - 1) / TILE;
+  const int nkb = (rq.t + TILE - 1) / TILE, last = min((rq.n + TILE - 1) / TILE, (seg + 1) * a.seg_tiles);   // (its last query tile + 1)
   const elem* q = static_cast<const elem*>(a.q) + rq.first * a.q_token + hd * a.q_head;
   const int* trow = a.table + r * a.table_ld;
   float* state = a.selected + ((int64_t)r * a.G + g) * a.state_ld;
@@ -753,13 +794,16 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
     for (int i = 0; i < PER; ++i)
       b2l16(reinterpret_cast<const char*>(q + rb * TILE * a.q_token), left * (int)a.q_token * T::ES, buf + 1024 * (wave + NWAVES * i), off[i]);
   };
-  for (int kb0 = blockIdx.x * NWAVES; kb0 < nkb; kb0 += gridDim.x * NWAVES) {
+  for (int kb0 = blockIdx.x / a.segments * NWAVES; kb0 < nkb; kb0 += gridDim.x / a.segments * NWAVES) {
     const int kb = kb0 + wave, j = kb * TILE + n;
     // tiles before this end before the workgroup's first key
-    int rb = (max(kb0 * TILE - rq.c, 0) / TILE) & ~3;   // (every fourth one begins a step)
-    load_q(rb, sQ0);
-    load_q(rb + U, sQ1);
-    load_q(rb + 2 * U, sQ2);
+    int rb = max((max(kb0 * TILE - rq.c, 0) / TILE) & ~3, seg * a.seg_tiles);   // (every fourth one begins a step)
+    const bool any = rb < last;
+    if (any) {
+      load_q(rb, sQ0);
+      load_q(rb + U, sQ1);
+      load_q(rb + 2 * U, sQ2);
+    }
     u32x4 kf[NS];
     {
       const int pg = j < rq.t ? trow[j >> a.pshift] : -1;
@@ -770,7 +814,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
       for (int s = 0; s < NS; ++s)
         kf[s] = ok ? *reinterpret_cast<const u32x4*>(k + (2 * s + h) * P::EPC) : u32x4{0, 0, 0, 0};
     }
-    float run = j < rq.c ? state[j] : 0.f;
+    float run = j < rq.c && seg == 0 ? state[j] : 0.f;
     const int64_t lplane = a.G * a.reach_ld;
     float* least = a.least + ((int64_t)((rq.first >> 5) + r) * a.G + g) * a.reach_ld + kb;   // (not used without a.least)
     const uint32_t end = (uint32_t)rq.t * 4, own = h == 0 && j < rq.t ? (uint32_t)j * 4 : end;   // byte offset of the lane's key in a row of histories
@@ -795,13 +839,13 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
           sum[u] = block_selection_sum(acc[u], false, j >= a.exempt ? j - qbase - u * TILE - 4 * h : 32, a.scale);
       }
       {
-        const bool kept = a.least != nullptr && (rb & 3) == 0 && rb < ntile && kb < nkb;
+        const bool kept = a.least != nullptr && seg == 0 && (rb & 3) == 0 && rb < last && kb < nkb;
         const float mn = kept ? least_of(j >= rq.t ? INFINITY : run == run ? run : -INFINITY) : 0.f;   // (a NaN keeps the tile)
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mn), rsrc(least + rb * lplane, kept ? 4 : 0), lane * 4, 0, 0);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {   // (every lane stores, past the row's end where it has no key or the tile is none)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(run), rsrc(cr + (rb + u) * plane, rb + u < ntile ? end : 0), own, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(run), rsrc(cr + (rb + u) * plane, rb + u < last ? end : 0), own, 0, 0);
         run += sum[u];
       }
       rb += U;
@@ -810,50 +854,72 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, floa
     };
     wait_loads();
     __syncthreads();
-    while (true) {
+    while (any) {
       step(sQ0, sQ3);
-      if (rb >= ntile) break;
+      if (rb >= last) break;
       step(sQ1, sQ0);
-      if (rb >= ntile) break;
+      if (rb >= last) break;
       step(sQ2, sQ1);
-      if (rb >= ntile) break;
+      if (rb >= last) break;
       step(sQ3, sQ2);
-      if (rb >= ntile) break;
+      if (rb >= last) break;
     }
     wait_loads();   // nothing on its way into LDS when the workgroup ends or takes its next keys
     __syncthreads();
-    if (h == 0 && j < rq.t) state[j] = run;
-    if (a.least != nullptr && kb < nkb && least_of(j < rq.t ? run : INFINITY) * REACH_F > REACH_WORTH) {
-      const int pg = j < rq.t ? trow[j >> a.pshift] : -1;
-      const bool ok = (uint32_t)pg < (uint32_t)a.pages;
-      constexpr int HB = NS <= 4 ? 4 : NS == 8 ? 2 : 1;   // heads whose rows are on their way at a time
-      for (int head = hd; head < hd + a.H / a.G; head += HB) {
-        u32x4 kr[HB][NS], vr[HB][NS];
+    if (a.segments == 1) {
+      if (h == 0 && j < rq.t) state[j] = run;
+      if (kb < nkb) paged_key_norms<P, D>(a, rq, r, g, kb, run);
+    } else if (h == 0 && j < rq.t) {
+      a.totals[(((int64_t)r * a.G + g) * a.segments + seg) * carry_ld + j] = run;
+    }
+  }
+}
+
+// The histories of the segments after the first, which begin at zero, raised by what the segments before have added; the
+// state, and what paged_carry leaves to do of least histories and key norms. Workgroup: 256 keys, a thread each, of SEG_PART
+// query tiles (the first two of the grid's y: the state and the norms).
+constexpr int SEG_PART = 16;
+template <class P, int D>
+__global__ __launch_bounds__(NTHREADS) void paged_carry_join_kernel(PagedCall a, float* __restrict__ carry, int64_t carry_ld) {
+  const int lane = threadIdx.x & 63, r = blockIdx.z / a.G, g = blockIdx.z % a.G, j = blockIdx.x * NTHREADS + threadIdx.x;
+  const PagedRequest rq = paged_request(a, r);
+  if (!rq.live || (a.ones && rq.n == 1) || (int)blockIdx.x * NTHREADS >= rq.t) return;
+  const float* totals = a.totals + ((int64_t)r * a.G + g) * a.segments * carry_ld + min(j, rq.t - 1);
+  auto before = [&](int seg) {
+    float sum = 0.f;
+    for (int i = 0; i < seg; ++i) sum += totals[i * carry_ld];
+    return sum;
+  };
+  if (blockIdx.y < 2) {   // one of every wavefront's two key tiles
+    const int kb = (j >> 6) * 2 + blockIdx.y;
+    const float run = before(a.segments), x = __shfl(run, (lane & 31) + 32 * blockIdx.y);
+    if (lane >> 5 == blockIdx.y && j < rq.t) a.selected[((int64_t)r * a.G + g) * a.state_ld + j] = run;
+    if (kb * TILE < rq.t) paged_key_norms<P, D>(a, rq, r, g, kb, x);
+    return;
+  }
+  const int rb0 = a.seg_tiles + ((int)blockIdx.y - 2) * SEG_PART, ntile = (rq.n + TILE - 1) / TILE;
+  // (tiles before a key's hold nothing of it)
+  const int first = max(rb0, (max((int)blockIdx.x * NTHREADS - rq.c, 0) / TILE) & ~3), last = min(rb0 + SEG_PART, ntile);
+  if (first >= last) return;
+  int seg = first / a.seg_tiles;
+  float base = before(seg);
+  const int64_t plane = a.G * carry_ld;
+  float* cr = carry + (int64_t)((rq.first >> 5) + r) * plane + g * carry_ld + min(j, rq.t - 1);
+  for (int rb = first; rb < last; rb += 4) {   // (segments begin at multiples of four)
+    if (rb >= (seg + 1) * a.seg_tiles) base += totals[seg++ * carry_ld];
+    float x[4];
 #pragma unroll
-        for (int b = 0; b < HB; ++b) {
-          const int hb = min(head + b, hd + a.H / a.G - 1);
-          const int64_t at = ((((int64_t)(ok ? pg : 0) * a.H + hb) << a.pshift) + (j & ((1 << a.pshift) - 1))) * D + h * P::EPC;
+    for (int u = 0; u < 4; ++u) x[u] = cr[min(rb + u, last - 1) * plane];
 #pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            kr[b][s] = *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.k_pages) + at + 2 * s * P::EPC);
-            vr[b][s] = *reinterpret_cast<const u32x4*>(static_cast<const elem*>(a.v_pages) + at + 2 * s * P::EPC);
-          }
-        }
+    for (int u = 0; u < 4; ++u) x[u] += base;
 #pragma unroll
-        for (int b = 0; b < HB; ++b) {
-          float kk = 0.f, vv = 0.f;
-#pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            kk = chunk_dot<P>(kr[b][s], kr[b][s], kk);
-            vv = chunk_dot<P>(vr[b][s], vr[b][s], vv);
-          }
-          const Halves k2 = halves(kk), v2 = halves(vv);
-          // (a row without a page is zeros)
-          const float x = !ok ? 0.f : (k2.lo + k2.hi < REACH_NORM2 && v2.lo + v2.hi < REACH_NORM2) ? k2.lo + k2.hi : INFINITY;
-          const float mx = -least_of(-x);
-          if (lane == 0 && head + b < hd + a.H / a.G) a.kn[((int64_t)r * a.H + head + b) * a.reach_ld + kb] = sqrtf(mx);
-        }
-      }
+    for (int u = 0; u < 4; ++u)
+      if (rb + u < last && j < rq.t) cr[(rb + u) * plane] = x[u];
+    if (a.least != nullptr) {
+      const float y = j >= rq.t ? INFINITY : x[0] == x[0] ? x[0] : -INFINITY;
+      float* least = a.least + ((int64_t)((rq.first >> 5) + r + rb) * a.G + g) * a.reach_ld;
+      const float lo = least_of(lane < 32 ? y : INFINITY), hi = least_of(lane < 32 ? INFINITY : y);
+      if ((lane & 31) == 0 && j < rq.t) least[j / TILE] = lane < 32 ? lo : hi;
     }
   }
 }
@@ -1773,11 +1839,18 @@ int paged_launch(const PagedLaunch& c) {
     a.kn = at(s.kn);
     a.reach_ld = s.ld / TILE;
   }
+  a.segments = s.segments;
+  a.seg_tiles = s.seg_tiles;
+  a.totals = s.segments > 1 ? at(s.totals) : nullptr;
   float *carry = at(s.carry), *ml = s.splits > 1 ? at(s.m) : nullptr, *o = s.splits > 1 ? at(s.o) : nullptr;
   {
     TimedLaunch timed(SA_KERNEL_SELECTION, c.st);
-    hipLaunchKernelGGL((paged_carry_kernel<P, D>), dim3((unsigned)s.carry_blocks, (unsigned)a.G, (unsigned)a.R), dim3(NTHREADS), 0, c.st,
-                       a, carry, s.ld);
+    hipLaunchKernelGGL((paged_carry_kernel<P, D>), dim3((unsigned)(s.carry_blocks * s.segments), (unsigned)a.G, (unsigned)a.R),
+                       dim3(NTHREADS), 0, c.st, a, carry, s.ld);
+    if (s.segments > 1)
+      hipLaunchKernelGGL((paged_carry_join_kernel<P, D>), dim3((unsigned)cdiv(a.max_len, NTHREADS),
+                         (unsigned)(2 + cdiv(cdiv(a.max_new, TILE) - s.seg_tiles, SEG_PART)), (unsigned)(a.R * a.G)), dim3(NTHREADS), 0,
+                         c.st, a, carry, s.ld);
   }
   {
     TimedLaunch timed(SA_KERNEL_FORWARD, c.st);

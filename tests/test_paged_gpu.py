@@ -458,3 +458,14 @@ def test_more_query_tiles_than_a_grid_dimension(cuda):
     # output; states of sums of sixteen fp32 products
     torch.testing.assert_close(out[at].float(), few.float(), rtol=2**-7, atol=2**-7)
     torch.testing.assert_close(state[some.to(cuda)], few_state, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("head_dim,heads,groups,exempt,rate", [(64, 4, 1, 1, 0.0), (32, 2, 2, 40, 0.1), (128, 1, 1, 1, 0.1)])
+def test_long_prompts_whose_histories_are_made_in_segments(cuda, dtype, head_dim, heads, groups, exempt, rate):
+    """Some three thousand queries of one request, few others: the walk along the queries is cut, at tiles that neither begin nor
+    end a request; a request that ends within the first segment, and one token."""
+    step = outgrown(Step([70, 300, 5], [2601, 1033, 1], heads=heads, head_dim=head_dim, groups=groups, dtype=dtype, exempt=exempt, seed=9),
+                    rate)
+    out, state = attend(step, cuda)
+    check(out, state, step, ROUNDED[dtype])
