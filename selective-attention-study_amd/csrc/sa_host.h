@@ -396,7 +396,7 @@ inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_
   // At least `many` of the requests have several new tokens, if N rows are shared out with at most max_new each; the
   // others may have one. A query tile for one row sweeps its keys at a fraction of HBM's rate, so where the others' keys can
   // be many, requests with one token run the kernels that stream them (a mixed batch of 40 requests at up to 8000 positions, 36
-  // of them generating, 16 heads: 337 -> 215 us); where they cannot, two more launches that find nothing would cost 7 us.
+  // of them generating, 16 heads: 337 -> 267 us); where they cannot, two more launches that find nothing would cost 7 us.
   const int64_t many = s.several ? std::min(cdiv(std::max<int64_t>(N - R, 0), max_new - 1), R) : 0;
   s.ones = !s.several || (R - many) * max_len * H >= ((int64_t)1 << 20);
   s.ld = align_up(max_len, TILE);
@@ -418,7 +418,8 @@ inline PagedShape paged_shape(int64_t R, int64_t N, int64_t H, int64_t G, int64_
     const int64_t rows = (int64_t)s.nw * TILE;
     const int64_t tiles = cdiv(max_len, TILE);
     // workgroups of live query tiles, about; their key tiles are shared out where they are no more than half of what the chip
-    // runs at once (one workgroup per CU, two, or eight of one wavefront)
+    // runs at once (one workgroup per CU, two, or eight of one wavefront): 128 of them over 1024 tiles, us, alone 1387, two
+    // parts each 797, four 806; 288 over up to 63 tiles alone 102, two parts 129.
     const int64_t workgroups = (s.ones ? cdiv(N, rows) + many / 2 : std::max(cdiv(N, rows), std::min(R, N))) * (H / s.hg);
     const int64_t target = s.hg == 4 ? 256 : s.nw == 4 ? 512 : 2048;
     s.splits = (int)std::max<int64_t>(1, std::min(target / workgroups, cdiv(tiles, SHARE_TILES)));

@@ -14,8 +14,9 @@
 //   page_plan, page_slots   the step's tables from the requests' lengths
 //   paged_append            new rows into the pages
 //   paged_carry             n > 1: each selector's history on entry to every 32-query tile, and the new state
-//   paged_fwd               n > 1: a wavefront's 32 queries of one or two heads over the key tiles of a span
-//   paged_join              the spans' partial results of a query joined
+//   paged_carry_join        the same where the queries are walked in segments: the segments' histories joined
+//   paged_fwd, paged_fwd4   n > 1: a wavefront's 32 queries of one or two heads over the key tiles, or a part of them
+//   paged_join              the parts of a query joined
 //   paged_step, paged_step_join    n = 1: the cache read once in fp32 arithmetic, split over workgroups
 
 #pragma once
@@ -149,10 +150,12 @@ static __device__ uint4 paged_zero_row;   // what rows without a page read
 
 // ---------------------------------------------------------------------------------------------
 // The step's tables. One workgroup (a step's scans run over the requests, some hundreds); bound by its latency: two block
-// scans and one round trip each for the lengths, the stack and the table. A step of 8 requests takes 5 us on the GPU.
+// scans and one round trip each for the lengths, the stack and the table. A step of 8 requests takes 2.9 us.
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_WAVES = PLAN_THREADS / 64;
-constexpr int PLAN_SLOTS = 4096;   // tokens up to which the same workgroup makes the slot map
+// Tokens up to which the same workgroup makes the slot map (8 requests, us, against a second kernel: 5.7 and 6.7 at 2048
+// tokens, 7.0 and 6.6 at 4096, 15.8 and 6.6 at 16384).
+constexpr int PLAN_SLOTS = 2048;
 constexpr int PLAN_BATCH = 8;      // loads of a table row under way at a time
 
 struct PlanCall {
@@ -586,15 +589,17 @@ __device__ __forceinline__ float least_of(float x) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// The key tiles of a workgroup's span that its rows can give weight to (as find_reach for the contiguous cache): for a tile
+// The key tiles that a workgroup's rows can give weight to (as find_reach for the contiguous cache): for a tile
 // before the rows, log2 weight <= s log2e |q| max |k| - log2e (least F) - (row maximum), the row maximum at least the row's logit
-// of its own key, which has no history. Below -REACH_ZERO a weight is an exact fp32 zero (in a part of several spans: once they
+// of its own key, which has no history. Below -REACH_ZERO a weight is an exact fp32 zero (in one part of several: once they
 // are joined), and the tile is left out for all of the workgroup's heads together; tiles for which a NaN or an infinity enters
-// the bound stay. A mask in LDS, bit i the span's i-th newest tile; past the mask's end every tile stays.
+// the bound stay. A mask in LDS, bit i the i-th newest tile; past the mask's end every tile stays. A chunk of
+// 4096 queries at 32768 keys, 16 heads, of N(0,1) inputs: 849 us -> 133; where the histories leave the oldest fifth without
+// weight 800 -> 770; where they are too small everywhere 98 -> 104 (prompts of 60 to 2000 tokens), the rows and norms for nothing.
 //
 // A part of several takes an equal share of the tiles that stay (of some SHARE_TILES at least: a short request's last parts may
-// be empty). Shares of the key range itself would leave the oldest parts idle and the newest ones with all the
-// work: SHAREFIG
+// be empty). Shares of the key range itself leave the oldest part idle where tiles are left out there, and the last ones of short requests:
+// the chunk above 824 -> 772 us, eight requests of up to 4000 keys 68 -> 63.
 struct PagedLive {
   const uint64_t* mask;   // NULL: every tile
   int hi, at, left;       // tiles; the next one's number, counted from the newest; how many to come
@@ -754,12 +759,12 @@ __device__ __forceinline__ void paged_key_norms(const PagedCall& a, const PagedR
 // its workgroup walks the request's query tiles, as sel_carry64_kernel does, U tiles at a time: a step rarely has keys
 // enough for more than one wavefront per SIMD, so the walk is bound by the latency of its own instructions and the U
 // products and sums are kept independent; the rows are loaded into LDS three steps ahead, once for the workgroup. At 4096
-// queries on 32768 keys (us): 48; one tile at a time from the L2 105, four at a time 64, through LDS one step ahead 55. Rows
-// of keys that no query of a tile sees hold no history: the forward masks those keys.
+// queries on 32768 keys (us, histories and state alone): 48; one tile at a time from the L2 105, four at a time 64, through LDS
+// one step ahead 55. Rows of keys that no query of a tile sees hold no history: the forward masks those keys.
 //
 // With a.least, also what the forward needs to leave out key tiles without weight (PagedLive): each key tile's least history
 // on entry to every fourth query tile, and, of key tiles whose least history at the end makes it possible, the largest
-// |k| of every head of the group (infinity where a key or a value is not finite, or a product could overflow).
+// |k| of every head of the group (infinity where a key or a value is not finite, or a product could overflow): 69 us, of that 16 to read the keys and values of 16 heads.
 template <class P, int D>
 __global__ __launch_bounds__(NTHREADS) void paged_carry_kernel(PagedCall a, float* __restrict__ carry, int64_t carry_ld) {
   typedef PagedTile<P, D> T;
@@ -1492,34 +1497,55 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
   paged_write<P, D>(a, w, rb + n, hd0 + u, z, mu, l, o, h, part_ml, part_o);
 }
 
-// The parts of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z (a part of no key: l_z = 0). A workgroup per row, a thread per four output columns.
+// The parts of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z (a part of no key: l_z = 0). A
+// workgroup per row, a thread per four output columns; bound by latency, so four parts are loaded at a time, the first
+// while the row's request is looked for (up to eight parts of 8 rows each of eight requests: 8.6 us a part at a
+// time, 5.0 so).
 template <class P, int D>
 __global__ __launch_bounds__(NTHREADS) void paged_join_kernel(PagedCall a, int splits, const float* __restrict__ part_ml,
                                                               const float* __restrict__ part_o) {
   typedef typename P::elem elem;
-  const int row = blockIdx.x;
+  constexpr int U = 4;
+  const int row = blockIdx.x, items = a.H * (D / 4);
+  float2 ml[U];
+  float4 x[U];
+  auto load = [&](int i, int z0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (z0 + u >= splits) continue;
+      const int64_t at = ((int64_t)(z0 + u) * a.N + row) * a.H + i / (D / 4);
+      ml[u] = *reinterpret_cast<const float2*>(part_ml + 2 * at);
+      x[u] = *reinterpret_cast<const float4*>(part_o + at * D + 4 * (i % (D / 4)));
+    }
+  };
+  if ((int)threadIdx.x < items) load(threadIdx.x, 0);
   const int r = find_request<true>(a.starts, a.R, row, 0);
   const PagedRequest rq = paged_request(a, r);
   const bool live = rq.live && row >= rq.first && row < rq.first + rq.n;
   if (live && a.ones && rq.n == 1) return;   // (paged_step_join's)
-  const int spans = live ? splits : 0;
   elem* out = static_cast<elem*>(a.out) + (int64_t)row * a.H * D;
-  for (int i = threadIdx.x; i < a.H * (D / 4); i += NTHREADS) {
-    const int hd = i / (D / 4);
-    float M = -INFINITY;
-    for (int z = 0; z < spans; ++z) M = fmaxf(M, part_ml[2 * (((int64_t)z * a.N + row) * a.H + hd)]);
-    float l = 0.f;
+  for (int i = threadIdx.x; i < items; i += NTHREADS) {
+    float M = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int z = 0; z < spans; ++z) {
-      const int64_t at = ((int64_t)z * a.N + row) * a.H + hd;
-      const float2 ml = *reinterpret_cast<const float2*>(part_ml + 2 * at);
-      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-      const float4 x = *reinterpret_cast<const float4*>(part_o + at * D + 4 * (i % (D / 4)));
-      l = fmaf(w, ml.y, l);
-      acc.x = fmaf(w, x.x, acc.x);
-      acc.y = fmaf(w, x.y, acc.y);
-      acc.z = fmaf(w, x.z, acc.z);
-      acc.w = fmaf(w, x.w, acc.w);
+    for (int z0 = 0; live && z0 < splits; z0 += U) {
+      if (z0 > 0 || i >= NTHREADS) load(i, z0);
+      float m_new = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) m_new = fmaxf(m_new, z0 + u < splits ? ml[u].x : -INFINITY);
+      const float alpha = M == -INFINITY ? 0.f : fast_exp2(M - m_new);
+      M = m_new;
+      l *= alpha;
+      acc = make_float4(acc.x * alpha, acc.y * alpha, acc.z * alpha, acc.w * alpha);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (z0 + u >= splits) continue;
+        const float w = ml[u].x == -INFINITY ? 0.f : fast_exp2(ml[u].x - M);
+        l = fmaf(w, ml[u].y, l);
+        acc.x = fmaf(w, x[u].x, acc.x);
+        acc.y = fmaf(w, x[u].y, acc.y);
+        acc.z = fmaf(w, x[u].z, acc.z);
+        acc.w = fmaf(w, x[u].w, acc.w);
+      }
     }
     const float inv = live ? 1.f / l : 0.f;
     const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
