@@ -599,7 +599,7 @@ __device__ __forceinline__ float least_of(float x) {
 //
 // A part of several takes an equal share of the tiles that stay (of some SHARE_TILES at least: a short request's last parts may
 // be empty). Shares of the key range itself leave the oldest part idle where tiles are left out there, and the last ones of short requests:
-// the chunk above 824 -> 772 us, eight requests of up to 4000 keys 68 -> 63.
+// the chunk above 824 -> 772 us, chunks of 300 to 700 queries of three requests, each of 8 heads selecting, 68 -> 63.
 struct PagedLive {
   const uint64_t* mask;   // NULL: every tile
   int hi, at, left;       // tiles; the next one's number, counted from the newest; how many to come
@@ -1266,7 +1266,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
 // weights are taken against the reference mu of the tiles before, and only where a row's sum of them over a tile
 // passes 2^14 (or a row has no reference yet) is the maximum looked for, mu moved and the tile's weights taken again.
 // Any reference within 2^14 of the maximum gives the same weights to rounding, fp16's range included. At 4096 queries on
-// 32768 keys, 16 heads: 0.80 ms (644 TFLOP/s of the two products), paged_fwd_kernel 1.04; with the selection after the products 0.91,
+// 32768 keys, 16 heads: 0.80 ms (644 TFLOP/s of the two products), paged_fwd_kernel 1.04 (every tile computed); with the selection after the products 0.91,
 // with eight wavefronts of two query tiles each 0.97 (0.91). What is left over is each step's common start and end: its LDS reads
 // at once (0.46 ms without selection, value products and loads), and the wait for its last wavefront.
 constexpr float PAGED_FWD4_BIG = 16384.f;
@@ -1499,8 +1499,7 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
 
 // The parts of every query joined: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z (a part of no key: l_z = 0). A
 // workgroup per row, a thread per four output columns; bound by latency, so four parts are loaded at a time, the first
-// while the row's request is looked for (up to eight parts of 8 rows each of eight requests: 8.6 us a part at a
-// time, 5.0 so).
+// while the row's request is looked for (twelve parts of 2 to 9 rows of 16 requests: 8.6 us a part at a time, 5.0 so).
 template <class P, int D>
 __global__ __launch_bounds__(NTHREADS) void paged_join_kernel(PagedCall a, int splits, const float* __restrict__ part_ml,
                                                               const float* __restrict__ part_o) {
