@@ -244,7 +244,8 @@ int sa_decode_noalloc(const void* q, const void* k, const void* v, float* out, f
  * A paged cache, for batches of requests of different lengths (no counterpart in the reference). k_pages and
  * v_pages are (pages, heads, page_size, head_dim), contiguous, page_size a power of two from 8 on; position j of
  * request r sits in page table[r][j / page_size], row j % page_size. Lengths, tables and counts are int32 on the
- * device: no entry point reads them on the host. head_dim 16, 32, 64 or 128; up to 65535 requests, 2^24 - 1 tokens.
+ * device: no entry point reads them on the host. head_dim 16, 32, 64 or 128; up to 65535 requests, 2^24 - 1 tokens,
+ * and what a launch of 2^32 threads holds.
  *
  * sa_page_plan: the tables of one step, from the requests' lengths. Request r has cached[r] positions in the cache
  * and gets new_tokens[r] new ones (0: none; negative counts as 0). free_pages[taken[0] .. pool) are the free pages,

@@ -78,10 +78,9 @@ struct PagedF32 {
 // ---------------------------------------------------------------------------------------------
 // Requests of a ragged batch. Tiles of 1 << sh query rows are numbered without a table of their own: request r's
 // tiles take the numbers from (starts[r] >> sh) + r on, as many as it can need (a request of n rows covers at most
-// ((starts[r] + n) >> sh) - (starts[r] >> sh) + 1 tiles), so N rows of R requests have (N >> sh) + R numbers. sh = 31
-// numbers the requests themselves, sh = 0 with `plain` the rows.
+// ((starts[r] + n) >> sh) - (starts[r] >> sh) + 1 tiles), so N rows of R requests have (N >> sh) + R numbers.
 //
-// The request that holds number x: the last r with first(r) <= x. All 64 lanes probe at once, 64-fold narrower each
+// The request that holds number x (ROWS: that holds row x): the last r with first(r) <= x. All 64 lanes probe at once, 64-fold narrower each
 // round: one round of loads up to 64 requests, two up to 4096. Called by whole wavefronts; any contents of `starts`
 // give an r in [0, R).
 template <bool ROWS>
@@ -930,9 +929,9 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_join_kernel(PagedCall a,
 }
 
 // ---------------------------------------------------------------------------------------------
-// The attention of a step of several tokens. Workgroup (HG heads of one selector and a key span, NW x 32 query rows of one
-// request, numbered as above, the last first): workgroups next to each other, which the XCDs take in turns, are of different
-// heads and spans, so that an XCD's L2 holds few heads' keys. As fwd64_kernel: a wavefront's 32
+// The attention of a step of several tokens. Workgroup (HG heads of one selector and a part of the key tiles, NW x 32 query
+// rows of one request, numbered as above, the last first): workgroups next to each other, which the XCDs take in turns, are of
+// different heads and parts, so that an XCD's L2 holds few heads' keys. As fwd64_kernel: a wavefront's 32
 // queries against one 32-key tile at a time, newest first, every operand loaded straight into LDS one tile ahead,
 // the selection (-F, through the wavefront's LDS rows) one tile ahead of the softmax. What differs is where rows come
 // from: each lane looks its row's page up one tile before the load.
@@ -942,7 +941,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_join_kernel(PagedCall a,
 //
 // P is rounded to the cache's type for the product with V (relative 2^-9 bf16, 2^-12 fp16 at random, the size of the
 // output's own rounding; fp32 not at all); logits, F, row statistics and sums are fp32.
-// The grid of the forward kernels: heads and spans, then query tiles, over y and z where a dimension's 65535 would not hold them.
+// The grid of the forward kernels: heads and parts, then query tiles, over y and z where a dimension's 65535 would not hold them.
 inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
   const int64_t rounds = cdiv(tiles, 32768);
   return dim3((unsigned)per_tile, (unsigned)cdiv(tiles, rounds), (unsigned)rounds);
@@ -950,7 +949,7 @@ inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
 __device__ __forceinline__ int last_tile_first() { return gridDim.y * gridDim.z - 1 - (blockIdx.z * gridDim.y + blockIdx.y); }
 
 // Workgroup number x (1 << SH rows, numbered as above), part z; false: nothing. Rows that no workgroup computes, those
-// behind the last request and those of requests left out, become zero here, COLS columns from col0 on, unless the spans are
+// behind the last request and those of requests left out, become zero here, COLS columns from col0 on, unless the parts are
 // joined afterwards (the join does it).
 template <class P, int SH, int COLS, int THREADS>
 __device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, int64_t row_elems, int col0, bool joined,
@@ -978,7 +977,7 @@ __device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, in
 }
 
 // A wavefront's results for the request's row `row` (lane = row; o transposed, 4 columns per quarter): the output, or the
-// span's part of it: reference m (log2 units), sum l, and the sums of weighted values.
+// part's share of it: reference m (log2 units), sum l, and the sums of weighted values.
 template <class P, int D>
 __device__ __forceinline__ void paged_write(const PagedCall& a, const PagedTiles& w, int row, int head, int z, float m, float l,
                                             const f32x16 (&o)[PagedTile<P, D>::DB], int h, float* part_ml, float* part_o) {

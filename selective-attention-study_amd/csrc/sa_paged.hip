@@ -10,6 +10,7 @@ using namespace sa_host;
 namespace {
 
 constexpr int64_t MAX_TOKENS = (int64_t)1 << 24, MAX_LEN = (int64_t)1 << 30;
+constexpr int64_t GRID_THREADS = ((int64_t)1 << 32) - NTHREADS;   // threads of a launch's first dimension
 
 // log2 of a page size, -1 if it is none: a power of two from 8 on
 int page_shift(int64_t page_size) {
@@ -97,7 +98,7 @@ int sa_paged_append(const void* k, int64_t k_token, int64_t k_head, const void* 
   if (!rows_ok(k, k_token, k_head, head_dim, ss) || !rows_ok(v, v_token, v_head, head_dim, ss) || !aligned(k_pages) ||
       !aligned(v_pages) || !slots)
     return SA_ERR_ARGUMENT;
-  if (tokens * heads * head_dim / 4 >= ((int64_t)1 << 31) * NTHREADS) return SA_ERR_ARGUMENT;
+  if (tokens * heads * (head_dim * es / 16) >= GRID_THREADS) return SA_ERR_ARGUMENT;
   AppendCall c{};
   c.k = k;
   c.v = v;
@@ -122,7 +123,7 @@ int sa_paged_append(const void* k, int64_t k_token, int64_t k_head, const void* 
 static bool paged_sizes_ok(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t max_new, int64_t max_len) {
   return batch_ok(requests, tokens) && heads >= 1 && heads < 65536 && groups >= 1 && heads % groups == 0 && max_new >= 1 &&
          max_new <= tokens && max_len >= 1 && max_len < MAX_LEN && tokens * heads < ((int64_t)1 << 30) &&
-         requests * heads + requests * groups * cdiv(max_len, 4 * NTHREADS) < ((int64_t)1 << 31);
+         (requests * heads + requests * groups * cdiv(max_len, 4 * NTHREADS)) * NTHREADS < GRID_THREADS;
 }
 
 int64_t sa_paged_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t head_dim,

@@ -172,6 +172,8 @@ def paged_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots: 
     _check_ints("slots", slots, tokens, device, torch.int64)
     if tokens >= 1 << 24:
         raise ValueError(f"a step holds up to 2^24 - 1 tokens; got {tokens}")
+    if tokens * heads * head_dim * k_pages.element_size() >= 1 << 36:   # (a thread per 16 bytes)
+        raise ValueError(f"{tokens} tokens of {heads} heads are too many for one launch")
     if tokens == 0:
         return
     lib = _lib.load()
@@ -214,6 +216,8 @@ def _check_step(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, leng
         max_new = tokens
     elif int(max_new) != max_new or max_new < 1:
         raise ValueError(f"max_new must be an integer >= 1; got {max_new}")
+    if requests * (heads + state[1] * -(-int(max_len) // 1024)) >= (1 << 24) - 1:   # (workgroups that join parts and write the state)
+        raise ValueError(f"a step of {requests} requests of {heads} heads and up to {max_len} positions is too large for one launch")
     return (requests, tokens, heads, state[1], head_dim, pages, page_size, width, min(int(max_new), tokens), int(max_len), ld,
             strides[1], dtype, device, _check_exempt(exempt))
 

@@ -138,3 +138,18 @@ def test_the_softmax_slot_has_no_pages():
     cfg = ModelConfig(vocab_size=97, n_layers=1, d_model=64, n_heads=4, context_length=64, attention="softmax")
     with pytest.raises(NotImplementedError, match="paged"):
         SelectiveLM(cfg).new_paged_cache(2, 4, 16)
+
+
+def test_launches_past_a_grid_are_refused():
+    """More workgroups or rows than a launch's first dimension holds (2^32 threads)."""
+    lib = _lib.load()
+    size = lambda requests, heads, max_len: lib.sa_paged_attention_workspace_bytes(requests, requests, heads, 1, 64, 1, max_len, 0)
+    assert size(65535, 16, 4096) > 0 and size(65535, 255, 1024) > 0 and size(65535, 256, 1024) == -1 and size(65535, 16, 1 << 18) == -1
+    fake = 1 << 20
+    append = [fake, 64, 64, fake, 64, 64, fake, fake, fake, 1 << 23, 64, 64, 100, 16, 0, 0, None]
+    assert lib.sa_paged_append(*append) == -1
+    kp = torch.zeros(1, 1, 8, 16).expand(1, 256, 8, 16).contiguous()
+    table, lengths = torch.zeros(65535, 128, dtype=torch.int32), torch.zeros(65535, dtype=torch.int32)
+    with pytest.raises(ValueError, match="too large"):
+        paged._check_step(torch.zeros(4, 256, 16), kp, kp, table, lengths, torch.zeros(65536, dtype=torch.int32),
+                          torch.zeros(65535, 1, 8), 1, 1, 8)
