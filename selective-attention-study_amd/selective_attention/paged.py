@@ -103,7 +103,7 @@ def _rows(x: Tensor) -> Tensor:
 
 
 def _call(device: torch.device, fn, *args) -> None:
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         _lib.check(fn(*args, _stream(device)))
     else:
         with torch.cuda.device(device):
@@ -145,7 +145,8 @@ def page_plan(cached: Tensor, new: Tensor, table: Tensor, free: Tensor, taken: T
     if finished is not None:
         _check_ints("finished", finished, requests, device, torch.bool)
     lib = _lib.load()
-    starts, lengths, after, now_taken = (torch.empty(n, device=device, dtype=torch.int32) for n in (requests + 1, requests, requests, 1))
+    starts, lengths, after, now_taken = torch.empty(3 * requests + 2, device=device, dtype=torch.int32).split(
+        (requests + 1, requests, requests, 1))
     slots = torch.empty(int(tokens), device=device, dtype=torch.int64)
     _call(device, lib.sa_page_plan, cached.data_ptr(), new.data_ptr(), None if finished is None else finished.data_ptr(),
           table.data_ptr(), ld, free.data_ptr(), taken.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
