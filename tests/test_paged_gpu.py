@@ -469,3 +469,15 @@ def test_long_prompts_whose_histories_are_made_in_segments(cuda, dtype, head_dim
                     rate)
     out, state = attend(step, cuda)
     check(out, state, step, ROUNDED[dtype])
+
+
+@pytest.mark.parametrize("head_dim,heads,new", [(64, 4, 34), (32, 1, 40)])
+def test_more_key_tiles_than_a_mask_holds(cuda, head_dim, heads, new):
+    """270000 positions, more than a workgroup's mask of 8192 key tiles; runs of keys with and without weight in turn, in
+    the mask and past it, their ends anywhere in a tile."""
+    step = Step([270000], [new], heads=heads, head_dim=head_dim, page_size=64, seed=11)
+    j = torch.arange(270000)
+    step.selected[0, 0, :270000] = torch.where((j // 997) % 3 == 0, 0.0, 300.0)
+    step.selected[0, 0, 0] = 0.0
+    out, state = attend(step, cuda)
+    check(out, state, step, ROUNDED[torch.bfloat16])
