@@ -32,9 +32,15 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // contracts one chunk per lane (lanes 0-31 the even, lanes 32-63 the odd chunk of their row): one bf16 or fp16
 // instruction, or four fp32 ones that take element e of both halves' chunks (the order of a contraction is free as
 // long as both operands have the same).
+//
+// Softmax weights are taken 2^LIFT times their size beside the row's reference (the factor cancels in the normalisation): an
+// fp16 number below 2^-14 has no more than its last bits, one below 2^-25 none, and a row's many small weights together
+// may be what its output is made of. At 2^10 a weight keeps half a step of fp16 down to 2^-24 of the largest, and is off by 2^-35 of
+// that at most below it: t keys by t 2^-35, half a step of an output at 2^24 of them.
 struct PagedBF16 {
   typedef uint16_t elem;
   static constexpr int EPC = 8;
+  static constexpr float LIFT = 0.f, BIG = 16384.f;   // (BIG: paged_fwd4_kernel)
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -50,6 +56,7 @@ struct PagedBF16 {
 struct PagedF16 {
   typedef uint16_t elem;
   static constexpr int EPC = 8;
+  static constexpr float LIFT = 10.f, BIG = 32768.f;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -65,6 +72,7 @@ struct PagedF16 {
 struct PagedF32 {
   typedef float elem;
   static constexpr int EPC = 4;
+  static constexpr float LIFT = 0.f;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -591,7 +599,7 @@ __device__ __forceinline__ float least_of(float x) {
 // The key tiles that a workgroup's rows can give weight to (as find_reach for the contiguous cache): for a tile
 // before the rows, log2 weight <= s log2e |q| max |k| - log2e (least F) - (row maximum), the row maximum at least the row's logit
 // of its own key, which has no history. Below -REACH_ZERO a weight is an exact fp32 zero (in one part of several: once they
-// are joined), and the tile is left out for all of the workgroup's heads together; tiles for which a NaN or an infinity enters
+// are joined; LIFTed ones: nothing beside the row's sum, at 2^-122 of it), and the tile is left out for all of the workgroup's heads together; tiles for which a NaN or an infinity enters
 // the bound stay. A mask in LDS, bit i the i-th newest tile; past the mask's end every tile stays. A chunk of
 // 4096 queries at 32768 keys, 16 heads, of N(0,1) inputs: 849 us -> 133; where the histories leave the oldest fifth without
 // weight 800 -> 770; where they are too small everywhere 98 -> 104 (prompts of 60 to 2000 tokens), the rows and norms for nothing.
@@ -939,8 +947,8 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_join_kernel(PagedCall a,
 // WHOLE: every head selects for itself (HG = 1): the wavefront's logits arrive with F already subtracted, and the
 // key tile is loaded once.
 //
-// P is rounded to the cache's type for the product with V (relative 2^-9 bf16, 2^-12 fp16 at random, the size of the
-// output's own rounding; fp32 not at all); logits, F, row statistics and sums are fp32.
+// P is rounded to the cache's type for the product with V (by half a step at most: relative 2^-8 bf16, 2^-11 fp16, of fp16
+// weights below 2^-24 of the largest 2^-35 of that; the size of the output's own rounding; fp32 not at all); logits, F, row statistics and sums are fp32.
 // The grid of the forward kernels: heads and parts, then query tiles, over y and z where a dimension's 65535 would not hold them.
 inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
   const int64_t rounds = cdiv(tiles, 32768);
@@ -1217,11 +1225,11 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[g][db][i] *= alpha;
         }
-        const float mu = (m[g] == -INFINITY) ? 0.f : m[g];
+        const float mu = (m[g] == -INFINITY) ? 0.f : m[g], ref = P::LIFT == 0.f ? -mu : P::LIFT - mu;
         float psum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float p = fast_exp2(fmaf(lg[i], sl2, -mu));
+          const float p = fast_exp2(fmaf(lg[i], sl2, ref));
           lg[i] = p;
           psum += p;
         }
@@ -1262,14 +1270,13 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
 //
 // What bounds paged_fwd_kernel is the vector unit: per head and tile 16 exponentials (256 cycles of a SIMD) and, of some 90
 // other instructions, half of a selection's 105 and the running maximum's. Here a quarter of a selection, and no maximum: the
-// weights are taken against the reference mu of the tiles before, and only where a row's sum of them over a tile
-// passes 2^14 (or a row has no reference yet) is the maximum looked for, mu moved and the tile's weights taken again.
-// Any reference within 2^14 of the maximum gives the same weights to rounding, fp16's range included. At 4096 queries on
+// weights are taken against the reference mu of the tiles before, and only where a row's sum of them over half a tile
+// passes BIG (or a row has no reference yet) is the maximum looked for, mu moved and the tile's weights taken again.
+// Any reference within 2^14 of the maximum gives the same bf16 weights to rounding; fp16's (LIFT times larger) stay within 2^5 of it,
+// so that none passes the type's largest number. At 4096 queries on
 // 32768 keys, 16 heads: 0.80 ms (644 TFLOP/s of the two products), paged_fwd_kernel 1.04 (every tile computed); with the selection after the products 0.91,
 // with eight wavefronts of two query tiles each 0.97 (0.91). What is left over is each step's common start and end: its LDS reads
 // at once (0.46 ms without selection, value products and loads), and the wait for its last wavefront.
-constexpr float PAGED_FWD4_BIG = 16384.f;
-
 template <class P>
 __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const float* __restrict__ carry, int64_t carry_ld,
                                                           int splits, float* __restrict__ part_ml, float* __restrict__ part_o) {
@@ -1387,9 +1394,10 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
     auto weights = [&]() __attribute__((always_inline)) {
       f32x16 p;
       float s = 0.f;
+      const float ref = P::LIFT == 0.f ? -mu : P::LIFT - mu;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        p[i] = fast_exp2(fmaf(lg[i], sl2, -mu));
+        p[i] = fast_exp2(fmaf(lg[i], sl2, ref));
         s += p[i];
       }
       psum = s;
@@ -1397,7 +1405,7 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
       pf[1] = P::pack(p, 1);
     };
     weights();
-    if (__builtin_expect(__any(!(psum <= PAGED_FWD4_BIG)), 0)) {
+    if (__builtin_expect(__any(!(psum <= P::BIG)), 0)) {
       float zmax = lg[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) zmax = fmaxf(zmax, lg[i]);

@@ -1,0 +1,56 @@
+"""Edges of the paged operators on an MI355X: weights far below a row's largest, bounds, rows of no request, values that are not
+finite. Bounds of the comparisons as in tests/paged_cases.py."""
+
+import pytest
+import torch
+
+import selective_attention as sa
+from paged_cases import Step, check
+
+pytestmark = pytest.mark.gpu
+
+HALVES = [torch.bfloat16, torch.float16]
+ROUNDED = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: None}
+
+
+def put(step, r, k=None, v=None):
+    """Other keys and values (H, t, D) of request r, in its pages too."""
+    pos = torch.arange(step.lengths[r])
+    at = step.table[r, pos // step.page_size].long(), slice(None), pos % step.page_size
+    for x, pages, mine in ((k, step.k_pages, step.k), (v, step.v_pages, step.v)):
+        if x is not None:
+            mine[r] = x.to(step.dtype)
+            pages[at] = mine[r].transpose(0, 1)
+
+
+def attend(step, device, **kw):
+    args = step.args(device)
+    out = sa.selective_attention_paged(*args, exempt=step.exempt, **kw)
+    torch.cuda.synchronize()
+    return out, args[-1]
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("head_dim,heads,groups,new", [(64, 2, 1, 2), (64, 2, 1, 40), (64, 4, 1, 40), (128, 2, 2, 40), (16, 2, 1, 3)])
+def test_one_key_above_a_long_tail(cuda, dtype, head_dim, heads, groups, new):
+    """Every row's weight is on position 0, the others' 2^-25.5 of it each, below what fp16 can hold beside 1; their values are
+    what the output is made of."""
+    c = 3000
+    step = Step([c], [new], heads=heads, head_dim=head_dim, groups=groups, dtype=dtype, exempt=c + new)   # (nothing selects)
+    step.selected[:, :, :c] = 0.0
+    g = torch.Generator().manual_seed(1)
+    step.q = torch.zeros(new, heads, head_dim)
+    step.q[..., 0] = head_dim**0.5                   # logits: a key's first element, times 1 and what rounding the root leaves
+    step.q = step.q.to(dtype)
+    k, v = torch.zeros(heads, c + new, head_dim), 4.0 + 4.0 * torch.rand(heads, c + new, head_dim, generator=g)
+    k[:, 0, 0] = 17.675 / float(step.q[0, 0, 0]) * head_dim**0.5   # 25.5 log 2
+    v[:, 0] = 0.0
+    put(step, 0, k, v)
+    out, _ = attend(step, cuda)
+    want, off, _, _ = step.exact(ROUNDED[dtype])
+    # fp16 weights are taken at 2^10 times their size beside the row's largest: rounded to 2^-25 where they are not normal
+    # numbers, 2^-35 of the largest (which is all but 2^-13 of the sum)
+    if dtype == torch.float16:
+        off = off + 2.0**-35 * step.v[0].double().sum(1)[None]
+    far = (out.double().cpu() - want).abs()
+    assert (far <= off).all(), f"off by {far.max():.3g} of {want.max():.3g}"
