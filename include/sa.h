@@ -40,6 +40,7 @@ extern "C" {
 #define SA_DTYPE_BF16 0
 #define SA_DTYPE_F32 1
 #define SA_DTYPE_F16 2          /* the paged cache's entry points only */
+#define SA_WIDE_WEIGHTS 16      /* sa_paged_attention: or'ed to a 16-bit dtype (fp32: no change) */
 
 #define SA_OK 0
 #define SA_ERR_ARGUMENT -1      /* a size, pointer or option is invalid */
@@ -285,7 +286,8 @@ int sa_paged_append(const void* k, int64_t k_token, int64_t k_head, const void* 
  * and state_ld. A request past them, or with fewer positions than new tokens, is left out: its state stays. Positions
  * whose page lies outside the cache read as zero keys and values. max_new 1 runs the single-token kernels, which read the
  * cache once; the workspace (16-byte aligned) depends on both bounds. The cache's arithmetic: logits, F, statistics and sums fp32; with several
- * tokens a bf16 or fp16 cache's products run on matrix instructions of that type, the weights rounded to it.
+ * tokens a bf16 or fp16 cache's products run on matrix instructions of that type, the softmax weights rounded to it, or with
+ * SA_WIDE_WEIGHTS as the sum of two numbers of it (relative 2^-16 bf16, 2^-22 fp16): the arithmetic of fp32 operands.
  */
 int64_t sa_paged_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t head_dim,
                                            int64_t max_new, int64_t max_len, int dtype);

@@ -365,6 +365,7 @@ struct PagedLaunch {
   int pshift;
   float scale;
   int exempt, head_dim;
+  bool wide;   // 16-bit caches: softmax weights not rounded to the cache's type
   hipStream_t st;
 };
 SA_HIDDEN int paged_bf16(const PagedLaunch& c);   // sa_paged_bf16.hip

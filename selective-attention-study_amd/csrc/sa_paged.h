@@ -50,6 +50,14 @@ struct PagedBF16 {
     for (int t = 0; t < 8; ++t) f[t] = (bf16_t)x[8 * s + t];
     return __builtin_bit_cast(u32x4, f);
   }
+  // what pack has rounded away, rounded in its turn (hi: pack's result): a weight as the sum of the two is off by 2^-16 of itself
+  static __device__ __forceinline__ u32x4 rest(const f32x16& x, u32x4 hi, int s) {
+    const bf16x8 h = __builtin_bit_cast(bf16x8, hi);
+    bf16x8 f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) f[t] = (bf16_t)(x[8 * s + t] - (float)h[t]);
+    return __builtin_bit_cast(u32x4, f);
+  }
   static __device__ __forceinline__ float to_float(elem x) { return __uint_as_float((uint32_t)x << 16); }
   static __device__ __forceinline__ elem to_elem(float x) { return __builtin_bit_cast(elem, (bf16_t)x); }
 };
@@ -64,6 +72,14 @@ struct PagedF16 {
     f16x8 f;
 #pragma unroll
     for (int t = 0; t < 8; ++t) f[t] = (_Float16)x[8 * s + t];
+    return __builtin_bit_cast(u32x4, f);
+  }
+  // (off by 2^-22 of the weight, or 2^-25 LIFTed)
+  static __device__ __forceinline__ u32x4 rest(const f32x16& x, u32x4 hi, int s) {
+    const f16x8 h = __builtin_bit_cast(f16x8, hi);
+    f16x8 f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) f[t] = (_Float16)(x[8 * s + t] - (float)h[t]);
     return __builtin_bit_cast(u32x4, f);
   }
   static __device__ __forceinline__ float to_float(elem x) { return (float)__builtin_bit_cast(_Float16, x); }
@@ -475,11 +491,18 @@ struct PagedTile {
     }
     return f;
   }
-  // o (columns 32 db ..) += V^T P for the tile's rows, P in the accumulator's layout (lane = query)
-  static __device__ __forceinline__ f32x16 values(const char* t, int lane, int db, const u32x4* pf, const f32x16& p, f32x16 o) {
+  // o (columns 32 db ..) += V^T P for the tile's rows, P in the accumulator's layout (lane = query); of a 16-bit type pf, and with
+  // WIDE pr, the weights' halves
+  template <bool WIDE>
+  static __device__ __forceinline__ f32x16 values(const char* t, int lane, int db, const u32x4* pf, const u32x4* pr, const f32x16& p,
+                                                  f32x16 o) {
     if constexpr (ES == 2) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) o = P::mma(value_frag(t, 0, lane, db, s), pf[s], o);
+      for (int s = 0; s < 2; ++s) {
+        const u32x4 v = value_frag(t, 0, lane, db, s);
+        o = P::mma(v, pf[s], o);
+        if constexpr (WIDE) o = P::mma(v, pr[s], o);
+      }
     } else {
       const int n = lane & 31, h = lane >> 5, d = (32 * db + n) & (D - 1);
 #pragma unroll
@@ -948,7 +971,10 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_join_kernel(PagedCall a,
 // key tile is loaded once.
 //
 // P is rounded to the cache's type for the product with V (by half a step at most: relative 2^-8 bf16, 2^-11 fp16, of fp16
-// weights below 2^-24 of the largest 2^-35 of that; the size of the output's own rounding; fp32 not at all); logits, F, row statistics and sums are fp32.
+// weights below 2^-24 of the largest 2^-35 of that; the size of the output's own rounding; fp32 not at all). WIDE: as the sum of
+// two numbers of that type (2^-16, 2^-22), in twice the value products, which is what fp32 operands come to, q, k and v
+// being of 16 bits as they are: a chunk of 4096 fp16 queries at 32768 keys, 16 heads, 757 -> 937 us, prompts of 60 to 2000
+// tokens 114 -> 136, chunks of 300 to 700 queries of three requests, each of 8 heads selecting, 62 -> 64. Logits, F, row statistics and sums are fp32.
 // The grid of the forward kernels: heads and parts, then query tiles, over y and z where a dimension's 65535 would not hold them.
 inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
   const int64_t rounds = cdiv(tiles, 32768);
@@ -1029,7 +1055,7 @@ struct FwdLds {
   };
 };
 
-template <class P, int D, int HG, int NW, bool WHOLE>
+template <class P, int D, int HG, int NW, bool WHOLE, bool WIDE>
 __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) == 2 && D <= 64) ? (HG == 1 ? 3 : 2) : 1)) void paged_fwd_kernel(
     PagedCall a, const float* __restrict__ carry, int64_t carry_ld, int splits, float* __restrict__ part_ml,
     float* __restrict__ part_o) {
@@ -1234,13 +1260,16 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
           psum += p;
         }
         l[g] += psum;
-        u32x4 pf[2];
+        u32x4 pf[2], pr[2];
         if constexpr (T::ES == 2) {
-          pf[0] = P::pack(lg, 0);
-          pf[1] = P::pack(lg, 1);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            pf[s] = P::pack(lg, s);
+            if constexpr (WIDE) pr[s] = P::rest(lg, pf[s], s);
+          }
         }
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[g][db] = T::values(B.v[g], lane, db, pf, lg, o[g][db]);
+        for (int db = 0; db < DB; ++db) o[g][db] = T::template values<WIDE>(B.v[g], lane, db, pf, pr, lg, o[g][db]);
       }
     }
     if (n1 >= 0 && n1 < my_end) select(n1, ODD ? sS0 : sS1, entry1);
@@ -1277,7 +1306,7 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
 // 32768 keys, 16 heads: 0.80 ms (644 TFLOP/s of the two products), paged_fwd_kernel 1.04 (every tile computed); with the selection after the products 0.91,
 // with eight wavefronts of two query tiles each 0.97 (0.91). What is left over is each step's common start and end: its LDS reads
 // at once (0.46 ms without selection, value products and loads), and the wait for its last wavefront.
-template <class P>
+template <class P, bool WIDE>
 __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const float* __restrict__ carry, int64_t carry_ld,
                                                           int splits, float* __restrict__ part_ml, float* __restrict__ part_o) {
   constexpr int D = 64, HG = 4, SH = 7, LDF = TILE + 4;
@@ -1374,22 +1403,25 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
 
   auto attend = [&](int kt, const Tiles& B, const float* F) __attribute__((always_inline)) {
     f32x16 lg;
+    auto logits = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const float4 f4 = *reinterpret_cast<const float4*>(F + n * LDF + 8 * q4 + 4 * h);
-      lg[4 * q4] = f4.x;
-      lg[4 * q4 + 1] = f4.y;
-      lg[4 * q4 + 2] = f4.z;
-      lg[4 * q4 + 3] = f4.w;
-    }
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 f4 = *reinterpret_cast<const float4*>(F + n * LDF + 8 * q4 + 4 * h);
+        lg[4 * q4] = f4.x;
+        lg[4 * q4 + 1] = f4.y;
+        lg[4 * q4 + 2] = f4.z;
+        lg[4 * q4 + 3] = f4.w;
+      }
 #pragma unroll
-    for (int s = 0; s < NS; ++s) lg = P::mma(T::row_frag(B.k[u], n, h, s), qf[s], lg);
-    if (kt * TILE + TILE - 1 > qpos0) {   // keys past a query
-      const int thr = qpos0 + n - kt * TILE - 4 * h;
+      for (int s = 0; s < NS; ++s) lg = P::mma(T::row_frag(B.k[u], n, h, s), qf[s], lg);
+      if (kt * TILE + TILE - 1 > qpos0) {   // keys past a query
+        const int thr = qpos0 + n - kt * TILE - 4 * h;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) lg[i] = crow(i, 0) <= thr ? lg[i] : -INFINITY;
-    }
-    u32x4 pf[2];
+        for (int i = 0; i < 16; ++i) lg[i] = crow(i, 0) <= thr ? lg[i] : -INFINITY;
+      }
+    };
+    logits();
+    u32x4 pf[2], pr[2];
     float psum;
     auto weights = [&]() __attribute__((always_inline)) {
       f32x16 p;
@@ -1401,11 +1433,18 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
         s += p[i];
       }
       psum = s;
-      pf[0] = P::pack(p, 0);
-      pf[1] = P::pack(p, 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        pf[t] = P::pack(p, t);
+        if constexpr (WIDE) pr[t] = P::rest(p, pf[t], t);
+      }
     };
     weights();
     if (__builtin_expect(__any(!(psum <= P::BIG)), 0)) {
+      if constexpr (WIDE) {   // the logits again: kept, they would not fit the registers beside the weights' halves
+        __asm__ volatile("" ::: "memory");   // (nor would what they were made from)
+        logits();
+      }
       float zmax = lg[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) zmax = fmaxf(zmax, lg[i]);
@@ -1424,8 +1463,11 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        o[db] = P::mma(T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s), pf[s], o[db]);
+      for (int s = 0; s < 2; ++s) {
+        const u32x4 v = T::value_frag(reinterpret_cast<const char*>(&B), HG * T::BYTES + u * T::BYTES, lane, db, s);
+        o[db] = P::mma(v, pf[s], o[db]);
+        if constexpr (WIDE) o[db] = P::mma(v, pr[s], o[db]);
+      }
   };
 
   PagedLive tiles{nullptr, w.kt_hi, 0, 0};
@@ -1835,11 +1877,36 @@ inline PagedCall paged_call(const PagedLaunch& c) {
   return a;
 }
 
-template <class P, int D, int HG, int NW, bool WHOLE>
-void launch_paged_fwd(const PagedCall& a, const PagedShape& s, const float* carry, float* ml, float* o, hipStream_t st) {
+template <class P, int D, int HG, int NW, bool WHOLE, bool WIDE>
+void launch_paged_tiles(const PagedCall& a, const PagedShape& s, const float* carry, float* ml, float* o, hipStream_t st) {
   const int64_t tiles = (int64_t)(a.N >> (NW == 4 ? 7 : 5)) + a.R;
-  hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE>), tile_grid((int64_t)a.H / HG * s.splits, tiles), dim3(NW * 64), 0, st,
-                     a, carry, s.ld, s.splits, ml, o);
+  hipLaunchKernelGGL((paged_fwd_kernel<P, D, HG, NW, WHOLE, WIDE>), tile_grid((int64_t)a.H / HG * s.splits, tiles), dim3(NW * 64), 0,
+                     st, a, carry, s.ld, s.splits, ml, o);
+}
+
+template <class P, int D, bool WIDE>
+void launch_paged_fwd(const PagedCall& a, const PagedShape& s, const float* carry, float* ml, float* o, hipStream_t st) {
+  const bool whole = a.G == a.H;
+  if constexpr (sizeof(typename P::elem) == 2 && D == 64) {
+    if (s.hg == 4)
+      hipLaunchKernelGGL((paged_fwd4_kernel<P, WIDE>), tile_grid((int64_t)a.H / 4 * s.splits, (a.N >> 7) + a.R), dim3(1024), 0, st, a,
+                         carry, s.ld, s.splits, ml, o);
+  }
+  if constexpr (sizeof(typename P::elem) == 2 && D <= 64) {
+    if (s.hg == 2) {
+      if (s.nw == 4) launch_paged_tiles<P, D, 2, 4, false, WIDE>(a, s, carry, ml, o, st);
+      else launch_paged_tiles<P, D, 2, 1, false, WIDE>(a, s, carry, ml, o, st);
+    }
+  }
+  if (s.hg == 1) {
+    if (s.nw == 4) {
+      if (whole) launch_paged_tiles<P, D, 1, 4, true, WIDE>(a, s, carry, ml, o, st);
+      else launch_paged_tiles<P, D, 1, 4, false, WIDE>(a, s, carry, ml, o, st);
+    } else {
+      if (whole) launch_paged_tiles<P, D, 1, 1, true, WIDE>(a, s, carry, ml, o, st);
+      else launch_paged_tiles<P, D, 1, 1, false, WIDE>(a, s, carry, ml, o, st);
+    }
+  }
 }
 
 template <class P, int D>
@@ -1886,26 +1953,11 @@ int paged_launch(const PagedLaunch& c) {
   }
   {
     TimedLaunch timed(SA_KERNEL_FORWARD, c.st);
-    const bool whole = a.G == a.H;
-    if constexpr (sizeof(typename P::elem) == 2 && D == 64) {
-      if (s.hg == 4)
-        hipLaunchKernelGGL((paged_fwd4_kernel<P>), tile_grid((int64_t)a.H / 4 * s.splits, (a.N >> 7) + a.R), dim3(1024), 0, c.st, a,
-                           carry, s.ld, s.splits, ml, o);
-    }
-    if constexpr (sizeof(typename P::elem) == 2 && D <= 64) {
-      if (s.hg == 2) {
-        if (s.nw == 4) launch_paged_fwd<P, D, 2, 4, false>(a, s, carry, ml, o, c.st);
-        else launch_paged_fwd<P, D, 2, 1, false>(a, s, carry, ml, o, c.st);
-      }
-    }
-    if (s.hg == 1) {
-      if (s.nw == 4) {
-        if (whole) launch_paged_fwd<P, D, 1, 4, true>(a, s, carry, ml, o, c.st);
-        else launch_paged_fwd<P, D, 1, 4, false>(a, s, carry, ml, o, c.st);
-      } else {
-        if (whole) launch_paged_fwd<P, D, 1, 1, true>(a, s, carry, ml, o, c.st);
-        else launch_paged_fwd<P, D, 1, 1, false>(a, s, carry, ml, o, c.st);
-      }
+    if constexpr (sizeof(typename P::elem) == 2) {
+      if (c.wide) launch_paged_fwd<P, D, true>(a, s, carry, ml, o, c.st);
+      else launch_paged_fwd<P, D, false>(a, s, carry, ml, o, c.st);
+    } else {
+      launch_paged_fwd<P, D, false>(a, s, carry, ml, o, c.st);
     }
   }
   if (s.splits > 1)

@@ -128,8 +128,9 @@ static bool paged_sizes_ok(int64_t requests, int64_t tokens, int64_t heads, int6
 
 int64_t sa_paged_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t heads, int64_t groups, int64_t head_dim,
                                            int64_t max_new, int64_t max_len, int dtype) {
-  if (!paged_sizes_ok(requests, tokens, heads, groups, max_new, max_len) || !head_dim_ok(head_dim) || !elem_size(dtype)) return -1;
-  return paged_shape(requests, tokens, heads, groups, head_dim, elem_size(dtype), max_new, max_len).total;
+  const int64_t es = elem_size(dtype & ~SA_WIDE_WEIGHTS);
+  if (!paged_sizes_ok(requests, tokens, heads, groups, max_new, max_len) || !head_dim_ok(head_dim) || !es) return -1;
+  return paged_shape(requests, tokens, heads, groups, head_dim, es, max_new, max_len).total;
 }
 
 int sa_paged_attention(const void* q, int64_t q_token, int64_t q_head, const void* k_pages, const void* v_pages, void* out,
@@ -138,6 +139,8 @@ int sa_paged_attention(const void* q, int64_t q_token, int64_t q_head, const voi
                        int64_t heads, int64_t groups, int64_t head_dim, int64_t pages, int64_t page_size, int64_t width,
                        int64_t max_new, int64_t max_len, float scale, int dtype, int exempt, void* stream) {
   const int sh = page_shift(page_size);
+  const bool wide = dtype & SA_WIDE_WEIGHTS;
+  dtype &= ~SA_WIDE_WEIGHTS;
   const int64_t es = elem_size(dtype);
   if (!es) return SA_ERR_DTYPE;
   if (!head_dim_ok(head_dim)) return SA_ERR_HEAD_DIM;
@@ -175,6 +178,7 @@ int sa_paged_attention(const void* q, int64_t q_token, int64_t q_head, const voi
   c.scale = scale;
   c.exempt = exempt;
   c.head_dim = (int)head_dim;
+  c.wide = wide;
   c.st = static_cast<hipStream_t>(stream);
   return dtype == SA_DTYPE_BF16 ? paged_bf16(c) : dtype == SA_DTYPE_F16 ? paged_f16(c) : paged_f32(c);
 }

@@ -19,6 +19,7 @@ LIB_PATH = os.environ.get("SA_HIP_LIBRARY") or os.path.join(os.path.dirname(os.p
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
 DTYPE_F16 = 2   # the paged cache's entry points
+WIDE_WEIGHTS = 16   # sa_paged_attention: or'ed to the dtype
 
 # Kernel ids of sa_timing_read.
 KERNEL_FORWARD = 0

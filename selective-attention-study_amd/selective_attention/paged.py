@@ -28,7 +28,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .kernels import DTYPES, HEAD_DIMS, _check_exempt, _stream
+from .kernels import DTYPES, HEAD_DIMS, _check_exempt, _resolve_precision, _stream
 
 _CODES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16}
 
@@ -225,7 +225,7 @@ def _check_step(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, leng
 
 def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, starts: Tensor,
                               selected: Tensor, exempt: int = 1, max_new: int | None = None,
-                              max_len: int | None = None) -> Tensor:
+                              max_len: int | None = None, dot_precision: str | None = None) -> Tensor:
     """Selective Attention of a step's new tokens over a paged cache that already holds their keys and values.
 
     q: (N, H, D) in the cache's dtype (any view with contiguous head rows); request r's queries are rows starts[r] ..
@@ -240,19 +240,26 @@ def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table
     kernels. A request that exceeds a bound, or has fewer positions than new tokens (0 where page_plan left it out), is
     left out: its rows are 0, its state stays. Positions whose table entry is not a page of the cache read as zeros.
 
-    No autograd. On a bf16 or fp16 cache steps of several tokens run that type's matrix instructions with the softmax
-    weights rounded to it; logits, F, softmax statistics and sums are fp32, as everything is for an fp32 cache and for
-    single tokens.
+    dot_precision, as the package's other entry points have it: None is "bf16" for a bf16 cache and fp32 arithmetic for the others.
+    On a bf16 or fp16 cache steps of several tokens run that type's matrix instructions. With "bf16" the softmax weights are
+    rounded to the cache's type for the product with the values; with "tf32" or "ieee" they are the sum of two such numbers
+    (bf16 to 2^-16, fp16 to 2^-22), which leaves fp32's accuracy, as products of 16-bit numbers are exact in it. Logits, F, softmax
+    statistics and sums are fp32 either way, as everything is for an fp32 cache and for single tokens. The output is
+    rounded to the cache's type.
+
+    No autograd.
     """
 
     _check_cuda(k_pages)
     (requests, tokens, heads, groups, head_dim, pages, page_size, width, max_new, max_len, table_ld, state_ld, dtype, device,
      exempt) = _check_step(q, k_pages, v_pages, table, lengths, starts, selected, exempt, max_new, max_len)
+    code = _CODES[dtype]
+    if _resolve_precision(dot_precision, dtype) == _lib.DTYPE_F32:
+        code |= _lib.WIDE_WEIGHTS
     out = torch.empty(tokens, heads, head_dim, device=device, dtype=dtype)
     if tokens == 0:
         return out
     lib = _lib.load()
-    code = _CODES[dtype]
     q = _rows(q)
     size = lib.sa_paged_attention_workspace_bytes(requests, tokens, heads, groups, head_dim, max_new, max_len, code)
     ws = torch.empty(size, device=device, dtype=torch.uint8)
@@ -313,10 +320,12 @@ def paged_append_reference(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tenso
 
 def selective_attention_paged_reference(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor,
                                         starts: Tensor, selected: Tensor, exempt: int = 1, max_new: int | None = None,
-                                        max_len: int | None = None) -> Tensor:
-    """selective_attention_paged, request after request, in fp32 (float64 for float64 inputs); any head dim."""
+                                        max_len: int | None = None, dot_precision: str | None = None) -> Tensor:
+    """selective_attention_paged, request after request, in fp32 whatever dot_precision (float64 for float64 inputs); any
+    head dim."""
 
     exempt = _check_exempt(exempt)
+    _resolve_precision(dot_precision, q.dtype)
     pages, heads, page_size, head_dim = k_pages.shape
     groups = selected.shape[1]
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32

@@ -54,3 +54,36 @@ def test_one_key_above_a_long_tail(cuda, dtype, head_dim, heads, groups, new):
         off = off + 2.0**-35 * step.v[0].double().sum(1)[None]
     far = (out.double().cpu() - want).abs()
     assert (far <= off).all(), f"off by {far.max():.3g} of {want.max():.3g}"
+
+
+# what a weight may be off by as the sum of two numbers of its type
+WIDE = {torch.bfloat16: 2.0**-16, torch.float16: 2.0**-22}
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("head_dim,heads,groups,page_size,exempt", [
+    (64, 4, 1, 16, 1), (64, 8, 2, 8, 3), (64, 2, 1, 32, 1), (64, 3, 3, 16, 1), (64, 3, 1, 16, 1), (128, 2, 1, 16, 16), (128, 2, 2, 64, 1),
+    (32, 4, 1, 16, 1), (16, 2, 1, 16, 1), (16, 2, 2, 32, 1)])
+@pytest.mark.parametrize("cached,new", [([0, 31, 64, 0], [33, 33, 60, 2]), ([9, 300], [7, 2]), ([700], [50])])
+def test_fp32_arithmetic_on_16_bit_caches(cuda, dtype, head_dim, heads, groups, page_size, exempt, cached, new):
+    """dot_precision "ieee" or "tf32": nothing is rounded to the cache's type but the output. The package's default for fp16."""
+    step = Step(cached, new, heads=heads, head_dim=head_dim, groups=groups, dtype=dtype, page_size=page_size, exempt=exempt)
+    out, state = attend(step, cuda, dot_precision="ieee")
+    # (fp16: 2^-35 of a row's largest weight besides, for each of at most 800 keys: less than 2^-25 of values of a size
+    # of 4, under half a step of the smallest output that is no zero)
+    check(out, state, step, WIDE[dtype])
+    assert torch.equal(out, attend(step, cuda, dot_precision="tf32")[0])
+    rounded, _ = attend(step, cuda, dot_precision="bf16")
+    assert not torch.equal(out, rounded)
+    assert torch.equal(attend(step, cuda)[0], out if dtype == torch.float16 else rounded)
+
+
+def test_precisions_that_change_nothing(cuda):
+    step = Step([9, 300], [7, 2], dtype=torch.float32)   # an fp32 cache
+    out, _ = attend(step, cuda)
+    assert all(torch.equal(out, attend(step, cuda, dot_precision=p)[0]) for p in ("ieee", "tf32", "bf16"))
+    step = Step([9, 300], [1, 1], dtype=torch.bfloat16)   # single tokens
+    out, _ = attend(step, cuda, max_new=1)
+    assert all(torch.equal(out, attend(step, cuda, max_new=1, dot_precision=p)[0]) for p in ("ieee", "tf32", "bf16"))
+    with pytest.raises(ValueError, match="dot_precision"):
+        attend(step, cuda, dot_precision="fp8")
