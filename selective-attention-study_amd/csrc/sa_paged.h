@@ -974,7 +974,9 @@ __global__ __launch_bounds__(NTHREADS) void paged_carry_join_kernel(PagedCall a,
 // weights below 2^-24 of the largest 2^-35 of that; the size of the output's own rounding; fp32 not at all). WIDE: as the sum of
 // two numbers of that type (2^-16, 2^-22), in twice the value products, which is what fp32 operands come to, q, k and v
 // being of 16 bits as they are: a chunk of 4096 fp16 queries at 32768 keys, 16 heads, 757 -> 937 us, prompts of 60 to 2000
-// tokens 114 -> 136, chunks of 300 to 700 queries of three requests, each of 8 heads selecting, 62 -> 64. Logits, F, row statistics and sums are fp32.
+// tokens 114 -> 136, chunks of 300 to 700 queries of three requests, each of 8 heads selecting, 62 -> 64. Logits, F, row
+// statistics and sums are fp32.
+
 // The grid of the forward kernels: heads and parts, then query tiles, over y and z where a dimension's 65535 would not hold them.
 inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
   const int64_t rounds = cdiv(tiles, 32768);

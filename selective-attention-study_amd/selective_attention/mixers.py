@@ -167,7 +167,7 @@ class SelectiveAttention(AttentionSlot):
             append, attend = paged.paged_append_reference, paged.selective_attention_paged_reference
         append(k, v, cache["k"], cache["v"], plan.slots)
         y = attend(q, cache["k"], cache["v"], table, plan.lengths, plan.starts, cache["selected"], exempt=self.exempt,
-                   max_new=max_new, max_len=max_len)
+                   max_new=max_new, max_len=max_len, dot_precision=self.dot_precision)
         return self.emit(y.transpose(0, 1)[None].to(x.dtype))
 
     def _chunk_listing(self, q: Tensor, keys: Tensor, vals: Tensor, state: Tensor, c0: int) -> Tensor:

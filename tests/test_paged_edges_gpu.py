@@ -6,6 +6,7 @@ import torch
 
 import selective_attention as sa
 from paged_cases import Step, check
+from selective_attention.model import ModelConfig, SelectiveLM
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,24 @@ def test_precisions_that_change_nothing(cuda):
     assert all(torch.equal(out, attend(step, cuda, max_new=1, dot_precision=p)[0]) for p in ("ieee", "tf32", "bf16"))
     with pytest.raises(ValueError, match="dot_precision"):
         attend(step, cuda, dot_precision="fp8")
+
+
+def test_the_slots_precision_reaches_the_kernels(cuda):
+    """A bf16 slot set to "ieee": its paged step is the operator's with fp32 arithmetic, and not the default's."""
+    torch.manual_seed(0)
+    cfg = ModelConfig(vocab_size=97, n_layers=1, d_model=256, n_heads=4, context_length=64)
+    slot = SelectiveLM(cfg).to(cuda, torch.bfloat16).eval().transformer.h[0].attn
+    x = torch.randn(1, 50, 256, device=cuda).bfloat16()
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)
+    got = {}
+    with torch.no_grad():
+        q, k, v = (y[0].transpose(0, 1) for y in slot.project(x))
+        for precision in (None, "ieee"):
+            cache, table = slot.new_pages(1, 4, 16, 64, cuda, torch.bfloat16), ints(2, 0, 1, 3).view(1, 4)
+            plan = sa.page_plan(ints(0), ints(50), table, ints(2, 0, 1, 3), ints(0), 16, 50)
+            slot.dot_precision = precision
+            got[precision] = slot.step_paged(x, cache, table, plan)
+            y = sa.selective_attention_paged(q, cache["k"], cache["v"], table, plan.lengths, plan.starts,
+                                             torch.zeros_like(cache["selected"]), dot_precision=precision)
+            assert torch.equal(got[precision], slot.emit(y.transpose(0, 1)[None]))
+    assert not torch.equal(got[None], got["ieee"])
