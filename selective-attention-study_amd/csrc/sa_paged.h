@@ -985,7 +985,7 @@ inline dim3 tile_grid(int64_t per_tile, int64_t tiles) {
 __device__ __forceinline__ int last_tile_first() { return gridDim.y * gridDim.z - 1 - (blockIdx.z * gridDim.y + blockIdx.y); }
 
 // Workgroup number x (1 << SH rows, numbered as above), part z; false: nothing. Rows that no workgroup computes, those
-// behind the last request and those of requests left out, become zero here, COLS columns from col0 on, unless the parts are
+// before the first request, behind the last and of requests left out, become zero here, COLS columns from col0 on, unless the parts are
 // joined afterwards (the join does it).
 template <class P, int SH, int COLS, int THREADS>
 __device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, int64_t row_elems, int col0, bool joined,
@@ -996,8 +996,9 @@ __device__ __forceinline__ bool paged_tiles(const PagedCall& a, int x, int z, in
   };
   const bool zeros = !joined && z == 0;
   if (zeros) {
-    const int hi = min((x + 1) << SH, a.N), lo = min(max(x << SH, a.starts[a.R]), hi);
+    const int first = x << SH, hi = min((x + 1) << SH, a.N), lo = min(max(first, a.starts[a.R]), hi);
     clear(lo, hi - lo);
+    if (first < a.starts[0]) clear(first, min(hi, a.starts[0]) - first);
   }
   w.r = find_request<false>(a.starts, a.R, x, SH);
   w.rq = paged_request(a, w.r);
@@ -1765,7 +1766,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_step_kernel(PagedCall a, float
 }
 
 // Block (r, head) for the first R * H blocks: the request's chunks' partials joined; without `ones` (every row is here) also
-// zeros for the rows of requests left out, and for those behind the last request, each block every R-th of them. Blocks
+// zeros for the rows of requests left out, and for those before the first request and behind the last, each block every R-th of them. Blocks
 // from there on: the new state rows, `sblocks` blocks of 1024 keys each.
 template <class P, int D>
 __global__ __launch_bounds__(NTHREADS) void paged_step_join_kernel(PagedCall a, const float* __restrict__ pm,
@@ -1797,6 +1798,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_step_join_kernel(PagedCall a, 
   if (!a.ones) {
     if (tid < D) {
       for (int64_t row = max(a.starts[a.R], 0) + (int64_t)r; row < a.N; row += a.R) row_of((int)row)[tid] = P::to_elem(0.f);
+      for (int64_t row = r; row < min(a.starts[0], a.N); row += a.R) row_of((int)row)[tid] = P::to_elem(0.f);
       if (!rq.live)
         for (int i = 0; i < rq.n; ++i) row_of(rq.first + i)[tid] = P::to_elem(0.f);
     }

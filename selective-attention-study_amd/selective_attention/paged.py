@@ -233,7 +233,7 @@ def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table
     every cached position the selection it has received (group g's heads are g*H/G ... and its selector is the
     first of them: G = 1 head 0 for all, G = H every head for itself); updated in place, the new positions' entries
     overwritten. Returns (N, H, D) in q's dtype: for every request what selective_attention_prefill (or, with one
-    token, selective_attention_decode) gives on its own contiguous cache. Rows behind the last request are 0.
+    token, selective_attention_decode) gives on its own contiguous cache. Rows of no request are 0.
 
     max_new, max_len: upper bounds, known to the caller, of a request's new tokens and of its positions (default: N, and
     what table and selected hold); they size the launch and its workspace, and max_new=1 runs the single-token

@@ -109,3 +109,20 @@ def test_the_slots_precision_reaches_the_kernels(cuda):
                                              torch.zeros_like(cache["selected"]), dot_precision=precision)
             assert torch.equal(got[precision], slot.emit(y.transpose(0, 1)[None]))
     assert not torch.equal(got[None], got["ieee"])
+
+
+@pytest.mark.parametrize("max_new", [1, 2, 40])
+def test_rows_before_the_first_request(cuda, max_new):
+    """starts[0] is not 0: a call on some of a step's requests. The rows of no request are zeros, whatever memory held."""
+    step = Step([70, 5, 40], [max_new, 1, max_new], dtype=torch.bfloat16)
+    args = step.args(cuda)
+    want, lead = sa.selective_attention_paged(*args, max_new=max_new), 300
+    args = step.args(cuda)
+    args[0] = torch.cat([args[0].new_zeros(lead, *args[0].shape[1:]), args[0], args[0].new_zeros(7, *args[0].shape[1:])])
+    args[5] = args[5] + lead
+    for _ in range(2):
+        junk = torch.full(args[0].shape, float("nan"), dtype=args[0].dtype, device=cuda)   # the block that the output takes
+        del junk
+        out = sa.selective_attention_paged(*args[:6], args[6].clone(), max_new=max_new)
+        assert (out[:lead] == 0).all() and (out[lead + step.tokens:] == 0).all()
+    assert not out.isnan().any() and torch.allclose(out[lead:lead + step.tokens].float(), want.float(), atol=2.0**-6)
