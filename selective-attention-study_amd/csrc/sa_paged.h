@@ -1716,7 +1716,7 @@ __global__ __launch_bounds__(NTHREADS) void paged_step_kernel(PagedCall a, float
     const float z = jok ? (raw - sel) * LOG2E : -INFINITY;
     const float m_new = fmaxf(m, wave_max(z));
     const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m - m_new);
-    const float p = jok && m_new > -INFINITY ? fast_exp2(z - m_new) : 0.f;
+    const float p = z != -INFINITY ? fast_exp2(z - m_new) : 0.f;   // (not where no key has weight; NaN where only NaNs are)
     l = fmaf(l, alpha, owner ? p : 0.f);
 #pragma unroll
     for (int e = 0; e < EPC; ++e) o[e] *= alpha;

@@ -126,3 +126,15 @@ def test_rows_before_the_first_request(cuda, max_new):
         out = sa.selective_attention_paged(*args[:6], args[6].clone(), max_new=max_new)
         assert (out[:lead] == 0).all() and (out[lead + step.tokens:] == 0).all()
     assert not out.isnan().any() and torch.allclose(out[lead:lead + step.tokens].float(), want.float(), atol=2.0**-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("new", [1, 2, 40])
+@pytest.mark.parametrize("head_dim,first", [(64, 64), (64, 0), (128, 320), (16, 1024)])
+def test_a_page_of_nan_is_not_lost(cuda, dtype, new, head_dim, first):
+    """Keys that are NaN a whole page long: every row that sees them is NaN, as for a single one."""
+    step = Step([1300], [new], heads=2, head_dim=head_dim, dtype=dtype, page_size=128)
+    at = first // 128 * 128
+    step.k_pages[int(step.table[0, at // 128]), 1] = float("nan")
+    out, _ = attend(step, cuda, max_new=new)
+    assert out[:, 1].isnan().all() and not out[:, 0].isnan().any()
