@@ -261,11 +261,18 @@ int sa_decode_noalloc(const void* q, const void* k, const void* v, float* out, f
  *   cached_out (requests) what the cache holds after the step
  *   slots      (tokens) page * page_size + row of every token; -1: a request left out, or a row behind the last
  *   taken_out  (1) may be `taken` itself
+ * sa_page_plan_within: the same, and a request with more than max_new new tokens, or more than max_len positions after them
+ * (up to width * page_size), is left out too: the bounds that the step's sa_paged_attention is given, which leaves such a
+ * request out, so that no cache holds positions that the attention has not seen.
  */
 int sa_page_plan(const int32_t* cached, const int32_t* new_tokens, const uint8_t* finished, int32_t* table, int64_t table_ld,
                  int32_t* free_pages, const int32_t* taken, int32_t* starts, int32_t* lengths, int32_t* cached_out,
                  int64_t* slots, int32_t* taken_out, int64_t requests, int64_t width, int64_t pool, int64_t tokens,
                  int64_t page_size, void* stream);
+int sa_page_plan_within(const int32_t* cached, const int32_t* new_tokens, const uint8_t* finished, int32_t* table, int64_t table_ld,
+                        int32_t* free_pages, const int32_t* taken, int32_t* starts, int32_t* lengths, int32_t* cached_out,
+                        int64_t* slots, int32_t* taken_out, int64_t requests, int64_t width, int64_t pool, int64_t tokens,
+                        int64_t page_size, int64_t max_new, int64_t max_len, void* stream);
 
 /* Writes tokens' key and value rows into the cache: row i to slot slots[i] (distinct; slots outside the cache: row left
  * out), rounded from src_dtype to the cache's dtype. k, v: element strides of a token and of a head, 16-byte

@@ -21,7 +21,7 @@ using namespace sa_host;
 
 extern "C" {
 
-int sa_abi_version(void) { return 8; }
+int sa_abi_version(void) { return 9; }
 
 int sa_timing_enable(int on) {
   TimingRegistry& r = timing();

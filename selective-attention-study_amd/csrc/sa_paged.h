@@ -191,6 +191,7 @@ struct PlanCall {
   int64_t* slots;
   int64_t table_ld;
   int R, W, F, N, pshift;
+  int max_new, max_len;   // of a request with new tokens (max_len within the row's pages)
   bool slots_here;   // the slot map too; else page_slots_kernel makes it
 };
 
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanCall a) {
     }
     const int64_t t = (int64_t)c + n;
     const int have = pages_of(c);
-    const bool fits = r < a.R && t <= ((int64_t)a.W << a.pshift);
+    const bool fits = r < a.R && (n > 0 ? n <= a.max_new && t <= a.max_len : t <= ((int64_t)a.W << a.pshift));
     const int need = fits ? pages_of(t) - have : 0;
     const Sum2 s = block_scan2(n, need, sh);
     const int64_t first = row + s.a - n, end = row + s.a, upto = given + s.b;

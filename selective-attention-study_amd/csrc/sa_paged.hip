@@ -53,9 +53,20 @@ int sa_page_plan(const int32_t* cached, const int32_t* new_tokens, const uint8_t
                  int32_t* free_pages, const int32_t* taken, int32_t* starts, int32_t* lengths, int32_t* cached_out,
                  int64_t* slots, int32_t* taken_out, int64_t requests, int64_t width, int64_t pool, int64_t tokens,
                  int64_t page_size, void* stream) {
+  if (page_shift(page_size) < 0 || width < 1 || width > MAX_LEN / page_size) return SA_ERR_ARGUMENT;
+  return sa_page_plan_within(cached, new_tokens, finished, table, table_ld, free_pages, taken, starts, lengths, cached_out, slots,
+                             taken_out, requests, width, pool, tokens, page_size, std::max<int64_t>(tokens, 1), width * page_size,
+                             stream);
+}
+
+int sa_page_plan_within(const int32_t* cached, const int32_t* new_tokens, const uint8_t* finished, int32_t* table, int64_t table_ld,
+                        int32_t* free_pages, const int32_t* taken, int32_t* starts, int32_t* lengths, int32_t* cached_out,
+                        int64_t* slots, int32_t* taken_out, int64_t requests, int64_t width, int64_t pool, int64_t tokens,
+                        int64_t page_size, int64_t max_new, int64_t max_len, void* stream) {
   const int sh = page_shift(page_size);
   if (requests < 1 || requests >= 65536 || tokens < 0 || tokens >= MAX_TOKENS || sh < 0) return SA_ERR_ARGUMENT;
-  if (width < 1 || table_ld < width || width * page_size > MAX_LEN || pool < 0 || pool > INT32_MAX) return SA_ERR_ARGUMENT;
+  if (width < 1 || table_ld < width || width > MAX_LEN / page_size || pool < 0 || pool > INT32_MAX) return SA_ERR_ARGUMENT;
+  if (max_new < 1 || max_len < 1 || max_len > width * page_size) return SA_ERR_ARGUMENT;
   if (!cached || !new_tokens || !table || !taken || !starts || !lengths || !cached_out || !taken_out) return SA_ERR_ARGUMENT;
   if ((pool > 0 && !free_pages) || (tokens > 0 && !slots)) return SA_ERR_ARGUMENT;
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -77,6 +88,8 @@ int sa_page_plan(const int32_t* cached, const int32_t* new_tokens, const uint8_t
   c.F = (int)pool;
   c.N = (int)tokens;
   c.pshift = sh;
+  c.max_new = (int)std::min(max_new, tokens);
+  c.max_len = (int)max_len;
   c.slots_here = tokens <= PLAN_SLOTS;
   const int threads = (int)std::min<int64_t>(std::max<int64_t>(align_up(requests, 64), 256), PLAN_THREADS);
   hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3((unsigned)threads), 0, st, c);

@@ -61,6 +61,7 @@ SIGNATURES = {
     "sa_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
     "sa_decode": (_I, [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I, _P]),
     "sa_page_plan": (_I, [_P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P]),
+    "sa_page_plan_within": (_I, [_P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "sa_paged_append": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _I, _P]),
     "sa_paged_attention_workspace_bytes": (_I64, [_I64] * 7 + [_I]),
     "sa_paged_attention": (_I, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64,

@@ -243,11 +243,11 @@ class SelectiveLM(nn.Module):
         request r's next ones (a prompt or a chunk of it, a generated token, none). finished (bool, optional): rows whose
         request has ended and that start anew in this step. max_new, max_len: bounds known to the caller
         (selective_attention_paged). Returns (R, vocab) logits after every request's last new token, and the step's plan: a
-        request whose plan.lengths is 0 was left out for want of pages, and rows without a new token in the step have
-        no meaningful logits."""
+        request whose plan.lengths is 0 was left out, for want of pages or past a bound (nothing of these tokens is cached:
+        they may come again in another step), and rows without a new token in the step have no meaningful logits."""
         make = paged.page_plan if tokens.is_cuda else paged.page_plan_reference
         plan = make(cache["cached"], new, cache["table"], cache["free"], cache["taken"], cache["page_size"], tokens.shape[0],
-                    finished)
+                    finished, max_new, max_len)
         cache["cached"].copy_(plan.cached)
         cache["taken"].copy_(plan.taken)
         x = self._embed(tokens[None])

@@ -8,7 +8,7 @@ pages of one pool (no reference counterpart: the reference's caches hold one bat
 
 One step of a batch, lengths and tables on the GPU throughout:
 
-    plan = page_plan(cached, new, table, free, taken, P, tokens)           # once
+    plan = page_plan(cached, new, table, free, taken, P, tokens)           # once (and any max_new, max_len of the attention)
     paged_append(k, v, k_pages, v_pages, plan.slots)                       # per layer
     y = selective_attention_paged(q, k_pages, v_pages, table, plan.lengths, plan.starts, selected)
 
@@ -72,6 +72,19 @@ def _check_table(table: Tensor, requests: int, device: torch.device) -> tuple[in
                      f"{table.dtype} {tuple(shape)} on {table.device}")
 
 
+def _check_bounds(max_new: int | None, max_len: int | None, tokens: int, holds: int) -> tuple[int, int]:
+    """(max_new, max_len) of a step of `tokens` tokens whose requests have room for `holds` positions."""
+    if max_len is None:
+        max_len = holds
+    elif int(max_len) != max_len or not 1 <= max_len <= holds:
+        raise ValueError(f"max_len must be an integer from 1 to the {holds} positions that there is room for; got {max_len}")
+    if max_new is None:
+        max_new = tokens
+    elif int(max_new) != max_new or max_new < 1:
+        raise ValueError(f"max_new must be an integer >= 1; got {max_new}")
+    return min(int(max_new), tokens), int(max_len)
+
+
 def _check_pages(k_pages: Tensor, v_pages: Tensor) -> tuple[int, int, int, int, torch.dtype, torch.device]:
     """(pages, heads, page size, head dim, dtype, device) of a cache; ValueError unless the kernels can use it."""
     shape, dtype, device = k_pages.shape, k_pages.dtype, k_pages.device
@@ -113,7 +126,7 @@ def _call(device: torch.device, fn, *args) -> None:
 # -- the operators ----------------------------------------------------------------------------------------
 
 def page_plan(cached: Tensor, new: Tensor, table: Tensor, free: Tensor, taken: Tensor, page_size: int, tokens: int,
-              finished: Tensor | None = None) -> PagePlan:
+              finished: Tensor | None = None, max_new: int | None = None, max_len: int | None = None) -> PagePlan:
     """The tables of one step, made on the GPU from the requests' lengths, without a look at them on the host.
 
     cached, new: (R,) int32, the positions each request has in the cache and the tokens it gets in this step (0: none).
@@ -122,9 +135,12 @@ def page_plan(cached: Tensor, new: Tensor, table: Tensor, free: Tensor, taken: T
     the last request are padding). finished: (R,) bool, optional: requests that have ended; their pages go back on the
     stack first (in place), and their rows start anew, with `new` tokens of another request or with none.
 
+    max_new, max_len: the bounds that the step's selective_attention_paged is given, which leaves requests past them out; they
+    are left out of the plan too (where `selected` holds fewer positions than the table, that is such a bound).
+
     Pages are handed out in request order, all that a request needs or none: a request whose pages are not there, whose
-    positions the table cannot hold or whose rows are not among `tokens` is left out of the step (its length 0, its slots
-    -1; `cached` of the plan stays what it was). `cached`, `new` and `taken` are not changed: the plan holds what follows.
+    positions the table cannot hold, whose rows are not among `tokens` or which is past a bound is left out of the step (its
+    length 0, its slots -1; `cached` of the plan stays what it was). `cached`, `new` and `taken` are not changed: the plan holds what follows.
     """
 
     _check_cuda(cached)
@@ -144,13 +160,16 @@ def page_plan(cached: Tensor, new: Tensor, table: Tensor, free: Tensor, taken: T
         raise ValueError("a table row may hold up to 2^30 positions")
     if finished is not None:
         _check_ints("finished", finished, requests, device, torch.bool)
+    tokens = int(tokens)
+    max_new, max_len = _check_bounds(max_new, max_len, tokens, width * page_size)
     lib = _lib.load()
     starts, lengths, after, now_taken = torch.empty(3 * requests + 2, device=device, dtype=torch.int32).split(
         (requests + 1, requests, requests, 1))
-    slots = torch.empty(int(tokens), device=device, dtype=torch.int64)
-    _call(device, lib.sa_page_plan, cached.data_ptr(), new.data_ptr(), None if finished is None else finished.data_ptr(),
+    slots = torch.empty(tokens, device=device, dtype=torch.int64)
+    _call(device, lib.sa_page_plan_within, cached.data_ptr(), new.data_ptr(), None if finished is None else finished.data_ptr(),
           table.data_ptr(), ld, free.data_ptr(), taken.data_ptr(), starts.data_ptr(), lengths.data_ptr(),
-          after.data_ptr(), slots.data_ptr(), now_taken.data_ptr(), requests, width, free.shape[0], int(tokens), page_size)
+          after.data_ptr(), slots.data_ptr(), now_taken.data_ptr(), requests, width, free.shape[0], tokens, page_size,
+          max(max_new, 1), max_len)
     return PagePlan(starts, lengths, after, slots, now_taken)
 
 
@@ -209,17 +228,10 @@ def _check_step(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, leng
     holds = min(width * page_size, state[2], (1 << 30) - 1)
     if holds < 1:
         raise ValueError("selected holds no position")
-    if max_len is None:
-        max_len = holds
-    elif int(max_len) != max_len or not 1 <= max_len <= holds:
-        raise ValueError(f"max_len must be an integer from 1 to the {holds} positions that table and selected hold; got {max_len}")
-    if max_new is None:
-        max_new = tokens
-    elif int(max_new) != max_new or max_new < 1:
-        raise ValueError(f"max_new must be an integer >= 1; got {max_new}")
-    if requests * (heads + state[1] * -(-int(max_len) // 1024)) >= (1 << 24) - 1:   # (workgroups that join parts and write the state)
+    max_new, max_len = _check_bounds(max_new, max_len, tokens, holds)
+    if requests * (heads + state[1] * -(-max_len // 1024)) >= (1 << 24) - 1:   # (workgroups that join parts and write the state)
         raise ValueError(f"a step of {requests} requests of {heads} heads and up to {max_len} positions is too large for one launch")
-    return (requests, tokens, heads, state[1], head_dim, pages, page_size, width, min(int(max_new), tokens), int(max_len), ld,
+    return (requests, tokens, heads, state[1], head_dim, pages, page_size, width, max_new, max_len, ld,
             strides[1], dtype, device, _check_exempt(exempt))
 
 
@@ -238,7 +250,8 @@ def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table
     max_new, max_len: upper bounds, known to the caller, of a request's new tokens and of its positions (default: N, and
     what table and selected hold); they size the launch and its workspace, and max_new=1 runs the single-token
     kernels. A request that exceeds a bound, or has fewer positions than new tokens (0 where page_plan left it out), is
-    left out: its rows are 0, its state stays. Positions whose table entry is not a page of the cache read as zeros.
+    left out: its rows are 0, its state stays (page_plan takes the same bounds, so that such a request's keys are not cached
+    either). Positions whose table entry is not a page of the cache read as zeros.
 
     dot_precision, as the package's other entry points have it: None is "bf16" for a bf16 cache and fp32 arithmetic for the others.
     On a bf16 or fp16 cache steps of several tokens run that type's matrix instructions. With "bf16" the softmax weights are
@@ -273,9 +286,10 @@ def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table
 # -- the same, written plainly ------------------------------------------------------------------------------
 
 def page_plan_reference(cached: Tensor, new: Tensor, table: Tensor, free: Tensor, taken: Tensor, page_size: int, tokens: int,
-                        finished: Tensor | None = None) -> PagePlan:
+                        finished: Tensor | None = None, max_new: int | None = None, max_len: int | None = None) -> PagePlan:
     """page_plan, request after request, on the host."""
 
+    max_new, max_len = _check_bounds(max_new, max_len, tokens, table.shape[1] * page_size)
     pages = lambda n: -(-n // page_size)
     stack, top = free.tolist(), int(taken)
     rows, ended = table.tolist(), [False] * len(table) if finished is None else finished.tolist()
@@ -287,7 +301,7 @@ def page_plan_reference(cached: Tensor, new: Tensor, table: Tensor, free: Tensor
     starts, lengths, after, slots = [0], [], [], []
     asked = given = 0   # pages, by the requests so far and to the last one served
     for row, c, n in zip(rows, have, (max(n, 0) for n in new.tolist())):
-        fits = pages(c + n) <= table.shape[1]
+        fits = pages(c + n) <= table.shape[1] and (n == 0 or (n <= max_new and c + n <= max_len))
         need = pages(c + n) - pages(c) if fits else 0
         asked += need
         served = fits and starts[-1] + n <= tokens and (need == 0 or asked <= len(stack) - top)

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from selective_attention import paged
+from selective_attention import _lib, paged
 from selective_attention.model import ModelConfig, SelectiveLM
 
 
@@ -35,3 +35,68 @@ def test_an_unknown_precision_is_refused():
     model.transformer.h[0].attn.dot_precision = "fp8"
     with pytest.raises(ValueError, match="dot_precision"), torch.no_grad():
         model.paged_step(torch.arange(5), ints(3, 2), model.new_paged_cache(2, 4, 16))
+
+
+def continued(model, device, bounds, left_out):
+    """Two prompts of which a bound leaves one out, the same prompt again without it, and a generated token of both: the
+    logits are those of each request's own prefill. `bounds` of the first step, `left_out` the request past it."""
+    g = torch.Generator().manual_seed(3)
+    counts = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)
+    prompts = [torch.randint(0, 97, (n,), generator=g).to(device) for n in (10, 3)]
+    next_ids = torch.randint(0, 97, (2,), generator=g).to(device)
+    cache = model.new_paged_cache(2, 8, 8, capacity=32)
+    with torch.no_grad():
+        _, plan = model.paged_step(torch.cat(prompts), counts(10, 3), cache, **bounds)
+        want = [0 if r == left_out else len(p) for r, p in enumerate(prompts)]
+        assert plan.lengths.tolist() == want and plan.cached.tolist() == want and cache["cached"].tolist() == want
+        rows = [slice(0, 10), slice(10, 13)]
+        assert (plan.slots[rows[left_out]] == -1).all() and (plan.slots[rows[1 - left_out]] >= 0).all()
+        assert int(cache["taken"]) == sum(-(-n // 8) for n in want)
+        again = [len(p) if r == left_out else 0 for r, p in enumerate(prompts)]
+        model.paged_step(prompts[left_out], counts(*again), cache)
+        logits, plan = model.paged_step(next_ids, counts(1, 1), cache, max_new=1)
+        assert plan.lengths.tolist() == [11, 4]
+        for r in range(2):
+            want = model(torch.cat([prompts[r], next_ids[r:r + 1]])[None])[0][0, 0]
+            torch.testing.assert_close(logits[r], want, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("bounds", [dict(max_new=4), dict(max_len=8), dict(max_new=9, max_len=32)])
+def test_a_request_past_a_bound_is_left_out_of_the_plan(bounds):
+    continued(small_model(), "cpu", bounds, 0)
+
+
+def test_plan_bounds_one_request_at_a_time():
+    """Both bounds, met and passed by one; a request without new tokens is past none of them."""
+    def plan(**kw):
+        table, free = torch.full((4, 8), -1, dtype=torch.int32), torch.arange(20, dtype=torch.int32)
+        for r, held in enumerate((2, 1, 1, 5)):
+            table[r, :held] = 10 + 5 * r + torch.arange(held)
+        return paged.page_plan_reference(ints(9, 4, 0, 40), ints(5, 6, 7, 0), table, free, ints(0), 8, 18, **kw)
+
+    assert plan().lengths.tolist() == [14, 10, 7, 40]
+    assert plan(max_new=7, max_len=14).lengths.tolist() == [14, 10, 7, 40]
+    assert plan(max_new=6, max_len=14).lengths.tolist() == [14, 10, 0, 40]
+    got = plan(max_new=7, max_len=13)
+    assert got.lengths.tolist() == [0, 10, 7, 40] and got.cached.tolist() == [9, 10, 7, 40] and got.starts.tolist() == [0, 5, 11, 18, 18]
+    assert got.slots[:5].eq(-1).all() and got.slots[5:].ge(0).all() and int(got.taken) == 2
+    for wrong in (dict(max_new=0), dict(max_new=1.5), dict(max_len=0), dict(max_len=65), dict(max_len=7.5)):
+        with pytest.raises(ValueError, match="max_"):
+            plan(**wrong)
+
+
+def test_a_refused_bound_leaves_the_cache_as_it_was():
+    model = small_model()
+    cache = model.new_paged_cache(2, 8, 8, capacity=32)
+    for wrong in (dict(max_new=0), dict(max_len=33), dict(max_len=0)):
+        with pytest.raises(ValueError, match="max_"), torch.no_grad():
+            model.paged_step(torch.arange(5), ints(3, 2), cache, **wrong)
+        assert not cache["cached"].any() and not cache["taken"].any() and (cache["table"] == -1).all()
+
+
+def test_abi_refuses_bounds_before_any_launch():
+    lib = _lib.load()
+    fake = 1 << 20   # never dereferenced: validation fails first
+    plan = [fake, fake, None, fake, 8, fake, fake, fake, fake, fake, fake, fake, 4, 8, 100, 10, 16, 10, 128, None]
+    for i, value in ((0, None), (4, 7), (12, 0), (15, -1), (16, 24), (17, 0), (17, -1), (18, 0), (18, 129)):
+        assert lib.sa_page_plan_within(*plan[:i], value, *plan[i + 1:]) == -1, i

@@ -1,12 +1,15 @@
 """Edges of the paged operators on an MI355X: weights far below a row's largest, bounds, rows of no request, values that are not
 finite. Bounds of the comparisons as in tests/paged_cases.py."""
 
+import random
+
 import pytest
 import torch
 
 import selective_attention as sa
-from paged_cases import Step, check
+from paged_cases import Server, Step, check
 from selective_attention.model import ModelConfig, SelectiveLM
+from test_paged_edges_cpu import continued, small_model
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +141,26 @@ def test_a_page_of_nan_is_not_lost(cuda, dtype, new, head_dim, first):
     step.k_pages[int(step.table[0, at // 128]), 1] = float("nan")
     out, _ = attend(step, cuda, max_new=new)
     assert out[:, 1].isnan().all() and not out[:, 0].isnan().any()
+
+
+@pytest.mark.parametrize("requests,width,pool,page_size,most", [(7, 6, 30, 16, 40), (70, 40, 2500, 16, 300), (1300, 5, 6000, 8, 12)])
+def test_plan_with_bounds_matches_the_plain_form(cuda, requests, width, pool, page_size, most):
+    rng = random.Random(requests)
+    a, b = Server(requests, width, pool, page_size), Server(requests, width, pool, page_size, cuda)
+    left_out = 0
+    for turn in range(8):
+        new = [rng.choice([0, 1, 1, 1, rng.randrange(most)]) for _ in range(requests)]
+        ended = [rng.random() < 0.1 for _ in range(requests)]
+        kw = dict(max_new=rng.choice([1, most // 2, most, 10**12]), max_len=rng.choice([page_size, width * page_size // 2 + 3, width * page_size]))
+        want, got = (s.step(lambda *args: plan(*args, **kw), new, None, ended)
+                     for s, plan in ((a, sa.page_plan_reference), (b, sa.page_plan)))
+        for name, x, y in zip(want._fields, want, got):
+            assert torch.equal(x, y.cpu()), (turn, name, kw)
+        assert torch.equal(a.table, b.table.cpu()) and torch.equal(a.free, b.free.cpu()), turn
+        left_out += sum(n > kw["max_new"] for n in new)
+    assert left_out > 0
+
+
+@pytest.mark.parametrize("bounds", [dict(max_new=4), dict(max_len=8)])
+def test_a_request_past_a_bound_is_left_out_of_the_plan(cuda, bounds):
+    continued(small_model().to(cuda), cuda, bounds, 0)
