@@ -240,17 +240,19 @@ class SelectiveLM(nn.Module):
     def paged_step(self, tokens: Tensor, new: Tensor, cache: dict, finished: Tensor | None = None, max_new: int | None = None,
                    max_len: int | None = None) -> tuple[Tensor, paged.PagePlan]:
         """One step of a batch of requests over a paged cache: `tokens` (N,), request after request, new[r] (int32) of them
-        request r's next ones (a prompt or a chunk of it, a generated token, none). finished (bool, optional): rows whose
-        request has ended and that start anew in this step. max_new, max_len: bounds known to the caller
-        (selective_attention_paged). Returns (R, vocab) logits after every request's last new token, and the step's plan: a
+        request r's next ones (a prompt or a chunk of it, a generated token, none; N may be 0, where requests only end).
+        finished (bool, optional): rows whose request has ended and that start anew in this step. max_new, max_len: bounds known
+        to the caller (selective_attention_paged). Returns (R, vocab) logits after every request's last new token, and the step's plan: a
         request whose plan.lengths is 0 was left out, for want of pages or past a bound (nothing of these tokens is cached:
         they may come again in another step), and rows without a new token in the step have no meaningful logits."""
+        x = self._embed(tokens[None])   # (ids that are none raise before the cache is touched)
         make = paged.page_plan if tokens.is_cuda else paged.page_plan_reference
         plan = make(cache["cached"], new, cache["table"], cache["free"], cache["taken"], cache["page_size"], tokens.shape[0],
                     finished, max_new, max_len)
         cache["cached"].copy_(plan.cached)
         cache["taken"].copy_(plan.taken)
-        x = self._embed(tokens[None])
+        if tokens.shape[0] == 0:   # (requests that only end)
+            return self._head(x.new_zeros(new.shape[0], x.shape[-1])), plan
         for block, layer in zip(self.transformer.h, cache["layers"]):
             x = block.step_paged(x, layer, cache["table"], plan, max_new, max_len)
         last = (plan.starts[1:] - 1).clamp_min(0).long()

@@ -100,3 +100,33 @@ def test_abi_refuses_bounds_before_any_launch():
     plan = [fake, fake, None, fake, 8, fake, fake, fake, fake, fake, fake, fake, 4, 8, 100, 10, 16, 10, 128, None]
     for i, value in ((0, None), (4, 7), (12, 0), (15, -1), (16, 24), (17, 0), (17, -1), (18, 0), (18, 129)):
         assert lib.sa_page_plan_within(*plan[:i], value, *plan[i + 1:]) == -1, i
+
+
+def retired(model, device):
+    """A step of no token, in which a request only ends; its pages serve the next."""
+    counts = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)
+    cache = model.new_paged_cache(2, 3, 8, capacity=24)
+    ids = torch.arange(40, device=device)
+    with torch.no_grad():
+        model.paged_step(ids[:19], counts(16, 3), cache)   # every page taken
+        logits, plan = model.paged_step(ids[:0], counts(0, 0), cache, torch.tensor([True, False], device=device))
+        assert logits.shape == (2, 97) and logits.dtype == model.lm_head.weight.dtype and not logits.isnan().any()
+        assert plan.lengths.tolist() == [0, 3] and cache["cached"].tolist() == [0, 3] and int(cache["taken"]) == 1
+        assert plan.starts.tolist() == [0, 0, 0] and plan.slots.numel() == 0
+        logits, plan = model.paged_step(ids[20:33], counts(12, 1), cache)
+        assert plan.lengths.tolist() == [12, 4] and int(cache["taken"]) == 3
+        for r, row in enumerate((ids[20:32], torch.cat([ids[16:19], ids[32:33]]))):
+            torch.testing.assert_close(logits[r], model(row[None])[0][0, 0], rtol=1e-4, atol=1e-4)
+
+
+def test_a_step_without_tokens():
+    retired(small_model(), "cpu")
+
+
+def test_ids_that_are_none_leave_the_cache_as_it_was():
+    model = small_model()
+    cache = model.new_paged_cache(2, 8, 8, capacity=32)
+    for wrong in (torch.zeros(5), torch.full((5,), 97)):
+        with pytest.raises((RuntimeError, IndexError)), torch.no_grad():
+            model.paged_step(wrong, ints(3, 2), cache)
+        assert not cache["cached"].any() and not cache["taken"].any() and (cache["table"] == -1).all()

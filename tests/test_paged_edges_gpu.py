@@ -9,7 +9,7 @@ import torch
 import selective_attention as sa
 from paged_cases import Server, Step, check
 from selective_attention.model import ModelConfig, SelectiveLM
-from test_paged_edges_cpu import continued, small_model
+from test_paged_edges_cpu import continued, retired, small_model
 
 pytestmark = pytest.mark.gpu
 
@@ -164,3 +164,7 @@ def test_plan_with_bounds_matches_the_plain_form(cuda, requests, width, pool, pa
 @pytest.mark.parametrize("bounds", [dict(max_new=4), dict(max_len=8)])
 def test_a_request_past_a_bound_is_left_out_of_the_plan(cuda, bounds):
     continued(small_model().to(cuda), cuda, bounds, 0)
+
+
+def test_a_step_without_tokens(cuda):
+    retired(small_model().to(cuda), cuda)
