@@ -45,7 +45,8 @@ class PagePlan(NamedTuple):
 
 # -- checks ---------------------------------------------------------------------------------------------
 
-# (A step's host work is of the size of its kernels' for small batches, so the checks read each attribute once.)
+# (A step's host work is of the size of its kernels' for small batches, so the checks read each attribute once. What the kernels
+# write or take whole may not be a view that is negated when read: its memory holds other values.)
 
 def _check_page_size(page_size: int) -> int:
     if int(page_size) != page_size or not 8 <= page_size <= 1 << 20 or page_size & (page_size - 1):
@@ -56,7 +57,8 @@ def _check_page_size(page_size: int) -> int:
 def _check_ints(name: str, t: Tensor, size: int | None, device: torch.device, dtype=torch.int32) -> None:
     """A contiguous vector of `size` (None: any) integers."""
     shape = t.shape
-    if t.dtype is not dtype or t.device != device or len(shape) != 1 or (size is not None and shape[0] != size) or not t.is_contiguous():
+    if (t.dtype is not dtype or t.device != device or len(shape) != 1 or (size is not None and shape[0] != size)
+            or not t.is_contiguous() or t.is_neg()):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {'any number of' if size is None else size} elements on "
                          f"{device}; got {t.dtype} {tuple(shape)} on {t.device}")
 
@@ -64,7 +66,8 @@ def _check_ints(name: str, t: Tensor, size: int | None, device: torch.device, dt
 def _check_table(table: Tensor, requests: int, device: torch.device) -> tuple[int, int]:
     """(row stride, width) of a block table."""
     shape = table.shape
-    if table.dtype is torch.int32 and table.device == device and len(shape) == 2 and shape[0] == requests and shape[1] >= 1:
+    if (table.dtype is torch.int32 and table.device == device and len(shape) == 2 and shape[0] == requests and shape[1] >= 1
+            and not table.is_neg()):
         ld, unit = table.stride()
         if unit == 1 and ld >= shape[1]:
             return ld, shape[1]
@@ -94,8 +97,9 @@ def _check_pages(k_pages: Tensor, v_pages: Tensor) -> tuple[int, int, int, int, 
         raise ValueError(f"the cache's dtype must be float16, bfloat16 or float32, one for both; got {dtype}, {v_pages.dtype}")
     if shape[3] not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}; got {shape[3]}")
-    if v_pages.device != device or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise ValueError("k_pages and v_pages must be contiguous, on one device")
+    if (v_pages.device != device or not (k_pages.is_contiguous() and v_pages.is_contiguous())
+            or k_pages.is_neg() or v_pages.is_neg()):
+        raise ValueError("k_pages and v_pages must be contiguous, on one device, with no negation pending")
     return shape[0], shape[1], _check_page_size(shape[2]), shape[3], dtype, device
 
 
@@ -106,7 +110,9 @@ def _check_cuda(t: Tensor) -> None:
 
 def _rows(x: Tensor) -> Tensor:
     """(N, H, D) rows as the kernels read them: 16-byte pieces of contiguous elements, tokens and heads any 16-byte
-    multiple apart (a slice of a packed projection is read in place), tokens less than 2^24 bytes; else a contiguous copy."""
+    multiple apart (a slice of a packed projection is read in place), tokens less than 2^24 bytes; else a contiguous copy (of
+    a view that is negated when read, too)."""
+    x = x.resolve_neg()
     size = x.element_size()
     token, head, unit = x.stride()
     if (unit == 1 and x.shape[2] <= token < (1 << 24) // size and head >= 0 and token * size % 16 == 0 and head * size % 16 == 0
@@ -222,7 +228,8 @@ def _check_step(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, leng
     ld, width = _check_table(table, requests, device)
     state, strides = selected.shape, selected.stride()
     if (len(state) != 3 or state[0] != requests or state[1] < 1 or heads % state[1] != 0 or selected.dtype is not torch.float32
-            or selected.device != device or strides[2] != 1 or strides[0] != state[1] * strides[1] or strides[1] < state[2]):
+            or selected.device != device or strides[2] != 1 or strides[0] != state[1] * strides[1] or strides[1] < state[2]
+            or selected.is_neg()):
         raise ValueError(f"selected must be a ({requests}, G, L) fp32 tensor with G dividing H, rows a fixed stride apart, "
                          f"on q's device; got {selected.dtype} {tuple(state)} on {selected.device}")
     holds = min(width * page_size, state[2], (1 << 30) - 1)

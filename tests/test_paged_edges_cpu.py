@@ -130,3 +130,17 @@ def test_ids_that_are_none_leave_the_cache_as_it_was():
         with pytest.raises((RuntimeError, IndexError)), torch.no_grad():
             model.paged_step(wrong, ints(3, 2), cache)
         assert not cache["cached"].any() and not cache["taken"].any() and (cache["table"] == -1).all()
+
+
+def test_a_pending_negation():
+    """Rows that are negated when read are laid out; tensors that the kernels write or take whole are refused."""
+    x = torch.randn(5, 4, 16).bfloat16()
+    rows = paged._rows(torch._neg_view(-x))
+    assert not rows.is_neg() and torch.equal(rows, x) and paged._rows(x) is x
+    kp, vp = torch.zeros(3, 4, 8, 16), torch.zeros(3, 4, 8, 16)
+    args = dict(q=torch.zeros(2, 4, 16), k_pages=kp, v_pages=vp, table=torch.zeros(1, 2, dtype=torch.int32), lengths=ints(2),
+                starts=ints(0, 2), selected=torch.zeros(1, 1, 16), exempt=1, max_new=None, max_len=None)
+    paged._check_step(**args)
+    for name in ("k_pages", "v_pages", "table", "lengths", "starts", "selected"):
+        with pytest.raises(ValueError):
+            paged._check_step(**{**args, name: torch._neg_view(args[name])})

@@ -168,3 +168,18 @@ def test_a_request_past_a_bound_is_left_out_of_the_plan(cuda, bounds):
 
 def test_a_step_without_tokens(cuda):
     retired(small_model().to(cuda), cuda)
+
+
+def test_a_pending_negation(cuda):
+    """Views that are negated when read: as the same values laid out."""
+    step = Step([30, 3], [20, 1], dtype=torch.bfloat16)
+    args = step.args(cuda)
+    want = sa.selective_attention_paged(*args)
+    args = step.args(cuda)
+    q = torch._neg_view(-args[0])
+    assert q.is_neg() and torch.equal(sa.selective_attention_paged(q, *args[1:]), want)
+    pages = [torch.zeros(4, 4, 16, 64, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    slots = torch.arange(21, device=cuda)
+    k = torch.randn(21, 4, 64, device=cuda).bfloat16()
+    sa.paged_append(torch._neg_view(-k), k, *pages, slots)
+    assert torch.equal(*pages) and pages[0].count_nonzero() > 0
