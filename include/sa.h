@@ -261,6 +261,7 @@ int sa_decode_noalloc(const void* q, const void* k, const void* v, float* out, f
  *   cached_out (requests) what the cache holds after the step
  *   slots      (tokens) page * page_size + row of every token; -1: a request left out, or a row behind the last
  *   taken_out  (1) may be `taken` itself
+ * A page belongs to one request: pages that two rows name are not counted, and go back whenever either has finished.
  * sa_page_plan_within: the same, and a request with more than max_new new tokens, or more than max_len positions after them
  * (up to width * page_size), is left out too: the bounds that the step's sa_paged_attention is given, which leaves such a
  * request out, so that no cache holds positions that the attention has not seen.

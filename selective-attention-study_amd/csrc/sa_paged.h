@@ -4,7 +4,7 @@
 // A cache is k_pages, v_pages (pages, H, P, D): a page holds P consecutive positions of one request, every head's
 // rows together, so that one head's keys of a page are P D contiguous elements. A request's positions are found
 // through its table row: position j in page table[r][j / P], row j % P. The per-key selection state belongs to the
-// request, not to the page (two requests that share a page have asked different queries): (R, G, L) fp32 rows.
+// request, not to the page (it depends on the request's own queries): (R, G, L) fp32 rows.
 //
 // Per request with c cached and n new tokens, t = c + n (operator: sa_kernels.h):
 //   F[i, j] = state[j] (j < c, else 0) + sum over the chunk's queries r < i of relu(s q_sel[r].k_sel[j]),

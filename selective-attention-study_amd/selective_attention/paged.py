@@ -3,8 +3,10 @@ pages of one pool (no reference counterpart: the reference's caches hold one bat
 
     k_pages, v_pages   (pages, H, P, D): P positions of one request per page, P a power of two from 8 on
     table              (R, W) int32: position j of request r is in page table[r, j // P], row j % P
-    selected           (R, G, L) fp32: the selection every cached position has received, per request (two requests
-                       that share a page have had different queries, so this state is not in the pages)
+    selected           (R, G, L) fp32: the selection every cached position has received, from the request's own queries
+
+A page belongs to one request: page_plan gives it out for one and takes it back when that one has ended, whoever else's
+table names it, and counts no holders. (The attention reads pages only, by tables of any making.)
 
 One step of a batch, lengths and tables on the GPU throughout:
 
@@ -139,7 +141,8 @@ def page_plan(cached: Tensor, new: Tensor, table: Tensor, free: Tensor, taken: T
     table: (R, W) int32, extended in place. free: (F,) int32, the pool's page ids, a stack of which the first
     `taken` (a (1,) int32 tensor) are in use. tokens: rows of the step's batch, at least the sum of `new` (rows behind
     the last request are padding). finished: (R,) bool, optional: requests that have ended; their pages go back on the
-    stack first (in place), and their rows start anew, with `new` tokens of another request or with none.
+    stack first (in place), and their rows start anew, with `new` tokens of another request or with none. (All the pages of their
+    `cached` positions: a row that was edited to name another's pages must not be finished here, nor that other one.)
 
     max_new, max_len: the bounds that the step's selective_attention_paged is given, which leaves requests past them out; they
     are left out of the plan too (where `selected` holds fewer positions than the table, that is such a bound).

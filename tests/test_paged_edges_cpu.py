@@ -1,8 +1,11 @@
 """Edges of the paged operators and of the decoder's paged_step without a GPU."""
 
+import random
+
 import pytest
 import torch
 
+from paged_cases import Server, pages_of
 from selective_attention import _lib, paged
 from selective_attention.model import ModelConfig, SelectiveLM
 
@@ -144,3 +147,24 @@ def test_a_pending_negation():
     for name in ("k_pages", "v_pages", "table", "lengths", "starts", "selected"):
         with pytest.raises(ValueError):
             paged._check_step(**{**args, name: torch._neg_view(args[name])})
+
+
+def one_holder(plan, device, seed):
+    """A server's steps, with ends, bounds and a pool that runs out: every page is free or held by one request, once."""
+    rng = random.Random(seed)
+    s = Server(9, 6, 30, 8, device, seed)
+    served = 0
+    for _ in range(40):
+        new = [rng.choice([0, 1, 1, rng.randrange(30)]) for _ in range(9)]
+        ended = [rng.random() < 0.15 for _ in range(9)]
+        kw = dict(max_new=rng.choice([None, 20]), max_len=rng.choice([None, 40]))
+        made = s.step(lambda *args: plan(*args, **kw), new, None, ended)
+        held = [s.table[r, :pages_of(int(s.cached[r]), 8)].tolist() for r in range(9)]
+        assert sorted(sum(held, []) + s.free[int(s.taken):].tolist()) == list(range(30))
+        served += int((made.lengths > 0).sum())
+    assert served > 40
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_page_has_one_holder(seed):
+    one_holder(paged.page_plan_reference, "cpu", seed)

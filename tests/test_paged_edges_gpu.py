@@ -9,7 +9,7 @@ import torch
 import selective_attention as sa
 from paged_cases import Server, Step, check
 from selective_attention.model import ModelConfig, SelectiveLM
-from test_paged_edges_cpu import continued, retired, small_model
+from test_paged_edges_cpu import continued, one_holder, retired, small_model
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +183,8 @@ def test_a_pending_negation(cuda):
     k = torch.randn(21, 4, 64, device=cuda).bfloat16()
     sa.paged_append(torch._neg_view(-k), k, *pages, slots)
     assert torch.equal(*pages) and pages[0].count_nonzero() > 0
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_page_has_one_holder(cuda, seed):
+    one_holder(sa.page_plan, cuda, seed)
