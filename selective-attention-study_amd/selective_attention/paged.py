@@ -263,6 +263,11 @@ def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table
     left out: its rows are 0, its state stays (page_plan takes the same bounds, so that such a request's keys are not cached
     either). Positions whose table entry is not a page of the cache read as zeros.
 
+    The state then holds the selection of all the step's queries. To keep only some of its tokens (a draft that is rejected
+    from somewhere on), put `selected` and page_plan's `cached` and `taken` back as they were before the step, in which no
+    request may have been `finished`, and run the tokens that are kept as a step of their own. (Lowering `cached` alone would
+    lose the pages past it.)
+
     dot_precision, as the package's other entry points have it: None is "bf16" for a bf16 cache and fp32 arithmetic for the others.
     On a bf16 or fp16 cache steps of several tokens run that type's matrix instructions. With "bf16" the softmax weights are
     rounded to the cache's type for the product with the values; with "tf32" or "ieee" they are the sum of two such numbers

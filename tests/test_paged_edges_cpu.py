@@ -168,3 +168,43 @@ def one_holder(plan, device, seed):
 @pytest.mark.parametrize("seed", range(4))
 def test_a_page_has_one_holder(seed):
     one_holder(paged.page_plan_reference, "cpu", seed)
+
+
+def taken_back(ops, device, dtype, rtol, atol):
+    """Drafted tokens verified in one step and two of four kept: with the counts and the state put back, and the kept tokens
+    run again, all is as if the others had never been. The drafts cross into pages that the kept tokens do not reach."""
+    plan, append, attend = ops
+    g = torch.Generator().manual_seed(4)
+    H, D, P = 2, 16, 8
+
+    class Row(Server):
+        def __init__(self):
+            super().__init__(2, 4, 8, P, device)
+            self.pages = [torch.zeros(8, H, P, D, dtype=dtype, device=device) for _ in range(2)]
+            self.selected = torch.zeros(2, 1, 4 * P, device=device)
+
+        def run(self, qkv, new):
+            made = self.step(plan, new)
+            append(qkv[:, 1], qkv[:, 2], *self.pages, made.slots)
+            return attend(qkv[:, 0], *self.pages, self.table, made.lengths, made.starts, self.selected, max_new=max(new))
+
+    tokens = lambda n: torch.randn(n, 3, H, D, generator=g).to(device, dtype)
+    prompt, draft, after = tokens(14 + 7), tokens(4 + 4), tokens(2)
+    kept = torch.cat([draft[:2], draft[4:6]])
+    a, b = Row(), Row()
+    a.run(prompt, [14, 7])
+    b.run(prompt, [14, 7])
+    before = a.cached, a.taken, a.selected.clone()
+    first = a.run(draft, [4, 4])
+    assert int(a.taken) == 5                      # one page more than the kept tokens need
+    a.cached, a.taken = before[:2]
+    a.selected.copy_(before[2])
+    again, want = a.run(kept, [2, 2]), b.run(kept, [2, 2])
+    assert torch.equal(again, want) and torch.equal(a.cached, b.cached) and torch.equal(a.taken, b.taken)
+    torch.testing.assert_close(torch.cat([first[:2], first[4:6]]), again, rtol=rtol, atol=atol)
+    assert torch.equal(a.run(after, [1, 1]), b.run(after, [1, 1])) and torch.equal(a.selected, b.selected)
+
+
+def test_a_step_is_taken_back():
+    taken_back((paged.page_plan_reference, paged.paged_append_reference, paged.selective_attention_paged_reference), "cpu",
+               torch.float32, 1e-5, 1e-6)

@@ -9,7 +9,7 @@ import torch
 import selective_attention as sa
 from paged_cases import Server, Step, check
 from selective_attention.model import ModelConfig, SelectiveLM
-from test_paged_edges_cpu import continued, one_holder, retired, small_model
+from test_paged_edges_cpu import continued, one_holder, retired, small_model, taken_back
 
 pytestmark = pytest.mark.gpu
 
@@ -188,3 +188,10 @@ def test_a_pending_negation(cuda):
 @pytest.mark.parametrize("seed", range(4))
 def test_a_page_has_one_holder(cuda, seed):
     one_holder(sa.page_plan, cuda, seed)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_step_is_taken_back(cuda, dtype):
+    # (fp32: sums of some twenty terms in another order; bf16: outputs and weights rounded, 2^-8 each, of values up to 4)
+    rtol, atol = (1e-5, 1e-5) if dtype == torch.float32 else (2.0**-7, 2.0**-5)
+    taken_back((sa.page_plan, sa.paged_append, sa.selective_attention_paged), cuda, dtype, rtol, atol)
