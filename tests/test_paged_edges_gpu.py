@@ -195,3 +195,44 @@ def test_a_step_is_taken_back(cuda, dtype):
     # (fp32: sums of some twenty terms in another order; bf16: outputs and weights rounded, 2^-8 each, of values up to 4)
     rtol, atol = (1e-5, 1e-5) if dtype == torch.float32 else (2.0**-7, 2.0**-5)
     taken_back((sa.page_plan, sa.paged_append, sa.selective_attention_paged), cuda, dtype, rtol, atol)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("precision", ["bf16", "ieee"])
+@pytest.mark.parametrize("heads,groups", [(4, 1), (8, 2), (2, 1)])
+@pytest.mark.parametrize("cached,new", [([300, 200], [70, 40]), ([1200], [40])])
+def test_large_logits_in_groups(cuda, dtype, precision, heads, groups, cached, new):
+    """Logits of up to some hundreds: rows whose softmax is one key, newer tiles outgrown by older ones."""
+    step = Step(cached, new, heads=heads, groups=groups, dtype=dtype, spread=4.0)
+    out, state = attend(step, cuda, dot_precision=precision)
+    check(out, state, step, ROUNDED[dtype] if precision == "bf16" else WIDE[dtype])
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("precision", ["bf16", "ieee"])
+@pytest.mark.parametrize("heads,groups", [(4, 1), (8, 2), (2, 1)])
+@pytest.mark.parametrize("c", [200, 1500])
+def test_older_tiles_outgrow_newer_ones(cuda, dtype, precision, heads, groups, c):
+    """Steps up of a row's logits from tile to tile, newest first: by slightly less than what the four-head kernel lets pass before
+    it looks for another maximum (2^14 of bf16 weights, 2^5 of fp16's over their 2^10), by slightly more, by far more, for all
+    rows and for every third row only. c = 1500: the tiles are shared out over workgroups."""
+    n = 40
+    step = Step([c], [n], heads=heads, groups=groups, dtype=dtype, exempt=c + n, page_size=8)   # (nothing selects)
+    step.selected[:, :, :c] = 0.0
+    g = torch.Generator().manual_seed(2)
+    log2 = 0.6931
+    k = 0.02 * torch.randn(heads, c + n, 64, generator=g)
+    steps = torch.zeros(c + n)
+    for at, up in ((c - 40, 4.9), (c - 80, 9.7), (c - 110, 9.7 + 13.9), (c - 140, 9.7 + 28.2), (c - 170, 24.0)):
+        steps[at:at + 5] = up * log2     # of every row
+    k[:, :, 0] = steps
+    k[:, c - 190:c - 185, 1] = 60.0 * log2   # of every third row: far more
+    k[:, c - 60, 1] = 14.1 * log2
+    put(step, 0, k, torch.randn(heads, c + n, 64, generator=g) + 0.5)
+    q = 0.02 * torch.randn(n, heads, 64, generator=g)
+    q[..., 0] = 8.0
+    q[..., 1] = 0.0
+    q[::3, :, 1] = 8.0
+    step.q = q.to(dtype)
+    out, state = attend(step, cuda, dot_precision=precision)
+    check(out, state, step, ROUNDED[dtype] if precision == "bf16" else WIDE[dtype])
