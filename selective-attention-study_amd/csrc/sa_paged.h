@@ -1406,8 +1406,8 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
   };
 
   auto attend = [&](int kt, const Tiles& B, const float* F) __attribute__((always_inline)) {
-    f32x16 lg;
     auto logits = [&]() __attribute__((always_inline)) {
+      f32x16 lg;
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const float4 f4 = *reinterpret_cast<const float4*>(F + n * LDF + 8 * q4 + 4 * h);
@@ -1423,8 +1423,9 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
 #pragma unroll
         for (int i = 0; i < 16; ++i) lg[i] = crow(i, 0) <= thr ? lg[i] : -INFINITY;
       }
+      return lg;
     };
-    logits();
+    f32x16 lg = logits();
     u32x4 pf[2], pr[2];
     float psum;
     auto weights = [&]() __attribute__((always_inline)) {
@@ -1447,7 +1448,7 @@ __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const flo
     if (__builtin_expect(__any(!(psum <= P::BIG)), 0)) {
       if constexpr (WIDE) {   // the logits again: kept, they would not fit the registers beside the weights' halves
         __asm__ volatile("" ::: "memory");   // (nor would what they were made from)
-        logits();
+        lg = logits();
       }
       float zmax = lg[0];
 #pragma unroll
