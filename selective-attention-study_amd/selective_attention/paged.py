@@ -23,6 +23,7 @@ The `_reference` functions are the same in plain torch (any device), as `kernels
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -47,8 +48,9 @@ class PagePlan(NamedTuple):
 
 # -- checks ---------------------------------------------------------------------------------------------
 
-# (A step's host work is of the size of its kernels' for small batches, so the checks read each attribute once. What the kernels
-# write or take whole may not be a view that is negated when read: its memory holds other values.)
+# (A step's host work is of the size of its kernels' for small batches, so the checks read each attribute once. A
+# negation can be pending on q, k and v only: what torch makes such views of, the imaginary parts of complex tensors, is no int
+# and not contiguous, and the other checks refuse it.)
 
 def _check_page_size(page_size: int) -> int:
     if int(page_size) != page_size or not 8 <= page_size <= 1 << 20 or page_size & (page_size - 1):
@@ -60,7 +62,7 @@ def _check_ints(name: str, t: Tensor, size: int | None, device: torch.device, dt
     """A contiguous vector of `size` (None: any) integers."""
     shape = t.shape
     if (t.dtype is not dtype or t.device != device or len(shape) != 1 or (size is not None and shape[0] != size)
-            or not t.is_contiguous() or t.is_neg()):
+            or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {'any number of' if size is None else size} elements on "
                          f"{device}; got {t.dtype} {tuple(shape)} on {t.device}")
 
@@ -68,8 +70,7 @@ def _check_ints(name: str, t: Tensor, size: int | None, device: torch.device, dt
 def _check_table(table: Tensor, requests: int, device: torch.device) -> tuple[int, int]:
     """(row stride, width) of a block table."""
     shape = table.shape
-    if (table.dtype is torch.int32 and table.device == device and len(shape) == 2 and shape[0] == requests and shape[1] >= 1
-            and not table.is_neg()):
+    if table.dtype is torch.int32 and table.device == device and len(shape) == 2 and shape[0] == requests and shape[1] >= 1:
         ld, unit = table.stride()
         if unit == 1 and ld >= shape[1]:
             return ld, shape[1]
@@ -90,6 +91,13 @@ def _check_bounds(max_new: int | None, max_len: int | None, tokens: int, holds: 
     return min(int(max_new), tokens), int(max_len)
 
 
+@functools.lru_cache(maxsize=None)
+def _attention_code(dot_precision: str | None, dtype: torch.dtype) -> int:
+    """sa_paged_attention's dtype argument."""
+    wide = _resolve_precision(dot_precision, dtype) == _lib.DTYPE_F32
+    return _CODES[dtype] | (_lib.WIDE_WEIGHTS if wide else 0)
+
+
 def _check_pages(k_pages: Tensor, v_pages: Tensor) -> tuple[int, int, int, int, torch.dtype, torch.device]:
     """(pages, heads, page size, head dim, dtype, device) of a cache; ValueError unless the kernels can use it."""
     shape, dtype, device = k_pages.shape, k_pages.dtype, k_pages.device
@@ -99,9 +107,8 @@ def _check_pages(k_pages: Tensor, v_pages: Tensor) -> tuple[int, int, int, int, 
         raise ValueError(f"the cache's dtype must be float16, bfloat16 or float32, one for both; got {dtype}, {v_pages.dtype}")
     if shape[3] not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}; got {shape[3]}")
-    if (v_pages.device != device or not (k_pages.is_contiguous() and v_pages.is_contiguous())
-            or k_pages.is_neg() or v_pages.is_neg()):
-        raise ValueError("k_pages and v_pages must be contiguous, on one device, with no negation pending")
+    if v_pages.device != device or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages must be contiguous, on one device")
     return shape[0], shape[1], _check_page_size(shape[2]), shape[3], dtype, device
 
 
@@ -114,11 +121,10 @@ def _rows(x: Tensor) -> Tensor:
     """(N, H, D) rows as the kernels read them: 16-byte pieces of contiguous elements, tokens and heads any 16-byte
     multiple apart (a slice of a packed projection is read in place), tokens less than 2^24 bytes; else a contiguous copy (of
     a view that is negated when read, too)."""
-    x = x.resolve_neg()
     size = x.element_size()
     token, head, unit = x.stride()
     if (unit == 1 and x.shape[2] <= token < (1 << 24) // size and head >= 0 and token * size % 16 == 0 and head * size % 16 == 0
-            and x.data_ptr() % 16 == 0):
+            and x.data_ptr() % 16 == 0 and not x.is_neg()):
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -231,8 +237,7 @@ def _check_step(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, leng
     ld, width = _check_table(table, requests, device)
     state, strides = selected.shape, selected.stride()
     if (len(state) != 3 or state[0] != requests or state[1] < 1 or heads % state[1] != 0 or selected.dtype is not torch.float32
-            or selected.device != device or strides[2] != 1 or strides[0] != state[1] * strides[1] or strides[1] < state[2]
-            or selected.is_neg()):
+            or selected.device != device or strides[2] != 1 or strides[0] != state[1] * strides[1] or strides[1] < state[2]):
         raise ValueError(f"selected must be a ({requests}, G, L) fp32 tensor with G dividing H, rows a fixed stride apart, "
                          f"on q's device; got {selected.dtype} {tuple(state)} on {selected.device}")
     holds = min(width * page_size, state[2], (1 << 30) - 1)
@@ -281,9 +286,7 @@ def selective_attention_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, table
     _check_cuda(k_pages)
     (requests, tokens, heads, groups, head_dim, pages, page_size, width, max_new, max_len, table_ld, state_ld, dtype, device,
      exempt) = _check_step(q, k_pages, v_pages, table, lengths, starts, selected, exempt, max_new, max_len)
-    code = _CODES[dtype]
-    if _resolve_precision(dot_precision, dtype) == _lib.DTYPE_F32:
-        code |= _lib.WIDE_WEIGHTS
+    code = _attention_code(dot_precision, dtype)
     out = torch.empty(tokens, heads, head_dim, device=device, dtype=dtype)
     if tokens == 0:
         return out
