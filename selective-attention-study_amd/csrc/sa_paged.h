@@ -625,7 +625,7 @@ __device__ __forceinline__ float least_of(float x) {
 // of its own key, which has no history. Below -REACH_ZERO a weight is an exact fp32 zero (in one part of several: once they
 // are joined; LIFTed ones: nothing beside the row's sum, at 2^-122 of it), and the tile is left out for all of the workgroup's heads together; tiles for which a NaN or an infinity enters
 // the bound stay. A mask in LDS, bit i the i-th newest tile; past the mask's end every tile stays. A chunk of
-// 4096 queries at 32768 keys, 16 heads, of N(0,1) inputs: 849 us -> 133; where the histories leave the oldest fifth without
+// 4096 queries at 32768 keys, 16 heads, of N(0,1) inputs: 849 us -> 133, the whole call; where the histories leave the oldest fifth without
 // weight 800 -> 770; where they are too small everywhere 98 -> 104 (prompts of 60 to 2000 tokens), the rows and norms for nothing.
 //
 // A part of several takes an equal share of the tiles that stay (of some SHARE_TILES at least: a short request's last parts may
@@ -1306,9 +1306,10 @@ __global__ __launch_bounds__(NW * 64, (NW == 1 ? 1 : (sizeof(typename P::elem) =
 // weights are taken against the reference mu of the tiles before, and only where a row's sum of them over half a tile
 // passes BIG (or a row has no reference yet) is the maximum looked for, mu moved and the tile's weights taken again.
 // Any reference within 2^14 of the maximum gives the same bf16 weights to rounding; fp16's (LIFT times larger) stay within 2^5 of it,
-// so that none passes the type's largest number. At 4096 queries on
-// 32768 keys, 16 heads: 0.80 ms (644 TFLOP/s of the two products), paged_fwd_kernel 1.04 (every tile computed); with the selection after the products 0.91,
-// with eight wavefronts of two query tiles each 0.97 (0.91). What is left over is each step's common start and end: its LDS reads
+// so that none passes the type's largest number.
+// At 4096 queries on 32768 keys, 16 heads, every tile computed, under the profiler: 0.78 ms (657 TFLOP/s of the two products; 0.80
+// before PagedLive's equal shares), paged_fwd_kernel 1.04, with the selection after the products 0.91, with eight wavefronts of two
+// query tiles each 0.97 (0.91). What is left over is each step's common start and end: its LDS reads
 // at once (0.46 ms without selection, value products and loads), and the wait for its last wavefront.
 template <class P, bool WIDE>
 __global__ __launch_bounds__(1024) void paged_fwd4_kernel(PagedCall a, const float* __restrict__ carry, int64_t carry_ld,
