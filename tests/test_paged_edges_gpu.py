@@ -236,3 +236,42 @@ def test_older_tiles_outgrow_newer_ones(cuda, dtype, precision, heads, groups, c
     step.q = q.to(dtype)
     out, state = attend(step, cuda, dot_precision=precision)
     check(out, state, step, ROUNDED[dtype] if precision == "bf16" else WIDE[dtype])
+
+
+def test_a_decoders_step_is_captured(cuda):
+    """paged_step in a graph, replayed as the requests grow, with a request that ends and starts again: the logits and the counts
+    of eager steps, bounds and all."""
+    torch.manual_seed(0)
+    cfg = ModelConfig(vocab_size=97, n_layers=2, d_model=256, n_heads=4, context_length=64)
+    model = SelectiveLM(cfg).to(cuda, torch.bfloat16).eval()
+    caches = [model.new_paged_cache(3, 12, 16, capacity=64) for _ in range(2)]
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)
+    tensors = lambda cache: [cache[k] for k in ("table", "free", "taken", "cached")] + [x for layer in cache["layers"] for x in layer.values()]
+    g = torch.Generator().manual_seed(1)
+    ids, new, ended = (torch.zeros(8, dtype=torch.int64, device=cuda), ints(0, 0, 0), torch.zeros(3, dtype=torch.bool, device=cuda))
+    with torch.no_grad():
+        prompt = torch.randint(0, 97, (20,), generator=g).to(cuda)
+        for cache in caches:
+            model.paged_step(prompt, ints(9, 11, 0), cache)
+        step = lambda cache: model.paged_step(ids, new, cache, ended, max_new=6, max_len=64)
+        kept = [x.clone() for x in tensors(caches[1])]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(caches[1])   # warm-up, undone below
+        torch.cuda.current_stream().wait_stream(side)
+        for x, y in zip(tensors(caches[1]), kept):
+            x.copy_(y)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits, plan = step(caches[1])
+        for counts, ends in (((1, 1, 6), None), ((2, 1, 1), None), ((7, 1, 0), None), ((3, 0, 5), (1, 0, 0)), ((1, 1, 1), None)):
+            ids.copy_(torch.randint(0, 97, (8,), generator=g))
+            new.copy_(ints(*counts))
+            ended.copy_(torch.tensor(ends or (0, 0, 0), device=cuda).bool())
+            graph.replay()
+            want, made = step(caches[0])
+            torch.cuda.synchronize()
+            rows = [r for r in range(3) if counts[r] and int(made.lengths[r])]
+            assert all(torch.equal(x, y) for x, y in zip(made, plan)) and torch.equal(want[rows], logits[rows]), counts
+            assert all(torch.equal(x, y) for x, y in zip(tensors(caches[0]), tensors(caches[1]))), counts
