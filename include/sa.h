@@ -39,7 +39,7 @@ extern "C" {
 
 #define SA_DTYPE_BF16 0
 #define SA_DTYPE_F32 1
-#define SA_DTYPE_F16 2          /* the paged cache's entry points only */
+#define SA_DTYPE_F16 2          /* the entry points from sa_page_plan on */
 #define SA_WIDE_WEIGHTS 16      /* sa_paged_attention: or'ed to a 16-bit dtype (fp32: no change) */
 
 #define SA_OK 0
@@ -304,6 +304,69 @@ int sa_paged_attention(const void* q, int64_t q_token, int64_t q_head, const voi
                        int64_t state_ld, void* workspace, int64_t workspace_bytes, int64_t requests, int64_t tokens,
                        int64_t heads, int64_t groups, int64_t head_dim, int64_t pages, int64_t page_size, int64_t width,
                        int64_t max_new, int64_t max_len, float scale, int dtype, int exempt, void* stream);
+
+/*
+ * The operators of a decoder around its attention layers. Element types are SA_DTYPE_*, of each tensor its own unless said
+ * otherwise; rows are contiguous, and an *_ld is the number of elements from a row to the next (0: one row for all).
+ * Arithmetic, statistics and sums are fp32, results are rounded once. Equal calls give equal bits.
+ *
+ * Layer norm, alone or after a residual addition:
+ *     s = x + branch (branch null: s = x and `sum` is not written), rounded to x's type and stored in `sum`
+ *     y = weight (s - mean) rstd + bias,   rstd = 1 / sqrt(var + eps) over the row's `width` (1 to 32768) elements
+ * bias may be null; mean, rstd (rows, fp32) are written where not null (the backward pass takes them). y and sum are
+ * (rows, width), sum of x's type; bias has the weight's.
+ * Backward: s (x without a branch), dy of y's type, ds (null: zero) of s's type; dx, dbranch (each may be null) get the same gradient in
+ * their own types; dweight, dbias (each may be null) the sums over the rows, for which the workspace (16-byte aligned) is.
+ */
+int sa_layer_norm(const void* x, int64_t x_ld, const void* branch, int64_t branch_ld, const void* weight, const void* bias, void* y,
+                  void* sum, float* mean, float* rstd, int64_t rows, int64_t width, float eps, int x_dtype, int branch_dtype,
+                  int y_dtype, int weight_dtype, void* stream);
+int64_t sa_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int sa_layer_norm_backward(const void* s, int64_t s_ld, const void* dy, int64_t dy_ld, const void* ds, int64_t ds_ld,
+                           const void* weight, const float* mean, const float* rstd, void* dx, void* dbranch, void* dweight,
+                           void* dbias, void* workspace, int64_t workspace_bytes, int64_t rows, int64_t width, int s_dtype,
+                           int branch_dtype, int y_dtype, int weight_dtype, void* stream);
+
+/*
+ * Embedding: out (tokens, width) = scale * weight rows at ids (int32 or int64: ids_bytes 4 or 8), all of one type. An id outside
+ * [0, vocab) gives a row of NaN and no gradient. Backward: dweight (vocab, width) = scale * the sums of dout's rows by id, in token
+ * order; every row is written, zeros for ids without a token. tokens < 2^30, vocab < 2^28, width < 2^24.
+ */
+int sa_embedding(const void* ids, int ids_bytes, const void* weight, int64_t weight_ld, void* out, int64_t tokens, int64_t vocab,
+                 int64_t width, float scale, int dtype, void* stream);
+int64_t sa_embedding_backward_workspace_bytes(int64_t tokens, int64_t vocab, int64_t width);
+int sa_embedding_backward(const void* ids, int ids_bytes, const void* dout, int64_t dout_ld, void* dweight, void* workspace,
+                          int64_t workspace_bytes, int64_t tokens, int64_t vocab, int64_t width, float scale, int dtype,
+                          void* stream);
+
+/*
+ * Softmax cross entropy over a vocabulary, from hidden states x (tokens, width) and the output head's weight (vocab, width), without
+ * the logits in memory:
+ *     loss_i = log sum_v exp(x_i . weight_v) - x_i . weight_{target_i};   0 where target_i = ignore
+ * reduction: SA_REDUCE_NONE loss (tokens), _MEAN over the tokens that are not ignored (NaN if there is none), _SUM: loss (1). A target
+ * outside [0, vocab) that is not `ignore` gives NaN. dtype: the type of the products' operands, to which x and weight are rounded where
+ * theirs differs; products accumulate in fp32.
+ * lse (tokens, fp32) and rows (64 + 2 tokens ints) are what the backward pass takes (tokens not ignored, and their normalisers); lse
+ * null: no backward pass follows (rows is scratch then). The workspace's size depends on the strides and alignment of x and weight, so its query takes the
+ * same pointers (which it does not read).
+ * Backward: dloss fp32, (tokens) or (1) by reduction; dx (tokens, width) of x's type, dweight (vocab, width) of weight's, 16-byte aligned;
+ * either may be null. The logits are computed again, a piece of the vocabulary at a time. 1 to 2^28 - 1 tokens and vocabulary
+ * rows, width up to 2^16.
+ */
+#define SA_REDUCE_NONE 0
+#define SA_REDUCE_MEAN 1
+#define SA_REDUCE_SUM 2
+int64_t sa_linear_xent_workspace_bytes(const void* x, int64_t x_ld, const void* weight, int64_t weight_ld, int64_t tokens,
+                                       int64_t vocab, int64_t width, int reduction, int train, int x_dtype, int weight_dtype, int dtype);
+int sa_linear_xent(const void* x, int64_t x_ld, const void* weight, int64_t weight_ld, const int64_t* targets, float* loss, float* lse,
+                   int32_t* rows, void* workspace, int64_t workspace_bytes, int64_t tokens, int64_t vocab, int64_t width,
+                   int64_t ignore, int reduction, int x_dtype, int weight_dtype, int dtype, void* stream);
+int64_t sa_linear_xent_backward_workspace_bytes(const void* weight, int64_t weight_ld, int64_t tokens, int64_t vocab, int64_t width,
+                                                int need_dx, int need_dweight, int weight_dtype, int dtype);
+int sa_linear_xent_backward(const void* x, int64_t x_ld, const void* weight, int64_t weight_ld, const int64_t* targets,
+                            const float* lse, const int32_t* rows, const float* dloss, void* dx, void* dweight, void* workspace,
+                            int64_t workspace_bytes, int64_t tokens, int64_t vocab, int64_t width, int reduction, int x_dtype,
+                            int weight_dtype, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,9 @@
 #   sa_f32.hip   fp32-storage kernels, the compiler's own accumulator placement
 #   sa_paged_bf16.hip, sa_paged_f16.hip, sa_paged_f32.hip  attention over a paged cache of that type
 #   sa_paged.hip the paged cache's C ABI, its tables and its write
+#   sa_norm.hip, sa_embed.hip  layer norm and embedding with their gradients, and their C ABI
+#   sa_xent_bf16.hip, sa_xent_f16.hip, sa_xent_f32.hip  the vocabulary loss with products of that type
+#   sa_xent.hip  its C ABI
 #   sa_abi.hip   the C ABI (host code only)
 # Every HIP compile: -packed-fp32-ops off (no v_pk_*_f32 from the compiler).
 set -euo pipefail
@@ -72,6 +75,18 @@ unit sa_paged_f32.hip sa_paged_f32.o &
 p11=$!
 unit sa_paged.hip sa_paged.o &
 p12=$!
+unit sa_norm.hip sa_norm.o &
+p13=$!
+unit sa_embed.hip sa_embed.o &
+p14=$!
+unit sa_xent_bf16.hip sa_xent_bf16.o -mllvm -amdgpu-mfma-vgpr-form &
+p15=$!
+unit sa_xent_f16.hip sa_xent_f16.o -mllvm -amdgpu-mfma-vgpr-form &
+p16=$!
+unit sa_xent_f32.hip sa_xent_f32.o &
+p17=$!
+unit sa_xent.hip sa_xent.o &
+p18=$!
 rc=0
 wait $p1 || rc=1
 wait $p2 || rc=1
@@ -85,9 +100,16 @@ wait $p9 || rc=1
 wait $p10 || rc=1
 wait $p11 || rc=1
 wait $p12 || rc=1
+wait $p13 || rc=1
+wait $p14 || rc=1
+wait $p15 || rc=1
+wait $p16 || rc=1
+wait $p17 || rc=1
+wait $p18 || rc=1
 [ $rc -eq 0 ] || { echo "build.sh: a compile failed" >&2; exit 1; }
 hipcc --offload-arch=gfx950 -shared -fPIC "$tmp/sa_bf16.o" "$tmp/sa_bf16_kv.o" "$tmp/sa_bf16_kv1.o" "$tmp/sa_bf16_kvg.o" "$tmp/sa_bf16_dec.o" "$tmp/sa_bf16_prep.o" "$tmp/sa_f32.o" \
   "$tmp/sa_paged_bf16.o" "$tmp/sa_paged_f16.o" "$tmp/sa_paged_f32.o" "$tmp/sa_paged.o" "$tmp/sa_abi.o" \
+  "$tmp/sa_norm.o" "$tmp/sa_embed.o" "$tmp/sa_xent_bf16.o" "$tmp/sa_xent_f16.o" "$tmp/sa_xent_f32.o" "$tmp/sa_xent.o" \
   -o "$out.tmp"
 mv "$out.tmp" "$out"
 echo "built $out"

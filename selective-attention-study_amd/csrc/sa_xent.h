@@ -1,0 +1,875 @@
+// Softmax cross entropy of a large vocabulary from hidden states and the output head's matrix (include/sa.h:
+// sa_linear_xent), without the logits kept.
+//
+//   l[i, v] = x_i . W_v;   lse_i = log sum_v exp l[i, v];   loss_i = lse_i - l[i, t_i]
+//   G[i, v] = exp(l[i, v] - lse_i) - [v = t_i];   dx_i = g_i sum_v G[i, v] W_v;   dW_v = sum_i g_i G[i, v] x_i
+//
+// Tokens whose target is ignored are taken out first (xent_rows: the kept tokens' numbers, in order, and how many; the
+// count stays on the device and bounds the launches that follow), so they cost nothing and nothing in their rows (a NaN, an
+// infinity) reaches a result.
+//
+//   xent_rows, xent_gather   the kept tokens' rows, in the products' type, padded to whole stages of the contraction
+//   xent_logits              logits of a tile (vocabulary x tokens: a lane holds one token's, so its maximum and sum are taken in
+//                            registers); a token's maximum, sum and target logit per tile of the vocabulary go to the workspace
+//   xent_join, xent_sum      the tiles' statistics joined: lse, loss; the mean or the sum
+//   xent_logits (again)      backward, a piece of the vocabulary at a time: the tile's logits computed again, G in the products' type
+//   xent_product             dX += G W_piece (fp32 in the workspace across the pieces), dW_piece = G^T X
+//   xent_finish_x, _w        scale, add the parts of a split contraction, convert
+//
+// All products run through one tile loop on matrix instructions with fp32 accumulation (Mainloop). Statistics, lse and losses are
+// fp32. G is rounded to the products' type: half a step of it (bf16 2^-9 to 2^-8 of each entry), the size of the gradients' own
+// rounding; fp16 holds G at 2^14 times its size, as a vocabulary's probabilities lie below that type's normal range. The factor
+// and a common g are applied to the fp32 sums; tokens' own g_i (reduction none) to G before it is rounded.
+
+#pragma once
+
+#include <math.h>
+
+#include "sa_lm.h"
+
+namespace sa_host {
+
+struct XentCall {
+  const void *x, *w;            // the caller's rows
+  const int64_t* targets;
+  const float* dloss;
+  float *loss, *lse;            // lse: per kept token, base 2; null where no backward pass follows
+  int* rows;                    // [0] kept tokens, [64 ..] their numbers, [64 + tokens ..] each token's place among them or -1
+  void *dx, *dw;
+  void* ws;
+  int64_t x_ld, w_ld, tokens, vocab, width, ignore;
+  int x_t, w_t, reduction;
+  int cus;
+  hipStream_t st;
+};
+int64_t xent_bytes_bf16(const XentCall& c, bool backward);
+int64_t xent_bytes_f16(const XentCall& c, bool backward);
+int64_t xent_bytes_f32(const XentCall& c, bool backward);
+int xent_bf16(const XentCall& c, bool backward);
+int xent_f16(const XentCall& c, bool backward);
+int xent_f32(const XentCall& c, bool backward);
+
+}  // namespace sa_host
+
+namespace {
+
+typedef float f32x16 __attribute__((__vector_size__(16 * sizeof(float))));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((__vector_size__(8 * sizeof(bf16_t))));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_void_ptr;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int ROWS_HEAD = 64;   // ints before the kept tokens' numbers
+
+// ---------------------------------------------------------------------------------------------
+// Operand types. A lane's operand of one step is 16 bytes of its row (lanes 0-31 the even, 32-63 the odd 16 bytes): one instruction for
+// 16-bit types, four for fp32, each of which contracts element e of both halves' four (the order of a contraction is
+// free as long as both operands have the same).
+
+struct XBF16 {
+  typedef uint16_t elem;
+  static constexpr int CODE = SA_DTYPE_BF16;
+  static constexpr float LIFT = 1.f;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+struct XF16 {
+  typedef uint16_t elem;
+  static constexpr int CODE = SA_DTYPE_F16;
+  static constexpr float LIFT = 16384.f;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+struct XF32 {
+  typedef float elem;
+  static constexpr int CODE = SA_DTYPE_F32;
+  static constexpr float LIFT = 1.f;
+  static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  }
+};
+
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+__device__ __forceinline__ lds_void_ptr lds_at(const void* p) { return (lds_void_ptr)(uint32_t)(uintptr_t)p; }
+// element i of a 32 x 32 accumulator: column lane % 32, row acc_row(i, lane / 32)
+__device__ __forceinline__ constexpr int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_t bytes) {   // loads past `bytes` give zero
+  const int64_t most = 0x7fffffff;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)(bytes < 0 ? 0 : bytes < most ? bytes : most), 0x00020000);
+}
+
+// ---------------------------------------------------------------------------------------------
+// One operand of a tile: EDGE rows (or columns) of the result, KB = 128 bytes of the contraction per stage.
+//
+// Plain: the matrix has the contraction along its rows. A stage holds EDGE rows of 128 bytes; the 16-byte chunk c of row r sits at
+// chunk c ^ (r mod 8), so that the 32 lanes of a fragment read (one chunk of 32 rows) touch all banks evenly.
+// Turned (TR): the matrix has the contraction down its columns (K, EDGE). A stage holds 128 / size rows of EDGE elements, and
+// the fragments are read transposed: 16-bit types by ds_read_b64_tr_b16 (lane i of 16 gets as element t the element i % 4 of
+// the 8 bytes that lane 4t + i/4 addresses: four rows of a 16-column range, whose 32 bytes sit at chunk c ^ 2 (r mod 4), so that
+// the four rows fall on different banks), fp32 by one 4-byte read per instruction (32 neighbours of a row).
+//
+// The loads go from memory straight into LDS: one instruction fills 64 consecutive 16-byte slots, and each lane fetches the
+// chunk that belongs in its slot. Rows past the resource's end read as zeros.
+template <class OP, int EDGE, bool TR, int WAVES>
+struct Operand {
+  static constexpr int ES = sizeof(typename OP::elem);
+  static constexpr int BYTES = EDGE * 128;
+  static constexpr int BK = 128 / ES;
+  static constexpr int ROW = TR ? EDGE * ES : 128;        // bytes of a staged row
+  static constexpr int LANES = ROW / 16 < 64 ? ROW / 16 : 64;   // lanes of an instruction on one row
+  static constexpr int RPI = 64 / LANES;                  // rows of an instruction
+  static constexpr int IPR = ROW / (16 * LANES);          // instructions of a row
+  static constexpr int LOADS = BYTES / 1024;              // instructions of a stage
+  static constexpr int PER = LOADS / WAVES;
+  static_assert(LOADS % WAVES == 0, "whole loads per wavefront");
+
+  __amdgpu_buffer_rsrc_t rs;
+  int lane_off, ld;   // bytes
+
+  // p: the tile's first row (plain) or column (turned), at the contraction's start; bytes: what may be read from there
+  __device__ __forceinline__ void open(const void* p, int64_t bytes, int64_t ld_elems) {
+    rs = resource(p, bytes);
+    ld = (int)(ld_elems * ES);
+    const int lane = threadIdx.x & 63;
+    const int r = lane / LANES, pos = lane % LANES;
+    int c;
+    if constexpr (!TR) c = pos ^ (r & 7);
+    else c = pos;   // (the turned swizzle depends on the row within four: below)
+    lane_off = r * ld + c * 16;
+  }
+  // stage k of the contraction into `to` (the wavefront's share)
+  __device__ __forceinline__ void load(uint8_t* to, int k, int wave) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int n = wave * PER + i;
+      int voff, soff;
+      if constexpr (!TR) {
+        voff = lane_off;
+        soff = n * RPI * ld + k * 128;
+      } else {
+        const int r0 = (n / IPR) * RPI;   // first row of the instruction
+        if constexpr (ES == 2) {
+          const int pos = lane % LANES + (n % IPR) * LANES, r = r0 + lane / LANES;
+          voff = (lane / LANES) * ld + ((pos ^ ((r & 3) << 1)) * 16);
+        } else {
+          voff = lane_off + (n % IPR) * 1024;
+        }
+        soff = (k * BK + r0) * ld;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(to + 1024 * n), 16, voff, soff, 0, 0);
+    }
+  }
+  // the fragment of step j (four per stage) of rows (columns) first .. first + 31
+  static __device__ __forceinline__ u32x4 frag(const uint8_t* t, int first, int j) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (!TR) {
+      const int r = first + (lane & 31);
+      return *reinterpret_cast<const u32x4*>(t + r * 128 + (((2 * j + h) ^ (lane & 7)) << 4));
+    } else if constexpr (ES == 2) {
+      const int g = lane >> 4, k = lane & 15;
+      u32x4 f;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int r = 16 * j + 8 * (g >> 1) + 4 * hf + (k >> 2);
+        const int c = (first >> 3) + 2 * (g & 1) + ((k & 3) >> 1);
+        typedef __attribute__((address_space(3))) short4v* lds_s4;
+        const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s4)(uint32_t)(uintptr_t)(t + r * ROW + ((c ^ ((r & 3) << 1)) << 4) + 8 * (k & 1)));
+        const uint2 u = __builtin_bit_cast(uint2, v);
+        f[2 * hf] = u.x;
+        f[2 * hf + 1] = u.y;
+      }
+      return f;
+    } else {
+      u32x4 f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f[e] = *reinterpret_cast<const uint32_t*>(t + (8 * j + 4 * h + e) * ROW + (first + (lane & 31)) * 4);
+      return f;
+    }
+  }
+};
+
+// A tile of WM x WN wavefronts, each TM x TN squares of 32: acc[a][b] += A B^T over `stages` of the contraction. Two stages in LDS, in
+// variables of their own (one array indexed by the stage's parity makes the compiler wait for the loads in flight before it reads).
+template <class OP, int WM_, int WN_, int TM_, int TN_, bool TRA, bool TRB>
+struct Mainloop {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
+  typedef Operand<OP, BM, TRA, WAVES> A;
+  typedef Operand<OP, BN, TRB, WAVES> B;
+  static constexpr int BK = A::BK;
+  struct Stage {
+    alignas(1024) uint8_t a[A::BYTES];
+    alignas(1024) uint8_t b[B::BYTES];
+  };
+  f32x16 acc[TM][TN];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TN; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
+  }
+  __device__ __forceinline__ void step(const Stage& s, int wm, int wn) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u32x4 fa[TM], fb[TN];
+#pragma unroll
+      for (int a = 0; a < TM; ++a) fa[a] = A::frag(s.a, (wm * TM + a) * 32, j);
+#pragma unroll
+      for (int b = 0; b < TN; ++b) fb[b] = B::frag(s.b, (wn * TN + b) * 32, j);
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) acc[a][b] = OP::mma(fa[a], fb[b], acc[a][b]);
+    }
+  }
+  static __device__ __forceinline__ void arrive() {   // the loads into the next stage are there, and everyone is done with this one
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+  // stages first .. last - 1
+  __device__ __forceinline__ void run(const A& oa, const B& ob, Stage& s0, Stage& s1, int first, int last) {
+    const int wave = wave_index(), wm = wave / WN, wn = wave % WN;
+    clear();
+    if (first >= last) return;
+    oa.load(s0.a, first, wave);
+    ob.load(s0.b, first, wave);
+    arrive();
+    for (int k = first; k < last; k += 2) {
+      if (k + 1 < last) {
+        oa.load(s1.a, k + 1, wave);
+        ob.load(s1.b, k + 1, wave);
+      }
+      step(s0, wm, wn);
+      arrive();
+      if (k + 1 >= last) break;
+      if (k + 2 < last) {
+        oa.load(s0.a, k + 2, wave);
+        ob.load(s0.b, k + 2, wave);
+      }
+      step(s1, wm, wn);
+      arrive();
+    }
+  }
+};
+
+// The tile of workgroup `id` among mt x nt: every XCD (workgroups go to the eight in turn) takes a contiguous run of tiles, in
+// bands of 8 along the first axis, so that the tiles that run together share rows in its L2. False past the last.
+__device__ __forceinline__ bool tile_of(int64_t id, int mt, int nt, int& m, int& n) {
+  const int64_t total = (int64_t)mt * nt, per = (total + 7) / 8;
+  const int64_t t = (id & 7) * per + (id >> 3);
+  if ((id >> 3) >= per || t >= total) return false;
+  const int band = (int)(t / (8 * (int64_t)nt));
+  const int high = min(8, mt - band * 8);
+  const int in = (int)(t - (int64_t)band * 8 * nt);
+  m = band * 8 + in % high;
+  n = in / high;
+  return true;
+}
+inline int64_t tiles_grid(int64_t mt, int64_t nt) { return 8 * cdiv(mt * nt, 8); }
+
+// ---------------------------------------------------------------------------------------------
+// The kept tokens, in order. One workgroup: 8192 tokens a round.
+
+__global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets, int64_t tokens, int64_t ignore, int* rows, float* each) {
+  __shared__ int count[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int base = 0;
+  for (int64_t i0 = 0; i0 < tokens; i0 += 8192) {
+    bool kept[8];
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t i = i0 + wave * 512 + u * 64 + lane;
+      kept[u] = i < tokens && targets[i] != ignore;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) n += (int)__popcll(__ballot(kept[u]));
+    __syncthreads();
+    if (lane == 0) count[wave] = n;
+    __syncthreads();
+    int at = base;
+    for (int w = 0; w < 16; ++w) {
+      at += w < wave ? count[w] : 0;
+      base += count[w];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t i = i0 + wave * 512 + u * 64 + lane;
+      const uint64_t mask = __ballot(kept[u]);
+      const int mine = at + (int)__popcll(mask & (((uint64_t)1 << lane) - 1));
+      if (kept[u]) rows[ROWS_HEAD + mine] = (int)i;
+      if (i < tokens) {
+        rows[ROWS_HEAD + tokens + i] = kept[u] ? mine : -1;
+        if (each && !kept[u]) each[i] = 0.f;
+      }
+      at += (int)__popcll(mask);
+    }
+  }
+  if (threadIdx.x == 0) rows[0] = base;
+}
+
+// Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i], times factor[i] where given.
+template <class OP>
+__global__ __launch_bounds__(NTHREADS) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
+                                                               const int* count, int64_t most, const float* factor,
+                                                               typename OP::elem* to, int padded) {
+  const int64_t rows = count ? *count : most;
+  const int per = padded / 4;
+  const bool quads = ((uintptr_t)from % (dtype == SA_DTYPE_F32 ? 16 : 8)) == 0 && ld % 4 == 0;
+  const int64_t n = rows * per;
+  for (int64_t k = (int64_t)blockIdx.x * NTHREADS + threadIdx.x; k < n; k += (int64_t)gridDim.x * NTHREADS) {
+    const int64_t i = k / per;
+    const int e = (int)(k - i * per) * 4;
+    const void* row = row_of(from, numbers_of ? numbers_of[i] : i, ld, dtype);
+    float x[4];
+    if (quads && e + 4 <= width) numbers<true>(fetch<true>(row, dtype, e, 1, width), dtype, x);
+    else numbers<false>(fetch<false>(row, dtype, e, 1, width), dtype, x);
+    if (factor) {
+      const float f = factor[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= f;
+    }
+    put<true>(to + i * padded, OP::CODE, e, 1, padded, x);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Logits of a tile: rows of the vocabulary (M) x tokens (N).
+
+struct LogitsCall {
+  const void *w, *x;
+  int64_t w_ld, x_ld;
+  const int64_t* targets;
+  const int* rows;          // null: tokens as they come, `tokens` of them
+  int64_t tokens, vocab;    // vocab: of the whole table
+  int64_t v0, v1;           // this launch's rows of it
+  int stages;               // of the contraction
+  int mt, nt;
+  float *top, *sum, *at;    // (mt, tokens) statistics, the targets' logits
+  const float* lse;         // backward: base 2
+  const float* factor;      // backward: of each kept token's row of G; null: 1
+  void* g;                  // (tokens, g_ld)
+  int64_t g_ld;
+};
+
+template <class OP, class L, bool GRAD>
+__global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits_kernel(LogitsCall c) {
+  typedef typename OP::elem elem;
+  constexpr int ES = sizeof(elem);
+  __shared__ typename L::Stage s0, s1;
+  const int64_t tokens = c.rows ? c.rows[0] : c.tokens;
+  int m, n;
+  if (!tile_of(blockIdx.x, c.mt, (int)((tokens + L::BN - 1) / L::BN), m, n)) return;
+  const int64_t v0 = c.v0 + (int64_t)m * L::BM, n0 = (int64_t)n * L::BN;
+  typename L::A oa;
+  typename L::B ob;
+  oa.open((const elem*)c.w + v0 * c.w_ld, ((c.v1 - v0 - 1) * c.w_ld + c.stages * L::BK) * ES, c.w_ld);
+  ob.open((const elem*)c.x + n0 * c.x_ld, ((tokens - n0 - 1) * c.x_ld + c.stages * L::BK) * ES, c.x_ld);
+  L l;
+  l.run(oa, ob, s0, s1, 0, c.stages);
+  const int lane = threadIdx.x & 63, wave = wave_index(), h = lane >> 5, wm = wave / L::WN, wn = wave % L::WN;
+  const int64_t vw = v0 + wm * L::TM * 32;   // the wavefront's first row of the vocabulary
+  const bool edge = vw + L::TM * 32 > c.v1;
+  if constexpr (!GRAD) {
+    float* top = reinterpret_cast<float*>(s0.a);   // [WM][BN], then the sums (everyone is done with the stages)
+    float* sum = top + L::WM * L::BN;
+#pragma unroll
+    for (int b = 0; b < L::TN; ++b) {
+      const int col = (wn * L::TN + b) * 32 + (lane & 31);
+      const int64_t i = n0 + col;
+      const int64_t t = i < tokens ? c.targets[c.rows ? c.rows[ROWS_HEAD + i] : i] : -1;
+      const int64_t tl = t - vw;
+      const bool hit = i < tokens && t < c.v1 && tl >= 0 && tl < L::TM * 32 && ((tl >> 2) & 1) == h;
+      if (__ballot(hit)) {
+#pragma unroll
+        for (int a = 0; a < L::TM; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (hit && tl == a * 32 + acc_row(r, h)) c.at[i] = l.acc[a][b][r];
+      }
+      if (edge) {
+#pragma unroll
+        for (int a = 0; a < L::TM; ++a)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (vw + a * 32 + acc_row(r, h) >= c.v1) l.acc[a][b][r] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int a = 0; a < L::TM; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, l.acc[a][b][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float ref = mx == -INFINITY ? 0.f : mx * LOG2E;   // (nothing but -inf: a sum of zeros, not of NaN)
+      float s = 0.f;
+#pragma unroll
+      for (int a = 0; a < L::TM; ++a)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(l.acc[a][b][r], LOG2E, -ref));
+      s += __shfl_xor(s, 32);
+      if (h == 0) top[wm * L::BN + col] = mx, sum[wm * L::BN + col] = s;
+    }
+    __syncthreads();
+    for (int col = threadIdx.x; col < L::BN; col += L::THREADS) {
+      const int64_t i = n0 + col;
+      if (i >= tokens) continue;
+      float mx = top[col], s = sum[col];
+#pragma unroll
+      for (int w = 1; w < L::WM; ++w) mx = fmaxf(mx, top[w * L::BN + col]);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      s *= __builtin_amdgcn_exp2f((top[col] - ref) * LOG2E);
+#pragma unroll
+      for (int w = 1; w < L::WM; ++w) s += sum[w * L::BN + col] * __builtin_amdgcn_exp2f((top[w * L::BN + col] - ref) * LOG2E);
+      c.top[m * c.tokens + i] = mx;
+      c.sum[m * c.tokens + i] = s;
+    }
+  } else {
+    // G of 32 tokens x the wavefront's rows goes through a part of LDS of its own, so that a token's row is stored in
+    // 16-byte pieces side by side. Chunk c of token row r sits at c ^ (r mod 8).
+    constexpr int RB = L::TM * 32 * ES;   // bytes of a token's row
+    static_assert(L::WAVES * 32 * RB <= (int)sizeof(s0), "the wavefronts' rows in a stage");
+    uint8_t* mine = reinterpret_cast<uint8_t*>(&s0) + wave * 32 * RB;
+#pragma unroll
+    for (int b = 0; b < L::TN; ++b) {
+      const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
+      const float lse = i < tokens ? c.lse[i] : INFINITY;
+      const float lift = (c.factor && i < tokens ? c.factor[i] : 1.f) * OP::LIFT;
+      const int64_t tl = (i < tokens ? c.targets[c.rows[ROWS_HEAD + i]] : -1) - vw;
+#pragma unroll
+      for (int a = 0; a < L::TM; ++a)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float p[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = a * 32 + 8 * q + 4 * h + r;
+            float x = __builtin_amdgcn_exp2f(fmaf(l.acc[a][b][4 * q + r], LOG2E, -lse));
+            if (tl == row) x -= 1.f;
+            if (edge && vw + row >= c.v1) x = 0.f;
+            p[r] = x * lift;
+          }
+          const int byte = (a * 32 + 8 * q + 4 * h) * ES;
+          put<true>(mine + (lane & 31) * RB + (((byte >> 4) ^ (lane & 7)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
+        }
+      __asm__ volatile("" ::: "memory");   // (a wavefront's own LDS accesses run in order)
+      constexpr int CPR = RB / 16;
+#pragma unroll
+      for (int k = 0; k < 32 * CPR / 64; ++k) {
+        const int slot = k * 64 + lane, r = slot / CPR, ch = slot % CPR;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ((ch ^ (r & 7)) << 4));
+        const int64_t j = n0 + (wn * L::TN + b) * 32 + r;
+        if (j < tokens) *reinterpret_cast<u32x4*>((elem*)c.g + j * c.g_ld + (vw - c.v0) + ch * (16 / ES)) = v;
+      }
+      __asm__ volatile("" ::: "memory");
+    }
+  }
+}
+
+// A token's statistics over the mt tiles joined: 8 lanes a token. lse (base 2), the loss, and the workgroup's sum of losses.
+__global__ __launch_bounds__(NTHREADS) void xent_join_kernel(LogitsCall c, float* lse, float* each, float* sums, int64_t ignore) {
+  __shared__ float part[NTHREADS / 32];
+  __shared__ float tm[8][33], ts[8][33];
+  const int64_t tokens = c.rows ? c.rows[0] : c.tokens;
+  const int x = threadIdx.x & 31, k = threadIdx.x >> 5;
+  float total = 0.f;
+  for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < tokens; i0 += (int64_t)gridDim.x * 32) {
+    const int64_t i = i0 + x;
+    float mx = -INFINITY, s = 0.f;
+    if (i < tokens) {
+#pragma unroll 4
+      for (int m = k; m < c.mt; m += 8) {
+        const float a = c.top[m * c.tokens + i], b = c.sum[m * c.tokens + i];
+        const float up = fmaxf(mx, a), ref = up == -INFINITY ? 0.f : up;
+        s = s * __builtin_amdgcn_exp2f((mx - ref) * LOG2E) + b * __builtin_amdgcn_exp2f((a - ref) * LOG2E);
+        mx = up;
+      }
+    }
+    __syncthreads();
+    tm[k][x] = mx, ts[k][x] = s;
+    __syncthreads();
+    if (k == 0 && i < tokens) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) mx = fmaxf(mx, tm[w][x]);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += ts[w][x] * __builtin_amdgcn_exp2f((tm[w][x] - ref) * LOG2E);
+      const int64_t token = c.rows ? c.rows[ROWS_HEAD + i] : i;
+      const int64_t t = c.targets[token];
+      // (a target outside the vocabulary has no logit: its loss and gradients become NaN)
+      const bool real = t >= 0 && t < c.vocab;
+      const float nan = __uint_as_float(0x7fc00000u);
+      const float ls = logf(s);
+      float loss = real ? (mx - c.at[i]) + ls : nan;
+      if (!c.rows && t == ignore) loss = 0.f;
+      if (lse) lse[i] = real ? fmaf(mx, LOG2E, log2f(s)) : nan;
+      if (each) each[token] = loss;
+      total += loss;
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) total += __shfl_xor(total, d);
+  if (x == 0) part[k] = total;   // (lanes of k > 0 hold zeros)
+  __syncthreads();
+  if (threadIdx.x == 0) sums[blockIdx.x] = part[0];
+}
+
+// The workgroups' sums added in a fixed order, over the tokens kept where a mean is asked for (none: 0 / 0, a NaN).
+__global__ __launch_bounds__(1024) void xent_sum_kernel(const float* sums, int n, const int* rows, float* loss) {
+  __shared__ float acc[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n; i += 1024) s += sums[i];
+#pragma unroll
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+  if (lane == 0) acc[wave] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0.f;
+  for (int w = 0; w < 16; ++w) s += acc[w];
+  *loss = rows ? s / (float)rows[0] : s;
+}
+
+// ---------------------------------------------------------------------------------------------
+// The backward pass's factors: scale[0] multiplies the sums of both products; factor[i] (reduction none) the kept token's row of G
+// before it is rounded, g_i / scale[0], with scale[0] the power of two at or below the largest |g|. So a row is rounded once, as
+// with one g for all; in fp16 the entries of rows whose g is less than 2^-10 of the largest lose their last bits.
+__global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, const int* rows, int reduction, float* scale, float* factor) {
+  __shared__ float acc[16];
+  const int tokens = rows[0];
+  if (!factor) {   // (no token kept: gradients of zeros, not 0 / 0)
+    if (threadIdx.x == 0) scale[0] = tokens == 0 ? 0.f : reduction == SA_REDUCE_MEAN ? dloss[0] / (float)tokens : dloss[0];
+    return;
+  }
+  float most = 0.f;
+  for (int i = threadIdx.x; i < tokens; i += 1024) most = fmaxf(most, fabsf(dloss[rows[ROWS_HEAD + i]]));
+#pragma unroll
+  for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  if ((threadIdx.x & 63) == 0) acc[threadIdx.x >> 6] = most;
+  __syncthreads();
+  for (int w = 0; w < 16; ++w) most = fmaxf(most, acc[w]);
+  const uint32_t e = min(max((__float_as_uint(most) >> 23) & 0xff, 1u), 253u);
+  const float unit = __uint_as_float(e << 23);
+  if (threadIdx.x == 0) scale[0] = unit;
+  for (int i = threadIdx.x; i < tokens; i += 1024) factor[i] = dloss[rows[ROWS_HEAD + i]] / unit;
+}
+
+// ---------------------------------------------------------------------------------------------
+// A product of the backward pass. A plain, (M, K): dX = G W; A turned, (K, M): dW = G^T X. B turned, (K, N).
+
+struct ProductCall {
+  const void *a, *b;
+  int64_t a_ld, b_ld;
+  const int* rows;          // kept tokens: M (dX) or K (dW)
+  int64_t m, n, k;          // M of dW, N, K of dX
+  int64_t b_cols;           // columns of b that may be read (whole 16-byte pieces)
+  int mt, nt, splits;
+  float* sums;              // [split][M rows][n_ld] where they go to the workspace
+  int64_t n_ld, m_rows;
+  int add;                  // onto what is there
+  void* out;                // dW's rows, where nothing is split
+  int64_t out_ld;
+  int out_t;
+  const float* scale;
+  float lift;
+};
+
+template <class OP, class L, bool DW>
+__global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_product_kernel(ProductCall c) {
+  typedef typename OP::elem elem;
+  constexpr int ES = sizeof(elem);
+  __shared__ typename L::Stage s0, s1;
+  const int64_t tokens = c.rows[0];
+  const int64_t M = DW ? c.m : tokens, K = DW ? tokens : c.k;
+  int m, n;
+  if (!tile_of(blockIdx.x, DW ? c.mt : (int)((M + L::BM - 1) / L::BM), c.nt, m, n)) return;
+  const int64_t m0 = (int64_t)m * L::BM, n0 = (int64_t)n * L::BN;
+  typename L::A oa;
+  typename L::B ob;
+  const int stages = (int)((K + L::BK - 1) / L::BK);
+  const int per = (stages + c.splits - 1) / c.splits;
+  const int first = min((int)blockIdx.y * per, stages), last = min(first + per, stages);
+  const int64_t k0 = (int64_t)first * L::BK;   // (offsets within a split stay below 2^31 bytes)
+  if constexpr (DW) oa.open((const elem*)c.a + k0 * c.a_ld + m0, ((K - k0) * c.a_ld - m0) * ES, c.a_ld);
+  else oa.open((const elem*)c.a + m0 * c.a_ld + k0, ((M - m0) * c.a_ld - k0) * ES, c.a_ld);
+  ob.open((const elem*)c.b + k0 * c.b_ld + n0, ((K - k0 - 1) * c.b_ld + c.b_cols - n0) * ES, c.b_ld);
+  L l;
+  l.run(oa, ob, s0, s1, 0, last - first);
+  const int lane = threadIdx.x & 63, wave = wave_index(), h = lane >> 5, wm = wave / L::WN, wn = wave % L::WN;
+  const float scale = c.out ? *c.scale * c.lift : 1.f;
+#pragma unroll
+  for (int a = 0; a < L::TM; ++a)
+#pragma unroll
+    for (int b = 0; b < L::TN; ++b) {
+      const int64_t col = n0 + (wn * L::TN + b) * 32 + (lane & 31);
+      if (col >= c.n) continue;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t row = m0 + (wm * L::TM + a) * 32 + acc_row(r, h);
+        if (row >= M) continue;
+        float x = l.acc[a][b][r];
+        if (c.out) {
+          void* at = row_of(c.out, row, c.out_ld, c.out_t);
+          if (c.out_t == SA_DTYPE_F32) ((float*)at)[col] = x * scale;
+          else ((uint16_t*)at)[col] = to16(x * scale, c.out_t);
+        } else {
+          float* at = c.sums + ((int64_t)blockIdx.y * c.m_rows + row) * c.n_ld + col;
+          *at = c.add ? *at + x : x;
+        }
+      }
+    }
+}
+
+// dX: a token's parts added, times its factor; zero rows for the tokens that are ignored. dW: the parts of a piece's rows.
+__global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums, int splits, int64_t split_stride, int64_t n_ld,
+                                                               const int* place, const float* scale, float lift,
+                                                               void* out, int64_t rows, int width, int dtype) {
+  const int64_t per = (width + 3) / 4;
+  const int64_t n = rows * per;
+  const bool quads = width % 4 == 0;
+  for (int64_t k = (int64_t)blockIdx.x * NTHREADS + threadIdx.x; k < n; k += (int64_t)gridDim.x * NTHREADS) {
+    const int64_t row = k / per;
+    const int e = (int)(k - row * per) * 4;
+    const int64_t at = place ? place[row] : row;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (at >= 0) {
+      for (int s = 0; s < splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + at * n_ld + e);
+        x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
+      }
+      const float f = *scale * lift;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= f;
+    }
+    if (quads) put<true>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
+    else put<false>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+
+template <class OP>
+struct XentConfigs {   // 16-bit products
+  typedef Mainloop<OP, 2, 4, 4, 2, false, false> Large;   // 256 x 256
+  typedef Mainloop<OP, 2, 2, 2, 2, false, false> Middle;  // 128 x 128
+  typedef Mainloop<OP, 4, 1, 1, 1, false, false> Small;   // 128 x 32
+  typedef Mainloop<OP, 2, 4, 4, 2, false, true> LargeX;
+  typedef Mainloop<OP, 2, 2, 2, 2, false, true> MiddleX;
+  typedef Mainloop<OP, 2, 4, 4, 2, true, true> LargeW;
+  typedef Mainloop<OP, 2, 2, 2, 2, true, true> MiddleW;
+};
+template <>
+struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per stage; one size)
+  typedef Mainloop<XF32, 2, 2, 2, 2, false, false> Large;
+  typedef Mainloop<XF32, 2, 2, 2, 2, false, false> Middle;
+  typedef Mainloop<XF32, 4, 1, 1, 1, false, false> Small;
+  typedef Mainloop<XF32, 2, 2, 2, 2, false, true> LargeX;
+  typedef Mainloop<XF32, 2, 2, 2, 2, false, true> MiddleX;
+  typedef Mainloop<XF32, 2, 2, 2, 2, true, true> LargeW;
+  typedef Mainloop<XF32, 2, 2, 2, 2, true, true> MiddleW;
+};
+
+constexpr int64_t SMALL_TOKENS = 32;      // one tile's tokens of the smallest kernel
+constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are
+constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of G
+constexpr int64_t MAX_LD_BYTES = 1 << 22;             // 256 rows within a buffer resource's 2 GiB
+
+// What a call does, from its sizes alone.
+template <class OP>
+struct XentShape {
+  static constexpr int ES = sizeof(typename OP::elem), BK = 128 / ES;
+  bool train, small, large, gather, copy_w;
+  int64_t padded, bm, mt, join_blocks;
+  // backward
+  int64_t piece, pieces;
+  bool large_x, large_w;
+  int splits_x, splits_w;
+  // workspace
+  int64_t x, w, top, sum, at, sums, factors, g, dx, dw, total;
+
+  XentShape(const XentCall& c, bool backward) {
+    train = c.lse != nullptr;
+    padded = align_up(c.width, BK);
+    small = c.tokens <= SMALL_TOKENS && !train;
+    large = !small && ES == 2 && cdiv(c.vocab, 256) * cdiv(c.tokens, 256) >= 2 * (int64_t)c.cus;
+    bm = large ? 256 : 128;
+    mt = cdiv(c.vocab, bm);
+    const bool x_ok = c.x_t == OP::CODE && padded == c.width && (uintptr_t)c.x % 16 == 0 && c.x_ld * ES % 16 == 0 &&
+                      c.x_ld >= c.width && c.x_ld * ES < MAX_LD_BYTES;
+    gather = train || c.reduction != SA_REDUCE_NONE || c.tokens > IN_PLACE_TOKENS || !x_ok;
+    copy_w = !(c.w_t == OP::CODE && padded == c.width && (uintptr_t)c.w % 16 == 0 && c.w_ld * ES % 16 == 0 &&
+               c.w_ld >= c.width && c.w_ld * ES < MAX_LD_BYTES);
+    join_blocks = std::min<int64_t>(cdiv(c.tokens, 32), 4096);
+    int64_t p = 0;
+    const auto take = [&p](int64_t bytes) {
+      const int64_t at = p;
+      p += align_up(bytes, 1024);
+      return at;
+    };
+    x = take(gather ? c.tokens * padded * ES : 0);
+    w = take(copy_w ? c.vocab * padded * ES : 0);
+    if (!backward) {
+      top = take(mt * c.tokens * 4);
+      sum = take(mt * c.tokens * 4);
+      at = take(c.tokens * 4);
+      sums = take(join_blocks * 4);
+    } else {
+      // Pieces of the vocabulary whose G fits PIECE_BYTES, in whole tiles, of about one size
+      const int64_t most = std::max<int64_t>(PIECE_BYTES / (c.tokens * ES) / 256 * 256, 256);
+      pieces = cdiv(c.vocab, most);
+      piece = align_up(cdiv(c.vocab, pieces), 256);
+      pieces = cdiv(c.vocab, piece);
+      const int64_t k_x = cdiv(piece, BK), k_w = cdiv(c.tokens, BK);
+      const auto split = [&](int64_t tiles, int64_t stages) {   // fill the chip where tiles are few: parts of 4 stages or more
+        return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(2 * c.cus, tiles), stages / 4, 16}));
+      };
+      large_x = ES == 2 && cdiv(c.tokens, 256) * cdiv(c.width, 256) >= c.cus / 2;
+      large_w = ES == 2 && (piece / 256) * cdiv(c.width, 256) >= c.cus / 4;
+      const int64_t tx = large_x ? 256 : 128, tw = large_w ? 256 : 128;
+      const int64_t tiles_x = cdiv(c.tokens, tx) * cdiv(c.width, tx), tiles_w = cdiv(piece, tw) * cdiv(c.width, tw);
+      splits_x = tiles_x >= c.cus / 2 ? 1 : split(tiles_x, k_x);
+      splits_w = tiles_w >= c.cus / 2 ? 1 : split(tiles_w, k_w);
+      // (a part's rows lie within 2^30 bytes)
+      const int64_t w_row = (copy_w ? padded : c.w_ld) * ES, x_row = std::max(padded, piece) * ES;
+      splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
+      splits_w = std::max(splits_w, (int)cdiv(c.tokens * x_row, (int64_t)1 << 30));
+      factors = take((c.tokens + 16) * 4);
+      g = take(c.tokens * piece * ES);
+      dx = take(c.dx ? splits_x * c.tokens * padded * 4 : 0);
+      dw = take(c.dw && splits_w > 1 ? splits_w * piece * padded * 4 : 0);
+    }
+    total = p;
+  }
+};
+
+template <class OP, class L, bool GRAD>
+void launch_logits(LogitsCall lc, int64_t tokens, hipStream_t st) {
+  lc.mt = (int)cdiv(lc.v1 - lc.v0, L::BM);
+  lc.nt = (int)cdiv(tokens, L::BN);
+  hipLaunchKernelGGL((xent_logits_kernel<OP, L, GRAD>), dim3((unsigned)tiles_grid(lc.mt, lc.nt)), dim3(L::THREADS), 0, st, lc);
+}
+template <class OP, class L, bool DW>
+void launch_product(ProductCall pc, int64_t rows, hipStream_t st) {
+  pc.mt = (int)cdiv(rows, L::BM);
+  pc.nt = (int)cdiv(pc.n, L::BN);
+  hipLaunchKernelGGL((xent_product_kernel<OP, L, DW>), dim3((unsigned)tiles_grid(pc.mt, pc.nt), (unsigned)pc.splits), dim3(L::THREADS),
+                     0, st, pc);
+}
+template <class OP>
+void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows,
+                   const float* factor, void* to, int64_t padded, hipStream_t st) {
+  const int64_t blocks = std::min<int64_t>(cdiv(rows * (padded / 4), NTHREADS), 16384);
+  hipLaunchKernelGGL((xent_gather_kernel<OP>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, from, ld, dtype, (int)width, numbers_of,
+                     count, rows, factor, (typename OP::elem*)to, (int)padded);
+}
+inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const float* scale,
+                          float lift, void* out, int64_t rows, int64_t width, int dtype, hipStream_t st) {
+  const int64_t blocks = std::min<int64_t>(cdiv(rows * cdiv(width, 4), NTHREADS), 16384);
+  hipLaunchKernelGGL(xent_finish_kernel, dim3((unsigned)blocks), dim3(NTHREADS), 0, st, sums, splits, split_stride, n_ld, place, scale,
+                     lift, out, rows, (int)width, dtype);
+}
+
+template <class OP>
+int xent_forward(const XentCall& c) {
+  typedef XentConfigs<OP> F;
+  const XentShape<OP> s(c, false);
+  char* ws = (char*)c.ws;
+  float* each = c.reduction == SA_REDUCE_NONE ? c.loss : nullptr;
+  LogitsCall lc{};
+  lc.targets = c.targets;
+  lc.tokens = c.tokens;
+  lc.vocab = c.vocab;
+  if (s.gather) {
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(1), dim3(1024), 0, c.st, c.targets, c.tokens, c.ignore, c.rows, each);
+    lc.rows = c.rows;
+    launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, ws + s.x, s.padded, c.st);
+    lc.x = ws + s.x, lc.x_ld = s.padded;
+  } else {
+    lc.x = c.x, lc.x_ld = c.x_ld;
+  }
+  if (s.copy_w) {
+    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, ws + s.w, s.padded, c.st);
+    lc.w = ws + s.w, lc.w_ld = s.padded;
+  } else {
+    lc.w = c.w, lc.w_ld = c.w_ld;
+  }
+  lc.v0 = 0, lc.v1 = c.vocab;
+  lc.stages = (int)(s.padded / s.BK);
+  lc.top = (float*)(ws + s.top), lc.sum = (float*)(ws + s.sum), lc.at = (float*)(ws + s.at);
+  if (s.small) launch_logits<OP, typename F::Small, false>(lc, c.tokens, c.st);
+  else if (s.large) launch_logits<OP, typename F::Large, false>(lc, c.tokens, c.st);
+  else launch_logits<OP, typename F::Middle, false>(lc, c.tokens, c.st);
+  lc.mt = (int)s.mt;
+  float* sums = each ? nullptr : (float*)(ws + s.sums);
+  hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)s.join_blocks), dim3(NTHREADS), 0, c.st, lc, c.lse, each, sums, c.ignore);
+  if (sums)
+    hipLaunchKernelGGL(xent_sum_kernel, dim3(1), dim3(1024), 0, c.st, sums, (int)s.join_blocks,
+                       c.reduction == SA_REDUCE_MEAN ? c.rows : nullptr, c.loss);
+  return launch_status();
+}
+
+template <class OP>
+int xent_backward(const XentCall& c) {
+  typedef XentConfigs<OP> F;
+  constexpr int ES = sizeof(typename OP::elem);
+  const XentShape<OP> s(c, true);
+  char* ws = (char*)c.ws;
+  float* scale = (float*)(ws + s.factors);
+  float* factor = c.reduction == SA_REDUCE_NONE ? scale + 16 : nullptr;
+  hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, scale, factor);
+  launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, ws + s.x, s.padded, c.st);
+  const void* w = c.w;
+  int64_t w_ld = c.w_ld;
+  if (s.copy_w) {
+    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, ws + s.w, s.padded, c.st);
+    w = ws + s.w, w_ld = s.padded;
+  }
+  for (int64_t v0 = 0; v0 < c.vocab; v0 += s.piece) {
+    const int64_t v1 = std::min(v0 + s.piece, c.vocab);
+    LogitsCall lc{};
+    lc.w = w, lc.w_ld = w_ld, lc.x = ws + s.x, lc.x_ld = s.padded, lc.targets = c.targets, lc.rows = c.rows, lc.tokens = c.tokens;
+    lc.vocab = c.vocab, lc.v0 = v0, lc.v1 = v1, lc.stages = (int)(s.padded / s.BK), lc.lse = c.lse, lc.factor = factor, lc.g = ws + s.g, lc.g_ld = s.piece;
+    if (ES == 2 && cdiv(v1 - v0, 256) * cdiv(c.tokens, 256) >= c.cus) launch_logits<OP, typename F::Large, true>(lc, c.tokens, c.st);
+    else launch_logits<OP, typename F::Middle, true>(lc, c.tokens, c.st);
+    if (c.dx) {
+      ProductCall pc{};
+      pc.a = lc.g, pc.a_ld = s.piece, pc.b = (const char*)w + v0 * w_ld * ES, pc.b_ld = w_ld, pc.rows = c.rows, pc.n = pc.b_cols = s.padded, pc.k = v1 - v0;
+      pc.splits = s.splits_x, pc.sums = (float*)(ws + s.dx), pc.n_ld = s.padded, pc.m_rows = c.tokens, pc.add = v0 > 0;
+      if (s.large_x) launch_product<OP, typename F::LargeX, false>(pc, c.tokens, c.st);
+      else launch_product<OP, typename F::MiddleX, false>(pc, c.tokens, c.st);
+    }
+    if (c.dw) {
+      ProductCall pc{};
+      pc.a = lc.g, pc.a_ld = s.piece, pc.b = ws + s.x, pc.b_ld = s.padded, pc.rows = c.rows, pc.m = v1 - v0, pc.n = c.width, pc.b_cols = s.padded;
+      pc.splits = s.splits_w, pc.lift = 1.f / OP::LIFT, pc.scale = scale;
+      char* out = (char*)c.dw + v0 * c.width * lm_elem_size(c.w_t);
+      if (s.splits_w == 1) pc.out = out, pc.out_ld = c.width, pc.out_t = c.w_t;
+      else pc.sums = (float*)(ws + s.dw), pc.n_ld = s.padded, pc.m_rows = s.piece;
+      if (s.large_w) launch_product<OP, typename F::LargeW, true>(pc, v1 - v0, c.st);
+      else launch_product<OP, typename F::MiddleW, true>(pc, v1 - v0, c.st);
+      if (s.splits_w > 1)
+        launch_finish(pc.sums, s.splits_w, s.piece * s.padded, s.padded, nullptr, scale, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t,
+                      c.st);
+    }
+  }
+  if (c.dx)
+    launch_finish((float*)(ws + s.dx), s.splits_x, c.tokens * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, scale,
+                  1.f / OP::LIFT, c.dx, c.tokens, c.width, c.x_t, c.st);
+  return launch_status();
+}
+
+}  // namespace

@@ -1,7 +1,8 @@
 """Selective Attention (Leviathan, Kalman, Matias; ICLR 2025) on MI355X HIP kernels.
 
 Same exports as the reference package (reference src/selective_attention/__init__.py:3-17), plus
-the chunked-prefill, cached-decode and packed-projection entry points, and those of a paged cache.
+the chunked-prefill, cached-decode and packed-projection entry points, those of a paged cache, and a decoder's operators around
+its attention layers.
 """
 
 from .kernels import (
@@ -14,6 +15,16 @@ from .kernels import (
     selective_attention_qkv,
     selective_attention_reference,
     selective_logits,
+)
+from .lm import (
+    add_layer_norm,
+    add_layer_norm_reference,
+    embedding,
+    embedding_reference,
+    layer_norm,
+    layer_norm_reference,
+    linear_cross_entropy,
+    linear_cross_entropy_reference,
 )
 from .paged import (
     PagePlan,
@@ -29,6 +40,14 @@ __all__ = [
     "HAS_HIP",
     "HAS_TRITON",
     "PagePlan",
+    "add_layer_norm",
+    "add_layer_norm_reference",
+    "embedding",
+    "embedding_reference",
+    "layer_norm",
+    "layer_norm_reference",
+    "linear_cross_entropy",
+    "linear_cross_entropy_reference",
     "page_plan",
     "page_plan_reference",
     "paged_append",

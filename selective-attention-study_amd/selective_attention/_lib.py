@@ -18,8 +18,10 @@ LIB_PATH = os.environ.get("SA_HIP_LIBRARY") or os.path.join(os.path.dirname(os.p
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
-DTYPE_F16 = 2   # the paged cache's entry points
+DTYPE_F16 = 2   # the entry points of the paged cache, the norms, the embedding and the vocabulary loss
 WIDE_WEIGHTS = 16   # sa_paged_attention: or'ed to the dtype
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}   # sa_linear_xent
 
 # Kernel ids of sa_timing_read.
 KERNEL_FORWARD = 0
@@ -66,6 +68,16 @@ SIGNATURES = {
     "sa_paged_attention_workspace_bytes": (_I64, [_I64] * 7 + [_I]),
     "sa_paged_attention": (_I, [_P, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64,
                                 _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I, _P]),
+    "sa_layer_norm": (_I, [_P, _I64, _P, _I64] + [_P] * 6 + [_I64, _I64, _F] + [_I] * 4 + [_P]),
+    "sa_layer_norm_backward_workspace_bytes": (_I64, [_I64, _I64]),
+    "sa_layer_norm_backward": (_I, [_P, _I64, _P, _I64, _P, _I64] + [_P] * 8 + [_I64, _I64, _I64] + [_I] * 4 + [_P]),
+    "sa_embedding": (_I, [_P, _I, _P, _I64, _P, _I64, _I64, _I64, _F, _I, _P]),
+    "sa_embedding_backward_workspace_bytes": (_I64, [_I64] * 3),
+    "sa_embedding_backward": (_I, [_P, _I, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _F, _I, _P]),
+    "sa_linear_xent_workspace_bytes": (_I64, [_P, _I64, _P] + [_I64] * 4 + [_I] * 5),
+    "sa_linear_xent": (_I, [_P, _I64, _P, _I64] + [_P] * 5 + [_I64] * 5 + [_I] * 4 + [_P]),
+    "sa_linear_xent_backward_workspace_bytes": (_I64, [_P] + [_I64] * 4 + [_I] * 4),
+    "sa_linear_xent_backward": (_I, [_P, _I64, _P, _I64] + [_P] * 7 + [_I64] * 4 + [_I] * 4 + [_P]),
     "sa_decode_noalloc": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _I, _P]),
 }
 

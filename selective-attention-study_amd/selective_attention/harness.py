@@ -12,7 +12,7 @@ Synthetic inputs only: token ids uniform over the GPT-2 vocabulary with <BOS> (5
 reference's window rule input = [bos] + window[:-1], targets = window (data.py:136-139);
 random-init weights. Times are HIP events around whole steps after warm-up.
 
-    python -m selective_attention.harness c3 [--geometry d768|d1024] [--steps K] [--warmup W]
+    python -m selective_attention.harness c3 [--geometry d768|d1024] [--path forward|loss] [--steps K] [--warmup W]
     python -m selective_attention.harness c4 [--tokens 131072] [--chunk 16384]
     python -m selective_attention.harness c5
     python -m selective_attention.harness decode [--tokens 131072]   (one decode step's HBM rate)
@@ -74,8 +74,9 @@ def model_flop_per_token(cfg: ModelConfig, seq: int) -> float:
 
 
 def train_step_rate(geometry: str = "d768", steps: int = 10, warmup: int = 3, seq: int = 16384, batch: int = 1,
-                    layers: int = 24) -> dict:
-    """C3: tokens per second of full training steps (forward, backward, grad clip, fused AdamW)."""
+                    layers: int = 24, path: str = "forward") -> dict:
+    """C3: tokens per second of full training steps (forward, backward, grad clip, fused AdamW). path: "forward" takes the loss
+    from SelectiveLM.forward, which makes the logits, "loss" from SelectiveLM.loss (lm.py's operators)."""
     dev = torch.device("cuda")
     cfg = ModelConfig(n_layers=layers, context_length=seq, **GEOMETRIES[geometry])
     torch.manual_seed(0)
@@ -86,7 +87,7 @@ def train_step_rate(geometry: str = "d768", steps: int = 10, warmup: int = 3, se
 
     def step():
         with torch.autocast("cuda", dtype=torch.bfloat16):
-            _, loss = model(idx, targets)
+            loss = model.loss(idx, targets) if path == "loss" else model(idx, targets)[1]
         loss.backward()
         torch.nn.utils.clip_grad_norm_(model.parameters(), 1.0)
         opt.step()
@@ -104,7 +105,7 @@ def train_step_rate(geometry: str = "d768", steps: int = 10, warmup: int = 3, se
     tokens = batch * seq
     flop = model_flop_per_token(cfg, seq) * tokens
     return {"config": f"C3 train step, {geometry} ({model.num_parameters()} params), {layers} layers, "
-                      f"{batch}x{seq} tokens, bf16 autocast, fused AdamW, eager",
+                      f"{batch}x{seq} tokens, bf16 autocast, fused AdamW, eager" + (", SelectiveLM.loss" if path == "loss" else ""),
             "tokens_per_s": tokens / (ms * 1e-3), "ms_per_step": ms, "model_tflops": flop / (ms * 1e-3) / 1e12,
             "attention_kernel_ms": attn_ms, "attention_share": attn_ms / ms,
             "per_layer_attention_ms": {name: t / layers for name, t in per_step.items()},
@@ -315,6 +316,7 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("which", choices=["c3", "c4", "c5", "decode", "copy"])
     ap.add_argument("--geometry", default=None, choices=sorted(GEOMETRIES))
+    ap.add_argument("--path", default="forward", choices=["forward", "loss"])
     ap.add_argument("--steps", type=int, default=None)
     ap.add_argument("--warmup", type=int, default=None)
     ap.add_argument("--layers", type=int, default=24)
@@ -326,7 +328,7 @@ def main(argv=None) -> int:
         return 2
     kw = {k: v for k, v in (("steps", a.steps), ("warmup", a.warmup)) if v is not None}
     if a.which == "c3":
-        res = train_step_rate(a.geometry or "d768", layers=a.layers, **kw)
+        res = train_step_rate(a.geometry or "d768", layers=a.layers, path=a.path, **kw)
     elif a.which == "c4":
         res = prefill_rate(a.tokens, a.chunk, a.geometry or "d1024", a.layers,
                            **({"reps": a.steps} if a.steps else {}), **({"warmup": a.warmup} if a.warmup is not None else {}))

@@ -26,7 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
-from . import mixers, paged
+from . import lm, mixers, paged
 from .slot import AttentionSlot
 
 
@@ -117,6 +117,14 @@ def attention_classes() -> dict:
 ATTENTION_TYPES = tuple(attention_classes())
 
 
+def _add_norm(norm: nn.LayerNorm, x: Tensor, branch: Tensor | None, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    """(norm(x + branch) in dtype, x + branch), by the fused operators (CPU tensors: their plain forms)."""
+    args = (norm.weight, norm.bias, norm.eps, dtype)
+    if branch is None:
+        return (lm.layer_norm if x.is_cuda else lm.layer_norm_reference)(x, *args), x
+    return (lm.add_layer_norm if x.is_cuda else lm.add_layer_norm_reference)(x, branch, *args)
+
+
 class Block(nn.Module):
     """Pre-norm residual block: x + attn(ln_1 x), then + mlp(ln_2 .). The cached forms run the same
     residual stream through the slot's prefill / chunk / decode operation."""
@@ -135,6 +143,13 @@ class Block(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         return self._through(x, self.attn(self.ln_1(x)))
 
+    def advance(self, x: Tensor, branch: Tensor | None, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+        """forward with the residual additions left to the norms that follow them (`_add_norm`): takes the stream and the branch
+        still to be added to it, returns the same."""
+        h, x = _add_norm(self.ln_1, x, branch, dtype)
+        h, x = _add_norm(self.ln_2, x, self.attn(h), dtype)
+        return x, self.mlp(h)
+
     def begin_cache(self, x: Tensor, capacity: int | None = None):
         mixed, cache = self.attn.begin_cache(self.ln_1(x), capacity)
         return self._through(x, mixed), cache
@@ -152,7 +167,8 @@ class Block(nn.Module):
 
 class SelectiveLM(nn.Module):
     """Decoder-only LM. forward(idx, targets=None) -> (logits, loss): with targets, every position's
-    logits and the mean cross-entropy (ignore_index -100); without, the last position's logits."""
+    logits and the mean cross-entropy (ignore_index -100); without, the last position's logits. loss(idx, targets): that
+    cross-entropy alone, by fused operators and without the logits."""
 
     def __init__(self, config: ModelConfig):
         super().__init__()
@@ -191,6 +207,25 @@ class SelectiveLM(nn.Module):
             return self._head(x[:, -1:]), None
         logits = self._head(x)
         return logits, F.cross_entropy(logits.flatten(0, 1), targets.flatten(), ignore_index=-100)
+
+    def loss(self, idx: Tensor, targets: Tensor, ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+        """The cross-entropy of forward(idx, targets) by the operators of lm.py, without the logits in memory: the embedding, every
+        residual addition with the norm after it, and the head with the loss run as one kernel each, forward and backward (CPU
+        tensors: their plain forms). reduction "none" gives every token's loss (B, T): a text's log likelihoods.
+
+        Under autocast the norms hand the layers and the head the autocast type, the stream between the blocks keeps the
+        embedding's, and the head's gradient is summed in fp32 (forward rounds it to the autocast type first), so the two
+        agree to that type's rounding."""
+        if idx.shape[1] > self.config.context_length:
+            raise ValueError(f"sequence length {idx.shape[1]} exceeds context_length {self.config.context_length}")
+        device, weight = idx.device.type, self.transformer.wte.weight
+        dtype = torch.get_autocast_dtype(device) if torch.is_autocast_enabled(device) else weight.dtype
+        x, branch = self.transformer.drop((lm.embedding if idx.is_cuda else lm.embedding_reference)(idx, weight)), None
+        for block in self.transformer.h:
+            x, branch = block.advance(x, branch, dtype)
+        h, _ = _add_norm(self.transformer.ln_f, x, branch, dtype)
+        head = lm.linear_cross_entropy if idx.is_cuda else lm.linear_cross_entropy_reference
+        return head(h, self.lm_head.weight, targets, ignore_index, reduction)
 
     def prefill(self, idx: Tensor, capacity: int | None = None):
         """The prompt in one pass: last-position logits and one cache per layer."""
