@@ -96,6 +96,8 @@ struct XF32 {
 };
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+// the same number in every lane, as a value the compiler keeps in a scalar register (after a division it would not know)
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ lds_void_ptr lds_at(const void* p) { return (lds_void_ptr)(uint32_t)(uintptr_t)p; }
 // element i of a 32 x 32 accumulator: column lane % 32, row acc_row(i, lane / 32)
 __device__ __forceinline__ constexpr int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
@@ -143,8 +145,8 @@ struct Operand {
     else c = pos;   // (the turned swizzle depends on the row within four: below)
     lane_off = r * ld + c * 16;
   }
-  // stage k of the contraction into `to` (the wavefront's share)
-  __device__ __forceinline__ void load(uint8_t* to, int k, int wave) const {
+  // stage k of the contraction into `to` (the wavefront's share), zeros from stage `last` on
+  __device__ __forceinline__ void load(uint8_t* to, int k, int last, int wave) const {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -163,7 +165,7 @@ struct Operand {
         }
         soff = (k * BK + r0) * ld;
       }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(to + 1024 * n), 16, voff, soff, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(to + 1024 * n), 16, voff, k < last ? soff : 0x7fffff00, 0, 0);
     }
   }
   // the fragment of step j (four per stage) of rows (columns) first .. first + 31
@@ -238,26 +240,21 @@ struct Mainloop {
     __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
-  // stages first .. last - 1
-  __device__ __forceinline__ void run(const A& oa, const B& ob, Stage& s0, Stage& s1, int first, int last) {
+  // `stages` of them, two a round (an odd one's last round ends with a stage of zeros: one way out of the loop keeps the sums in
+  // the registers they are in)
+  __device__ __forceinline__ void run(const A& oa, const B& ob, Stage& s0, Stage& s1, int stages) {
     const int wave = wave_index(), wm = wave / WN, wn = wave % WN;
     clear();
-    if (first >= last) return;
-    oa.load(s0.a, first, wave);
-    ob.load(s0.b, first, wave);
+    oa.load(s0.a, 0, stages, wave);
+    ob.load(s0.b, 0, stages, wave);
     arrive();
-    for (int k = first; k < last; k += 2) {
-      if (k + 1 < last) {
-        oa.load(s1.a, k + 1, wave);
-        ob.load(s1.b, k + 1, wave);
-      }
+    for (int k = 0; k < stages; k += 2) {
+      oa.load(s1.a, k + 1, stages, wave);
+      ob.load(s1.b, k + 1, stages, wave);
       step(s0, wm, wn);
       arrive();
-      if (k + 1 >= last) break;
-      if (k + 2 < last) {
-        oa.load(s0.a, k + 2, wave);
-        ob.load(s0.b, k + 2, wave);
-      }
+      oa.load(s0.a, k + 2, stages, wave);
+      ob.load(s0.b, k + 2, stages, wave);
       step(s1, wm, wn);
       arrive();
     }
@@ -273,8 +270,8 @@ __device__ __forceinline__ bool tile_of(int64_t id, int mt, int nt, int& m, int&
   const int band = (int)(t / (8 * (int64_t)nt));
   const int high = min(8, mt - band * 8);
   const int in = (int)(t - (int64_t)band * 8 * nt);
-  m = band * 8 + in % high;
-  n = in / high;
+  n = uniform(in / high);
+  m = uniform(band * 8 + in - n * high);
   return true;
 }
 inline int64_t tiles_grid(int64_t mt, int64_t nt) { return 8 * cdiv(mt * nt, 8); }
@@ -378,7 +375,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
   oa.open((const elem*)c.w + v0 * c.w_ld, ((c.v1 - v0 - 1) * c.w_ld + c.stages * L::BK) * ES, c.w_ld);
   ob.open((const elem*)c.x + n0 * c.x_ld, ((tokens - n0 - 1) * c.x_ld + c.stages * L::BK) * ES, c.x_ld);
   L l;
-  l.run(oa, ob, s0, s1, 0, c.stages);
+  l.run(oa, ob, s0, s1, c.stages);
   const int lane = threadIdx.x & 63, wave = wave_index(), h = lane >> 5, wm = wave / L::WN, wn = wave % L::WN;
   const int64_t vw = v0 + wm * L::TM * 32;   // the wavefront's first row of the vocabulary
   const bool edge = vw + L::TM * 32 > c.v1;
@@ -393,11 +390,13 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
       const int64_t tl = t - vw;
       const bool hit = i < tokens && t < c.v1 && tl >= 0 && tl < L::TM * 32 && ((tl >> 2) & 1) == h;
       if (__ballot(hit)) {
+        const int want = (int)(hit ? tl : -1);
+        float mine = 0.f;
 #pragma unroll
         for (int a = 0; a < L::TM; ++a)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (hit && tl == a * 32 + acc_row(r, h)) c.at[i] = l.acc[a][b][r];
+          for (int r = 0; r < 16; ++r) mine = want == a * 32 + acc_row(r, h) ? l.acc[a][b][r] : mine;
+        if (hit) c.at[i] = mine;
       }
       if (edge) {
 #pragma unroll
@@ -441,12 +440,19 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
     constexpr int RB = L::TM * 32 * ES;   // bytes of a token's row
     static_assert(L::WAVES * 32 * RB <= (int)sizeof(s0), "the wavefronts' rows in a stage");
     uint8_t* mine = reinterpret_cast<uint8_t*>(&s0) + wave * 32 * RB;
-#pragma unroll
+    // (rows past the last token lie past the resource's end: such stores are dropped)
+    const int g_row = (int)(c.g_ld * ES);
+    const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES);
+    const int left = edge ? (int)(c.v1 - vw) : L::TM * 32;   // rows of the vocabulary
+#pragma unroll 1
     for (int b = 0; b < L::TN; ++b) {
       const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
-      const float lse = i < tokens ? c.lse[i] : INFINITY;
-      const float lift = (c.factor && i < tokens ? c.factor[i] : 1.f) * OP::LIFT;
-      const int64_t tl = (i < tokens ? c.targets[c.rows[ROWS_HEAD + i]] : -1) - vw;
+      const bool real = i < tokens;
+      const float lse = real ? c.lse[i] : INFINITY;
+      const float lift = (c.factor && real ? c.factor[i] : 1.f) * OP::LIFT;
+      const int64_t t = real ? c.targets[c.rows[ROWS_HEAD + i]] - vw : -1;
+      const int tl = t >= 0 && t < L::TM * 32 ? (int)t : -1;
+      uint8_t* to = mine + (lane & 31) * RB;
 #pragma unroll
       for (int a = 0; a < L::TM; ++a)
 #pragma unroll
@@ -455,13 +461,16 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int row = a * 32 + 8 * q + 4 * h + r;
-            float x = __builtin_amdgcn_exp2f(fmaf(l.acc[a][b][4 * q + r], LOG2E, -lse));
-            if (tl == row) x -= 1.f;
-            if (edge && vw + row >= c.v1) x = 0.f;
+            float x = l.acc[a][0][4 * q + r];
+#pragma unroll
+            for (int o = 1; o < L::TN; ++o) x = b == o ? l.acc[a][o][4 * q + r] : x;
+            x = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, -lse));
+            x = tl == row ? x - 1.f : x;
+            x = row < left ? x : 0.f;
             p[r] = x * lift;
           }
           const int byte = (a * 32 + 8 * q + 4 * h) * ES;
-          put<true>(mine + (lane & 31) * RB + (((byte >> 4) ^ (lane & 7)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
+          put<true>(to + (((byte >> 4) ^ (lane & 7)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
         }
       __asm__ volatile("" ::: "memory");   // (a wavefront's own LDS accesses run in order)
       constexpr int CPR = RB / 16;
@@ -469,8 +478,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
       for (int k = 0; k < 32 * CPR / 64; ++k) {
         const int slot = k * 64 + lane, r = slot / CPR, ch = slot % CPR;
         const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ((ch ^ (r & 7)) << 4));
-        const int64_t j = n0 + (wn * L::TN + b) * 32 + r;
-        if (j < tokens) *reinterpret_cast<u32x4*>((elem*)c.g + j * c.g_ld + (vw - c.v0) + ch * (16 / ES)) = v;
+        __builtin_amdgcn_raw_buffer_store_b128(v, rs, r * g_row + ch * 16, (wn * L::TN + b) * 32 * g_row, 0);
       }
       __asm__ volatile("" ::: "memory");
     }
@@ -592,45 +600,62 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_produc
   typedef typename OP::elem elem;
   constexpr int ES = sizeof(elem);
   __shared__ typename L::Stage s0, s1;
-  const int64_t tokens = c.rows[0];
+  const int64_t tokens = uniform(c.rows[0]);
   const int64_t M = DW ? c.m : tokens, K = DW ? tokens : c.k;
   int m, n;
   if (!tile_of(blockIdx.x, DW ? c.mt : (int)((M + L::BM - 1) / L::BM), c.nt, m, n)) return;
   const int64_t m0 = (int64_t)m * L::BM, n0 = (int64_t)n * L::BN;
-  typename L::A oa;
-  typename L::B ob;
   const int stages = (int)((K + L::BK - 1) / L::BK);
   const int per = (stages + c.splits - 1) / c.splits;
-  const int first = min((int)blockIdx.y * per, stages), last = min(first + per, stages);
+  const int first = uniform(min((int)blockIdx.y * per, stages)), last = uniform(min(first + per, stages));
   const int64_t k0 = (int64_t)first * L::BK;   // (offsets within a split stay below 2^31 bytes)
+  typename L::A oa;
+  typename L::B ob;
   if constexpr (DW) oa.open((const elem*)c.a + k0 * c.a_ld + m0, ((K - k0) * c.a_ld - m0) * ES, c.a_ld);
   else oa.open((const elem*)c.a + m0 * c.a_ld + k0, ((M - m0) * c.a_ld - k0) * ES, c.a_ld);
   ob.open((const elem*)c.b + k0 * c.b_ld + n0, ((K - k0 - 1) * c.b_ld + c.b_cols - n0) * ES, c.b_ld);
   L l;
-  l.run(oa, ob, s0, s1, 0, last - first);
+  l.run(oa, ob, s0, s1, last - first);
   const int lane = threadIdx.x & 63, wave = wave_index(), h = lane >> 5, wm = wave / L::WN, wn = wave % L::WN;
+  // rows past M lie past the resource's end, columns past N get an offset there: such stores are dropped
+  const int es = c.out ? (c.out_t == SA_DTYPE_F32 ? 4 : 2) : 4;
+  const int64_t ld = c.out ? c.out_ld : c.n_ld;
+  uint8_t* base = (uint8_t*)c.out + m0 * ld * es;
+  if (!c.out) base = (uint8_t*)(c.sums + ((int64_t)blockIdx.y * c.m_rows + m0) * ld);
+  const __amdgpu_buffer_rsrc_t rs = resource(base, min(M - m0, (int64_t)L::BM) * ld * es);
   const float scale = c.out ? *c.scale * c.lift : 1.f;
-#pragma unroll
-  for (int a = 0; a < L::TM; ++a)
+  const int row_bytes = (int)ld * es;
+  const auto each = [&](auto&& put_sixteen) {
 #pragma unroll
     for (int b = 0; b < L::TN; ++b) {
       const int64_t col = n0 + (wn * L::TN + b) * 32 + (lane & 31);
-      if (col >= c.n) continue;
+      const int at = col < c.n ? (int)col * es + 4 * h * row_bytes : 0x7ffffff0;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = m0 + (wm * L::TM + a) * 32 + acc_row(r, h);
-        if (row >= M) continue;
-        float x = l.acc[a][b][r];
-        if (c.out) {
-          void* at = row_of(c.out, row, c.out_ld, c.out_t);
-          if (c.out_t == SA_DTYPE_F32) ((float*)at)[col] = x * scale;
-          else ((uint16_t*)at)[col] = to16(x * scale, c.out_t);
-        } else {
-          float* at = c.sums + ((int64_t)blockIdx.y * c.m_rows + row) * c.n_ld + col;
-          *at = c.add ? *at + x : x;
-        }
-      }
+      for (int a = 0; a < L::TM; ++a) put_sixteen(l.acc[a][b], at, (wm * L::TM + a) * 32);
     }
+  };
+  if (es == 2) {
+    each([&](const f32x16& x, int at, int row) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        __builtin_amdgcn_raw_buffer_store_b16(to16(x[r] * scale, c.out_t), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
+    });
+  } else if (c.add) {
+    each([&](const f32x16& x, int at, int row) {
+      float y[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) y[r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, at, (row + acc_row(r, 0)) * row_bytes, 0));
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[r] + x[r]), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
+    });
+  } else {
+    each([&](const f32x16& x, int at, int row) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[r] * scale), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
+    });
+  }
 }
 
 // dX: a token's parts added, times its factor; zero rows for the tokens that are ignored. dW: the parts of a piece's rows.
