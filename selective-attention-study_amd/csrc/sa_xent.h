@@ -110,11 +110,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_
 // One operand of a tile: EDGE rows (or columns) of the result, KB = 128 bytes of the contraction per stage.
 //
 // Plain: the matrix has the contraction along its rows. A stage holds EDGE rows of 128 bytes; the 16-byte chunk c of row r sits at
-// chunk c ^ (r mod 8), so that the 32 lanes of a fragment read (one chunk of 32 rows) touch all banks evenly.
+// chunk c ^ (r / 2 mod 8): a fragment read takes one chunk of 16 rows a pass over 64 banks, and the eight rows of either parity then take
+// eight chunks (c ^ (r mod 8) has rows r and r + 8 in the same banks: the counters show every read twice as long).
 // Turned (TR): the matrix has the contraction down its columns (K, EDGE). A stage holds 128 / size rows of EDGE elements, and
 // the fragments are read transposed: 16-bit types by ds_read_b64_tr_b16 (lane i of 16 gets as element t the element i % 4 of
-// the 8 bytes that lane 4t + i/4 addresses: four rows of a 16-column range, whose 32 bytes sit at chunk c ^ 2 (r mod 4), so that
-// the four rows fall on different banks), fp32 by one 4-byte read per instruction (32 neighbours of a row).
+// the 8 bytes that lane 4t + i/4 addresses: two groups of 16 read 64 bytes of each of four rows a pass, which sit at chunk c ^ 4 (r
+// mod 4), in banks of their own), fp32 by one 4-byte read per instruction (32 neighbours of a row).
 //
 // The loads go from memory straight into LDS: one instruction fills 64 consecutive 16-byte slots, and each lane fetches the
 // chunk that belongs in its slot. Rows past the resource's end read as zeros.
@@ -132,7 +133,7 @@ struct Operand {
   static_assert(LOADS % WAVES == 0, "whole loads per wavefront");
 
   __amdgpu_buffer_rsrc_t rs;
-  int lane_off, ld;   // bytes
+  int lane_off, odd_off, ld;   // bytes; plain: of the even and of the odd instructions, whose rows' swizzles differ
 
   // p: the tile's first row (plain) or column (turned), at the contraction's start; bytes: what may be read from there
   __device__ __forceinline__ void open(const void* p, int64_t bytes, int64_t ld_elems) {
@@ -140,10 +141,9 @@ struct Operand {
     ld = (int)(ld_elems * ES);
     const int lane = threadIdx.x & 63;
     const int r = lane / LANES, pos = lane % LANES;
-    int c;
-    if constexpr (!TR) c = pos ^ (r & 7);
-    else c = pos;   // (the turned swizzle depends on the row within four: below)
+    const int c = TR ? pos : pos ^ (r >> 1);   // (the turned swizzle: below)
     lane_off = r * ld + c * 16;
+    odd_off = r * ld + (c ^ 4) * 16;
   }
   // stage k of the contraction into `to` (the wavefront's share), zeros from stage `last` on
   __device__ __forceinline__ void load(uint8_t* to, int k, int last, int wave) const {
@@ -153,13 +153,13 @@ struct Operand {
       const int n = wave * PER + i;
       int voff, soff;
       if constexpr (!TR) {
-        voff = lane_off;
+        voff = n & 1 ? odd_off : lane_off;
         soff = n * RPI * ld + k * 128;
       } else {
         const int r0 = (n / IPR) * RPI;   // first row of the instruction
         if constexpr (ES == 2) {
           const int pos = lane % LANES + (n % IPR) * LANES, r = r0 + lane / LANES;
-          voff = (lane / LANES) * ld + ((pos ^ ((r & 3) << 1)) * 16);
+          voff = (lane / LANES) * ld + ((pos ^ ((r & 3) << 2)) * 16);
         } else {
           voff = lane_off + (n % IPR) * 1024;
         }
@@ -173,7 +173,7 @@ struct Operand {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     if constexpr (!TR) {
       const int r = first + (lane & 31);
-      return *reinterpret_cast<const u32x4*>(t + r * 128 + (((2 * j + h) ^ (lane & 7)) << 4));
+      return *reinterpret_cast<const u32x4*>(t + r * 128 + (((2 * j + h) ^ ((lane >> 1) & 7)) << 4));
     } else if constexpr (ES == 2) {
       const int g = lane >> 4, k = lane & 15;
       u32x4 f;
@@ -183,7 +183,7 @@ struct Operand {
         const int c = (first >> 3) + 2 * (g & 1) + ((k & 3) >> 1);
         typedef __attribute__((address_space(3))) short4v* lds_s4;
         const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s4)(uint32_t)(uintptr_t)(t + r * ROW + ((c ^ ((r & 3) << 1)) << 4) + 8 * (k & 1)));
+            (lds_s4)(t + r * ROW + ((c ^ ((r & 3) << 2)) << 4) + 8 * (k & 1)));
         const uint2 u = __builtin_bit_cast(uint2, v);
         f[2 * hf] = u.x;
         f[2 * hf + 1] = u.y;
@@ -222,23 +222,43 @@ struct Mainloop {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
   }
-  __device__ __forceinline__ void step(const Stage& s, int wm, int wn) {
+  struct Frags {
+    u32x4 a[TM], b[TN];
+  };
+  static __device__ __forceinline__ void read(Frags& f, const Stage& s, int j, int wm, int wn) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u32x4 fa[TM], fb[TN];
+    for (int a = 0; a < TM; ++a) f.a[a] = A::frag(s.a, (wm * TM + a) * 32, j);
 #pragma unroll
-      for (int a = 0; a < TM; ++a) fa[a] = A::frag(s.a, (wm * TM + a) * 32, j);
-#pragma unroll
-      for (int b = 0; b < TN; ++b) fb[b] = B::frag(s.b, (wn * TN + b) * 32, j);
-#pragma unroll
-      for (int a = 0; a < TM; ++a)
-#pragma unroll
-        for (int b = 0; b < TN; ++b) acc[a][b] = OP::mma(fa[a], fb[b], acc[a][b]);
-    }
+    for (int b = 0; b < TN; ++b) f.b[b] = B::frag(s.b, (wn * TN + b) * 32, j);
+    __builtin_amdgcn_sched_barrier(0);   // (the reads go out before the products that hide them)
   }
-  static __device__ __forceinline__ void arrive() {   // the loads into the next stage are there, and everyone is done with this one
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __device__ __forceinline__ void multiply(const Frags& f) {
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TN; ++b) acc[a][b] = OP::mma(f.a[a], f.b[b], acc[a][b]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  static __device__ __forceinline__ void arrive() {   // the loads into the next stage are there, and everyone has read this one
+    __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
+  }
+  // The products of `now`, whose first step is in f0, while the loads of two stages on go into the LDS that its last read frees. Each
+  // step's operands are read while the products of the step before run, across the barrier too: the last step's are in
+  // registers by then.
+  __device__ __forceinline__ void stage(const A& oa, const B& ob, Stage& now, const Stage& next, int k, int stages, Frags& f0, Frags& f1,
+                                        int wave, int wm, int wn) {
+    read(f1, now, 1, wm, wn);
+    multiply(f0);
+    read(f0, now, 2, wm, wn);
+    multiply(f1);
+    read(f1, now, 3, wm, wn);
+    multiply(f0);
+    arrive();
+    oa.load(now.a, k + 2, stages, wave);
+    ob.load(now.b, k + 2, stages, wave);
+    read(f0, next, 0, wm, wn);
+    multiply(f1);
   }
   // `stages` of them, two a round (an odd one's last round ends with a stage of zeros: one way out of the loop keeps the sums in
   // the registers they are in)
@@ -248,16 +268,15 @@ struct Mainloop {
     oa.load(s0.a, 0, stages, wave);
     ob.load(s0.b, 0, stages, wave);
     arrive();
+    oa.load(s1.a, 1, stages, wave);
+    ob.load(s1.b, 1, stages, wave);
+    Frags f0, f1;
+    read(f0, s0, 0, wm, wn);
     for (int k = 0; k < stages; k += 2) {
-      oa.load(s1.a, k + 1, stages, wave);
-      ob.load(s1.b, k + 1, stages, wave);
-      step(s0, wm, wn);
-      arrive();
-      oa.load(s0.a, k + 2, stages, wave);
-      ob.load(s0.b, k + 2, stages, wave);
-      step(s1, wm, wn);
-      arrive();
+      stage(oa, ob, s0, s1, k, stages, f0, f1, wave, wm, wn);
+      stage(oa, ob, s1, s0, k + 1, stages, f0, f1, wave, wm, wn);
     }
+    arrive();   // (the last loads, of zeros, are in: the LDS may be used)
   }
 };
 
