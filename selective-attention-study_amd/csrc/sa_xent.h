@@ -107,33 +107,36 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_
 }
 
 // ---------------------------------------------------------------------------------------------
-// One operand of a tile: EDGE rows (or columns) of the result, KB = 128 bytes of the contraction per stage.
+// One operand of a tile: EDGE rows (or columns) of the result, KB = 64 bytes of the contraction per stage.
 //
-// Plain: the matrix has the contraction along its rows. A stage holds EDGE rows of 128 bytes; the 16-byte chunk c of row r sits at
-// chunk c ^ (r / 2 mod 8): a fragment read takes one chunk of 16 rows a pass over 64 banks, and the eight rows of either parity then take
-// eight chunks (c ^ (r mod 8) has rows r and r + 8 in the same banks: the counters show every read twice as long).
-// Turned (TR): the matrix has the contraction down its columns (K, EDGE). A stage holds 128 / size rows of EDGE elements, and
+// Plain: the matrix has the contraction along its rows. A stage holds EDGE rows of 64 bytes; the 16-byte chunk c of row r sits at
+// chunk c ^ (r / 4 mod 4): a fragment read takes one chunk of 16 rows a pass over 64 banks, and the four rows that share banks then
+// take four chunks.
+// Turned (TR): the matrix has the contraction down its columns (K, EDGE). A stage holds 64 / size rows of EDGE elements, and
 // the fragments are read transposed: 16-bit types by ds_read_b64_tr_b16 (lane i of 16 gets as element t the element i % 4 of
 // the 8 bytes that lane 4t + i/4 addresses: two groups of 16 read 64 bytes of each of four rows a pass, which sit at chunk c ^ 4 (r
 // mod 4), in banks of their own), fp32 by one 4-byte read per instruction (32 neighbours of a row).
+// (Measured on the bank-conflict counter: none. With chunks at c ^ (r mod 8) and c ^ 2 (r mod 4) every read took twice as long.)
 //
 // The loads go from memory straight into LDS: one instruction fills 64 consecutive 16-byte slots, and each lane fetches the
 // chunk that belongs in its slot. Rows past the resource's end read as zeros.
+constexpr int KB = 64;
+
 template <class OP, int EDGE, bool TR, int WAVES>
 struct Operand {
   static constexpr int ES = sizeof(typename OP::elem);
-  static constexpr int BYTES = EDGE * 128;
-  static constexpr int BK = 128 / ES;
-  static constexpr int ROW = TR ? EDGE * ES : 128;        // bytes of a staged row
+  static constexpr int BYTES = EDGE * KB;
+  static constexpr int BK = KB / ES;
+  static constexpr int ROW = TR ? EDGE * ES : KB;               // bytes of a staged row
   static constexpr int LANES = ROW / 16 < 64 ? ROW / 16 : 64;   // lanes of an instruction on one row
-  static constexpr int RPI = 64 / LANES;                  // rows of an instruction
-  static constexpr int IPR = ROW / (16 * LANES);          // instructions of a row
-  static constexpr int LOADS = BYTES / 1024;              // instructions of a stage
-  static constexpr int PER = LOADS / WAVES;
+  static constexpr int RPI = 64 / LANES;                        // rows of an instruction
+  static constexpr int IPR = ROW / (16 * LANES);                // instructions of a row
+  static constexpr int LOADS = BYTES / 1024;                    // instructions of a stage
+  static constexpr int PER = LOADS / WAVES;                     // and of a wavefront
   static_assert(LOADS % WAVES == 0, "whole loads per wavefront");
 
   __amdgpu_buffer_rsrc_t rs;
-  int lane_off, odd_off, ld;   // bytes; plain: of the even and of the odd instructions, whose rows' swizzles differ
+  int lane_off, ld;   // bytes
 
   // p: the tile's first row (plain) or column (turned), at the contraction's start; bytes: what may be read from there
   __device__ __forceinline__ void open(const void* p, int64_t bytes, int64_t ld_elems) {
@@ -141,9 +144,7 @@ struct Operand {
     ld = (int)(ld_elems * ES);
     const int lane = threadIdx.x & 63;
     const int r = lane / LANES, pos = lane % LANES;
-    const int c = TR ? pos : pos ^ (r >> 1);   // (the turned swizzle: below)
-    lane_off = r * ld + c * 16;
-    odd_off = r * ld + (c ^ 4) * 16;
+    lane_off = r * ld + (TR ? pos : pos ^ ((r >> 2) & 3)) * 16;   // (the turned swizzle: below)
   }
   // stage k of the contraction into `to` (the wavefront's share), zeros from stage `last` on
   __device__ __forceinline__ void load(uint8_t* to, int k, int last, int wave) const {
@@ -151,10 +152,9 @@ struct Operand {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int n = wave * PER + i;
-      int voff, soff;
+      int voff = lane_off, soff;
       if constexpr (!TR) {
-        voff = n & 1 ? odd_off : lane_off;
-        soff = n * RPI * ld + k * 128;
+        soff = n * RPI * ld + k * KB;
       } else {
         const int r0 = (n / IPR) * RPI;   // first row of the instruction
         if constexpr (ES == 2) {
@@ -168,12 +168,12 @@ struct Operand {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(to + 1024 * n), 16, voff, k < last ? soff : 0x7fffff00, 0, 0);
     }
   }
-  // the fragment of step j (four per stage) of rows (columns) first .. first + 31
+  // the fragment of step j (two per stage) of rows (columns) first .. first + 31
   static __device__ __forceinline__ u32x4 frag(const uint8_t* t, int first, int j) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     if constexpr (!TR) {
       const int r = first + (lane & 31);
-      return *reinterpret_cast<const u32x4*>(t + r * 128 + (((2 * j + h) ^ ((lane >> 1) & 7)) << 4));
+      return *reinterpret_cast<const u32x4*>(t + r * KB + (((2 * j + h) ^ ((lane >> 2) & 3)) << 4));
     } else if constexpr (ES == 2) {
       const int g = lane >> 4, k = lane & 15;
       u32x4 f;
@@ -182,8 +182,9 @@ struct Operand {
         const int r = 16 * j + 8 * (g >> 1) + 4 * hf + (k >> 2);
         const int c = (first >> 3) + 2 * (g & 1) + ((k & 3) >> 1);
         typedef __attribute__((address_space(3))) short4v* lds_s4;
-        const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s4)(t + r * ROW + ((c ^ ((r & 3) << 2)) << 4) + 8 * (k & 1)));
+        // (one sum: after a chain of additions the compiler no longer knows which variable is read, and waits for all loads in flight)
+        const int at = r * ROW + ((c ^ ((r & 3) << 2)) << 4) + 8 * (k & 1);
+        const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + at));
         const uint2 u = __builtin_bit_cast(uint2, v);
         f[2 * hf] = u.x;
         f[2 * hf + 1] = u.y;
@@ -199,18 +200,23 @@ struct Operand {
   }
 };
 
-// A tile of WM x WN wavefronts, each TM x TN squares of 32: acc[a][b] += A B^T over `stages` of the contraction. Two stages in LDS, in
-// variables of their own (one array indexed by the stage's parity makes the compiler wait for the loads in flight before it reads).
+// A tile of WM x WN wavefronts, each TM x TN squares of 32: acc[a][b] += A B^T over `stages` of the contraction. A ring of four stages in
+// LDS, in variables of their own (one array indexed by the stage makes the compiler wait for the loads in flight before it
+// reads): while one is multiplied, the loads of the next three are under way, since a stage of the larger tiles (32 KB, 1024
+// cycles of the matrix units) is over before memory has answered.
 template <class OP, int WM_, int WN_, int TM_, int TN_, bool TRA, bool TRB>
 struct Mainloop {
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
   typedef Operand<OP, BM, TRA, WAVES> A;
   typedef Operand<OP, BN, TRB, WAVES> B;
-  static constexpr int BK = A::BK;
+  static constexpr int BK = A::BK, LOADS = A::PER + B::PER;
   struct Stage {
     alignas(1024) uint8_t a[A::BYTES];
     alignas(1024) uint8_t b[B::BYTES];
+  };
+  struct Frags {
+    u32x4 a[TM], b[TN];
   };
   f32x16 acc[TM][TN];
 
@@ -222,9 +228,6 @@ struct Mainloop {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
   }
-  struct Frags {
-    u32x4 a[TM], b[TN];
-  };
   static __device__ __forceinline__ void read(Frags& f, const Stage& s, int j, int wm, int wn) {
 #pragma unroll
     for (int a = 0; a < TM; ++a) f.a[a] = A::frag(s.a, (wm * TM + a) * 32, j);
@@ -239,44 +242,44 @@ struct Mainloop {
       for (int b = 0; b < TN; ++b) acc[a][b] = OP::mma(f.a[a], f.b[b], acc[a][b]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  static __device__ __forceinline__ void arrive() {   // the loads into the next stage are there, and everyone has read this one
-    __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __syncthreads();
+  // everyone has read what they wanted, and all but everyone's last PENDING loads are there
+  template <int PENDING>
+  static __device__ __forceinline__ void arrive() {
+    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PENDING) : "memory");
   }
-  // The products of `now`, whose first step is in f0, while the loads of two stages on go into the LDS that its last read frees. Each
-  // step's operands are read while the products of the step before run, across the barrier too: the last step's are in
-  // registers by then.
+  static __device__ __forceinline__ void load(const A& oa, const B& ob, Stage& s, int k, int stages, int wave) {
+    oa.load(s.a, k, stages, wave);
+    ob.load(s.b, k, stages, wave);
+  }
+  // The products of stage k, in `now`, whose first step's operands are in f0. Each step's are read while the products of the step before
+  // run, across the barrier too: the last step's are in registers by then, and `now` takes stage k + 4.
   __device__ __forceinline__ void stage(const A& oa, const B& ob, Stage& now, const Stage& next, int k, int stages, Frags& f0, Frags& f1,
                                         int wave, int wm, int wn) {
     read(f1, now, 1, wm, wn);
     multiply(f0);
-    read(f0, now, 2, wm, wn);
-    multiply(f1);
-    read(f1, now, 3, wm, wn);
-    multiply(f0);
-    arrive();
-    oa.load(now.a, k + 2, stages, wave);
-    ob.load(now.b, k + 2, stages, wave);
+    arrive<2 * LOADS>();
+    load(oa, ob, now, k + 4, stages, wave);
     read(f0, next, 0, wm, wn);
     multiply(f1);
   }
-  // `stages` of them, two a round (an odd one's last round ends with a stage of zeros: one way out of the loop keeps the sums in
-  // the registers they are in)
-  __device__ __forceinline__ void run(const A& oa, const B& ob, Stage& s0, Stage& s1, int stages) {
+  // (Stages past the last are of zeros: one way out of the loop keeps the sums in the registers they are in.)
+  __device__ __forceinline__ void run(const A& oa, const B& ob, Stage& s0, Stage& s1, Stage& s2, Stage& s3, int stages) {
     const int wave = wave_index(), wm = wave / WN, wn = wave % WN;
     clear();
-    oa.load(s0.a, 0, stages, wave);
-    ob.load(s0.b, 0, stages, wave);
-    arrive();
-    oa.load(s1.a, 1, stages, wave);
-    ob.load(s1.b, 1, stages, wave);
+    load(oa, ob, s0, 0, stages, wave);
+    load(oa, ob, s1, 1, stages, wave);
+    load(oa, ob, s2, 2, stages, wave);
+    load(oa, ob, s3, 3, stages, wave);
+    arrive<3 * LOADS>();
     Frags f0, f1;
     read(f0, s0, 0, wm, wn);
-    for (int k = 0; k < stages; k += 2) {
+    for (int k = 0; k < stages; k += 4) {
       stage(oa, ob, s0, s1, k, stages, f0, f1, wave, wm, wn);
-      stage(oa, ob, s1, s0, k + 1, stages, f0, f1, wave, wm, wn);
+      stage(oa, ob, s1, s2, k + 1, stages, f0, f1, wave, wm, wn);
+      stage(oa, ob, s2, s3, k + 2, stages, f0, f1, wave, wm, wn);
+      stage(oa, ob, s3, s0, k + 3, stages, f0, f1, wave, wm, wn);
     }
-    arrive();   // (the last loads, of zeros, are in: the LDS may be used)
+    arrive<0>();   // (the last loads, of zeros, are in: the LDS may be used)
   }
 };
 
@@ -384,7 +387,7 @@ template <class OP, class L, bool GRAD>
 __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits_kernel(LogitsCall c) {
   typedef typename OP::elem elem;
   constexpr int ES = sizeof(elem);
-  __shared__ typename L::Stage s0, s1;
+  __shared__ typename L::Stage s0, s1, s2, s3;
   const int64_t tokens = c.rows ? c.rows[0] : c.tokens;
   int m, n;
   if (!tile_of(blockIdx.x, c.mt, (int)((tokens + L::BN - 1) / L::BN), m, n)) return;
@@ -394,7 +397,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
   oa.open((const elem*)c.w + v0 * c.w_ld, ((c.v1 - v0 - 1) * c.w_ld + c.stages * L::BK) * ES, c.w_ld);
   ob.open((const elem*)c.x + n0 * c.x_ld, ((tokens - n0 - 1) * c.x_ld + c.stages * L::BK) * ES, c.x_ld);
   L l;
-  l.run(oa, ob, s0, s1, c.stages);
+  l.run(oa, ob, s0, s1, s2, s3, c.stages);
   const int lane = threadIdx.x & 63, wave = wave_index(), h = lane >> 5, wm = wave / L::WN, wn = wave % L::WN;
   const int64_t vw = v0 + wm * L::TM * 32;   // the wavefront's first row of the vocabulary
   const bool edge = vw + L::TM * 32 > c.v1;
@@ -457,8 +460,9 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
     // G of 32 tokens x the wavefront's rows goes through a part of LDS of its own, so that a token's row is stored in
     // 16-byte pieces side by side. Chunk c of token row r sits at c ^ (r mod 8).
     constexpr int RB = L::TM * 32 * ES;   // bytes of a token's row
-    static_assert(L::WAVES * 32 * RB <= (int)sizeof(s0), "the wavefronts' rows in a stage");
-    uint8_t* mine = reinterpret_cast<uint8_t*>(&s0) + wave * 32 * RB;
+    constexpr int FIT = (int)sizeof(s0) / (32 * RB);   // wavefronts' rows in a stage
+    static_assert(L::WAVES <= 2 * FIT, "and in two");
+    uint8_t* mine = (wave < FIT ? s0.a : s1.a) + wave % FIT * 32 * RB;
     // (rows past the last token lie past the resource's end: such stores are dropped)
     const int g_row = (int)(c.g_ld * ES);
     const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES);
@@ -618,7 +622,7 @@ template <class OP, class L, bool DW>
 __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_product_kernel(ProductCall c) {
   typedef typename OP::elem elem;
   constexpr int ES = sizeof(elem);
-  __shared__ typename L::Stage s0, s1;
+  __shared__ typename L::Stage s0, s1, s2, s3;
   const int64_t tokens = uniform(c.rows[0]);
   const int64_t M = DW ? c.m : tokens, K = DW ? tokens : c.k;
   int m, n;
@@ -634,7 +638,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_produc
   else oa.open((const elem*)c.a + m0 * c.a_ld + k0, ((M - m0) * c.a_ld - k0) * ES, c.a_ld);
   ob.open((const elem*)c.b + k0 * c.b_ld + n0, ((K - k0 - 1) * c.b_ld + c.b_cols - n0) * ES, c.b_ld);
   L l;
-  l.run(oa, ob, s0, s1, last - first);
+  l.run(oa, ob, s0, s1, s2, s3, last - first);
   const int lane = threadIdx.x & 63, wave = wave_index(), h = lane >> 5, wm = wave / L::WN, wn = wave % L::WN;
   // rows past M lie past the resource's end, columns past N get an offset there: such stores are dropped
   const int es = c.out ? (c.out_t == SA_DTYPE_F32 ? 4 : 2) : 4;
@@ -710,7 +714,7 @@ template <class OP>
 struct XentConfigs {   // 16-bit products
   typedef Mainloop<OP, 2, 4, 4, 2, false, false> Large;   // 256 x 256
   typedef Mainloop<OP, 2, 2, 2, 2, false, false> Middle;  // 128 x 128
-  typedef Mainloop<OP, 4, 1, 1, 1, false, false> Small;   // 128 x 32
+  typedef Mainloop<OP, 4, 1, 1, 2, false, false> Small;   // 128 x 64
   typedef Mainloop<OP, 2, 4, 4, 2, false, true> LargeX;
   typedef Mainloop<OP, 2, 2, 2, 2, false, true> MiddleX;
   typedef Mainloop<OP, 2, 4, 4, 2, true, true> LargeW;
@@ -720,14 +724,14 @@ template <>
 struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per stage; one size)
   typedef Mainloop<XF32, 2, 2, 2, 2, false, false> Large;
   typedef Mainloop<XF32, 2, 2, 2, 2, false, false> Middle;
-  typedef Mainloop<XF32, 4, 1, 1, 1, false, false> Small;
+  typedef Mainloop<XF32, 4, 1, 1, 2, false, false> Small;
   typedef Mainloop<XF32, 2, 2, 2, 2, false, true> LargeX;
   typedef Mainloop<XF32, 2, 2, 2, 2, false, true> MiddleX;
   typedef Mainloop<XF32, 2, 2, 2, 2, true, true> LargeW;
   typedef Mainloop<XF32, 2, 2, 2, 2, true, true> MiddleW;
 };
 
-constexpr int64_t SMALL_TOKENS = 32;      // one tile's tokens of the smallest kernel
+constexpr int64_t SMALL_TOKENS = 64;      // one tile's tokens of the smallest kernel
 constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of G
 constexpr int64_t MAX_LD_BYTES = 1 << 22;             // 256 rows within a buffer resource's 2 GiB
@@ -735,7 +739,7 @@ constexpr int64_t MAX_LD_BYTES = 1 << 22;             // 256 rows within a buffe
 // What a call does, from its sizes alone.
 template <class OP>
 struct XentShape {
-  static constexpr int ES = sizeof(typename OP::elem), BK = 128 / ES;
+  static constexpr int ES = sizeof(typename OP::elem), BK = KB / ES;
   bool train, small, large, gather, copy_w;
   int64_t padded, bm, mt, join_blocks;
   // backward
