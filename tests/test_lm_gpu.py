@@ -213,7 +213,7 @@ def embed_check(ids, w, scale, y=None, dy=None, dw=None):
 
 
 EMBEDS = [(1, 1, 1), (1, 300, 64), (31, 5, 7), (32, 1, 256), (33, 1, 256), (64, 2, 257), (1000, 257, 768), (4097, 50304, 96),
-          (5000, 256, 1001), (8193, 1000, 33), (20000, 3, 64), (16384, 70001, 40)]
+          (5000, 256, 1001), (8193, 1000, 33), (20000, 3, 64), (16384, 70001, 40), (3000, 600001, 8)]
 
 
 @pytest.mark.parametrize("tokens,vocab,width", EMBEDS)
