@@ -200,6 +200,12 @@ struct Operand {
   }
 };
 
+template <int A_BYTES, int B_BYTES>
+struct StageOf {
+  alignas(1024) uint8_t a[A_BYTES];
+  alignas(1024) uint8_t b[B_BYTES];
+};
+
 // A tile of WM x WN wavefronts, each TM x TN squares of 32: acc[a][b] += A B^T over `stages` of the contraction. A ring of four stages in
 // LDS, in variables of their own (one array indexed by the stage makes the compiler wait for the loads in flight before it
 // reads): while one is multiplied, the loads of the next three are under way, since a stage of the larger tiles (32 KB, 1024
@@ -211,10 +217,7 @@ struct Mainloop {
   typedef Operand<OP, BM, TRA, WAVES> A;
   typedef Operand<OP, BN, TRB, WAVES> B;
   static constexpr int BK = A::BK, LOADS = A::PER + B::PER;
-  struct Stage {
-    alignas(1024) uint8_t a[A::BYTES];
-    alignas(1024) uint8_t b[B::BYTES];
-  };
+  typedef StageOf<A::BYTES, B::BYTES> Stage;
   struct Frags {
     u32x4 a[TM], b[TN];
   };
@@ -384,13 +387,13 @@ struct LogitsCall {
 };
 
 template <class OP, class L, bool GRAD>
-__global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits_kernel(LogitsCall c) {
+__device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typename L::Stage& s0, typename L::Stage& s1,
+                                            typename L::Stage& s2, typename L::Stage& s3) {
   typedef typename OP::elem elem;
   constexpr int ES = sizeof(elem);
-  __shared__ typename L::Stage s0, s1, s2, s3;
   const int64_t tokens = c.rows ? c.rows[0] : c.tokens;
   int m, n;
-  if (!tile_of(blockIdx.x, c.mt, (int)((tokens + L::BN - 1) / L::BN), m, n)) return;
+  if (!tile_of(id, c.mt, (int)((tokens + L::BN - 1) / L::BN), m, n)) return;
   const int64_t v0 = c.v0 + (int64_t)m * L::BM, n0 = (int64_t)n * L::BN;
   typename L::A oa;
   typename L::B ob;
@@ -508,6 +511,12 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
   }
 }
 
+template <class OP, class L>
+__global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits_kernel(LogitsCall c) {
+  __shared__ typename L::Stage s0, s1, s2, s3;
+  logits_tile<OP, L, false>(c, blockIdx.x, s0, s1, s2, s3);
+}
+
 // A token's statistics over the mt tiles joined: 8 lanes a token. lse (base 2), the loss, and the workgroup's sum of losses.
 __global__ __launch_bounds__(NTHREADS) void xent_join_kernel(LogitsCall c, float* lse, float* each, float* sums, int64_t ignore) {
   __shared__ float part[NTHREADS / 32];
@@ -619,18 +628,18 @@ struct ProductCall {
 };
 
 template <class OP, class L, bool DW>
-__global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_product_kernel(ProductCall c) {
+__device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, int part, typename L::Stage& s0, typename L::Stage& s1,
+                                             typename L::Stage& s2, typename L::Stage& s3) {
   typedef typename OP::elem elem;
   constexpr int ES = sizeof(elem);
-  __shared__ typename L::Stage s0, s1, s2, s3;
   const int64_t tokens = uniform(c.rows[0]);
   const int64_t M = DW ? c.m : tokens, K = DW ? tokens : c.k;
   int m, n;
-  if (!tile_of(blockIdx.x, DW ? c.mt : (int)((M + L::BM - 1) / L::BM), c.nt, m, n)) return;
+  if (!tile_of(id, DW ? c.mt : (int)((M + L::BM - 1) / L::BM), c.nt, m, n)) return;
   const int64_t m0 = (int64_t)m * L::BM, n0 = (int64_t)n * L::BN;
   const int stages = (int)((K + L::BK - 1) / L::BK);
   const int per = (stages + c.splits - 1) / c.splits;
-  const int first = uniform(min((int)blockIdx.y * per, stages)), last = uniform(min(first + per, stages));
+  const int first = uniform(min(part * per, stages)), last = uniform(min(first + per, stages));
   const int64_t k0 = (int64_t)first * L::BK;   // (offsets within a split stay below 2^31 bytes)
   typename L::A oa;
   typename L::B ob;
@@ -644,7 +653,7 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_produc
   const int es = c.out ? (c.out_t == SA_DTYPE_F32 ? 4 : 2) : 4;
   const int64_t ld = c.out ? c.out_ld : c.n_ld;
   uint8_t* base = (uint8_t*)c.out + m0 * ld * es;
-  if (!c.out) base = (uint8_t*)(c.sums + ((int64_t)blockIdx.y * c.m_rows + m0) * ld);
+  if (!c.out) base = (uint8_t*)(c.sums + ((int64_t)part * c.m_rows + m0) * ld);
   const __amdgpu_buffer_rsrc_t rs = resource(base, min(M - m0, (int64_t)L::BM) * ld * es);
   const float scale = c.out ? *c.scale * c.lift : 1.f;
   const int row_bytes = (int)ld * es;
@@ -678,6 +687,29 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_produc
       for (int r = 0; r < 16; ++r)
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[r] * scale), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
     });
+  }
+}
+
+// One pass of the backward over the vocabulary: dX's and dW's products of a piece and G of the next one, which do not depend on
+// each other, in one launch. The products of a piece are a few hundred long tiles (dW's contract over all tokens), fewer than two rounds
+// of the chip or just over one; the many short tiles of G fill what they leave idle. Workgroups start in order: the longest first.
+struct PassCall {
+  LogitsCall g;
+  ProductCall x, w;
+  int x_at, x_tiles, x_end, w_at, w_tiles, w_end, g_at;   // workgroups: of a part of the contraction, of all parts
+};
+template <class OP, class LG, class LX, class LW>
+__global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass_kernel(PassCall c) {
+  __shared__ typename LG::Stage s0, s1, s2, s3;
+  const int id = blockIdx.x;
+  if (id >= c.x_at && id < c.x_end) {
+    const int part = uniform((id - c.x_at) / c.x_tiles);
+    product_tile<OP, LX, false>(c.x, id - c.x_at - part * c.x_tiles, part, s0, s1, s2, s3);
+  } else if (id >= c.w_at && id < c.w_end) {
+    const int part = uniform((id - c.w_at) / c.w_tiles);
+    product_tile<OP, LW, true>(c.w, id - c.w_at - part * c.w_tiles, part, s0, s1, s2, s3);
+  } else {
+    logits_tile<OP, LG, true>(c.g, id - c.g_at, s0, s1, s2, s3);
   }
 }
 
@@ -733,7 +765,7 @@ struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per st
 
 constexpr int64_t SMALL_TOKENS = 64;      // one tile's tokens of the smallest kernel
 constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are
-constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of G
+constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of a piece's G, of which there are two at a time
 constexpr int64_t MAX_LD_BYTES = 1 << 22;             // 256 rows within a buffer resource's 2 GiB
 
 // What a call does, from its sizes alone.
@@ -744,10 +776,10 @@ struct XentShape {
   int64_t padded, bm, mt, join_blocks;
   // backward
   int64_t piece, pieces;
-  bool large_x, large_w;
-  int splits_x, splits_w;
+  bool large_pass;
+  int splits_x, splits_w, splits_last;   // parts of dX's contraction, of dW's, and of that in the last pass
   // workspace
-  int64_t x, w, top, sum, at, sums, factors, g, dx, dw, total;
+  int64_t x, w, top, sum, at, sums, factors, g, g2, dx, dw, total;
 
   XentShape(const XentCall& c, bool backward) {
     train = c.lse != nullptr;
@@ -781,41 +813,67 @@ struct XentShape {
       pieces = cdiv(c.vocab, most);
       piece = align_up(cdiv(c.vocab, pieces), 256);
       pieces = cdiv(c.vocab, piece);
-      const int64_t k_x = cdiv(piece, BK), k_w = cdiv(c.tokens, BK);
-      const auto split = [&](int64_t tiles, int64_t stages) {   // fill the chip where tiles are few: parts of 4 stages or more
-        return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(2 * c.cus, tiles), stages / 4, 16}));
-      };
-      large_x = ES == 2 && cdiv(c.tokens, 256) * cdiv(c.width, 256) >= c.cus / 2;
-      large_w = ES == 2 && (piece / 256) * cdiv(c.width, 256) >= c.cus / 4;
-      const int64_t tx = large_x ? 256 : 128, tw = large_w ? 256 : 128;
-      const int64_t tiles_x = cdiv(c.tokens, tx) * cdiv(c.width, tx), tiles_w = cdiv(piece, tw) * cdiv(c.width, tw);
-      splits_x = tiles_x >= c.cus / 2 ? 1 : split(tiles_x, k_x);
-      splits_w = tiles_w >= c.cus / 2 ? 1 : split(tiles_w, k_w);
+      // Tiles as large as leave every CU a few to do, and no contraction longer than a CU's share of a pass (half of it in the
+      // last, where no tiles of G fill up): a part more costs its sums' way through memory
+      const int64_t k_x = cdiv(piece, BK), k_w = cdiv(c.tokens, BK), k_g = padded / BK;
+      const auto tiles = [&](int64_t edge, int64_t m, int64_t n) { return cdiv(m, edge) * cdiv(n, edge); };
+      large_pass = ES == 2 && tiles(256, c.tokens, c.width) + tiles(256, piece, c.width) + tiles(256, c.tokens, piece) / 4 >= c.cus;
+      const int64_t edge = large_pass ? 256 : 128, slots = large_pass ? c.cus : 2 * (int64_t)c.cus;
+      const int64_t products = (c.dx ? tiles(edge, c.tokens, c.width) * k_x : 0) + (c.dw ? tiles(edge, piece, c.width) * k_w : 0);
+      const int64_t share = cdiv(products + (pieces > 1 ? tiles(edge, c.tokens, piece) * (k_g + 8) : products / 2), slots);
+      const int64_t share_last = std::max<int64_t>(cdiv(products, 2 * slots), 1);
+      const auto parts = [](int64_t stages, int64_t of) { return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(stages, of), stages / 8, 16})); };
+      splits_x = parts(k_x, pieces > 1 ? share : share_last);
+      splits_w = parts(k_w, share);
+      splits_last = parts(k_w, share_last);
       // (a part's rows lie within 2^30 bytes)
       const int64_t w_row = (copy_w ? padded : c.w_ld) * ES, x_row = std::max(padded, piece) * ES;
       splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
       splits_w = std::max(splits_w, (int)cdiv(c.tokens * x_row, (int64_t)1 << 30));
+      splits_last = std::max(splits_last, splits_w);
       factors = take((c.tokens + 16) * 4);
       g = take(c.tokens * piece * ES);
+      g2 = take(pieces > 1 ? c.tokens * piece * ES : 0);
       dx = take(c.dx ? splits_x * c.tokens * padded * 4 : 0);
-      dw = take(c.dw && splits_w > 1 ? splits_w * piece * padded * 4 : 0);
+      dw = take(c.dw && splits_last > 1 ? splits_last * piece * padded * 4 : 0);
     }
     total = p;
   }
 };
 
-template <class OP, class L, bool GRAD>
+template <class OP, class L>
 void launch_logits(LogitsCall lc, int64_t tokens, hipStream_t st) {
   lc.mt = (int)cdiv(lc.v1 - lc.v0, L::BM);
   lc.nt = (int)cdiv(tokens, L::BN);
-  hipLaunchKernelGGL((xent_logits_kernel<OP, L, GRAD>), dim3((unsigned)tiles_grid(lc.mt, lc.nt)), dim3(L::THREADS), 0, st, lc);
+  hipLaunchKernelGGL((xent_logits_kernel<OP, L>), dim3((unsigned)tiles_grid(lc.mt, lc.nt)), dim3(L::THREADS), 0, st, lc);
 }
-template <class OP, class L, bool DW>
-void launch_product(ProductCall pc, int64_t rows, hipStream_t st) {
-  pc.mt = (int)cdiv(rows, L::BM);
-  pc.nt = (int)cdiv(pc.n, L::BN);
-  hipLaunchKernelGGL((xent_product_kernel<OP, L, DW>), dim3((unsigned)tiles_grid(pc.mt, pc.nt), (unsigned)pc.splits), dim3(L::THREADS),
-                     0, st, pc);
+// g, x, w: what the pass does (null: not that)
+template <class OP, class LG, class LX, class LW>
+void launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w, int64_t tokens, hipStream_t st) {
+  PassCall pc{};
+  int64_t at = 0;
+  const auto place = [&at](ProductCall& c, int64_t m, int edge_m, int edge_n, int& begin, int& tiles, int& end) {
+    c.mt = (int)cdiv(m, edge_m);
+    c.nt = (int)cdiv(c.n, edge_n);
+    tiles = (int)tiles_grid(c.mt, c.nt);
+    begin = (int)at;
+    end = (int)(at += (int64_t)tiles * c.splits);
+  };
+  const auto put_x = [&] {
+    if (x) pc.x = *x, place(pc.x, tokens, LX::BM, LX::BN, pc.x_at, pc.x_tiles, pc.x_end);
+  };
+  const bool x_first = x && w && cdiv(x->k, x->splits) > cdiv(tokens, w->splits);
+  if (x_first) put_x();
+  if (w) pc.w = *w, place(pc.w, w->m, LW::BM, LW::BN, pc.w_at, pc.w_tiles, pc.w_end);
+  if (!x_first) put_x();
+  if (g) {
+    pc.g = *g;
+    pc.g.mt = (int)cdiv(g->v1 - g->v0, LG::BM);
+    pc.g.nt = (int)cdiv(tokens, LG::BN);
+    pc.g_at = (int)at;
+    at += tiles_grid(pc.g.mt, pc.g.nt);
+  }
+  hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
 }
 template <class OP>
 void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows,
@@ -858,9 +916,9 @@ int xent_forward(const XentCall& c) {
   lc.v0 = 0, lc.v1 = c.vocab;
   lc.stages = (int)(s.padded / s.BK);
   lc.top = (float*)(ws + s.top), lc.sum = (float*)(ws + s.sum), lc.at = (float*)(ws + s.at);
-  if (s.small) launch_logits<OP, typename F::Small, false>(lc, c.tokens, c.st);
-  else if (s.large) launch_logits<OP, typename F::Large, false>(lc, c.tokens, c.st);
-  else launch_logits<OP, typename F::Middle, false>(lc, c.tokens, c.st);
+  if (s.small) launch_logits<OP, typename F::Small>(lc, c.tokens, c.st);
+  else if (s.large) launch_logits<OP, typename F::Large>(lc, c.tokens, c.st);
+  else launch_logits<OP, typename F::Middle>(lc, c.tokens, c.st);
   lc.mt = (int)s.mt;
   float* sums = each ? nullptr : (float*)(ws + s.sums);
   hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)s.join_blocks), dim3(NTHREADS), 0, c.st, lc, c.lse, each, sums, c.ignore);
@@ -886,33 +944,32 @@ int xent_backward(const XentCall& c) {
     launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, ws + s.w, s.padded, c.st);
     w = ws + s.w, w_ld = s.padded;
   }
-  for (int64_t v0 = 0; v0 < c.vocab; v0 += s.piece) {
-    const int64_t v1 = std::min(v0 + s.piece, c.vocab);
-    LogitsCall lc{};
-    lc.w = w, lc.w_ld = w_ld, lc.x = ws + s.x, lc.x_ld = s.padded, lc.targets = c.targets, lc.rows = c.rows, lc.tokens = c.tokens;
-    lc.vocab = c.vocab, lc.v0 = v0, lc.v1 = v1, lc.stages = (int)(s.padded / s.BK), lc.lse = c.lse, lc.factor = factor, lc.g = ws + s.g, lc.g_ld = s.piece;
-    if (ES == 2 && cdiv(v1 - v0, 256) * cdiv(c.tokens, 256) >= c.cus) launch_logits<OP, typename F::Large, true>(lc, c.tokens, c.st);
-    else launch_logits<OP, typename F::Middle, true>(lc, c.tokens, c.st);
-    if (c.dx) {
-      ProductCall pc{};
-      pc.a = lc.g, pc.a_ld = s.piece, pc.b = (const char*)w + v0 * w_ld * ES, pc.b_ld = w_ld, pc.rows = c.rows, pc.n = pc.b_cols = s.padded, pc.k = v1 - v0;
-      pc.splits = s.splits_x, pc.sums = (float*)(ws + s.dx), pc.n_ld = s.padded, pc.m_rows = c.tokens, pc.add = v0 > 0;
-      if (s.large_x) launch_product<OP, typename F::LargeX, false>(pc, c.tokens, c.st);
-      else launch_product<OP, typename F::MiddleX, false>(pc, c.tokens, c.st);
+  // pass p: G of piece p, and the products of piece p - 1
+  for (int64_t p = 0; p <= s.pieces; ++p) {
+    LogitsCall g{};
+    if (p < s.pieces) {
+      g.w = w, g.w_ld = w_ld, g.x = ws + s.x, g.x_ld = s.padded, g.targets = c.targets, g.rows = c.rows, g.tokens = c.tokens;
+      g.vocab = c.vocab, g.v0 = p * s.piece, g.v1 = std::min(g.v0 + s.piece, c.vocab), g.stages = (int)(s.padded / s.BK);
+      g.lse = c.lse, g.factor = factor, g.g = ws + (p & 1 ? s.g2 : s.g), g.g_ld = s.piece;
     }
-    if (c.dw) {
-      ProductCall pc{};
-      pc.a = lc.g, pc.a_ld = s.piece, pc.b = ws + s.x, pc.b_ld = s.padded, pc.rows = c.rows, pc.m = v1 - v0, pc.n = c.width, pc.b_cols = s.padded;
-      pc.splits = s.splits_w, pc.lift = 1.f / OP::LIFT, pc.scale = scale;
-      char* out = (char*)c.dw + v0 * c.width * lm_elem_size(c.w_t);
-      if (s.splits_w == 1) pc.out = out, pc.out_ld = c.width, pc.out_t = c.w_t;
-      else pc.sums = (float*)(ws + s.dw), pc.n_ld = s.padded, pc.m_rows = s.piece;
-      if (s.large_w) launch_product<OP, typename F::LargeW, true>(pc, v1 - v0, c.st);
-      else launch_product<OP, typename F::MiddleW, true>(pc, v1 - v0, c.st);
-      if (s.splits_w > 1)
-        launch_finish(pc.sums, s.splits_w, s.piece * s.padded, s.padded, nullptr, scale, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t,
-                      c.st);
+    ProductCall px{}, pw{};
+    const int64_t v0 = (p - 1) * s.piece, v1 = std::min(v0 + s.piece, c.vocab);
+    char* out = (char*)c.dw + v0 * c.width * lm_elem_size(c.w_t);
+    if (p > 0) {
+      px.a = pw.a = ws + (p & 1 ? s.g : s.g2), px.a_ld = pw.a_ld = s.piece, px.rows = pw.rows = c.rows;
+      px.b = (const char*)w + v0 * w_ld * ES, px.b_ld = w_ld, px.n = px.b_cols = s.padded, px.k = v1 - v0;
+      px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = c.tokens, px.add = p > 1;
+      pw.b = ws + s.x, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
+      pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / OP::LIFT, pw.scale = scale;
+      if (pw.splits == 1) pw.out = out, pw.out_ld = c.width, pw.out_t = c.w_t;
+      else pw.sums = (float*)(ws + s.dw), pw.n_ld = s.padded, pw.m_rows = s.piece;
     }
+    const LogitsCall* pg = p < s.pieces ? &g : nullptr;
+    const ProductCall *x = p > 0 && c.dx ? &px : nullptr, *y = p > 0 && c.dw ? &pw : nullptr;
+    if (s.large_pass) launch_pass<OP, typename F::Large, typename F::LargeX, typename F::LargeW>(pg, x, y, c.tokens, c.st);
+    else launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st);
+    if (y && pw.splits > 1)
+      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, scale, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t, c.st);
   }
   if (c.dx)
     launch_finish((float*)(ws + s.dx), s.splits_x, c.tokens * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, scale,
