@@ -68,69 +68,109 @@ def _ptr(t: Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+# (A short step's host work is of the size of its kernels', half of it on autograd's own thread: the implementations below allocate
+# what they return and nothing else, None in the place of what is not asked for, and read each attribute once. The custom ops, which
+# can return tensors only, put empty ones there.)
+
+def _empty(like: Tensor, dtype: torch.dtype) -> Tensor:
+    """A contiguous tensor of like's shape and device."""
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+def _filled(*results: Tensor | None, like: Tensor) -> tuple[Tensor, ...]:
+    return tuple(like.new_empty(0) if r is None else r for r in results)
+
+
+def _mode_plain(plain: bool, *tensors: Tensor | None) -> bool:
+    """_plain in a backward pass, of the gradients that arrive: what was saved was looked at in the forward pass."""
+    return plain and _plain(*[t for t in tensors if t is not None])
+
+
+def _sized(device: torch.device, query, *args) -> int:
+    """A workspace size that depends on the device's compute units."""
+    if device.index == torch._C._cuda_getDevice():
+        return query(*args)
+    with torch.cuda.device(device):
+        return query(*args)
+
+
 # -- layer norm -------------------------------------------------------------------------------------------
 
-def _norm_impl(x: Tensor, branch: Optional[Tensor], weight: Tensor, bias: Optional[Tensor], eps: float, dtype: int,
-               stats: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """sa_layer_norm: y, the sum (empty without a branch), and the rows' mean and rstd (2, rows), empty without `stats`."""
-    width, device = weight.shape[0], x.device
+def _norm_impl(x: Tensor, branch: Optional[Tensor], weight: Tensor, bias: Optional[Tensor], eps: float, dtype: int, stats: bool):
+    """sa_layer_norm: y, the sum (None without a branch), and the rows' mean and rstd (2, rows), None without `stats`."""
+    width, device, code = weight.shape[0], x.device, _CODES[x.dtype]
     rows = x.numel() // width
-    y = torch.empty(x.shape, device=device, dtype=_TYPES[dtype])
-    total = torch.empty(x.shape if branch is not None else (0,), device=device, dtype=x.dtype)
-    held = torch.empty(2, rows if stats else 0, device=device, dtype=torch.float32)
+    y = _empty(x, _TYPES[dtype])
+    total = None if branch is None else _empty(x, x.dtype)
+    held = torch.empty(2, rows, device=device, dtype=torch.float32) if stats else None
     if rows == 0:
         return y, total, held
     x, x_ld = _rows(x, width)
-    branch_ld = 0
+    branch_ld = branch_code = 0
     if branch is not None:
         branch, branch_ld = _rows(branch, width)
+        branch_code = _CODES[branch.dtype]
     weight = _vector(weight)
-    bias = None if bias is None else _vector(bias)
+    if bias is not None:
+        bias = _vector(bias)
+    mean = None if held is None else held.data_ptr()
     _call(device, _lib.load().sa_layer_norm, x.data_ptr(), x_ld, _ptr(branch), branch_ld, weight.data_ptr(), _ptr(bias),
-          y.data_ptr(), _ptr(total) if branch is not None else None, held.data_ptr() if stats else None,
-          held.data_ptr() + 4 * rows if stats else None, rows, width, eps, _CODES[x.dtype], 0 if branch is None else _CODES[branch.dtype], dtype,
+          y.data_ptr(), _ptr(total), mean, None if mean is None else mean + 4 * rows, rows, width, eps, code, branch_code, dtype,
           _CODES[weight.dtype])
     return y, total, held
 
 
-_norm_op = _custom_op("layer_norm_forward", _norm_impl)
+def _norm_dense(x: Tensor, branch: Optional[Tensor], weight: Tensor, bias: Optional[Tensor], eps: float, dtype: int,
+                stats: bool) -> tuple[Tensor, Tensor, Tensor]:
+    y, total, held = _norm_impl(x, branch, weight, bias, eps, dtype, stats)
+    return (y, *_filled(total, like=x), *_filled(held, like=x.new_empty(0, dtype=torch.float32)))
+
+
+_norm_op = _custom_op("layer_norm_forward", _norm_dense)
 
 
 @_norm_op.register_fake
 def _norm_fake(x, branch, weight, bias, eps, dtype, stats):
-    rows = x.numel() // weight.shape[0] if stats else 0
     return (x.new_empty(x.shape, dtype=_TYPES[dtype]), x.new_empty(x.shape if branch is not None else (0,)),
-            x.new_empty((2, rows), dtype=torch.float32))
+            x.new_empty((2, x.numel() // weight.shape[0]) if stats else (0,), dtype=torch.float32))
 
 
 def _norm_backward_impl(s: Tensor, dy: Tensor, ds: Optional[Tensor], weight: Tensor, stats: Tensor, branch_dtype: int,
-                        need_x: bool, need_weight: bool, need_bias: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-    """sa_layer_norm_backward: dx, the branch's gradient (empty where it is of dx's type, whose values it has: branch_dtype is then -1),
-    dweight and dbias (empty where not needed)."""
-    width, device = weight.shape[0], s.device
+                        need_x: bool, need_weight: bool, need_bias: bool):
+    """sa_layer_norm_backward: dx, the branch's gradient (None where it is of dx's type, whose values it has: branch_dtype is then -1),
+    dweight and dbias (None where not needed)."""
+    width, device, code = weight.shape[0], s.device, _CODES[s.dtype]
     rows = s.numel() // width
     lib = _lib.load()
-    dx = torch.empty(s.shape if need_x else (0,), device=device, dtype=s.dtype)
-    other = branch_dtype >= 0
-    dbranch = torch.empty(s.shape if other else (0,), device=device, dtype=_TYPES[branch_dtype] if other else s.dtype)
-    dweight, dbias = (torch.empty(width if n else 0, device=device, dtype=weight.dtype) for n in (need_weight, need_bias))
+    dx = _empty(s, s.dtype) if need_x else None
+    dbranch = _empty(s, _TYPES[branch_dtype]) if branch_dtype >= 0 else None
+    weight = _vector(weight)
+    dweight = torch.empty_like(weight) if need_weight else None
+    dbias = torch.empty_like(weight) if need_bias else None
     s, s_ld = _rows(s, width)
     dy, dy_ld = _rows(dy, width)
-    ds_ld = 0
+    ds_ld = size = 0
     if ds is not None:
         ds, ds_ld = _rows(ds, width)
-    weight = _vector(weight)
-    sums = need_weight or need_bias
-    size = lib.sa_layer_norm_backward_workspace_bytes(rows, width) if sums else 0
-    ws = torch.empty(size, device=device, dtype=torch.uint8)
-    _call(device, lib.sa_layer_norm_backward, s.data_ptr(), s_ld, dy.data_ptr(), dy_ld, _ptr(ds), ds_ld, weight.data_ptr(),
-          stats.data_ptr(), stats.data_ptr() + 4 * rows, dx.data_ptr() if need_x else None, dbranch.data_ptr() if other else None,
-          dweight.data_ptr() if need_weight else None, dbias.data_ptr() if need_bias else None, ws.data_ptr() if sums else None, size,
-          rows, width, _CODES[s.dtype], branch_dtype if other else 0, _CODES[dy.dtype], _CODES[weight.dtype])
+    ws = None
+    if need_weight or need_bias:
+        size = lib.sa_layer_norm_backward_workspace_bytes(rows, width)
+        ws = torch.empty(size, device=device, dtype=torch.uint8)
+    mean = stats.data_ptr()
+    _call(device, lib.sa_layer_norm_backward, s.data_ptr(), s_ld, dy.data_ptr(), dy_ld, _ptr(ds), ds_ld, weight.data_ptr(), mean,
+          mean + 4 * rows, _ptr(dx), _ptr(dbranch), _ptr(dweight), _ptr(dbias), _ptr(ws), size, rows, width, code, max(branch_dtype, 0),
+          _CODES[dy.dtype], _CODES[weight.dtype])
     return dx, dbranch, dweight, dbias
 
 
-_norm_backward_op = _custom_op("layer_norm_backward", _norm_backward_impl)
+def _norm_backward_dense(s: Tensor, dy: Tensor, ds: Optional[Tensor], weight: Tensor, stats: Tensor, branch_dtype: int,
+                         need_x: bool, need_weight: bool, need_bias: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    dx, dbranch, dweight, dbias = _norm_backward_impl(s, dy, ds, weight, stats, branch_dtype, need_x, need_weight, need_bias)
+    other = s if branch_dtype < 0 else s.new_empty(0, dtype=_TYPES[branch_dtype])
+    return (*_filled(dx, like=s), *_filled(dbranch, like=other), *_filled(dweight, dbias, like=weight))
+
+
+_norm_backward_op = _custom_op("layer_norm_backward", _norm_backward_dense)
 
 
 @_norm_backward_op.register_fake
@@ -146,27 +186,30 @@ class _LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, branch, weight, bias, eps, dtype):
-        given = [t for t in (x, branch, weight, bias) if t is not None]
-        forward = _norm_impl if _plain(*given) else _norm_op
-        y, total, stats = forward(x, branch, weight, bias, eps, _CODES[dtype], True)
-        ctx.save_for_backward(x if branch is None else total, weight, stats)
-        ctx.branch_dtype = None if branch is None else branch.dtype
+        ctx.plain = plain = _plain(*[t for t in (x, branch, weight, bias) if t is not None])
+        y, total, stats = (_norm_impl if plain else _norm_op)(x, branch, weight, bias, eps, _CODES[dtype], True)
         ctx.set_materialize_grads(False)
-        return y if branch is None else (y, total)
+        if branch is None:
+            ctx.save_for_backward(x, weight, stats)
+            ctx.branch_dtype = None
+            return y
+        ctx.save_for_backward(total, weight, stats)
+        ctx.branch_dtype = branch.dtype
+        return y, total
 
     @staticmethod
     def backward(ctx, dy, ds=None):
         s, weight, stats = ctx.saved_tensors
-        need_x, need_branch, need_weight, need_bias = ctx.needs_input_grad[:4]
+        need_x, need_branch, need_weight, need_bias, _, _ = ctx.needs_input_grad
         if dy is None:   # (only the sum was used)
             if ds is None:
                 return (None,) * 6
             dy = torch.zeros_like(s)
         other = need_branch and ctx.branch_dtype != s.dtype
-        given = [t for t in (s, dy, ds, weight, stats) if t is not None]
-        backward = _norm_backward_impl if _plain(*given) else _norm_backward_op
-        dx, dbranch, dweight, dbias = backward(s, dy, ds, weight, stats, _CODES[ctx.branch_dtype] if other else -1,
-                                               need_x or (need_branch and not other), need_weight, need_bias)
+        plain = _mode_plain(ctx.plain, dy, ds)
+        dx, dbranch, dweight, dbias = (_norm_backward_impl if plain else _norm_backward_op)(
+            s, dy, ds, weight, stats, _CODES[ctx.branch_dtype] if other else -1, need_x or (need_branch and not other), need_weight,
+            need_bias)
         return (dx if need_x else None, (dbranch if other else dx) if need_branch else None, dweight if need_weight else None,
                 dbias if need_bias else None, None, None)
 
@@ -199,8 +242,8 @@ def _norm(x, branch, weight, bias, eps, dtype):
     eps, dtype = _check_norm(x, branch, weight, bias, eps, dtype)
     if _wants_grad(x, branch, weight, bias):
         return _LayerNormFn.apply(x, branch, weight, bias, eps, dtype)
-    given = [t for t in (x, branch, weight, bias) if t is not None]
-    y, total, _ = (_norm_impl if _plain(*given) else _norm_op)(x, branch, weight, bias, eps, _CODES[dtype], False)
+    plain = _plain(*[t for t in (x, branch, weight, bias) if t is not None])
+    y, total, _ = (_norm_impl if plain else _norm_op)(x, branch, weight, bias, eps, _CODES[dtype], False)
     return y if branch is None else (y, total)
 
 
@@ -226,12 +269,13 @@ def add_layer_norm(x: Tensor, branch: Tensor, weight: Tensor, bias: Tensor | Non
 def _embedding_impl(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
     """sa_embedding: (*ids.shape, C)."""
     vocab, width = weight.shape
-    out = torch.empty(*ids.shape, width, device=weight.device, dtype=weight.dtype)
-    if ids.numel() == 0:
+    out = weight.new_empty((*ids.shape, width))
+    tokens = ids.numel()
+    if tokens == 0:
         return out
     ids = ids.contiguous()
     weight, ld = _rows(weight, width)
-    _call(weight.device, _lib.load().sa_embedding, ids.data_ptr(), ids.element_size(), weight.data_ptr(), ld, out.data_ptr(), ids.numel(),
+    _call(weight.device, _lib.load().sa_embedding, ids.data_ptr(), ids.element_size(), weight.data_ptr(), ld, out.data_ptr(), tokens,
           vocab, width, scale, _CODES[weight.dtype])
     return out
 
@@ -248,7 +292,7 @@ def _embedding_backward_impl(ids: Tensor, dout: Tensor, vocab: int, scale: float
     """sa_embedding_backward: (vocab, C) in dout's dtype."""
     width, tokens = dout.shape[-1], ids.numel()
     lib = _lib.load()
-    dweight = torch.empty(vocab, width, device=dout.device, dtype=dout.dtype)
+    dweight = dout.new_empty((vocab, width))
     ids = ids.contiguous()
     dout, ld = _rows(dout, width)
     size = lib.sa_embedding_backward_workspace_bytes(tokens, vocab, width)
@@ -271,12 +315,13 @@ class _EmbeddingFn(torch.autograd.Function):
     def forward(ctx, ids, weight, scale):
         ctx.save_for_backward(ids)
         ctx.vocab, ctx.scale = weight.shape[0], scale
-        return (_embedding_impl if _plain(ids, weight) else _embedding_op)(ids, weight, scale)
+        ctx.plain = plain = _plain(ids, weight)
+        return (_embedding_impl if plain else _embedding_op)(ids, weight, scale)
 
     @staticmethod
     def backward(ctx, dout):
         ids, = ctx.saved_tensors
-        backward = _embedding_backward_impl if _plain(ids, dout) else _embedding_backward_op
+        backward = _embedding_backward_impl if _mode_plain(ctx.plain, dout) else _embedding_backward_op
         return None, backward(ids, dout, ctx.vocab, ctx.scale), None
 
 
@@ -301,9 +346,8 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0) -> Tensor:
 
 # -- the vocabulary loss ------------------------------------------------------------------------------------
 
-def _xent_impl(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reduction: int, code: int,
-               train: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """sa_linear_xent on x (N, C): the loss, and for the backward pass (`train`; else empty) lse (N,) and the kept tokens."""
+def _xent_impl(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reduction: int, code: int, train: bool):
+    """sa_linear_xent on x (N, C): the loss, and for the backward pass (`train`; else None) lse (N,) and the kept tokens."""
     tokens, width = x.shape
     vocab, device = weight.shape[0], x.device
     lib = _lib.load()
@@ -312,19 +356,24 @@ def _xent_impl(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reductio
     targets = targets.contiguous()
     none = reduction == _lib.REDUCTIONS["none"]
     loss = torch.empty((tokens,) if none else (), device=device, dtype=torch.float32)
-    lse = torch.empty(tokens if train else 0, device=device, dtype=torch.float32)
+    lse = torch.empty(tokens, device=device, dtype=torch.float32) if train else None
     rows = torch.empty(64 + 2 * tokens, device=device, dtype=torch.int32)
-    with torch.cuda.device(device):   # (the size depends on the device's compute units)
-        size = lib.sa_linear_xent_workspace_bytes(x.data_ptr(), x_ld, weight.data_ptr(), w_ld, tokens, vocab, width, reduction, train,
-                                                  _CODES[x.dtype], _CODES[weight.dtype], code)
+    x_code, w_code, x_ptr, w_ptr = _CODES[x.dtype], _CODES[weight.dtype], x.data_ptr(), weight.data_ptr()
+    size = _sized(device, lib.sa_linear_xent_workspace_bytes, x_ptr, x_ld, w_ptr, w_ld, tokens, vocab, width, reduction, train, x_code,
+                  w_code, code)
     ws = torch.empty(size, device=device, dtype=torch.uint8)
-    _call(device, lib.sa_linear_xent, x.data_ptr(), x_ld, weight.data_ptr(), w_ld, targets.data_ptr(), loss.data_ptr(),
-          lse.data_ptr() if train else None, rows.data_ptr(), ws.data_ptr(), size, tokens, vocab, width, ignore, reduction,
-          _CODES[x.dtype], _CODES[weight.dtype], code)
-    return loss, lse, rows if train else rows.new_empty(0)
+    _call(device, lib.sa_linear_xent, x_ptr, x_ld, w_ptr, w_ld, targets.data_ptr(), loss.data_ptr(), _ptr(lse), rows.data_ptr(),
+          ws.data_ptr(), size, tokens, vocab, width, ignore, reduction, x_code, w_code, code)
+    return loss, lse, rows if train else None
 
 
-_xent_op = _custom_op("linear_cross_entropy_forward", _xent_impl)
+def _xent_dense(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reduction: int, code: int,
+                train: bool) -> tuple[Tensor, Tensor, Tensor]:
+    loss, lse, rows = _xent_impl(x, weight, targets, ignore, reduction, code, train)
+    return (loss, *_filled(lse, like=loss), *_filled(rows, like=x.new_empty(0, dtype=torch.int32)))
+
+
+_xent_op = _custom_op("linear_cross_entropy_forward", _xent_dense)
 
 
 @_xent_op.register_fake
@@ -336,27 +385,31 @@ def _xent_fake(x, weight, targets, ignore, reduction, code, train):
 
 
 def _xent_backward_impl(x: Tensor, weight: Tensor, targets: Tensor, lse: Tensor, rows: Tensor, dloss: Tensor, reduction: int, code: int,
-                        need_x: bool, need_weight: bool) -> tuple[Tensor, Tensor]:
-    """sa_linear_xent_backward: dx and dweight in their tensors' types (empty where not needed)."""
+                        need_x: bool, need_weight: bool):
+    """sa_linear_xent_backward: dx and dweight in their tensors' types (None where not needed)."""
     tokens, width = x.shape
     vocab, device = weight.shape[0], x.device
     lib = _lib.load()
-    dx = torch.empty(x.shape if need_x else (0,), device=device, dtype=x.dtype)
-    dweight = torch.empty(weight.shape if need_weight else (0,), device=device, dtype=weight.dtype)
+    dx = _empty(x, x.dtype) if need_x else None
+    dweight = _empty(weight, weight.dtype) if need_weight else None
     x, x_ld = _rows(x, width)
     weight, w_ld = _rows(weight, width)
     targets, dloss = targets.contiguous(), _vector(dloss)
-    with torch.cuda.device(device):
-        size = lib.sa_linear_xent_backward_workspace_bytes(weight.data_ptr(), w_ld, tokens, vocab, width, need_x, need_weight,
-                                                           _CODES[weight.dtype], code)
+    w_code, w_ptr = _CODES[weight.dtype], weight.data_ptr()
+    size = _sized(device, lib.sa_linear_xent_backward_workspace_bytes, w_ptr, w_ld, tokens, vocab, width, need_x, need_weight, w_code, code)
     ws = torch.empty(size, device=device, dtype=torch.uint8)
-    _call(device, lib.sa_linear_xent_backward, x.data_ptr(), x_ld, weight.data_ptr(), w_ld, targets.data_ptr(), lse.data_ptr(),
-          rows.data_ptr(), dloss.data_ptr(), dx.data_ptr() if need_x else None, dweight.data_ptr() if need_weight else None,
-          ws.data_ptr(), size, tokens, vocab, width, reduction, _CODES[x.dtype], _CODES[weight.dtype], code)
+    _call(device, lib.sa_linear_xent_backward, x.data_ptr(), x_ld, w_ptr, w_ld, targets.data_ptr(), lse.data_ptr(), rows.data_ptr(),
+          dloss.data_ptr(), _ptr(dx), _ptr(dweight), ws.data_ptr(), size, tokens, vocab, width, reduction, _CODES[x.dtype], w_code, code)
     return dx, dweight
 
 
-_xent_backward_op = _custom_op("linear_cross_entropy_backward", _xent_backward_impl)
+def _xent_backward_dense(x: Tensor, weight: Tensor, targets: Tensor, lse: Tensor, rows: Tensor, dloss: Tensor, reduction: int, code: int,
+                         need_x: bool, need_weight: bool) -> tuple[Tensor, Tensor]:
+    dx, dweight = _xent_backward_impl(x, weight, targets, lse, rows, dloss, reduction, code, need_x, need_weight)
+    return (*_filled(dx, like=x), *_filled(dweight, like=weight))
+
+
+_xent_backward_op = _custom_op("linear_cross_entropy_backward", _xent_backward_dense)
 
 
 @_xent_backward_op.register_fake
@@ -369,7 +422,8 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, targets, ignore, reduction, code):
-        loss, lse, rows = (_xent_impl if _plain(x, weight, targets) else _xent_op)(x, weight, targets, ignore, reduction, code, True)
+        ctx.plain = plain = _plain(x, weight, targets)
+        loss, lse, rows = (_xent_impl if plain else _xent_op)(x, weight, targets, ignore, reduction, code, True)
         ctx.save_for_backward(x, weight, targets, lse, rows)
         ctx.reduction, ctx.code = reduction, code
         return loss
@@ -378,7 +432,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
     def backward(ctx, dloss):
         x, weight, targets, lse, rows = ctx.saved_tensors
         need_x, need_weight = ctx.needs_input_grad[:2]
-        backward = _xent_backward_impl if _plain(x, weight, targets, lse, rows, dloss) else _xent_backward_op
+        backward = _xent_backward_impl if _mode_plain(ctx.plain, dloss) else _xent_backward_op
         dx, dweight = backward(x, weight, targets, lse, rows, dloss, ctx.reduction, ctx.code, need_x, need_weight)
         return dx if need_x else None, dweight if need_weight else None, None, None, None, None
 
