@@ -517,19 +517,22 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
   logits_tile<OP, L, false>(c, blockIdx.x, s0, s1, s2, s3);
 }
 
-// A token's statistics over the mt tiles joined: 8 lanes a token. lse (base 2), the loss, and the workgroup's sum of losses.
+// A token's statistics over the mt tiles joined: `TOKENS` tokens a workgroup, NTHREADS / TOKENS lanes each. lse (base 2), the loss, and the
+// workgroup's sum of losses. (32 tokens where there are many, four where a few tokens' 400 tiles are all there is to
+// read: 8 tokens of 50304 words 8.1 us with 8 lanes each, 4.7 with 64.)
+template <int TOKENS>
 __global__ __launch_bounds__(NTHREADS) void xent_join_kernel(LogitsCall c, float* lse, float* each, float* sums, int64_t ignore) {
-  __shared__ float part[NTHREADS / 32];
-  __shared__ float tm[8][33], ts[8][33];
+  constexpr int LANES = NTHREADS / TOKENS;
+  __shared__ float tm[LANES][TOKENS + 1], ts[LANES][TOKENS + 1], out[TOKENS];
   const int64_t tokens = c.rows ? c.rows[0] : c.tokens;
-  const int x = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int x = threadIdx.x % TOKENS, k = threadIdx.x / TOKENS;
   float total = 0.f;
-  for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < tokens; i0 += (int64_t)gridDim.x * 32) {
+  for (int64_t i0 = (int64_t)blockIdx.x * TOKENS; i0 < tokens; i0 += (int64_t)gridDim.x * TOKENS) {
     const int64_t i = i0 + x;
     float mx = -INFINITY, s = 0.f;
     if (i < tokens) {
-#pragma unroll 4
-      for (int m = k; m < c.mt; m += 8) {
+#pragma unroll 8
+      for (int m = k; m < c.mt; m += LANES) {
         const float a = c.top[m * c.tokens + i], b = c.sum[m * c.tokens + i];
         const float up = fmaxf(mx, a), ref = up == -INFINITY ? 0.f : up;
         s = s * __builtin_amdgcn_exp2f((mx - ref) * LOG2E) + b * __builtin_amdgcn_exp2f((a - ref) * LOG2E);
@@ -540,19 +543,16 @@ __global__ __launch_bounds__(NTHREADS) void xent_join_kernel(LogitsCall c, float
     tm[k][x] = mx, ts[k][x] = s;
     __syncthreads();
     if (k == 0 && i < tokens) {
-#pragma unroll
-      for (int w = 1; w < 8; ++w) mx = fmaxf(mx, tm[w][x]);
+      for (int w = 1; w < LANES; ++w) mx = fmaxf(mx, tm[w][x]);
       const float ref = mx == -INFINITY ? 0.f : mx;
       s = 0.f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) s += ts[w][x] * __builtin_amdgcn_exp2f((tm[w][x] - ref) * LOG2E);
+      for (int w = 0; w < LANES; ++w) s += ts[w][x] * __builtin_amdgcn_exp2f((tm[w][x] - ref) * LOG2E);
       const int64_t token = c.rows ? c.rows[ROWS_HEAD + i] : i;
       const int64_t t = c.targets[token];
       // (a target outside the vocabulary has no logit: its loss and gradients become NaN)
       const bool real = t >= 0 && t < c.vocab;
       const float nan = __uint_as_float(0x7fc00000u);
-      const float ls = logf(s);
-      float loss = real ? (mx - c.at[i]) + ls : nan;
+      float loss = real ? (mx - c.at[i]) + logf(s) : nan;
       if (!c.rows && t == ignore) loss = 0.f;
       if (lse) lse[i] = real ? fmaf(mx, LOG2E, log2f(s)) : nan;
       if (each) each[token] = loss;
@@ -560,11 +560,12 @@ __global__ __launch_bounds__(NTHREADS) void xent_join_kernel(LogitsCall c, float
     }
   }
   if (!sums) return;
-#pragma unroll
-  for (int d = 16; d; d >>= 1) total += __shfl_xor(total, d);
-  if (x == 0) part[k] = total;   // (lanes of k > 0 hold zeros)
+  if (k == 0) out[x] = total;
   __syncthreads();
-  if (threadIdx.x == 0) sums[blockIdx.x] = part[0];
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < TOKENS; ++w) total += out[w];
+    sums[blockIdx.x] = total;
+  }
 }
 
 // The workgroups' sums added in a fixed order, over the tokens kept where a mean is asked for (none: 0 / 0, a NaN).
@@ -766,6 +767,7 @@ struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per st
 constexpr int64_t SMALL_TOKENS = 64;      // one tile's tokens of the smallest kernel
 constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of a piece's G, of which there are two at a time
+constexpr int64_t JOIN_FEW = 1024;        // tokens up to which the join takes 64 lanes for each
 constexpr int64_t MAX_LD_BYTES = 1 << 22;             // 256 rows within a buffer resource's 2 GiB
 
 // What a call does, from its sizes alone.
@@ -773,7 +775,7 @@ template <class OP>
 struct XentShape {
   static constexpr int ES = sizeof(typename OP::elem), BK = KB / ES;
   bool train, small, large, gather, copy_w;
-  int64_t padded, bm, mt, join_blocks;
+  int64_t padded, bm, mt, join_tokens, join_blocks;
   // backward
   int64_t piece, pieces;
   bool large_pass;
@@ -793,7 +795,8 @@ struct XentShape {
     gather = train || c.reduction != SA_REDUCE_NONE || c.tokens > IN_PLACE_TOKENS || !x_ok;
     copy_w = !(c.w_t == OP::CODE && padded == c.width && (uintptr_t)c.w % 16 == 0 && c.w_ld * ES % 16 == 0 &&
                c.w_ld >= c.width && c.w_ld * ES < MAX_LD_BYTES);
-    join_blocks = std::min<int64_t>(cdiv(c.tokens, 32), 4096);
+    join_tokens = c.tokens <= JOIN_FEW ? 4 : 32;
+    join_blocks = std::min<int64_t>(cdiv(c.tokens, join_tokens), 4096);
     int64_t p = 0;
     const auto take = [&p](int64_t bytes) {
       const int64_t at = p;
@@ -921,7 +924,9 @@ int xent_forward(const XentCall& c) {
   else launch_logits<OP, typename F::Middle>(lc, c.tokens, c.st);
   lc.mt = (int)s.mt;
   float* sums = each ? nullptr : (float*)(ws + s.sums);
-  hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)s.join_blocks), dim3(NTHREADS), 0, c.st, lc, c.lse, each, sums, c.ignore);
+  const dim3 joins((unsigned)s.join_blocks);
+  if (s.join_tokens == 4) hipLaunchKernelGGL((xent_join_kernel<4>), joins, dim3(NTHREADS), 0, c.st, lc, c.lse, each, sums, c.ignore);
+  else hipLaunchKernelGGL((xent_join_kernel<32>), joins, dim3(NTHREADS), 0, c.st, lc, c.lse, each, sums, c.ignore);
   if (sums)
     hipLaunchKernelGGL(xent_sum_kernel, dim3(1), dim3(1024), 0, c.st, sums, (int)s.join_blocks,
                        c.reduction == SA_REDUCE_MEAN ? c.rows : nullptr, c.loss);
