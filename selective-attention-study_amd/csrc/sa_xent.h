@@ -17,13 +17,17 @@
 //   xent_finish_x, _w        scale, add the parts of a split contraction, convert
 //
 // All products run through one tile loop on matrix instructions with fp32 accumulation (Mainloop). Statistics, lse and losses are
-// fp32. G is rounded to the products' type: half a step of it (bf16 2^-9 to 2^-8 of each entry), the size of the gradients' own
-// rounding; fp16 holds G at 2^14 times its size, as a vocabulary's probabilities lie below that type's normal range. The factor
-// and a common g are applied to the fp32 sums; tokens' own g_i (reduction none) to G before it is rounded.
+// fp32. G is rounded to 11 bits: it is held in fp16 at 2^14 times its size (a vocabulary's probabilities lie below that type's normal
+// range), for bf16 operands too, which the backward pass holds in fp16 times the power of two that brings their largest to
+// 2^14: exactly, but for numbers 2^32 times smaller than that, and at the same rate. (With G in bf16 the gradients' error was 1.4 to
+// 1.6 times that of their own rounding; so it is that rounding alone.) The factors and a common g are applied to the
+// fp32 sums; tokens' own g_i (reduction none) to G before it is rounded.
 
 #pragma once
 
 #include <math.h>
+
+#include <type_traits>
 
 #include "sa_lm.h"
 
@@ -34,7 +38,8 @@ struct XentCall {
   const int64_t* targets;
   const float* dloss;
   float *loss, *lse;            // lse: per kept token, base 2; null where no backward pass follows
-  int* rows;                    // [0] kept tokens, [64 ..] their numbers, [64 + tokens ..] each token's place among them or -1
+  int* rows;                    // [0] kept tokens, [64 ..] largest magnitudes (MAXIMA of weight, of x), [ROWS_HEAD ..] the kept tokens'
+                                // numbers, [ROWS_HEAD + tokens ..] each token's place among them or -1
   void *dx, *dw;
   void* ws;
   int64_t x_ld, w_ld, tokens, vocab, width, ignore;
@@ -61,23 +66,27 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_void_ptr;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int ROWS_HEAD = 64;   // ints before the kept tokens' numbers
+constexpr int MAXIMA = 512;                    // workgroups that look for the largest magnitude of a matrix
+constexpr int ROWS_HEAD = 64 + 2 * MAXIMA;     // ints before the kept tokens' numbers
+static_assert(ROWS_HEAD == SA_XENT_ROWS, "as the header says");
 
 // ---------------------------------------------------------------------------------------------
 // Operand types. A lane's operand of one step is 16 bytes of its row (lanes 0-31 the even, 32-63 the odd 16 bytes): one instruction for
 // 16-bit types, four for fp32, each of which contracts element e of both halves' four (the order of a contraction is
 // free as long as both operands have the same).
 
+struct XF16;
 struct XBF16 {
   typedef uint16_t elem;
+  typedef XF16 Back;   // the backward pass's operands
   static constexpr int CODE = SA_DTYPE_BF16;
-  static constexpr float LIFT = 1.f;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 };
 struct XF16 {
   typedef uint16_t elem;
+  typedef XF16 Back;
   static constexpr int CODE = SA_DTYPE_F16;
   static constexpr float LIFT = 16384.f;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
@@ -86,6 +95,7 @@ struct XF16 {
 };
 struct XF32 {
   typedef float elem;
+  typedef XF32 Back;
   static constexpr int CODE = SA_DTYPE_F32;
   static constexpr float LIFT = 1.f;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
@@ -302,11 +312,57 @@ __device__ __forceinline__ bool tile_of(int64_t id, int mt, int nt, int& m, int&
 inline int64_t tiles_grid(int64_t mt, int64_t nt) { return 8 * cdiv(mt * nt, 8); }
 
 // ---------------------------------------------------------------------------------------------
-// The kept tokens, in order. One workgroup: 8192 tokens a round.
+// The largest of the workgroup's values (NaN left out), as the workgroup's own number of `maxima`.
+__device__ __forceinline__ void put_maximum(float most, float (&acc)[16], int* maxima, int at) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  if ((threadIdx.x & 63) == 0) acc[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < (int)blockDim.x / 64; ++w) most = fmaxf(most, acc[w]);
+  maxima[at] = (int)__float_as_uint(most);
+}
 
-__global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets, int64_t tokens, int64_t ignore, int* rows, float* each) {
+// The kept tokens, in order: the first workgroup, 8192 tokens a round. The others (a backward pass of bf16 operands follows) look for the
+// largest magnitude of the weight meanwhile.
+
+struct Matrix {
+  const void* p;
+  int64_t ld, rows;
+  int width, dtype;
+};
+__global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets, int64_t tokens, int64_t ignore, int* rows, float* each,
+                                                         Matrix w) {
   __shared__ int count[16];
+  __shared__ float acc[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (blockIdx.x > 0) {
+    const int per = (w.width + 3) / 4;
+    const int64_t n = w.rows * per;
+    const bool quads = (uintptr_t)w.p % (w.dtype == SA_DTYPE_F32 ? 16 : 8) == 0 && w.ld % 4 == 0 && w.width % 4 == 0;
+    float most = 0.f;
+    constexpr int AHEAD = 8;   // loads in flight
+    for (int64_t k0 = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; k0 < n; k0 += (int64_t)MAXIMA * 1024 * AHEAD) {
+      Quad q[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t k = k0 + (int64_t)u * MAXIMA * 1024, row = k / per;
+        const int e = (int)(k - row * per) * 4;
+        const void* at = row_of(w.p, row, w.ld, w.dtype);
+        q[u] = quads ? fetch<true>(at, w.dtype, e, 1, k < n ? w.width : 0) : fetch<false>(at, w.dtype, e, 1, k < n ? w.width : 0);
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        float x[4];
+        if (quads) numbers<true>(q[u], w.dtype, x);
+        else numbers<false>(q[u], w.dtype, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[j]));
+      }
+    }
+    put_maximum(most, acc, rows + 64, blockIdx.x - 1);
+    return;
+  }
   int base = 0;
   for (int64_t i0 = 0; i0 < tokens; i0 += 8192) {
     bool kept[8];
@@ -342,15 +398,19 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets,
   if (threadIdx.x == 0) rows[0] = base;
 }
 
-// Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i], times factor[i] where given.
-template <class OP>
+// Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i]; FIRST: rounded to bf16 first and
+// taken *unit times. maxima: each workgroup's largest magnitude (MAXIMA workgroups then).
+template <class OP, bool FIRST>
 __global__ __launch_bounds__(NTHREADS) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
-                                                               const int* count, int64_t most, const float* factor,
+                                                               const int* count, int64_t most, const float* unit, int* maxima,
                                                                typename OP::elem* to, int padded) {
+  __shared__ float acc[16];
   const int64_t rows = count ? *count : most;
   const int per = padded / 4;
   const bool quads = ((uintptr_t)from % (dtype == SA_DTYPE_F32 ? 16 : 8)) == 0 && ld % 4 == 0;
   const int64_t n = rows * per;
+  const float by = FIRST ? *unit : 1.f;
+  float top = 0.f;
   for (int64_t k = (int64_t)blockIdx.x * NTHREADS + threadIdx.x; k < n; k += (int64_t)gridDim.x * NTHREADS) {
     const int64_t i = k / per;
     const int e = (int)(k - i * per) * 4;
@@ -358,17 +418,23 @@ __global__ __launch_bounds__(NTHREADS) void xent_gather_kernel(const void* from,
     float x[4];
     if (quads && e + 4 <= width) numbers<true>(fetch<true>(row, dtype, e, 1, width), dtype, x);
     else numbers<false>(fetch<false>(row, dtype, e, 1, width), dtype, x);
-    if (factor) {
-      const float f = factor[i];
+    if constexpr (FIRST) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] *= f;
+      for (int j = 0; j < 4; ++j) x[j] = stored(x[j], SA_DTYPE_BF16) * by;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[j]));
     put<true>(to + i * padded, OP::CODE, e, 1, padded, x);
   }
+  if (maxima) put_maximum(top, acc, maxima, blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------------------------
 // Logits of a tile: rows of the vocabulary (M) x tokens (N).
+
+struct Factors {   // xent_factors_kernel
+  float g, w, x, from_w, from_x;
+};
 
 struct LogitsCall {
   const void *w, *x;
@@ -382,6 +448,7 @@ struct LogitsCall {
   float *top, *sum, *at;    // (mt, tokens) statistics, the targets' logits
   const float* lse;         // backward: base 2
   const float* factor;      // backward: of each kept token's row of G; null: 1
+  const Factors* units;     // backward
   void* g;                  // (tokens, g_ld)
   int64_t g_ld;
 };
@@ -470,6 +537,8 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
     const int g_row = (int)(c.g_ld * ES);
     const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES);
     const int left = edge ? (int)(c.v1 - vw) : L::TM * 32;   // rows of the vocabulary
+    const Factors units = *c.units;
+    const float to_w = units.from_w * LOG2E, to_x = units.from_x;   // (one after the other: their product may leave fp32's range)
 #pragma unroll 1
     for (int b = 0; b < L::TN; ++b) {
       const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
@@ -490,7 +559,7 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
             float x = l.acc[a][0][4 * q + r];
 #pragma unroll
             for (int o = 1; o < L::TN; ++o) x = b == o ? l.acc[a][o][4 * q + r] : x;
-            x = __builtin_amdgcn_exp2f(fmaf(x, LOG2E, -lse));
+            x = __builtin_amdgcn_exp2f(fmaf(x * to_w, to_x, -lse));
             x = tl == row ? x - 1.f : x;
             x = row < left ? x : 0.f;
             p[r] = x * lift;
@@ -585,27 +654,56 @@ __global__ __launch_bounds__(1024) void xent_sum_kernel(const float* sums, int n
 }
 
 // ---------------------------------------------------------------------------------------------
-// The backward pass's factors: scale[0] multiplies the sums of both products; factor[i] (reduction none) the kept token's row of G
-// before it is rounded, g_i / scale[0], with scale[0] the power of two at or below the largest |g|. So a row is rounded once, as
-// with one g for all; in fp16 the entries of rows whose g is less than 2^-10 of the largest lose their last bits.
-__global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, const int* rows, int reduction, float* scale, float* factor) {
-  __shared__ float acc[16];
+// The backward pass's factors. w and x: the units weight and x are held in, powers of two, from_w and from_x back from them; g multiplies the sums of
+// both products. factor[i] (reduction none): of the kept token's row of G before it is rounded, g_i relative to the power of two at or below the
+// largest |g|, which g then is. So a row is rounded once, as with one g for all; the entries of rows whose g is less
+// than 2^-10 of the largest lose their last bits.
+__device__ __forceinline__ uint32_t exponent_of(float x) { return (__float_as_uint(x) >> 23) & 0xff; }
+__global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, const int* rows, int reduction, bool scaled, Factors* out,
+                                                            float* factor) {
+  __shared__ float acc[16], maxima[2];
   const int tokens = rows[0];
-  if (!factor) {   // (no token kept: gradients of zeros, not 0 / 0)
-    if (threadIdx.x == 0) scale[0] = tokens == 0 ? 0.f : reduction == SA_REDUCE_MEAN ? dloss[0] / (float)tokens : dloss[0];
-    return;
-  }
-  float most = 0.f;
-  for (int i = threadIdx.x; i < tokens; i += 1024) most = fmaxf(most, fabsf(dloss[rows[ROWS_HEAD + i]]));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (scaled) {
+    float most = __uint_as_float((uint32_t)rows[64 + threadIdx.x]);   // half of the threads of either matrix
 #pragma unroll
-  for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  if ((threadIdx.x & 63) == 0) acc[threadIdx.x >> 6] = most;
-  __syncthreads();
-  for (int w = 0; w < 16; ++w) most = fmaxf(most, acc[w]);
-  const uint32_t e = min(max((__float_as_uint(most) >> 23) & 0xff, 1u), 253u);
-  const float unit = __uint_as_float(e << 23);
-  if (threadIdx.x == 0) scale[0] = unit;
-  for (int i = threadIdx.x; i < tokens; i += 1024) factor[i] = dloss[rows[ROWS_HEAD + i]] / unit;
+    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if (lane == 0) acc[wave] = most;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      most = 0.f;
+      for (int w = 0; w < 8; ++w) most = fmaxf(most, acc[threadIdx.x * 8 + w]);
+      maxima[threadIdx.x] = most;
+    }
+    __syncthreads();
+  }
+  static_assert(MAXIMA == 512, "half of the threads");
+  float g;
+  if (!factor) {   // (no token kept: gradients of zeros, not 0 / 0)
+    g = tokens == 0 ? 0.f : reduction == SA_REDUCE_MEAN ? dloss[0] / (float)tokens : dloss[0];
+  } else {
+    float most = 0.f;
+    for (int i = threadIdx.x; i < tokens; i += 1024) most = fmaxf(most, fabsf(dloss[rows[ROWS_HEAD + i]]));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if (lane == 0) acc[wave] = most;
+    __syncthreads();
+    for (int w = 0; w < 16; ++w) most = fmaxf(most, acc[w]);
+    g = __uint_as_float(min(max(exponent_of(most), 1u), 253u) << 23);
+    for (int i = threadIdx.x; i < tokens; i += 1024) factor[i] = dloss[rows[ROWS_HEAD + i]] / g;
+  }
+  if (threadIdx.x) return;
+  Factors f{g, 1.f, 1.f, 1.f, 1.f};
+  if (scaled) {   // the largest comes to 2^14 .. 2^15; nothing but zeros stays as it is
+    const auto unit = [](float most, float& to, float& from) {
+      const int e = most == 0.f ? 0 : min(14 - ((int)exponent_of(most) - 127), 126);
+      to = __uint_as_float((uint32_t)(127 + e) << 23);
+      from = __uint_as_float((uint32_t)(127 - e) << 23);
+    };
+    unit(maxima[0], f.w, f.from_w);
+    unit(maxima[1], f.x, f.from_x);
+  }
+  *out = f;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -624,7 +722,7 @@ struct ProductCall {
   void* out;                // dW's rows, where nothing is split
   int64_t out_ld;
   int out_t;
-  const float* scale;
+  const Factors* units;
   float lift;
 };
 
@@ -656,7 +754,8 @@ __device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, i
   uint8_t* base = (uint8_t*)c.out + m0 * ld * es;
   if (!c.out) base = (uint8_t*)(c.sums + ((int64_t)part * c.m_rows + m0) * ld);
   const __amdgpu_buffer_rsrc_t rs = resource(base, min(M - m0, (int64_t)L::BM) * ld * es);
-  const float scale = c.out ? *c.scale * c.lift : 1.f;
+  // (the unit last and alone: with g it may leave fp32's range)
+  const float scale = c.out ? c.units->g * c.lift : 1.f, unit = c.out ? c.units->from_x : 1.f;
   const int row_bytes = (int)ld * es;
   const auto each = [&](auto&& put_sixteen) {
 #pragma unroll
@@ -671,7 +770,7 @@ __device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, i
     each([&](const f32x16& x, int at, int row) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        __builtin_amdgcn_raw_buffer_store_b16(to16(x[r] * scale, c.out_t), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
+        __builtin_amdgcn_raw_buffer_store_b16(to16(x[r] * scale * unit, c.out_t), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
     });
   } else if (c.add) {
     each([&](const f32x16& x, int at, int row) {
@@ -686,7 +785,7 @@ __device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, i
     each([&](const f32x16& x, int at, int row) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[r] * scale), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[r] * scale * unit), rs, at, (row + acc_row(r, 0)) * row_bytes, 0);
     });
   }
 }
@@ -716,7 +815,7 @@ __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass
 
 // dX: a token's parts added, times its factor; zero rows for the tokens that are ignored. dW: the parts of a piece's rows.
 __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums, int splits, int64_t split_stride, int64_t n_ld,
-                                                               const int* place, const float* scale, float lift,
+                                                               const int* place, const Factors* units, const float* unit, float lift,
                                                                void* out, int64_t rows, int width, int dtype) {
   const int64_t per = (width + 3) / 4;
   const int64_t n = rows * per;
@@ -731,9 +830,9 @@ __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums
         const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + at * n_ld + e);
         x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
       }
-      const float f = *scale * lift;
+      const float f = units->g * lift, u = *unit;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] *= f;
+      for (int j = 0; j < 4; ++j) x[j] = x[j] * f * u;
     }
     if (quads) put<true>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
     else put<false>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
@@ -783,7 +882,8 @@ struct XentShape {
   // workspace
   int64_t x, w, top, sum, at, sums, factors, g, g2, dx, dw, total;
 
-  XentShape(const XentCall& c, bool backward) {
+  // scaled: bf16 operands held in fp16, copies both
+  XentShape(const XentCall& c, bool backward, bool scaled = false) {
     train = c.lse != nullptr;
     padded = align_up(c.width, BK);
     small = c.tokens <= SMALL_TOKENS && !train;
@@ -793,7 +893,7 @@ struct XentShape {
     const bool x_ok = c.x_t == OP::CODE && padded == c.width && (uintptr_t)c.x % 16 == 0 && c.x_ld * ES % 16 == 0 &&
                       c.x_ld >= c.width && c.x_ld * ES < MAX_LD_BYTES;
     gather = train || c.reduction != SA_REDUCE_NONE || c.tokens > IN_PLACE_TOKENS || !x_ok;
-    copy_w = !(c.w_t == OP::CODE && padded == c.width && (uintptr_t)c.w % 16 == 0 && c.w_ld * ES % 16 == 0 &&
+    copy_w = scaled || !(c.w_t == OP::CODE && padded == c.width && (uintptr_t)c.w % 16 == 0 && c.w_ld * ES % 16 == 0 &&
                c.w_ld >= c.width && c.w_ld * ES < MAX_LD_BYTES);
     join_tokens = c.tokens <= JOIN_FEW ? 4 : 32;
     join_blocks = std::min<int64_t>(cdiv(c.tokens, join_tokens), 4096);
@@ -834,7 +934,7 @@ struct XentShape {
       splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
       splits_w = std::max(splits_w, (int)cdiv(c.tokens * x_row, (int64_t)1 << 30));
       splits_last = std::max(splits_last, splits_w);
-      factors = take((c.tokens + 16) * 4);
+      factors = take((c.tokens + 64) * 4);
       g = take(c.tokens * piece * ES);
       g2 = take(pieces > 1 ? c.tokens * piece * ES : 0);
       dx = take(c.dx ? splits_x * c.tokens * padded * 4 : 0);
@@ -878,18 +978,23 @@ void launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
   }
   hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
 }
-template <class OP>
+template <class OP, bool FIRST = false>
 void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows,
-                   const float* factor, void* to, int64_t padded, hipStream_t st) {
-  const int64_t blocks = std::min<int64_t>(cdiv(rows * (padded / 4), NTHREADS), 16384);
-  hipLaunchKernelGGL((xent_gather_kernel<OP>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, from, ld, dtype, (int)width, numbers_of,
-                     count, rows, factor, (typename OP::elem*)to, (int)padded);
+                   const float* unit, int* maxima, void* to, int64_t padded, hipStream_t st) {
+  const int64_t blocks = maxima ? MAXIMA : std::min<int64_t>(cdiv(rows * (padded / 4), NTHREADS), 16384);
+  hipLaunchKernelGGL((xent_gather_kernel<OP, FIRST>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, from, ld, dtype, (int)width, numbers_of,
+                     count, rows, unit, maxima, (typename OP::elem*)to, (int)padded);
 }
-inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const float* scale,
-                          float lift, void* out, int64_t rows, int64_t width, int dtype, hipStream_t st) {
+inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const Factors* units,
+                          const float* unit, float lift, void* out, int64_t rows, int64_t width, int dtype, hipStream_t st) {
   const int64_t blocks = std::min<int64_t>(cdiv(rows * cdiv(width, 4), NTHREADS), 16384);
-  hipLaunchKernelGGL(xent_finish_kernel, dim3((unsigned)blocks), dim3(NTHREADS), 0, st, sums, splits, split_stride, n_ld, place, scale,
-                     lift, out, rows, (int)width, dtype);
+  hipLaunchKernelGGL(xent_finish_kernel, dim3((unsigned)blocks), dim3(NTHREADS), 0, st, sums, splits, split_stride, n_ld, place, units,
+                     unit, lift, out, rows, (int)width, dtype);
+}
+
+template <class OP>
+int64_t xent_bytes(const XentCall& c, bool backward) {
+  return backward ? XentShape<typename OP::Back>(c, true, !std::is_same<OP, typename OP::Back>::value).total : XentShape<OP>(c, false).total;
 }
 
 template <class OP>
@@ -903,15 +1008,18 @@ int xent_forward(const XentCall& c) {
   lc.tokens = c.tokens;
   lc.vocab = c.vocab;
   if (s.gather) {
-    hipLaunchKernelGGL(xent_rows_kernel, dim3(1), dim3(1024), 0, c.st, c.targets, c.tokens, c.ignore, c.rows, each);
+    const bool maxima = s.train && !std::is_same<OP, typename OP::Back>::value;
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(maxima ? 1 + MAXIMA : 1), dim3(1024), 0, c.st, c.targets, c.tokens, c.ignore, c.rows, each,
+                       Matrix{c.w, c.w_ld, c.vocab, (int)c.width, c.w_t});
     lc.rows = c.rows;
-    launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, ws + s.x, s.padded, c.st);
+    launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, maxima ? c.rows + 64 + MAXIMA : nullptr,
+                      ws + s.x, s.padded, c.st);
     lc.x = ws + s.x, lc.x_ld = s.padded;
   } else {
     lc.x = c.x, lc.x_ld = c.x_ld;
   }
   if (s.copy_w) {
-    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, ws + s.w, s.padded, c.st);
+    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, nullptr, ws + s.w, s.padded, c.st);
     lc.w = ws + s.w, lc.w_ld = s.padded;
   } else {
     lc.w = c.w, lc.w_ld = c.w_ld;
@@ -933,20 +1041,22 @@ int xent_forward(const XentCall& c) {
   return launch_status();
 }
 
-template <class OP>
+template <class FROM>
 int xent_backward(const XentCall& c) {
+  typedef typename FROM::Back OP;
   typedef XentConfigs<OP> F;
   constexpr int ES = sizeof(typename OP::elem);
-  const XentShape<OP> s(c, true);
+  constexpr bool SCALED = !std::is_same<FROM, OP>::value;
+  const XentShape<OP> s(c, true, SCALED);
   char* ws = (char*)c.ws;
-  float* scale = (float*)(ws + s.factors);
-  float* factor = c.reduction == SA_REDUCE_NONE ? scale + 16 : nullptr;
-  hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, scale, factor);
-  launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, ws + s.x, s.padded, c.st);
+  Factors* units = (Factors*)(ws + s.factors);
+  float* factor = c.reduction == SA_REDUCE_NONE ? (float*)units + 64 : nullptr;
+  hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, SCALED, units, factor);
+  launch_gather<OP, SCALED>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, &units->x, nullptr, ws + s.x, s.padded, c.st);
   const void* w = c.w;
   int64_t w_ld = c.w_ld;
   if (s.copy_w) {
-    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, ws + s.w, s.padded, c.st);
+    launch_gather<OP, SCALED>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, &units->w, nullptr, ws + s.w, s.padded, c.st);
     w = ws + s.w, w_ld = s.padded;
   }
   // pass p: G of piece p, and the products of piece p - 1
@@ -955,7 +1065,7 @@ int xent_backward(const XentCall& c) {
     if (p < s.pieces) {
       g.w = w, g.w_ld = w_ld, g.x = ws + s.x, g.x_ld = s.padded, g.targets = c.targets, g.rows = c.rows, g.tokens = c.tokens;
       g.vocab = c.vocab, g.v0 = p * s.piece, g.v1 = std::min(g.v0 + s.piece, c.vocab), g.stages = (int)(s.padded / s.BK);
-      g.lse = c.lse, g.factor = factor, g.g = ws + (p & 1 ? s.g2 : s.g), g.g_ld = s.piece;
+      g.lse = c.lse, g.factor = factor, g.units = units, g.g = ws + (p & 1 ? s.g2 : s.g), g.g_ld = s.piece;
     }
     ProductCall px{}, pw{};
     const int64_t v0 = (p - 1) * s.piece, v1 = std::min(v0 + s.piece, c.vocab);
@@ -965,7 +1075,7 @@ int xent_backward(const XentCall& c) {
       px.b = (const char*)w + v0 * w_ld * ES, px.b_ld = w_ld, px.n = px.b_cols = s.padded, px.k = v1 - v0;
       px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = c.tokens, px.add = p > 1;
       pw.b = ws + s.x, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
-      pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / OP::LIFT, pw.scale = scale;
+      pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / OP::LIFT, pw.units = units;
       if (pw.splits == 1) pw.out = out, pw.out_ld = c.width, pw.out_t = c.w_t;
       else pw.sums = (float*)(ws + s.dw), pw.n_ld = s.padded, pw.m_rows = s.piece;
     }
@@ -974,10 +1084,10 @@ int xent_backward(const XentCall& c) {
     if (s.large_pass) launch_pass<OP, typename F::Large, typename F::LargeX, typename F::LargeW>(pg, x, y, c.tokens, c.st);
     else launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st);
     if (y && pw.splits > 1)
-      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, scale, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t, c.st);
+      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t, c.st);
   }
   if (c.dx)
-    launch_finish((float*)(ws + s.dx), s.splits_x, c.tokens * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, scale,
+    launch_finish((float*)(ws + s.dx), s.splits_x, c.tokens * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, units, &units->from_w,
                   1.f / OP::LIFT, c.dx, c.tokens, c.width, c.x_t, c.st);
   return launch_status();
 }

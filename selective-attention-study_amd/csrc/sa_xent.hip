@@ -16,7 +16,7 @@ bool on_elements(const void* p, int dtype) { return (uintptr_t)p % lm_elem_size(
 bool on_16(const void* p) { return (uintptr_t)p % 16 == 0; }
 bool xent_ld_ok(int64_t ld) { return ld >= 0 && ld < ((int64_t)1 << 40); }
 
-int64_t xent_bytes(const XentCall& c, int dtype, bool backward) {
+int64_t xent_space(const XentCall& c, int dtype, bool backward) {
   return dtype == SA_DTYPE_BF16 ? xent_bytes_bf16(c, backward) : dtype == SA_DTYPE_F16 ? xent_bytes_f16(c, backward) : xent_bytes_f32(c, backward);
 }
 int xent_run(const XentCall& c, int dtype, bool backward) {
@@ -34,7 +34,7 @@ int64_t sa_linear_xent_workspace_bytes(const void* x, int64_t x_ld, const void* 
   XentCall c{};
   c.x = x, c.x_ld = x_ld, c.w = weight, c.w_ld = weight_ld, c.tokens = tokens, c.vocab = vocab, c.width = width;
   c.reduction = reduction, c.x_t = x_dtype, c.w_t = weight_dtype, c.lse = train ? &lse : nullptr, c.cus = device_cus();
-  return xent_bytes(c, dtype, false);
+  return xent_space(c, dtype, false);
 }
 
 int sa_linear_xent(const void* x, int64_t x_ld, const void* weight, int64_t weight_ld, const int64_t* targets, float* loss, float* lse,
@@ -51,7 +51,7 @@ int sa_linear_xent(const void* x, int64_t x_ld, const void* weight, int64_t weig
   c.x = x, c.x_ld = x_ld, c.w = weight, c.w_ld = weight_ld, c.targets = targets, c.loss = loss, c.lse = lse, c.rows = rows;
   c.ws = workspace, c.tokens = tokens, c.vocab = vocab, c.width = width, c.ignore = ignore, c.reduction = reduction;
   c.x_t = x_dtype, c.w_t = weight_dtype, c.cus = device_cus(), c.st = static_cast<hipStream_t>(stream);
-  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < xent_bytes(c, dtype, false)) return SA_ERR_WORKSPACE;
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < xent_space(c, dtype, false)) return SA_ERR_WORKSPACE;
   return xent_run(c, dtype, false);
 }
 
@@ -62,7 +62,7 @@ int64_t sa_linear_xent_backward_workspace_bytes(const void* weight, int64_t weig
   XentCall c{};
   c.w = weight, c.w_ld = weight_ld, c.tokens = tokens, c.vocab = vocab, c.width = width, c.w_t = weight_dtype, c.x_t = dtype;
   c.dx = need_dx ? &some : nullptr, c.dw = need_dweight ? &some : nullptr, c.lse = (float*)&c, c.cus = device_cus();
-  return xent_bytes(c, dtype, true);
+  return xent_space(c, dtype, true);
 }
 
 int sa_linear_xent_backward(const void* x, int64_t x_ld, const void* weight, int64_t weight_ld, const int64_t* targets,
@@ -82,7 +82,7 @@ int sa_linear_xent_backward(const void* x, int64_t x_ld, const void* weight, int
   c.rows = const_cast<int32_t*>(rows), c.dloss = dloss, c.dx = dx, c.dw = dweight;
   c.ws = workspace, c.tokens = tokens, c.vocab = vocab, c.width = width, c.reduction = reduction;
   c.x_t = x_dtype, c.w_t = weight_dtype, c.cus = device_cus(), c.st = static_cast<hipStream_t>(stream);
-  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < xent_bytes(c, dtype, true)) return SA_ERR_WORKSPACE;
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < xent_space(c, dtype, true)) return SA_ERR_WORKSPACE;
   return xent_run(c, dtype, true);
 }
 

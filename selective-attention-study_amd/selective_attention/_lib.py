@@ -22,6 +22,7 @@ DTYPE_F16 = 2   # the entry points of the paged cache, the norms, the embedding 
 WIDE_WEIGHTS = 16   # sa_paged_attention: or'ed to the dtype
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}   # sa_linear_xent
+XENT_ROWS = 1088   # SA_XENT_ROWS
 
 # Kernel ids of sa_timing_read.
 KERNEL_FORWARD = 0

@@ -357,7 +357,7 @@ def _xent_impl(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reductio
     none = reduction == _lib.REDUCTIONS["none"]
     loss = torch.empty((tokens,) if none else (), device=device, dtype=torch.float32)
     lse = torch.empty(tokens, device=device, dtype=torch.float32) if train else None
-    rows = torch.empty(64 + 2 * tokens, device=device, dtype=torch.int32)
+    rows = torch.empty(_lib.XENT_ROWS + 2 * tokens, device=device, dtype=torch.int32)
     x_code, w_code, x_ptr, w_ptr = _CODES[x.dtype], _CODES[weight.dtype], x.data_ptr(), weight.data_ptr()
     size = _sized(device, lib.sa_linear_xent_workspace_bytes, x_ptr, x_ld, w_ptr, w_ld, tokens, vocab, width, reduction, train, x_code,
                   w_code, code)
@@ -381,7 +381,7 @@ def _xent_fake(x, weight, targets, ignore, reduction, code, train):
     f32 = dict(dtype=torch.float32)
     tokens = x.shape[0]
     return (x.new_empty((tokens,) if reduction == 0 else (), **f32), x.new_empty((tokens if train else 0,), **f32),
-            x.new_empty((64 + 2 * tokens if train else 0,), dtype=torch.int32))
+            x.new_empty((_lib.XENT_ROWS + 2 * tokens if train else 0,), dtype=torch.int32))
 
 
 def _xent_backward_impl(x: Tensor, weight: Tensor, targets: Tensor, lse: Tensor, rows: Tensor, dloss: Tensor, reduction: int, code: int,

@@ -290,8 +290,9 @@ def xent_check(x, w, t, reduction, operand, loss, dloss=None, dx=None, dw=None, 
 
     Logits: a sum of C products in fp32, off by at most dl = (C + 2) u sum|x w|. lse: dl, and u times the additions (128 rows of a tile in turn, 9
     more, then every eighth of the tiles and 8) plus 2^-22 of rounding in the exponentials and logarithm for arguments below 2^6.
-    G = (p - onehot) f is rounded to the operands' type, off by half a step and p (2 dl + dlse) before that (fp16: 2^-39 of the
-    factors' unit below its normal numbers); a gradient adds V (tokens) products of it in fp32."""
+    G = (p - onehot) f is rounded to fp16 at 2^14 times its size (fp32 operands: not at all), off by half a step of it, 2^-11, or 2^-39 of the
+    factors' unit below its normal numbers, and p (2 dl + dlse) before that; bf16 operands are held in fp16 with the largest at
+    2^14, the smallest off by 2^-39 of that. A gradient adds V (tokens) products in fp32."""
     x64, w64 = x.to(operand).double(), w.to(operand).double()
     kept = t != ignore
     x64, at = x64[kept], t[kept]
@@ -317,19 +318,24 @@ def xent_check(x, w, t, reduction, operand, loss, dloss=None, dx=None, dw=None, 
     G[torch.arange(len(at), device="cuda"), at] -= 1.0
     f = dloss.double().expand(t.shape[0])[kept] if reduction == "none" else dloss.double() / (len(at) if reduction == "mean" else 1) + 0 * at
     unit = f.abs().max() if len(at) else 0.0
-    e_G = (half(operand) + U) * G.abs() + p * (2 * dl + e_lse)[:, None] * 1.01 + 3 * U * p
-    e_G = e_G * f.abs()[:, None] + (2.0 ** -38 * unit if operand is F16 else 0.0)
+    fine, unit = (0.0, 0.0) if operand is F32 else (half(F16), unit)
+    e_G = (fine + U) * G.abs() + p * (2 * dl + e_lse)[:, None] * 1.01 + 3 * U * p
+    e_G = e_G * f.abs()[:, None] + 2.0 ** -38 * unit
+    low = 2.0 ** -38 if operand is BF16 else 0.0
     G = G * f[:, None]
     if dx is not None:
         want = torch.zeros(x.shape, dtype=F64, device="cuda")
         bound = torch.zeros_like(want)
         want[kept] = G @ w64
-        bound[kept] = (e_G + (w.shape[0] + 8) * U * G.abs()) @ w64.abs()
+        bound[kept] = (e_G + (w.shape[0] + 8) * U * G.abs()) @ w64.abs() + low * w64.abs().max() * G.abs().sum(1, keepdim=True)
         assert (dx[~kept] == 0).all()
         assert_within(dx, want, bound * 1.01 + rounding(want, x.dtype), "dx")
     if dw is not None:
         want = G.T @ x64
-        assert_within(dw, want, ((e_G + (len(at) + 8) * U * G.abs()).T @ x64.abs()) * 1.01 + rounding(want, w.dtype), "dw")
+        bound = (e_G + (len(at) + 8) * U * G.abs()).T @ x64.abs()
+        if len(at):
+            bound += low * x64.abs().max() * G.abs().sum(0)[:, None]
+        assert_within(dw, want, bound * 1.01 + rounding(want, w.dtype), "dw")
 
 
 def xent_run(x, w, t, reduction, dloss=None, need=(True, True), **kw):
@@ -464,6 +470,11 @@ def test_linear_cross_entropy_edges(cuda):
     each, _, dx, dw = xent_run(ill, w, t, "none")
     sound = torch.arange(40, device="cuda") != 4
     assert each[4].isnan() and each[sound].isfinite().all() and dx[4].isnan().all() and dx[sound].isfinite().all() and dw.isnan().all()
+    # operands far from 1, of any size that bf16 has: the products' units come back out
+    for xs, wscale in ((2.0 ** 60, 2.0 ** -60), (2.0 ** -100, 2.0 ** 95), (2.0 ** -20, 2.0 ** -110), (2.0 ** 30, 0.0)):
+        xb, wb = x * xs, w * wscale
+        loss, dloss, dx, dw = xent_run(xb, wb, t, "mean")
+        xent_check(xb, wb, t, "mean", BF16, loss, dloss, dx, dw)
     # factors of very different sizes, zero among them
     dloss = torch.tensor([1e4, 1.0, 1e-3, 0.0], device="cuda").repeat(10)
     for dt in (BF16, F16, F32):
