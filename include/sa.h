@@ -346,7 +346,7 @@ int sa_embedding_backward(const void* ids, int ids_bytes, const void* dout, int6
  * reduction: SA_REDUCE_NONE loss (tokens), _MEAN over the tokens that are not ignored (NaN if there is none), _SUM: loss (1). A target
  * outside [0, vocab) that is not `ignore` gives NaN. dtype: the type of the products' operands, to which x and weight are rounded where
  * theirs differs; products accumulate in fp32.
- * lse (tokens, fp32) and rows (SA_XENT_ROWS + 2 tokens ints) are what the backward pass takes (tokens not ignored, and their normalisers); lse
+ * lse (2 tokens, fp32) and rows (SA_XENT_ROWS + 2 tokens ints) are what the backward pass takes (which tokens are kept, their normalisers); lse
  * null: no backward pass follows (rows is scratch then). The workspace's size depends on the strides and alignment of x and weight, so its query takes the
  * same pointers (which it does not read).
  * Backward: dloss fp32, (tokens) or (1) by reduction; dx (tokens, width) of x's type, dweight (vocab, width) of weight's, 16-byte aligned;

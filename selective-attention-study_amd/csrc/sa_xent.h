@@ -37,7 +37,8 @@ struct XentCall {
   const void *x, *w;            // the caller's rows
   const int64_t* targets;
   const float* dloss;
-  float *loss, *lse;            // lse: per kept token, base 2; null where no backward pass follows
+  float *loss, *lse;            // lse: the kept tokens' largest logits, then (from tokens on) 1 / sum of exp beside those; null where no
+                                // backward pass follows
   int* rows;                    // [0] kept tokens, [64 ..] largest magnitudes (MAXIMA of weight, of x), [ROWS_HEAD ..] the kept tokens'
                                 // numbers, [ROWS_HEAD + tokens ..] each token's place among them or -1
   void *dx, *dw;
@@ -446,7 +447,7 @@ struct LogitsCall {
   int stages;               // of the contraction
   int mt, nt;
   float *top, *sum, *at;    // (mt, tokens) statistics, the targets' logits
-  const float* lse;         // backward: base 2
+  const float* lse;         // backward: XentCall's
   const float* factor;      // backward: of each kept token's row of G; null: 1
   const Factors* units;     // backward
   void* g;                  // (tokens, g_ld)
@@ -537,14 +538,14 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
     const int g_row = (int)(c.g_ld * ES);
     const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES);
     const int left = edge ? (int)(c.v1 - vw) : L::TM * 32;   // rows of the vocabulary
-    const Factors units = *c.units;
-    const float to_w = units.from_w * LOG2E, to_x = units.from_x;   // (one after the other: their product may leave fp32's range)
+    const Factors units = *c.units;   // (multiplied by one after the other: their product may leave fp32's range)
 #pragma unroll 1
     for (int b = 0; b < L::TN; ++b) {
       const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
       const bool real = i < tokens;
-      const float lse = real ? c.lse[i] : INFINITY;
-      const float lift = (c.factor && real ? c.factor[i] : 1.f) * OP::LIFT;
+      // (beside the largest logit, whose distance is exact where weights are large: log of the sum alone is off by 2^-21)
+      const float top = real ? c.lse[i] : 0.f;
+      const float lift = (c.factor && real ? c.factor[i] : 1.f) * OP::LIFT, over = real ? c.lse[c.tokens + i] * lift : 0.f;
       const int64_t t = real ? c.targets[c.rows[ROWS_HEAD + i]] - vw : -1;
       const int tl = t >= 0 && t < L::TM * 32 ? (int)t : -1;
       uint8_t* to = mine + (lane & 31) * RB;
@@ -559,10 +560,9 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
             float x = l.acc[a][0][4 * q + r];
 #pragma unroll
             for (int o = 1; o < L::TN; ++o) x = b == o ? l.acc[a][o][4 * q + r] : x;
-            x = __builtin_amdgcn_exp2f(fmaf(x * to_w, to_x, -lse));
-            x = tl == row ? x - 1.f : x;
-            x = row < left ? x : 0.f;
-            p[r] = x * lift;
+            x = __builtin_amdgcn_exp2f(fmaf(x * units.from_w, units.from_x, -top) * LOG2E) * over;
+            x = tl == row ? x - lift : x;
+            p[r] = row < left ? x : 0.f;
           }
           const int byte = (a * 32 + 8 * q + 4 * h) * ES;
           put<true>(to + (((byte >> 4) ^ (lane & 7)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
@@ -586,8 +586,8 @@ __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits
   logits_tile<OP, L, false>(c, blockIdx.x, s0, s1, s2, s3);
 }
 
-// A token's statistics over the mt tiles joined: `TOKENS` tokens a workgroup, NTHREADS / TOKENS lanes each. lse (base 2), the loss, and the
-// workgroup's sum of losses. (32 tokens where there are many, four where a few tokens' 400 tiles are all there is to
+// A token's statistics over the mt tiles joined: `TOKENS` tokens a workgroup, NTHREADS / TOKENS lanes each. What the backward pass takes of them, the loss, and
+// the workgroup's sum of losses. (32 tokens where there are many, four where a few tokens' 400 tiles are all there is to
 // read: 8 tokens of 50304 words 8.1 us with 8 lanes each, 4.7 with 64.)
 template <int TOKENS>
 __global__ __launch_bounds__(NTHREADS) void xent_join_kernel(LogitsCall c, float* lse, float* each, float* sums, int64_t ignore) {
@@ -623,7 +623,7 @@ __global__ __launch_bounds__(NTHREADS) void xent_join_kernel(LogitsCall c, float
       const float nan = __uint_as_float(0x7fc00000u);
       float loss = real ? (mx - c.at[i]) + logf(s) : nan;
       if (!c.rows && t == ignore) loss = 0.f;
-      if (lse) lse[i] = real ? fmaf(mx, LOG2E, log2f(s)) : nan;
+      if (lse) lse[i] = mx, lse[c.tokens + i] = real ? 1.f / s : nan;
       if (each) each[token] = loss;
       total += loss;
     }

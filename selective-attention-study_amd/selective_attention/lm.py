@@ -347,7 +347,8 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0) -> Tensor:
 # -- the vocabulary loss ------------------------------------------------------------------------------------
 
 def _xent_impl(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reduction: int, code: int, train: bool):
-    """sa_linear_xent on x (N, C): the loss, and for the backward pass (`train`; else None) lse (N,) and the kept tokens."""
+    """sa_linear_xent on x (N, C): the loss, and for the backward pass (`train`; else None) the kept tokens'
+    largest logits and reciprocal sums (2, N), and which those are."""
     tokens, width = x.shape
     vocab, device = weight.shape[0], x.device
     lib = _lib.load()
@@ -356,7 +357,7 @@ def _xent_impl(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reductio
     targets = targets.contiguous()
     none = reduction == _lib.REDUCTIONS["none"]
     loss = torch.empty((tokens,) if none else (), device=device, dtype=torch.float32)
-    lse = torch.empty(tokens, device=device, dtype=torch.float32) if train else None
+    lse = torch.empty(2, tokens, device=device, dtype=torch.float32) if train else None
     rows = torch.empty(_lib.XENT_ROWS + 2 * tokens, device=device, dtype=torch.int32)
     x_code, w_code, x_ptr, w_ptr = _CODES[x.dtype], _CODES[weight.dtype], x.data_ptr(), weight.data_ptr()
     size = _sized(device, lib.sa_linear_xent_workspace_bytes, x_ptr, x_ld, w_ptr, w_ld, tokens, vocab, width, reduction, train, x_code,
@@ -380,7 +381,7 @@ _xent_op = _custom_op("linear_cross_entropy_forward", _xent_dense)
 def _xent_fake(x, weight, targets, ignore, reduction, code, train):
     f32 = dict(dtype=torch.float32)
     tokens = x.shape[0]
-    return (x.new_empty((tokens,) if reduction == 0 else (), **f32), x.new_empty((tokens if train else 0,), **f32),
+    return (x.new_empty((tokens,) if reduction == 0 else (), **f32), x.new_empty((2, tokens) if train else (0,), **f32),
             x.new_empty((_lib.XENT_ROWS + 2 * tokens if train else 0,), dtype=torch.int32))
 
 
@@ -418,7 +419,7 @@ def _xent_backward_fake(x, weight, targets, lse, rows, dloss, reduction, code, n
 
 
 class _LinearCrossEntropyFn(torch.autograd.Function):
-    """Keeps x, weight, a number per token (lse) and the kept tokens' places; the backward pass computes the logits again."""
+    """Keeps x, weight, two numbers per token and the kept tokens' places; the backward pass computes the logits again."""
 
     @staticmethod
     def forward(ctx, x, weight, targets, ignore, reduction, code):
