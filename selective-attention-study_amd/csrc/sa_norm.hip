@@ -23,7 +23,7 @@ struct NormCall {
   void *y, *s, *dx, *dbranch;
   float *mean, *rstd, *part;
   int64_t x_ld, branch_ld, dy_ld, ds_ld, rows;
-  int width, x_t, branch_t, y_t, w_t;
+  int width, x_t, branch_t, y_t, w_t, sums;   // sums: rows of part (dw, db)
   float eps;
 };
 
@@ -162,13 +162,13 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_backward_kernel(NormCa
     }
   }
   if (!c.part) return;
-  // part[workgroup][2][width]: the wavefronts' sums are added in order
-  float* mine = c.part + (int64_t)blockIdx.x * 2 * c.width;
+  // part[workgroup][sums][width]: the wavefronts' sums are added in order
+  float* mine = c.part + (int64_t)blockIdx.x * c.sums * c.width;
   if constexpr (PER == 1) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       put<VEC>(mine, SA_DTYPE_F32, first_of<G, VEC>(v, lane), G, c.width, dw[v]);
-      put<VEC>(mine + c.width, SA_DTYPE_F32, first_of<G, VEC>(v, lane), G, c.width, db[v]);
+      if (c.sums > 1) put<VEC>(mine + c.width, SA_DTYPE_F32, first_of<G, VEC>(v, lane), G, c.width, db[v]);
     }
   } else {
     __shared__ float acc[2][V * 4][64];
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_backward_kernel(NormCa
 #pragma unroll
         for (int j = 0; j < 4; ++j) a[j] = acc[0][v * 4 + j][lane], b[j] = acc[1][v * 4 + j][lane];
         put<VEC>(mine, SA_DTYPE_F32, first_of<G, VEC>(v, lane), G, c.width, a);
-        put<VEC>(mine + c.width, SA_DTYPE_F32, first_of<G, VEC>(v, lane), G, c.width, b);
+        if (c.sums > 1) put<VEC>(mine + c.width, SA_DTYPE_F32, first_of<G, VEC>(v, lane), G, c.width, b);
       }
     }
   }
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const float* part, int 
   if (e < width) {
     const float* p = part + (int64_t)blockIdx.y * width + e;
 #pragma unroll 8
-    for (int i = k; i < parts; i += 16) sum += p[(int64_t)i * 2 * width];
+    for (int i = k; i < parts; i += 16) sum += p[(int64_t)i * gridDim.y * width];
   }
   acc[k][x] = sum;
   __syncthreads();
@@ -221,11 +221,10 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const float* part, int 
 
 constexpr int64_t MAX_WIDTH = 32768;
 
-// Workgroups of the backward: enough to fill every CU (two of four wavefronts each, one of 16), few enough that their sums
-// are little beside the rows; no more than there are rows for.
+// Workgroups of the backward: enough to fill every CU, few enough that their sums are little beside the rows, of which
+// there is one at a time and wavefront up to 2048 wide, and one a workgroup beyond.
 int64_t norm_parts(int64_t rows, int64_t width) {
-  const int64_t per = width <= 2048 ? 4 : 1;
-  return std::max<int64_t>(1, std::min<int64_t>(512, cdiv(rows, per)));
+  return std::max<int64_t>(1, width <= 2048 ? std::min<int64_t>(512, cdiv(rows, 4)) : std::min<int64_t>(256, rows));
 }
 
 template <int G, int V, bool VEC>
@@ -306,7 +305,7 @@ int sa_layer_norm_backward(const void* s, int64_t s_ld, const void* dy, int64_t 
     return SA_ERR_WORKSPACE;
   NormCall c{};
   c.x = s, c.dy = dy, c.ds = ds, c.w = weight, c.mean = const_cast<float*>(mean), c.rstd = const_cast<float*>(rstd);
-  c.dx = dx, c.dbranch = dbranch, c.part = sums ? (float*)workspace : nullptr;
+  c.dx = dx, c.dbranch = dbranch, c.part = sums ? (float*)workspace : nullptr, c.sums = dbias ? 2 : 1;
   c.x_ld = s_ld, c.dy_ld = dy_ld, c.ds_ld = ds_ld, c.rows = rows, c.width = (int)width;
   c.x_t = s_dtype, c.branch_t = dbranch ? branch_dtype : s_dtype, c.y_t = y_dtype, c.w_t = weight_dtype;
   const bool vec = width % 4 == 0 && quads_ok(s, s_ld, s_dtype) && quads_ok(dy, dy_ld, y_dtype) && quads_ok(ds, ds_ld, s_dtype) &&
@@ -315,7 +314,7 @@ int sa_layer_norm_backward(const void* s, int64_t s_ld, const void* dy, int64_t 
   if (vec) launch_norm<true>(c, true, st);   // (no rows: sums of nothing)
   else launch_norm<false>(c, true, st);
   if (sums)
-    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)cdiv(width, 64), 2), dim3(1024), 0, st, c.part,
+    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)cdiv(width, 64), (unsigned)c.sums), dim3(1024), 0, st, c.part,
                        (int)norm_parts(rows, width), (int)width, dweight, dbias, weight_dtype);
   return launch_status();
 }

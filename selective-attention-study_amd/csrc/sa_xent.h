@@ -952,7 +952,7 @@ void launch_logits(LogitsCall lc, int64_t tokens, hipStream_t st) {
 }
 // g, x, w: what the pass does (null: not that)
 template <class OP, class LG, class LX, class LW>
-void launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w, int64_t tokens, hipStream_t st) {
+bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w, int64_t tokens, hipStream_t st) {
   PassCall pc{};
   int64_t at = 0;
   const auto place = [&at](ProductCall& c, int64_t m, int edge_m, int edge_n, int& begin, int& tiles, int& end) {
@@ -976,7 +976,9 @@ void launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
     pc.g_at = (int)at;
     at += tiles_grid(pc.g.mt, pc.g.nt);
   }
+  if (at * LG::THREADS >= ((int64_t)1 << 32)) return false;   // more threads than a launch takes
   hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
+  return true;
 }
 template <class OP, bool FIRST = false>
 void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows,
@@ -1081,8 +1083,9 @@ int xent_backward(const XentCall& c) {
     }
     const LogitsCall* pg = p < s.pieces ? &g : nullptr;
     const ProductCall *x = p > 0 && c.dx ? &px : nullptr, *y = p > 0 && c.dw ? &pw : nullptr;
-    if (s.large_pass) launch_pass<OP, typename F::Large, typename F::LargeX, typename F::LargeW>(pg, x, y, c.tokens, c.st);
-    else launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st);
+    if (!(s.large_pass ? launch_pass<OP, typename F::Large, typename F::LargeX, typename F::LargeW>(pg, x, y, c.tokens, c.st)
+                       : launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st)))
+      return SA_ERR_ARGUMENT;
     if (y && pw.splits > 1)
       launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t, c.st);
   }

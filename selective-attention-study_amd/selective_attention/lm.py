@@ -82,8 +82,9 @@ def _filled(*results: Tensor | None, like: Tensor) -> tuple[Tensor, ...]:
 
 
 def _mode_plain(plain: bool, *tensors: Tensor | None) -> bool:
-    """_plain in a backward pass, of the gradients that arrive: what was saved was looked at in the forward pass."""
-    return plain and _plain(*[t for t in tensors if t is not None])
+    """_plain in a backward pass, of the gradients that arrive: what was saved was looked at in the forward pass. Where a second
+    derivative may follow (create_graph) it is the op that runs, which raises then."""
+    return plain and not torch.is_grad_enabled() and _plain(*[t for t in tensors if t is not None])
 
 
 def _sized(device: torch.device, query, *args) -> int:
@@ -465,10 +466,10 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, ignore_inde
     dot_precision: None takes the products' operands in x's dtype, "bf16" in bf16, "tf32" and "ieee" in fp32 (no TF32 on this
     hardware); x and weight are rounded to it where they are of another type (the fp32 weight of a bf16 autocast step), products
     are summed in fp32. Gradients have x's and weight's own types. The probabilities that enter the gradients' products are
-    rounded to the operands' type (bf16: 2^-9 of each, of the size of a bf16 gradient's own rounding).
+    rounded to 11 bits for bf16 and fp16 operands, not at all for fp32.
 
-    The backward pass computes the logits again, a piece of the vocabulary at a time: its scratch memory is up to about
-    256 MB and fp32 sums of x's size. C up to 65536, up to 2^28 - 1 tokens and vocabulary rows, 2^37 logits."""
+    The backward pass computes the logits again, a piece of the vocabulary at a time: its scratch memory is two pieces of up to 256 MB, fp32
+    sums of x's size, and copies of x and, but for fp16 and fp32 rows that lie as the kernels read them, of weight. C up to 65536, up to 2^28 - 1 tokens and vocabulary rows, 2^37 logits."""
 
     _check_float("x", x)
     _check_float("weight", weight, x.device)

@@ -650,8 +650,10 @@ def test_refusals(cuda):
     ):
         with pytest.raises(ValueError):
             call()
-    # a second derivative
+    # a second derivative, of gradients that depend on the leaf through what arrives or through what was saved
     leaf = x.clone().requires_grad_()
-    d, = torch.autograd.grad(sa.layer_norm(leaf, w).square().sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(d.sum(), leaf)
+    for f in (lambda: sa.layer_norm(leaf, w).square().sum(), lambda: sa.layer_norm(leaf, w).sum(), lambda: sa.linear_cross_entropy(leaf, x, t),
+              lambda: sa.embedding(t, leaf).square().sum()):
+        d, = torch.autograd.grad(f(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(d.sum() + leaf.sum(), leaf)
