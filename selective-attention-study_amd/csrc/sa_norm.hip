@@ -5,7 +5,7 @@
 //   dx = dbranch = r (u - mean(u) - h mean(u h)) + ds,  u = dy w;   dw = sum over rows of dy h,  db = sum of dy
 //
 // Bound by memory: the forward reads x and branch and writes y and s once, the backward reads s, dy and ds and writes dx once. A row
-// stays in the registers of the lanes that loaded it (a wavefront up to 2048 wide, a workgroup of 4 or 16 wavefronts beyond), so its mean
+// stays in the registers of the lanes that loaded it (a wavefront up to 1024 wide, a workgroup of 4 to 16 wavefronts beyond), so its mean
 // and the sum of its squared deviations are two exact passes over registers, not a difference of sums. Everything is fp32 in
 // between; outputs are rounded once.
 //
@@ -66,6 +66,16 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(NormCall c) {
 #pragma unroll
       for (int v = 0; v < V; ++v) qb[v] = fetch<VEC>(br, c.branch_t, first_of<G, VEC>(v, lane), G, c.width);
     }
+    // rows shared by wavefronts wait for each other twice: the weights are asked for before that
+    constexpr bool EARLY = G > 64 && V <= 2;
+    Quad qw[V], qc[V];
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        qw[v] = fetch<VEC>(c.w, c.w_t, first_of<G, VEC>(v, lane), G, c.width);
+        if (c.b) qc[v] = fetch<VEC>(c.b, c.w_t, first_of<G, VEC>(v, lane), G, c.width);
+      }
+    }
     float s[V][4];
     float sum = 0.f;
 #pragma unroll
@@ -98,8 +108,8 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(NormCall c) {
     for (int v = 0; v < V; ++v) {
       const int e = first_of<G, VEC>(v, lane);
       float w[4], b[4] = {0.f, 0.f, 0.f, 0.f};
-      numbers<VEC>(fetch<VEC>(c.w, c.w_t, e, G, c.width), c.w_t, w);
-      if (c.b) numbers<VEC>(fetch<VEC>(c.b, c.w_t, e, G, c.width), c.w_t, b);
+      numbers<VEC>(EARLY ? qw[v] : fetch<VEC>(c.w, c.w_t, e, G, c.width), c.w_t, w);
+      if (c.b) numbers<VEC>(EARLY ? qc[v] : fetch<VEC>(c.b, c.w_t, e, G, c.width), c.w_t, b);
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = s[v][j] * r * w[j] + b[j];
       put<VEC>(yr, c.y_t, e, G, c.width, w);
@@ -119,8 +129,8 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_backward_kernel(NormCa
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[v][j] = db[v][j] = 0.f;
   }
-  for (int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / G; row < c.rows; row += (int64_t)gridDim.x * PER) {
-    Quad qs[V], qy[V], qd[V];
+  Quad qs[V], qy[V], qd[V];
+  const auto load = [&](int64_t row) {
     const void *sr = row_of(c.x, row, c.x_ld, c.x_t), *yr = row_of(c.dy, row, c.dy_ld, c.y_t);
 #pragma unroll
     for (int v = 0; v < V; ++v) qs[v] = fetch<VEC>(sr, c.x_t, first_of<G, VEC>(v, lane), G, c.width);
@@ -131,13 +141,29 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_backward_kernel(NormCa
 #pragma unroll
       for (int v = 0; v < V; ++v) qd[v] = fetch<VEC>(dr, c.x_t, first_of<G, VEC>(v, lane), G, c.width);
     }
+  };
+  // Rows that a workgroup shares: the next one's loads are under way while one is worked on (2048 x 8192 bf16: 53 -> 38 us). Rows of
+  // a wavefront have other wavefronts for that, and lose more of them to the registers (16384 x 768: 43 -> 52 us).
+  constexpr bool AHEAD = G > 64 && G < 1024;
+  const int64_t stride = (int64_t)gridDim.x * PER;
+  int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / G;
+  if (AHEAD && row < c.rows) load(row);
+  for (; row < c.rows; row += stride) {
+    if (!AHEAD) load(row);
     const float mean = c.mean[row], r = c.rstd[row];
-    float h[V][4], u[V][4];
-    float su = 0.f, suh = 0.f;
+    float h[V][4], u[V][4], d[V][4];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       numbers<VEC>(qs[v], c.x_t, h[v]);
       numbers<VEC>(qy[v], c.y_t, u[v]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[v][j] = 0.f;
+      if (c.ds) numbers<VEC>(qd[v], c.x_t, d[v]);
+    }
+    if (AHEAD && row + stride < c.rows) load(row + stride);
+    float su = 0.f, suh = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int e = first_of<G, VEC>(v, lane) + (VEC ? j : j * G);
@@ -153,12 +179,10 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_backward_kernel(NormCa
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int e = first_of<G, VEC>(v, lane);
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
-      if (c.ds) numbers<VEC>(qd[v], c.x_t, d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] += r * (u[v][j] - mu - h[v][j] * muh);
-      if (c.dx) put<VEC>(row_of(c.dx, row, c.width, c.x_t), c.x_t, e, G, c.width, d);
-      if (c.dbranch) put<VEC>(row_of(c.dbranch, row, c.width, c.branch_t), c.branch_t, e, G, c.width, d);
+      for (int j = 0; j < 4; ++j) d[v][j] += r * (u[v][j] - mu - h[v][j] * muh);
+      if (c.dx) put<VEC>(row_of(c.dx, row, c.width, c.x_t), c.x_t, e, G, c.width, d[v]);
+      if (c.dbranch) put<VEC>(row_of(c.dbranch, row, c.width, c.branch_t), c.branch_t, e, G, c.width, d[v]);
     }
   }
   if (!c.part) return;
@@ -222,33 +246,47 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const float* part, int 
 constexpr int64_t MAX_WIDTH = 32768;
 
 // Workgroups of the backward: enough to fill every CU, few enough that their sums are little beside the rows, of which
-// there is one at a time and wavefront up to 2048 wide, and one a workgroup beyond.
+// there is one at a time and wavefront up to 1024 wide, and one a workgroup beyond.
 int64_t norm_parts(int64_t rows, int64_t width) {
-  return std::max<int64_t>(1, width <= 2048 ? std::min<int64_t>(512, cdiv(rows, 4)) : std::min<int64_t>(256, rows));
+  return std::max<int64_t>(1, width <= 1024 ? std::min<int64_t>(512, cdiv(rows, 4)) : std::min<int64_t>(width <= 4096 ? 512 : 256, rows));
 }
 
+// Lanes of a row and quads of a lane by width. The forward takes more lanes than the backward, which keeps three rows' worth of sums and
+// weights in registers: two workgroups on a CU work while others wait for their rows.
 template <int G, int V, bool VEC>
-void launch_norm(const NormCall& c, bool backward, hipStream_t st) {
-  constexpr int PER = norm_threads<G>() / G;
-  if (backward) {
-    hipLaunchKernelGGL((norm_backward_kernel<G, V, VEC>), dim3((unsigned)norm_parts(c.rows, c.width)), dim3(norm_threads<G>()), 0, st, c);
-  } else {
-    const int64_t blocks = std::min<int64_t>(cdiv(c.rows, PER), LAUNCH_BLOCKS);
-    hipLaunchKernelGGL((norm_kernel<G, V, VEC>), dim3((unsigned)blocks), dim3(norm_threads<G>()), 0, st, c);
-  }
+void launch_forward(const NormCall& c, hipStream_t st) {
+  const int64_t blocks = std::min<int64_t>(cdiv(c.rows, norm_threads<G>() / G), LAUNCH_BLOCKS);
+  hipLaunchKernelGGL((norm_kernel<G, V, VEC>), dim3((unsigned)blocks), dim3(norm_threads<G>()), 0, st, c);
+}
+template <int G, int V, bool VEC>
+void launch_backward(const NormCall& c, hipStream_t st) {
+  hipLaunchKernelGGL((norm_backward_kernel<G, V, VEC>), dim3((unsigned)norm_parts(c.rows, c.width)), dim3(norm_threads<G>()), 0, st, c);
 }
 template <bool VEC>
-void launch_norm(const NormCall& c, bool backward, hipStream_t st) {
+void launch_forward(const NormCall& c, hipStream_t st) {
   const int w = c.width;
-  if (w <= 256) launch_norm<64, 1, VEC>(c, backward, st);
-  else if (w <= 512) launch_norm<64, 2, VEC>(c, backward, st);
-  else if (w <= 768) launch_norm<64, 3, VEC>(c, backward, st);
-  else if (w <= 1024) launch_norm<64, 4, VEC>(c, backward, st);
-  else if (w <= 2048) launch_norm<64, 8, VEC>(c, backward, st);
-  else if (w <= 4096) launch_norm<256, 4, VEC>(c, backward, st);
-  else if (w <= 8192) launch_norm<256, 8, VEC>(c, backward, st);
-  else if (w <= 16384) launch_norm<1024, 4, VEC>(c, backward, st);
-  else launch_norm<1024, 8, VEC>(c, backward, st);
+  if (w <= 256) launch_forward<64, 1, VEC>(c, st);
+  else if (w <= 512) launch_forward<64, 2, VEC>(c, st);
+  else if (w <= 768) launch_forward<64, 3, VEC>(c, st);
+  else if (w <= 1024) launch_forward<64, 4, VEC>(c, st);
+  else if (w <= 2048) launch_forward<256, 2, VEC>(c, st);
+  else if (w <= 4096) launch_forward<512, 2, VEC>(c, st);
+  else if (w <= 8192) launch_forward<1024, 2, VEC>(c, st);
+  else if (w <= 16384) launch_forward<1024, 4, VEC>(c, st);
+  else launch_forward<1024, 8, VEC>(c, st);
+}
+template <bool VEC>
+void launch_backward(const NormCall& c, hipStream_t st) {
+  const int w = c.width;
+  if (w <= 256) launch_backward<64, 1, VEC>(c, st);
+  else if (w <= 512) launch_backward<64, 2, VEC>(c, st);
+  else if (w <= 768) launch_backward<64, 3, VEC>(c, st);
+  else if (w <= 1024) launch_backward<64, 4, VEC>(c, st);
+  else if (w <= 2048) launch_backward<256, 2, VEC>(c, st);
+  else if (w <= 4096) launch_backward<256, 4, VEC>(c, st);
+  else if (w <= 8192) launch_backward<512, 4, VEC>(c, st);
+  else if (w <= 16384) launch_backward<1024, 4, VEC>(c, st);
+  else launch_backward<1024, 8, VEC>(c, st);
 }
 
 bool norm_sizes_ok(int64_t rows, int64_t width) { return rows >= 0 && rows < ((int64_t)1 << 40) && width >= 1 && width <= MAX_WIDTH; }
@@ -278,8 +316,8 @@ int sa_layer_norm(const void* x, int64_t x_ld, const void* branch, int64_t branc
                    quads_ok(weight, 0, weight_dtype) && quads_ok(bias, 0, weight_dtype) && quads_ok(y, width, y_dtype) &&
                    quads_ok(sum, width, x_dtype);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (vec) launch_norm<true>(c, false, st);
-  else launch_norm<false>(c, false, st);
+  if (vec) launch_forward<true>(c, st);
+  else launch_forward<false>(c, st);
   return launch_status();
 }
 
@@ -311,8 +349,8 @@ int sa_layer_norm_backward(const void* s, int64_t s_ld, const void* dy, int64_t 
   const bool vec = width % 4 == 0 && quads_ok(s, s_ld, s_dtype) && quads_ok(dy, dy_ld, y_dtype) && quads_ok(ds, ds_ld, s_dtype) &&
                    quads_ok(weight, 0, weight_dtype) && quads_ok(dx, width, s_dtype) && quads_ok(dbranch, width, c.branch_t);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (vec) launch_norm<true>(c, true, st);   // (no rows: sums of nothing)
-  else launch_norm<false>(c, true, st);
+  if (vec) launch_backward<true>(c, st);   // (no rows: sums of nothing)
+  else launch_backward<false>(c, st);
   if (sums)
     hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)cdiv(width, 64), (unsigned)c.sums), dim3(1024), 0, st, c.part,
                        (int)norm_parts(rows, width), (int)width, dweight, dbias, weight_dtype);
