@@ -338,27 +338,31 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets,
   __shared__ float acc[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (blockIdx.x > 0) {
-    const int per = (w.width + 3) / 4;
-    const int64_t n = w.rows * per;
+    // rows that follow each other are one; else a wavefront takes rows in turn
     const bool quads = (uintptr_t)w.p % (w.dtype == SA_DTYPE_F32 ? 16 : 8) == 0 && w.ld % 4 == 0 && w.width % 4 == 0;
+    const bool flat = quads && w.ld == w.width;
+    constexpr int64_t RUN = 2048;   // elements of a flat matrix's row: a wavefront's loads in flight
+    const int64_t elements = w.rows * w.width, n = flat ? (elements + RUN - 1) / RUN : w.rows;
     float most = 0.f;
     constexpr int AHEAD = 8;   // loads in flight
-    for (int64_t k0 = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; k0 < n; k0 += (int64_t)MAXIMA * 1024 * AHEAD) {
-      Quad q[AHEAD];
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * 16 + wave; i < n; i += MAXIMA * 16) {
+      const void* row = row_of(w.p, flat ? i * RUN : i, flat ? 1 : w.ld, w.dtype);
+      const int width = flat ? (int)min(RUN, elements - i * RUN) : w.width;
+      for (int e0 = 0; e0 < width; e0 += 256 * AHEAD) {
+        Quad q[AHEAD];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int64_t k = k0 + (int64_t)u * MAXIMA * 1024, row = k / per;
-        const int e = (int)(k - row * per) * 4;
-        const void* at = row_of(w.p, row, w.ld, w.dtype);
-        q[u] = quads ? fetch<true>(at, w.dtype, e, 1, k < n ? w.width : 0) : fetch<false>(at, w.dtype, e, 1, k < n ? w.width : 0);
-      }
+        for (int u = 0; u < AHEAD; ++u) {
+          const int e = e0 + 256 * u + 4 * lane;
+          q[u] = quads ? fetch<true>(row, w.dtype, e, 1, width) : fetch<false>(row, w.dtype, e, 1, width);
+        }
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        float x[4];
-        if (quads) numbers<true>(q[u], w.dtype, x);
-        else numbers<false>(q[u], w.dtype, x);
+        for (int u = 0; u < AHEAD; ++u) {
+          float x[4];
+          if (quads) numbers<true>(q[u], w.dtype, x);
+          else numbers<false>(q[u], w.dtype, x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[j]));
+          for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[j]));
+        }
       }
     }
     put_maximum(most, acc, rows + 64, blockIdx.x - 1);
@@ -402,30 +406,36 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets,
 // Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i]; FIRST: rounded to bf16 first and
 // taken *unit times. maxima: each workgroup's largest magnitude (MAXIMA workgroups then).
 template <class OP, bool FIRST>
-__global__ __launch_bounds__(NTHREADS) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
+__global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
                                                                const int* count, int64_t most, const float* unit, int* maxima,
                                                                typename OP::elem* to, int padded) {
   __shared__ float acc[16];
   const int64_t rows = count ? *count : most;
-  const int per = padded / 4;
-  const bool quads = ((uintptr_t)from % (dtype == SA_DTYPE_F32 ? 16 : 8)) == 0 && ld % 4 == 0;
-  const int64_t n = rows * per;
+  const int lane = threadIdx.x & 63;
+  const bool quads = ((uintptr_t)from % (dtype == SA_DTYPE_F32 ? 16 : 8)) == 0 && ld % 4 == 0 && width % 4 == 0;
   const float by = FIRST ? *unit : 1.f;
   float top = 0.f;
-  for (int64_t k = (int64_t)blockIdx.x * NTHREADS + threadIdx.x; k < n; k += (int64_t)gridDim.x * NTHREADS) {
-    const int64_t i = k / per;
-    const int e = (int)(k - i * per) * 4;
+  constexpr int AHEAD = 4;   // loads in flight: a wavefront's of a row
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 64) + wave_index(); i < rows; i += (int64_t)gridDim.x * (blockDim.x / 64)) {
     const void* row = row_of(from, numbers_of ? numbers_of[i] : i, ld, dtype);
-    float x[4];
-    if (quads && e + 4 <= width) numbers<true>(fetch<true>(row, dtype, e, 1, width), dtype, x);
-    else numbers<false>(fetch<false>(row, dtype, e, 1, width), dtype, x);
-    if constexpr (FIRST) {
+    for (int e0 = 4 * lane; e0 < padded; e0 += 256 * AHEAD) {
+      Quad q[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = stored(x[j], SA_DTYPE_BF16) * by;
+      for (int u = 0; u < AHEAD; ++u)
+        q[u] = quads ? fetch<true>(row, dtype, e0 + 256 * u, 1, width) : fetch<false>(row, dtype, e0 + 256 * u, 1, width);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        float x[4];
+        if (quads) numbers<true>(q[u], dtype, x);
+        else numbers<false>(q[u], dtype, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (FIRST) x[j] = stored(x[j], SA_DTYPE_BF16) * by;
+          top = fmaxf(top, fabsf(x[j]));
+        }
+        put<true>(to + i * padded, OP::CODE, e0 + 256 * u, 1, padded, x);
+      }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[j]));
-    put<true>(to + i * padded, OP::CODE, e, 1, padded, x);
   }
   if (maxima) put_maximum(top, acc, maxima, blockIdx.x);
 }
@@ -926,7 +936,7 @@ struct XentShape {
       const int64_t share = cdiv(products + (pieces > 1 ? tiles(edge, c.tokens, piece) * (k_g + 8) : products / 2), slots);
       const int64_t share_last = std::max<int64_t>(cdiv(products, 2 * slots), 1);
       const auto parts = [](int64_t stages, int64_t of) { return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(stages, of), stages / 8, 16})); };
-      splits_x = parts(k_x, pieces > 1 ? share : share_last);
+      splits_x = parts(k_x, pieces > 1 ? cdiv(share, 2) : share_last);   // (ignored tokens shorten all but this)
       splits_w = parts(k_w, share);
       splits_last = parts(k_w, share_last);
       // (a part's rows lie within 2^30 bytes)
@@ -983,9 +993,9 @@ bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
 template <class OP, bool FIRST = false>
 void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows,
                    const float* unit, int* maxima, void* to, int64_t padded, hipStream_t st) {
-  const int64_t blocks = maxima ? MAXIMA : std::min<int64_t>(cdiv(rows * (padded / 4), NTHREADS), 16384);
-  hipLaunchKernelGGL((xent_gather_kernel<OP, FIRST>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, from, ld, dtype, (int)width, numbers_of,
-                     count, rows, unit, maxima, (typename OP::elem*)to, (int)padded);
+  const int64_t blocks = maxima ? MAXIMA : std::min<int64_t>(cdiv(rows, NWAVES), 16384);
+  hipLaunchKernelGGL((xent_gather_kernel<OP, FIRST>), dim3((unsigned)blocks), dim3(maxima ? 1024 : NTHREADS), 0, st, from, ld, dtype, (int)width,
+                     numbers_of, count, rows, unit, maxima, (typename OP::elem*)to, (int)padded);
 }
 inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const Factors* units,
                           const float* unit, float lift, void* out, int64_t rows, int64_t width, int dtype, hipStream_t st) {
