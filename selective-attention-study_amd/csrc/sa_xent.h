@@ -873,8 +873,8 @@ struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per st
   typedef Mainloop<XF32, 2, 2, 2, 2, true, true> MiddleW;
 };
 
-constexpr int64_t SMALL_TOKENS = 64;      // one tile's tokens of the smallest kernel
-constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are
+constexpr int64_t SMALL_TOKENS = 64;      // one tile's tokens of the smallest kernel (8 tokens x 50304 x 768, weight out of HBM: 20.0 us, 21.5 by 128 x 128)
+constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are (250 tokens 40 us, listed and gathered 47)
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of a piece's G, of which there are two at a time
 constexpr int64_t JOIN_FEW = 1024;        // tokens up to which the join takes 64 lanes for each
 constexpr int64_t MAX_LD_BYTES = 1 << 22;             // 256 rows within a buffer resource's 2 GiB
@@ -897,7 +897,11 @@ struct XentShape {
     train = c.lse != nullptr;
     padded = align_up(c.width, BK);
     small = c.tokens <= SMALL_TOKENS && !train;
-    large = !small && ES == 2 && cdiv(c.vocab, 256) * cdiv(c.tokens, 256) >= 2 * (int64_t)c.cus;
+    // Tiles of 256 x 256 where every CU has one and the last tokens' are not mostly empty (four wavefronts' of 128 x 128 else).
+    // Forward, us, large / middle, tokens x words x 768: 400 x 50304 58 / 64, 1000 x 16384 40 / 47, 2000 x 50304 183 / 197; 128 x 50304
+    // 27 / 25 (197 tiles), 300 x 33000 54 / 42 (212 of the second 256 tokens missing).
+    const bool whole = cdiv(c.tokens, 256) * 256 * 4 <= cdiv(c.tokens, 128) * 128 * 5;
+    large = !small && ES == 2 && whole && cdiv(c.vocab, 256) * cdiv(c.tokens, 256) >= c.cus;
     bm = large ? 256 : 128;
     mt = cdiv(c.vocab, bm);
     const bool x_ok = c.x_t == OP::CODE && padded == c.width && (uintptr_t)c.x % 16 == 0 && c.x_ld * ES % 16 == 0 &&
@@ -926,19 +930,24 @@ struct XentShape {
       pieces = cdiv(c.vocab, most);
       piece = align_up(cdiv(c.vocab, pieces), 256);
       pieces = cdiv(c.vocab, piece);
-      // Tiles as large as leave every CU a few to do, and no contraction longer than a CU's share of a pass (half of it in the
-      // last, where no tiles of G fill up): a part more costs its sums' way through memory
+      // The same choice by a pass's tiles (backward, us, large / middle: 2048 x 50304 x 768 589 / 645, 4096 x 16384 x 1024 455 / 498, 500 x
+      // 50304 x 768 229 / 237; 100 x 50304 x 768 143 / 117, 2000 x 4000 x 1024 109 / 95). No contraction is longer than a CU's
+      // share of a pass, or twice that in the last, where no tiles of G fill up; parts' sums go through memory. dX's is held to half of
+      // the share, as ignored tokens shorten everything else (5003 x 50257 x 1024, a third ignored, in 1 / 2 / 3 / 4 parts:
+      // 1453 / 1201 / 1199 / 1205 us; 1000 x 16384 x 768 in 2 / 4 / 8 / 16: 217 / 151 / 130 / 136; 100 x 50304 x 768 in 4 / 8 / 16: 153 / 117 / 114).
+      // dW's over few tokens is best whole (1000 x 16384 x 768 in 1 / 2 parts 136 / 175), over 16384 x 50304 the last piece's
+      // in 1 / 2 / 3 / 6 4138 / 4070 / 4056 / 4063. Pieces of 64 / 128 / 256 / 512 MB there: 4405 / 4160 / 4039 / 4016.
       const int64_t k_x = cdiv(piece, BK), k_w = cdiv(c.tokens, BK), k_g = padded / BK;
       const auto tiles = [&](int64_t edge, int64_t m, int64_t n) { return cdiv(m, edge) * cdiv(n, edge); };
-      large_pass = ES == 2 && tiles(256, c.tokens, c.width) + tiles(256, piece, c.width) + tiles(256, c.tokens, piece) / 4 >= c.cus;
+      large_pass = ES == 2 && whole && tiles(256, c.tokens, c.width) + tiles(256, piece, c.width) + tiles(256, c.tokens, piece) / 4 >= c.cus;
       const int64_t edge = large_pass ? 256 : 128, slots = large_pass ? c.cus : 2 * (int64_t)c.cus;
       const int64_t products = (c.dx ? tiles(edge, c.tokens, c.width) * k_x : 0) + (c.dw ? tiles(edge, piece, c.width) * k_w : 0);
       const int64_t share = cdiv(products + (pieces > 1 ? tiles(edge, c.tokens, piece) * (k_g + 8) : products / 2), slots);
       const int64_t share_last = std::max<int64_t>(cdiv(products, 2 * slots), 1);
       const auto parts = [](int64_t stages, int64_t of) { return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(stages, of), stages / 8, 16})); };
-      splits_x = parts(k_x, pieces > 1 ? cdiv(share, 2) : share_last);   // (ignored tokens shorten all but this)
+      splits_x = parts(k_x, pieces > 1 ? cdiv(share, 2) : 2 * share_last);
       splits_w = parts(k_w, share);
-      splits_last = parts(k_w, share_last);
+      splits_last = parts(k_w, 2 * share_last);
       // (a part's rows lie within 2^30 bytes)
       const int64_t w_row = (copy_w ? padded : c.w_ld) * ES, x_row = std::max(padded, piece) * ES;
       splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
