@@ -47,27 +47,31 @@ __device__ __forceinline__ int64_t id_at(const EmbedCall& c, int64_t i) {
 
 // ---------------------------------------------------------------------------------------------
 
-// A thread per four elements; an id outside the table gives a row of NaN, as there is no row to read and nothing on the
-// host knows of it.
+// 1 << shift lanes a row (as many as have four elements each, up to a wavefront); an id outside the table gives a row of NaN, as
+// there is no row to read and nothing on the host knows of it.
 template <bool VEC>
-__global__ __launch_bounds__(NTHREADS) void embed_kernel(EmbedCall c) {
-  const int per = (c.width + 3) / 4;
-  const int64_t n = c.tokens * per;
-  for (int64_t k = (int64_t)blockIdx.x * NTHREADS + threadIdx.x; k < n; k += (int64_t)gridDim.x * NTHREADS) {
-    const int64_t i = k / per;
-    const int q = (int)(k - i * per);
-    const int e = VEC ? 4 * q : q, gap = VEC ? 1 : per;
+__global__ __launch_bounds__(NTHREADS) void embed_kernel(EmbedCall c, int shift) {
+  const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1);
+  const int rows = NTHREADS >> shift;
+  for (int64_t i = (int64_t)blockIdx.x * rows + (threadIdx.x >> shift); i < c.tokens; i += (int64_t)gridDim.x * rows) {
     const int64_t id = id_at(c, i);
-    float x[4];
-    if (id >= 0 && id < c.vocab) {
-      numbers<VEC>(fetch<VEC>(row_of(c.w, id, c.w_ld, c.dtype), c.dtype, e, gap, c.width), c.dtype, x);
+    const bool real = id >= 0 && id < c.vocab;
+    const void* from = row_of(c.w, real ? id : 0, c.w_ld, c.dtype);
+    void* to = row_of(c.y, i, c.width, c.dtype);
+    constexpr int AHEAD = 4;   // loads in flight
+    for (int e0 = VEC ? 4 * lane : lane; e0 < c.width; e0 += 4 * lanes * AHEAD) {
+      Quad q[AHEAD];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] *= c.scale;
-    } else {
+      for (int u = 0; u < AHEAD; ++u) q[u] = fetch<VEC>(from, c.dtype, e0 + 4 * lanes * u, lanes, real ? c.width : 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(0x7fc00000u);
+      for (int u = 0; u < AHEAD; ++u) {
+        float x[4];
+        numbers<VEC>(q[u], c.dtype, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = real ? x[j] * c.scale : __uint_as_float(0x7fc00000u);
+        put<VEC>(to, c.dtype, e0 + 4 * lanes * u, lanes, c.width, x);
+      }
     }
-    put<VEC>(row_of(c.y, i, c.width, c.dtype), c.dtype, e, gap, c.width, x);
   }
 }
 
@@ -384,10 +388,12 @@ int sa_embedding(const void* ids, int ids_bytes, const void* weight, int64_t wei
   c.ids = ids, c.ids64 = ids_bytes == 8, c.w = weight, c.w_ld = weight_ld, c.y = out, c.tokens = tokens, c.vocab = vocab;
   c.width = (int)width, c.scale = scale, c.dtype = dtype;
   const bool vec = width % 4 == 0 && quads_ok(weight, weight_ld, dtype) && quads_ok(out, width, dtype);
-  const int64_t blocks = std::min<int64_t>(cdiv(tokens * cdiv(width, 4), NTHREADS), LAUNCH_BLOCKS);
+  int shift = 0;
+  while (shift < 6 && (4 << shift) < width) ++shift;
+  const int64_t blocks = std::min<int64_t>(cdiv(tokens, NTHREADS >> shift), LAUNCH_BLOCKS);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (vec) hipLaunchKernelGGL((embed_kernel<true>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, c);
-  else hipLaunchKernelGGL((embed_kernel<false>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, c);
+  if (vec) hipLaunchKernelGGL((embed_kernel<true>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, c, shift);
+  else hipLaunchKernelGGL((embed_kernel<false>), dim3((unsigned)blocks), dim3(NTHREADS), 0, st, c, shift);
   return launch_status();
 }
 

@@ -827,25 +827,24 @@ __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass
 __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums, int splits, int64_t split_stride, int64_t n_ld,
                                                                const int* place, const Factors* units, const float* unit, float lift,
                                                                void* out, int64_t rows, int width, int dtype) {
-  const int64_t per = (width + 3) / 4;
-  const int64_t n = rows * per;
+  const int lane = threadIdx.x & 63;
   const bool quads = width % 4 == 0;
-  for (int64_t k = (int64_t)blockIdx.x * NTHREADS + threadIdx.x; k < n; k += (int64_t)gridDim.x * NTHREADS) {
-    const int64_t row = k / per;
-    const int e = (int)(k - row * per) * 4;
+  const float f = units->g * lift, u = *unit;
+  for (int64_t row = (int64_t)blockIdx.x * NWAVES + wave_index(); row < rows; row += (int64_t)gridDim.x * NWAVES) {
     const int64_t at = place ? place[row] : row;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (at >= 0) {
-      for (int s = 0; s < splits; ++s) {
-        const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + at * n_ld + e);
-        x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
-      }
-      const float f = units->g * lift, u = *unit;
+    for (int e = 4 * lane; e < width; e += 256) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+      if (at >= 0) {
+        for (int s = 0; s < splits; ++s) {
+          const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + at * n_ld + e);
+          x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
+        }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = x[j] * f * u;
+        for (int j = 0; j < 4; ++j) x[j] = x[j] * f * u;
+      }
+      if (quads) put<true>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
+      else put<false>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
     }
-    if (quads) put<true>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
-    else put<false>(row_of(out, row, width, dtype), dtype, e, 1, width, x);
   }
 }
 
@@ -1008,7 +1007,7 @@ void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const
 }
 inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const Factors* units,
                           const float* unit, float lift, void* out, int64_t rows, int64_t width, int dtype, hipStream_t st) {
-  const int64_t blocks = std::min<int64_t>(cdiv(rows * cdiv(width, 4), NTHREADS), 16384);
+  const int64_t blocks = std::min<int64_t>(cdiv(rows, NWAVES), 16384);
   hipLaunchKernelGGL(xent_finish_kernel, dim3((unsigned)blocks), dim3(NTHREADS), 0, st, sums, splits, split_stride, n_ld, place, units,
                      unit, lift, out, rows, (int)width, dtype);
 }
