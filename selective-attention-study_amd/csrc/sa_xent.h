@@ -22,6 +22,10 @@
 // 2^14: exactly, but for numbers 2^32 times smaller than that, and at the same rate. (With G in bf16 the gradients' error was 1.4 to
 // 1.6 times that of their own rounding; so it is that rounding alone.) The factors and a common g are applied to the
 // fp32 sums; tokens' own g_i (reduction none) to G before it is rounded.
+//
+// Bound by the matrix units and, with all of them busy, by power (1.9 GHz). Measured, 16384 tokens x 50304 x 768 bf16: the forward pass's products
+// 1.2-1.35 ms (0.95-1.05 PFLOP/s with the statistics; torch's own product of that shape 1.13), the backward's eight passes 0.48-0.53
+// each (three products: 0.95-1.0 PFLOP/s), all else 0.12. Few tokens: by the weight's way from HBM (8 tokens 15.8-20 us for 77 MB).
 
 #pragma once
 
