@@ -12,15 +12,16 @@
 //   xent_logits              logits of a tile (vocabulary x tokens: a lane holds one token's, so its maximum and sum are taken in
 //                            registers); a token's maximum, sum and target logit per tile of the vocabulary go to the workspace
 //   xent_join, xent_sum      the tiles' statistics joined: lse, loss; the mean or the sum
-//   xent_logits (again)      backward, a piece of the vocabulary at a time: the tile's logits computed again, G in the products' type
-//   xent_product             dX += G W_piece (fp32 in the workspace across the pieces), dW_piece = G^T X
-//   xent_finish_x, _w        scale, add the parts of a split contraction, convert
+//   xent_factors             backward: what the sums and G are multiplied by
+//   xent_pass                a piece of the vocabulary at a time: the logits computed again, and G of them; beside it the products of
+//                            the piece before, dX += G W_piece (fp32 in the workspace across the pieces), dW_piece = G^T X
+//   xent_finish              the parts of a split contraction added, scaled, converted
 //
 // All products run through one tile loop on matrix instructions with fp32 accumulation (Mainloop). Statistics, lse and losses are
 // fp32. G is rounded to 11 bits: it is held in fp16 at 2^14 times its size (a vocabulary's probabilities lie below that type's normal
 // range), for bf16 operands too, which the backward pass holds in fp16 times the power of two that brings their largest to
 // 2^14: exactly, but for numbers 2^32 times smaller than that, and at the same rate. (With G in bf16 the gradients' error was 1.4 to
-// 1.6 times that of their own rounding; so it is that rounding alone.) The factors and a common g are applied to the
+// 1.6 times that of their own rounding; so it is that rounding's.) The factors and a common g are applied to the
 // fp32 sums; tokens' own g_i (reduction none) to G before it is rounded.
 //
 // Bound by the matrix units and, with all of them busy, by power (1.9 GHz). Measured, 16384 tokens x 50304 x 768 bf16: the forward pass's products
@@ -317,7 +318,12 @@ __device__ __forceinline__ bool tile_of(int64_t id, int mt, int nt, int& m, int&
 inline int64_t tiles_grid(int64_t mt, int64_t nt) { return 8 * cdiv(mt * nt, 8); }
 
 // ---------------------------------------------------------------------------------------------
-// The largest of the workgroup's values (NaN left out), as the workgroup's own number of `maxima`.
+// The larger of two magnitudes, x's if it is a number: an infinity or a NaN has no say in what unit the others are held in.
+__device__ __forceinline__ float larger(float most, float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? fmaxf(most, a) : most;
+}
+// The largest of the workgroup's values, as the workgroup's own number of `maxima`.
 __device__ __forceinline__ void put_maximum(float most, float (&acc)[16], int* maxima, int at) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets,
           if (quads) numbers<true>(q[u], w.dtype, x);
           else numbers<false>(q[u], w.dtype, x);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(x[j]));
+          for (int j = 0; j < 4; ++j) most = larger(most, x[j]);
         }
       }
     }
@@ -435,7 +441,7 @@ __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if constexpr (FIRST) x[j] = stored(x[j], SA_DTYPE_BF16) * by;
-          top = fmaxf(top, fabsf(x[j]));
+          top = larger(top, x[j]);
         }
         put<true>(to + i * padded, OP::CODE, e0 + 256 * u, 1, padded, x);
       }

@@ -470,6 +470,11 @@ def test_linear_cross_entropy_edges(cuda):
     each, _, dx, dw = xent_run(ill, w, t, "none")
     sound = torch.arange(40, device="cuda") != 4
     assert each[4].isnan() and each[sound].isfinite().all() and dx[4].isnan().all() and dx[sound].isfinite().all() and dw.isnan().all()
+    clean = xent_run(x, w, t, "none")
+    ill[4, 0] = math.inf   # (the others' gradients are what they are without it)
+    each, _, dx, dw = xent_run(ill, w, t, "none")
+    assert not each[4].isfinite() and not dx[4].isfinite().any() and torch.equal(each[sound], clean[0][sound])
+    assert torch.equal(dx[sound], clean[2][sound])
     # operands far from 1, of any size that bf16 has: the products' units come back out
     for xs, wscale in ((2.0 ** 60, 2.0 ** -60), (2.0 ** -100, 2.0 ** 95), (2.0 ** -20, 2.0 ** -110), (2.0 ** 30, 0.0)):
         xb, wb = x * xs, w * wscale
@@ -657,3 +662,83 @@ def test_refusals(cuda):
         d, = torch.autograd.grad(f(), leaf, create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(d.sum() + leaf.sum(), leaf)
+
+
+# -- sizes past 32 bits ---------------------------------------------------------------------------------------
+
+def test_layer_norm_past_32_bits(cuda):
+    """Rows behind element 2^31 give what they give alone."""
+    rows, width = (1 << 31) // 1024 + 70, 1024
+    g = torch.Generator(device="cuda").manual_seed(21)
+    x = torch.empty(rows, width, device="cuda", dtype=BF16).normal_(generator=g)
+    branch, w = x.flip(0), (1 + 0.1 * randn(g, width)).bfloat16()
+    leaves = [t.requires_grad_() for t in (x, branch, w)]
+    y, s = sa.add_layer_norm(*leaves)
+    dx, _, dw = torch.autograd.grad((y, s), leaves, (y.detach(), s.detach()))
+    for part in (slice(rows - 90, rows), slice(0, 64)):
+        few = [x.detach()[part].clone().requires_grad_(), branch.detach()[part].clone().requires_grad_(), w]
+        y2, s2 = sa.add_layer_norm(*few)
+        dx2, = torch.autograd.grad((y2, s2), few[0], (y2.detach(), s2.detach()))
+        assert torch.equal(y[part], y2) and torch.equal(s[part], s2) and torch.equal(dx[part], dx2)
+    # dw is a sum over 2^21 rows of about 1: within bf16's own rounding of fp32 sums of 4100 rows' sums each
+    h = torch.zeros(width, dtype=F64, device="cuda")
+    for a in range(0, rows, 1 << 18):
+        part = s.detach()[a:a + (1 << 18)].double()
+        c = part - part.mean(-1, keepdim=True)
+        h += (y.detach()[a:a + (1 << 18)].double() * c / torch.sqrt(c.square().mean(-1, keepdim=True) + 1e-5)).sum(0)
+    assert ((dw.double() - h).abs() <= 2 * half(BF16) * h.abs()).all()
+
+
+def test_embedding_past_32_bits(cuda):
+    vocab, width, tokens = (1 << 31) // 1024 + 3000, 1024, 5000
+    g = torch.Generator(device="cuda").manual_seed(22)
+    w = torch.empty(vocab, width, device="cuda", dtype=BF16).normal_(generator=g).requires_grad_()
+    ids = vocab - 1 - torch.randint(4000, (tokens,), device="cuda", generator=g)
+    dy = randn(g, tokens, width).bfloat16()
+    y = sa.embedding(ids, w)
+    assert torch.equal(y, w.detach()[ids])
+    dw, = torch.autograd.grad(y, w, dy)
+    first = vocab - 4000
+    embed_check(ids - first, w.detach()[first:], 1.0, None, dy, dw[first:])
+    assert (dw[:first] == 0).all()
+
+
+@pytest.mark.parametrize("pull", [20.0, 3.0])
+def test_linear_cross_entropy_past_32_bits(cuda, pull):
+    """A weight of more than 2^31 elements; the words behind that are found, and get their gradient. Targets of weight 1 (pull 20) and of
+    about a hundredth.
+
+    Bounds as in xent_check: G = (p - onehot) / n is off by half a step of it, and by p (2 dl + dlse) / n whatever remains of p - 1."""
+    n, width = 40, 8192
+    vocab = (1 << 31) // width + 900
+    g = torch.Generator(device="cuda").manual_seed(23)
+    w = torch.empty(vocab, width, device="cuda", dtype=BF16).normal_(std=0.02, generator=g)
+    t = vocab - 1 - torch.randint(800, (n,), device="cuda", generator=g)
+    t[:8] = torch.arange(8, device="cuda")
+    x = (randn(g, n, width) + pull * w[t].float()).bfloat16()
+    loss, dloss, dx, dw = xent_run(x, w, t, "mean")
+    parts = [slice(a, a + 16384) for a in range(0, vocab, 16384)]
+    x64 = x.double()
+    l = torch.cat([x64 @ w[p].double().T for p in parts], 1)
+    dl = (width + 2) * U * torch.stack([(x64.abs() @ w[p].double().abs().T).amax(1) for p in parts]).amax(0)
+    lse = torch.logsumexp(l, 1)
+    e_lse = dl + U * (160 + vocab / 1024) + 2.0 ** -22 * (4 + lse.abs())
+    at = torch.arange(n, device="cuda")
+    each = lse - l[at, t]
+    assert abs(loss.double() - each.mean()) <= (dl + e_lse + 5 * U * (lse.abs() + each)).mean()
+    e_G = torch.exp(l - lse[:, None])   # p
+    G = e_G.clone()
+    G[at, t] -= 1.0
+    e_G *= (2 * dl + e_lse)[:, None] * 1.01 + 3 * U
+    e_G += (half(F16) + (vocab + 8) * U) * G.abs() + 2.0 ** -38
+    e_G /= n
+    G /= n
+    for p in (slice(vocab - 900, vocab), slice(0, 300)):
+        want = G[:, p].T @ x64
+        bound = e_G[:, p].T @ x64.abs() + 2.0 ** -38 * x64.abs().max() * G[:, p].abs().sum(0)[:, None]
+        assert_within(dw[p], want, bound * 1.01 + rounding(want, BF16), "dw")
+    want, bound = (torch.zeros(n, width, device="cuda", dtype=F64) for _ in range(2))
+    for p in parts:
+        want += G[:, p] @ w[p].double()
+        bound += e_G[:, p] @ w[p].double().abs()
+    assert_within(dx, want, bound * 1.01 + 2.0 ** -38 * G.abs().sum(1, keepdim=True) + rounding(want, BF16), "dx")
