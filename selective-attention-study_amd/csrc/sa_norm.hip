@@ -13,7 +13,7 @@
 // are added in LDS, and norm_join adds the workgroups' rows of sums in a fixed order. No atomics: equal calls give equal bits.
 //
 // Measured: 16384 x 768, fp32 stream, bf16 branch and result, forward 31 us (4.8 TB/s), backward 44 (4.6 TB/s) and 4 for the join; 2048 x 8192 bf16
-// 46, 38 and 4; 5003 x 1001 fp32 13, 22 and 4. A copy of 4 GiB runs at 4.7 TB/s.
+// 30, 38 and 4; 5003 x 1001 fp32 13, 22 and 4. A copy of 4 GiB runs at 4.7 TB/s.
 
 #include <math.h>
 
@@ -54,13 +54,21 @@ constexpr int norm_threads() { return G == 64 ? NTHREADS : G; }
 template <int G, bool VEC>
 __device__ __forceinline__ int first_of(int v, int lane) { return VEC ? (v * G + lane) * 4 : v * 4 * G + lane; }
 
+// Rows that a workgroup shares: as many workgroups as fit on the chip walk over them with the weights in registers and the next row's
+// loads under way (us, with a workgroup per row: 2048 x 8192 bf16 30, 44; 4096 x 4096 29, 34; up to 2048 wide and for a wavefront's rows
+// there are enough of them on a CU without: 8192 and 16384 x 2048 together 42, 39).
+template <int G, int V>
+constexpr bool norm_walks() { return (G == 256 || G == 512) && V == 4; }
+
 template <int G, int V, bool VEC>
-__global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(NormCall c) {
+__global__ __launch_bounds__(norm_threads<G>(), (norm_walks<G, V>() ? 4 : 1)) void norm_kernel(NormCall c) {
   __shared__ float red[G / 64];
   constexpr int PER = norm_threads<G>() / G;
+  constexpr bool WALK = norm_walks<G, V>();
   const int lane = threadIdx.x % G;
-  for (int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / G; row < c.rows; row += (int64_t)gridDim.x * PER) {
-    Quad qx[V], qb[V];
+  const int64_t stride = (int64_t)gridDim.x * PER;
+  Quad qx[V], qb[V];
+  const auto load = [&](int64_t row) {
     const void* xr = row_of(c.x, row, c.x_ld, c.x_t);
 #pragma unroll
     for (int v = 0; v < V; ++v) qx[v] = fetch<VEC>(xr, c.x_t, first_of<G, VEC>(v, lane), G, c.width);
@@ -69,31 +77,39 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(NormCall c) {
 #pragma unroll
       for (int v = 0; v < V; ++v) qb[v] = fetch<VEC>(br, c.branch_t, first_of<G, VEC>(v, lane), G, c.width);
     }
-    // rows shared by wavefronts wait for each other twice: the weights are asked for before that
-    constexpr bool EARLY = G > 64 && V <= 2;
-    Quad qw[V], qc[V];
-    if constexpr (EARLY) {
+  };
+  int64_t row = (int64_t)blockIdx.x * PER + threadIdx.x / G;
+  float w[V][4], b[V][4];
+  const auto weights = [&](int v) {
+    const int e = first_of<G, VEC>(v, lane);
+    numbers<VEC>(fetch<VEC>(c.w, c.w_t, e, G, c.width), c.w_t, w[v]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        qw[v] = fetch<VEC>(c.w, c.w_t, first_of<G, VEC>(v, lane), G, c.width);
-        if (c.b) qc[v] = fetch<VEC>(c.b, c.w_t, first_of<G, VEC>(v, lane), G, c.width);
-      }
-    }
+    for (int j = 0; j < 4; ++j) b[v][j] = 0.f;
+    if (c.b) numbers<VEC>(fetch<VEC>(c.b, c.w_t, e, G, c.width), c.w_t, b[v]);
+  };
+  if constexpr (WALK) {
+    if (row < c.rows) load(row);
+#pragma unroll
+    for (int v = 0; v < V; ++v) weights(v);
+  }
+  for (; row < c.rows; row += stride) {
+    if constexpr (!WALK) load(row);
     float s[V][4];
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       numbers<VEC>(qx[v], c.x_t, s[v]);
       if (c.branch) {
-        float b[4];
-        numbers<VEC>(qb[v], c.branch_t, b);
+        float d[4];
+        numbers<VEC>(qb[v], c.branch_t, d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[v][j] = stored(s[v][j] + b[j], c.x_t);
+        for (int j = 0; j < 4; ++j) s[v][j] = stored(s[v][j] + d[j], c.x_t);
         put<VEC>(row_of(c.s, row, c.width, c.x_t), c.x_t, first_of<G, VEC>(v, lane), G, c.width, s[v]);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum += s[v][j];
     }
+    if (WALK && row + stride < c.rows) load(row + stride);
     const float mean = row_sum<G>(sum, red) / (float)c.width;
     float square = 0.f;
 #pragma unroll
@@ -109,13 +125,11 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(NormCall c) {
     void* yr = row_of(c.y, row, c.width, c.y_t);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int e = first_of<G, VEC>(v, lane);
-      float w[4], b[4] = {0.f, 0.f, 0.f, 0.f};
-      numbers<VEC>(EARLY ? qw[v] : fetch<VEC>(c.w, c.w_t, e, G, c.width), c.w_t, w);
-      if (c.b) numbers<VEC>(EARLY ? qc[v] : fetch<VEC>(c.b, c.w_t, e, G, c.width), c.w_t, b);
+      if constexpr (!WALK) weights(v);
+      float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = s[v][j] * r * w[j] + b[j];
-      put<VEC>(yr, c.y_t, e, G, c.width, w);
+      for (int j = 0; j < 4; ++j) y[j] = s[v][j] * r * w[v][j] + b[v][j];
+      put<VEC>(yr, c.y_t, first_of<G, VEC>(v, lane), G, c.width, y);
     }
   }
 }
@@ -254,42 +268,30 @@ int64_t norm_parts(int64_t rows, int64_t width) {
   return std::max<int64_t>(1, width <= 1024 ? std::min<int64_t>(512, cdiv(rows, 4)) : std::min<int64_t>(width <= 4096 ? 512 : 256, rows));
 }
 
-// Lanes of a row and quads of a lane by width. The forward takes more lanes than the backward, which keeps three rows' worth of sums and
-// weights in registers: two workgroups on a CU work while others wait for their rows.
+// Lanes of a row and quads of a lane by width.
 template <int G, int V, bool VEC>
-void launch_forward(const NormCall& c, hipStream_t st) {
-  const int64_t blocks = std::min<int64_t>(cdiv(c.rows, norm_threads<G>() / G), LAUNCH_BLOCKS);
-  hipLaunchKernelGGL((norm_kernel<G, V, VEC>), dim3((unsigned)blocks), dim3(norm_threads<G>()), 0, st, c);
-}
-template <int G, int V, bool VEC>
-void launch_backward(const NormCall& c, hipStream_t st) {
-  hipLaunchKernelGGL((norm_backward_kernel<G, V, VEC>), dim3((unsigned)norm_parts(c.rows, c.width)), dim3(norm_threads<G>()), 0, st, c);
+void launch_norm(const NormCall& c, bool backward, hipStream_t st) {
+  const dim3 threads(norm_threads<G>());
+  if (backward) {
+    hipLaunchKernelGGL((norm_backward_kernel<G, V, VEC>), dim3((unsigned)norm_parts(c.rows, c.width)), threads, 0, st, c);
+  } else {
+    const int64_t most = norm_walks<G, V>() ? (int64_t)device_cus() * (1024 / G) : LAUNCH_BLOCKS;
+    const int64_t blocks = std::min<int64_t>(cdiv(c.rows, norm_threads<G>() / G), most);
+    hipLaunchKernelGGL((norm_kernel<G, V, VEC>), dim3((unsigned)blocks), threads, 0, st, c);
+  }
 }
 template <bool VEC>
-void launch_forward(const NormCall& c, hipStream_t st) {
+void launch_norm(const NormCall& c, bool backward, hipStream_t st) {
   const int w = c.width;
-  if (w <= 256) launch_forward<64, 1, VEC>(c, st);
-  else if (w <= 512) launch_forward<64, 2, VEC>(c, st);
-  else if (w <= 768) launch_forward<64, 3, VEC>(c, st);
-  else if (w <= 1024) launch_forward<64, 4, VEC>(c, st);
-  else if (w <= 2048) launch_forward<256, 2, VEC>(c, st);
-  else if (w <= 4096) launch_forward<512, 2, VEC>(c, st);
-  else if (w <= 8192) launch_forward<1024, 2, VEC>(c, st);
-  else if (w <= 16384) launch_forward<1024, 4, VEC>(c, st);
-  else launch_forward<1024, 8, VEC>(c, st);
-}
-template <bool VEC>
-void launch_backward(const NormCall& c, hipStream_t st) {
-  const int w = c.width;
-  if (w <= 256) launch_backward<64, 1, VEC>(c, st);
-  else if (w <= 512) launch_backward<64, 2, VEC>(c, st);
-  else if (w <= 768) launch_backward<64, 3, VEC>(c, st);
-  else if (w <= 1024) launch_backward<64, 4, VEC>(c, st);
-  else if (w <= 2048) launch_backward<256, 2, VEC>(c, st);
-  else if (w <= 4096) launch_backward<256, 4, VEC>(c, st);
-  else if (w <= 8192) launch_backward<512, 4, VEC>(c, st);
-  else if (w <= 16384) launch_backward<1024, 4, VEC>(c, st);
-  else launch_backward<1024, 8, VEC>(c, st);
+  if (w <= 256) launch_norm<64, 1, VEC>(c, backward, st);
+  else if (w <= 512) launch_norm<64, 2, VEC>(c, backward, st);
+  else if (w <= 768) launch_norm<64, 3, VEC>(c, backward, st);
+  else if (w <= 1024) launch_norm<64, 4, VEC>(c, backward, st);
+  else if (w <= 2048) launch_norm<256, 2, VEC>(c, backward, st);
+  else if (w <= 4096) launch_norm<256, 4, VEC>(c, backward, st);
+  else if (w <= 8192) launch_norm<512, 4, VEC>(c, backward, st);
+  else if (w <= 16384) launch_norm<1024, 4, VEC>(c, backward, st);
+  else launch_norm<1024, 8, VEC>(c, backward, st);
 }
 
 bool norm_sizes_ok(int64_t rows, int64_t width) { return rows >= 0 && rows < ((int64_t)1 << 40) && width >= 1 && width <= MAX_WIDTH; }
@@ -319,8 +321,8 @@ int sa_layer_norm(const void* x, int64_t x_ld, const void* branch, int64_t branc
                    quads_ok(weight, 0, weight_dtype) && quads_ok(bias, 0, weight_dtype) && quads_ok(y, width, y_dtype) &&
                    quads_ok(sum, width, x_dtype);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (vec) launch_forward<true>(c, st);
-  else launch_forward<false>(c, st);
+  if (vec) launch_norm<true>(c, false, st);
+  else launch_norm<false>(c, false, st);
   return launch_status();
 }
 
@@ -352,8 +354,8 @@ int sa_layer_norm_backward(const void* s, int64_t s_ld, const void* dy, int64_t 
   const bool vec = width % 4 == 0 && quads_ok(s, s_ld, s_dtype) && quads_ok(dy, dy_ld, y_dtype) && quads_ok(ds, ds_ld, s_dtype) &&
                    quads_ok(weight, 0, weight_dtype) && quads_ok(dx, width, s_dtype) && quads_ok(dbranch, width, c.branch_t);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (vec) launch_backward<true>(c, st);   // (no rows: sums of nothing)
-  else launch_backward<false>(c, st);
+  if (vec) launch_norm<true>(c, true, st);   // (no rows: sums of nothing)
+  else launch_norm<false>(c, true, st);
   if (sums)
     hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)cdiv(width, 64), (unsigned)c.sums), dim3(1024), 0, st, c.part,
                        (int)norm_parts(rows, width), (int)width, dweight, dbias, weight_dtype);
