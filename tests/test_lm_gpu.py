@@ -170,6 +170,13 @@ def test_layer_norm_edges(cuda):
     y, s = sa.add_layer_norm(x[:1], x[:1], w)
     dx, = torch.autograd.grad((y, s), x, (torch.zeros_like(y), torch.ones_like(s)))
     assert (dx[0] == 2).all() and (dx[1:] == 0).all()
+    # two leaves that get the same gradient have it in memory of their own, also where it adds to what is there
+    two = [torch.randn(5, 96, device="cuda", requires_grad=True) for _ in range(2)]
+    for k in (1, 2):
+        y, s = sa.add_layer_norm(*two, w.detach())
+        (y.sum() + 2.0 * s.sum()).backward()
+        assert two[0].grad.data_ptr() != two[1].grad.data_ptr() and torch.equal(two[0].grad, two[1].grad)
+        assert (two[0].grad - 2.0 * k).abs().max() < 1e-4   # (y's rows sum to 0 whatever x is: |u| = 1, rstd < 2, 200 u of it)
     frozen = x[:2].detach()
     dw, = torch.autograd.grad(sa.layer_norm(frozen, w), w, torch.ones(2, 96, device="cuda"))
     assert dw.shape == w.shape
