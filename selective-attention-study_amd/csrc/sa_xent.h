@@ -549,8 +549,9 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
     }
   } else {
     // G of 32 tokens x the wavefront's rows goes through a part of LDS of its own, so that a token's row is stored in
-    // 16-byte pieces side by side. Chunk c of token row r sits at c ^ (r mod 8).
+    // 16-byte pieces side by side. Chunk c of token row r sits at c ^ (r mod 8, or mod as many as there are).
     constexpr int RB = L::TM * 32 * ES;   // bytes of a token's row
+    constexpr int CPR = RB / 16, TURN = CPR < 8 ? CPR - 1 : 7;
     constexpr int FIT = (int)sizeof(s0) / (32 * RB);   // wavefronts' rows in a stage
     static_assert(L::WAVES <= 2 * FIT, "and in two");
     uint8_t* mine = (wave < FIT ? s0.a : s1.a) + wave % FIT * 32 * RB;
@@ -585,14 +586,13 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
             p[r] = row < left ? x : 0.f;
           }
           const int byte = (a * 32 + 8 * q + 4 * h) * ES;
-          put<true>(to + (((byte >> 4) ^ (lane & 7)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
+          put<true>(to + (((byte >> 4) ^ (lane & TURN)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
         }
       __asm__ volatile("" ::: "memory");   // (a wavefront's own LDS accesses run in order)
-      constexpr int CPR = RB / 16;
 #pragma unroll
       for (int k = 0; k < 32 * CPR / 64; ++k) {
         const int slot = k * 64 + lane, r = slot / CPR, ch = slot % CPR;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ((ch ^ (r & 7)) << 4));
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ((ch ^ (r & TURN)) << 4));
         __builtin_amdgcn_raw_buffer_store_b128(v, rs, r * g_row + ch * 16, (wn * L::TN + b) * 32 * g_row, 0);
       }
       __asm__ volatile("" ::: "memory");
@@ -820,16 +820,21 @@ struct PassCall {
 };
 template <class OP, class LG, class LX, class LW>
 __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass_kernel(PassCall c) {
-  __shared__ typename LG::Stage s0, s1, s2, s3;
+  typedef typename std::conditional<(sizeof(typename LW::Stage) > sizeof(typename LG::Stage)), typename LW::Stage, typename LG::Stage>::type S;
+  static_assert(sizeof(typename LX::Stage) <= sizeof(S) && LG::THREADS == LX::THREADS && LG::THREADS == LW::THREADS, "one launch for all");
+  __shared__ S s0, s1, s2, s3;
   const int id = blockIdx.x;
   if (id >= c.x_at && id < c.x_end) {
     const int part = uniform((id - c.x_at) / c.x_tiles);
-    product_tile<OP, LX, false>(c.x, id - c.x_at - part * c.x_tiles, part, s0, s1, s2, s3);
+    typedef typename LX::Stage X;
+    product_tile<OP, LX, false>(c.x, id - c.x_at - part * c.x_tiles, part, (X&)s0, (X&)s1, (X&)s2, (X&)s3);
   } else if (id >= c.w_at && id < c.w_end) {
     const int part = uniform((id - c.w_at) / c.w_tiles);
-    product_tile<OP, LW, true>(c.w, id - c.w_at - part * c.w_tiles, part, s0, s1, s2, s3);
+    typedef typename LW::Stage W;
+    product_tile<OP, LW, true>(c.w, id - c.w_at - part * c.w_tiles, part, (W&)s0, (W&)s1, (W&)s2, (W&)s3);
   } else {
-    logits_tile<OP, LG, true>(c.g, id - c.g_at, s0, s1, s2, s3);
+    typedef typename LG::Stage G;
+    logits_tile<OP, LG, true>(c.g, id - c.g_at, (G&)s0, (G&)s1, (G&)s2, (G&)s3);
   }
 }
 
@@ -845,6 +850,7 @@ __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums
     for (int e = 4 * lane; e < width; e += 256) {
       float x[4] = {0.f, 0.f, 0.f, 0.f};
       if (at >= 0) {
+#pragma unroll 8
         for (int s = 0; s < splits; ++s) {
           const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + at * n_ld + e);
           x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
@@ -868,6 +874,7 @@ struct XentConfigs {   // 16-bit products
   typedef Mainloop<OP, 4, 1, 1, 2, false, false> Small;   // 128 x 64
   typedef Mainloop<OP, 2, 4, 4, 2, false, true> LargeX;
   typedef Mainloop<OP, 2, 2, 2, 2, false, true> MiddleX;
+  typedef Mainloop<OP, 2, 2, 1, 2, false, true> SmallX;   // 64 x 128
   typedef Mainloop<OP, 2, 4, 4, 2, true, true> LargeW;
   typedef Mainloop<OP, 2, 2, 2, 2, true, true> MiddleW;
 };
@@ -878,11 +885,15 @@ struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per st
   typedef Mainloop<XF32, 4, 1, 1, 2, false, false> Small;
   typedef Mainloop<XF32, 2, 2, 2, 2, false, true> LargeX;
   typedef Mainloop<XF32, 2, 2, 2, 2, false, true> MiddleX;
+  typedef Mainloop<XF32, 2, 2, 1, 2, false, true> SmallX;
   typedef Mainloop<XF32, 2, 2, 2, 2, true, true> LargeW;
   typedef Mainloop<XF32, 2, 2, 2, 2, true, true> MiddleW;
 };
 
-constexpr int64_t SMALL_TOKENS = 64;      // one tile's tokens of the smallest kernel (8 tokens x 50304 x 768, weight out of HBM: 20.0 us, 21.5 by 128 x 128)
+// One tile's tokens of the smallest kernels. Us by 128 x 64 / 128 x 128: 8 tokens x 50304 x 768, no gradient, weight out of HBM 20.0 / 21.5; training,
+// forward and backward: fp32 64 x 50304 x 768 67 / 109 and 183 / 323, fp16 33 x 32000 x 2048 40 / 42 and 122 / 140, bf16 64 x 50304 x 768
+// 56 / 58 and 122 / 118.
+constexpr int64_t SMALL_TOKENS = 64;
 constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are (250 tokens 40 us, listed and gathered 47)
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of a piece's G, of which there are two at a time
 constexpr int64_t JOIN_FEW = 1024;        // tokens up to which the join takes 64 lanes for each (calls, us, 64 / 8 lanes: 1000 tokens 110 / 112, 4096 345 / 340)
@@ -905,7 +916,7 @@ struct XentShape {
   XentShape(const XentCall& c, bool backward, bool scaled = false) {
     train = c.lse != nullptr;
     padded = align_up(c.width, BK);
-    small = c.tokens <= SMALL_TOKENS && !train;
+    small = c.tokens <= SMALL_TOKENS;
     // Tiles of 256 x 256 where every CU has one and the last tokens' are not mostly empty (four wavefronts' of 128 x 128 else).
     // Forward, us, large / middle, tokens x words x 768: 400 x 50304 58 / 64, 1000 x 16384 40 / 47, 2000 x 50304 183 / 197; 128 x 50304
     // 27 / 25 (197 tiles), 300 x 33000 54 / 42 (212 of the second 256 tokens missing).
@@ -953,10 +964,15 @@ struct XentShape {
       const int64_t products = (c.dx ? tiles(edge, c.tokens, c.width) * k_x : 0) + (c.dw ? tiles(edge, piece, c.width) * k_w : 0);
       const int64_t share = cdiv(products + (pieces > 1 ? tiles(edge, c.tokens, piece) * (k_g + 8) : products / 2), slots);
       const int64_t share_last = std::max<int64_t>(cdiv(products, 2 * slots), 1);
-      const auto parts = [](int64_t stages, int64_t of) { return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(stages, of), stages / 8, 16})); };
-      splits_x = parts(k_x, pieces > 1 ? cdiv(share, 2) : 2 * share_last);
-      splits_w = parts(k_w, share);
-      splits_last = parts(k_w, 2 * share_last);
+      const auto parts = [](int64_t stages, int64_t of, int64_t most) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(stages, of), stages / 8, most}));
+      };
+      // A part more costs dX's sums once more through memory: up to 64 parts where they take no more than 32 MB, 16 at least (few tokens have
+      // few tiles and long contractions; with the smallest tiles, fp32 3 x 68497 x 768 430 -> 242 us, 5 x 68536 x 128 311 -> 119).
+      const int64_t most_x = std::min<int64_t>(std::max<int64_t>(((int64_t)32 << 20) / (c.tokens * padded * 4), 16), 64);
+      splits_x = parts(k_x, pieces > 1 ? cdiv(share, 2) : 2 * share_last, most_x);
+      splits_w = parts(k_w, share, 16);
+      splits_last = parts(k_w, 2 * share_last, 16);
       // (a part's rows lie within 2^30 bytes)
       const int64_t w_row = (copy_w ? padded : c.w_ld) * ES, x_row = std::max(padded, piece) * ES;
       splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
@@ -1111,8 +1127,9 @@ int xent_backward(const XentCall& c) {
     }
     const LogitsCall* pg = p < s.pieces ? &g : nullptr;
     const ProductCall *x = p > 0 && c.dx ? &px : nullptr, *y = p > 0 && c.dw ? &pw : nullptr;
-    if (!(s.large_pass ? launch_pass<OP, typename F::Large, typename F::LargeX, typename F::LargeW>(pg, x, y, c.tokens, c.st)
-                       : launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st)))
+    if (!(s.small        ? launch_pass<OP, typename F::Small, typename F::SmallX, typename F::MiddleW>(pg, x, y, c.tokens, c.st)
+          : s.large_pass ? launch_pass<OP, typename F::Large, typename F::LargeX, typename F::LargeW>(pg, x, y, c.tokens, c.st)
+                         : launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st)))
       return SA_ERR_ARGUMENT;
     if (y && pw.splits > 1)
       launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t, c.st);
