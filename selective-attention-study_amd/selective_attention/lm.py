@@ -16,6 +16,7 @@ Each has a gradient but no second derivative.
 The `_reference` functions are the same in plain torch, on any device.
 """
 
+import math
 from typing import Optional
 
 import torch
@@ -360,6 +361,8 @@ def _xent_impl(x: Tensor, weight: Tensor, targets: Tensor, ignore: int, reductio
     loss = torch.empty((tokens,) if none else (), device=device, dtype=torch.float32)
     lse = torch.empty(2, tokens, device=device, dtype=torch.float32) if train else None
     rows = torch.empty(_lib.XENT_ROWS + 2 * tokens, device=device, dtype=torch.int32)
+    if tokens == 0:   # (a mean, or a sum, of nothing; no gradient reads the rest)
+        return loss.fill_(math.nan if reduction == _lib.REDUCTIONS["mean"] else 0.0), lse, rows if train else None
     x_code, w_code, x_ptr, w_ptr = _CODES[x.dtype], _CODES[weight.dtype], x.data_ptr(), weight.data_ptr()
     size = _sized(device, lib.sa_linear_xent_workspace_bytes, x_ptr, x_ld, w_ptr, w_ld, tokens, vocab, width, reduction, train, x_code,
                   w_code, code)
@@ -394,6 +397,8 @@ def _xent_backward_impl(x: Tensor, weight: Tensor, targets: Tensor, lse: Tensor,
     lib = _lib.load()
     dx = _empty(x, x.dtype) if need_x else None
     dweight = _empty(weight, weight.dtype) if need_weight else None
+    if tokens == 0:
+        return dx, dweight.zero_() if need_weight else None
     x, x_ld = _rows(x, width)
     weight, w_ld = _rows(weight, width)
     targets, dloss = targets.contiguous(), _vector(dloss)
@@ -481,9 +486,6 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, ignore_inde
     tokens = targets.numel()
     if width > MAX_HEAD_WIDTH or tokens >= 1 << 28 or vocab >= 1 << 28 or -(-tokens // 128) * -(-vocab // 128) >= 1 << 23:
         raise ValueError(f"{tokens} tokens of {width} columns over {vocab} words are too many for one call")
-    if tokens == 0:   # (nothing to sum; the gradients are zeros)
-        nothing = x.float().sum() + 0.0 * weight[:1].float().sum()
-        return x.float().sum(-1) if reduction == "none" else nothing * 0.0 if reduction == "sum" else nothing * float("nan")
     flat, targets = x.reshape(tokens, width), targets.reshape(tokens)
     if _wants_grad(x, weight):
         loss = _LinearCrossEntropyFn.apply(flat, weight, targets, ignore, code, operands)

@@ -1,0 +1,37 @@
+"""Edges of the operators around the attention layers on the GPU: batches without a token, gradients of very different sizes and
+infinite ones, a word with all the weight, 16-bit views, operands and rows of probabilities past 2^31 bytes, forward-mode derivatives.
+
+U, half and the bounds are test_lm_gpu's."""
+
+import math
+
+import pytest
+import torch
+
+import selective_attention as sa
+from test_lm_gpu import BF16, F16, F32
+
+pytestmark = pytest.mark.gpu
+
+THREE = pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=lambda t: str(t)[6:])
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("shape", [(0,), (0, 5), (3, 0)], ids=str)
+@THREE
+def test_no_tokens(cuda, reduction, shape, dtype):
+    """A batch without a token: the loss of no terms, gradients of zeros of either tensor or both, whatever weight holds."""
+    for first in (1.0, math.inf, math.nan):
+        w = torch.ones(7, 16, device="cuda", dtype=dtype)
+        w[0] = first
+        x, t = torch.empty(*shape, 16, device="cuda", dtype=dtype), torch.empty(shape, device="cuda", dtype=torch.int64)
+        scored = sa.linear_cross_entropy(x, w, t, reduction=reduction)
+        for need in ((True, True), (True, False), (False, True)):
+            x, w = x.detach().requires_grad_(need[0]), w.detach().requires_grad_(need[1])
+            loss = sa.linear_cross_entropy(x, w, t, reduction=reduction)
+            for each in (loss, scored):
+                assert each.dtype is F32 and each.shape == (shape if reduction == "none" else ())
+                assert each.isnan() if reduction == "mean" else (each == 0).all()
+            leaves = [a for a, n in zip((x, w), need) if n]
+            for a, d in zip(leaves, torch.autograd.grad(loss, leaves, torch.full_like(loss, 2.0))):
+                assert d.shape == a.shape and d.dtype is dtype and (d == 0).all()
