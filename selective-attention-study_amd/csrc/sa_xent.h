@@ -676,7 +676,7 @@ __global__ __launch_bounds__(1024) void xent_sum_kernel(const float* sums, int n
 // ---------------------------------------------------------------------------------------------
 // The backward pass's factors. w and x: the units weight and x are held in, powers of two, from_w and from_x back from them; g multiplies the sums of
 // both products. factor[i] (reduction none): of the kept token's row of G before it is rounded, g_i relative to the power of two at or below the
-// largest |g|, which g then is. So a row is rounded once, as with one g for all; the entries of rows whose g is less
+// largest |g| that is a number, which g then is. So a row is rounded once, as with one g for all; the entries of rows whose g is less
 // than 2^-10 of the largest lose their last bits.
 __device__ __forceinline__ uint32_t exponent_of(float x) { return (__float_as_uint(x) >> 23) & 0xff; }
 __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, const int* rows, int reduction, bool scaled, Factors* out,
@@ -703,7 +703,7 @@ __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, 
     g = tokens == 0 ? 0.f : reduction == SA_REDUCE_MEAN ? dloss[0] / (float)tokens : dloss[0];
   } else {
     float most = 0.f;
-    for (int i = threadIdx.x; i < tokens; i += 1024) most = fmaxf(most, fabsf(dloss[rows[ROWS_HEAD + i]]));
+    for (int i = threadIdx.x; i < tokens; i += 1024) most = larger(most, dloss[rows[ROWS_HEAD + i]]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
     if (lane == 0) acc[wave] = most;

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import selective_attention as sa
-from test_lm_gpu import BF16, F16, F32
+from test_lm_gpu import BF16, F16, F32, randn, xent_inputs, xent_run
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,20 @@ def test_no_tokens(cuda, reduction, shape, dtype):
             leaves = [a for a, n in zip((x, w), need) if n]
             for a, d in zip(leaves, torch.autograd.grad(loss, leaves, torch.full_like(loss, 2.0))):
                 assert d.shape == a.shape and d.dtype is dtype and (d == 0).all()
+
+
+@THREE
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan], ids=str)
+def test_a_gradient_that_is_no_number(cuda, dtype, bad):
+    """One token's incoming gradient is an infinity or a NaN: its own dx and all of dW are none either, the other tokens' dx keep their bits."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    x, w, t = xent_inputs(g, 70, 400, 64, dtype, dtype)
+    dloss = randn(g, 70)
+    dloss[3], dloss[4] = 4.0, 0.25   # (the largest is another's)
+    clean = xent_run(x, w, t, "none", dloss)
+    dloss = dloss.clone()
+    dloss[4] = bad
+    loss, _, dx, dw = xent_run(x, w, t, "none", dloss)
+    sound = torch.arange(70, device="cuda") != 4
+    assert torch.equal(loss, clean[0]) and torch.equal(dx[sound], clean[2][sound])
+    assert not dx[4].isfinite().any() and not dw.isfinite().any()
