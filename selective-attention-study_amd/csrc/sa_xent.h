@@ -117,8 +117,10 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ lds_void_ptr lds_at(const void* p) { return (lds_void_ptr)(uint32_t)(uintptr_t)p; }
 // element i of a 32 x 32 accumulator: column lane % 32, row acc_row(i, lane / 32)
 __device__ __forceinline__ constexpr int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_t bytes) {   // loads past `bytes` give zero
-  const int64_t most = 0x7fffffff;
+// Loads past `bytes` give zero; so does any at PAST or behind it, however much there is (what a tile means to read lies below).
+constexpr int PAST = 0x7fffff00;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_t bytes) {
+  const int64_t most = PAST;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)(bytes < 0 ? 0 : bytes < most ? bytes : most), 0x00020000);
 }
 
@@ -181,7 +183,7 @@ struct Operand {
         }
         soff = (k * BK + r0) * ld;
       }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(to + 1024 * n), 16, voff, k < last ? soff : 0x7fffff00, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, lds_at(to + 1024 * n), 16, voff, k < last ? soff : PAST, 0, 0);
     }
   }
   // the fragment of step j (two per stage) of rows (columns) first .. first + 31

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import selective_attention as sa
-from test_lm_gpu import BF16, F16, F32, randn, xent_inputs, xent_run
+from test_lm_gpu import BF16, F16, F32, randn, xent_check, xent_inputs, xent_run
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,21 @@ def test_a_gradient_that_is_no_number(cuda, dtype, bad):
     sound = torch.arange(70, device="cuda") != 4
     assert torch.equal(loss, clean[0]) and torch.equal(dx[sound], clean[2][sound])
     assert not dx[4].isfinite().any() and not dw.isfinite().any()
+
+
+@pytest.mark.parametrize("dtype,width", [(BF16, 96), (F32, 48)], ids=["bf16", "f32"])
+def test_tokens_past_31_bits(cuda, dtype, width):
+    """More than 2^31 bytes of rows, whose contraction is no multiple of the loop's four stages: the stages behind it read nothing, so that the NaN
+    of a token 2^31 - 256 bytes behind the first reaches no other."""
+    n, row = (1 << 31) // 192 + 1000, 192   # bytes
+    g = torch.Generator(device="cuda").manual_seed(35)
+    x = torch.empty(n, width, device="cuda", dtype=dtype).normal_(generator=g)
+    ill = torch.tensor([0x7fffff00 // row, (0x7fffff00 + 63) // row], device="cuda").unique()
+    x[ill] = math.nan
+    w, t = randn(g, 40, width).to(dtype), torch.randint(40, (n,), device="cuda", generator=g)
+    each = sa.linear_cross_entropy(x, w, t, reduction="none")
+    sound = torch.ones(n, device="cuda", dtype=torch.bool)
+    sound[ill] = False
+    assert each[ill].isnan().all() and each[sound].isfinite().all()
+    for part in (slice(0, 300), slice(n - 300, n)):
+        xent_check(x[part], w, t[part], "none", dtype, each[part])
