@@ -899,7 +899,7 @@ constexpr int64_t SMALL_TOKENS = 64;
 constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are (250 tokens 40 us, listed and gathered 47)
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of a piece's G, of which there are two at a time
 constexpr int64_t JOIN_FEW = 1024;        // tokens up to which the join takes 64 lanes for each (calls, us, 64 / 8 lanes: 1000 tokens 110 / 112, 4096 345 / 340)
-constexpr int64_t MAX_LD_BYTES = 1 << 22;             // 256 rows within a buffer resource's 2 GiB
+constexpr int64_t MAX_LD_BYTES = 1 << 22;             // of a row: 256 within a buffer resource's 2 GiB, their offsets within 31 bits
 
 // What a call does, from its sizes alone.
 template <class OP>
@@ -947,8 +947,8 @@ struct XentShape {
       at = take(c.tokens * 4);
       sums = take(join_blocks * 4);
     } else {
-      // Pieces of the vocabulary whose G fits PIECE_BYTES, in whole tiles, of about one size
-      const int64_t most = std::max<int64_t>(PIECE_BYTES / (c.tokens * ES) / 256 * 256, 256);
+      // Pieces of the vocabulary whose G fits PIECE_BYTES (and a token's row of it MAX_LD_BYTES), in whole tiles, of about one size
+      const int64_t most = std::max<int64_t>(std::min(PIECE_BYTES / (c.tokens * ES), MAX_LD_BYTES / ES) / 256 * 256, 256);
       pieces = cdiv(c.vocab, most);
       piece = align_up(cdiv(c.vocab, pieces), 256);
       pieces = cdiv(c.vocab, piece);

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import selective_attention as sa
-from test_lm_gpu import BF16, F16, F32, randn, xent_check, xent_inputs, xent_run
+from test_lm_gpu import BF16, F16, F32, F64, U, assert_within, half, randn, rounding, xent_check, xent_inputs, xent_run
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,39 @@ def test_tokens_past_31_bits(cuda, dtype, width):
     assert each[ill].isnan().all() and each[sound].isfinite().all()
     for part in (slice(0, 300), slice(n - 300, n)):
         xent_check(x[part], w, t[part], "none", dtype, each[part])
+
+
+def test_words_past_26_bits(cuda):
+    """Two tokens over more than 2^26 words, whose rows of G are longer than 2^27 bytes: in pieces, each of which lies within a tile's offsets."""
+    n, vocab, width = 2, (1 << 26) + 70000, 32
+    g = torch.Generator(device="cuda").manual_seed(36)
+    w = torch.empty(vocab, width, device="cuda", dtype=F16).normal_(generator=g)
+    t = torch.tensor([vocab - 5, 12345], device="cuda")
+    x = randn(g, n, width).half()
+    loss, _, dx, dw = xent_run(x, w, t, "sum")
+    parts = [slice(a, min(a + (1 << 22), vocab)) for a in range(0, vocab, 1 << 22)]
+    x64 = x.double()
+    l = torch.cat([x64 @ w[p].double().T for p in parts], 1)
+    dl = (width + 2) * U * torch.stack([(x64.abs() @ w[p].double().abs().T).amax(1) for p in parts]).amax(0)
+    lse = torch.logsumexp(l, 1)
+    e_lse = dl + U * (160 + vocab / 1024) + 2.0 ** -22 * (4 + lse.abs())
+    at = torch.arange(n, device="cuda")
+    each = lse - l[at, t]
+    assert abs(loss.double() - each.sum()) <= (dl + e_lse + 5 * U * (lse.abs() + each)).sum()
+    p_all = torch.exp(l - lse[:, None])
+    del l
+    want, bound = (torch.zeros(n, width, device="cuda", dtype=F64) for _ in range(2))
+    for part in parts:
+        p = p_all[:, part]
+        G = p.clone()
+        for i in range(n):
+            if part.start <= int(t[i]) < part.stop:
+                G[i, int(t[i]) - part.start] -= 1.0
+        e_G = (half(F16) + U) * G.abs() + p * (2 * dl + e_lse)[:, None] * 1.01 + 3 * U * p + 2.0 ** -38
+        w64 = w[part].double()
+        dw_part = G.T @ x64
+        assert_within(dw[part], dw_part, (e_G + (n + 8) * U * G.abs()).T @ x64.abs() * 1.01 + rounding(dw_part, F16), "dw")
+        want += G @ w64
+        # (a piece of the vocabulary has at most 2^21 words, and there are 33 of up to 64 parts)
+        bound += (e_G + ((1 << 21) + 100) * U * G.abs()) @ w64.abs()
+    assert_within(dx, want, bound * 1.01 + rounding(want, F16), "dx")
