@@ -526,12 +526,15 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, l.acc[a][b][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float ref = mx == -INFINITY ? 0.f : mx * LOG2E;   // (nothing but -inf: a sum of zeros, not of NaN)
+      // (Nothing but -inf: a sum of zeros, not of NaN. The difference is taken before the factor: as l LOG2E - round(mx LOG2E) in one instruction the
+      // largest's own term is not 1, and a loss of 0 comes out off by up to 2^-24 of its logit, either way. What it costs: 16384 x 50304 x
+      // 768 bf16 1230 -> 1241 us, 4096 x 50304 x 256 153 -> 157.)
+      const float ref = mx == -INFINITY ? 0.f : mx;
       float s = 0.f;
 #pragma unroll
       for (int a = 0; a < L::TM; ++a)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(fmaf(l.acc[a][b][r], LOG2E, -ref));
+        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((l.acc[a][b][r] - ref) * LOG2E);
       s += __shfl_xor(s, 32);
       if (h == 0) top[wm * L::BN + col] = mx, sum[wm * L::BN + col] = s;
     }

@@ -54,6 +54,26 @@ def test_a_gradient_that_is_no_number(cuda, dtype, bad):
     assert not dx[4].isfinite().any() and not dw.isfinite().any()
 
 
+@pytest.mark.parametrize("n", [20, 200, 600])
+@pytest.mark.parametrize("dtype,far", [(BF16, 1.0), (F16, 1.0), (F32, 1.0), (BF16, 2.0 ** 116), (F32, 2.0 ** 116)], ids=str)
+def test_a_word_with_all_the_weight(cuda, dtype, n, far):
+    """The target's logit is 60 to 4000 (or near the end of fp32's range) and the others' are 25 or more below it: the loss is 0 but for 700 e^-25 <
+    2^-26, and never below 0. The largest's own term of the sum is 1 and the others' do not change it; the gradient is at most that of
+    the target's row, a step of 2^-23 in its probability, and of the others'."""
+    g = torch.Generator(device="cuda").manual_seed(33)
+    w = randn(g, 700, 256).sign() / 16   # (rows of norm 1; two have a product of at most 0.5)
+    assert (w @ w.T - torch.eye(700, device="cuda")).max() < 0.5
+    t = torch.randint(700, (n,), device="cuda", generator=g)
+    x = (far * torch.randint(60, 4000, (n, 1), device="cuda", generator=g) * w[t]).to(dtype)   # (sums of 256 equal numbers: exact)
+    x[0] = (far * 4000 * w[t[0]]).to(dtype)
+    w = w.to(dtype)
+    loss, _, dx, dw = xent_run(x, w, t, "none", torch.ones(n, device="cuda"))
+    for each in (loss, sa.linear_cross_entropy(x, w, t, reduction="none")):
+        assert (each >= 0).all() and each.max() <= 2.0 ** -23
+    assert dx.abs().max() <= 2.0 ** -22 / 16
+    assert 0 <= sa.linear_cross_entropy(x, w, t) <= 2.0 ** -23
+
+
 @pytest.mark.parametrize("dtype,width", [(BF16, 96), (F32, 48)], ids=["bf16", "f32"])
 def test_tokens_past_31_bits(cuda, dtype, width):
     """More than 2^31 bytes of rows, whose contraction is no multiple of the loop's four stages: the stages behind it read nothing, so that the NaN
