@@ -22,7 +22,8 @@
 // range), for bf16 operands too, which the backward pass holds in fp16 times the power of two that brings their largest to
 // 2^14: exactly, but for numbers 2^32 times smaller than that, and at the same rate. (With G in bf16 the gradients' error was 1.4 to
 // 1.6 times that of their own rounding; so it is that rounding's.) The factors and a common g are applied to the
-// fp32 sums; tokens' own g_i (reduction none) to G before it is rounded.
+// fp32 sums. Tokens' own g_i (reduction none): G_i takes g_i over the power of two below it before it is rounded, the sum dx_i that power; dW
+// sums over tokens, so it reads a second copy of x whose rows have their powers (16-bit types; fp32 puts all of g_i into G_i).
 //
 // Bound by the matrix units and, with all of them busy, by power (1.9 GHz). Measured, 16384 tokens x 50304 x 768 bf16: the forward pass's products
 // 1.2-1.35 ms (0.95-1.05 PFLOP/s with the statistics; torch's own product of that shape 1.13), the backward's eight passes 0.48-0.53
@@ -415,12 +416,18 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets,
   if (threadIdx.x == 0) rows[0] = base;
 }
 
+struct Factors {   // xent_factors_kernel
+  float g, w, x, rows, from_w, from_x, from_rows;
+};
+
 // Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i]; FIRST: rounded to bf16 first and
-// taken *unit times. maxima: each workgroup's largest magnitude (MAXIMA workgroups then).
+// taken *unit times. maxima: each workgroup's largest magnitude (MAXIMA workgroups then). also: the same rows units->rows times, and times the row's
+// power over the largest number's (a row whose power is above that is none).
 template <class OP, bool FIRST>
 __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
                                                                const int* count, int64_t most, const float* unit, int* maxima,
-                                                               typename OP::elem* to, int padded) {
+                                                               typename OP::elem* to, int padded, typename OP::elem* also,
+                                                               const float* power, const Factors* units) {
   __shared__ float acc[16];
   const int64_t rows = count ? *count : most;
   const int lane = threadIdx.x & 63;
@@ -430,6 +437,7 @@ __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int
   constexpr int AHEAD = 4;   // loads in flight: a wavefront's of a row
   for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 64) + wave_index(); i < rows; i += (int64_t)gridDim.x * (blockDim.x / 64)) {
     const void* row = row_of(from, numbers_of ? numbers_of[i] : i, ld, dtype);
+    const float again = also ? fminf(power[i] / units->g, 1.f) * units->rows : 0.f;
     for (int e0 = 4 * lane; e0 < padded; e0 += 256 * AHEAD) {
       Quad q[AHEAD];
 #pragma unroll
@@ -440,12 +448,16 @@ __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int
         float x[4];
         if (quads) numbers<true>(q[u], dtype, x);
         else numbers<false>(q[u], dtype, x);
+        float y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if constexpr (FIRST) x[j] = stored(x[j], SA_DTYPE_BF16) * by;
+          if constexpr (FIRST) x[j] = stored(x[j], SA_DTYPE_BF16);
+          y[j] = x[j] * again;
+          if constexpr (FIRST) x[j] *= by;
           top = larger(top, x[j]);
         }
         put<true>(to + i * padded, OP::CODE, e0 + 256 * u, 1, padded, x);
+        if (also) put<true>(also + i * padded, OP::CODE, e0 + 256 * u, 1, padded, y);
       }
     }
   }
@@ -454,10 +466,6 @@ __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int
 
 // ---------------------------------------------------------------------------------------------
 // Logits of a tile: rows of the vocabulary (M) x tokens (N).
-
-struct Factors {   // xent_factors_kernel
-  float g, w, x, from_w, from_x;
-};
 
 struct LogitsCall {
   const void *w, *x;
@@ -679,18 +687,20 @@ __global__ __launch_bounds__(1024) void xent_sum_kernel(const float* sums, int n
 }
 
 // ---------------------------------------------------------------------------------------------
-// The backward pass's factors. w and x: the units weight and x are held in, powers of two, from_w and from_x back from them; g multiplies the sums of
-// both products. factor[i] (reduction none): of the kept token's row of G before it is rounded, g_i relative to the power of two at or below the
-// largest |g| that is a number, which g then is. So a row is rounded once, as with one g for all; the entries of rows whose g is less
-// than 2^-10 of the largest lose their last bits.
+// The backward pass's factors. w and x: the units weight and x are held in, powers of two (`scaled`), from_w and from_x back from them; rows and
+// from_rows: of the x that dW's products read, where that is a copy of its own. g multiplies the sums of both products.
+// Reduction none: g is the power of two at or below the largest |g_i| that is a number, for dW's sums. With `power` that at or below each kept
+// token's own |g_i| goes there, for its dX, and g_i over it to `factor`, for its row of G before it is rounded: so G_i has all its bits
+// whatever the others are (with one unit for all a row of 1e-8 of the largest was off by 1.8%). Without (fp32's range needs none)
+// factor is g_i / g.
 __device__ __forceinline__ uint32_t exponent_of(float x) { return (__float_as_uint(x) >> 23) & 0xff; }
 __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, const int* rows, int reduction, bool scaled, Factors* out,
-                                                            float* factor) {
+                                                            float* factor, float* power) {
   __shared__ float acc[16], maxima[2];
   const int tokens = rows[0];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (scaled) {
-    float most = __uint_as_float((uint32_t)rows[64 + threadIdx.x]);   // half of the threads of either matrix
+  if (scaled || power) {   // half of the threads look at either matrix's largest magnitudes
+    float most = scaled || threadIdx.x >= MAXIMA ? __uint_as_float((uint32_t)rows[64 + threadIdx.x]) : 0.f;
 #pragma unroll
     for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
     if (lane == 0) acc[wave] = most;
@@ -703,6 +713,7 @@ __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, 
     __syncthreads();
   }
   static_assert(MAXIMA == 512, "half of the threads");
+  const auto below = [](float x) { return __uint_as_float(min(max(exponent_of(x), 1u), 254u) << 23); };   // a power of two
   float g;
   if (!factor) {   // (no token kept: gradients of zeros, not 0 / 0)
     g = tokens == 0 ? 0.f : reduction == SA_REDUCE_MEAN ? dloss[0] / (float)tokens : dloss[0];
@@ -714,20 +725,25 @@ __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, 
     if (lane == 0) acc[wave] = most;
     __syncthreads();
     for (int w = 0; w < 16; ++w) most = fmaxf(most, acc[w]);
-    g = __uint_as_float(min(max(exponent_of(most), 1u), 253u) << 23);
-    for (int i = threadIdx.x; i < tokens; i += 1024) factor[i] = dloss[rows[ROWS_HEAD + i]] / g;
+    g = below(most);
+    for (int i = threadIdx.x; i < tokens; i += 1024) {
+      const float mine = dloss[rows[ROWS_HEAD + i]], to = power ? below(mine) : g;
+      factor[i] = mine / to;
+      if (power) power[i] = to;
+    }
   }
   if (threadIdx.x) return;
-  Factors f{g, 1.f, 1.f, 1.f, 1.f};
-  if (scaled) {   // the largest comes to 2^14 .. 2^15; nothing but zeros stays as it is
-    const auto unit = [](float most, float& to, float& from) {
-      const int e = most == 0.f ? 0 : min(14 - ((int)exponent_of(most) - 127), 126);
-      to = __uint_as_float((uint32_t)(127 + e) << 23);
-      from = __uint_as_float((uint32_t)(127 - e) << 23);
-    };
+  Factors f{g, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+  const auto unit = [](float most, float& to, float& from) {   // the largest comes to 2^14 .. 2^15; nothing but zeros stays as it is
+    const int e = most == 0.f ? 0 : min(14 - ((int)exponent_of(most) - 127), 126);
+    to = __uint_as_float((uint32_t)(127 + e) << 23);
+    from = __uint_as_float((uint32_t)(127 - e) << 23);
+  };
+  if (scaled) {
     unit(maxima[0], f.w, f.from_w);
     unit(maxima[1], f.x, f.from_x);
   }
+  if (scaled || power) unit(maxima[1], f.rows, f.from_rows);
   *out = f;
 }
 
@@ -780,7 +796,7 @@ __device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, i
   if (!c.out) base = (uint8_t*)(c.sums + ((int64_t)part * c.m_rows + m0) * ld);
   const __amdgpu_buffer_rsrc_t rs = resource(base, min(M - m0, (int64_t)L::BM) * ld * es);
   // (the unit last and alone: with g it may leave fp32's range)
-  const float scale = c.out ? c.units->g * c.lift : 1.f, unit = c.out ? c.units->from_x : 1.f;
+  const float scale = c.out ? c.units->g * c.lift : 1.f, unit = c.out ? c.units->from_rows : 1.f;
   const int row_bytes = (int)ld * es;
   const auto each = [&](auto&& put_sixteen) {
 #pragma unroll
@@ -843,15 +859,16 @@ __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass
   }
 }
 
-// dX: a token's parts added, times its factor; zero rows for the tokens that are ignored. dW: the parts of a piece's rows.
+// dX: a token's parts added, times g or its own power; zero rows for the tokens that are ignored. dW: the parts of a piece's rows.
 __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums, int splits, int64_t split_stride, int64_t n_ld,
                                                                const int* place, const Factors* units, const float* unit, float lift,
-                                                               void* out, int64_t rows, int width, int dtype) {
+                                                               const float* power, void* out, int64_t rows, int width, int dtype) {
   const int lane = threadIdx.x & 63;
   const bool quads = width % 4 == 0;
-  const float f = units->g * lift, u = *unit;
+  const float u = *unit;
   for (int64_t row = (int64_t)blockIdx.x * NWAVES + wave_index(); row < rows; row += (int64_t)gridDim.x * NWAVES) {
     const int64_t at = place ? place[row] : row;
+    const float f = (power && at >= 0 ? power[at] : units->g) * lift;
     for (int e = 4 * lane; e < width; e += 256) {
       float x[4] = {0.f, 0.f, 0.f, 0.f};
       if (at >= 0) {
@@ -915,7 +932,7 @@ struct XentShape {
   bool large_pass;
   int splits_x, splits_w, splits_last;   // parts of dX's contraction, of dW's, and of that in the last pass
   // workspace
-  int64_t x, w, top, sum, at, sums, factors, g, g2, dx, dw, total;
+  int64_t x, w, top, sum, at, sums, factors, rows, g, g2, dx, dw, total;
 
   // scaled: bf16 operands held in fp16, copies both
   XentShape(const XentCall& c, bool backward, bool scaled = false) {
@@ -983,7 +1000,8 @@ struct XentShape {
       splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
       splits_w = std::max(splits_w, (int)cdiv(c.tokens * x_row, (int64_t)1 << 30));
       splits_last = std::max(splits_last, splits_w);
-      factors = take((c.tokens + 64) * 4);
+      factors = take((2 * c.tokens + 64) * 4);
+      rows = take(c.dw && ES == 2 ? c.tokens * padded * ES : 0);   // (the query of its size does not know the reduction)
       g = take(c.tokens * piece * ES);
       g2 = take(pieces > 1 ? c.tokens * piece * ES : 0);
       dx = take(c.dx ? splits_x * c.tokens * padded * 4 : 0);
@@ -1031,16 +1049,18 @@ bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
 }
 template <class OP, bool FIRST = false>
 void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows,
-                   const float* unit, int* maxima, void* to, int64_t padded, hipStream_t st) {
+                   const float* unit, int* maxima, void* to, int64_t padded, hipStream_t st, void* also = nullptr,
+                   const float* power = nullptr, const Factors* units = nullptr) {
   const int64_t blocks = maxima ? MAXIMA : std::min<int64_t>(cdiv(rows, NWAVES), 16384);
   hipLaunchKernelGGL((xent_gather_kernel<OP, FIRST>), dim3((unsigned)blocks), dim3(maxima ? 1024 : NTHREADS), 0, st, from, ld, dtype, (int)width,
-                     numbers_of, count, rows, unit, maxima, (typename OP::elem*)to, (int)padded);
+                     numbers_of, count, rows, unit, maxima, (typename OP::elem*)to, (int)padded, (typename OP::elem*)also, power, units);
 }
 inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const Factors* units,
-                          const float* unit, float lift, void* out, int64_t rows, int64_t width, int dtype, hipStream_t st) {
+                          const float* unit, float lift, const float* power, void* out, int64_t rows, int64_t width, int dtype,
+                          hipStream_t st) {
   const int64_t blocks = std::min<int64_t>(cdiv(rows, NWAVES), 16384);
   hipLaunchKernelGGL(xent_finish_kernel, dim3((unsigned)blocks), dim3(NTHREADS), 0, st, sums, splits, split_stride, n_ld, place, units,
-                     unit, lift, out, rows, (int)width, dtype);
+                     unit, lift, power, out, rows, (int)width, dtype);
 }
 
 template <class OP>
@@ -1059,8 +1079,9 @@ int xent_forward(const XentCall& c) {
   lc.tokens = c.tokens;
   lc.vocab = c.vocab;
   if (s.gather) {
-    const bool maxima = s.train && !std::is_same<OP, typename OP::Back>::value;
-    hipLaunchKernelGGL(xent_rows_kernel, dim3(maxima ? 1 + MAXIMA : 1), dim3(1024), 0, c.st, c.targets, c.tokens, c.ignore, c.rows, each,
+    const bool scaled = s.train && !std::is_same<OP, typename OP::Back>::value;
+    const bool maxima = scaled || (s.train && s.ES == 2 && each);   // of x
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(scaled ? 1 + MAXIMA : 1), dim3(1024), 0, c.st, c.targets, c.tokens, c.ignore, c.rows, each,
                        Matrix{c.w, c.w_ld, c.vocab, (int)c.width, c.w_t});
     lc.rows = c.rows;
     launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, maxima ? c.rows + 64 + MAXIMA : nullptr,
@@ -1102,8 +1123,11 @@ int xent_backward(const XentCall& c) {
   char* ws = (char*)c.ws;
   Factors* units = (Factors*)(ws + s.factors);
   float* factor = c.reduction == SA_REDUCE_NONE ? (float*)units + 64 : nullptr;
-  hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, SCALED, units, factor);
-  launch_gather<OP, SCALED>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, &units->x, nullptr, ws + s.x, s.padded, c.st);
+  float* power = factor && ES == 2 ? factor + c.tokens : nullptr;
+  void* rows = power && c.dw ? ws + s.rows : nullptr;   // the x that dW reads
+  hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, SCALED, units, factor, power);
+  launch_gather<OP, SCALED>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, &units->x, nullptr, ws + s.x, s.padded, c.st,
+                            rows, power, units);
   const void* w = c.w;
   int64_t w_ld = c.w_ld;
   if (s.copy_w) {
@@ -1125,7 +1149,7 @@ int xent_backward(const XentCall& c) {
       px.a = pw.a = ws + (p & 1 ? s.g : s.g2), px.a_ld = pw.a_ld = s.piece, px.rows = pw.rows = c.rows;
       px.b = (const char*)w + v0 * w_ld * ES, px.b_ld = w_ld, px.n = px.b_cols = s.padded, px.k = v1 - v0;
       px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = c.tokens, px.add = p > 1;
-      pw.b = ws + s.x, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
+      pw.b = rows ? rows : ws + s.x, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
       pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / OP::LIFT, pw.units = units;
       if (pw.splits == 1) pw.out = out, pw.out_ld = c.width, pw.out_t = c.w_t;
       else pw.sums = (float*)(ws + s.dw), pw.n_ld = s.padded, pw.m_rows = s.piece;
@@ -1137,11 +1161,11 @@ int xent_backward(const XentCall& c) {
                          : launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st)))
       return SA_ERR_ARGUMENT;
     if (y && pw.splits > 1)
-      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / OP::LIFT, out, v1 - v0, c.width, c.w_t, c.st);
+      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_rows, 1.f / OP::LIFT, nullptr, out, v1 - v0, c.width, c.w_t, c.st);
   }
   if (c.dx)
     launch_finish((float*)(ws + s.dx), s.splits_x, c.tokens * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, units, &units->from_w,
-                  1.f / OP::LIFT, c.dx, c.tokens, c.width, c.x_t, c.st);
+                  1.f / OP::LIFT, power, c.dx, c.tokens, c.width, c.x_t, c.st);
   return launch_status();
 }
 

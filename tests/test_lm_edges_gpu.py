@@ -54,6 +54,44 @@ def test_a_gradient_that_is_no_number(cuda, dtype, bad):
     assert not dx[4].isfinite().any() and not dw.isfinite().any()
 
 
+@THREE
+@pytest.mark.parametrize("n,vocab,width", [(50, 3001, 96), (300, 700, 200)])
+def test_gradients_of_very_different_sizes(cuda, dtype, n, vocab, width):
+    """Tokens' incoming gradients from 1 down to 1e-12, and 0: every row of dx is as exact as it is alone.
+
+    As in xent_check, with each token's own f in the place of the largest: G_i = (p - onehot) f is held at 2^14 times its size beside the power of two
+    at or below f_i, so its entries are off by half a step of fp16, or by 2^-39 of that power below fp16's normal numbers. In dW the rest of f_i is on
+    the rows of x, the largest at 2^14: those are off by 2^-39 of the largest x f / (factor below 2) where they fall below fp16's normal numbers."""
+    g = torch.Generator(device="cuda").manual_seed(32)
+    x, w, t = xent_inputs(g, n, vocab, width, dtype, dtype)
+    f = torch.pow(10.0, -12 * torch.rand(n, device="cuda", generator=g)) * torch.where(torch.rand(n, device="cuda", generator=g) < 0.5, -1.0, 1.0)
+    f[0], f[1], f[2], f[3] = 1.0, 1e-12, 0.0, -1e-9
+    _, _, dx, dw = xent_run(x, w, t, "none", f)
+    x64, w64, f64 = x.double(), w.double(), f.double()
+    l = x64 @ w64.T
+    dl = (width + 2) * U * (x64.abs() @ w64.abs().T).amax(1)
+    lse = torch.logsumexp(l, 1)
+    e_lse = dl + U * (160 + vocab / 1024) + 2.0 ** -22 * (4 + lse.abs())
+    p = torch.exp(l - lse[:, None])
+    G = p.clone()
+    G[torch.arange(n, device="cuda"), t] -= 1.0
+    fine, tiny = (0.0, 0.0) if dtype is F32 else (half(F16), 2.0 ** -38)
+    e_G = (fine + U) * G.abs() + p * (2 * dl + e_lse)[:, None] * 1.01 + 3 * U * p + tiny
+    size = f64.abs()[:, None]
+    want = f64[:, None] * (G @ w64)
+    bound = ((e_G + (vocab + 8) * U * G.abs()) * size) @ w64.abs()
+    if dtype is BF16:
+        bound += 2.0 ** -38 * w64.abs().max() * (size * G.abs()).sum(1, keepdim=True)
+    assert (dx[2] == 0).all()
+    assert_within(dx, want, bound * 1.01 + rounding(want, dtype), "dx")
+    want = (f64[:, None] * G).T @ x64
+    bound = ((e_G + (n + 8) * U * G.abs()) * size).T @ x64.abs() + tiny * x64.abs().max() * G.abs().sum(0)[:, None]
+    assert_within(dw, want, bound * 1.01 + rounding(want, dtype), "dw")
+    other = f.clone()
+    other[::2] *= 1e7
+    assert torch.equal(xent_run(x, w, t, "none", other)[2][1::2], dx[1::2])
+
+
 @pytest.mark.parametrize("n", [20, 200, 600])
 @pytest.mark.parametrize("dtype,far", [(BF16, 1.0), (F16, 1.0), (F32, 1.0), (BF16, 2.0 ** 116), (F32, 2.0 ** 116)], ids=str)
 def test_a_word_with_all_the_weight(cuda, dtype, n, far):
