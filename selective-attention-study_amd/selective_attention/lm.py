@@ -11,7 +11,7 @@ its own where the docstring does not tie them together; arithmetic, statistics a
 equal bits. The calls allocate from torch's caching allocator and launch on the current stream of their tensors' device, so
 they can be captured into a graph, backward passes too. (As with any operator, capture a backward pass on leaves that no
 eager graph still holds: torch accumulates into a leaf on the stream that first used it, and a capture cannot wait for another stream.)
-Each has a gradient but no second derivative.
+Each has a gradient; second derivatives, forward-mode ones and torch.func's transforms raise.
 
 The `_reference` functions are the same in plain torch, on any device.
 """
@@ -20,6 +20,7 @@ import math
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch import Tensor
 
 from . import _lib
@@ -62,7 +63,9 @@ def _vector(x: Tensor) -> Tensor:
 
 
 def _wants_grad(*tensors: Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether the call goes through its autograd function: one of the tensors wants a gradient, or may have a forward-mode tangent, which
+    the function refuses and the op would drop."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or forward_ad._current_level >= 0
 
 
 def _ptr(t: Tensor | None):

@@ -7,6 +7,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import selective_attention as sa
 from test_lm_gpu import BF16, F16, F32, F64, U, assert_within, half, randn, rounding, xent_check, xent_inputs, xent_run
@@ -164,3 +165,22 @@ def test_words_past_26_bits(cuda):
         # (a piece of the vocabulary has at most 2^21 words, and there are 33 of up to 64 parts)
         bound += (e_G + ((1 << 21) + 100) * U * G.abs()) @ w64.abs()
     assert_within(dx, want, bound * 1.01 + rounding(want, F16), "dx")
+
+
+def test_forward_mode_derivatives_are_refused(cuda):
+    """The operators have no forward-mode derivative and no batching rule, and say so: a tangent is not dropped."""
+    x, w = torch.randn(4, 8, device="cuda"), torch.randn(8, device="cuda")
+    ids = torch.tensor([1, 0, 3, 2], device="cuda")
+    calls = (lambda v: sa.layer_norm(v, w), lambda v: sa.add_layer_norm(x, v, w)[0], lambda v: sa.layer_norm(x, w, v[0]),
+             lambda v: sa.embedding(ids, v), lambda v: sa.linear_cross_entropy(v, x, ids), lambda v: sa.linear_cross_entropy(x, v, ids))
+    with forward_ad.dual_level():
+        for call in calls:
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    call(forward_ad.make_dual(x, torch.ones_like(x)))
+            call(x)   # (without a tangent there is nothing to refuse)
+    for call in calls:
+        for transformed in (lambda: torch.func.jvp(call, (x,), (torch.ones_like(x),)), lambda: torch.func.grad(lambda v: call(v).sum())(x),
+                            lambda: torch.func.vmap(call)(x.expand(3, 4, 8))):
+            with pytest.raises(RuntimeError):
+                transformed()
