@@ -113,6 +113,27 @@ def test_a_word_with_all_the_weight(cuda, dtype, n, far):
     assert 0 <= sa.linear_cross_entropy(x, w, t) <= 2.0 ** -23
 
 
+VIEWS = {"columns": ((40, 200), lambda b: b[:, 64:128]), "offset": ((40, 65), lambda b: b[:, 1:]), "wide": ((40, 192), lambda b: b[:, 128:]),
+         "every second": ((80, 64), lambda b: b[::2]), "one row": ((1, 64), lambda b: b.expand(40, 64)),
+         "transposed": ((64, 40), lambda b: b.T)}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("xv", VIEWS)
+@pytest.mark.parametrize("wv", VIEWS)
+def test_sixteen_bit_views(cuda, dtype, xv, wv):
+    """Views of 16-bit tensors: rows read in place a stride apart, rows of odd alignment, one row for all."""
+    g = torch.Generator(device="cuda").manual_seed(34)
+    x, w = (view(randn(g, *(s if i == 0 else tuple(2 * e if e in (40, 80) else e for e in s))).to(dtype))
+            for i, (s, view) in enumerate((VIEWS[xv], VIEWS[wv])))
+    assert not x.is_contiguous() and not w.is_contiguous() and x.shape[1] == w.shape[1] == 64
+    t = torch.randint(w.shape[0], (40,), device="cuda", generator=g)
+    t[::7] = -100
+    loss, dloss, dx, dw = xent_run(x, w, t, "mean")
+    xent_check(x, w, t, "mean", dtype, loss, dloss, dx, dw)
+    xent_check(x, w, t, "none", dtype, sa.linear_cross_entropy(x, w, t, reduction="none"))
+
+
 @pytest.mark.parametrize("dtype,width", [(BF16, 96), (F32, 48)], ids=["bf16", "f32"])
 def test_tokens_past_31_bits(cuda, dtype, width):
     """More than 2^31 bytes of rows, whose contraction is no multiple of the loop's four stages: the stages behind it read nothing, so that the NaN
