@@ -18,12 +18,13 @@
 //   xent_finish              the parts of a split contraction added, scaled, converted
 //
 // All products run through one tile loop on matrix instructions with fp32 accumulation (Mainloop). Statistics, lse and losses are
-// fp32. G is rounded to 11 bits: it is held in fp16 at 2^14 times its size (a vocabulary's probabilities lie below that type's normal
-// range), for bf16 operands too, which the backward pass holds in fp16 times the power of two that brings their largest to
-// 2^14: exactly, but for numbers 2^32 times smaller than that, and at the same rate. (With G in bf16 the gradients' error was 1.4 to
-// 1.6 times that of their own rounding; so it is that rounding's.) The factors and a common g are applied to the
-// fp32 sums. Tokens' own g_i (reduction none): G_i takes g_i over the power of two below it before it is rounded, the sum dx_i that power; dW
-// sums over tokens, so it reads a second copy of x whose rows have their powers (16-bit types; fp32 puts all of g_i into G_i).
+// fp32. Both passes take the logits from the same operands, so that the probabilities are the forward's whatever the rows hold. G is rounded to
+// 11 bits: it is held in fp16 at 2^14 times its size (a vocabulary's probabilities lie below that type's normal range). Its products with bf16
+// operands hold these in fp16 too, times the power of two that brings their largest to 2^14: exactly, but for numbers 2^31 times smaller
+// than that, which are off by 2^-39 of it, and at the same rate. (With G in bf16 the gradients' error was 1.4 to 1.6 times that of their own
+// rounding; so it is that rounding's.) The factors and a common g are applied to the fp32 sums. Tokens' own g_i (reduction none): G_i takes
+// g_i over the power of two below it before it is rounded, the sum dx_i that power; dW sums over tokens, so it reads a copy of x whose rows have their
+// powers (16-bit types; fp32 puts all of g_i into G_i).
 //
 // Bound by the matrix units and, with all of them busy, by power (1.9 GHz). Measured, 16384 tokens x 50304 x 768 bf16: the forward pass's products
 // 1.2-1.35 ms (0.95-1.05 PFLOP/s with the statistics; torch's own product of that shape 1.13), the backward's eight passes 0.48-0.53
@@ -85,7 +86,7 @@ static_assert(ROWS_HEAD == SA_XENT_ROWS, "as the header says");
 struct XF16;
 struct XBF16 {
   typedef uint16_t elem;
-  typedef XF16 Back;   // the backward pass's operands
+  typedef XF16 Back;   // what G is held in, and what it is multiplied with
   static constexpr int CODE = SA_DTYPE_BF16;
   static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -417,27 +418,25 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const int64_t* targets,
 }
 
 struct Factors {   // xent_factors_kernel
-  float g, w, x, rows, from_w, from_x, from_rows;
+  float g, w, x, from_w, from_x;
 };
 
-// Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i]; FIRST: rounded to bf16 first and
-// taken *unit times. maxima: each workgroup's largest magnitude (MAXIMA workgroups then). also: the same rows units->rows times, and times the row's
-// power over the largest number's (a row whose power is above that is none).
-template <class OP, bool FIRST>
+// Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i], where `to` is not null. maxima: each workgroup's largest
+// magnitude (MAXIMA workgroups then). also (null: none): the same rows, rounded to that type first, in the type that G is held in and *unit times; with
+// `power` also times the row's power over *g, the largest number's (a row whose power is above that is none).
+template <class OP>
 __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
-                                                               const int* count, int64_t most, const float* unit, int* maxima,
-                                                               typename OP::elem* to, int padded, typename OP::elem* also,
-                                                               const float* power, const Factors* units) {
+                                                           const int* count, int64_t most, int* maxima, typename OP::elem* to, int padded,
+                                                           typename OP::Back::elem* also, const float* unit, const float* power, const float* g) {
   __shared__ float acc[16];
   const int64_t rows = count ? *count : most;
   const int lane = threadIdx.x & 63;
   const bool quads = ((uintptr_t)from % (dtype == SA_DTYPE_F32 ? 16 : 8)) == 0 && ld % 4 == 0 && width % 4 == 0;
-  const float by = FIRST ? *unit : 1.f;
   float top = 0.f;
   constexpr int AHEAD = 4;   // loads in flight: a wavefront's of a row
   for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 64) + wave_index(); i < rows; i += (int64_t)gridDim.x * (blockDim.x / 64)) {
     const void* row = row_of(from, numbers_of ? numbers_of[i] : i, ld, dtype);
-    const float again = also ? fminf(power[i] / units->g, 1.f) * units->rows : 0.f;
+    const float by = !also ? 0.f : power ? fminf(power[i] / *g, 1.f) * *unit : *unit;
     for (int e0 = 4 * lane; e0 < padded; e0 += 256 * AHEAD) {
       Quad q[AHEAD];
 #pragma unroll
@@ -448,16 +447,13 @@ __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int
         float x[4];
         if (quads) numbers<true>(q[u], dtype, x);
         else numbers<false>(q[u], dtype, x);
-        float y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (FIRST) x[j] = stored(x[j], SA_DTYPE_BF16);
-          y[j] = x[j] * again;
-          if constexpr (FIRST) x[j] *= by;
-          top = larger(top, x[j]);
-        }
-        put<true>(to + i * padded, OP::CODE, e0 + 256 * u, 1, padded, x);
-        if (also) put<true>(also + i * padded, OP::CODE, e0 + 256 * u, 1, padded, y);
+        for (int j = 0; j < 4; ++j) top = larger(top, x[j]);
+        if (to) put<true>(to + i * padded, OP::CODE, e0 + 256 * u, 1, padded, x);
+        if (!also) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = stored(x[j], OP::CODE) * by;
+        put<true>(also + i * padded, OP::Back::CODE, e0 + 256 * u, 1, padded, x);
       }
     }
   }
@@ -479,11 +475,11 @@ struct LogitsCall {
   float *top, *sum, *at;    // (mt, tokens) statistics, the targets' logits
   const float* lse;         // backward: XentCall's
   const float* factor;      // backward: of each kept token's row of G; null: 1
-  const Factors* units;     // backward
   void* g;                  // (tokens, g_ld)
   int64_t g_ld;
 };
 
+// (OP: what G is held in, of as many bits as the operands)
 template <class OP, class L, bool GRAD>
 __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typename L::Stage& s0, typename L::Stage& s1,
                                             typename L::Stage& s2, typename L::Stage& s3) {
@@ -572,7 +568,6 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
     const int g_row = (int)(c.g_ld * ES);
     const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES);
     const int left = edge ? (int)(c.v1 - vw) : L::TM * 32;   // rows of the vocabulary
-    const Factors units = *c.units;   // (multiplied by one after the other: their product may leave fp32's range)
 #pragma unroll 1
     for (int b = 0; b < L::TN; ++b) {
       const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
@@ -594,7 +589,7 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
             float x = l.acc[a][0][4 * q + r];
 #pragma unroll
             for (int o = 1; o < L::TN; ++o) x = b == o ? l.acc[a][o][4 * q + r] : x;
-            x = __builtin_amdgcn_exp2f(fmaf(x * units.from_w, units.from_x, -top) * LOG2E) * over;
+            x = __builtin_amdgcn_exp2f((x - top) * LOG2E) * over;
             x = tl == row ? x - lift : x;
             p[r] = row < left ? x : 0.f;
           }
@@ -687,8 +682,8 @@ __global__ __launch_bounds__(1024) void xent_sum_kernel(const float* sums, int n
 }
 
 // ---------------------------------------------------------------------------------------------
-// The backward pass's factors. w and x: the units weight and x are held in, powers of two (`scaled`), from_w and from_x back from them; rows and
-// from_rows: of the x that dW's products read, where that is a copy of its own. g multiplies the sums of both products.
+// The backward pass's factors. w and x: the units that the products with G hold weight and x in, powers of two (`scaled`; x's with `power`, too),
+// from_w and from_x back from them. g multiplies the sums of both products.
 // Reduction none: g is the power of two at or below the largest |g_i| that is a number, for dW's sums. With `power` that at or below each kept
 // token's own |g_i| goes there, for its dX, and g_i over it to `factor`, for its row of G before it is rounded: so G_i has all its bits
 // whatever the others are (with one unit for all a row of 1e-8 of the largest was off by 1.8%). Without (fp32's range needs none)
@@ -733,17 +728,14 @@ __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, 
     }
   }
   if (threadIdx.x) return;
-  Factors f{g, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+  Factors f{g, 1.f, 1.f, 1.f, 1.f};
   const auto unit = [](float most, float& to, float& from) {   // the largest comes to 2^14 .. 2^15; nothing but zeros stays as it is
     const int e = most == 0.f ? 0 : min(14 - ((int)exponent_of(most) - 127), 126);
     to = __uint_as_float((uint32_t)(127 + e) << 23);
     from = __uint_as_float((uint32_t)(127 - e) << 23);
   };
-  if (scaled) {
-    unit(maxima[0], f.w, f.from_w);
-    unit(maxima[1], f.x, f.from_x);
-  }
-  if (scaled || power) unit(maxima[1], f.rows, f.from_rows);
+  if (scaled) unit(maxima[0], f.w, f.from_w);
+  if (scaled || power) unit(maxima[1], f.x, f.from_x);
   *out = f;
 }
 
@@ -796,7 +788,7 @@ __device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, i
   if (!c.out) base = (uint8_t*)(c.sums + ((int64_t)part * c.m_rows + m0) * ld);
   const __amdgpu_buffer_rsrc_t rs = resource(base, min(M - m0, (int64_t)L::BM) * ld * es);
   // (the unit last and alone: with g it may leave fp32's range)
-  const float scale = c.out ? c.units->g * c.lift : 1.f, unit = c.out ? c.units->from_rows : 1.f;
+  const float scale = c.out ? c.units->g * c.lift : 1.f, unit = c.out ? c.units->from_x : 1.f;
   const int row_bytes = (int)ld * es;
   const auto each = [&](auto&& put_sixteen) {
 #pragma unroll
@@ -925,6 +917,7 @@ constexpr int64_t MAX_LD_BYTES = 1 << 22;             // of a row: 256 within a 
 template <class OP>
 struct XentShape {
   static constexpr int ES = sizeof(typename OP::elem), BK = KB / ES;
+  static constexpr bool SCALED = !std::is_same<OP, typename OP::Back>::value;   // weight and x have copies for the products with G
   bool train, small, large, gather, copy_w;
   int64_t padded, bm, mt, join_tokens, join_blocks;
   // backward
@@ -932,10 +925,9 @@ struct XentShape {
   bool large_pass;
   int splits_x, splits_w, splits_last;   // parts of dX's contraction, of dW's, and of that in the last pass
   // workspace
-  int64_t x, w, top, sum, at, sums, factors, rows, g, g2, dx, dw, total;
+  int64_t x, w, top, sum, at, sums, factors, x_back, w_back, g, g2, dx, dw, total;
 
-  // scaled: bf16 operands held in fp16, copies both
-  XentShape(const XentCall& c, bool backward, bool scaled = false) {
+  XentShape(const XentCall& c, bool backward) {
     train = c.lse != nullptr;
     padded = align_up(c.width, BK);
     small = c.tokens <= SMALL_TOKENS;
@@ -949,7 +941,7 @@ struct XentShape {
     const bool x_ok = c.x_t == OP::CODE && padded == c.width && (uintptr_t)c.x % 16 == 0 && c.x_ld * ES % 16 == 0 &&
                       c.x_ld >= c.width && c.x_ld * ES < MAX_LD_BYTES;
     gather = train || c.reduction != SA_REDUCE_NONE || c.tokens > IN_PLACE_TOKENS || !x_ok;
-    copy_w = scaled || !(c.w_t == OP::CODE && padded == c.width && (uintptr_t)c.w % 16 == 0 && c.w_ld * ES % 16 == 0 &&
+    copy_w = !(c.w_t == OP::CODE && padded == c.width && (uintptr_t)c.w % 16 == 0 && c.w_ld * ES % 16 == 0 &&
                c.w_ld >= c.width && c.w_ld * ES < MAX_LD_BYTES);
     join_tokens = c.tokens <= JOIN_FEW ? 4 : 32;
     join_blocks = std::min<int64_t>(cdiv(c.tokens, join_tokens), 4096);
@@ -996,12 +988,13 @@ struct XentShape {
       splits_w = parts(k_w, share, 16);
       splits_last = parts(k_w, 2 * share_last, 16);
       // (a part's rows lie within 2^30 bytes)
-      const int64_t w_row = (copy_w ? padded : c.w_ld) * ES, x_row = std::max(padded, piece) * ES;
+      const int64_t w_row = (SCALED || copy_w ? padded : c.w_ld) * ES, x_row = std::max(padded, piece) * ES;
       splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
       splits_w = std::max(splits_w, (int)cdiv(c.tokens * x_row, (int64_t)1 << 30));
       splits_last = std::max(splits_last, splits_w);
       factors = take((2 * c.tokens + 64) * 4);
-      rows = take(c.dw && ES == 2 ? c.tokens * padded * ES : 0);   // (the query of its size does not know the reduction)
+      x_back = take(c.dw && ES == 2 ? c.tokens * padded * ES : 0);   // (fp16: with reduction none alone, which the query of the size does not know)
+      w_back = take(c.dx && SCALED ? c.vocab * padded * ES : 0);
       g = take(c.tokens * piece * ES);
       g2 = take(pieces > 1 ? c.tokens * piece * ES : 0);
       dx = take(c.dx ? splits_x * c.tokens * padded * 4 : 0);
@@ -1047,13 +1040,13 @@ bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
   hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
   return true;
 }
-template <class OP, bool FIRST = false>
-void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows,
-                   const float* unit, int* maxima, void* to, int64_t padded, hipStream_t st, void* also = nullptr,
-                   const float* power = nullptr, const Factors* units = nullptr) {
+template <class OP>
+void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows, int* maxima,
+                   void* to, int64_t padded, hipStream_t st, void* also = nullptr, const float* unit = nullptr, const float* power = nullptr,
+                   const float* g = nullptr) {
   const int64_t blocks = maxima ? MAXIMA : std::min<int64_t>(cdiv(rows, NWAVES), 16384);
-  hipLaunchKernelGGL((xent_gather_kernel<OP, FIRST>), dim3((unsigned)blocks), dim3(maxima ? 1024 : NTHREADS), 0, st, from, ld, dtype, (int)width,
-                     numbers_of, count, rows, unit, maxima, (typename OP::elem*)to, (int)padded, (typename OP::elem*)also, power, units);
+  hipLaunchKernelGGL((xent_gather_kernel<OP>), dim3((unsigned)blocks), dim3(maxima ? 1024 : NTHREADS), 0, st, from, ld, dtype, (int)width,
+                     numbers_of, count, rows, maxima, (typename OP::elem*)to, (int)padded, (typename OP::Back::elem*)also, unit, power, g);
 }
 inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const Factors* units,
                           const float* unit, float lift, const float* power, void* out, int64_t rows, int64_t width, int dtype,
@@ -1065,7 +1058,7 @@ inline void launch_finish(const float* sums, int splits, int64_t split_stride, i
 
 template <class OP>
 int64_t xent_bytes(const XentCall& c, bool backward) {
-  return backward ? XentShape<typename OP::Back>(c, true, !std::is_same<OP, typename OP::Back>::value).total : XentShape<OP>(c, false).total;
+  return XentShape<OP>(c, backward).total;
 }
 
 template <class OP>
@@ -1079,19 +1072,19 @@ int xent_forward(const XentCall& c) {
   lc.tokens = c.tokens;
   lc.vocab = c.vocab;
   if (s.gather) {
-    const bool scaled = s.train && !std::is_same<OP, typename OP::Back>::value;
+    const bool scaled = s.train && s.SCALED;
     const bool maxima = scaled || (s.train && s.ES == 2 && each);   // of x
     hipLaunchKernelGGL(xent_rows_kernel, dim3(scaled ? 1 + MAXIMA : 1), dim3(1024), 0, c.st, c.targets, c.tokens, c.ignore, c.rows, each,
                        Matrix{c.w, c.w_ld, c.vocab, (int)c.width, c.w_t});
     lc.rows = c.rows;
-    launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, maxima ? c.rows + 64 + MAXIMA : nullptr,
+    launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, maxima ? c.rows + 64 + MAXIMA : nullptr,
                       ws + s.x, s.padded, c.st);
     lc.x = ws + s.x, lc.x_ld = s.padded;
   } else {
     lc.x = c.x, lc.x_ld = c.x_ld;
   }
   if (s.copy_w) {
-    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, nullptr, ws + s.w, s.padded, c.st);
+    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, ws + s.w, s.padded, c.st);
     lc.w = ws + s.w, lc.w_ld = s.padded;
   } else {
     lc.w = c.w, lc.w_ld = c.w_ld;
@@ -1113,59 +1106,59 @@ int xent_forward(const XentCall& c) {
   return launch_status();
 }
 
-template <class FROM>
+template <class OP>
 int xent_backward(const XentCall& c) {
-  typedef typename FROM::Back OP;
+  typedef typename OP::Back BACK;
   typedef XentConfigs<OP> F;
-  constexpr int ES = sizeof(typename OP::elem);
-  constexpr bool SCALED = !std::is_same<FROM, OP>::value;
-  const XentShape<OP> s(c, true, SCALED);
+  typedef XentConfigs<BACK> B;
+  constexpr int ES = sizeof(typename BACK::elem);
+  const XentShape<OP> s(c, true);
   char* ws = (char*)c.ws;
   Factors* units = (Factors*)(ws + s.factors);
   float* factor = c.reduction == SA_REDUCE_NONE ? (float*)units + 64 : nullptr;
   float* power = factor && ES == 2 ? factor + c.tokens : nullptr;
-  void* rows = power && c.dw ? ws + s.rows : nullptr;   // the x that dW reads
-  hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, SCALED, units, factor, power);
-  launch_gather<OP, SCALED>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, &units->x, nullptr, ws + s.x, s.padded, c.st,
-                            rows, power, units);
-  const void* w = c.w;
-  int64_t w_ld = c.w_ld;
-  if (s.copy_w) {
-    launch_gather<OP, SCALED>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, &units->w, nullptr, ws + s.w, s.padded, c.st);
-    w = ws + s.w, w_ld = s.padded;
-  }
+  hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, s.SCALED, units, factor, power);
+  const char* x_back = ws + (s.SCALED || power ? s.x_back : s.x);   // dW's
+  launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, ws + s.x, s.padded, c.st,
+                    c.dw && (s.SCALED || power) ? ws + s.x_back : nullptr, &units->x, power, &units->g);
+  const char *w = s.copy_w ? ws + s.w : (const char*)c.w, *w_back = s.SCALED ? ws + s.w_back : w;   // dX's
+  const int64_t w_ld = s.copy_w ? s.padded : c.w_ld, w_back_ld = s.SCALED ? s.padded : w_ld;
+  void* const scaled_w = s.SCALED && c.dx ? ws + s.w_back : nullptr;
+  if (s.copy_w || scaled_w)
+    launch_gather<OP>(c.w, c.w_ld, c.w_t, c.width, nullptr, nullptr, c.vocab, nullptr, s.copy_w ? ws + s.w : nullptr, s.padded, c.st, scaled_w,
+                      &units->w);
   // pass p: G of piece p, and the products of piece p - 1
   for (int64_t p = 0; p <= s.pieces; ++p) {
     LogitsCall g{};
     if (p < s.pieces) {
       g.w = w, g.w_ld = w_ld, g.x = ws + s.x, g.x_ld = s.padded, g.targets = c.targets, g.rows = c.rows, g.tokens = c.tokens;
       g.vocab = c.vocab, g.v0 = p * s.piece, g.v1 = std::min(g.v0 + s.piece, c.vocab), g.stages = (int)(s.padded / s.BK);
-      g.lse = c.lse, g.factor = factor, g.units = units, g.g = ws + (p & 1 ? s.g2 : s.g), g.g_ld = s.piece;
+      g.lse = c.lse, g.factor = factor, g.g = ws + (p & 1 ? s.g2 : s.g), g.g_ld = s.piece;
     }
     ProductCall px{}, pw{};
     const int64_t v0 = (p - 1) * s.piece, v1 = std::min(v0 + s.piece, c.vocab);
     char* out = (char*)c.dw + v0 * c.width * lm_elem_size(c.w_t);
     if (p > 0) {
       px.a = pw.a = ws + (p & 1 ? s.g : s.g2), px.a_ld = pw.a_ld = s.piece, px.rows = pw.rows = c.rows;
-      px.b = (const char*)w + v0 * w_ld * ES, px.b_ld = w_ld, px.n = px.b_cols = s.padded, px.k = v1 - v0;
+      px.b = w_back + v0 * w_back_ld * ES, px.b_ld = w_back_ld, px.n = px.b_cols = s.padded, px.k = v1 - v0;
       px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = c.tokens, px.add = p > 1;
-      pw.b = rows ? rows : ws + s.x, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
-      pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / OP::LIFT, pw.units = units;
+      pw.b = x_back, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
+      pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / BACK::LIFT, pw.units = units;
       if (pw.splits == 1) pw.out = out, pw.out_ld = c.width, pw.out_t = c.w_t;
       else pw.sums = (float*)(ws + s.dw), pw.n_ld = s.padded, pw.m_rows = s.piece;
     }
     const LogitsCall* pg = p < s.pieces ? &g : nullptr;
     const ProductCall *x = p > 0 && c.dx ? &px : nullptr, *y = p > 0 && c.dw ? &pw : nullptr;
-    if (!(s.small        ? launch_pass<OP, typename F::Small, typename F::SmallX, typename F::MiddleW>(pg, x, y, c.tokens, c.st)
-          : s.large_pass ? launch_pass<OP, typename F::Large, typename F::LargeX, typename F::LargeW>(pg, x, y, c.tokens, c.st)
-                         : launch_pass<OP, typename F::Middle, typename F::MiddleX, typename F::MiddleW>(pg, x, y, c.tokens, c.st)))
+    if (!(s.small        ? launch_pass<BACK, typename F::Small, typename B::SmallX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)
+          : s.large_pass ? launch_pass<BACK, typename F::Large, typename B::LargeX, typename B::LargeW>(pg, x, y, c.tokens, c.st)
+                         : launch_pass<BACK, typename F::Middle, typename B::MiddleX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)))
       return SA_ERR_ARGUMENT;
     if (y && pw.splits > 1)
-      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_rows, 1.f / OP::LIFT, nullptr, out, v1 - v0, c.width, c.w_t, c.st);
+      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / BACK::LIFT, nullptr, out, v1 - v0, c.width, c.w_t, c.st);
   }
   if (c.dx)
     launch_finish((float*)(ws + s.dx), s.splits_x, c.tokens * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, units, &units->from_w,
-                  1.f / OP::LIFT, power, c.dx, c.tokens, c.width, c.x_t, c.st);
+                  1.f / BACK::LIFT, power, c.dx, c.tokens, c.width, c.x_t, c.st);
   return launch_status();
 }
 

@@ -205,3 +205,38 @@ def test_forward_mode_derivatives_are_refused(cuda):
                             lambda: torch.func.vmap(call)(x.expand(3, 4, 8))):
             with pytest.raises(RuntimeError):
                 transformed()
+
+
+@pytest.mark.parametrize("of", ["x", "weight", "both"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_rows_far_beyond_the_others(cuda, of, reduction):
+    """A row of x, or of weight, 2^40 times as large as the others: the backward pass has the forward's probabilities all the same.
+
+    Bounds as in xent_check with each logit's own dl (the largest's alone would cover everything): the sum of the exponentials is off by what
+    those that have weight are. The gradients' products hold x and weight beside their largest number, off by 2^-38 of that times
+    the G it meets: so dx is as exact as ever beside a row of x, dw beside one of weight."""
+    n, vocab, width = 200, 900, 64
+    g = torch.Generator(device="cuda").manual_seed(37)
+    x, w, t = xent_inputs(g, n, vocab, width, BF16, BF16)
+    if of != "weight":
+        x[7] *= 2.0 ** 40
+    if of != "x":
+        w[9] *= 2.0 ** 40
+    f = randn(g, n) if reduction == "none" else torch.full((n,), 1.0 / n, device="cuda")
+    each, _, dx, dw = xent_run(x, w, t, reduction, f if reduction == "none" else None)
+    x64, w64, f = x.double(), w.double(), f.double()[:, None]
+    l = x64 @ w64.T
+    p = torch.softmax(l, 1)
+    dl = (width + 2) * U * (x64.abs() @ w64.abs().T)
+    e_lse = ((p * dl).sum(1) + U * (160 + vocab / 1024) + 2.0 ** -22 * (4 + torch.logsumexp(l, 1).abs()))[:, None]
+    G = p.clone()
+    G[torch.arange(n, device="cuda"), t] -= 1.0
+    e_G = (half(F16) + U) * G.abs() + p * (2 * dl + e_lse) * 1.01 + 3 * U * p + 2.0 ** -38
+    want, size = f * (G @ w64), (f * G).abs()
+    bound = ((e_G * f.abs() + (vocab + 8) * U * size) @ w64.abs() + 2.0 ** -38 * w64.abs().max() * size.sum(1, keepdim=True)) * 1.01
+    assert_within(dx, want, bound + rounding(want, BF16), "dx")
+    if of == "x":
+        assert (bound[torch.arange(n, device="cuda") != 7] < 0.01 * f.abs().max()).all()
+    want = (f * G).T @ x64
+    bound = (e_G * f.abs() + (n + 8) * U * size).T @ x64.abs() + 2.0 ** -38 * x64.abs().max() * f.abs().max() * G.abs().sum(0)[:, None]
+    assert_within(dw, want, bound * 1.01 + rounding(want, BF16), "dw")
