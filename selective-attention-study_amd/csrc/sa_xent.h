@@ -1073,7 +1073,7 @@ int xent_forward(const XentCall& c) {
   lc.vocab = c.vocab;
   if (s.gather) {
     const bool scaled = s.train && s.SCALED;
-    const bool maxima = scaled || (s.train && s.ES == 2 && each);   // of x
+    const bool maxima = s.train && s.ES == 2;   // of x (fp16: for a backward pass with reduction none, whatever the forward's)
     hipLaunchKernelGGL(xent_rows_kernel, dim3(scaled ? 1 + MAXIMA : 1), dim3(1024), 0, c.st, c.targets, c.tokens, c.ignore, c.rows, each,
                        Matrix{c.w, c.w_ld, c.vocab, (int)c.width, c.w_t});
     lc.rows = c.rows;

@@ -10,6 +10,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import selective_attention as sa
+from selective_attention import lm
 from test_lm_gpu import BF16, F16, F32, F64, U, assert_within, half, randn, rounding, xent_check, xent_inputs, xent_run
 
 pytestmark = pytest.mark.gpu
@@ -240,3 +241,19 @@ def test_rows_far_beyond_the_others(cuda, of, reduction):
     want = (f * G).T @ x64
     bound = (e_G * f.abs() + (n + 8) * U * size).T @ x64.abs() + 2.0 ** -38 * x64.abs().max() * f.abs().max() * G.abs().sum(0)[:, None]
     assert_within(dw, want, bound * 1.01 + rounding(want, BF16), "dw")
+
+
+@THREE
+def test_reductions_of_the_two_passes(cuda, dtype):
+    """What the forward pass leaves serves a backward pass of either reduction."""
+    g = torch.Generator(device="cuda").manual_seed(38)
+    x, w, t = xent_inputs(g, 90, 300, 64, dtype, dtype, ignored=0.2)
+    code, none, total = lm._CODES[dtype], 0, 2
+    dloss, one = randn(g, 90), torch.full((1,), 0.75, device="cuda")
+    for forward in (none, 1, total):
+        torch.full((4096,), 0x7f7f7f7f, device="cuda", dtype=torch.int32)   # (what is left in memory is no magnitude)
+        _, lse, rows = lm._xent_impl(x, w, t, -100, forward, code, True)
+        got = [lm._xent_backward_impl(x, w, t, lse, rows, d, r, code, True, True) for r, d in ((none, dloss), (total, one))]
+        if forward == none:
+            want = got
+        assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q)), forward
