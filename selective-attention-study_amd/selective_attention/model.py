@@ -215,7 +215,10 @@ class SelectiveLM(nn.Module):
 
         Under autocast the norms hand the layers and the head the autocast type, the stream between the blocks keeps the
         embedding's, and the head's gradient is summed in fp32 (forward rounds it to the autocast type first), so the two
-        agree to that type's rounding."""
+        agree to that type's rounding.
+
+        The operators take the modules' parameters: forward hooks on the embedding, the norms, the head and the blocks do not run, and what
+        wraps the model's forward (a data-parallel wrapper) does not see this call. 64-bit parameters are refused on the GPU."""
         if idx.shape[1] > self.config.context_length:
             raise ValueError(f"sequence length {idx.shape[1]} exceeds context_length {self.config.context_length}")
         device, weight = idx.device.type, self.transformer.wte.weight
