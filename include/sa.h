@@ -350,7 +350,7 @@ int sa_embedding_backward(const void* ids, int ids_bytes, const void* dout, int6
  * null: no backward pass follows (rows is scratch then). The workspace's size depends on the strides and alignment of x and weight, so its query takes the
  * same pointers (which it does not read).
  * Backward: dloss fp32, (tokens) or (1) by reduction; dx (tokens, width) of x's type, dweight (vocab, width) of weight's, 16-byte aligned;
- * either may be null. The logits are computed again, a piece of the vocabulary at a time. 1 to 2^28 - 1 tokens and vocabulary
+ * either may be null; the reduction may be another than the forward's. The logits are computed again, a piece of the vocabulary at a time. 1 to 2^28 - 1 tokens and vocabulary
  * rows, width up to 2^16.
  */
 #define SA_XENT_ROWS 1088

@@ -13,7 +13,8 @@
 // are added in LDS, and norm_join adds the workgroups' rows of sums in a fixed order. No atomics: equal calls give equal bits.
 //
 // Measured: 16384 x 768, fp32 stream, bf16 branch and result, forward 31 us (4.8 TB/s), backward 44 (4.6 TB/s) and 4 for the join; 2048 x 8192 bf16
-// 30, 38 and 4; 5003 x 1001 fp32 13, 22 and 4. A copy of 4 GiB runs at 4.7 TB/s.
+// 30, 38 and 4; 5003 x 1001 fp32 13, 22 and 4. A copy of 4 GiB runs at 4.7 TB/s. Wider than 8192, 1024 threads leave 128 registers each and the rest
+// spills: 2048 x 12000 bf16 70 and with gradients 268, 1024 x 32768 127 and 613 (their bytes at that rate 42 and 84, 57 and 114).
 
 #include <math.h>
 

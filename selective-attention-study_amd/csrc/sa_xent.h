@@ -26,9 +26,9 @@
 // g_i over the power of two below it before it is rounded, the sum dx_i that power; dW sums over tokens, so it reads a copy of x whose rows have their
 // powers (16-bit types; fp32 puts all of g_i into G_i).
 //
-// Bound by the matrix units and, with all of them busy, by power (1.9 GHz). Measured, 16384 tokens x 50304 x 768 bf16: the forward pass's products
-// 1.2-1.35 ms (0.95-1.05 PFLOP/s with the statistics; torch's own product of that shape 1.13), the backward's eight passes 0.48-0.53
-// each (three products: 0.95-1.0 PFLOP/s), all else 0.12. Few tokens: by the weight's way from HBM (8 tokens 15.8-20 us for 77 MB).
+// Bound by the matrix units and, with all of them busy, by power (1.8-1.9 GHz). Measured, 16384 tokens x 50304 x 768 bf16: the forward pass's products
+// 1.2-1.4 ms (0.9-1.05 PFLOP/s with the statistics; torch's own product of that shape 1.13), the backward's eight passes 0.48-0.53
+// each (three products: 0.95-1.0 PFLOP/s), all else 0.15. Few tokens: by the weight's way from HBM (8 tokens 15.8-20 us for 77 MB).
 
 #pragma once
 
@@ -906,7 +906,7 @@ struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per st
 
 // One tile's tokens of the smallest kernels. Us by 128 x 64 / 128 x 128: 8 tokens x 50304 x 768, no gradient, weight out of HBM 20.0 / 21.5; training,
 // forward and backward: fp32 64 x 50304 x 768 67 / 109 and 183 / 323, fp16 33 x 32000 x 2048 40 / 42 and 122 / 140, bf16 64 x 50304 x 768
-// 56 / 58 and 122 / 118.
+// 56 / 58 and 122 / 118 (8 less than now that the logits' weight and dX's are two).
 constexpr int64_t SMALL_TOKENS = 64;
 constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are (250 tokens 40 us, listed and gathered 47)
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of a piece's G, of which there are two at a time
