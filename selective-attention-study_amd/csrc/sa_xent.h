@@ -19,7 +19,8 @@
 //
 // All products run through one tile loop on matrix instructions with fp32 accumulation (Mainloop). Statistics, lse and losses are
 // fp32. Both passes take the logits from the same operands, so that the probabilities are the forward's whatever the rows hold. G is rounded to
-// 11 bits: it is held in fp16 at 2^14 times its size (a vocabulary's probabilities lie below that type's normal range). Its products with bf16
+// 11 bits (few tokens' with fp16 operands to 22, in two numbers): it is held in fp16 at 2^14 times its size (a vocabulary's probabilities lie below
+// that type's normal range). Its products with bf16
 // operands hold these in fp16 too, times the power of two that brings their largest to 2^14: exactly, but for numbers 2^31 times smaller
 // than that, which are off by 2^-39 of it, and at the same rate. (With G in bf16 the gradients' error was 1.4 to 1.6 times that of their own
 // rounding; so it is that rounding's.) The factors and a common g are applied to the fp32 sums. Tokens' own g_i (reduction none): G_i takes
@@ -423,11 +424,12 @@ struct Factors {   // xent_factors_kernel
 
 // Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i], where `to` is not null. maxima: each workgroup's largest
 // magnitude (MAXIMA workgroups then). also (null: none): the same rows, rounded to that type first, in the type that G is held in and *unit times; with
-// `power` also times the row's power over *g, the largest number's (a row whose power is above that is none).
+// `power` also times the row's power over *g, the largest number's (a row whose power is above that is none). twice: these once more, behind the last.
 template <class OP>
 __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
                                                            const int* count, int64_t most, int* maxima, typename OP::elem* to, int padded,
-                                                           typename OP::Back::elem* also, const float* unit, const float* power, const float* g) {
+                                                           typename OP::Back::elem* also, const float* unit, const float* power, const float* g,
+                                                           bool twice) {
   __shared__ float acc[16];
   const int64_t rows = count ? *count : most;
   const int lane = threadIdx.x & 63;
@@ -454,6 +456,7 @@ __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = stored(x[j], OP::CODE) * by;
         put<true>(also + i * padded, OP::Back::CODE, e0 + 256 * u, 1, padded, x);
+        if (twice) put<true>(also + (rows + i) * padded, OP::Back::CODE, e0 + 256 * u, 1, padded, x);
       }
     }
   }
@@ -479,8 +482,8 @@ struct LogitsCall {
   int64_t g_ld;
 };
 
-// (OP: what G is held in, of as many bits as the operands)
-template <class OP, class L, bool GRAD>
+// (OP: what G is held in, of as many bits as the operands. TWICE: what its rounding leaves is held in as many rows again, behind the kept tokens'.)
+template <class OP, class L, bool GRAD, bool TWICE>
 __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typename L::Stage& s0, typename L::Stage& s1,
                                             typename L::Stage& s2, typename L::Stage& s3) {
   typedef typename OP::elem elem;
@@ -566,10 +569,13 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
     uint8_t* mine = (wave < FIT ? s0.a : s1.a) + wave % FIT * 32 * RB;
     // (rows past the last token lie past the resource's end: such stores are dropped)
     const int g_row = (int)(c.g_ld * ES);
-    const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES);
+    const int64_t bytes = min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES;
+    const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), bytes);
+    const __amdgpu_buffer_rsrc_t rest = TWICE ? resource((elem*)c.g + (tokens + n0) * c.g_ld + (vw - c.v0), bytes) : rs;
     const int left = edge ? (int)(c.v1 - vw) : L::TM * 32;   // rows of the vocabulary
 #pragma unroll 1
-    for (int b = 0; b < L::TN; ++b) {
+    for (int part = 0; part < (TWICE ? 2 : 1) * L::TN; ++part) {
+      const int b = TWICE ? part >> 1 : part;
       const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
       const bool real = i < tokens;
       // (beside the largest logit, whose distance is exact where weights are large: log of the sum alone is off by 2^-21)
@@ -591,6 +597,7 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
             for (int o = 1; o < L::TN; ++o) x = b == o ? l.acc[a][o][4 * q + r] : x;
             x = __builtin_amdgcn_exp2f((x - top) * LOG2E) * over;
             x = tl == row ? x - lift : x;
+            if (TWICE && (part & 1)) x -= stored(x, OP::CODE);   // (infinities: a NaN, in a row that has them already)
             p[r] = row < left ? x : 0.f;
           }
           const int byte = (a * 32 + 8 * q + 4 * h) * ES;
@@ -601,7 +608,7 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
       for (int k = 0; k < 32 * CPR / 64; ++k) {
         const int slot = k * 64 + lane, r = slot / CPR, ch = slot % CPR;
         const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ((ch ^ (r & TURN)) << 4));
-        __builtin_amdgcn_raw_buffer_store_b128(v, rs, r * g_row + ch * 16, (wn * L::TN + b) * 32 * g_row, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(v, TWICE && (part & 1) ? rest : rs, r * g_row + ch * 16, (wn * L::TN + b) * 32 * g_row, 0);
       }
       __asm__ volatile("" ::: "memory");
     }
@@ -611,7 +618,7 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
 template <class OP, class L>
 __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits_kernel(LogitsCall c) {
   __shared__ typename L::Stage s0, s1, s2, s3;
-  logits_tile<OP, L, false>(c, blockIdx.x, s0, s1, s2, s3);
+  logits_tile<OP, L, false, false>(c, blockIdx.x, s0, s1, s2, s3);
 }
 
 // A token's statistics over the mt tiles joined: `TOKENS` tokens a workgroup, NTHREADS / TOKENS lanes each. What the backward pass takes of them, the loss, and
@@ -745,7 +752,8 @@ __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, 
 struct ProductCall {
   const void *a, *b;
   int64_t a_ld, b_ld;
-  const int* rows;          // kept tokens: M (dX) or K (dW)
+  const int* rows;          // kept tokens: M (dX) or K (dW), `times` over
+  int times;
   int64_t m, n, k;          // M of dW, N, K of dX
   int64_t b_cols;           // columns of b that may be read (whole 16-byte pieces)
   int mt, nt, splits;
@@ -764,7 +772,7 @@ __device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, i
                                              typename L::Stage& s2, typename L::Stage& s3) {
   typedef typename OP::elem elem;
   constexpr int ES = sizeof(elem);
-  const int64_t tokens = uniform(c.rows[0]);
+  const int64_t tokens = uniform(c.rows[0] * c.times);
   const int64_t M = DW ? c.m : tokens, K = DW ? tokens : c.k;
   int m, n;
   if (!tile_of(id, DW ? c.mt : (int)((M + L::BM - 1) / L::BM), c.nt, m, n)) return;
@@ -831,7 +839,7 @@ struct PassCall {
   ProductCall x, w;
   int x_at, x_tiles, x_end, w_at, w_tiles, w_end, g_at;   // workgroups: of a part of the contraction, of all parts
 };
-template <class OP, class LG, class LX, class LW>
+template <class OP, class LG, class LX, class LW, bool TWICE>
 __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass_kernel(PassCall c) {
   typedef typename std::conditional<(sizeof(typename LW::Stage) > sizeof(typename LG::Stage)), typename LW::Stage, typename LG::Stage>::type S;
   static_assert(sizeof(typename LX::Stage) <= sizeof(S) && LG::THREADS == LX::THREADS && LG::THREADS == LW::THREADS, "one launch for all");
@@ -847,14 +855,16 @@ __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass
     product_tile<OP, LW, true>(c.w, id - c.w_at - part * c.w_tiles, part, (W&)s0, (W&)s1, (W&)s2, (W&)s3);
   } else {
     typedef typename LG::Stage G;
-    logits_tile<OP, LG, true>(c.g, id - c.g_at, (G&)s0, (G&)s1, (G&)s2, (G&)s3);
+    logits_tile<OP, LG, true, TWICE>(c.g, id - c.g_at, (G&)s0, (G&)s1, (G&)s2, (G&)s3);
   }
 }
 
-// dX: a token's parts added, times g or its own power; zero rows for the tokens that are ignored. dW: the parts of a piece's rows.
+// dX: a token's parts added (and those `kept` rows behind them, where that is not null), times g or its own power; zero rows for the tokens that are
+// ignored. dW: the parts of a piece's rows.
 __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums, int splits, int64_t split_stride, int64_t n_ld,
                                                                const int* place, const Factors* units, const float* unit, float lift,
-                                                               const float* power, void* out, int64_t rows, int width, int dtype) {
+                                                               const float* power, const int* kept, void* out, int64_t rows, int width,
+                                                               int dtype) {
   const int lane = threadIdx.x & 63;
   const bool quads = width % 4 == 0;
   const float u = *unit;
@@ -868,6 +878,14 @@ __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums
         for (int s = 0; s < splits; ++s) {
           const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + at * n_ld + e);
           x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
+        }
+        if (kept) {
+          const int64_t behind = at + *kept;
+#pragma unroll 8
+          for (int s = 0; s < splits; ++s) {
+            const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + behind * n_ld + e);
+            x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = x[j] * f * u;
@@ -906,7 +924,7 @@ struct XentConfigs<XF32> {   // (fp32 tiles are half as large in elements per st
 
 // One tile's tokens of the smallest kernels. Us by 128 x 64 / 128 x 128: 8 tokens x 50304 x 768, no gradient, weight out of HBM 20.0 / 21.5; training,
 // forward and backward: fp32 64 x 50304 x 768 67 / 109 and 183 / 323, fp16 33 x 32000 x 2048 40 / 42 and 122 / 140, bf16 64 x 50304 x 768
-// 56 / 58 and 122 / 118 (8 less than now that the logits' weight and dX's are two).
+// 56 / 58 and 122 / 118 (backward 26 and 8 less than now that fp16's G is two numbers, and bf16's weight read in two types).
 constexpr int64_t SMALL_TOKENS = 64;
 constexpr int64_t IN_PLACE_TOKENS = 256;  // up to here a forward pass reads the rows as they are (250 tokens 40 us, listed and gathered 47)
 constexpr int64_t PIECE_BYTES = (int64_t)256 << 20;   // of a piece's G, of which there are two at a time
@@ -918,7 +936,7 @@ template <class OP>
 struct XentShape {
   static constexpr int ES = sizeof(typename OP::elem), BK = KB / ES;
   static constexpr bool SCALED = !std::is_same<OP, typename OP::Back>::value;   // weight and x have copies for the products with G
-  bool train, small, large, gather, copy_w;
+  bool train, small, large, gather, copy_w, twice;
   int64_t padded, bm, mt, join_tokens, join_blocks;
   // backward
   int64_t piece, pieces;
@@ -953,6 +971,11 @@ struct XentShape {
     };
     x = take(gather ? c.tokens * padded * ES : 0);
     w = take(copy_w ? c.vocab * padded * ES : 0);
+    // Few tokens with fp16 operands: G in two numbers of 11 bits each. With one its rounding was beside the gradients' own, the same for a whole row, so
+    // that few rows' errors do not even out: of 40 calls each, 1 / 2 / 8 / 32 / 64 tokens, dx's error was up to 2.5 / 1.8 / 1.6 / 1.5 / 1.46 times that
+    // rounding's, 1.3 at the median, as for more tokens; with two 1.03. (Forward and backward, us: 8 x 50304 x 768 113 -> 126, 64 x 50304 x 768 121 ->
+    // 140, 33 x 32000 x 2048 165 -> 191.)
+    twice = ES == 2 && !SCALED && small;
     if (!backward) {
       top = take(mt * c.tokens * 4);
       sum = take(mt * c.tokens * 4);
@@ -960,7 +983,8 @@ struct XentShape {
       sums = take(join_blocks * 4);
     } else {
       // Pieces of the vocabulary whose G fits PIECE_BYTES (and a token's row of it MAX_LD_BYTES), in whole tiles, of about one size
-      const int64_t most = std::max<int64_t>(std::min(PIECE_BYTES / (c.tokens * ES), MAX_LD_BYTES / ES) / 256 * 256, 256);
+      const int64_t held = twice ? 2 * c.tokens : c.tokens;   // rows of G
+      const int64_t most = std::max<int64_t>(std::min(PIECE_BYTES / (held * ES), MAX_LD_BYTES / ES) / 256 * 256, 256);
       pieces = cdiv(c.vocab, most);
       piece = align_up(cdiv(c.vocab, pieces), 256);
       pieces = cdiv(c.vocab, piece);
@@ -971,11 +995,11 @@ struct XentShape {
       // 1453 / 1201 / 1199 / 1205 us; 1000 x 16384 x 768 in 2 / 4 / 8 / 16: 217 / 151 / 130 / 136; 100 x 50304 x 768 in 4 / 8 / 16: 153 / 117 / 114).
       // dW's over few tokens is best whole (1000 x 16384 x 768 in 1 / 2 parts 136 / 175), over 16384 x 50304 the last piece's
       // in 1 / 2 / 3 / 6 4138 / 4070 / 4056 / 4063. Pieces of 64 / 128 / 256 / 512 MB there: 4405 / 4160 / 4039 / 4016.
-      const int64_t k_x = cdiv(piece, BK), k_w = cdiv(c.tokens, BK), k_g = padded / BK;
+      const int64_t k_x = cdiv(piece, BK), k_w = cdiv(held, BK), k_g = padded / BK;
       const auto tiles = [&](int64_t edge, int64_t m, int64_t n) { return cdiv(m, edge) * cdiv(n, edge); };
       large_pass = ES == 2 && whole && tiles(256, c.tokens, c.width) + tiles(256, piece, c.width) + tiles(256, c.tokens, piece) / 4 >= c.cus;
       const int64_t edge = large_pass ? 256 : 128, slots = large_pass ? c.cus : 2 * (int64_t)c.cus;
-      const int64_t products = (c.dx ? tiles(edge, c.tokens, c.width) * k_x : 0) + (c.dw ? tiles(edge, piece, c.width) * k_w : 0);
+      const int64_t products = (c.dx ? tiles(edge, held, c.width) * k_x : 0) + (c.dw ? tiles(edge, piece, c.width) * k_w : 0);
       const int64_t share = cdiv(products + (pieces > 1 ? tiles(edge, c.tokens, piece) * (k_g + 8) : products / 2), slots);
       const int64_t share_last = std::max<int64_t>(cdiv(products, 2 * slots), 1);
       const auto parts = [](int64_t stages, int64_t of, int64_t most) {
@@ -983,21 +1007,21 @@ struct XentShape {
       };
       // A part more costs dX's sums once more through memory: up to 64 parts where they take no more than 32 MB, 16 at least (few tokens have
       // few tiles and long contractions; with the smallest tiles, fp32 3 x 68497 x 768 430 -> 242 us, 5 x 68536 x 128 311 -> 119).
-      const int64_t most_x = std::min<int64_t>(std::max<int64_t>(((int64_t)32 << 20) / (c.tokens * padded * 4), 16), 64);
+      const int64_t most_x = std::min<int64_t>(std::max<int64_t>(((int64_t)32 << 20) / (held * padded * 4), 16), 64);
       splits_x = parts(k_x, pieces > 1 ? cdiv(share, 2) : 2 * share_last, most_x);
       splits_w = parts(k_w, share, 16);
       splits_last = parts(k_w, 2 * share_last, 16);
       // (a part's rows lie within 2^30 bytes)
       const int64_t w_row = (SCALED || copy_w ? padded : c.w_ld) * ES, x_row = std::max(padded, piece) * ES;
       splits_x = std::max(splits_x, (int)cdiv(piece * w_row, (int64_t)1 << 30));
-      splits_w = std::max(splits_w, (int)cdiv(c.tokens * x_row, (int64_t)1 << 30));
+      splits_w = std::max(splits_w, (int)cdiv(held * x_row, (int64_t)1 << 30));
       splits_last = std::max(splits_last, splits_w);
       factors = take((2 * c.tokens + 64) * 4);
-      x_back = take(c.dw && ES == 2 ? c.tokens * padded * ES : 0);   // (fp16: with reduction none alone, which the query of the size does not know)
+      x_back = take(c.dw && ES == 2 ? held * padded * ES : 0);   // (many tokens, fp16: with reduction none alone, which the size's query does not know)
       w_back = take(c.dx && SCALED ? c.vocab * padded * ES : 0);
-      g = take(c.tokens * piece * ES);
-      g2 = take(pieces > 1 ? c.tokens * piece * ES : 0);
-      dx = take(c.dx ? splits_x * c.tokens * padded * 4 : 0);
+      g = take(held * piece * ES);
+      g2 = take(pieces > 1 ? held * piece * ES : 0);
+      dx = take(c.dx ? splits_x * held * padded * 4 : 0);
       dw = take(c.dw && splits_last > 1 ? splits_last * piece * padded * 4 : 0);
     }
     total = p;
@@ -1011,8 +1035,9 @@ void launch_logits(LogitsCall lc, int64_t tokens, hipStream_t st) {
   hipLaunchKernelGGL((xent_logits_kernel<OP, L>), dim3((unsigned)tiles_grid(lc.mt, lc.nt)), dim3(L::THREADS), 0, st, lc);
 }
 // g, x, w: what the pass does (null: not that)
-template <class OP, class LG, class LX, class LW>
+template <class OP, bool TWICE, class LG, class LX, class LW>
 bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w, int64_t tokens, hipStream_t st) {
+  const int64_t held = TWICE ? 2 * tokens : tokens;
   PassCall pc{};
   int64_t at = 0;
   const auto place = [&at](ProductCall& c, int64_t m, int edge_m, int edge_n, int& begin, int& tiles, int& end) {
@@ -1023,9 +1048,9 @@ bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
     end = (int)(at += (int64_t)tiles * c.splits);
   };
   const auto put_x = [&] {
-    if (x) pc.x = *x, place(pc.x, tokens, LX::BM, LX::BN, pc.x_at, pc.x_tiles, pc.x_end);
+    if (x) pc.x = *x, place(pc.x, held, LX::BM, LX::BN, pc.x_at, pc.x_tiles, pc.x_end);
   };
-  const bool x_first = x && w && cdiv(x->k, x->splits) > cdiv(tokens, w->splits);
+  const bool x_first = x && w && cdiv(x->k, x->splits) > cdiv(held, w->splits);
   if (x_first) put_x();
   if (w) pc.w = *w, place(pc.w, w->m, LW::BM, LW::BN, pc.w_at, pc.w_tiles, pc.w_end);
   if (!x_first) put_x();
@@ -1037,23 +1062,23 @@ bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
     at += tiles_grid(pc.g.mt, pc.g.nt);
   }
   if (at * LG::THREADS >= ((int64_t)1 << 32)) return false;   // more threads than a launch takes
-  hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
+  hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW, TWICE>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
   return true;
 }
 template <class OP>
 void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows, int* maxima,
                    void* to, int64_t padded, hipStream_t st, void* also = nullptr, const float* unit = nullptr, const float* power = nullptr,
-                   const float* g = nullptr) {
+                   const float* g = nullptr, bool twice = false) {
   const int64_t blocks = maxima ? MAXIMA : std::min<int64_t>(cdiv(rows, NWAVES), 16384);
   hipLaunchKernelGGL((xent_gather_kernel<OP>), dim3((unsigned)blocks), dim3(maxima ? 1024 : NTHREADS), 0, st, from, ld, dtype, (int)width,
-                     numbers_of, count, rows, maxima, (typename OP::elem*)to, (int)padded, (typename OP::Back::elem*)also, unit, power, g);
+                     numbers_of, count, rows, maxima, (typename OP::elem*)to, (int)padded, (typename OP::Back::elem*)also, unit, power, g, twice);
 }
 inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const Factors* units,
-                          const float* unit, float lift, const float* power, void* out, int64_t rows, int64_t width, int dtype,
-                          hipStream_t st) {
+                          const float* unit, float lift, const float* power, const int* kept, void* out, int64_t rows, int64_t width,
+                          int dtype, hipStream_t st) {
   const int64_t blocks = std::min<int64_t>(cdiv(rows, NWAVES), 16384);
   hipLaunchKernelGGL(xent_finish_kernel, dim3((unsigned)blocks), dim3(NTHREADS), 0, st, sums, splits, split_stride, n_ld, place, units,
-                     unit, lift, power, out, rows, (int)width, dtype);
+                     unit, lift, power, kept, out, rows, (int)width, dtype);
 }
 
 template <class OP>
@@ -1118,9 +1143,11 @@ int xent_backward(const XentCall& c) {
   float* factor = c.reduction == SA_REDUCE_NONE ? (float*)units + 64 : nullptr;
   float* power = factor && ES == 2 ? factor + c.tokens : nullptr;
   hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, s.SCALED, units, factor, power);
-  const char* x_back = ws + (s.SCALED || power ? s.x_back : s.x);   // dW's
+  const int64_t held = s.twice ? 2 * c.tokens : c.tokens;   // rows of G
+  const bool two = s.SCALED || power || s.twice;
+  const char* x_back = ws + (two ? s.x_back : s.x);   // dW's
   launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, ws + s.x, s.padded, c.st,
-                    c.dw && (s.SCALED || power) ? ws + s.x_back : nullptr, &units->x, power, &units->g);
+                    c.dw && two ? ws + s.x_back : nullptr, &units->x, power, &units->g, s.twice);
   const char *w = s.copy_w ? ws + s.w : (const char*)c.w, *w_back = s.SCALED ? ws + s.w_back : w;   // dX's
   const int64_t w_ld = s.copy_w ? s.padded : c.w_ld, w_back_ld = s.SCALED ? s.padded : w_ld;
   void* const scaled_w = s.SCALED && c.dx ? ws + s.w_back : nullptr;
@@ -1139,9 +1166,9 @@ int xent_backward(const XentCall& c) {
     const int64_t v0 = (p - 1) * s.piece, v1 = std::min(v0 + s.piece, c.vocab);
     char* out = (char*)c.dw + v0 * c.width * lm_elem_size(c.w_t);
     if (p > 0) {
-      px.a = pw.a = ws + (p & 1 ? s.g : s.g2), px.a_ld = pw.a_ld = s.piece, px.rows = pw.rows = c.rows;
+      px.a = pw.a = ws + (p & 1 ? s.g : s.g2), px.a_ld = pw.a_ld = s.piece, px.rows = pw.rows = c.rows, px.times = pw.times = s.twice ? 2 : 1;
       px.b = w_back + v0 * w_back_ld * ES, px.b_ld = w_back_ld, px.n = px.b_cols = s.padded, px.k = v1 - v0;
-      px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = c.tokens, px.add = p > 1;
+      px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = held, px.add = p > 1;
       pw.b = x_back, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
       pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / BACK::LIFT, pw.units = units;
       if (pw.splits == 1) pw.out = out, pw.out_ld = c.width, pw.out_t = c.w_t;
@@ -1149,16 +1176,17 @@ int xent_backward(const XentCall& c) {
     }
     const LogitsCall* pg = p < s.pieces ? &g : nullptr;
     const ProductCall *x = p > 0 && c.dx ? &px : nullptr, *y = p > 0 && c.dw ? &pw : nullptr;
-    if (!(s.small        ? launch_pass<BACK, typename F::Small, typename B::SmallX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)
-          : s.large_pass ? launch_pass<BACK, typename F::Large, typename B::LargeX, typename B::LargeW>(pg, x, y, c.tokens, c.st)
-                         : launch_pass<BACK, typename F::Middle, typename B::MiddleX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)))
+    constexpr bool TWICE = ES == 2 && !s.SCALED;   // (of the smallest)
+    if (!(s.small        ? launch_pass<BACK, TWICE, typename F::Small, typename B::SmallX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)
+          : s.large_pass ? launch_pass<BACK, false, typename F::Large, typename B::LargeX, typename B::LargeW>(pg, x, y, c.tokens, c.st)
+                         : launch_pass<BACK, false, typename F::Middle, typename B::MiddleX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)))
       return SA_ERR_ARGUMENT;
     if (y && pw.splits > 1)
-      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / BACK::LIFT, nullptr, out, v1 - v0, c.width, c.w_t, c.st);
+      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / BACK::LIFT, nullptr, nullptr, out, v1 - v0, c.width, c.w_t, c.st);
   }
   if (c.dx)
-    launch_finish((float*)(ws + s.dx), s.splits_x, c.tokens * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, units, &units->from_w,
-                  1.f / BACK::LIFT, power, c.dx, c.tokens, c.width, c.x_t, c.st);
+    launch_finish((float*)(ws + s.dx), s.splits_x, held * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, units, &units->from_w,
+                  1.f / BACK::LIFT, power, s.twice ? c.rows : nullptr, c.dx, c.tokens, c.width, c.x_t, c.st);
   return launch_status();
 }
 

@@ -257,3 +257,37 @@ def test_reductions_of_the_two_passes(cuda, dtype):
         if forward == none:
             want = got
         assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q)), forward
+
+
+@pytest.mark.parametrize("n", [1, 2, 7, 32, 33, 64])
+@pytest.mark.parametrize("reduction", [0, 1])
+def test_few_tokens_in_fp16(cuda, n, reduction):
+    """Up to 64 tokens with fp16 operands have G in two numbers, to 22 bits: seen in fp32 gradients of fp32 tensors of fp16 numbers.
+
+    Bounds as in xent_check, with 2^-22 of G in the place of 2^-11."""
+    vocab, width = 700, 16
+    g = torch.Generator(device="cuda").manual_seed(39)
+    x, w, t = xent_inputs(g, n, vocab, width, F16, F16, ignored=0.2)
+    t[0] = 5
+    kept = t != -100
+    code = lm._CODES[F16]
+    dloss = randn(g, n) if reduction == 0 else torch.ones((), device="cuda")
+    _, lse, rows = lm._xent_impl(x.float(), w.float(), t, -100, reduction, code, True)
+    dx, dw = lm._xent_backward_impl(x.float(), w.float(), t, lse, rows, dloss, reduction, code, True, True)
+    x64, w64, at = x.double()[kept], w.double(), t[kept]
+    f = (dloss.double()[kept] if reduction == 0 else torch.full((len(at),), 1.0 / len(at), device="cuda", dtype=F64))[:, None]
+    l = x64 @ w64.T
+    dl = (width + 2) * U * (x64.abs() @ w64.abs().T).amax(1)
+    lse64 = torch.logsumexp(l, 1)
+    e_lse = dl + U * (160 + vocab / 1024) + 2.0 ** -22 * (4 + lse64.abs())
+    p = torch.exp(l - lse64[:, None])
+    G = p.clone()
+    G[torch.arange(len(at), device="cuda"), at] -= 1.0
+    e_G = ((2.0 ** -22 + 3 * U) * G.abs() + p * (2 * dl + e_lse)[:, None] * 1.01 + 3 * U * p + 2.0 ** -38) * f.abs()
+    G = G * f
+    want = G @ w64
+    assert (dx[~kept] == 0).all()
+    assert_within(dx[kept], want, ((e_G + (2 * vocab + 8) * U * G.abs()) @ w64.abs()) * 1.01 + rounding(want, F32), "dx")
+    want = G.T @ x64
+    assert_within(dw, want, ((e_G + (2 * n + 8) * U * G.abs()).T @ x64.abs() + 2.0 ** -38 * x64.abs().max() * f.abs().max() * p.sum(0)[:, None]) * 1.01
+                  + rounding(want, F32), "dw")
