@@ -235,6 +235,7 @@ template <class OP, int WM_, int WN_, int TM_, int TN_, bool TRA, bool TRB>
 struct Mainloop {
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
+  static constexpr bool TWO_NUMBERS = std::is_same<OP, XF16>::value;   // (halves_of)
   typedef Operand<OP, BM, TRA, WAVES> A;
   typedef Operand<OP, BN, TRB, WAVES> B;
   static constexpr int BK = A::BK, LOADS = A::PER + B::PER;
@@ -422,16 +423,25 @@ struct Factors {   // xent_factors_kernel
   float g, w, x, from_w, from_x;
 };
 
+// In how many numbers of 11 bits G holds the probabilities of `kept` tokens, where it has `held` rows. With one its rounding is beside the gradients' own
+// with fp16 operands, the same for a whole row, so that few rows' errors do not even out: of 40 calls each, 1 / 2 / 8 / 32 / 64 tokens,
+// dx's error was up to 2.5 / 1.8 / 1.6 / 1.5 / 1.46 times that rounding's, 1.3 at the median, as for more tokens; with two 1.03. (Forward and backward,
+// us: 8 x 50304 x 768 113 -> 126, 64 x 50304 x 768 121 -> 140, 33 x 32000 x 2048 165 -> 191. held 0: one.)
+constexpr int TWICE_TOKENS = 64;
+__device__ __forceinline__ int halves_of(int kept, int64_t held) { return kept <= TWICE_TOKENS && 2 * (int64_t)kept <= held ? 2 : 1; }
+
 // Rows in the products' type, zeros behind the width: to[i] = from[numbers ? numbers[i] : i], where `to` is not null. maxima: each workgroup's largest
 // magnitude (MAXIMA workgroups then). also (null: none): the same rows, rounded to that type first, in the type that G is held in and *unit times; with
-// `power` also times the row's power over *g, the largest number's (a row whose power is above that is none). twice: these once more, behind the last.
+// `power` also times the row's power over *g, the largest number's (a row whose power is above that is none). held: where G has two
+// numbers (halves_of) the rows that dW reads, also's or else to's, once more behind the last.
 template <class OP>
 __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int64_t ld, int dtype, int width, const int* numbers_of,
                                                            const int* count, int64_t most, int* maxima, typename OP::elem* to, int padded,
                                                            typename OP::Back::elem* also, const float* unit, const float* power, const float* g,
-                                                           bool twice) {
+                                                           int64_t held) {
   __shared__ float acc[16];
   const int64_t rows = count ? *count : most;
+  const bool twice = held && halves_of((int)rows, held) == 2;
   const int lane = threadIdx.x & 63;
   const bool quads = ((uintptr_t)from % (dtype == SA_DTYPE_F32 ? 16 : 8)) == 0 && ld % 4 == 0 && width % 4 == 0;
   float top = 0.f;
@@ -452,6 +462,7 @@ __global__ __launch_bounds__(1024) void xent_gather_kernel(const void* from, int
 #pragma unroll
         for (int j = 0; j < 4; ++j) top = larger(top, x[j]);
         if (to) put<true>(to + i * padded, OP::CODE, e0 + 256 * u, 1, padded, x);
+        if (twice && !also) put<true>(to + (rows + i) * padded, OP::CODE, e0 + 256 * u, 1, padded, x);
         if (!also) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = stored(x[j], OP::CODE) * by;
@@ -478,12 +489,14 @@ struct LogitsCall {
   float *top, *sum, *at;    // (mt, tokens) statistics, the targets' logits
   const float* lse;         // backward: XentCall's
   const float* factor;      // backward: of each kept token's row of G; null: 1
-  void* g;                  // (tokens, g_ld)
+  void* g;                  // (tokens, g_ld), or two rows of a token: halves_of(kept tokens, held)
+  int64_t held;
   int64_t g_ld;
 };
 
-// (OP: what G is held in, of as many bits as the operands. TWICE: what its rounding leaves is held in as many rows again, behind the kept tokens'.)
-template <class OP, class L, bool GRAD, bool TWICE>
+// (OP: what G is held in, of as many bits as the operands. Where G has two numbers, the second, what rounding the first leaves, is in as many
+// rows again behind the kept tokens'.)
+template <class OP, class L, bool GRAD>
 __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typename L::Stage& s0, typename L::Stage& s1,
                                             typename L::Stage& s2, typename L::Stage& s3) {
   typedef typename OP::elem elem;
@@ -571,54 +584,58 @@ __device__ __forceinline__ void logits_tile(const LogitsCall& c, int64_t id, typ
     const int g_row = (int)(c.g_ld * ES);
     const int64_t bytes = min(tokens - n0, (int64_t)L::BN) * g_row - (vw - c.v0) * ES;
     const __amdgpu_buffer_rsrc_t rs = resource((elem*)c.g + n0 * c.g_ld + (vw - c.v0), bytes);
-    const __amdgpu_buffer_rsrc_t rest = TWICE ? resource((elem*)c.g + (tokens + n0) * c.g_ld + (vw - c.v0), bytes) : rs;
+    const int halves = uniform(halves_of((int)tokens, c.held));
     const int left = edge ? (int)(c.v1 - vw) : L::TM * 32;   // rows of the vocabulary
+    const auto half_of_g = [&](auto second, const __amdgpu_buffer_rsrc_t& rs) {
 #pragma unroll 1
-    for (int part = 0; part < (TWICE ? 2 : 1) * L::TN; ++part) {
-      const int b = TWICE ? part >> 1 : part;
-      const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
-      const bool real = i < tokens;
-      // (beside the largest logit, whose distance is exact where weights are large: log of the sum alone is off by 2^-21)
-      const float top = real ? c.lse[i] : 0.f;
-      const float lift = (c.factor && real ? c.factor[i] : 1.f) * OP::LIFT, over = real ? c.lse[c.tokens + i] * lift : 0.f;
-      const int64_t t = real ? c.targets[c.rows[ROWS_HEAD + i]] - vw : -1;
-      const int tl = t >= 0 && t < L::TM * 32 ? (int)t : -1;
-      uint8_t* to = mine + (lane & 31) * RB;
+      for (int b = 0; b < L::TN; ++b) {
+        const int64_t i = n0 + (wn * L::TN + b) * 32 + (lane & 31);
+        const bool real = i < tokens;
+        // (beside the largest logit, whose distance is exact where weights are large: log of the sum alone is off by 2^-21)
+        const float top = real ? c.lse[i] : 0.f;
+        const float lift = (c.factor && real ? c.factor[i] : 1.f) * OP::LIFT, over = real ? c.lse[c.tokens + i] * lift : 0.f;
+        const int64_t t = real ? c.targets[c.rows[ROWS_HEAD + i]] - vw : -1;
+        const int tl = t >= 0 && t < L::TM * 32 ? (int)t : -1;
+        uint8_t* to = mine + (lane & 31) * RB;
 #pragma unroll
-      for (int a = 0; a < L::TM; ++a)
+        for (int a = 0; a < L::TM; ++a)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float p[4];
+          for (int q = 0; q < 4; ++q) {
+            float p[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = a * 32 + 8 * q + 4 * h + r;
-            float x = l.acc[a][0][4 * q + r];
+            for (int r = 0; r < 4; ++r) {
+              const int row = a * 32 + 8 * q + 4 * h + r;
+              float x = l.acc[a][0][4 * q + r];
 #pragma unroll
-            for (int o = 1; o < L::TN; ++o) x = b == o ? l.acc[a][o][4 * q + r] : x;
-            x = __builtin_amdgcn_exp2f((x - top) * LOG2E) * over;
-            x = tl == row ? x - lift : x;
-            if (TWICE && (part & 1)) x -= stored(x, OP::CODE);   // (infinities: a NaN, in a row that has them already)
-            p[r] = row < left ? x : 0.f;
+              for (int o = 1; o < L::TN; ++o) x = b == o ? l.acc[a][o][4 * q + r] : x;
+              x = __builtin_amdgcn_exp2f((x - top) * LOG2E) * over;
+              x = tl == row ? x - lift : x;
+              if constexpr (second) x -= stored(x, OP::CODE);   // (an infinity: a NaN, in a row that has them already)
+              p[r] = row < left ? x : 0.f;
+            }
+            const int byte = (a * 32 + 8 * q + 4 * h) * ES;
+            put<true>(to + (((byte >> 4) ^ (lane & TURN)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
           }
-          const int byte = (a * 32 + 8 * q + 4 * h) * ES;
-          put<true>(to + (((byte >> 4) ^ (lane & TURN)) << 4) + (byte & 15), OP::CODE, 0, 1, 4, p);
-        }
-      __asm__ volatile("" ::: "memory");   // (a wavefront's own LDS accesses run in order)
+        __asm__ volatile("" ::: "memory");   // (a wavefront's own LDS accesses run in order)
 #pragma unroll
-      for (int k = 0; k < 32 * CPR / 64; ++k) {
-        const int slot = k * 64 + lane, r = slot / CPR, ch = slot % CPR;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ((ch ^ (r & TURN)) << 4));
-        __builtin_amdgcn_raw_buffer_store_b128(v, TWICE && (part & 1) ? rest : rs, r * g_row + ch * 16, (wn * L::TN + b) * 32 * g_row, 0);
+        for (int k = 0; k < 32 * CPR / 64; ++k) {
+          const int slot = k * 64 + lane, r = slot / CPR, ch = slot % CPR;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * RB + ((ch ^ (r & TURN)) << 4));
+          __builtin_amdgcn_raw_buffer_store_b128(v, rs, r * g_row + ch * 16, (wn * L::TN + b) * 32 * g_row, 0);
+        }
+        __asm__ volatile("" ::: "memory");
       }
-      __asm__ volatile("" ::: "memory");
-    }
+    };
+    half_of_g(std::false_type{}, rs);
+    if constexpr (L::TWO_NUMBERS)
+      if (halves == 2) half_of_g(std::true_type{}, resource((elem*)c.g + (tokens + n0) * c.g_ld + (vw - c.v0), bytes));
   }
 }
 
 template <class OP, class L>
 __global__ __launch_bounds__(L::THREADS, L::WAVES >= 8 ? 2 : 1) void xent_logits_kernel(LogitsCall c) {
   __shared__ typename L::Stage s0, s1, s2, s3;
-  logits_tile<OP, L, false, false>(c, blockIdx.x, s0, s1, s2, s3);
+  logits_tile<OP, L, false>(c, blockIdx.x, s0, s1, s2, s3);
 }
 
 // A token's statistics over the mt tiles joined: `TOKENS` tokens a workgroup, NTHREADS / TOKENS lanes each. What the backward pass takes of them, the loss, and
@@ -752,8 +769,8 @@ __global__ __launch_bounds__(1024) void xent_factors_kernel(const float* dloss, 
 struct ProductCall {
   const void *a, *b;
   int64_t a_ld, b_ld;
-  const int* rows;          // kept tokens: M (dX) or K (dW), `times` over
-  int times;
+  const int* rows;          // kept tokens: M (dX) or K (dW), as many times over as G has numbers (halves_of, held)
+  int64_t held;
   int64_t m, n, k;          // M of dW, N, K of dX
   int64_t b_cols;           // columns of b that may be read (whole 16-byte pieces)
   int mt, nt, splits;
@@ -772,7 +789,7 @@ __device__ __forceinline__ void product_tile(const ProductCall& c, int64_t id, i
                                              typename L::Stage& s2, typename L::Stage& s3) {
   typedef typename OP::elem elem;
   constexpr int ES = sizeof(elem);
-  const int64_t tokens = uniform(c.rows[0] * c.times);
+  const int64_t tokens = uniform(c.rows[0] * halves_of(c.rows[0], c.held));
   const int64_t M = DW ? c.m : tokens, K = DW ? tokens : c.k;
   int m, n;
   if (!tile_of(id, DW ? c.mt : (int)((M + L::BM - 1) / L::BM), c.nt, m, n)) return;
@@ -839,7 +856,7 @@ struct PassCall {
   ProductCall x, w;
   int x_at, x_tiles, x_end, w_at, w_tiles, w_end, g_at;   // workgroups: of a part of the contraction, of all parts
 };
-template <class OP, class LG, class LX, class LW, bool TWICE>
+template <class OP, class LG, class LX, class LW>
 __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass_kernel(PassCall c) {
   typedef typename std::conditional<(sizeof(typename LW::Stage) > sizeof(typename LG::Stage)), typename LW::Stage, typename LG::Stage>::type S;
   static_assert(sizeof(typename LX::Stage) <= sizeof(S) && LG::THREADS == LX::THREADS && LG::THREADS == LW::THREADS, "one launch for all");
@@ -855,19 +872,20 @@ __global__ __launch_bounds__(LG::THREADS, LG::WAVES >= 8 ? 2 : 1) void xent_pass
     product_tile<OP, LW, true>(c.w, id - c.w_at - part * c.w_tiles, part, (W&)s0, (W&)s1, (W&)s2, (W&)s3);
   } else {
     typedef typename LG::Stage G;
-    logits_tile<OP, LG, true, TWICE>(c.g, id - c.g_at, (G&)s0, (G&)s1, (G&)s2, (G&)s3);
+    logits_tile<OP, LG, true>(c.g, id - c.g_at, (G&)s0, (G&)s1, (G&)s2, (G&)s3);
   }
 }
 
-// dX: a token's parts added (and those `kept` rows behind them, where that is not null), times g or its own power; zero rows for the tokens that are
+// dX: a token's parts added (and those *kept rows behind them, where G has two numbers: halves_of, held), times g or its own power; zero rows for the tokens that are
 // ignored. dW: the parts of a piece's rows.
 __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums, int splits, int64_t split_stride, int64_t n_ld,
                                                                const int* place, const Factors* units, const float* unit, float lift,
-                                                               const float* power, const int* kept, void* out, int64_t rows, int width,
-                                                               int dtype) {
+                                                               const float* power, const int* kept, int64_t held, void* out, int64_t rows,
+                                                               int width, int dtype) {
   const int lane = threadIdx.x & 63;
   const bool quads = width % 4 == 0;
   const float u = *unit;
+  const bool two = held && halves_of(*kept, held) == 2;
   for (int64_t row = (int64_t)blockIdx.x * NWAVES + wave_index(); row < rows; row += (int64_t)gridDim.x * NWAVES) {
     const int64_t at = place ? place[row] : row;
     const float f = (power && at >= 0 ? power[at] : units->g) * lift;
@@ -879,7 +897,7 @@ __global__ __launch_bounds__(NTHREADS) void xent_finish_kernel(const float* sums
           const float4 v = *reinterpret_cast<const float4*>(sums + s * split_stride + at * n_ld + e);
           x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
         }
-        if (kept) {
+        if (two) {
           const int64_t behind = at + *kept;
 #pragma unroll 8
           for (int s = 0; s < splits; ++s) {
@@ -936,9 +954,10 @@ template <class OP>
 struct XentShape {
   static constexpr int ES = sizeof(typename OP::elem), BK = KB / ES;
   static constexpr bool SCALED = !std::is_same<OP, typename OP::Back>::value;   // weight and x have copies for the products with G
-  bool train, small, large, gather, copy_w, twice;
+  bool train, small, large, gather, copy_w;
   int64_t padded, bm, mt, join_tokens, join_blocks;
   // backward
+  int64_t held;   // rows of G
   int64_t piece, pieces;
   bool large_pass;
   int splits_x, splits_w, splits_last;   // parts of dX's contraction, of dW's, and of that in the last pass
@@ -969,13 +988,10 @@ struct XentShape {
       p += align_up(bytes, 1024);
       return at;
     };
-    x = take(gather ? c.tokens * padded * ES : 0);
+    // (few tokens: room for two numbers of each, whatever is kept; more: where half of the rows are enough for what is kept)
+    held = backward && ES == 2 && !SCALED && c.tokens <= TWICE_TOKENS ? 2 * c.tokens : c.tokens;
+    x = take(gather ? held * padded * ES : 0);
     w = take(copy_w ? c.vocab * padded * ES : 0);
-    // Few tokens with fp16 operands: G in two numbers of 11 bits each. With one its rounding was beside the gradients' own, the same for a whole row, so
-    // that few rows' errors do not even out: of 40 calls each, 1 / 2 / 8 / 32 / 64 tokens, dx's error was up to 2.5 / 1.8 / 1.6 / 1.5 / 1.46 times that
-    // rounding's, 1.3 at the median, as for more tokens; with two 1.03. (Forward and backward, us: 8 x 50304 x 768 113 -> 126, 64 x 50304 x 768 121 ->
-    // 140, 33 x 32000 x 2048 165 -> 191.)
-    twice = ES == 2 && !SCALED && small;
     if (!backward) {
       top = take(mt * c.tokens * 4);
       sum = take(mt * c.tokens * 4);
@@ -983,7 +999,6 @@ struct XentShape {
       sums = take(join_blocks * 4);
     } else {
       // Pieces of the vocabulary whose G fits PIECE_BYTES (and a token's row of it MAX_LD_BYTES), in whole tiles, of about one size
-      const int64_t held = twice ? 2 * c.tokens : c.tokens;   // rows of G
       const int64_t most = std::max<int64_t>(std::min(PIECE_BYTES / (held * ES), MAX_LD_BYTES / ES) / 256 * 256, 256);
       pieces = cdiv(c.vocab, most);
       piece = align_up(cdiv(c.vocab, pieces), 256);
@@ -1035,9 +1050,9 @@ void launch_logits(LogitsCall lc, int64_t tokens, hipStream_t st) {
   hipLaunchKernelGGL((xent_logits_kernel<OP, L>), dim3((unsigned)tiles_grid(lc.mt, lc.nt)), dim3(L::THREADS), 0, st, lc);
 }
 // g, x, w: what the pass does (null: not that)
-template <class OP, bool TWICE, class LG, class LX, class LW>
-bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w, int64_t tokens, hipStream_t st) {
-  const int64_t held = TWICE ? 2 * tokens : tokens;
+// held: rows of G
+template <class OP, class LG, class LX, class LW>
+bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w, int64_t tokens, int64_t held, hipStream_t st) {
   PassCall pc{};
   int64_t at = 0;
   const auto place = [&at](ProductCall& c, int64_t m, int edge_m, int edge_n, int& begin, int& tiles, int& end) {
@@ -1062,23 +1077,23 @@ bool launch_pass(const LogitsCall* g, const ProductCall* x, const ProductCall* w
     at += tiles_grid(pc.g.mt, pc.g.nt);
   }
   if (at * LG::THREADS >= ((int64_t)1 << 32)) return false;   // more threads than a launch takes
-  hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW, TWICE>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
+  hipLaunchKernelGGL((xent_pass_kernel<OP, LG, LX, LW>), dim3((unsigned)at), dim3(LG::THREADS), 0, st, pc);
   return true;
 }
 template <class OP>
 void launch_gather(const void* from, int64_t ld, int dtype, int64_t width, const int* numbers_of, const int* count, int64_t rows, int* maxima,
                    void* to, int64_t padded, hipStream_t st, void* also = nullptr, const float* unit = nullptr, const float* power = nullptr,
-                   const float* g = nullptr, bool twice = false) {
+                   const float* g = nullptr, int64_t held = 0) {
   const int64_t blocks = maxima ? MAXIMA : std::min<int64_t>(cdiv(rows, NWAVES), 16384);
   hipLaunchKernelGGL((xent_gather_kernel<OP>), dim3((unsigned)blocks), dim3(maxima ? 1024 : NTHREADS), 0, st, from, ld, dtype, (int)width,
-                     numbers_of, count, rows, maxima, (typename OP::elem*)to, (int)padded, (typename OP::Back::elem*)also, unit, power, g, twice);
+                     numbers_of, count, rows, maxima, (typename OP::elem*)to, (int)padded, (typename OP::Back::elem*)also, unit, power, g, held);
 }
 inline void launch_finish(const float* sums, int splits, int64_t split_stride, int64_t n_ld, const int* place, const Factors* units,
-                          const float* unit, float lift, const float* power, const int* kept, void* out, int64_t rows, int64_t width,
-                          int dtype, hipStream_t st) {
+                          const float* unit, float lift, const float* power, const int* kept, int64_t held, void* out, int64_t rows,
+                          int64_t width, int dtype, hipStream_t st) {
   const int64_t blocks = std::min<int64_t>(cdiv(rows, NWAVES), 16384);
   hipLaunchKernelGGL(xent_finish_kernel, dim3((unsigned)blocks), dim3(NTHREADS), 0, st, sums, splits, split_stride, n_ld, place, units,
-                     unit, lift, power, kept, out, rows, (int)width, dtype);
+                     unit, lift, power, kept, held, out, rows, (int)width, dtype);
 }
 
 template <class OP>
@@ -1143,11 +1158,11 @@ int xent_backward(const XentCall& c) {
   float* factor = c.reduction == SA_REDUCE_NONE ? (float*)units + 64 : nullptr;
   float* power = factor && ES == 2 ? factor + c.tokens : nullptr;
   hipLaunchKernelGGL(xent_factors_kernel, dim3(1), dim3(1024), 0, c.st, c.dloss, c.rows, c.reduction, s.SCALED, units, factor, power);
-  const int64_t held = s.twice ? 2 * c.tokens : c.tokens;   // rows of G
-  const bool two = s.SCALED || power || s.twice;
+  const int64_t held = ES == 2 && !s.SCALED ? s.held : 0;   // (0: G in one number)
+  const bool two = s.SCALED || power;
   const char* x_back = ws + (two ? s.x_back : s.x);   // dW's
   launch_gather<OP>(c.x, c.x_ld, c.x_t, c.width, c.rows + ROWS_HEAD, c.rows, c.tokens, nullptr, ws + s.x, s.padded, c.st,
-                    c.dw && two ? ws + s.x_back : nullptr, &units->x, power, &units->g, s.twice);
+                    c.dw && two ? ws + s.x_back : nullptr, &units->x, power, &units->g, held);
   const char *w = s.copy_w ? ws + s.w : (const char*)c.w, *w_back = s.SCALED ? ws + s.w_back : w;   // dX's
   const int64_t w_ld = s.copy_w ? s.padded : c.w_ld, w_back_ld = s.SCALED ? s.padded : w_ld;
   void* const scaled_w = s.SCALED && c.dx ? ws + s.w_back : nullptr;
@@ -1160,15 +1175,15 @@ int xent_backward(const XentCall& c) {
     if (p < s.pieces) {
       g.w = w, g.w_ld = w_ld, g.x = ws + s.x, g.x_ld = s.padded, g.targets = c.targets, g.rows = c.rows, g.tokens = c.tokens;
       g.vocab = c.vocab, g.v0 = p * s.piece, g.v1 = std::min(g.v0 + s.piece, c.vocab), g.stages = (int)(s.padded / s.BK);
-      g.lse = c.lse, g.factor = factor, g.g = ws + (p & 1 ? s.g2 : s.g), g.g_ld = s.piece;
+      g.lse = c.lse, g.factor = factor, g.held = held, g.g = ws + (p & 1 ? s.g2 : s.g), g.g_ld = s.piece;
     }
     ProductCall px{}, pw{};
     const int64_t v0 = (p - 1) * s.piece, v1 = std::min(v0 + s.piece, c.vocab);
     char* out = (char*)c.dw + v0 * c.width * lm_elem_size(c.w_t);
     if (p > 0) {
-      px.a = pw.a = ws + (p & 1 ? s.g : s.g2), px.a_ld = pw.a_ld = s.piece, px.rows = pw.rows = c.rows, px.times = pw.times = s.twice ? 2 : 1;
+      px.a = pw.a = ws + (p & 1 ? s.g : s.g2), px.a_ld = pw.a_ld = s.piece, px.rows = pw.rows = c.rows, px.held = pw.held = held;
       px.b = w_back + v0 * w_back_ld * ES, px.b_ld = w_back_ld, px.n = px.b_cols = s.padded, px.k = v1 - v0;
-      px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = held, px.add = p > 1;
+      px.splits = s.splits_x, px.sums = (float*)(ws + s.dx), px.n_ld = s.padded, px.m_rows = s.held, px.add = p > 1;
       pw.b = x_back, pw.b_ld = pw.b_cols = s.padded, pw.m = v1 - v0, pw.n = c.width;
       pw.splits = p == s.pieces ? s.splits_last : s.splits_w, pw.lift = 1.f / BACK::LIFT, pw.units = units;
       if (pw.splits == 1) pw.out = out, pw.out_ld = c.width, pw.out_t = c.w_t;
@@ -1176,17 +1191,16 @@ int xent_backward(const XentCall& c) {
     }
     const LogitsCall* pg = p < s.pieces ? &g : nullptr;
     const ProductCall *x = p > 0 && c.dx ? &px : nullptr, *y = p > 0 && c.dw ? &pw : nullptr;
-    constexpr bool TWICE = ES == 2 && !s.SCALED;   // (of the smallest)
-    if (!(s.small        ? launch_pass<BACK, TWICE, typename F::Small, typename B::SmallX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)
-          : s.large_pass ? launch_pass<BACK, false, typename F::Large, typename B::LargeX, typename B::LargeW>(pg, x, y, c.tokens, c.st)
-                         : launch_pass<BACK, false, typename F::Middle, typename B::MiddleX, typename B::MiddleW>(pg, x, y, c.tokens, c.st)))
+    if (!(s.small        ? launch_pass<BACK, typename F::Small, typename B::SmallX, typename B::MiddleW>(pg, x, y, c.tokens, s.held, c.st)
+          : s.large_pass ? launch_pass<BACK, typename F::Large, typename B::LargeX, typename B::LargeW>(pg, x, y, c.tokens, s.held, c.st)
+                         : launch_pass<BACK, typename F::Middle, typename B::MiddleX, typename B::MiddleW>(pg, x, y, c.tokens, s.held, c.st)))
       return SA_ERR_ARGUMENT;
     if (y && pw.splits > 1)
-      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / BACK::LIFT, nullptr, nullptr, out, v1 - v0, c.width, c.w_t, c.st);
+      launch_finish(pw.sums, pw.splits, s.piece * s.padded, s.padded, nullptr, units, &units->from_x, 1.f / BACK::LIFT, nullptr, nullptr, 0, out, v1 - v0, c.width, c.w_t, c.st);
   }
   if (c.dx)
-    launch_finish((float*)(ws + s.dx), s.splits_x, held * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, units, &units->from_w,
-                  1.f / BACK::LIFT, power, s.twice ? c.rows : nullptr, c.dx, c.tokens, c.width, c.x_t, c.st);
+    launch_finish((float*)(ws + s.dx), s.splits_x, s.held * s.padded, s.padded, c.rows + ROWS_HEAD + c.tokens, units, &units->from_w,
+                  1.f / BACK::LIFT, power, c.rows, held, c.dx, c.tokens, c.width, c.x_t, c.st);
   return launch_status();
 }
 

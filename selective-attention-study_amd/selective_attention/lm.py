@@ -474,7 +474,7 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, ignore_inde
     dot_precision: None takes the products' operands in x's dtype, "bf16" in bf16, "tf32" and "ieee" in fp32 (no TF32 on this
     hardware); x and weight are rounded to it where they are of another type (the fp32 weight of a bf16 autocast step), products
     are summed in fp32. Gradients have x's and weight's own types. The probabilities that enter the gradients' products are
-    rounded to 11 bits for bf16 and fp16 operands (to 22 for up to 64 tokens in fp16), not at all for fp32. (bf16 operands enter these in fp16 times a power of two: exactly, but
+    rounded to 11 bits for bf16 and fp16 operands (to 22 in fp16 where no more than 64 tokens are kept of 64 or of twice as many), not at all for fp32. (bf16 operands enter these in fp16 times a power of two: exactly, but
     for numbers 2^31 times smaller than the largest of x or weight, which are off by 2^-39 of that; "ieee" has no such limit.) With "none" each token's
     row of probabilities has a unit of its own, by the gradient that arrives for it, so that small ones beside large ones keep their bits in x's
     gradient; in weight's, where they are added, what is 2^28 times smaller than the largest (of x times the gradient that arrives) loses bits.

@@ -259,17 +259,19 @@ def test_reductions_of_the_two_passes(cuda, dtype):
         assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q)), forward
 
 
-@pytest.mark.parametrize("n", [1, 2, 7, 32, 33, 64])
+@pytest.mark.parametrize("n,vocab,ignored", [(1, 700, 0.2), (2, 700, 0.2), (7, 700, 0.2), (32, 700, 0.2), (33, 700, 0.2), (64, 700, 0.2),
+                                             (300, 700, 0.95), (2000, 700, 0.98), (5000, 20000, 0.992)])
 @pytest.mark.parametrize("reduction", [0, 1])
-def test_few_tokens_in_fp16(cuda, n, reduction):
-    """Up to 64 tokens with fp16 operands have G in two numbers, to 22 bits: seen in fp32 gradients of fp32 tensors of fp16 numbers.
+def test_few_tokens_in_fp16(cuda, n, vocab, ignored, reduction):
+    """Up to 64 tokens that are not ignored, with fp16 operands, have G in two numbers, to 22 bits: seen in fp32 gradients of fp32 tensors of fp16 numbers.
 
     Bounds as in xent_check, with 2^-22 of G in the place of 2^-11."""
-    vocab, width = 700, 16
+    width = 16
     g = torch.Generator(device="cuda").manual_seed(39)
-    x, w, t = xent_inputs(g, n, vocab, width, F16, F16, ignored=0.2)
+    x, w, t = xent_inputs(g, n, vocab, width, F16, F16, ignored=ignored)
     t[0] = 5
     kept = t != -100
+    assert kept.sum() <= 64
     code = lm._CODES[F16]
     dloss = randn(g, n) if reduction == 0 else torch.ones((), device="cuda")
     _, lse, rows = lm._xent_impl(x.float(), w.float(), t, -100, reduction, code, True)
@@ -289,5 +291,5 @@ def test_few_tokens_in_fp16(cuda, n, reduction):
     assert (dx[~kept] == 0).all()
     assert_within(dx[kept], want, ((e_G + (2 * vocab + 8) * U * G.abs()) @ w64.abs()) * 1.01 + rounding(want, F32), "dx")
     want = G.T @ x64
-    assert_within(dw, want, ((e_G + (2 * n + 8) * U * G.abs()).T @ x64.abs() + 2.0 ** -38 * x64.abs().max() * f.abs().max() * p.sum(0)[:, None]) * 1.01
+    assert_within(dw, want, ((e_G + (2 * len(at) + 8) * U * G.abs()).T @ x64.abs() + 2.0 ** -38 * x64.abs().max() * f.abs().max() * p.sum(0)[:, None]) * 1.01
                   + rounding(want, F32), "dw")
